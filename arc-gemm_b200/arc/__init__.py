@@ -12,6 +12,12 @@ the GEMM path is what this package covers):
 * `a8w4_matmul_bf16(x, (wp, sb))`     quantize_int8 followed by the A8W4 GEMM
 * `fp8_fp4_gemm_nt(a, b, out, recipe_a, recipe_b)`  FP8 x FP4 with UE8M0 block scales, the
   recipe and call shape of the reference's own A8W4 test
+* `linear(x, w, bias, residual, activation=...)`  bf16 linear layer, its epilogue in the GEMM,
+  differentiable
+* `grouped_matmul(x, w, offsets)`     rows sorted by expert times the expert's bf16 weights,
+  differentiable
+* `a8w4_grouped_matmul((x, sa), (wp, sb), offsets)`  the same on int8 x int4
+* `group_rows(ids, num_groups)`       a router's choices -> (offsets, rows, positions)
 * `quant`, `math`, `parallel`, `testing` helpers
 
 The kernels are AOT-built into libarcb200.so for sm_100a (`python -m arc.build`).
@@ -20,6 +26,8 @@ from . import math, parallel, quant
 from ._lib import ArcError, describe_plan, device_status, kernel_name, version
 from .a8w4 import (a8w4_gemm_nt, a8w4_matmul, a8w4_matmul_bf16, fp8_fp4_gemm_nt, prepack_weights,
                    quantize_int8)
+from .grouped import a8w4_grouped_matmul, group_rows, grouped_matmul
+from .linear import linear
 from .mm import matmul
 
 __all__ = [
@@ -30,6 +38,10 @@ __all__ = [
     "fp8_fp4_gemm_nt",
     "quantize_int8",
     "prepack_weights",
+    "linear",
+    "grouped_matmul",
+    "a8w4_grouped_matmul",
+    "group_rows",
     "ArcError",
     "describe_plan",
     "device_status",

@@ -20,6 +20,8 @@ ARC_ERR_DEVICE_TIMEOUT = 5
 
 # Bits of arc_device_status (arc-gemm_b200/csrc/sm100.cuh): which kind of wait timed out.
 STATUS_TIMEOUT_PEER = 1 << 6
+# Not a wait: a grouped product read offsets that decrease or leave its rows.
+STATUS_BAD_OFFSETS = 1 << 7
 
 
 class ArcError(RuntimeError):
@@ -48,6 +50,7 @@ class Plan(ctypes.Structure):
 # Every symbol include/arc_b200.h declares, with its ctypes signature.
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_int64
 SIGNATURES = {
     "arc_version": ([], _I),
     "arc_status_string": ([_I], ctypes.c_char_p),
@@ -73,12 +76,26 @@ SIGNATURES = {
     "arc_a8w4_gemm_prepacked": ([_P, _P, _P, _P, _P, _I, _I, _I, _I, _P], _I),
     "arc_a8w4_gemm_ex": ([_P, _P, _P, _P, _P, _I, _I, _I, _I, ctypes.c_uint, _P, _P], _I),
     "arc_a8w4_gemm_gather_ex": ([_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_uint, _P], _I),
+    "arc_linear_bf16": ([_P] * 6 + [_I] * 3 + [_L] * 5 + [_I, _P], _I),
+    "arc_linear_dz_workspace_bytes": ([_I, _I, ctypes.POINTER(ctypes.c_size_t)], _I),
+    "arc_linear_dz": ([_P] * 5 + [ctypes.c_size_t, _I, _I] + [_L] * 3 + [_I, _P], _I),
+    "arc_grouped_matmul": ([_P] * 4 + [_I] * 4 + [_L] * 4 + [ctypes.c_uint, _P], _I),
+    "arc_grouped_matmul_dx": ([_P] * 4 + [_I] * 4 + [_L] * 4 + [ctypes.c_uint, _P], _I),
+    "arc_grouped_matmul_dw": ([_P] * 4 + [_I] * 4 + [_L] * 4 + [_P], _I),
+    "arc_a8w4_grouped_gemm": ([_P] * 6 + [_I] * 5 + [ctypes.c_uint, _P], _I),
+    "arc_group_rows_workspace_bytes": ([_I, _I, ctypes.POINTER(ctypes.c_size_t)], _I),
+    "arc_group_rows": ([_P, _I, _P, _P, _P, _P, ctypes.c_size_t, _I, _I, _I, _P], _I),
     "arc_a8w4_gemm_gather_sync": ([_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_uint, _P], _I),
 }
 
 # Flags of arc_a8w4_gemm_ex / arc_a8w4_gemm_gather_ex (include/arc_b200.h).
 A8W4_PREPACKED = 1
 A8W4_STATIC_WEIGHTS = 2
+# Flag of the grouped products: rows of no group are set to zero.
+GROUPED_ZERO_OTHERS = 4
+
+# Activations of arc_linear_bf16 (include/arc_b200.h).
+ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 # Operation codes of arc_kernel_name (include/arc_b200.h).
 OP_MATMUL_BF16, OP_A8W4, OP_FP8_FP4 = 0, 1, 2

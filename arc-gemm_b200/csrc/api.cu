@@ -143,6 +143,7 @@ struct DeviceState {
   int max_clusters4 = 0;  // co-resident 4-CTA clusters of the decode kernel
   int max_bf16_pairs = 0;  // co-resident CTA pairs of the bf16 pair kernel
   int max_fp8fp4_pairs = 0;  // co-resident CTA pairs of the FP8 x FP4 pair kernel
+  int max_linear_pairs = 0;  // co-resident CTA pairs of the linear pair kernel
 };
 DeviceState g_dev[kMaxDevices];
 
@@ -187,6 +188,9 @@ bool decode_stream(int G, int S, int num_items, int grid) {
 #define ARC_A8W4_VARIANTS(X) \
   X(64, 1, 4)                \
   X(128, 2, 3)
+
+cudaError_t linear_init(DeviceState& st);          // api_linear.cuh
+cudaError_t grouped_init(DeviceState& st, bool* regs_ok);  // api_grouped.cuh
 
 int init_device(int dev) {
   DeviceState& st = g_dev[dev];
@@ -279,6 +283,13 @@ int init_device(int dev) {
         return;
       }
     }
+    if (e == cudaSuccess) e = linear_init(st);
+    if (e == cudaSuccess) e = grouped_init(st, &regs_ok);
+    if (e == cudaSuccess && !regs_ok) {
+      st.status = fail(ARC_ERR_UNSUPPORTED,
+                       "gemm_a8w4_grouped_kernel was compiled with an unexpected register count");
+      return;
+    }
     if (e != cudaSuccess) {
       st.status = cuda_fail(e, "cudaFuncSetAttribute");
       return;
@@ -354,6 +365,14 @@ int current_device(int* dev) {
   const cudaError_t e = cudaGetDevice(dev);
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   if (*dev < 0 || *dev >= kMaxDevices) return fail(ARC_ERR_NO_DEVICE, "device %d out of range", *dev);
+  // A thread that has not launched anything yet (an autograd thread, say) has no context
+  // bound, and encoding a tensor map, a driver call, needs one.
+  thread_local int bound = -1;
+  if (bound != *dev) {
+    const cudaError_t s = cudaSetDevice(*dev);
+    if (s != cudaSuccess) return cuda_fail(s, "cudaSetDevice");
+    bound = *dev;
+  }
   return init_device(*dev);
 }
 
@@ -462,6 +481,23 @@ cudaError_t launch_ex(Kern kernel, const P& p, uint32_t grid, uint32_t threads, 
   cfg.attrs = attr;
   cfg.numAttrs = n;
   return cudaLaunchKernelEx(&cfg, kernel, p);
+}
+
+// The same without a cluster, for any grid and arguments.
+template <typename... Formal, typename... Actual>
+cudaError_t launch_grid(void (*kernel)(Formal...), dim3 grid, uint32_t threads, size_t smem, cudaStream_t stream,
+                        Actual... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = stream;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  return cudaLaunchKernelEx(&cfg, kernel, Formal(args)...);
 }
 
 // Launch the decode instantiation of the mode (stream or chunk) and of the partials dump.
@@ -1372,3 +1408,6 @@ int arc_device_status(int device, uint32_t* status, int clear) {
 }
 
 }  // extern "C"
+
+#include "api_linear.cuh"
+#include "api_grouped.cuh"

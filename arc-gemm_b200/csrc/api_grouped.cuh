@@ -1,0 +1,192 @@
+// api_grouped.cuh — host side of the grouped A8W4 product and of the row grouping. Included by
+// api.cu, whose helpers it uses.
+#pragma once
+
+#include "api_linear.cuh"
+#include "group_rows.cuh"
+
+namespace {
+
+namespace GQ = arcb::a8w4;
+namespace GR = arcb::rows;
+
+// Token tile, epilogue warpgroups, load stages of the grouped A8W4 instantiations.
+#define ARC_A8W4_GROUPED_VARIANTS(X) X(16, 1, 4) X(32, 1, 4) X(64, 1, 4) X(128, 2, 3)
+
+template <uint32_t BT, uint32_t EWG, uint32_t LS_>
+constexpr size_t a8w4_grouped_smem() {
+  return sizeof(GQ::GroupedSmem<BT, EWG, LS_>) + 1024;
+}
+
+cudaError_t grouped_init(DeviceState&, bool* regs_ok) {
+  cudaError_t e = cudaSuccess;
+#define ARC_SET_ATTR(BT, EWG, LSN)                                                                    \
+  static_assert(a8w4_grouped_smem<BT, EWG, LSN>() <= 232448, "shared memory fits in 227 KB");         \
+  if (e == cudaSuccess) {                                                                             \
+    e = allow_smem(GQ::gemm_a8w4_grouped_kernel<BT, EWG, LSN>, a8w4_grouped_smem<BT, EWG, LSN>());    \
+  }                                                                                                   \
+  if (e == cudaSuccess) {                                                                             \
+    cudaFuncAttributes fa;                                                                            \
+    e = cudaFuncGetAttributes(&fa, GQ::gemm_a8w4_grouped_kernel<BT, EWG, LSN>);                       \
+    if (e == cudaSuccess && fa.numRegs != static_cast<int>(GQ::Cfg<BT, EWG, LSN>::kLaunchRegs)) {     \
+      *regs_ok = false;                                                                               \
+    }                                                                                                 \
+  }
+  ARC_A8W4_GROUPED_VARIANTS(ARC_SET_ATTR)
+#undef ARC_SET_ATTR
+  const int most = static_cast<int>(GR::smem_bytes(GR::kMaxBuckets - 1));
+  for (const void* k : {reinterpret_cast<const void*>(GR::place_rows_kernel<int32_t>),
+                        reinterpret_cast<const void*>(GR::place_rows_kernel<int64_t>)}) {
+    if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
+  }
+  return e;
+}
+
+template <uint32_t BT, uint32_t EWG, uint32_t LS_>
+cudaError_t launch_a8w4_grouped(const GQ::GroupedParams& p, uint32_t grid, cudaStream_t stream) {
+  return launch_ex(GQ::gemm_a8w4_grouped_kernel<BT, EWG, LS_>, p, grid, GQ::Cfg<BT, EWG, LS_>::kThreads,
+                   a8w4_grouped_smem<BT, EWG, LS_>(), 1, stream);
+}
+
+// Blocks of the row grouping: one up to kOneBlockSlots slots, else one per SM of the largest
+// part (the workspace size must not depend on the device).
+constexpr uint32_t kRowBlocks = 148;
+uint32_t group_rows_blocks(uint32_t slots, uint32_t* per_block) {
+  if (slots <= GR::kOneBlockSlots) {
+    *per_block = GR::kOneBlockSlots;
+    return 1;
+  }
+  *per_block = ceil_div(ceil_div(slots, kRowBlocks), GR::kThreads) * GR::kThreads;
+  return ceil_div(slots, *per_block);
+}
+
+}  // namespace
+
+extern "C" {
+
+int arc_a8w4_grouped_gemm(const int8_t* A, const float* sa, const uint8_t* Wp, const uint16_t* sb,
+                          const int32_t* offsets, uint16_t* C, int T, int E, int N, int K, int group, unsigned flags,
+                          cudaStream_t stream) {
+  const char* what = "arc_a8w4_grouped_gemm";
+  g_last_error[0] = '\0';
+  if (sa == nullptr || sb == nullptr || offsets == nullptr) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  }
+  if (int st = grouped_check(what, A, Wp, C, offsets, T, E, N, K)) return st;
+  if (flags & ~(ARC_A8W4_PREPACKED | ARC_GROUPED_ZERO_OTHERS)) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: unknown flags 0x%x", what, flags);
+  }
+  if (group != static_cast<int>(GQ::kGroupK) || K % group != 0 || N % 8 != 0) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: need group == 128, K %% 128 == 0 and N %% 8 == 0 (group=%d N=%d K=%d)", what,
+                group, N, K);
+  }
+  if (!aligned16(A) || !aligned16(Wp) || !aligned16(C) || (reinterpret_cast<uintptr_t>(sa) & 3u) ||
+      (reinterpret_cast<uintptr_t>(sb) & 1u)) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: A, Wp and C must be 16-byte aligned", what);
+  }
+  if (int64_t(E) * N > 0x7FFFFFFF) return fail(ARC_ERR_UNSUPPORTED, "%s: E * N must be below 2^31", what);
+  int dev = 0;
+  if (int st = current_device(&dev)) return st;
+  const uint32_t live = E < T ? E : T;  // groups that can have rows
+  const uint32_t avg = ceil_div(T, live);
+  const uint32_t BT = avg <= 16 ? 16u : avg <= 32 ? 32u : avg <= 64 ? 64u : 128u;
+  GQ::GroupedParams p = {};
+  if (int st = encode_2d(&p.tm_tok, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A, K, T, K, GQ::kGroupK, BT,
+                         CU_TENSOR_MAP_SWIZZLE_128B, "A")) {
+    return st;
+  }
+  if (int st = encode_2d(&p.tm_wp, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, Wp, K / 2, uint64_t(E) * N, K / 2,
+                         GQ::kPackedRow * GQ::kGps, GQ::kRows, CU_TENSOR_MAP_SWIZZLE_128B, "Wp")) {
+    return st;
+  }
+  p.sa = sa;
+  p.sb = sb;
+  p.out = C;
+  p.partials = nullptr;
+  p.M = T;
+  p.N = N;
+  p.K = K;
+  p.G = K / GQ::kGroupK;
+  p.ldsb = p.G;
+  p.ldc = N;
+  p.R = GQ::kRows;
+  p.tiles_n = ceil_div(N, GQ::kRows);
+  p.split = (flags & ARC_A8W4_PREPACKED) ? 1u : 0u;
+  p.groups = {offsets, static_cast<uint32_t>(E), static_cast<uint32_t>(T)};
+  p.zero_others = (flags & ARC_GROUPED_ZERO_OTHERS) ? 1u : 0u;
+  const uint64_t tiles = uint64_t(live + T / BT) * p.tiles_n;
+  const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
+  const uint32_t grid = tiles < sms ? static_cast<uint32_t>(tiles) : sms;
+  const cudaError_t e = BT == 16   ? launch_a8w4_grouped<16, 1, 4>(p, grid, stream)
+                        : BT == 32 ? launch_a8w4_grouped<32, 1, 4>(p, grid, stream)
+                        : BT == 64 ? launch_a8w4_grouped<64, 1, 4>(p, grid, stream)
+                                   : launch_a8w4_grouped<128, 2, 3>(p, grid, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "gemm_a8w4_grouped_kernel launch");
+  return ARC_OK;
+}
+
+int arc_group_rows_workspace_bytes(int slots, int E, size_t* bytes) {
+  if (bytes == nullptr || slots <= 0 || E <= 0 || E > static_cast<int>(arcb::lin::kMaxGroups)) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "arc_group_rows_workspace_bytes: bad argument");
+  }
+  uint32_t per_block = 0;
+  const uint32_t blocks = group_rows_blocks(slots, &per_block);
+  *bytes = blocks == 1 ? 0 : size_t(blocks) * (E + 1) * sizeof(uint32_t);
+  return ARC_OK;
+}
+
+int arc_group_rows(const void* ids, int id_bytes, int32_t* offsets, int32_t* rows, int32_t* positions, void* workspace,
+                   size_t workspace_bytes, int slots, int top, int E, cudaStream_t stream) {
+  const char* what = "arc_group_rows";
+  g_last_error[0] = '\0';
+  if (ids == nullptr || offsets == nullptr || rows == nullptr || positions == nullptr) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  }
+  if (slots <= 0 || top <= 0 || E <= 0) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: sizes must be positive (slots=%d top=%d E=%d)", what, slots, top, E);
+  }
+  if (slots > 0x7FFFFFFF - (1 << 20)) return fail(ARC_ERR_UNSUPPORTED, "%s: too many slots (%d)", what, slots);
+  if (E > static_cast<int>(arcb::lin::kMaxGroups)) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: at most %u groups (got %d)", what, arcb::lin::kMaxGroups, E);
+  }
+  if (id_bytes != 4 && id_bytes != 8) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: ids are 4- or 8-byte integers (got %d bytes)", what, id_bytes);
+  }
+  if ((reinterpret_cast<uintptr_t>(ids) & (id_bytes - 1)) || (reinterpret_cast<uintptr_t>(offsets) & 3u) ||
+      (reinterpret_cast<uintptr_t>(rows) & 3u) || (reinterpret_cast<uintptr_t>(positions) & 3u)) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: misaligned pointer", what);
+  }
+  uint32_t per_block = 0;
+  const uint32_t blocks = group_rows_blocks(slots, &per_block);
+  const size_t need = blocks == 1 ? 0 : size_t(blocks) * (E + 1) * sizeof(uint32_t);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3u))) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 4-byte aligned workspace of %zu bytes", what, need);
+  }
+  int dev = 0;
+  if (int st = current_device(&dev)) return st;
+  GR::Params p = {};
+  p.ids = ids;
+  p.offsets = offsets;
+  p.rows = rows;
+  p.positions = positions;
+  p.counts = blocks == 1 ? nullptr : static_cast<uint32_t*>(workspace);
+  p.slots = slots;
+  p.top = top;
+  p.groups = E;
+  p.blocks = blocks;
+  p.per_block = per_block;
+  cudaError_t e;
+  if (blocks > 1) {
+    const size_t hist = size_t(E + 1) * 4;
+    e = id_bytes == 4 ? launch_grid(GR::count_rows_kernel<int32_t>, dim3(blocks), GR::kThreads, hist, stream, p)
+                      : launch_grid(GR::count_rows_kernel<int64_t>, dim3(blocks), GR::kThreads, hist, stream, p);
+    if (e != cudaSuccess) return cuda_fail(e, "count_rows_kernel launch");
+  }
+  const size_t smem = GR::smem_bytes(E);
+  e = id_bytes == 4 ? launch_grid(GR::place_rows_kernel<int32_t>, dim3(blocks), GR::kThreads, smem, stream, p)
+                    : launch_grid(GR::place_rows_kernel<int64_t>, dim3(blocks), GR::kThreads, smem, stream, p);
+  if (e != cudaSuccess) return cuda_fail(e, "place_rows_kernel launch");
+  return ARC_OK;
+}
+
+}  // extern "C"

@@ -1,0 +1,428 @@
+// api_linear.cuh — host side of the linear layer and the grouped products: argument checks,
+// tensor maps, the choice between the streaming and the pair kernel, launches. Included by
+// api.cu, whose helpers it uses.
+#pragma once
+
+#include "gemm_linear_pair.cuh"
+#include "gemm_linear_stream.cuh"
+#include "linear_backward.cuh"
+
+namespace {
+
+namespace LS = arcb::linstream;
+namespace LP = arcb::linpair;
+namespace LB = arcb::linbwd;
+
+// Row-major matrices [groups][rows][cols] (bf16), `ld` elements between rows and
+// `group_stride` between groups.
+int encode_groups_3d(CUtensorMap* map, const void* ptr, uint64_t cols, uint64_t rows, uint64_t groups, uint64_t ld,
+                     uint64_t group_stride, uint32_t box_cols, uint32_t box_rows, const char* what) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[3] = {cols, rows, groups};
+  const cuuint64_t strides[2] = {ld * 2, group_stride * 2};
+  const cuuint32_t box[3] = {box_cols, box_rows, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, static_cast<int>(r));
+  }
+  return ARC_OK;
+}
+
+// Widest vector that every row of a bf16 matrix allows (lin::store_row32).
+uint32_t row_vec(const void* p, uint64_t ld, uint64_t group_stride = 0) {
+  const uint64_t bits = reinterpret_cast<uintptr_t>(p) | (ld * 2) | (group_stride * 2);
+  return (bits & 31u) == 0 ? 2u : (bits & 15u) == 0 ? 1u : 0u;
+}
+
+// The kernel for a product with row groups: out[rows][cols], `num_kb` contraction blocks.
+//
+// Pairs (256 x 256 tiles) when the groups' rows fill such tiles and there are tiles enough to
+// give most pairs one; else the streaming kernel, its row tile the smallest that holds an
+// average group's rows, with the contraction split over a cluster until the two block slots
+// of every SM have work (at least kMinKb blocks of 64 each).
+//
+// ARC_LINEAR_PLAN="pair" | "BN:S" (tests and tuning) forces the choice where it is valid.
+struct LinearPlan {
+  bool pair;
+  uint32_t bn, splits, row_tiles;
+};
+constexpr uint32_t kStreamMinKb = 4;
+
+int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t num_kb, LinearPlan* plan) {
+  const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
+  const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
+  const uint32_t live = groups < rows ? groups : rows;  // groups that can have rows
+  const uint32_t avg = ceil_div(rows, live);
+  const uint64_t pair_tiles = uint64_t(ceil_div(avg, LP::kTile)) * live * ceil_div(cols, LP::kTile);
+  plan->pair = max_pairs > 0 && avg > 128 && pair_tiles * 2 > max_pairs;
+  plan->bn = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
+  uint32_t forced = 0;
+  if (const char* env = getenv("ARC_LINEAR_PLAN")) {
+    unsigned bn = 0, s = 0;
+    if (strcmp(env, "pair") == 0 && max_pairs > 0) {
+      plan->pair = true;
+    } else if (sscanf(env, "%u:%u", &bn, &s) == 2 && (bn == 16 || bn == 32 || bn == 64 || bn == 128) &&
+               (s == 1 || s == 2 || s == 4 || s == 8)) {
+      plan->pair = false;
+      plan->bn = bn;
+      forced = s;
+    } else {
+      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_LINEAR_PLAN must be 'pair' or 'BN:S' (got '%s')", env);
+    }
+  }
+  // With groups the host knows only a bound: a group of c rows has at most c / bn + 1 tiles.
+  plan->row_tiles = groups == 1 ? ceil_div(rows, plan->bn) : live + rows / plan->bn;
+  const uint64_t tiles = uint64_t(plan->row_tiles) * ceil_div(cols, LS::kRows);
+  plan->splits = 1;
+  for (uint32_t s : {8u, 4u, 2u}) {
+    if (forced != 0 ? (s == forced && s <= num_kb) : (tiles * s <= 2 * sms && num_kb >= s * kStreamMinKb)) {
+      plan->splits = s;
+      break;
+    }
+  }
+  return ARC_OK;
+}
+
+template <uint32_t BN, bool W_MN>
+cudaError_t launch_stream(const LS::Params& p, uint32_t grid, cudaStream_t stream) {
+  return launch_ex(LS::gemm_linear_stream_kernel<BN, W_MN>, p, grid, LS::kThreads, LS::smem_bytes<BN>(), p.splits,
+                   stream);
+}
+
+template <bool W_MN>
+cudaError_t launch_stream_bn(const LS::Params& p, uint32_t bn, uint32_t grid, cudaStream_t stream) {
+  return bn == 16   ? launch_stream<16, W_MN>(p, grid, stream)
+         : bn == 32 ? launch_stream<32, W_MN>(p, grid, stream)
+         : bn == 64 ? launch_stream<64, W_MN>(p, grid, stream)
+                    : launch_stream<128, W_MN>(p, grid, stream);
+}
+
+#define ARC_LINEAR_STREAM_VARIANTS(X) X(16, false) X(32, false) X(64, false) X(128, false) \
+  X(16, true) X(32, true) X(64, true) X(128, true)
+
+cudaError_t linear_init(DeviceState& st) {
+  cudaError_t e = cudaSuccess;
+#define ARC_SET_ATTR(BN, MN) \
+  if (e == cudaSuccess) e = allow_smem(LS::gemm_linear_stream_kernel<BN, MN>, LS::smem_bytes<BN>());
+  ARC_LINEAR_STREAM_VARIANTS(ARC_SET_ATTR)
+#undef ARC_SET_ATTR
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, false, false>, LP::kSmemBytes);
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, true, false>, LP::kSmemBytes);
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<true, true, true>, LP::kSmemBytes);
+  if (e != cudaSuccess) return e;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(st.sms, 1, 1);
+  cfg.blockDim = dim3(LP::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = LP::kSmemBytes;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = 2;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  e = cudaOccupancyMaxActiveClusters(&n, LP::gemm_linear_pair_kernel<true, true, true>, &cfg);
+  st.max_linear_pairs = e == cudaSuccess ? n : 0;
+  return e;
+}
+
+// out[rows][cols] = epilogue of a [rows][inner] times w, per group. grad = false: w is
+// [E][cols][inner]; grad = true: w is [E][inner][cols] (the gradient of the rows).
+int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& groups, uint16_t* out, uint32_t cols,
+                uint32_t inner, uint64_t lda, uint64_t ldw, uint64_t w_stride, uint64_t ldo,
+                const arcb::lin::Epilogue& epi, bool grad, bool zero_others, cudaStream_t stream) {
+  int dev = 0;
+  if (int st = current_device(&dev)) return st;
+  const uint32_t num_kb = ceil_div(inner, arcb::lin::BK);
+  LinearPlan plan;
+  if (int st = linear_plan(dev, groups.rows, groups.num, cols, num_kb, &plan)) return st;
+  const uint64_t w_rows = grad ? inner : cols, w_cols = grad ? cols : inner;
+  cudaError_t e;
+  if (plan.pair) {
+    LP::Params p = {};
+    if (int st = encode_groups_3d(&p.tm_a, a, inner, groups.rows, 1, lda, uint64_t(groups.rows) * lda, 64,
+                                  LP::kRowsPerCta, "rows")) {
+      return st;
+    }
+    if (int st = encode_groups_3d(&p.tm_b, w, w_cols, w_rows, groups.num, ldw, w_stride, 64,
+                                  grad ? 64 : LP::kRowsPerCta, "weights")) {
+      return st;
+    }
+    p.out = out;
+    p.ldo = ldo;
+    p.groups = groups;
+    p.epi = epi;
+    p.epi.vec_out = row_vec(out, ldo);
+    p.M = groups.rows;
+    p.N = cols;
+    p.tiles_m = ceil_div(groups.rows, LP::kTile);
+    p.tiles_n = ceil_div(cols, LP::kTile);
+    p.num_kb = num_kb;
+    p.zero_others = zero_others ? 1u : 0u;
+    const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
+    const uint64_t tiles =
+        (groups.offsets == nullptr ? uint64_t(p.tiles_m)
+                                   : uint64_t(groups.num < groups.rows ? groups.num : groups.rows) +
+                                         groups.rows / LP::kTile) *
+        p.tiles_n;
+    const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
+    e = grad ? launch_ex(LP::gemm_linear_pair_kernel<false, true, false>, p, grid, LP::kThreads, LP::kSmemBytes, 2,
+                         stream)
+             : launch_ex(LP::gemm_linear_pair_kernel<false, false, false>, p, grid, LP::kThreads, LP::kSmemBytes, 2,
+                         stream);
+    if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
+    return ARC_OK;
+  }
+  LS::Params p = {};
+  if (int st = encode_groups_3d(&p.tm_w, w, w_cols, w_rows, groups.num, ldw, w_stride, 64, grad ? 64 : LS::kRows,
+                                "weights")) {
+    return st;
+  }
+  if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a, inner, groups.rows, lda, 64, plan.bn,
+                         CU_TENSOR_MAP_SWIZZLE_128B, "rows")) {
+    return st;
+  }
+  p.out = out;
+  p.ldo = ldo;
+  p.groups = groups;
+  p.epi = epi;
+  p.cols = cols;
+  p.tiles_n = ceil_div(cols, LS::kRows);
+  p.num_kb = num_kb;
+  p.splits = plan.splits;
+  p.zero_others = zero_others ? 1u : 0u;
+  const uint64_t grid = uint64_t(plan.row_tiles) * p.tiles_n * plan.splits;
+  if (grid > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
+  e = grad ? launch_stream_bn<true>(p, plan.bn, static_cast<uint32_t>(grid), stream)
+           : launch_stream_bn<false>(p, plan.bn, static_cast<uint32_t>(grid), stream);
+  if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_stream_kernel launch");
+  return ARC_OK;
+}
+
+// Checks shared by the grouped entry points.
+int grouped_check(const char* what, const void* a, const void* b, const void* c, const int32_t* offsets, int T, int E,
+                  int N, int K) {
+  if (a == nullptr || b == nullptr || c == nullptr) return fail(ARC_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (T <= 0 || E <= 0 || N <= 0 || K <= 0) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: sizes must be positive (T=%d E=%d N=%d K=%d)", what, T, E, N, K);
+  }
+  if (E > static_cast<int>(arcb::lin::kMaxGroups)) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: at most %u groups (got %d)", what, arcb::lin::kMaxGroups, E);
+  }
+  if (offsets == nullptr && E != 1) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: null offsets mean one group, got %d", what, E);
+  }
+  if (reinterpret_cast<uintptr_t>(offsets) & 3u) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: offsets must be 4-byte aligned", what);
+  }
+  return ARC_OK;
+}
+
+int operand_check(const char* what, const char* name, const void* p, int64_t ld, int64_t cols) {
+  if (ld < cols) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: leading dimension of %s too small (%lld < %lld)", what, name,
+                static_cast<long long>(ld), static_cast<long long>(cols));
+  }
+  if (!aligned16(p) || ld % 8 != 0) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: %s must be 16-byte aligned with a leading dimension that is a multiple of 8",
+                what, name);
+  }
+  return ARC_OK;
+}
+
+int output_check(const char* what, const char* name, const void* p, int64_t ld, int64_t cols) {
+  if (ld < cols) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: leading dimension of %s too small (%lld < %lld)", what, name,
+                static_cast<long long>(ld), static_cast<long long>(cols));
+  }
+  if (reinterpret_cast<uintptr_t>(p) & 1u) return fail(ARC_ERR_UNSUPPORTED, "%s: %s is misaligned", what, name);
+  return ARC_OK;
+}
+
+// Row blocks of the dz pass: enough blocks to fill the GPU several times over, at least 16
+// rows each.
+uint32_t dz_row_blocks(uint32_t M, uint32_t N, uint32_t sms) {
+  const uint32_t col_blocks = ceil_div(N, LB::kColsPerBlock);
+  const uint32_t want = ceil_div(6 * sms, col_blocks), most = ceil_div(M, 16);
+  return want < most ? want : most;
+}
+constexpr uint32_t kDzSms = 148;  // the workspace size must not depend on the device
+
+}  // namespace
+
+extern "C" {
+
+int arc_linear_bf16(const uint16_t* x, const uint16_t* w, const uint16_t* bias, const uint16_t* residual,
+                    uint16_t* out, uint16_t* z, int M, int N, int K, int64_t ldx, int64_t ldw, int64_t ldr,
+                    int64_t ldo, int64_t ldz, int activation, cudaStream_t stream) {
+  const char* what = "arc_linear_bf16";
+  g_last_error[0] = '\0';
+  if (x == nullptr || w == nullptr || out == nullptr) return fail(ARC_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  if (M <= 0 || N <= 0 || K <= 0) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: sizes must be positive (M=%d N=%d K=%d)", what, M, N, K);
+  }
+  if (activation < ARC_ACT_NONE || activation > ARC_ACT_SILU) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, activation);
+  }
+  if (int st = operand_check(what, "x", x, ldx, K)) return st;
+  if (int st = operand_check(what, "w", w, ldw, K)) return st;
+  if (int st = output_check(what, "out", out, ldo, N)) return st;
+  if (residual != nullptr) {
+    if (int st = output_check(what, "residual", residual, ldr, N)) return st;
+  }
+  if (z != nullptr) {
+    if (int st = output_check(what, "z", z, ldz, N)) return st;
+  }
+  if (reinterpret_cast<uintptr_t>(bias) & 1u) return fail(ARC_ERR_UNSUPPORTED, "%s: bias is misaligned", what);
+  arcb::lin::Epilogue epi = {};
+  epi.bias = bias;
+  epi.residual = residual;
+  epi.z = z;
+  epi.ldr = residual != nullptr ? ldr : 0;
+  epi.ldz = z != nullptr ? ldz : 0;
+  epi.act = static_cast<uint32_t>(activation);
+  epi.vec_bias = row_vec(bias, 0);
+  epi.vec_residual = row_vec(residual, epi.ldr);
+  epi.vec_z = row_vec(z, epi.ldz);
+  const arcb::lin::Groups groups = {nullptr, 1u, static_cast<uint32_t>(M)};
+  return linear_rows(x, w, groups, out, N, K, ldx, ldw, uint64_t(N) * ldw, ldo, epi, false, false, stream);
+}
+
+int arc_linear_dz_workspace_bytes(int M, int N, size_t* bytes) {
+  if (bytes == nullptr || M <= 0 || N <= 0) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "arc_linear_dz_workspace_bytes: bad argument");
+  }
+  *bytes = size_t(dz_row_blocks(M, N, kDzSms)) * N * sizeof(float);
+  return ARC_OK;
+}
+
+int arc_linear_dz(const uint16_t* dy, const uint16_t* z, uint16_t* dz, uint16_t* dbias, void* workspace,
+                  size_t workspace_bytes, int M, int N, int64_t lddy, int64_t ldz, int64_t lddz, int activation,
+                  cudaStream_t stream) {
+  const char* what = "arc_linear_dz";
+  g_last_error[0] = '\0';
+  if (dy == nullptr || (dz == nullptr && dbias == nullptr)) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  }
+  if (M <= 0 || N <= 0) return fail(ARC_ERR_INVALID_ARGUMENT, "%s: sizes must be positive (M=%d N=%d)", what, M, N);
+  if (activation < ARC_ACT_NONE || activation > ARC_ACT_SILU) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, activation);
+  }
+  if (activation != ARC_ACT_NONE && z == nullptr) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: an activation's gradient needs z", what);
+  }
+  if (int st = output_check(what, "dy", dy, lddy, N)) return st;
+  if (z != nullptr) {
+    if (int st = output_check(what, "z", z, ldz, N)) return st;
+  }
+  if (dz != nullptr) {
+    if (int st = output_check(what, "dz", dz, lddz, N)) return st;
+  }
+  if (reinterpret_cast<uintptr_t>(dbias) & 1u) return fail(ARC_ERR_UNSUPPORTED, "%s: dbias is misaligned", what);
+  const uint32_t row_blocks = dz_row_blocks(M, N, kDzSms);
+  if (dbias != nullptr && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 3u) ||
+                           workspace_bytes < size_t(row_blocks) * N * sizeof(float))) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: dbias needs a 4-byte aligned workspace of %zu bytes", what,
+                size_t(row_blocks) * N * sizeof(float));
+  }
+  int dev = 0;
+  if (int st = current_device(&dev)) return st;
+  LB::Params p = {};
+  p.dy = dy;
+  p.z = activation == ARC_ACT_NONE ? nullptr : z;
+  p.dz = dz;
+  p.partial = dbias != nullptr ? static_cast<float*>(workspace) : nullptr;
+  p.lddy = lddy;
+  p.ldz = ldz;
+  p.lddz = lddz;
+  p.M = M;
+  p.N = N;
+  p.act = static_cast<uint32_t>(activation);
+  p.rows_per_block = ceil_div(M, row_blocks);
+  const bool vec = N % 8 == 0 && row_vec(dy, lddy) != 0 && (p.z == nullptr || row_vec(z, ldz) != 0) &&
+                   (dz == nullptr || row_vec(dz, lddz) != 0);
+  const dim3 grid(ceil_div(N, LB::kColsPerBlock), row_blocks, 1);
+  cudaError_t e = vec ? launch_grid(LB::linear_dz_kernel<true>, grid, LB::kThreads, 0, stream, p)
+                      : launch_grid(LB::linear_dz_kernel<false>, grid, LB::kThreads, 0, stream, p);
+  if (e != cudaSuccess) return cuda_fail(e, "linear_dz_kernel launch");
+  if (dbias != nullptr) {
+    e = launch_grid(LB::linear_dbias_kernel, dim3(ceil_div(N, LB::kThreads), 1, 1), LB::kThreads, 0, stream,
+                    static_cast<const float*>(p.partial), dbias, uint32_t(N), row_blocks);
+    if (e != cudaSuccess) return cuda_fail(e, "linear_dbias_kernel launch");
+  }
+  return ARC_OK;
+}
+
+int arc_grouped_matmul(const uint16_t* x, const uint16_t* w, const int32_t* offsets, uint16_t* out, int T, int E,
+                       int N, int K, int64_t ldx, int64_t ldw, int64_t w_stride, int64_t ldo, unsigned flags,
+                       cudaStream_t stream) {
+  const char* what = "arc_grouped_matmul";
+  g_last_error[0] = '\0';
+  if (int st = grouped_check(what, x, w, out, offsets, T, E, N, K)) return st;
+  if (flags & ~ARC_GROUPED_ZERO_OTHERS) return fail(ARC_ERR_INVALID_ARGUMENT, "%s: unknown flags 0x%x", what, flags);
+  if (int st = operand_check(what, "x", x, ldx, K)) return st;
+  if (int st = operand_check(what, "w", w, ldw, K)) return st;
+  if (int st = operand_check(what, "w's groups", w, w_stride, int64_t(N - 1) * ldw + K)) return st;
+  if (int st = output_check(what, "out", out, ldo, N)) return st;
+  const arcb::lin::Groups groups = {offsets, static_cast<uint32_t>(E), static_cast<uint32_t>(T)};
+  return linear_rows(x, w, groups, out, N, K, ldx, ldw, w_stride, ldo, arcb::lin::Epilogue{}, false,
+                     (flags & ARC_GROUPED_ZERO_OTHERS) != 0 && offsets != nullptr, stream);
+}
+
+int arc_grouped_matmul_dx(const uint16_t* dy, const uint16_t* w, const int32_t* offsets, uint16_t* dx, int T, int E,
+                          int N, int K, int64_t lddy, int64_t ldw, int64_t w_stride, int64_t lddx, unsigned flags,
+                          cudaStream_t stream) {
+  const char* what = "arc_grouped_matmul_dx";
+  g_last_error[0] = '\0';
+  if (int st = grouped_check(what, dy, w, dx, offsets, T, E, N, K)) return st;
+  if (flags & ~ARC_GROUPED_ZERO_OTHERS) return fail(ARC_ERR_INVALID_ARGUMENT, "%s: unknown flags 0x%x", what, flags);
+  if (int st = operand_check(what, "dy", dy, lddy, N)) return st;
+  if (int st = operand_check(what, "w", w, ldw, K)) return st;
+  if (int st = operand_check(what, "w's groups", w, w_stride, int64_t(N - 1) * ldw + K)) return st;
+  if (int st = output_check(what, "dx", dx, lddx, K)) return st;
+  const arcb::lin::Groups groups = {offsets, static_cast<uint32_t>(E), static_cast<uint32_t>(T)};
+  return linear_rows(dy, w, groups, dx, K, N, lddy, ldw, w_stride, lddx, arcb::lin::Epilogue{}, true,
+                     (flags & ARC_GROUPED_ZERO_OTHERS) != 0 && offsets != nullptr, stream);
+}
+
+int arc_grouped_matmul_dw(const uint16_t* dy, const uint16_t* x, const int32_t* offsets, uint16_t* dw, int T, int E,
+                          int N, int K, int64_t lddy, int64_t ldx, int64_t lddw, int64_t dw_stride,
+                          cudaStream_t stream) {
+  const char* what = "arc_grouped_matmul_dw";
+  g_last_error[0] = '\0';
+  if (int st = grouped_check(what, dy, x, dw, offsets, T, E, N, K)) return st;
+  if (int st = operand_check(what, "dy", dy, lddy, N)) return st;
+  if (int st = operand_check(what, "x", x, ldx, K)) return st;
+  if (int st = output_check(what, "dw", dw, lddw, K)) return st;
+  if (int st = output_check(what, "dw's groups", dw, dw_stride, int64_t(N - 1) * lddw + K)) return st;
+  int dev = 0;
+  if (int st = current_device(&dev)) return st;
+  const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
+  if (max_pairs == 0) return fail(ARC_ERR_UNSUPPORTED, "%s: no CTA pair fits on this device", what);
+  LP::Params p = {};
+  if (int st = encode_groups_3d(&p.tm_a, dy, N, T, 1, lddy, uint64_t(T) * lddy, 64, 64, "dy")) return st;
+  if (int st = encode_groups_3d(&p.tm_b, x, K, T, 1, ldx, uint64_t(T) * ldx, 64, 64, "x")) return st;
+  p.out = dw;
+  p.ldo = lddw;
+  p.out_group = dw_stride;
+  p.groups = {offsets, static_cast<uint32_t>(E), static_cast<uint32_t>(T)};
+  p.epi.vec_out = row_vec(dw, lddw, dw_stride);
+  p.M = N;
+  p.N = K;
+  p.tiles_m = ceil_div(N, LP::kTile);
+  p.tiles_n = ceil_div(K, LP::kTile);
+  const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n * E;
+  if (tiles > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "%s: too many tiles for one launch", what);
+  const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
+  const cudaError_t e = launch_ex(LP::gemm_linear_pair_kernel<true, true, true>, p, grid, LP::kThreads, LP::kSmemBytes,
+                                  2, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
+  return ARC_OK;
+}
+
+}  // extern "C"

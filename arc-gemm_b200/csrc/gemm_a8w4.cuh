@@ -53,6 +53,9 @@
 // gemm_a8w4_decode.cuh instead.
 #pragma once
 
+#include <type_traits>
+
+#include "linear_common.cuh"
 #include "sm100.cuh"
 
 namespace arcb {
@@ -96,16 +99,23 @@ struct Params {
   uint32_t split;      // Wp in the pre-packed layout (expand_piece)
 };
 
+// The grouped product: the rows of group e times the weight rows [e*N, (e+1)*N) of Wp and sb.
+// tm_wp then covers all groups' rows; M is the number of token rows.
+struct GroupedParams : Params {
+  lin::Groups groups;
+  uint32_t zero_others;  // zero the output rows of no group
+};
+
 template <uint32_t BT, uint32_t EWG, uint32_t LS>
 struct Cfg {
-  static_assert(BT == 64 || BT == 128, "token tile");
+  static_assert(BT == 16 || BT == 32 || BT == 64 || BT == 128, "token tile");
   static_assert(EWG == 1 || EWG == 2, "epilogue warpgroups");
   static_assert(LS >= 2 && LS <= kDoneRing && kUnpacked <= kDoneRing && kAccPairs < kDoneRing,
                 "each waiter must stay within one phase of its completion barrier");
   static constexpr uint32_t kThreads = 256 + 128 * EWG;
   static constexpr uint32_t kCols = BT / EWG;               // columns per epilogue thread
-  static constexpr uint32_t kChunk = 32;                    // TMEM columns per load
-  static constexpr uint32_t kTmemCols = kAccPairs * kGps * BT;  // 256 or 512
+  static constexpr uint32_t kChunk = kCols < 32 ? kCols : 32;  // TMEM columns per load
+  static constexpr uint32_t kTmemCols = kAccPairs * kGps * BT;  // 64 to 512
   static constexpr uint32_t kTokBytes = BT * kGroupK;       // one group's token box
   static constexpr uint32_t kWpBytes = kRows * kPackedRow * kGps;
   static constexpr uint32_t kWBytes = kRows * kGroupK;      // one group's unpacked tile
@@ -135,6 +145,11 @@ struct alignas(1024) Smem {
   uint32_t abort;
 };
 
+template <uint32_t BT, uint32_t EWG, uint32_t LS>
+struct alignas(1024) GroupedSmem : Smem<BT, EWG, LS> {
+  uint32_t prefix[lin::kMaxGroups + 1];  // row tiles of the groups before each one
+};
+
 // Parity of the completion of mma_done that belongs to step si.
 __device__ __forceinline__ uint32_t done_parity(uint32_t si) { return (si / kDoneRing) & 1u; }
 
@@ -143,6 +158,8 @@ __device__ __forceinline__ uint32_t done_parity(uint32_t si) { return (si / kDon
 // ---------------------------------------------------------------------------------
 struct Work {
   uint32_t m0, n0, g_begin, g_end;
+  uint32_t m_end;  // end of the tile's token rows
+  uint32_t w_row;  // weight row of output column 0 (grouped: the group's first)
 };
 
 // Tile order for the persistent decomposition: weight tiles of one band of token
@@ -166,6 +183,33 @@ __device__ __forceinline__ bool next_work(const Params& p, uint32_t& cursor, Wor
   tile_of(p, t, mt, nt);
   w.m0 = mt * BT;
   w.n0 = nt * p.R;
+  w.g_begin = 0;
+  w.g_end = p.G;
+  w.m_end = p.M;
+  w.w_row = 0;
+  return true;
+}
+
+// The grouped walk: group after group, inside a group the order of tile_of.
+template <uint32_t BT>
+__device__ __forceinline__ bool next_work_grouped(const GroupedParams& p, const uint32_t* prefix, uint32_t& cursor,
+                                                  Work& w) {
+  const uint32_t t = blockIdx.x + cursor * gridDim.x;
+  if (t >= prefix[p.groups.num] * p.tiles_n) return false;
+  ++cursor;
+  constexpr uint32_t kBand = 4;
+  const uint32_t e = lin::group_of_tile(prefix, p.groups.num, t / p.tiles_n);
+  const uint32_t tiles_m = prefix[e + 1] - prefix[e];
+  uint32_t rem = t - prefix[e] * p.tiles_n;
+  const uint32_t band = rem / (kBand * p.tiles_n);
+  rem -= band * kBand * p.tiles_n;
+  const uint32_t m_first = band * kBand;
+  const uint32_t m_cnt = min(kBand, tiles_m - m_first);
+  const uint32_t first = lin::group_begin(p.groups, e);
+  w.m0 = first + (m_first + rem % m_cnt) * BT;
+  w.m_end = first + lin::group_count(p.groups, e);
+  w.n0 = rem / m_cnt * p.R;
+  w.w_row = e * p.N;
   w.g_begin = 0;
   w.g_end = p.G;
   return true;
@@ -200,11 +244,12 @@ __device__ __forceinline__ void expand_piece(const uint4& x, uint32_t split, uin
 // ---------------------------------------------------------------------------------
 // Kernel
 // ---------------------------------------------------------------------------------
-template <uint32_t BT, uint32_t EWG, uint32_t LS>
-__global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
-    gemm_a8w4_kernel(const __grid_constant__ Params p) {
+// P: Params (one weight matrix) or GroupedParams (row groups, each with its own).
+template <uint32_t BT, uint32_t EWG, uint32_t LS, typename P>
+__device__ __forceinline__ void gemm_a8w4_body(const P& p) {
+  constexpr bool kGrouped = std::is_same<P, GroupedParams>::value;
   using C = Cfg<BT, EWG, LS>;
-  using S_t = Smem<BT, EWG, LS>;
+  using S_t = typename std::conditional<kGrouped, GroupedSmem<BT, EWG, LS>, Smem<BT, EWG, LS>>::type;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   S_t& s = *reinterpret_cast<S_t*>(smem_raw + smem_align_pad(smem_raw));
   const uint32_t warp = warp_idx_sync();
@@ -254,6 +299,18 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
   // dependent launch); global memory is only touched after it has completed.
   pdl_wait();
   if (threadIdx.x == 0) probe_mark(57);
+  if constexpr (kGrouped) {
+    if (warp == 2) lin::group_tiles_prefix(p.groups, BT, s.prefix);
+    if (p.zero_others) lin::zero_other_rows(p.groups, p.out, p.ldc, p.N, blockIdx.x, gridDim.x);
+    __syncthreads();
+  }
+  const auto next = [&](uint32_t& cursor, Work& w) {
+    if constexpr (kGrouped) {
+      return next_work_grouped<BT>(p, s.prefix, cursor, w);
+    } else {
+      return next_work<BT>(p, cursor, w);
+    }
+  };
 
   // Register moves sit inside each role's branch, so that the compiler gives every
   // role's code the budget of that role.
@@ -264,7 +321,7 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
       uint32_t stage = 0, si = 0, cursor = 0;
       Work w;
       bool ok = true;
-      while (ok && next_work<BT>(p, cursor, w)) {
+      while (ok && next(cursor, w)) {
         for (uint32_t t = 0; t < steps_per_tile; ++t, ++si) {
           // Stage `stage` last served step si - LS; its UMMAs (which ran after the
           // unpack warps had read the packed half) must have retired.
@@ -288,7 +345,7 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
             }
           }
           tma_load_2d(&p.tm_wp, &s.load_full[stage], s.wp[stage], int32_t(g0 * kPackedRow),
-                      int32_t(w.n0), kCacheEvictFirst);
+                      int32_t(w.w_row + w.n0), kCacheEvictFirst);
           if (++stage == LS) stage = 0;
         }
       }
@@ -306,7 +363,7 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
       uint32_t stage = 0, phase = 0, us = 0, uphase = 0, si = 0, cursor = 0;
       Work w;
       bool ok = true;
-      while (ok && next_work<BT>(p, cursor, w)) {
+      while (ok && next(cursor, w)) {
         for (uint32_t t = 0; t < steps_per_tile; ++t, ++si) {
           const uint32_t pair = si % kAccPairs;
           const uint32_t acc_parity = (si / kAccPairs - 1u) & 1u;
@@ -369,7 +426,7 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
     const uint32_t c16 = ut & 3u;
     Work w;
     bool ok = true;
-    while (ok && next_work<BT>(p, cursor, w)) {
+    while (ok && next(cursor, w)) {
       for (uint32_t t = 0; t < steps_per_tile; ++t, ++si) {
         // Packed tile landed, and the UMMAs that read w[us] last time have retired
         // (both tested at once).
@@ -430,7 +487,7 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
     uint32_t pre = 0;  // step si's partials seen complete by an early test
     Work w;
     bool ok = true;
-    while (ok && next_work<BT>(p, cursor, w)) {
+    while (ok && next(cursor, w)) {
       const uint32_t n = w.n0 + nl;
       const bool n_valid = (nl < p.R) && (n < p.N);
       uint64_t acc[kPairs];
@@ -442,7 +499,7 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
       // latency every group, so with 16-byte-aligned rows (the usual case) the
       // scales come in 8-group vectors two windows ahead: `win0` holds the scales
       // of the next groups (consumed 16 bits at a time), `win1` the 8 after those.
-      const uint16_t* sb_row = p.sb + size_t(n) * p.ldsb;
+      const uint16_t* sb_row = p.sb + (size_t(w.w_row) + n) * p.ldsb;
       uint4 win0 = make_uint4(0, 0, 0, 0), win1 = make_uint4(0, 0, 0, 0);
       float s_next = 0.f;
       if (n_valid && w.g_begin < w.g_end) {
@@ -491,7 +548,11 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
           uint32_t r[C::kCols];
 #pragma unroll
           for (uint32_t c0 = 0; c0 < C::kCols; c0 += C::kChunk) {
-            tmem_ld_32x32b_x32(t_row + c0, *reinterpret_cast<uint32_t(*)[32]>(r + c0));
+            if constexpr (C::kChunk == 16) {
+              tmem_ld_32x32b_x16(t_row + c0, *reinterpret_cast<uint32_t(*)[16]>(r + c0));
+            } else {
+              tmem_ld_32x32b_x32(t_row + c0, *reinterpret_cast<uint32_t(*)[32]>(r + c0));
+            }
           }
           // Ask early whether the next step's partials are ready; the answer arrives
           // while the loads are in flight.
@@ -508,7 +569,7 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
 #pragma unroll
             for (uint32_t j = 0; j < C::kCols; ++j) {
               const uint32_t m = w.m0 + col0 + j;
-              if (m < p.M) {
+              if (m < w.m_end) {
                 p.partials[(size_t(m) * p.N + n) * p.G + g] =
                     static_cast<int32_t>(r[j] - kBiasBits) >> 4;
               }
@@ -541,10 +602,10 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
           float a0, a1;
           f32x2_unpack(acc[j], a0, a1);
           const uint32_t m = w.m0 + col0 + 2 * j;
-          if (m < p.M) {
+          if (m < w.m_end) {
             o[size_t(m) * p.ldc] = __bfloat16_as_ushort(__float2bfloat16_rn(a0 * __ldg(p.sa + m)));
           }
-          if (m + 1 < p.M) {
+          if (m + 1 < w.m_end) {
             o[size_t(m + 1) * p.ldc] =
                 __bfloat16_as_ushort(__float2bfloat16_rn(a1 * __ldg(p.sa + m + 1)));
           }
@@ -563,6 +624,18 @@ __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
     tc_fence_after_sync();
     tmem_dealloc(tmem_base, C::kTmemCols);
   }
+}
+
+template <uint32_t BT, uint32_t EWG, uint32_t LS>
+__global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
+    gemm_a8w4_kernel(const __grid_constant__ Params p) {
+  gemm_a8w4_body<BT, EWG, LS>(p);
+}
+
+template <uint32_t BT, uint32_t EWG, uint32_t LS>
+__global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
+    gemm_a8w4_grouped_kernel(const __grid_constant__ GroupedParams p) {
+  gemm_a8w4_body<BT, EWG, LS>(p);
 }
 
 }  // namespace a8w4

@@ -1,0 +1,110 @@
+// linear_backward.cuh — what lies between a linear layer's output gradient and its two products.
+//
+//   dz[m, n] = dy[m, n] * act'(z[m, n])     dbias[n] = sum_m dz[m, n]
+//
+// One pass over dy and z writes dz (bf16: it is the next two products' tensor-core operand)
+// and sums the unrounded dz by column in fp32, each block its own rows; a second, small kernel
+// adds the blocks' sums in order, so the result does not depend on timing. HBM-bound: 6 bytes
+// per element with an activation.
+#pragma once
+
+#include "linear_common.cuh"
+
+namespace arcb {
+namespace linbwd {
+
+constexpr uint32_t kThreads = 256;
+constexpr uint32_t kColsPerBlock = 256;  // 32 threads x 8 columns
+constexpr uint32_t kRowLanes = 8;
+
+struct Params {
+  const uint16_t* dy;  // [M][lddy]
+  const uint16_t* z;   // [M][ldz] or null (no activation)
+  uint16_t* dz;        // [M][lddz] or null
+  float* partial;      // [gridDim.y][N] or null
+  uint64_t lddy, ldz, lddz;
+  uint32_t M, N, act, rows_per_block;
+};
+
+// VEC: every row of dy, z and dz is 16-byte aligned and N is a multiple of 8.
+template <bool VEC>
+__global__ void __launch_bounds__(kThreads) linear_dz_kernel(const Params p) {
+  __shared__ float sums[kRowLanes][kColsPerBlock];
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t tx = threadIdx.x & 31u, ty = threadIdx.x >> 5;
+  const uint32_t n0 = blockIdx.x * kColsPerBlock;
+  const uint32_t m_begin = blockIdx.y * p.rows_per_block;
+  const uint32_t m_end = min(p.M, m_begin + p.rows_per_block);
+  float acc[8];
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j) acc[j] = 0.f;
+  if (VEC) {
+    const uint32_t n = n0 + tx * 8u;
+    if (n < p.N) {
+#pragma unroll 4
+      for (uint32_t m = m_begin + ty; m < m_end; m += kRowLanes) {
+        const uint4 g = __ldg(reinterpret_cast<const uint4*>(p.dy + size_t(m) * p.lddy + n));
+        float v[8] = {__uint_as_float(g.x << 16), __uint_as_float(g.x & 0xFFFF0000u),
+                      __uint_as_float(g.y << 16), __uint_as_float(g.y & 0xFFFF0000u),
+                      __uint_as_float(g.z << 16), __uint_as_float(g.z & 0xFFFF0000u),
+                      __uint_as_float(g.w << 16), __uint_as_float(g.w & 0xFFFF0000u)};
+        if (p.z != nullptr) {
+          const uint4 a = __ldg(reinterpret_cast<const uint4*>(p.z + size_t(m) * p.ldz + n));
+          const float zv[8] = {__uint_as_float(a.x << 16), __uint_as_float(a.x & 0xFFFF0000u),
+                               __uint_as_float(a.y << 16), __uint_as_float(a.y & 0xFFFF0000u),
+                               __uint_as_float(a.z << 16), __uint_as_float(a.z & 0xFFFF0000u),
+                               __uint_as_float(a.w << 16), __uint_as_float(a.w & 0xFFFF0000u)};
+#pragma unroll
+          for (uint32_t j = 0; j < 8; ++j) v[j] *= lin::act_slope(zv[j], p.act);
+        }
+        if (p.dz != nullptr) {
+          *reinterpret_cast<uint4*>(p.dz + size_t(m) * p.lddz + n) =
+              make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                         pack_bf16x2(v[6], v[7]));
+        }
+#pragma unroll
+        for (uint32_t j = 0; j < 8; ++j) acc[j] += v[j];
+      }
+    }
+  } else {
+    for (uint32_t m = m_begin + ty; m < m_end; m += kRowLanes) {
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t n = n0 + j * 32u + tx;
+        if (n < p.N) {
+          float v = bf16_bits_to_float(__ldg(p.dy + size_t(m) * p.lddy + n));
+          if (p.z != nullptr) v *= lin::act_slope(bf16_bits_to_float(__ldg(p.z + size_t(m) * p.ldz + n)), p.act);
+          if (p.dz != nullptr) p.dz[size_t(m) * p.lddz + n] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+          acc[j] += v;
+        }
+      }
+    }
+  }
+  if (p.partial == nullptr) return;
+#pragma unroll
+  for (uint32_t j = 0; j < 8; ++j) sums[ty][VEC ? tx * 8u + j : j * 32u + tx] = acc[j];
+  __syncthreads();
+  const uint32_t n = n0 + threadIdx.x;
+  if (n < p.N) {
+    float v = 0.f;
+#pragma unroll
+    for (uint32_t i = 0; i < kRowLanes; ++i) v += sums[i][threadIdx.x];
+    p.partial[size_t(blockIdx.y) * p.N + n] = v;
+  }
+}
+
+__global__ void __launch_bounds__(kThreads) linear_dbias_kernel(const float* partial, uint16_t* dbias, uint32_t N,
+                                                               uint32_t blocks) {
+  pdl_launch_dependents();
+  pdl_wait();
+  const uint32_t n = blockIdx.x * kThreads + threadIdx.x;
+  if (n >= N) return;
+  float v = 0.f;
+#pragma unroll 8
+  for (uint32_t i = 0; i < blocks; ++i) v += partial[size_t(i) * N + n];
+  dbias[n] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
+}
+
+}  // namespace linbwd
+}  // namespace arcb

@@ -1,0 +1,252 @@
+// linear_common.cuh — what the linear and grouped product kernels share: the row groups, the
+// epilogue's activation functions and the 16-bit row vectors of 32 columns.
+#pragma once
+
+#include "sm100.cuh"
+
+namespace arcb {
+namespace lin {
+
+constexpr uint32_t BK = 64;  // contraction elements per block: one 128-byte swizzle row
+constexpr uint32_t kUmmaK = 16;
+constexpr uint32_t kMaxGroups = 1024;
+
+// ---------------------------------------------------------------------------------
+// Row groups: group e owns rows [offsets[e], offsets[e+1]) of a [rows] x ... matrix. The
+// offsets live on the GPU, so the host knows only `rows`; every bound is clamped to it when
+// it is read, which keeps all accesses in range whatever the offsets hold. A null `offsets`
+// is one group of all rows.
+// ---------------------------------------------------------------------------------
+struct Groups {
+  const int32_t* offsets;  // [num + 1] or null
+  uint32_t num, rows;
+};
+
+__device__ __forceinline__ uint32_t group_bound(const Groups& g, uint32_t e) {
+  if (g.offsets == nullptr) return e == 0u ? 0u : g.rows;
+  const int32_t v = __ldg(g.offsets + e);
+  return v < 0 ? 0u : min(static_cast<uint32_t>(v), g.rows);
+}
+
+__device__ __forceinline__ uint32_t group_begin(const Groups& g, uint32_t e) { return group_bound(g, e); }
+__device__ __forceinline__ uint32_t group_count(const Groups& g, uint32_t e) {
+  const uint32_t a = group_bound(g, e), b = group_bound(g, e + 1u);
+  return b > a ? b - a : 0u;
+}
+
+// One warp: prefix[e] = tiles of the groups before e (each group has ceil(count / tile)
+// row tiles), prefix[num] = all of them. Offsets that decrease or leave [0, rows] set the
+// status bit that arc_device_status reports.
+__device__ __forceinline__ void group_tiles_prefix(const Groups& g, uint32_t tile, uint32_t* prefix) {
+  const uint32_t lane = threadIdx.x & 31u;
+  uint32_t base = 0;
+  for (uint32_t e0 = 0; e0 < g.num; e0 += 32u) {
+    const uint32_t e = e0 + lane;
+    uint32_t c = 0;
+    if (e < g.num) {
+      if (g.offsets != nullptr) {
+        const int32_t a = __ldg(g.offsets + e), b = __ldg(g.offsets + e + 1u);
+        if (a < 0 || b < a || static_cast<uint32_t>(b) > g.rows) atomicOr(&g_arc_status, kStatusBadOffsets);
+      }
+      c = (group_count(g, e) + tile - 1u) / tile;
+    }
+    uint32_t incl = c;
+#pragma unroll
+    for (uint32_t d = 1; d < 32u; d <<= 1) {
+      const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += o;
+    }
+    if (e < g.num) prefix[e] = base + incl - c;
+    base += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  if (lane == 0) prefix[g.num] = base;
+}
+
+// The group that row tile t belongs to: the last e with prefix[e] <= t (t < prefix[num]), so
+// that groups without rows, whose prefix equals their successor's, are passed over.
+__device__ __forceinline__ uint32_t group_of_tile(const uint32_t* prefix, uint32_t num, uint32_t t) {
+  uint32_t lo = 0, hi = num;
+  while (hi - lo > 1u) {
+    const uint32_t mid = (lo + hi) >> 1;
+    if (prefix[mid] <= t) {
+      lo = mid;
+    } else {
+      hi = mid;
+    }
+  }
+  return lo;
+}
+
+// Zero the output rows that belong to no group (before the first and behind the last),
+// striped over the blocks of the grid; every thread of the block takes part.
+__device__ __forceinline__ void zero_other_rows(const Groups& g, uint16_t* out, size_t ldo, uint32_t cols,
+                                                uint32_t block, uint32_t num_blocks) {
+  const uint32_t first = group_bound(g, 0), last = group_bound(g, g.num);
+  const uint32_t behind = last < g.rows ? g.rows - last : 0u;
+  for (uint32_t i = block; i < first + behind; i += num_blocks) {
+    uint16_t* row = out + size_t(i < first ? i : last + (i - first)) * ldo;
+    for (uint32_t c = threadIdx.x; c < cols; c += blockDim.x) row[c] = 0;
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// Activations (fp32). gelu is the erf form, gelu_tanh the tanh form.
+// ---------------------------------------------------------------------------------
+enum Act : uint32_t { kActNone = 0, kActRelu = 1, kActGelu = 2, kActGeluTanh = 3, kActSilu = 4 };
+
+constexpr float kSqrtHalf = 0.70710678118654752f;
+constexpr float kSqrt2OverPi = 0.79788456080286536f;
+constexpr float kInvSqrt2Pi = 0.39894228040143268f;
+constexpr float kGeluCubic = 0.044715f;
+
+__device__ __forceinline__ float sigmoidf(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+
+// The tanh form's argument. 1 + tanh(u) = 2 sigmoid(2u), which keeps its relative accuracy
+// in the lower tail, where 1 + tanh(u) would cancel.
+__device__ __forceinline__ float gelu_tanh_arg(float z) {
+  return 2.f * kSqrt2OverPi * (z + kGeluCubic * z * z * z);
+}
+
+// In the lower tail 1 + erf cancels to an absolute error of about 2^-24 |z|, far below the
+// output's own rounding for every value that is not itself about that small.
+__device__ __forceinline__ float act_value(float z, uint32_t act) {
+  switch (act) {
+    case kActRelu:
+      return z > 0.f ? z : (z != z ? z : 0.f);
+    case kActGelu:
+      return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+    case kActGeluTanh:
+      return z * sigmoidf(gelu_tanh_arg(z));
+    case kActSilu:
+      return z * sigmoidf(z);
+    default:
+      return z;
+  }
+}
+
+// d act / d z.
+__device__ __forceinline__ float act_slope(float z, uint32_t act) {
+  switch (act) {
+    case kActRelu:
+      return z > 0.f ? 1.f : 0.f;
+    case kActGelu:
+      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
+    case kActGeluTanh: {
+      const float s = sigmoidf(gelu_tanh_arg(z));
+      return s + z * s * (1.f - s) * (2.f * kSqrt2OverPi) * (1.f + 3.f * kGeluCubic * z * z);
+    }
+    case kActSilu: {
+      const float s = sigmoidf(z);
+      return s * (1.f + z * (1.f - s));
+    }
+    default:
+      return 1.f;
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// 32 consecutive bf16 columns of one row, of which `cols` are in range. `vec` is the widest
+// access every row allows: 2 = 32 bytes, 1 = 16 bytes, 0 = single elements (the host derives
+// it from the base address and the leading dimension). Full vectors go out wide, the ragged
+// end element by element.
+// ---------------------------------------------------------------------------------
+__device__ __forceinline__ void st_global_32b(void* p, const uint32_t* v) {
+  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
+               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+               : "memory");
+}
+
+__device__ __forceinline__ void ld_global_32b(const void* p, uint32_t* v) {
+  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
+               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
+                 "=r"(v[7])
+               : "l"(p)
+               : "memory");
+}
+
+__device__ __forceinline__ void store_row32(uint16_t* p, const uint32_t (&v)[16], uint32_t cols, uint32_t vec) {
+  if (vec == 2u && cols >= 32u) {
+    st_global_32b(p, v);
+    st_global_32b(p + 16, v + 8);
+  } else if (vec != 0u && cols >= 32u) {
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      *reinterpret_cast<uint4*>(p + 8 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 32; ++j) {
+      if (j < cols) p[j] = static_cast<uint16_t>(v[j >> 1] >> ((j & 1u) * 16u));
+    }
+  }
+}
+
+__device__ __forceinline__ void load_row32(const uint16_t* p, uint32_t (&v)[16], uint32_t cols, uint32_t vec) {
+  if (vec == 2u && cols >= 32u) {
+    ld_global_32b(p, v);
+    ld_global_32b(p + 16, v + 8);
+  } else if (vec != 0u && cols >= 32u) {
+#pragma unroll
+    for (uint32_t j = 0; j < 4; ++j) {
+      const uint4 x = *reinterpret_cast<const uint4*>(p + 8 * j);
+      v[4 * j] = x.x;
+      v[4 * j + 1] = x.y;
+      v[4 * j + 2] = x.z;
+      v[4 * j + 3] = x.w;
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < 16; ++j) v[j] = 0u;
+#pragma unroll
+    for (uint32_t j = 0; j < 32; ++j) {
+      if (j < cols) v[j >> 1] |= static_cast<uint32_t>(p[j]) << ((j & 1u) * 16u);
+    }
+  }
+}
+
+// What follows the product: bias, the activation and the residual, and where the value in
+// front of the activation is kept for a backward pass.
+struct Epilogue {
+  const uint16_t* bias;      // [N] or null
+  const uint16_t* residual;  // [M][ldr] or null
+  uint16_t* z;               // [M][ldz] or null: x w^T + bias, bf16
+  uint64_t ldr, ldz;
+  uint32_t act;
+  uint32_t vec_bias, vec_residual, vec_z, vec_out;
+};
+
+// Shared-memory descriptor of an MN-major operand as a TMA load with the 128-byte swizzle
+// leaves it: chunks of 64 M (or N) elements, each chunk 64 contraction rows of 128 bytes.
+//   leading byte offset  between chunks (64 rows x 128 bytes = 8192)
+//   stride byte offset   between groups of 8 contraction rows (1024)
+// A step of 16 along the contraction is 16 rows, 2048 bytes.
+constexpr uint32_t kMnChunkBytes = 64 * 128;
+constexpr uint32_t kMnStepBytes = 16 * 128;
+__device__ __forceinline__ uint64_t make_sw128_mnmajor_desc(const void* smem_tile) {
+  const uint32_t addr = smem_u32(smem_tile);
+  uint64_t desc = 0;
+  desc |= static_cast<uint64_t>((addr >> 4) & 0x3FFFu);
+  desc |= static_cast<uint64_t>(kMnChunkBytes >> 4) << 16;
+  desc |= static_cast<uint64_t>(1024u >> 4) << 32;
+  desc |= static_cast<uint64_t>(1u) << 46;
+  desc |= static_cast<uint64_t>(2u) << 61;
+  return desc;
+}
+
+template <bool MN>
+__device__ __forceinline__ uint64_t operand_desc(const void* tile) {
+  return MN ? make_sw128_mnmajor_desc(tile) : make_sw128_kmajor_desc(tile);
+}
+// Bytes from one contraction step of 16 to the next.
+template <bool MN>
+__host__ __device__ constexpr uint32_t operand_step() {
+  return MN ? kMnStepBytes : kUmmaK * 2;
+}
+
+template <bool A_MN, bool B_MN>
+__host__ __device__ constexpr uint32_t idesc_of(uint32_t m, uint32_t n) {
+  return idesc_bf16_f32(m, n) | (A_MN ? 1u << 15 : 0u) | (B_MN ? 1u << 16 : 0u);
+}
+
+}  // namespace lin
+}  // namespace arcb

@@ -36,6 +36,7 @@ enum : uint32_t {
   kStatusTimeoutDrain = 1u << 4,
   kStatusTimeoutScales = 1u << 5,
   kStatusTimeoutPeer = 1u << 6,
+  kStatusBadOffsets = 1u << 7,  // group offsets that decrease or leave the rows
 };
 
 // One word per loaded module; every kernel in this translation unit ORs into it.
@@ -201,6 +202,34 @@ __device__ __forceinline__ bool mbar_wait_poll(uint64_t* bar, uint32_t parity,
           atomicOr(&g_arc_status, err_bit);
           return false;
         }
+      }
+    }
+  }
+}
+
+// mbar_wait with an acquire at cluster scope, for a barrier that a CTA of the cluster arrives
+// on after writing its own shared memory.
+__device__ __forceinline__ bool mbar_wait_cluster(uint64_t* bar, uint32_t parity, volatile uint32_t* abort,
+                                                  uint32_t err_bit) {
+  const uint32_t addr = smem_u32(bar);
+  const uint64_t start = globaltimer_ns();
+#pragma unroll 1
+  for (uint32_t it = 1;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity)
+        : "memory");
+    if (ok) return true;
+    if ((it & 15u) == 0u) {
+      if (*abort) return false;
+      if (globaltimer_ns() - start > kWaitTimeoutNs) {
+        *abort = 1u;
+        atomicOr(&g_arc_status, err_bit);
+        return false;
       }
     }
   }

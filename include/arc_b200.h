@@ -291,6 +291,84 @@ int arc_quantize_int8(const void *x, int8_t *q, float *sa, int M, int K, int ldx
                       cudaStream_t stream);
 
 /*
+ * Linear layer: out[m,n] = act( sum_k x[m,k] w[n,k] + bias[n] ) + residual[m,n], bf16 with
+ * fp32 accumulation, bias, activation and addition, rounded once. The epilogue runs in the
+ * GEMM; no reference counterpart beyond the product itself (arc/mm.py:71-79).
+ *   x [M][ldx], w [N][ldw], bias [N] or NULL, residual [M][ldr] or NULL, out [M][ldo]
+ *   z [M][ldz] or NULL: receives x w^T + bias in bf16, what arc_linear_dz needs later
+ * Requirements: M, N, K >= 1 (any sizes); x and w 16-byte aligned with leading dimensions
+ * that are multiples of 8; the others need 2-byte alignment only (aligned rows are
+ * faster). residual may be out itself.
+ */
+#define ARC_ACT_NONE 0
+#define ARC_ACT_RELU 1
+#define ARC_ACT_GELU 2      /* erf form */
+#define ARC_ACT_GELU_TANH 3 /* tanh form */
+#define ARC_ACT_SILU 4
+int arc_linear_bf16(const uint16_t *x, const uint16_t *w, const uint16_t *bias, const uint16_t *residual,
+                    uint16_t *out, uint16_t *z, int M, int N, int K, int64_t ldx, int64_t ldw, int64_t ldr,
+                    int64_t ldo, int64_t ldz, int activation, cudaStream_t stream);
+
+/*
+ * First step of the linear layer's backward pass: dz = dy * act'(z) (bf16, dz may be NULL)
+ * and dbias[n] = sum_m of the unrounded dz (dbias may be NULL). The gradients of x and w are
+ * then arc_grouped_matmul_dx and arc_grouped_matmul_dw of dz with NULL offsets and E = 1.
+ * workspace (4-byte aligned, arc_linear_dz_workspace_bytes; needed for dbias only) is
+ * written and read on `stream`; its contents need no initialisation.
+ */
+int arc_linear_dz_workspace_bytes(int M, int N, size_t *bytes);
+int arc_linear_dz(const uint16_t *dy, const uint16_t *z, uint16_t *dz, uint16_t *dbias, void *workspace,
+                  size_t workspace_bytes, int M, int N, int64_t lddy, int64_t ldz, int64_t lddz, int activation,
+                  cudaStream_t stream);
+
+/*
+ * Grouped product and its gradients, bf16 with fp32 accumulation. Rows are sorted by group:
+ * group e owns the rows [offsets[e], offsets[e+1]) (offsets [E+1] int32 on the device, read
+ * by the kernel, clamped to [0, T]), and has its own weights w + e * w_stride, [N][ldw].
+ *   arc_grouped_matmul     out[t,n] = sum_k x[t,k] w[e,n,k]
+ *   arc_grouped_matmul_dx  dx[t,k]  = sum_n dy[t,n] w[e,n,k]
+ *   arc_grouped_matmul_dw  dw[e,n,k] = sum_{t in e} dy[t,n] x[t,k]   (zeros for an empty group)
+ * Rows of no group are left as they are, or set to zero with ARC_GROUPED_ZERO_OTHERS; what
+ * they hold in x and dy never reaches a result. NULL offsets (E = 1): one group of all rows.
+ * Offsets that decrease or leave [0, T] give unspecified values inside the output and set
+ * bit 7 of arc_device_status. Requirements: 1 <= E <= 1024; x, w and dy 16-byte aligned,
+ * leading dimensions and w_stride multiples of 8; outputs 2-byte aligned.
+ */
+#define ARC_GROUPED_ZERO_OTHERS 4u
+int arc_grouped_matmul(const uint16_t *x, const uint16_t *w, const int32_t *offsets, uint16_t *out, int T, int E,
+                       int N, int K, int64_t ldx, int64_t ldw, int64_t w_stride, int64_t ldo, unsigned flags,
+                       cudaStream_t stream);
+int arc_grouped_matmul_dx(const uint16_t *dy, const uint16_t *w, const int32_t *offsets, uint16_t *dx, int T, int E,
+                          int N, int K, int64_t lddy, int64_t ldw, int64_t w_stride, int64_t lddx, unsigned flags,
+                          cudaStream_t stream);
+int arc_grouped_matmul_dw(const uint16_t *dy, const uint16_t *x, const int32_t *offsets, uint16_t *dw, int T, int E,
+                          int N, int K, int64_t lddy, int64_t ldx, int64_t lddw, int64_t dw_stride,
+                          cudaStream_t stream);
+
+/*
+ * A8W4 grouped product: arc_a8w4_gemm_ex for every group's rows with the group's weights,
+ *   C[t,n] = bf16( sa[t] * sum_g f32(sb[e,n,g]) * P[t,n,g] ),  A [T][K], sa [T],
+ *   Wp [E][N][K/2], sb [E][N][K/128], C [T][N], all contiguous; offsets as above (not NULL).
+ * flags: ARC_A8W4_PREPACKED, ARC_GROUPED_ZERO_OTHERS. Requirements: group == 128,
+ * K % 128 == 0, N % 8 == 0, E <= 1024, E * N < 2^31; A, Wp and C 16-byte aligned.
+ */
+int arc_a8w4_grouped_gemm(const int8_t *A, const float *sa, const uint8_t *Wp, const uint16_t *sb,
+                          const int32_t *offsets, uint16_t *C, int T, int E, int N, int K, int group, unsigned flags,
+                          cudaStream_t stream);
+
+/*
+ * Sorts a router's choices by group (stable): ids [slots] (id_bytes 4 or 8, signed; slots =
+ * tokens * top), an id outside [0, E) chooses no group and is placed behind the last one.
+ *   offsets   [E+1]    first place of each group; offsets[E] counts the choices with a group
+ *   rows      [slots]  token (slot / top) at each place
+ *   positions [slots]  place of each choice
+ * workspace: arc_group_rows_workspace_bytes (0 for few slots), no initialisation needed.
+ */
+int arc_group_rows_workspace_bytes(int slots, int E, size_t *bytes);
+int arc_group_rows(const void *ids, int id_bytes, int32_t *offsets, int32_t *rows, int32_t *positions, void *workspace,
+                   size_t workspace_bytes, int slots, int top, int E, cudaStream_t stream);
+
+/*
  * Probe builds only (libarcb200_probe.so, compiled with -DARC_PROBE and loaded by the
  * Python package when the ARC_PROBE environment variable is set). Attaches a device
  * buffer of at least 64 uint64 per CTA; every kernel launched afterwards on the
@@ -316,7 +394,8 @@ int arc_kernel_name(int op, int M, int N, int K, char *name, int len);
 
 /*
  * Device status word of `device`: a bit mask of the pipeline waits that timed out
- * since it was last cleared (0 = healthy). Synchronises the device. When `clear`
+ * since it was last cleared, and bit 7 for group offsets that decrease or leave the rows
+ * (0 = healthy). Synchronises the device. When `clear`
  * is nonzero the word is reset to 0 after reading.
  */
 int arc_device_status(int device, uint32_t *status, int clear);
