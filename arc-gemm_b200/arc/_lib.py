@@ -6,6 +6,7 @@ raises. Building it is `python -m arc.build` (or `__graft_entry__.build()`).
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import threading
 
@@ -77,8 +78,8 @@ SIGNATURES = {
     "arc_a8w4_gemm_ex": ([_P, _P, _P, _P, _P, _I, _I, _I, _I, ctypes.c_uint, _P, _P], _I),
     "arc_a8w4_gemm_gather_ex": ([_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_uint, _P], _I),
     "arc_linear_bf16": ([_P] * 6 + [_I] * 3 + [_L] * 5 + [_I, _P], _I),
-    "arc_linear_dz_workspace_bytes": ([_I, _I, ctypes.POINTER(ctypes.c_size_t)], _I),
-    "arc_linear_dz": ([_P] * 5 + [ctypes.c_size_t, _I, _I] + [_L] * 3 + [_I, _P], _I),
+    "arc_linear_backward_workspace_bytes": ([_I] * 4 + [ctypes.POINTER(ctypes.c_size_t)], _I),
+    "arc_linear_backward": ([_P] * 8 + [ctypes.c_size_t] + [_I] * 3 + [_L] * 6 + [_I, _P], _I),
     "arc_grouped_matmul": ([_P] * 4 + [_I] * 4 + [_L] * 4 + [ctypes.c_uint, _P], _I),
     "arc_grouped_matmul_dx": ([_P] * 4 + [_I] * 4 + [_L] * 4 + [ctypes.c_uint, _P], _I),
     "arc_grouped_matmul_dw": ([_P] * 4 + [_I] * 4 + [_L] * 4 + [_P], _I),
@@ -135,6 +136,28 @@ def check(status: int, what: str) -> None:
         detail = L.arc_last_error().decode(errors="replace")
         kind = L.arc_status_string(status).decode(errors="replace")
         raise ArcError(status, f"{what}: {kind}: {detail}")
+
+
+def call_on(device, fn, what: str, *args) -> None:
+    """fn(*args, stream) on the device's current stream, with the device made current."""
+    import torch
+
+    index = device.index
+    if torch.cuda.current_device() == index:
+        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    else:
+        with torch.cuda.device(index):
+            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
+    if status != ARC_OK:
+        check(status, what)
+
+
+@functools.lru_cache(maxsize=1024)
+def workspace_bytes(name: str, *sizes: int) -> int:
+    """What the library's workspace query `name` says for these sizes."""
+    size = ctypes.c_size_t(0)
+    check(getattr(lib(), name)(*sizes, ctypes.byref(size)), name)
+    return size.value
 
 
 def describe_plan(M: int, N: int, K: int, num_sms: int = 148) -> dict:

@@ -16,14 +16,12 @@ decrease or leave the rows give unspecified values and set bit 7 of `arc.device_
 """
 from __future__ import annotations
 
-import ctypes
-
 import torch
 
-from ._lib import A8W4_PREPACKED, GROUPED_ZERO_OTHERS, check, lib
+from ._lib import A8W4_PREPACKED, GROUPED_ZERO_OTHERS, call_on, lib, workspace_bytes
 from .a8w4 import GROUP_K, _expect
-from .linear import _padded, _same_device, product_dw, product_dx, product_rows
-from .mm import _require_cuda_bf16, _stream_ptr
+from .linear import _padded, _same_device, product_rows
+from .mm import _require_cuda_bf16
 from .quant import TensorPair
 
 MAX_GROUPS = 1024
@@ -47,11 +45,9 @@ def _product_groups(w: torch.Tensor) -> torch.Tensor:
 def _forward(x, w, offsets, out, zero_others):
     t, k = x.shape
     e, n, _ = w.shape
-    with torch.cuda.device(x.device):
-        check(lib().arc_grouped_matmul(
-            x.data_ptr(), w.data_ptr(), offsets.data_ptr(), out.data_ptr(), t, e, n, k, x.stride(0), w.stride(1),
-            w.stride(0), out.stride(0), GROUPED_ZERO_OTHERS if zero_others else 0, _stream_ptr(x.device)),
-            "arc.grouped_matmul")
+    call_on(x.device, lib().arc_grouped_matmul, "arc.grouped_matmul", x.data_ptr(), w.data_ptr(), offsets.data_ptr(),
+            out.data_ptr(), t, e, n, k, x.stride(0), w.stride(1), w.stride(0), out.stride(0),
+            GROUPED_ZERO_OTHERS if zero_others else 0)
     return out
 
 
@@ -59,7 +55,7 @@ class _Grouped(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, w, offsets):
         x, w = product_rows(x), _product_groups(w)
-        out = torch.empty((x.shape[0], w.shape[1]), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty((x.shape[0], w.shape[1]))
         if x.shape[0] > 0:
             _forward(x, w, offsets, out, True)
         ctx.save_for_backward(x, w, offsets)
@@ -72,13 +68,18 @@ class _Grouped(torch.autograd.Function):
         need_x, need_w, _ = ctx.needs_input_grad
         if x.shape[0] == 0:
             return x.new_empty(x.shape) if need_x else None, w.new_zeros(w.shape) if need_w else None, None
+        dy = product_rows(dy)
+        (t, k), (e, n, _) = x.shape, w.shape
         dx = dw = None
-        with torch.cuda.device(x.device):
-            dy = product_rows(dy)
-            if need_x:
-                dx = product_dx(dy, w, offsets, True, "arc.grouped_matmul backward")
-            if need_w:
-                dw = product_dw(dy, x, offsets, w.shape[0], "arc.grouped_matmul backward")
+        if need_x:
+            dx = x.new_empty((t, k))
+            call_on(x.device, lib().arc_grouped_matmul_dx, "arc.grouped_matmul backward", dy.data_ptr(), w.data_ptr(),
+                    offsets.data_ptr(), dx.data_ptr(), t, e, n, k, dy.stride(0), w.stride(1), w.stride(0), k,
+                    GROUPED_ZERO_OTHERS)
+        if need_w:
+            dw = w.new_empty((e, n, k))
+            call_on(x.device, lib().arc_grouped_matmul_dw, "arc.grouped_matmul backward", dy.data_ptr(), x.data_ptr(),
+                    offsets.data_ptr(), dw.data_ptr(), t, e, n, k, dy.stride(0), x.stride(0), k, n * k)
         return dx, dw, None
 
 
@@ -112,7 +113,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
         return _Grouped.apply(x, w, offsets)
     fresh = out is None
     if fresh:
-        out = torch.empty((t, n), dtype=torch.bfloat16, device=dev)
+        out = x.new_empty((t, n))
     else:
         _require_cuda_bf16(out, "out")
         if tuple(out.shape) != (t, n) or out.device != dev or out.stride(1) != 1 or out.stride(0) < n:
@@ -157,11 +158,8 @@ def a8w4_grouped_matmul(a: TensorPair, b: TensorPair, offsets: torch.Tensor, out
     if t == 0:
         return out
     flags = (A8W4_PREPACKED if prepacked else 0) | (GROUPED_ZERO_OTHERS if fresh else 0)
-    with torch.cuda.device(dev):
-        check(lib().arc_a8w4_grouped_gemm(x.data_ptr(), sa.data_ptr(), wp.data_ptr(), sb.data_ptr(),
-                                          offsets.data_ptr(), out.data_ptr(), t, e, n, k, GROUP_K, flags,
-                                          _stream_ptr(dev)),
-              "arc.a8w4_grouped_matmul")
+    call_on(dev, lib().arc_a8w4_grouped_gemm, "arc.a8w4_grouped_matmul", x.data_ptr(), sa.data_ptr(), wp.data_ptr(),
+            sb.data_ptr(), offsets.data_ptr(), out.data_ptr(), t, e, n, k, GROUP_K, flags)
     return out
 
 
@@ -187,17 +185,12 @@ def group_rows(ids: torch.Tensor, num_groups: int) -> tuple[torch.Tensor, torch.
     if slots == 0:
         return (torch.zeros(num_groups + 1, dtype=torch.int32, device=dev),
                 torch.empty(0, dtype=torch.int32, device=dev), torch.empty(ids.shape, dtype=torch.int32, device=dev))
-    offsets = torch.empty(num_groups + 1, dtype=torch.int32, device=dev)
-    rows = torch.empty(slots, dtype=torch.int32, device=dev)
-    positions = torch.empty(ids.shape, dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
-        size = ctypes.c_size_t(0)
-        check(lib().arc_group_rows_workspace_bytes(slots, num_groups, ctypes.byref(size)),
-              "arc_group_rows_workspace_bytes")
-        workspace = torch.empty(size.value, dtype=torch.uint8, device=dev) if size.value else None
-        check(lib().arc_group_rows(ids.data_ptr(), ids.element_size(), offsets.data_ptr(), rows.data_ptr(),
-                                   positions.data_ptr(), workspace.data_ptr() if workspace is not None else None,
-                                   size.value, slots, ids.shape[1] if ids.dim() == 2 else 1, num_groups,
-                                   _stream_ptr(dev)),
-              "arc.group_rows")
+    offsets = ids.new_empty(num_groups + 1, dtype=torch.int32)
+    rows = ids.new_empty(slots, dtype=torch.int32)
+    positions = ids.new_empty(ids.shape, dtype=torch.int32)
+    size = workspace_bytes("arc_group_rows_workspace_bytes", slots, num_groups)
+    workspace = ids.new_empty(size, dtype=torch.uint8) if size else None
+    call_on(dev, lib().arc_group_rows, "arc.group_rows", ids.data_ptr(), ids.element_size(), offsets.data_ptr(),
+            rows.data_ptr(), positions.data_ptr(), workspace.data_ptr() if size else None, size, slots,
+            ids.shape[1] if ids.dim() == 2 else 1, num_groups)
     return offsets, rows, positions

@@ -20,8 +20,8 @@ from __future__ import annotations
 
 import torch
 
-from ._lib import ACTIVATIONS, GROUPED_ZERO_OTHERS, check, lib
-from .mm import _require_cuda_bf16, _row_major, _stream_ptr
+from ._lib import ACTIVATIONS, call_on, lib, workspace_bytes
+from .mm import _require_cuda_bf16, _row_major
 
 
 def _same_device(t: torch.Tensor, name: str, dev: torch.device) -> None:
@@ -43,39 +43,12 @@ def product_rows(t: torch.Tensor) -> torch.Tensor:
 
 
 def _forward(x, w, bias, residual, activation, out, z):
-    m, k = x.shape
-    n = w.shape[0]
-    with torch.cuda.device(x.device):
-        check(lib().arc_linear_bf16(
-            x.data_ptr(), w.data_ptr(), bias.data_ptr() if bias is not None else None,
-            residual.data_ptr() if residual is not None else None, out.data_ptr(),
-            z.data_ptr() if z is not None else None, m, n, k, x.stride(0), w.stride(0),
-            residual.stride(0) if residual is not None else 0, out.stride(0),
-            z.stride(0) if z is not None else 0, activation, _stream_ptr(x.device)), "arc.linear")
+    call_on(x.device, lib().arc_linear_bf16, "arc.linear", x.data_ptr(), w.data_ptr(),
+            bias.data_ptr() if bias is not None else None, residual.data_ptr() if residual is not None else None,
+            out.data_ptr(), z.data_ptr() if z is not None else None, x.shape[0], w.shape[0], x.shape[1],
+            x.stride(0), w.stride(0), residual.stride(0) if residual is not None else 0, out.stride(0),
+            z.stride(0) if z is not None else 0, activation)
     return out
-
-
-def product_dx(dz, w, offsets, zero_others, what):
-    """dx [T, K] = dz [T, N] . w [E, N, K], row group by row group (offsets None: one group)."""
-    t, n = dz.shape
-    e, _, k = w.shape
-    dx = torch.empty((t, k), dtype=torch.bfloat16, device=dz.device)
-    check(lib().arc_grouped_matmul_dx(
-        dz.data_ptr(), w.data_ptr(), offsets.data_ptr() if offsets is not None else None, dx.data_ptr(),
-        t, e, n, k, dz.stride(0), w.stride(1), w.stride(0), k, GROUPED_ZERO_OTHERS if zero_others else 0,
-        _stream_ptr(dz.device)), what)
-    return dx
-
-
-def product_dw(dz, x, offsets, groups, what):
-    """dw [E, N, K] = dz [T, N]^T . x [T, K] of each row group."""
-    t, n = dz.shape
-    k = x.shape[1]
-    dw = torch.empty((groups, n, k), dtype=torch.bfloat16, device=dz.device)
-    check(lib().arc_grouped_matmul_dw(
-        dz.data_ptr(), x.data_ptr(), offsets.data_ptr() if offsets is not None else None, dw.data_ptr(),
-        t, groups, n, k, dz.stride(0), x.stride(0), k, n * k, _stream_ptr(dz.device)), what)
-    return dw
 
 
 class _Linear(torch.autograd.Function):
@@ -83,7 +56,7 @@ class _Linear(torch.autograd.Function):
     def forward(ctx, x, w, bias, residual, activation):
         m, n = x.shape[0], w.shape[0]
         x, w = product_rows(x), product_rows(w)
-        out = torch.empty((m, n), dtype=torch.bfloat16, device=x.device)
+        out = x.new_empty((m, n))
         z = None
         if m > 0:
             if activation != 0 and any(ctx.needs_input_grad[:3]):
@@ -100,52 +73,25 @@ class _Linear(torch.autograd.Function):
         need_x, need_w, need_bias, need_residual, _ = ctx.needs_input_grad
         m, k = x.shape
         n = w.shape[0]
-        dev = x.device
+        dx = x.new_empty((m, k)) if need_x else None
+        dw = w.new_empty((n, k)) if need_w else None
+        dbias = w.new_empty((n,)) if need_bias else None
         dresidual = dy if need_residual else None
         if not (need_x or need_w or need_bias):
             return None, None, None, dresidual, None
         if m == 0:
-            return (x.new_empty((0, k)) if need_x else None, w.new_zeros((n, k)) if need_w else None,
-                    w.new_zeros((n,)) if need_bias else None, dresidual, None)
-        with torch.cuda.device(dev):
-            if dy.stride(1) != 1 or dy.stride(0) < n:
-                dy = dy.contiguous()  # an expanded or transposed gradient
-            products = need_x or need_w
-            dz, dbias = dy, None
-            if need_bias or (products and z is not None):
-                L = lib()
-                dz = None
-                if products and z is not None:
-                    dz = _padded(m, n, device=dev)
-                workspace, size = None, 0
-                if need_bias:
-                    dbias = torch.empty((n,), dtype=torch.bfloat16, device=dev)
-                    size = dz_workspace_bytes(m, n)
-                    workspace = torch.empty((size,), dtype=torch.uint8, device=dev)
-                check(L.arc_linear_dz(
-                    dy.data_ptr(), z.data_ptr() if z is not None else None,
-                    dz.data_ptr() if dz is not None else None, dbias.data_ptr() if need_bias else None,
-                    workspace.data_ptr() if need_bias else None, size, m, n, dy.stride(0),
-                    z.stride(0) if z is not None else 0, dz.stride(0) if dz is not None else 0, ctx.activation,
-                    _stream_ptr(dev)), "arc.linear backward")
-                if dz is None:
-                    dz = dy
-            dx = dw = None
-            if products:
-                dz = product_rows(dz)
-                if need_x:
-                    dx = product_dx(dz, w.unsqueeze(0), None, False, "arc.linear backward")
-                if need_w:
-                    dw = product_dw(dz, x, None, 1, "arc.linear backward")[0]
+            return (dx, dw.zero_() if need_w else None, dbias.zero_() if need_bias else None, dresidual, None)
+        if dy.stride(1) != 1 or dy.stride(0) < n:
+            dy = dy.contiguous()  # an expanded or transposed gradient
+        need_dz = (need_x or need_w) and (z is not None or dy.stride(0) % 8 != 0 or dy.data_ptr() % 16 != 0)
+        size = workspace_bytes("arc_linear_backward_workspace_bytes", m, n, need_dz, need_bias)
+        workspace = x.new_empty(((size + 1) // 2,)) if size else None
+        call_on(x.device, lib().arc_linear_backward, "arc.linear backward", dy.data_ptr(), x.data_ptr(), w.data_ptr(),
+                z.data_ptr() if z is not None else None, dx.data_ptr() if need_x else None,
+                dw.data_ptr() if need_w else None, dbias.data_ptr() if need_bias else None,
+                workspace.data_ptr() if size else None, size, m, n, k, dy.stride(0), x.stride(0), w.stride(0),
+                z.stride(0) if z is not None else 0, k, k, ctx.activation)
         return dx, dw, dbias, dresidual, None
-
-
-def dz_workspace_bytes(m: int, n: int) -> int:
-    import ctypes
-
-    size = ctypes.c_size_t(0)
-    check(lib().arc_linear_dz_workspace_bytes(m, n, ctypes.byref(size)), "arc_linear_dz_workspace_bytes")
-    return size.value
 
 
 def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
@@ -191,7 +137,7 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
             raise ValueError("out cannot be given when an input requires a gradient")
         return _Linear.apply(x, w, bias, residual, code)
     if out is None:
-        out = torch.empty((m, n), dtype=torch.bfloat16, device=dev)
+        out = x.new_empty((m, n))
     else:
         _require_cuda_bf16(out, "out")
         if tuple(out.shape) != (m, n) or out.device != dev or out.stride(1) != 1 or out.stride(0) < n:

@@ -204,6 +204,35 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
   return ARC_OK;
 }
 
+// dw[e][n][k] = sum over the rows t of group e of dy[t][n] x[t][k].
+int linear_dw(const char* what, const uint16_t* dy, const uint16_t* x, const arcb::lin::Groups& groups, uint16_t* dw,
+              uint32_t N, uint32_t K, uint64_t lddy, uint64_t ldx, uint64_t lddw, uint64_t dw_stride,
+              cudaStream_t stream) {
+  int dev = 0;
+  if (int st = current_device(&dev)) return st;
+  const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
+  if (max_pairs == 0) return fail(ARC_ERR_UNSUPPORTED, "%s: no CTA pair fits on this device", what);
+  LP::Params p = {};
+  if (int st = encode_groups_3d(&p.tm_a, dy, N, groups.rows, 1, lddy, uint64_t(groups.rows) * lddy, 64, 64, "dy")) return st;
+  if (int st = encode_groups_3d(&p.tm_b, x, K, groups.rows, 1, ldx, uint64_t(groups.rows) * ldx, 64, 64, "x")) return st;
+  p.out = dw;
+  p.ldo = lddw;
+  p.out_group = dw_stride;
+  p.groups = groups;
+  p.epi.vec_out = row_vec(dw, lddw, dw_stride);
+  p.M = N;
+  p.N = K;
+  p.tiles_m = ceil_div(N, LP::kTile);
+  p.tiles_n = ceil_div(K, LP::kTile);
+  const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n * groups.num;
+  if (tiles > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "%s: too many tiles for one launch", what);
+  const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
+  const cudaError_t e = launch_ex(LP::gemm_linear_pair_kernel<true, true, true>, p, grid, LP::kThreads, LP::kSmemBytes,
+                                  2, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
+  return ARC_OK;
+}
+
 // Checks shared by the grouped entry points.
 int grouped_check(const char* what, const void* a, const void* b, const void* c, const int32_t* offsets, int T, int E,
                   int N, int K) {
@@ -246,12 +275,14 @@ int output_check(const char* what, const char* name, const void* p, int64_t ld, 
 
 // Row blocks of the dz pass: enough blocks to fill the GPU several times over, at least 16
 // rows each.
-uint32_t dz_row_blocks(uint32_t M, uint32_t N, uint32_t sms) {
-  const uint32_t col_blocks = ceil_div(N, LB::kColsPerBlock);
-  const uint32_t want = ceil_div(6 * sms, col_blocks), most = ceil_div(M, 16);
+constexpr uint32_t kDzBlocks = 6 * 148;  // of the whole grid; the workspace size must not depend on the device
+uint32_t dz_row_blocks(uint32_t M, uint32_t N) {
+  const uint32_t want = ceil_div(kDzBlocks, ceil_div(N, LB::kColsPerBlock)), most = ceil_div(M, 16);
   return want < most ? want : most;
 }
-constexpr uint32_t kDzSms = 148;  // the workspace size must not depend on the device
+// dz lies in the workspace with rows that TMA can read.
+uint64_t dz_ld(uint32_t N) { return (uint64_t(N) + 7) / 8 * 8; }
+size_t dz_bytes(uint32_t M, uint32_t N) { return (size_t(M) * dz_ld(N) * 2 + 255) / 256 * 256; }
 
 }  // namespace
 
@@ -293,23 +324,28 @@ int arc_linear_bf16(const uint16_t* x, const uint16_t* w, const uint16_t* bias, 
   return linear_rows(x, w, groups, out, N, K, ldx, ldw, uint64_t(N) * ldw, ldo, epi, false, false, stream);
 }
 
-int arc_linear_dz_workspace_bytes(int M, int N, size_t* bytes) {
+int arc_linear_backward_workspace_bytes(int M, int N, int need_dz, int need_dbias, size_t* bytes) {
   if (bytes == nullptr || M <= 0 || N <= 0) {
-    return fail(ARC_ERR_INVALID_ARGUMENT, "arc_linear_dz_workspace_bytes: bad argument");
+    return fail(ARC_ERR_INVALID_ARGUMENT, "arc_linear_backward_workspace_bytes: bad argument");
   }
-  *bytes = size_t(dz_row_blocks(M, N, kDzSms)) * N * sizeof(float);
+  *bytes = (need_dz ? dz_bytes(M, N) : 0) +
+           (need_dbias ? size_t(dz_row_blocks(M, N)) * N * sizeof(float) : 0);
   return ARC_OK;
 }
 
-int arc_linear_dz(const uint16_t* dy, const uint16_t* z, uint16_t* dz, uint16_t* dbias, void* workspace,
-                  size_t workspace_bytes, int M, int N, int64_t lddy, int64_t ldz, int64_t lddz, int activation,
-                  cudaStream_t stream) {
-  const char* what = "arc_linear_dz";
+int arc_linear_backward(const uint16_t* dy, const uint16_t* x, const uint16_t* w, const uint16_t* z, uint16_t* dx,
+                        uint16_t* dw, uint16_t* dbias, void* workspace, size_t workspace_bytes, int M, int N, int K,
+                        int64_t lddy, int64_t ldx, int64_t ldw, int64_t ldz, int64_t lddx, int64_t lddw,
+                        int activation, cudaStream_t stream) {
+  const char* what = "arc_linear_backward";
   g_last_error[0] = '\0';
-  if (dy == nullptr || (dz == nullptr && dbias == nullptr)) {
+  if (dy == nullptr || (dx == nullptr && dw == nullptr && dbias == nullptr) || (dx != nullptr && w == nullptr) ||
+      (dw != nullptr && x == nullptr)) {
     return fail(ARC_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
   }
-  if (M <= 0 || N <= 0) return fail(ARC_ERR_INVALID_ARGUMENT, "%s: sizes must be positive (M=%d N=%d)", what, M, N);
+  if (M <= 0 || N <= 0 || K <= 0) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: sizes must be positive (M=%d N=%d K=%d)", what, M, N, K);
+  }
   if (activation < ARC_ACT_NONE || activation > ARC_ACT_SILU) {
     return fail(ARC_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, activation);
   }
@@ -317,45 +353,67 @@ int arc_linear_dz(const uint16_t* dy, const uint16_t* z, uint16_t* dz, uint16_t*
     return fail(ARC_ERR_INVALID_ARGUMENT, "%s: an activation's gradient needs z", what);
   }
   if (int st = output_check(what, "dy", dy, lddy, N)) return st;
-  if (z != nullptr) {
-    if (int st = output_check(what, "z", z, ldz, N)) return st;
+  if (activation == ARC_ACT_NONE) {
+    z = nullptr;
+  } else if (int st = output_check(what, "z", z, ldz, N)) {
+    return st;
   }
-  if (dz != nullptr) {
-    if (int st = output_check(what, "dz", dz, lddz, N)) return st;
+  if (dx != nullptr) {
+    if (int st = operand_check(what, "w", w, ldw, K)) return st;
+    if (int st = output_check(what, "dx", dx, lddx, K)) return st;
+  }
+  if (dw != nullptr) {
+    if (int st = operand_check(what, "x", x, ldx, K)) return st;
+    if (int st = output_check(what, "dw", dw, lddw, K)) return st;
   }
   if (reinterpret_cast<uintptr_t>(dbias) & 1u) return fail(ARC_ERR_UNSUPPORTED, "%s: dbias is misaligned", what);
-  const uint32_t row_blocks = dz_row_blocks(M, N, kDzSms);
-  if (dbias != nullptr && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 3u) ||
-                           workspace_bytes < size_t(row_blocks) * N * sizeof(float))) {
-    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: dbias needs a 4-byte aligned workspace of %zu bytes", what,
-                size_t(row_blocks) * N * sizeof(float));
+  // The products read dy itself where there is nothing to multiply it by and TMA can read it.
+  const bool products = dx != nullptr || dw != nullptr;
+  const bool need_dz = products && (z != nullptr || !aligned16(dy) || lddy % 8 != 0);
+  const uint32_t row_blocks = dz_row_blocks(M, N);
+  const size_t dz_size = need_dz ? dz_bytes(M, N) : 0;
+  const size_t need = dz_size + (dbias != nullptr ? size_t(row_blocks) * N * sizeof(float) : 0);
+  if (need > 0 && (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need)) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
   }
   int dev = 0;
   if (int st = current_device(&dev)) return st;
-  LB::Params p = {};
-  p.dy = dy;
-  p.z = activation == ARC_ACT_NONE ? nullptr : z;
-  p.dz = dz;
-  p.partial = dbias != nullptr ? static_cast<float*>(workspace) : nullptr;
-  p.lddy = lddy;
-  p.ldz = ldz;
-  p.lddz = lddz;
-  p.M = M;
-  p.N = N;
-  p.act = static_cast<uint32_t>(activation);
-  p.rows_per_block = ceil_div(M, row_blocks);
-  const bool vec = N % 8 == 0 && row_vec(dy, lddy) != 0 && (p.z == nullptr || row_vec(z, ldz) != 0) &&
-                   (dz == nullptr || row_vec(dz, lddz) != 0);
-  const dim3 grid(ceil_div(N, LB::kColsPerBlock), row_blocks, 1);
-  cudaError_t e = vec ? launch_grid(LB::linear_dz_kernel<true>, grid, LB::kThreads, 0, stream, p)
-                      : launch_grid(LB::linear_dz_kernel<false>, grid, LB::kThreads, 0, stream, p);
-  if (e != cudaSuccess) return cuda_fail(e, "linear_dz_kernel launch");
-  if (dbias != nullptr) {
-    e = launch_grid(LB::linear_dbias_kernel, dim3(ceil_div(N, LB::kThreads), 1, 1), LB::kThreads, 0, stream,
-                    static_cast<const float*>(p.partial), dbias, uint32_t(N), row_blocks);
-    if (e != cudaSuccess) return cuda_fail(e, "linear_dbias_kernel launch");
+  if (need_dz || dbias != nullptr) {
+    LB::Params p = {};
+    p.dy = dy;
+    p.z = z;
+    p.dz = need_dz ? static_cast<uint16_t*>(workspace) : nullptr;
+    p.partial = dbias != nullptr ? reinterpret_cast<float*>(static_cast<uint8_t*>(workspace) + dz_size) : nullptr;
+    p.lddy = lddy;
+    p.ldz = ldz;
+    p.lddz = dz_ld(N);
+    p.M = M;
+    p.N = N;
+    p.act = static_cast<uint32_t>(activation);
+    p.rows_per_block = ceil_div(M, row_blocks);
+    const bool vec = N % 8 == 0 && row_vec(dy, lddy) != 0 && (z == nullptr || row_vec(z, ldz) != 0);
+    const dim3 grid(ceil_div(N, LB::kColsPerBlock), row_blocks, 1);
+    cudaError_t e = vec ? launch_grid(LB::linear_dz_kernel<true>, grid, LB::kThreads, 0, stream, p)
+                        : launch_grid(LB::linear_dz_kernel<false>, grid, LB::kThreads, 0, stream, p);
+    if (e != cudaSuccess) return cuda_fail(e, "linear_dz_kernel launch");
+    if (dbias != nullptr) {
+      e = launch_grid(LB::linear_dbias_kernel, dim3(ceil_div(N, LB::kThreads), 1, 1), LB::kThreads, 0, stream,
+                      static_cast<const float*>(p.partial), dbias, uint32_t(N), row_blocks);
+      if (e != cudaSuccess) return cuda_fail(e, "linear_dbias_kernel launch");
+    }
+    if (need_dz) {
+      dy = p.dz;
+      lddy = p.lddz;
+    }
   }
-  return ARC_OK;
+  const arcb::lin::Groups groups = {nullptr, 1u, static_cast<uint32_t>(M)};
+  if (dx != nullptr) {
+    if (int st = linear_rows(dy, w, groups, dx, K, N, lddy, ldw, uint64_t(N) * ldw, lddx, arcb::lin::Epilogue{}, true,
+                             false, stream)) {
+      return st;
+    }
+  }
+  return dw != nullptr ? linear_dw(what, dy, x, groups, dw, N, K, lddy, ldx, lddw, 0, stream) : ARC_OK;
 }
 
 int arc_grouped_matmul(const uint16_t* x, const uint16_t* w, const int32_t* offsets, uint16_t* out, int T, int E,
@@ -400,29 +458,8 @@ int arc_grouped_matmul_dw(const uint16_t* dy, const uint16_t* x, const int32_t* 
   if (int st = operand_check(what, "x", x, ldx, K)) return st;
   if (int st = output_check(what, "dw", dw, lddw, K)) return st;
   if (int st = output_check(what, "dw's groups", dw, dw_stride, int64_t(N - 1) * lddw + K)) return st;
-  int dev = 0;
-  if (int st = current_device(&dev)) return st;
-  const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
-  if (max_pairs == 0) return fail(ARC_ERR_UNSUPPORTED, "%s: no CTA pair fits on this device", what);
-  LP::Params p = {};
-  if (int st = encode_groups_3d(&p.tm_a, dy, N, T, 1, lddy, uint64_t(T) * lddy, 64, 64, "dy")) return st;
-  if (int st = encode_groups_3d(&p.tm_b, x, K, T, 1, ldx, uint64_t(T) * ldx, 64, 64, "x")) return st;
-  p.out = dw;
-  p.ldo = lddw;
-  p.out_group = dw_stride;
-  p.groups = {offsets, static_cast<uint32_t>(E), static_cast<uint32_t>(T)};
-  p.epi.vec_out = row_vec(dw, lddw, dw_stride);
-  p.M = N;
-  p.N = K;
-  p.tiles_m = ceil_div(N, LP::kTile);
-  p.tiles_n = ceil_div(K, LP::kTile);
-  const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n * E;
-  if (tiles > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "%s: too many tiles for one launch", what);
-  const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
-  const cudaError_t e = launch_ex(LP::gemm_linear_pair_kernel<true, true, true>, p, grid, LP::kThreads, LP::kSmemBytes,
-                                  2, stream);
-  if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
-  return ARC_OK;
+  const arcb::lin::Groups groups = {offsets, static_cast<uint32_t>(E), static_cast<uint32_t>(T)};
+  return linear_dw(what, dy, x, groups, dw, N, K, lddy, ldx, lddw, dw_stride, stream);
 }
 
 }  // extern "C"

@@ -49,21 +49,23 @@ struct alignas(1024) Smem {
       uint8_t x[Cfg<BN>::kStages][Cfg<BN>::kXBytes];
     };
     float part[BN][kRows];
+    uint32_t prefix[lin::kMaxGroups + 1];  // only until the block knows its tile
   };
   uint64_t full[Cfg<BN>::kStages];
   uint64_t empty[Cfg<BN>::kStages];
   uint64_t done;
   uint32_t tmem_base;
   uint32_t abort;
-  uint32_t prefix[lin::kMaxGroups + 1];
 };
 
 template <uint32_t BN>
 constexpr size_t smem_bytes() {
   return sizeof(Smem<BN>) + 1024;
 }
-static_assert(smem_bytes<16>() <= 115 * 1024 && smem_bytes<32>() <= 115 * 1024 && smem_bytes<64>() <= 115 * 1024 &&
-                  smem_bytes<128>() <= 115 * 1024,
+// 228 KB of shared memory per SM, of which the system takes 1 KB per block.
+constexpr size_t kHalfSm = (228 / 2 - 1) * 1024;
+static_assert(smem_bytes<16>() <= kHalfSm && smem_bytes<32>() <= kHalfSm && smem_bytes<64>() <= kHalfSm &&
+                  smem_bytes<128>() <= kHalfSm,
               "two blocks per SM");
 
 struct Params {
@@ -142,6 +144,11 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_linear_stream_kernel(const _
       row_end = first + lin::group_count(p.groups, e);
       f0 = nt * kRows;
     }
+  }
+  if (p.groups.offsets != nullptr) {
+    // The table's bytes go to the TMA loads now: order the reads above before them.
+    fence_proxy_async_smem();
+    __syncthreads();
   }
   const uint32_t kb0 = p.num_kb * rank / p.splits, kb1 = p.num_kb * (rank + 1u) / p.splits;
 

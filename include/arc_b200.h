@@ -295,7 +295,7 @@ int arc_quantize_int8(const void *x, int8_t *q, float *sa, int M, int K, int ldx
  * fp32 accumulation, bias, activation and addition, rounded once. The epilogue runs in the
  * GEMM; no reference counterpart beyond the product itself (arc/mm.py:71-79).
  *   x [M][ldx], w [N][ldw], bias [N] or NULL, residual [M][ldr] or NULL, out [M][ldo]
- *   z [M][ldz] or NULL: receives x w^T + bias in bf16, what arc_linear_dz needs later
+ *   z [M][ldz] or NULL: receives x w^T + bias in bf16, what arc_linear_backward needs later
  * Requirements: M, N, K >= 1 (any sizes); x and w 16-byte aligned with leading dimensions
  * that are multiples of 8; the others need 2-byte alignment only (aligned rows are
  * faster). residual may be out itself.
@@ -310,16 +310,21 @@ int arc_linear_bf16(const uint16_t *x, const uint16_t *w, const uint16_t *bias, 
                     int64_t ldo, int64_t ldz, int activation, cudaStream_t stream);
 
 /*
- * First step of the linear layer's backward pass: dz = dy * act'(z) (bf16, dz may be NULL)
- * and dbias[n] = sum_m of the unrounded dz (dbias may be NULL). The gradients of x and w are
- * then arc_grouped_matmul_dx and arc_grouped_matmul_dw of dz with NULL offsets and E = 1.
- * workspace (4-byte aligned, arc_linear_dz_workspace_bytes; needed for dbias only) is
- * written and read on `stream`; its contents need no initialisation.
+ * Gradients of arc_linear_bf16 for the output gradient dy (the residual's gradient is dy):
+ *   dz = dy * act'(z)   dx = dz w   dw = dz^T x   dbias[n] = sum_m dz[m,n]
+ * dx, dw and dbias may be NULL (not wanted; w is needed for dx, x for dw). z is what the
+ * forward call left there (NULL without an activation). dz is rounded to bf16 as operand of the
+ * products and kept in the workspace; dbias sums the unrounded values in fp32.
+ * workspace: 16-byte aligned, no initialisation needed, written and read on `stream`.
+ * arc_linear_backward_workspace_bytes: need_dz if dx or dw is wanted and there is an activation
+ * or dy is not 16-byte aligned with lddy % 8 == 0; need_dbias if dbias is wanted.
+ * Alignment of x and w as in arc_linear_bf16, 2 bytes for the others.
  */
-int arc_linear_dz_workspace_bytes(int M, int N, size_t *bytes);
-int arc_linear_dz(const uint16_t *dy, const uint16_t *z, uint16_t *dz, uint16_t *dbias, void *workspace,
-                  size_t workspace_bytes, int M, int N, int64_t lddy, int64_t ldz, int64_t lddz, int activation,
-                  cudaStream_t stream);
+int arc_linear_backward_workspace_bytes(int M, int N, int need_dz, int need_dbias, size_t *bytes);
+int arc_linear_backward(const uint16_t *dy, const uint16_t *x, const uint16_t *w, const uint16_t *z, uint16_t *dx,
+                        uint16_t *dw, uint16_t *dbias, void *workspace, size_t workspace_bytes, int M, int N, int K,
+                        int64_t lddy, int64_t ldx, int64_t ldw, int64_t ldz, int64_t lddx, int64_t lddw,
+                        int activation, cudaStream_t stream);
 
 /*
  * Grouped product and its gradients, bf16 with fp32 accumulation. Rows are sorted by group:

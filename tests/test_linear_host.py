@@ -33,18 +33,24 @@ def test_linear_checks(native_lib, p):
     assert call(bias=p + 1) == UNS and call(out=p + 1) == UNS
 
 
-def test_dz_checks(native_lib, p):
-    f = native_lib.arc_linear_dz
+def test_linear_backward_checks(native_lib, p):
+    f = native_lib.arc_linear_backward
     size = ctypes.c_size_t(0)
-    assert native_lib.arc_linear_dz_workspace_bytes(0, 8, ctypes.byref(size)) == BAD
-    assert native_lib.arc_linear_dz_workspace_bytes(64, 8, ctypes.byref(size)) == 0 and size.value >= 32
+    query = native_lib.arc_linear_backward_workspace_bytes
+    assert query(0, 8, 1, 1, ctypes.byref(size)) == BAD
+    assert query(64, 9, 1, 0, ctypes.byref(size)) == 0 and size.value >= 64 * 16 * 2
+    assert query(64, 9, 0, 0, ctypes.byref(size)) == 0 and size.value == 0
+    assert query(64, 9, 0, 1, ctypes.byref(size)) == 0 and size.value >= 9 * 4
 
-    def call(dy=p, z=p, dz=p, db=p, ws=p, wsb=4096, m=4, n=8, lddy=8, ldz=8, lddz=8, act=2):
-        return f(dy, z, dz, db, ws, wsb, m, n, lddy, ldz, lddz, act, None)
+    def call(dy=p, x=p, w=p, z=p, dx=p, dw=p, db=p, ws=p, wsb=4096, m=4, n=8, k=16, lddy=8, ldx=16, ldw=16, ldz=8,
+             lddx=16, lddw=16, act=2):
+        return f(dy, x, w, z, dx, dw, db, ws, wsb, m, n, k, lddy, ldx, ldw, ldz, lddx, lddw, act, None)
 
-    assert call(dy=None) == BAD and call(dz=None, db=None) == BAD
-    assert call(m=0) == BAD and call(act=9) == BAD and call(z=None) == BAD
-    assert call(lddy=7) == BAD and call(ldz=7) == BAD and call(lddz=7) == BAD
+    assert call(dy=None) == BAD and call(dx=None, dw=None, db=None) == BAD
+    assert call(x=None) == BAD and call(w=None) == BAD and call(z=None) == BAD
+    assert call(m=0) == BAD and call(k=0) == BAD and call(act=9) == BAD
+    assert call(lddy=7) == BAD and call(ldz=7) == BAD and call(lddx=15) == BAD and call(lddw=15) == BAD
+    assert call(ldx=20) == UNS and call(w=p + 2) == UNS
     assert call(ws=None) == BAD and call(wsb=4) == BAD and call(ws=p + 2) == BAD
     assert call(db=p + 1) == UNS
 
