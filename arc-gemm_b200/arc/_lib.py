@@ -83,7 +83,8 @@ SIGNATURES = {
     "arc_grouped_matmul": ([_P] * 4 + [_I] * 4 + [_L] * 4 + [ctypes.c_uint, _P], _I),
     "arc_grouped_matmul_dx": ([_P] * 4 + [_I] * 4 + [_L] * 4 + [ctypes.c_uint, _P], _I),
     "arc_grouped_matmul_dw": ([_P] * 4 + [_I] * 4 + [_L] * 4 + [_P], _I),
-    "arc_a8w4_grouped_gemm": ([_P] * 6 + [_I] * 5 + [ctypes.c_uint, _P], _I),
+    "arc_a8w4_grouped_workspace_bytes": ([_I] * 3 + [ctypes.POINTER(ctypes.c_size_t)], _I),
+    "arc_a8w4_grouped_gemm": ([_P] * 7 + [ctypes.c_size_t] + [_I] * 5 + [ctypes.c_uint, _P], _I),
     "arc_group_rows_workspace_bytes": ([_I, _I, ctypes.POINTER(ctypes.c_size_t)], _I),
     "arc_group_rows": ([_P, _I, _P, _P, _P, _P, ctypes.c_size_t, _I, _I, _I, _P], _I),
     "arc_a8w4_gemm_gather_sync": ([_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_uint, _P], _I),

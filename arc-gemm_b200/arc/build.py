@@ -29,7 +29,7 @@ STAMP = ROOT / "_build" / "libarcb200.hash"
 SOURCES = ["api.cu"]
 HEADERS = ["sm100.cuh", "peer_barrier.cuh", "gemm_bf16.cuh", "gemm_bf16_pair.cuh", "gemm_a8w4.cuh", "gemm_a8w4_decode.cuh", "quantize.cuh",
            "gemm_fp8fp4.cuh", "gemm_fp8fp4_pair.cuh", "prepack.cuh", "linear_common.cuh",
-           "gemm_linear_stream.cuh", "gemm_linear_pair.cuh", "linear_backward.cuh", "group_rows.cuh",
+           "gemm_linear_stream.cuh", "gemm_linear_pair.cuh", "gemm_grouped_pair.cuh", "linear_backward.cuh", "group_rows.cuh",
            "api_linear.cuh", "api_grouped.cuh"]
 
 NVCC_FLAGS = [

@@ -158,8 +158,11 @@ def a8w4_grouped_matmul(a: TensorPair, b: TensorPair, offsets: torch.Tensor, out
     if t == 0:
         return out
     flags = (A8W4_PREPACKED if prepacked else 0) | (GROUPED_ZERO_OTHERS if fresh else 0)
+    size = workspace_bytes("arc_a8w4_grouped_workspace_bytes", t, e, k)
+    workspace = x.new_empty(size) if size else None
     call_on(dev, lib().arc_a8w4_grouped_gemm, "arc.a8w4_grouped_matmul", x.data_ptr(), sa.data_ptr(), wp.data_ptr(),
-            sb.data_ptr(), offsets.data_ptr(), out.data_ptr(), t, e, n, k, GROUP_K, flags)
+            sb.data_ptr(), offsets.data_ptr(), out.data_ptr(), workspace.data_ptr() if size else None, size, t, e, n, k,
+            GROUP_K, flags)
     return out
 
 

@@ -42,6 +42,34 @@ cudaError_t grouped_init(DeviceState&, bool* regs_ok) {
   return e;
 }
 
+// Int4 codes [groups][rows][bytes].
+int encode_codes_3d(CUtensorMap* map, const void* ptr, uint64_t bytes, uint64_t rows, uint64_t groups) {
+  EncodeTiledFn fn = encode_fn();
+  if (fn == nullptr) return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[3] = {bytes, rows, groups};
+  const cuuint64_t strides[2] = {bytes, bytes * rows};
+  const cuuint32_t box[3] = {GP::kScaleGroup / 2, GP::kRowsPerCta, 1};
+  const cuuint32_t estr[3] = {1, 1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 3, const_cast<void*>(ptr), dims, strides, box, estr,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) {
+    return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled(codes) failed with CUresult %d", static_cast<int>(r));
+  }
+  return ARC_OK;
+}
+
+// Whether a grouped A8W4 product takes the pair kernel (scales in the operand) rather than the
+// int32 kernel (scales on the partial sums): groups of more than a row tile of the latter on
+// average. ARC_A8W4_GROUPED="wide" | "narrow" (tests and tuning) forces one.
+bool a8w4_grouped_wide(uint32_t T, uint32_t E) {
+  if (const char* env = getenv("ARC_A8W4_GROUPED")) {
+    if (strcmp(env, "wide") == 0) return true;
+    if (strcmp(env, "narrow") == 0) return false;
+  }
+  return ceil_div(T, E < T ? E : T) > 128;
+}
+
 template <uint32_t BT, uint32_t EWG, uint32_t LS_>
 cudaError_t launch_a8w4_grouped(const GQ::GroupedParams& p, uint32_t grid, cudaStream_t stream) {
   return launch_ex(GQ::gemm_a8w4_grouped_kernel<BT, EWG, LS_>, p, grid, GQ::Cfg<BT, EWG, LS_>::kThreads,
@@ -64,9 +92,17 @@ uint32_t group_rows_blocks(uint32_t slots, uint32_t* per_block) {
 
 extern "C" {
 
+int arc_a8w4_grouped_workspace_bytes(int T, int E, int K, size_t* bytes) {
+  if (bytes == nullptr || T <= 0 || E <= 0 || K <= 0) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "arc_a8w4_grouped_workspace_bytes: bad argument");
+  }
+  *bytes = a8w4_grouped_wide(T, E) ? size_t(T) * K * 2 : 0;
+  return ARC_OK;
+}
+
 int arc_a8w4_grouped_gemm(const int8_t* A, const float* sa, const uint8_t* Wp, const uint16_t* sb,
-                          const int32_t* offsets, uint16_t* C, int T, int E, int N, int K, int group, unsigned flags,
-                          cudaStream_t stream) {
+                          const int32_t* offsets, uint16_t* C, void* workspace, size_t workspace_bytes, int T, int E,
+                          int N, int K, int group, unsigned flags, cudaStream_t stream) {
   const char* what = "arc_a8w4_grouped_gemm";
   g_last_error[0] = '\0';
   if (sa == nullptr || sb == nullptr || offsets == nullptr) {
@@ -90,6 +126,42 @@ int arc_a8w4_grouped_gemm(const int8_t* A, const float* sa, const uint8_t* Wp, c
   const uint32_t live = E < T ? E : T;  // groups that can have rows
   const uint32_t avg = ceil_div(T, live);
   const uint32_t BT = avg <= 16 ? 16u : avg <= 32 ? 32u : avg <= 64 ? 64u : 128u;
+  const arcb::lin::Groups groups = {offsets, static_cast<uint32_t>(E), static_cast<uint32_t>(T)};
+  const bool zero_others = (flags & ARC_GROUPED_ZERO_OTHERS) != 0;
+  if (a8w4_grouped_wide(T, E)) {
+    if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < size_t(T) * K * 2) {
+      return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what,
+                  size_t(T) * K * 2);
+    }
+    const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
+    if (max_pairs == 0) return fail(ARC_ERR_UNSUPPORTED, "%s: no CTA pair fits on this device", what);
+    const uint64_t pieces = uint64_t(T) * K / 16;
+    const uint64_t want = (pieces + GP::kWidenThreads - 1) / GP::kWidenThreads;
+    const uint64_t cap = uint64_t(g_dev[dev].sms) * 8;
+    cudaError_t e = launch_grid(GP::widen_rows_kernel, dim3(static_cast<uint32_t>(want < cap ? want : cap)),
+                                GP::kWidenThreads, 0, stream, reinterpret_cast<const uint4*>(A),
+                                static_cast<uint4*>(workspace), pieces);
+    if (e != cudaSuccess) return cuda_fail(e, "widen_rows_kernel launch");
+    GP::Params p = {};
+    if (int st = encode_codes_3d(&p.tm_w, Wp, K / 2, N, E)) return st;
+    if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, workspace, K, T, K, GP::kSubK, GP::kBox,
+                           CU_TENSOR_MAP_SWIZZLE_128B, "rows")) {
+      return st;
+    }
+    if (int st = encode_2d(&p.tm_xs, CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 2, workspace, K, T, K, GP::kSubK, GP::kSmallBox,
+                           CU_TENSOR_MAP_SWIZZLE_128B, "rows")) {
+      return st;
+    }
+    p.sa = sa;
+    p.sb = sb;
+    p.G = K / GP::kScaleGroup;
+    p.num_kb = K / GP::kSubK;
+    p.split = (flags & ARC_A8W4_PREPACKED) ? 1u : 0u;
+    e = grouped_pair_launch(p, groups, C, N, N, zero_others, max_pairs, GP::gemm_grouped_pair_kernel<false, true>,
+                            GP::threads<true>(), GP::smem_bytes<true>(), stream);
+    if (e != cudaSuccess) return cuda_fail(e, "gemm_grouped_pair_kernel launch");
+    return ARC_OK;
+  }
   GQ::GroupedParams p = {};
   if (int st = encode_2d(&p.tm_tok, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, A, K, T, K, GQ::kGroupK, BT,
                          CU_TENSOR_MAP_SWIZZLE_128B, "A")) {
@@ -112,8 +184,8 @@ int arc_a8w4_grouped_gemm(const int8_t* A, const float* sa, const uint8_t* Wp, c
   p.R = GQ::kRows;
   p.tiles_n = ceil_div(N, GQ::kRows);
   p.split = (flags & ARC_A8W4_PREPACKED) ? 1u : 0u;
-  p.groups = {offsets, static_cast<uint32_t>(E), static_cast<uint32_t>(T)};
-  p.zero_others = (flags & ARC_GROUPED_ZERO_OTHERS) ? 1u : 0u;
+  p.groups = groups;
+  p.zero_others = zero_others ? 1u : 0u;
   const uint64_t tiles = uint64_t(live + T / BT) * p.tiles_n;
   const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
   const uint32_t grid = tiles < sms ? static_cast<uint32_t>(tiles) : sms;

@@ -3,6 +3,7 @@
 // api.cu, whose helpers it uses.
 #pragma once
 
+#include "gemm_grouped_pair.cuh"
 #include "gemm_linear_pair.cuh"
 #include "gemm_linear_stream.cuh"
 #include "linear_backward.cuh"
@@ -11,6 +12,7 @@ namespace {
 
 namespace LS = arcb::linstream;
 namespace LP = arcb::linpair;
+namespace GP = arcb::grouppair;
 namespace LB = arcb::linbwd;
 
 // Row-major matrices [groups][rows][cols] (bf16), `ld` elements between rows and
@@ -38,12 +40,12 @@ uint32_t row_vec(const void* p, uint64_t ld, uint64_t group_stride = 0) {
   return (bits & 31u) == 0 ? 2u : (bits & 15u) == 0 ? 1u : 0u;
 }
 
-// The kernel for a product with row groups: out[rows][cols], `num_kb` contraction blocks.
+// The kernel for a product of rows, in one group or several.
 //
-// Pairs (256 x 256 tiles) when the groups' rows fill such tiles and there are tiles enough to
-// give most pairs one; else the streaming kernel, its row tile the smallest that holds an
+// Pairs (256 x 256 tiles) when the groups' rows fill half such a tile and there are tiles for
+// half of the pairs; else the streaming kernel, its row tile the smallest that holds an
 // average group's rows, with the contraction split over a cluster until the two block slots
-// of every SM have work (at least kMinKb blocks of 64 each).
+// of every SM have work (at least kStreamMinKb blocks of 64 each).
 //
 // ARC_LINEAR_PLAN="pair" | "BN:S" (tests and tuning) forces the choice where it is valid.
 struct LinearPlan {
@@ -113,11 +115,15 @@ cudaError_t linear_init(DeviceState& st) {
   if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, false, false>, LP::kSmemBytes);
   if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, true, false>, LP::kSmemBytes);
   if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<true, true, true>, LP::kSmemBytes);
+  if (e == cudaSuccess) e = allow_smem(GP::gemm_grouped_pair_kernel<false, false>, GP::smem_bytes<false>());
+  if (e == cudaSuccess) e = allow_smem(GP::gemm_grouped_pair_kernel<true, false>, GP::smem_bytes<false>());
+  if (e == cudaSuccess) e = allow_smem(GP::gemm_grouped_pair_kernel<false, true>, GP::smem_bytes<true>());
   if (e != cudaSuccess) return e;
+  // How many pairs of the largest of these kernels fit at once.
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3(st.sms, 1, 1);
-  cfg.blockDim = dim3(LP::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = LP::kSmemBytes;
+  cfg.blockDim = dim3(GP::threads<true>(), 1, 1);
+  cfg.dynamicSmemBytes = GP::smem_bytes<true>();
   cudaLaunchAttribute attr[1];
   attr[0].id = cudaLaunchAttributeClusterDimension;
   attr[0].val.clusterDim.x = 2;
@@ -126,9 +132,27 @@ cudaError_t linear_init(DeviceState& st) {
   cfg.attrs = attr;
   cfg.numAttrs = 1;
   int n = 0;
-  e = cudaOccupancyMaxActiveClusters(&n, LP::gemm_linear_pair_kernel<true, true, true>, &cfg);
+  e = cudaOccupancyMaxActiveClusters(&n, GP::gemm_grouped_pair_kernel<false, true>, &cfg);
   st.max_linear_pairs = e == cudaSuccess ? n : 0;
   return e;
+}
+
+// The walk's fields and the launch of the grouped pair kernel (its maps are set by the caller).
+cudaError_t grouped_pair_launch(GP::Params& p, const arcb::lin::Groups& groups, uint16_t* out, uint64_t ldo,
+                                uint32_t cols, bool zero_others, uint32_t max_pairs, void (*kernel)(GP::Params),
+                                uint32_t threads, size_t smem, cudaStream_t stream) {
+  p.out = out;
+  p.ldo = ldo;
+  p.groups = groups;
+  p.cols = cols;
+  p.tiles_f = ceil_div(cols, GP::kTileF);
+  p.pair_store = cols % 2 == 0 && ldo % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
+  p.zero_others = zero_others ? 1u : 0u;
+  // The host knows only a bound: a group of c rows has at most c / kTileT + 1 row tiles.
+  const uint64_t tiles = uint64_t((groups.num < groups.rows ? groups.num : groups.rows) + groups.rows / GP::kTileT) *
+                         p.tiles_f;
+  const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
+  return launch_ex(kernel, p, grid, threads, smem, 2, stream);
 }
 
 // out[rows][cols] = epilogue of a [rows][inner] times w, per group. grad = false: w is
@@ -143,19 +167,40 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
   if (int st = linear_plan(dev, groups.rows, groups.num, cols, num_kb, &plan)) return st;
   const uint64_t w_rows = grad ? inner : cols, w_cols = grad ? cols : inner;
   cudaError_t e;
+  const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
+  if (plan.pair && groups.offsets != nullptr) {
+    GP::Params p = {};
+    if (int st = encode_groups_3d(&p.tm_w, w, w_cols, w_rows, groups.num, ldw, w_stride, 64,
+                                  grad ? 64 : GP::kRowsPerCta, "weights")) {
+      return st;
+    }
+    if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a, inner, groups.rows, lda, GP::kSubK,
+                           GP::kBox, CU_TENSOR_MAP_SWIZZLE_128B, "rows")) {
+      return st;
+    }
+    if (int st = encode_2d(&p.tm_xs, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a, inner, groups.rows, lda, GP::kSubK,
+                           GP::kSmallBox, CU_TENSOR_MAP_SWIZZLE_128B, "rows")) {
+      return st;
+    }
+    p.num_kb = num_kb;
+    e = grouped_pair_launch(p, groups, out, ldo, cols, zero_others, max_pairs,
+                            grad ? GP::gemm_grouped_pair_kernel<true, false> : GP::gemm_grouped_pair_kernel<false, false>,
+                            GP::threads<false>(), GP::smem_bytes<false>(), stream);
+    if (e != cudaSuccess) return cuda_fail(e, "gemm_grouped_pair_kernel launch");
+    return ARC_OK;
+  }
   if (plan.pair) {
     LP::Params p = {};
     if (int st = encode_groups_3d(&p.tm_a, a, inner, groups.rows, 1, lda, uint64_t(groups.rows) * lda, 64,
                                   LP::kRowsPerCta, "rows")) {
       return st;
     }
-    if (int st = encode_groups_3d(&p.tm_b, w, w_cols, w_rows, groups.num, ldw, w_stride, 64,
-                                  grad ? 64 : LP::kRowsPerCta, "weights")) {
+    if (int st = encode_groups_3d(&p.tm_b, w, w_cols, w_rows, 1, ldw, w_stride, 64, grad ? 64 : LP::kRowsPerCta,
+                                  "weights")) {
       return st;
     }
     p.out = out;
     p.ldo = ldo;
-    p.groups = groups;
     p.epi = epi;
     p.epi.vec_out = row_vec(out, ldo);
     p.M = groups.rows;
@@ -163,13 +208,8 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
     p.tiles_m = ceil_div(groups.rows, LP::kTile);
     p.tiles_n = ceil_div(cols, LP::kTile);
     p.num_kb = num_kb;
-    p.zero_others = zero_others ? 1u : 0u;
-    const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
-    const uint64_t tiles =
-        (groups.offsets == nullptr ? uint64_t(p.tiles_m)
-                                   : uint64_t(groups.num < groups.rows ? groups.num : groups.rows) +
-                                         groups.rows / LP::kTile) *
-        p.tiles_n;
+    const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
+    if (tiles > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
     const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
     e = grad ? launch_ex(LP::gemm_linear_pair_kernel<false, true, false>, p, grid, LP::kThreads, LP::kSmemBytes, 2,
                          stream)

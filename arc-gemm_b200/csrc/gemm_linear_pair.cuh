@@ -1,7 +1,7 @@
-// gemm_linear_pair.cuh — the linear layer's and the grouped products' large form, on CTA pairs.
+// gemm_linear_pair.cuh — the linear layer's large form and the weight gradients, on CTA pairs.
 //
-//   rows mode:         out[t, f]    = epilogue( sum_k a[t, k] b[e(t), f, k] )    (row groups)
-//   contraction mode:  out[e, i, j] = sum_{t in group e} a[t, i] b[t, j]         (weight gradient)
+//   rows:               out[t, f]    = epilogue( sum_k a[t, k] b[f, k] )
+//   contraction groups: out[e, i, j] = sum_{t in group e} a[t, i] b[t, j]     (weight gradient)
 //
 // Bound by the tensor pipe: a pair runs 256 x 256 x 16 UMMAs (cta_group::2), each CTA holding
 // half of A's and half of B's rows, so that per 64 of the contraction a CTA's shared memory is
@@ -13,18 +13,15 @@
 // (the forward product); an MN-major one has the output index contiguous: w in the gradient
 // of the rows, both operands in the gradient of the weights. No transposed copy is made.
 //
-// Groups. Rows mode: the tiles of group e start at its first row; rows of the next group that
-// a tile's box also covers give accumulator rows that are not stored. Contraction mode: the
-// last block of a group may hold rows of the next one, which must not enter the sums, whatever
-// they hold (infinities and NaN included, so one zeroed operand is not enough). The steps of 16
-// that lie wholly behind the group are not issued; the rows behind it inside the last step are
-// overwritten with zeros in shared memory, in both operands, by a warp of each CTA between the
-// load's arrival and the product.
+// Contraction groups. The last block of a group may hold rows of the next one, which must not
+// enter the sums, whatever they hold (infinities and NaN included, so one zeroed operand is not
+// enough). The steps of 16 that lie wholly behind the group are not issued; the rows behind it
+// inside the last step are overwritten with zeros in shared memory, in both operands, by a warp
+// of each CTA between the load's arrival and the product.
 //
-// Roles (256 threads per CTA): warp 0 TMA producer, warp 1 UMMA issuer (rank 0), warp 2 TMEM
-// owner and tile table, warp 3 zeroes a group's tail (contraction mode), warps 4-7 epilogue: a
-// thread owns one output row and takes 32 columns at a time, which it stores as two 32-byte
-// sectors.
+// Roles (384 threads per CTA): warp 0 TMA producer, warp 1 UMMA issuer (rank 0), warp 2 TMEM
+// owner, warp 3 zeroes a group's tail, warps 4-11 epilogue: two warpgroups take 32 columns in
+// turn, a thread owns one output row and stores 32 columns as two 32-byte sectors.
 #pragma once
 
 #include "gemm_bf16_pair.cuh"
@@ -39,7 +36,8 @@ using lin::kUmmaK;
 constexpr uint32_t kRowsPerCta = 128;
 constexpr uint32_t kTile = 256;  // pair tile, both directions
 constexpr uint32_t kStages = 6;
-constexpr uint32_t kThreads = 256;
+constexpr uint32_t kEpiWarps = 8;
+constexpr uint32_t kThreads = 32 * (4 + kEpiWarps);
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kBandM = 8;  // row tiles per raster band (L2 reuse)
 constexpr uint32_t kOperandBytes = kRowsPerCta * BK * 2;
@@ -57,8 +55,6 @@ struct alignas(1024) Smem {
   uint64_t drain;
   uint32_t tmem_base;
   uint32_t abort;
-  uint32_t epi_ok;
-  uint32_t prefix[lin::kMaxGroups + 1];
 };
 constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
 static_assert(kSmemBytes <= 232448, "shared memory fits in 227 KB");
@@ -69,36 +65,34 @@ struct Params {
   uint16_t* out;
   uint64_t ldo;        // elements between output rows
   uint64_t out_group;  // contraction mode: elements between the groups' outputs
-  lin::Groups groups;
+  lin::Groups groups;  // contraction groups (rows: unused)
   lin::Epilogue epi;
-  uint32_t M, N;       // contraction mode: the output's rows; rows mode takes M from the groups
-  uint32_t tiles_m;    // contraction mode, or one group: row tiles
-  uint32_t tiles_n, num_kb;
-  uint32_t zero_others;
+  uint32_t M, N;       // output rows (of a group) and columns
+  uint32_t tiles_m, tiles_n, num_kb;
 };
 
 // One tile of the walk.
 struct Tile {
-  uint32_t e;            // group
-  uint32_t m0, m_end;    // first output row of the pair tile, end of its rows
-  uint32_t n0;
-  uint32_t k0;           // contraction mode: first contraction row
-  uint32_t num_kb;       // blocks of 64
-  uint32_t last_steps;   // UMMA steps of the last block (4 unless a group ends inside it)
-  uint32_t tail_rows;    // valid rows of the last block if it needs zeroing, else 0
+  uint32_t e;           // group
+  uint32_t m0, n0;
+  uint32_t k0;          // first contraction row
+  uint32_t num_kb;      // blocks of 64
+  uint32_t last_steps;  // UMMA steps of the last block (4 unless a group ends inside it)
+  uint32_t tail_rows;   // valid rows of the last block if it needs zeroing, else 0
 };
 
 template <bool ALONG_K>
-__device__ __forceinline__ bool tile_at(const Params& p, const uint32_t* prefix, uint32_t t, Tile& w) {
-  uint32_t rem, tiles_m;
-  w.tail_rows = 0;
+__device__ __forceinline__ bool tile_at(const Params& p, uint32_t t, Tile& w) {
+  const uint32_t per = p.tiles_m * p.tiles_n;
+  w.e = 0;
+  w.k0 = 0;
+  w.num_kb = p.num_kb;
   w.last_steps = BK / kUmmaK;
+  w.tail_rows = 0;
   if (ALONG_K) {
-    const uint32_t per = p.tiles_m * p.tiles_n;
     w.e = t / per;
     if (w.e >= p.groups.num) return false;
-    rem = t - w.e * per;
-    tiles_m = p.tiles_m;
+    t -= w.e * per;
     w.k0 = lin::group_begin(p.groups, w.e);
     const uint32_t cnt = lin::group_count(p.groups, w.e);
     w.num_kb = (cnt + BK - 1u) / BK;
@@ -106,35 +100,15 @@ __device__ __forceinline__ bool tile_at(const Params& p, const uint32_t* prefix,
     w.last_steps = (last + kUmmaK - 1u) / kUmmaK;
     // Rows past the matrix are zero as TMA fills them.
     if ((last % kUmmaK) != 0u && w.k0 + cnt < p.groups.rows) w.tail_rows = last;
-  } else {
-    if (p.groups.offsets == nullptr) {
-      if (t >= p.tiles_m * p.tiles_n) return false;
-      w.e = 0;
-      rem = t;
-      tiles_m = p.tiles_m;
-    } else {
-      if (t >= prefix[p.groups.num] * p.tiles_n) return false;
-      w.e = lin::group_of_tile(prefix, p.groups.num, t / p.tiles_n);
-      rem = t - prefix[w.e] * p.tiles_n;
-      tiles_m = prefix[w.e + 1] - prefix[w.e];
-    }
-    w.k0 = 0;
-    w.num_kb = p.num_kb;
+  } else if (t >= per) {
+    return false;
   }
-  const uint32_t band = rem / (kBandM * p.tiles_n);
-  rem -= band * kBandM * p.tiles_n;
+  const uint32_t band = t / (kBandM * p.tiles_n);
+  const uint32_t rem = t - band * kBandM * p.tiles_n;
   const uint32_t m_first = band * kBandM;
-  const uint32_t m_cnt = min(kBandM, tiles_m - m_first);
-  const uint32_t mb = m_first + rem % m_cnt;
+  const uint32_t m_cnt = min(kBandM, p.tiles_m - m_first);
+  w.m0 = (m_first + rem % m_cnt) * kTile;
   w.n0 = rem / m_cnt * kTile;
-  if (ALONG_K) {
-    w.m0 = mb * kTile;
-    w.m_end = p.M;
-  } else {
-    const uint32_t first = lin::group_begin(p.groups, w.e);
-    w.m0 = first + mb * kTile;
-    w.m_end = first + lin::group_count(p.groups, w.e);
-  }
   return true;
 }
 
@@ -159,7 +133,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     }
     for (uint32_t i = 0; i < 2; ++i) {
       mbar_init(&s.tmem_full[i], 1);
-      mbar_init(&s.tmem_empty[i], 8);  // 4 epilogue warps x 2 CTAs
+      mbar_init(&s.tmem_empty[i], 2 * kEpiWarps);  // of both CTAs
     }
     mbar_init(&s.drain, 1);
     s.abort = 0;
@@ -171,7 +145,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
   if (warp == 2) {
     tmem_alloc_pair(&s.tmem_base, kTmemCols);
     tmem_relinquish_pair();
-    if (!ALONG_K && p.groups.offsets != nullptr) lin::group_tiles_prefix(p.groups, kTile, s.prefix);
   }
   tc_fence_before_sync();
   __syncthreads();
@@ -179,7 +152,6 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
   tc_fence_after_sync();
   pdl_launch_dependents();
   const uint32_t tmem_base = s.tmem_base;
-  if (!ALONG_K && p.zero_others) lin::zero_other_rows(p.groups, p.out, p.ldo, p.N, blockIdx.x, gridDim.x);
 
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
@@ -189,8 +161,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       const uint32_t row0 = rank * kRowsPerCta;
       Tile w;
       bool ok = true;
-      for (uint32_t t = pair; ok && tile_at<ALONG_K>(p, s.prefix, t, w); t += num_pairs) {
-        const int32_t za = 0, zb = ALONG_K ? 0 : int32_t(w.e);
+      for (uint32_t t = pair; ok && tile_at<ALONG_K>(p, t, w); t += num_pairs) {
         for (uint32_t kb = 0; kb < w.num_kb; ++kb) {
           if (!mbar_wait(&s.empty[stage], phase ^ 1u, abort, kStatusTimeoutProducer)) {
             ok = false;
@@ -210,16 +181,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
           }
           const int32_t k = int32_t(w.k0 + kb * BK), m = int32_t(w.m0 + row0), n = int32_t(w.n0 + row0);
           if (A_MN) {
-            tma_load_3d_pair(&p.tm_a, bar, s.a[stage], m, k, za, kCacheEvictNormal);
-            tma_load_3d_pair(&p.tm_a, bar, s.a[stage] + lin::kMnChunkBytes, m + 64, k, za, kCacheEvictNormal);
+            tma_load_3d_pair(&p.tm_a, bar, s.a[stage], m, k, 0, kCacheEvictNormal);
+            tma_load_3d_pair(&p.tm_a, bar, s.a[stage] + lin::kMnChunkBytes, m + 64, k, 0, kCacheEvictNormal);
           } else {
-            tma_load_3d_pair(&p.tm_a, bar, s.a[stage], k, m, za, kCacheEvictNormal);
+            tma_load_3d_pair(&p.tm_a, bar, s.a[stage], k, m, 0, kCacheEvictNormal);
           }
           if (B_MN) {
-            tma_load_3d_pair(&p.tm_b, bar, s.b[stage], n, k, zb, kCacheEvictNormal);
-            tma_load_3d_pair(&p.tm_b, bar, s.b[stage] + lin::kMnChunkBytes, n + 64, k, zb, kCacheEvictNormal);
+            tma_load_3d_pair(&p.tm_b, bar, s.b[stage], n, k, 0, kCacheEvictNormal);
+            tma_load_3d_pair(&p.tm_b, bar, s.b[stage] + lin::kMnChunkBytes, n + 64, k, 0, kCacheEvictNormal);
           } else {
-            tma_load_3d_pair(&p.tm_b, bar, s.b[stage], k, n, zb, kCacheEvictNormal);
+            tma_load_3d_pair(&p.tm_b, bar, s.b[stage], k, n, 0, kCacheEvictNormal);
           }
           ++issued;
           if (++stage == kStages) {
@@ -243,21 +214,24 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     }
   } else if (warp == 1) {
     // ------------------------------------------------------------ UMMA issuer (rank 0)
-    if (rank == 0 && lane == 0) {
+    // The whole warp walks (uniform values stay in uniform registers, fewer instructions per
+    // stage), one lane issues.
+    if (rank == 0) {
+      const bool leader = elect_one();
       constexpr uint32_t idesc = lin::idesc_of<A_MN, B_MN>(kTile, kTile);
       uint32_t stage = 0, phase = 0, local = 0;
       bool ok = true;
       Tile w;
-      for (uint32_t t = pair; ok && tile_at<ALONG_K>(p, s.prefix, t, w); t += num_pairs) {
+      for (uint32_t t = pair; ok && tile_at<ALONG_K>(p, t, w); t += num_pairs) {
         if (w.num_kb == 0u) continue;  // a group without rows: the epilogue stores zeros
         const uint32_t acc = local & 1u;
         const uint32_t acc_phase = (local >> 1) & 1u;
         ++local;
-        if (!mbar_wait(&s.tmem_empty[acc], acc_phase ^ 1u, abort, kStatusTimeoutMma)) break;
+        if (!__all_sync(0xffffffffu, mbar_wait(&s.tmem_empty[acc], acc_phase ^ 1u, abort, kStatusTimeoutMma))) break;
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + acc * kTile;
         for (uint32_t kb = 0; kb < w.num_kb; ++kb) {
-          if (!mbar_wait(&s.full[stage], phase, abort, kStatusTimeoutMma)) {
+          if (!__all_sync(0xffffffffu, mbar_wait(&s.full[stage], phase, abort, kStatusTimeoutMma))) {
             ok = false;
             break;
           }
@@ -267,22 +241,25 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
           const uint32_t steps = kb + 1u == w.num_kb ? w.last_steps : BK / kUmmaK;
 #pragma unroll
           for (uint32_t k = 0; k < BK / kUmmaK; ++k) {
-            if (!ALONG_K || k < steps) {
+            if (leader && (!ALONG_K || k < steps)) {
               umma_bf16_pair(d_tmem, desc_advance(adesc, k * lin::operand_step<A_MN>()),
                              desc_advance(bdesc, k * lin::operand_step<B_MN>()), idesc, (kb | k) != 0u ? 1u : 0u);
             }
           }
-          umma_commit_pair(&s.empty[stage], 0x3);
+          if (leader) umma_commit_pair(&s.empty[stage], 0x3);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok) umma_commit_pair(&s.tmem_full[acc], 0x3);
+        if (ok && leader) umma_commit_pair(&s.tmem_full[acc], 0x3);
       }
       // Every pair UMMA must retire before either CTA releases TMEM or exits.
-      umma_commit_pair(&s.drain, 0x1);
-      mbar_drain(&s.drain, 0);
+      if (leader) {
+        umma_commit_pair(&s.drain, 0x1);
+        mbar_drain(&s.drain, 0);
+      }
+      __syncwarp();
     }
   } else if (warp == 3) {
     // ------------------------------------------------------------ a group's tail
@@ -290,7 +267,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       uint32_t stage = 0, parity = 0;  // parity: per stage, of its next tail
       Tile w;
       bool ok = true;
-      for (uint32_t t = pair; ok && tile_at<ALONG_K>(p, s.prefix, t, w); t += num_pairs) {
+      for (uint32_t t = pair; ok && tile_at<ALONG_K>(p, t, w); t += num_pairs) {
         if (w.num_kb == 0u) continue;
         const uint32_t st = (stage + w.num_kb - 1u) % kStages;
         stage = (stage + w.num_kb) % kStages;
@@ -323,19 +300,19 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
   } else if (warp >= 4) {
     // ------------------------------------------------------------ epilogue (both CTAs)
     const uint32_t q = warp & 3u;
-    const uint32_t et = threadIdx.x - 128;
+    const uint32_t wg = (warp - 4u) >> 2;
     const uint32_t row = q * 32 + lane;
     const uint32_t empty0[2] = {map_to_rank(&s.tmem_empty[0], 0), map_to_rank(&s.tmem_empty[1], 0)};
     uint32_t local = 0;
     Tile w;
-    for (uint32_t t = pair; tile_at<ALONG_K>(p, s.prefix, t, w); t += num_pairs) {
+    for (uint32_t t = pair; tile_at<ALONG_K>(p, t, w); t += num_pairs) {
       const uint32_t m = w.m0 + rank * kRowsPerCta + row;
-      const bool valid = m < w.m_end;
+      const bool valid = m < p.M;
       uint16_t* out = p.out + (ALONG_K ? size_t(w.e) * p.out_group : 0u) + size_t(valid ? m : 0u) * p.ldo;
       if (ALONG_K && w.num_kb == 0u) {
         const uint32_t zero[16] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
 #pragma unroll 1
-        for (uint32_t n = w.n0; n < min(w.n0 + kTile, p.N) && valid; n += 32u) {
+        for (uint32_t n = w.n0 + wg * 32u; n < min(w.n0 + kTile, p.N) && valid; n += 64u) {
           lin::store_row32(out + n, zero, p.N - n, p.epi.vec_out);
         }
         __syncwarp();
@@ -344,28 +321,26 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       const uint32_t acc = local & 1u;
       const uint32_t acc_phase = (local >> 1) & 1u;
       ++local;
-      if (et == 0) {
-        s.epi_ok = mbar_wait(&s.tmem_full[acc], acc_phase, abort, kStatusTimeoutEpilogue) ? 1u : 0u;
+      // The residual comes from memory: its first columns are asked for before the wait, the
+      // next ones while the present are worked on.
+      const bool with_residual = !ALONG_K && p.epi.residual != nullptr && valid;
+      const uint16_t* residual = p.epi.residual + (with_residual ? size_t(m) * p.epi.ldr : 0u);
+      uint32_t res[16];
+      if (with_residual && w.n0 + wg * 32u < p.N) {
+        lin::load_row32(residual + w.n0 + wg * 32u, res, p.N - (w.n0 + wg * 32u), p.epi.vec_residual);
       }
-      named_barrier_sync(1, 128);
-      const uint32_t go = *reinterpret_cast<volatile uint32_t*>(&s.epi_ok);
-      named_barrier_sync(1, 128);  // everyone has read it before the next tile's wait may write it
-      if (go == 0u) break;
+      if (!__all_sync(0xffffffffu, mbar_wait(&s.tmem_full[acc], acc_phase, abort, kStatusTimeoutEpilogue))) break;
       tc_fence_after_sync();
       const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * kTile;
 #pragma unroll 1
-      for (uint32_t c = 0; c < kTile / 32u; ++c) {
+      for (uint32_t c = wg; c < kTile / 32u; c += 2u) {
         const uint32_t n = w.n0 + c * 32u;
         const uint32_t cols = n < p.N ? p.N - n : 0u;  // columns in range (more than 32: all)
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_row + c * 32u, r);
-        uint32_t res[16];
         const bool live = valid && cols != 0u;
-        if (!ALONG_K && live && p.epi.residual != nullptr) {
-          lin::load_row32(p.epi.residual + size_t(m) * p.epi.ldr + n, res, cols, p.epi.vec_residual);
-        }
         tmem_ld_wait();
-        if (c == kTile / 32u - 1u) {
+        if (c + 2u >= kTile / 32u) {
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster(empty0[acc]);
@@ -403,11 +378,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
               default:
                 break;
             }
-            if (p.epi.residual != nullptr) {
+            if (with_residual) {
 #pragma unroll
               for (uint32_t i = 0; i < 16; ++i) {
                 r[2 * i] = __float_as_uint(__uint_as_float(r[2 * i]) + __uint_as_float(res[i] << 16));
                 r[2 * i + 1] = __float_as_uint(__uint_as_float(r[2 * i + 1]) + __uint_as_float(res[i] & 0xFFFF0000u));
+              }
+              const uint32_t n2 = n + 64u;
+              if (c + 2u < kTile / 32u && n2 < p.N) {
+                lin::load_row32(residual + n2, res, p.N - n2, p.epi.vec_residual);
               }
             }
           }

@@ -107,14 +107,28 @@ __device__ __forceinline__ float gelu_tanh_arg(float z) {
   return 2.f * kSqrt2OverPi * (z + kGeluCubic * z * z * z);
 }
 
-// In the lower tail 1 + erf cancels to an absolute error of about 2^-24 |z|, far below the
-// output's own rounding for every value that is not itself about that small.
+// e = exp(-x^2) and q = 1 - erf(x) for x = |z| / sqrt(2), by formula 7.1.26 of Abramowitz and
+// Stegun (Handbook of Mathematical Functions): q = (a1 t + ... + a5 t^5) e with t = 1 / (1 + p x),
+// off by at most 1.5e-7. The erf form's value and slope need both, and 2 Phi(z) = 1 + erf is q
+// itself below zero, so nothing cancels in the lower tail.
+__device__ __forceinline__ float erfc_of(float z, float& e) {
+  const float x = fabsf(z) * kSqrtHalf;
+  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
+  e = __expf(-x * x);
+  const float poly =
+      t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
+  return poly * e;
+}
+
 __device__ __forceinline__ float act_value(float z, uint32_t act) {
   switch (act) {
     case kActRelu:
       return z > 0.f ? z : (z != z ? z : 0.f);
-    case kActGelu:
-      return 0.5f * z * (1.f + erff(z * kSqrtHalf));
+    case kActGelu: {
+      float e;
+      const float q = erfc_of(z, e);
+      return 0.5f * z * (z < 0.f ? q : 2.f - q);
+    }
     case kActGeluTanh:
       return z * sigmoidf(gelu_tanh_arg(z));
     case kActSilu:
@@ -129,8 +143,11 @@ __device__ __forceinline__ float act_slope(float z, uint32_t act) {
   switch (act) {
     case kActRelu:
       return z > 0.f ? 1.f : 0.f;
-    case kActGelu:
-      return 0.5f * (1.f + erff(z * kSqrtHalf)) + z * kInvSqrt2Pi * __expf(-0.5f * z * z);
+    case kActGelu: {
+      float e;
+      const float q = erfc_of(z, e);
+      return 0.5f * (z < 0.f ? q : 2.f - q) + z * kInvSqrt2Pi * e;
+    }
     case kActGeluTanh: {
       const float s = sigmoidf(gelu_tanh_arg(z));
       return s + z * s * (1.f - s) * (2.f * kSqrt2OverPi) * (1.f + 3.f * kGeluCubic * z * z);

@@ -356,10 +356,16 @@ int arc_grouped_matmul_dw(const uint16_t *dy, const uint16_t *x, const int32_t *
  *   Wp [E][N][K/2], sb [E][N][K/128], C [T][N], all contiguous; offsets as above (not NULL).
  * flags: ARC_A8W4_PREPACKED, ARC_GROUPED_ZERO_OTHERS. Requirements: group == 128,
  * K % 128 == 0, N % 8 == 0, E <= 1024, E * N < 2^31; A, Wp and C 16-byte aligned.
+ * Few rows per group: the int32 partials are exact and the scales multiply them in fp32. Many
+ * (more than 128 on average): code times scale is the tensor cores' fp16 operand, exactly, and
+ * the sum over K runs in fp32; scales below 2^-24 of their weight row's largest may round.
+ * workspace: 16-byte aligned, arc_a8w4_grouped_workspace_bytes (0 for few rows per group), no
+ * initialisation needed.
  */
+int arc_a8w4_grouped_workspace_bytes(int T, int E, int K, size_t *bytes);
 int arc_a8w4_grouped_gemm(const int8_t *A, const float *sa, const uint8_t *Wp, const uint16_t *sb,
-                          const int32_t *offsets, uint16_t *C, int T, int E, int N, int K, int group, unsigned flags,
-                          cudaStream_t stream);
+                          const int32_t *offsets, uint16_t *C, void *workspace, size_t workspace_bytes, int T, int E,
+                          int N, int K, int group, unsigned flags, cudaStream_t stream);
 
 /*
  * Sorts a router's choices by group (stable): ids [slots] (id_bytes 4 or 8, signed; slots =

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import arc
+from arc import _lib
 from arc._lib import STATUS_BAD_OFFSETS
 from linear_bounds import H, SUM, assert_within, normal
 
@@ -158,38 +159,81 @@ def _a8w4(sizes, behind, n, k, seed=0):
     return (x, sa), (wp, sb), _offsets(sizes)
 
 
-@pytest.mark.parametrize("sizes,behind", [*SPLITS, ([300, 0, 200], 1), ([20, 30, 25], 0), ([50, 60], 5)])
-@pytest.mark.parametrize("n,k", [(8, 128), (264, 384), (128, 1024)])
-@pytest.mark.parametrize("prepacked", [False, True])
-def test_a8w4_grouped(cuda_device, sizes, behind, n, k, prepacked):
-    """Every group's rows against arc.a8w4_matmul's definition in 64 bits: the int32 partial sums are
-    exact, the fp32 scale sum is off by at most (G + 8) 2^-23 of its terms' magnitude (the bias kept in
-    the accumulators included: 2^-9 of a term's scale and group of four), one rounding to bf16."""
-    a, (wp, sb), offsets = _a8w4(sizes, behind, n, k)
-    x, sa = a
-    packed = arc.prepack_weights(wp.view(-1, k // 2)).view_as(wp) if prepacked else wp
+@pytest.fixture(params=["narrow", "wide"])
+def a8w4_kernel(request, monkeypatch):
+    """Both kernels on every size: int32 partial sums, or scales in the fp16 operand."""
+    monkeypatch.setenv("ARC_A8W4_GROUPED", request.param)
+    _lib.workspace_bytes.cache_clear()
+    yield request.param
+    _lib.workspace_bytes.cache_clear()
+
+
+def _check_a8w4(kernel, a, b, sizes, offsets, prepacked=False):
+    """Every group's rows against the definition in 64 bits. int32 partial sums are exact and the fp32
+    scale sum is off by at most (G + 8) 2^-23 of its terms' magnitude, plus the rounding beside the bias
+    kept in the accumulators (2^-24 of four terms of 1.5 * 2^23 / 16). Scales in the operand: an fp32 sum
+    over K of exact products, and 2^-29 of the row's largest scale for a code whose scale fp16 rounds."""
+    (x, sa), (wp, sb) = a, b
+    e, n, k2 = wp.shape
+    k = 2 * k2
+    packed = arc.prepack_weights(wp.view(-1, k2)).view_as(wp) if prepacked else wp
     got = arc.a8w4_grouped_matmul(a, (packed, sb), offsets, prepacked=prepacked)
     total = sum(sizes)
     assert (got[total:] == 0).all()
     codes = torch.stack((wp & 15, wp >> 4), -1).flatten(-2).to(torch.int64)
     codes = torch.where(codes >= 8, codes - 16, codes).double()
-    for e, (r0, r1) in enumerate(_spans(sizes)):
+    for i, (r0, r1) in enumerate(_spans(sizes)):
         if r0 == r1:
             continue
-        p = torch.einsum("tgk,ngk->tng", x[r0:r1].double().view(r1 - r0, -1, 128), codes[e].view(n, -1, 128))
-        terms = p * sb[e].double()
-        want = sa[r0:r1].double()[:, None] * terms.sum(-1)
-        bias = 4 * 1.5 * 2.0 ** 23 / 16 * sb[e].double().amax(-1) * 2.0 ** -24  # rounding beside four biased terms
-        err = sa[r0:r1].double()[:, None] * ((k // 128 + 8) * SUM * terms.abs().sum(-1) + (k // 128) * bias)
-        assert_within(got[r0:r1], want, err + H * (want.abs() + err), f"group {e}")
+        xe, scale = x[r0:r1].double(), sa[r0:r1].double()[:, None]
+        w = codes[i] * sb[i].double().repeat_interleave(128, 1)
+        want = scale * (xe @ w.T)
+        if kernel == "narrow":
+            p = torch.einsum("tgk,ngk->tng", xe.view(r1 - r0, -1, 128), codes[i].view(n, -1, 128))
+            mag = (p * sb[i].double()).abs().sum(-1)
+            bias = 4 * 1.5 * 2.0 ** 23 / 16 * sb[i].double().abs().amax(-1) * 2.0 ** -24
+            err = scale * ((k // 128 + 8) * SUM * mag + (k // 128) * bias)
+        else:
+            small = 2.0 ** -29 * sb[i].double().abs().amax(-1)
+            err = scale * ((k + 4) * SUM * (xe.abs() @ w.abs().T) + xe.abs().sum(-1, keepdim=True) * small)
+        assert_within(got[r0:r1], want, err + H * (want.abs() + err) + 1e-38, f"group {i}")
     out = torch.full_like(got, 2.0)
     arc.a8w4_grouped_matmul(a, (packed, sb), offsets, out=out, prepacked=prepacked)
     assert torch.equal(out[:total], got[:total]) and (out[total:] == 2).all()
     assert arc.device_status(0) == 0
 
 
+@pytest.mark.parametrize("sizes,behind", [*SPLITS, ([300, 0, 200], 1), ([20, 30, 25], 0), ([50, 60], 5)])
+@pytest.mark.parametrize("n,k", [(8, 128), (264, 384), (520, 1024)])
+@pytest.mark.parametrize("prepacked", [False, True])
+def test_a8w4_grouped(cuda_device, a8w4_kernel, sizes, behind, n, k, prepacked):
+    a, b, offsets = _a8w4(sizes, behind, n, k)
+    _check_a8w4(a8w4_kernel, a, b, sizes, offsets, prepacked)
+
+
+@pytest.mark.parametrize("k", [1024, 640])
+def test_a8w4_scales(cuda_device, a8w4_kernel, k):
+    """Scales that differ by many powers of two inside a row, zero, negative, tiny and huge ones."""
+    a, (wp, sb), offsets = _a8w4([40, 300], 0, 64, k)
+    g = torch.arange(k // 128, device="cuda")
+    sb[:, :8] *= torch.exp2(-4.0 * g).to(torch.bfloat16)
+    sb[:, 8:16] *= torch.exp2(-4.0 * g.flip(0)).to(torch.bfloat16)
+    sb[:, 16:24] = 0
+    sb[:, 24:32, 1] = 0
+    sb[:, 32:40] *= -1
+    sb[:, 40:48] *= 2.0 ** -100
+    sb[:, 48:56] *= 2.0 ** 60
+    _check_a8w4(a8w4_kernel, a, (wp, sb), [40, 300], offsets)
+
+
+def test_a8w4_kernels_are_chosen_by_rows(cuda_device):
+    for sizes in ([128, 100], [400, 300], [1, 0, 1500]):
+        a, b, offsets = _a8w4(sizes, 0, 136, 256)
+        _check_a8w4("wide" if sum(sizes) > 128 * len(sizes) else "narrow", a, b, sizes, offsets)
+
+
 def test_a8w4_one_group_is_a8w4_matmul(cuda_device):
-    a, (wp, sb), offsets = _a8w4([200], 0, 256, 512)
+    a, (wp, sb), offsets = _a8w4([100], 0, 256, 512)
     assert torch.equal(arc.a8w4_grouped_matmul(a, (wp, sb), offsets), arc.a8w4_matmul(a, (wp[0], sb[0])))
 
 

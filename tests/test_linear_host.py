@@ -76,8 +76,14 @@ def test_grouped_checks(native_lib, p):
 def test_a8w4_grouped_checks(native_lib, p):
     f = native_lib.arc_a8w4_grouped_gemm
 
+    size = ctypes.c_size_t(0)
+    query = native_lib.arc_a8w4_grouped_workspace_bytes
+    assert query(4, 0, 128, ctypes.byref(size)) == BAD
+    assert query(64, 2, 128, ctypes.byref(size)) == 0 and size.value == 0
+    assert query(640, 2, 128, ctypes.byref(size)) == 0 and size.value == 640 * 128 * 2
+
     def call(a=p, sa=p, wp=p, sb=p, off=p, c=p, t=4, e=2, n=8, k=128, group=128, flags=0):
-        return f(a, sa, wp, sb, off, c, t, e, n, k, group, flags, None)
+        return f(a, sa, wp, sb, off, c, None, 0, t, e, n, k, group, flags, None)
 
     for name in ("a", "sa", "wp", "sb", "off", "c"):
         assert call(**{name: None}) == BAD
