@@ -10,30 +10,36 @@ namespace {
 namespace GQ = arcb::a8w4;
 namespace GR = arcb::rows;
 
-// Token tile, epilogue warpgroups, load stages of the grouped A8W4 instantiations.
-#define ARC_A8W4_GROUPED_VARIANTS(X) X(16, 1, 4) X(32, 1, 4) X(64, 1, 4) X(128, 2, 3)
+// The grouped int32 kernel by token tile.
+template <uint32_t BT, uint32_t EWG, uint32_t LSN, uint32_t UWG, uint32_t UNP, uint32_t OCC>
+struct A8w4Grouped {
+  static constexpr uint32_t kPerSm = OCC;
+  using Cfg = GQ::Cfg<BT, EWG, LSN, UWG, UNP, OCC>;
+  static constexpr size_t kSmem = sizeof(GQ::GroupedSmem<BT, EWG, LSN, UWG, UNP>) + 1024;
+  static_assert(kSmem + 1024 <= 228 * 1024 / OCC, "OCC blocks fit in an SM's 228 KB");
+  static constexpr auto kKernel = GQ::gemm_a8w4_grouped_kernel<BT, EWG, LSN, UWG, UNP, OCC>;
+};
+using A8w4Grouped16 = A8w4Grouped<16, 1, 2, 1, 2, 2>;
+using A8w4Grouped32 = A8w4Grouped<32, 1, 4, 2, 3, 1>;
+using A8w4Grouped64 = A8w4Grouped<64, 1, 4, 2, 2, 1>;
+using A8w4Grouped128 = A8w4Grouped<128, 2, 3, 1, 2, 1>;
 
-template <uint32_t BT, uint32_t EWG, uint32_t LS_>
-constexpr size_t a8w4_grouped_smem() {
-  return sizeof(GQ::GroupedSmem<BT, EWG, LS_>) + 1024;
+// The register moves between warpgroups need exactly the launch count they were sized for.
+template <typename V>
+cudaError_t a8w4_grouped_attr(bool* regs_ok) {
+  cudaError_t e = allow_smem(V::kKernel, V::kSmem);
+  cudaFuncAttributes fa;
+  if (e == cudaSuccess) e = cudaFuncGetAttributes(&fa, V::kKernel);
+  if (e == cudaSuccess && fa.numRegs != static_cast<int>(V::Cfg::kLaunchRegs)) *regs_ok = false;
+  return e;
 }
 
 cudaError_t grouped_init(DeviceState&, bool* regs_ok) {
   cudaError_t e = cudaSuccess;
-#define ARC_SET_ATTR(BT, EWG, LSN)                                                                    \
-  static_assert(a8w4_grouped_smem<BT, EWG, LSN>() <= 232448, "shared memory fits in 227 KB");         \
-  if (e == cudaSuccess) {                                                                             \
-    e = allow_smem(GQ::gemm_a8w4_grouped_kernel<BT, EWG, LSN>, a8w4_grouped_smem<BT, EWG, LSN>());    \
-  }                                                                                                   \
-  if (e == cudaSuccess) {                                                                             \
-    cudaFuncAttributes fa;                                                                            \
-    e = cudaFuncGetAttributes(&fa, GQ::gemm_a8w4_grouped_kernel<BT, EWG, LSN>);                       \
-    if (e == cudaSuccess && fa.numRegs != static_cast<int>(GQ::Cfg<BT, EWG, LSN>::kLaunchRegs)) {     \
-      *regs_ok = false;                                                                               \
-    }                                                                                                 \
-  }
-  ARC_A8W4_GROUPED_VARIANTS(ARC_SET_ATTR)
-#undef ARC_SET_ATTR
+  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped16>(regs_ok);
+  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped32>(regs_ok);
+  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped64>(regs_ok);
+  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped128>(regs_ok);
   const int most = static_cast<int>(GR::smem_bytes(GR::kMaxBuckets - 1));
   for (const void* k : {reinterpret_cast<const void*>(GR::place_rows_kernel<int32_t>),
                         reinterpret_cast<const void*>(GR::place_rows_kernel<int64_t>)}) {
@@ -70,10 +76,11 @@ bool a8w4_grouped_wide(uint32_t T, uint32_t E) {
   return ceil_div(T, E < T ? E : T) > 128;
 }
 
-template <uint32_t BT, uint32_t EWG, uint32_t LS_>
-cudaError_t launch_a8w4_grouped(const GQ::GroupedParams& p, uint32_t grid, cudaStream_t stream) {
-  return launch_ex(GQ::gemm_a8w4_grouped_kernel<BT, EWG, LS_>, p, grid, GQ::Cfg<BT, EWG, LS_>::kThreads,
-                   a8w4_grouped_smem<BT, EWG, LS_>(), 1, stream);
+template <typename V>
+cudaError_t launch_a8w4_grouped(const GQ::GroupedParams& p, uint64_t tiles, uint32_t sms, cudaStream_t stream) {
+  const uint32_t slots = sms * V::kPerSm;
+  const uint32_t grid = tiles < slots ? static_cast<uint32_t>(tiles) : slots;
+  return launch_ex(V::kKernel, p, grid, V::Cfg::kThreads, V::kSmem, 1, stream);
 }
 
 // Blocks of the row grouping: one up to kOneBlockSlots slots, else one per SM of the largest
@@ -86,6 +93,9 @@ uint32_t group_rows_blocks(uint32_t slots, uint32_t* per_block) {
   }
   *per_block = ceil_div(ceil_div(slots, kRowBlocks), GR::kThreads) * GR::kThreads;
   return ceil_div(slots, *per_block);
+}
+size_t group_rows_workspace(uint32_t blocks, uint32_t groups) {
+  return blocks == 1 ? 0 : size_t(GR::counts_ld(blocks)) * (groups + 1) * sizeof(uint32_t);
 }
 
 }  // namespace
@@ -188,11 +198,10 @@ int arc_a8w4_grouped_gemm(const int8_t* A, const float* sa, const uint8_t* Wp, c
   p.zero_others = zero_others ? 1u : 0u;
   const uint64_t tiles = uint64_t(live + T / BT) * p.tiles_n;
   const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
-  const uint32_t grid = tiles < sms ? static_cast<uint32_t>(tiles) : sms;
-  const cudaError_t e = BT == 16   ? launch_a8w4_grouped<16, 1, 4>(p, grid, stream)
-                        : BT == 32 ? launch_a8w4_grouped<32, 1, 4>(p, grid, stream)
-                        : BT == 64 ? launch_a8w4_grouped<64, 1, 4>(p, grid, stream)
-                                   : launch_a8w4_grouped<128, 2, 3>(p, grid, stream);
+  const cudaError_t e = BT == 16   ? launch_a8w4_grouped<A8w4Grouped16>(p, tiles, sms, stream)
+                        : BT == 32 ? launch_a8w4_grouped<A8w4Grouped32>(p, tiles, sms, stream)
+                        : BT == 64 ? launch_a8w4_grouped<A8w4Grouped64>(p, tiles, sms, stream)
+                                   : launch_a8w4_grouped<A8w4Grouped128>(p, tiles, sms, stream);
   if (e != cudaSuccess) return cuda_fail(e, "gemm_a8w4_grouped_kernel launch");
   return ARC_OK;
 }
@@ -203,7 +212,7 @@ int arc_group_rows_workspace_bytes(int slots, int E, size_t* bytes) {
   }
   uint32_t per_block = 0;
   const uint32_t blocks = group_rows_blocks(slots, &per_block);
-  *bytes = blocks == 1 ? 0 : size_t(blocks) * (E + 1) * sizeof(uint32_t);
+  *bytes = group_rows_workspace(blocks, E);
   return ARC_OK;
 }
 
@@ -230,9 +239,9 @@ int arc_group_rows(const void* ids, int id_bytes, int32_t* offsets, int32_t* row
   }
   uint32_t per_block = 0;
   const uint32_t blocks = group_rows_blocks(slots, &per_block);
-  const size_t need = blocks == 1 ? 0 : size_t(blocks) * (E + 1) * sizeof(uint32_t);
-  if (need > 0 && (workspace == nullptr || workspace_bytes < need || (reinterpret_cast<uintptr_t>(workspace) & 3u))) {
-    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 4-byte aligned workspace of %zu bytes", what, need);
+  const size_t need = group_rows_workspace(blocks, E);
+  if (need > 0 && (workspace == nullptr || workspace_bytes < need || !aligned16(workspace))) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
   }
   int dev = 0;
   if (int st = current_device(&dev)) return st;

@@ -106,13 +106,17 @@ struct GroupedParams : Params {
   uint32_t zero_others;  // zero the output rows of no group
 };
 
-template <uint32_t BT, uint32_t EWG, uint32_t LS>
+// UWG: unpack warpgroups (on alternate steps), UNP: unpacked stages, OCC: CTAs per SM.
+template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG = 1, uint32_t UNP = kUnpacked, uint32_t OCC = 1>
 struct Cfg {
   static_assert(BT == 16 || BT == 32 || BT == 64 || BT == 128, "token tile");
   static_assert(EWG == 1 || EWG == 2, "epilogue warpgroups");
-  static_assert(LS >= 2 && LS <= kDoneRing && kUnpacked <= kDoneRing && kAccPairs < kDoneRing,
+  static_assert(LS >= 2 && LS <= kDoneRing && UNP <= kDoneRing && kAccPairs < kDoneRing,
                 "each waiter must stay within one phase of its completion barrier");
-  static constexpr uint32_t kThreads = 256 + 128 * EWG;
+  static_assert(UWG == 1 || (UWG == 2 && EWG == 1), "unpack warpgroups");
+  static_assert(OCC == 1 || (OCC == 2 && UWG == 1 && EWG == 1), "CTAs per SM");
+  static constexpr uint32_t kEpiWarp = 4 + 4 * UWG;  // first epilogue warp
+  static constexpr uint32_t kThreads = 128 + 128 * UWG + 128 * EWG;
   static constexpr uint32_t kCols = BT / EWG;               // columns per epilogue thread
   static constexpr uint32_t kChunk = kCols < 32 ? kCols : 32;  // TMEM columns per load
   static constexpr uint32_t kTmemCols = kAccPairs * kGps * BT;  // 64 to 512
@@ -122,31 +126,31 @@ struct Cfg {
   // Register budget: the producer/UMMA and unpack warpgroups drop to kRegsLow and
   // the epilogue warpgroup(s) rise to kRegsHigh, out of kLaunchRegs per thread at
   // launch (the most 1 CTA/SM allows; the host checks the compiled count).
-  static constexpr uint32_t kLaunchRegs = EWG == 2 ? 128 : 168;
+  static constexpr uint32_t kLaunchRegs = OCC == 2 ? 80 : EWG + UWG == 3 ? 128 : 168;
   static constexpr bool kSplitRegs = true;
-  static constexpr uint32_t kRegsLow = EWG == 2 ? 80 : 112;
-  static constexpr uint32_t kRegsHigh = EWG == 2 ? 176 : 232;
-  static_assert(256 * kRegsLow + 128 * EWG * kRegsHigh <= kThreads * kLaunchRegs,
+  static constexpr uint32_t kRegsLow = OCC == 2 ? 72 : EWG == 2 ? 80 : UWG == 2 ? 96 : 112;
+  static constexpr uint32_t kRegsHigh = OCC == 2 ? 96 : EWG == 2 ? 176 : UWG == 2 ? 224 : 232;
+  static_assert((128 + 128 * UWG) * kRegsLow + 128 * EWG * kRegsHigh <= kThreads * kLaunchRegs,
                 "register shares exceed the launch budget");
   static_assert(kCols % kChunk == 0, "epilogue column split");
 };
 
-template <uint32_t BT, uint32_t EWG, uint32_t LS>
+template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG = 1, uint32_t UNP = kUnpacked>
 struct alignas(1024) Smem {
-  using C = Cfg<BT, EWG, LS>;
-  uint8_t w[kUnpacked][kGps][C::kWBytes];       // unpacked int8, SW128 (UMMA A)
+  using C = Cfg<BT, EWG, LS, UWG, UNP>;
+  uint8_t w[UNP][kGps][C::kWBytes];       // unpacked int8, SW128 (UMMA A)
   uint8_t tok[LS][kGps][C::kTokBytes];          // tokens, SW128 (UMMA B)
   uint8_t wp[LS][C::kWpBytes];                  // packed int4 [128 rows][2 x 64 B], SW128
   uint64_t load_full[LS];                       // TMA bytes landed (tokens + packed W)
-  uint64_t w_full[kUnpacked];                   // 4 unpack warps wrote w[u]
+  uint64_t w_full[UNP];                         // 4 unpack warps wrote w[u]
   uint64_t mma_done[kDoneRing];                 // the UMMAs of step si retired
   uint64_t tmem_empty[kAccPairs];               // epilogue read accumulator pair a
   uint32_t tmem_base;
   uint32_t abort;
 };
 
-template <uint32_t BT, uint32_t EWG, uint32_t LS>
-struct alignas(1024) GroupedSmem : Smem<BT, EWG, LS> {
+template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG, uint32_t UNP>
+struct alignas(1024) GroupedSmem : Smem<BT, EWG, LS, UWG, UNP> {
   uint32_t prefix[lin::kMaxGroups + 1];  // row tiles of the groups before each one
 };
 
@@ -245,11 +249,12 @@ __device__ __forceinline__ void expand_piece(const uint4& x, uint32_t split, uin
 // Kernel
 // ---------------------------------------------------------------------------------
 // P: Params (one weight matrix) or GroupedParams (row groups, each with its own).
-template <uint32_t BT, uint32_t EWG, uint32_t LS, typename P>
+template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG, uint32_t UNP, uint32_t OCC, typename P>
 __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
   constexpr bool kGrouped = std::is_same<P, GroupedParams>::value;
-  using C = Cfg<BT, EWG, LS>;
-  using S_t = typename std::conditional<kGrouped, GroupedSmem<BT, EWG, LS>, Smem<BT, EWG, LS>>::type;
+  using C = Cfg<BT, EWG, LS, UWG, UNP, OCC>;
+  using S_t =
+      typename std::conditional<kGrouped, GroupedSmem<BT, EWG, LS, UWG, UNP>, Smem<BT, EWG, LS, UWG, UNP>>::type;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   S_t& s = *reinterpret_cast<S_t*>(smem_raw + smem_align_pad(smem_raw));
   const uint32_t warp = warp_idx_sync();
@@ -267,7 +272,7 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
     tma_prefetch_desc(&p.tm_tok);
     tma_prefetch_desc(&p.tm_wp);
     for (uint32_t i = 0; i < LS; ++i) mbar_init(&s.load_full[i], 1);
-    for (uint32_t i = 0; i < kUnpacked; ++i) mbar_init(&s.w_full[i], 4);  // one per unpack warp
+    for (uint32_t i = 0; i < UNP; ++i) mbar_init(&s.w_full[i], 4);  // one per unpack warp
     for (uint32_t i = 0; i < kDoneRing; ++i) mbar_init(&s.mma_done[i], 1);  // UMMA commit
     for (uint32_t i = 0; i < kAccPairs; ++i) mbar_init(&s.tmem_empty[i], 4 * EWG);
     s.abort = 0;
@@ -281,9 +286,9 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
   __syncthreads();
   tc_fence_after_sync();
   const uint32_t tmem_base = s.tmem_base;
-  if (warp >= 8) {
+  if (warp >= C::kEpiWarp) {
     // Arm every accumulator with the bias before the first UMMA may touch it.
-    const uint32_t ew = warp - 8;
+    const uint32_t ew = warp - C::kEpiWarp;
     const uint32_t row = tmem_base + (((ew & 3u) * 32u) << 16) + (ew >> 2) * C::kCols;
 #pragma unroll
     for (uint32_t b = 0; b < kAccPairs * kGps; ++b) {
@@ -400,7 +405,7 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
             stage = 0;
             phase ^= 1u;
           }
-          if (++us == kUnpacked) {
+          if (++us == UNP) {
             us = 0;
             uphase ^= 1u;
           }
@@ -409,10 +414,10 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
       // The last commit covers every UMMA this thread issued.
       if (si > 0u) mbar_drain(&s.mma_done[(si - 1u) % kDoneRing], done_parity(si - 1u));
     }
-  } else if (warp >= 4 && warp < 8) {
+  } else if (warp >= 4 && warp < C::kEpiWarp) {
     // ------------------------------------------------------------ unpack warpgroup
     if constexpr (C::kSplitRegs) regs_release<C::kRegsLow>();
-    const uint32_t ut = threadIdx.x - 128;  // 0..127
+    const uint32_t ut = (threadIdx.x - 128) % 128;  // within the warpgroup
     uint32_t stage = 0, phase = 0, us = 0, si = 0, cursor = 0;
     // Each warp waits for itself (no warpgroup barrier per step). The packed stage is
     // [128 rows][kGps x 64 B], landed by TMA with the 128-byte swizzle (16-byte chunk
@@ -428,55 +433,57 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
     bool ok = true;
     while (ok && next(cursor, w)) {
       for (uint32_t t = 0; t < steps_per_tile; ++t, ++si) {
-        // Packed tile landed, and the UMMAs that read w[us] last time have retired
-        // (both tested at once).
-        const uint32_t t1 = mbar_test(&s.load_full[stage], phase);
-        const uint32_t t2 = si >= kUnpacked ? mbar_test(&s.mma_done[(si - kUnpacked) % kDoneRing],
-                                                        done_parity(si - kUnpacked))
-                                            : 1u;
-        if (!mbar_wait_all2(&s.load_full[stage], phase, t1,
-                             &s.mma_done[(si - kUnpacked) % kDoneRing], done_parity(si - kUnpacked), t2,
-                             abort, kStatusTimeoutUnpack)) {
-          ok = false;
-          break;
-        }
-        if (ut == 0 && si - 4u < 8u) probe_mark(24 + si - 4u);
-        const uint8_t* src = s.wp[stage];
-        uint4 x[8];
+        if (UWG == 1 || si % UWG == (warp - 4u) / 4u) {  // alternate steps
+          // Packed tile landed, and the UMMAs that read w[us] last time have retired
+          // (both tested at once).
+          const uint32_t t1 = mbar_test(&s.load_full[stage], phase);
+          const uint32_t t2 = si >= UNP ? mbar_test(&s.mma_done[(si - UNP) % kDoneRing],
+                                                          done_parity(si - UNP))
+                                              : 1u;
+          if (!mbar_wait_all2(&s.load_full[stage], phase, t1,
+                               &s.mma_done[(si - UNP) % kDoneRing], done_parity(si - UNP), t2,
+                               abort, kStatusTimeoutUnpack)) {
+            ok = false;
+            break;
+          }
+          if (ut == 0 && si - 4u < 8u) probe_mark(24 + si - 4u);
+          const uint8_t* src = s.wp[stage];
+          uint4 x[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-          const uint32_t r = (i & 3u) * 32u + (ut >> 2), j = (i >> 2) * 4u + c16;
-          x[i] = *reinterpret_cast<const uint4*>(src + r * (kGps * kPackedRow) + ((j ^ (r & 7u)) << 4));
-        }
+          for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t r = (i & 3u) * 32u + (ut >> 2), j = (i >> 2) * 4u + c16;
+            x[i] = *reinterpret_cast<const uint4*>(src + r * (kGps * kPackedRow) + ((j ^ (r & 7u)) << 4));
+          }
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-          const uint32_t r = (i & 3u) * 32u + (ut >> 2);
-          uint4 lo, hi;
-          expand_piece(x[i], p.split, lo, hi);
-          uint8_t* row = s.w[us][i >> 2] + r * kGroupK;
-          *reinterpret_cast<uint4*>(row + (((2u * c16) ^ (r & 7u)) << 4)) = lo;
-          *reinterpret_cast<uint4*>(row + (((2u * c16 + 1u) ^ (r & 7u)) << 4)) = hi;
+          for (uint32_t i = 0; i < 8; ++i) {
+            const uint32_t r = (i & 3u) * 32u + (ut >> 2);
+            uint4 lo, hi;
+            expand_piece(x[i], p.split, lo, hi);
+            uint8_t* row = s.w[us][i >> 2] + r * kGroupK;
+            *reinterpret_cast<uint4*>(row + (((2u * c16) ^ (r & 7u)) << 4)) = lo;
+            *reinterpret_cast<uint4*>(row + (((2u * c16 + 1u) ^ (r & 7u)) << 4)) = hi;
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          // The warp's reads of wp[stage] completed before this arrival, and the UMMAs
+          // of this step (whose commit frees the load stage) wait for it.
+          if (lane == 0) mbar_arrive(&s.w_full[us]);
+          if (ut == 0 && si - 4u < 8u) probe_mark(32 + si - 4u);
         }
-        fence_proxy_async_smem();
-        __syncwarp();
-        // The warp's reads of wp[stage] completed before this arrival, and the UMMAs
-        // of this step (whose commit frees the load stage) wait for it.
-        if (lane == 0) mbar_arrive(&s.w_full[us]);
-        if (ut == 0 && si - 4u < 8u) probe_mark(32 + si - 4u);
         if (++stage == LS) {
           stage = 0;
           phase ^= 1u;
         }
-        if (++us == kUnpacked) us = 0;
+        if (++us == UNP) us = 0;
       }
     }
-  } else if (warp >= 8) {
+  } else if (warp >= C::kEpiWarp) {
     // ------------------------------------------------------------ epilogue
     if constexpr (C::kSplitRegs) regs_claim<C::kRegsHigh>();
-    const uint32_t ew = warp - 8;            // 0 .. 4*EWG-1
+    const uint32_t ew = warp - C::kEpiWarp;            // 0 .. 4*EWG-1
     const uint32_t q = ew & 3u;              // TMEM lane quarter
     const uint32_t hh = ew >> 2;             // column block of this warpgroup
-    const uint32_t et = threadIdx.x - 256;   // 0 .. 128*EWG-1
+    const uint32_t et = threadIdx.x - 32 * C::kEpiWarp;   // 0 .. 128*EWG-1
     const uint32_t nl = q * 32 + lane;       // weight row (output column) within the tile
     const uint32_t col0 = hh * C::kCols;     // first token column of this thread
     constexpr uint32_t kPairs = C::kCols / 2;
@@ -629,13 +636,13 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
 template <uint32_t BT, uint32_t EWG, uint32_t LS>
 __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
     gemm_a8w4_kernel(const __grid_constant__ Params p) {
-  gemm_a8w4_body<BT, EWG, LS>(p);
+  gemm_a8w4_body<BT, EWG, LS, 1, kUnpacked, 1>(p);
 }
 
-template <uint32_t BT, uint32_t EWG, uint32_t LS>
-__global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
+template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG, uint32_t UNP, uint32_t OCC>
+__global__ void __launch_bounds__(Cfg<BT, EWG, LS, UWG, UNP, OCC>::kThreads, OCC)
     gemm_a8w4_grouped_kernel(const __grid_constant__ GroupedParams p) {
-  gemm_a8w4_body<BT, EWG, LS>(p);
+  gemm_a8w4_body<BT, EWG, LS, UWG, UNP, OCC>(p);
 }
 
 }  // namespace a8w4

@@ -373,7 +373,8 @@ int arc_a8w4_grouped_gemm(const int8_t *A, const float *sa, const uint8_t *Wp, c
  *   offsets   [E+1]    first place of each group; offsets[E] counts the choices with a group
  *   rows      [slots]  token (slot / top) at each place
  *   positions [slots]  place of each choice
- * workspace: arc_group_rows_workspace_bytes (0 for few slots), no initialisation needed.
+ * workspace: 16-byte aligned, arc_group_rows_workspace_bytes (0 for few slots), no
+ * initialisation needed.
  */
 int arc_group_rows_workspace_bytes(int slots, int E, size_t *bytes);
 int arc_group_rows(const void *ids, int id_bytes, int32_t *offsets, int32_t *rows, int32_t *positions, void *workspace,
