@@ -6,11 +6,10 @@ raises. Building it is `python -m arc.build` (or `__graft_entry__.build()`).
 from __future__ import annotations
 
 import ctypes
-import functools
 import os
 import threading
 
-from .build import LIB_PATH, PROBE_LIB_PATH
+from .build import LIB_PATH, PROBE_LIB_PATH, TORCH_OPS_PATH
 
 ARC_OK = 0
 ARC_ERR_INVALID_ARGUMENT = 1
@@ -93,9 +92,6 @@ SIGNATURES = {
 # Flags of arc_a8w4_gemm_ex / arc_a8w4_gemm_gather_ex (include/arc_b200.h).
 A8W4_PREPACKED = 1
 A8W4_STATIC_WEIGHTS = 2
-# Flag of the grouped products: rows of no group are set to zero.
-GROUPED_ZERO_OTHERS = 4
-
 # Activations of arc_linear_bf16 (include/arc_b200.h).
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
@@ -139,26 +135,27 @@ def check(status: int, what: str) -> None:
         raise ArcError(status, f"{what}: {kind}: {detail}")
 
 
-def call_on(device, fn, what: str, *args) -> None:
-    """fn(*args, stream) on the device's current stream, with the device made current."""
-    import torch
-
-    index = device.index
-    if torch.cuda.current_device() == index:
-        status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    else:
-        with torch.cuda.device(index):
-            status = fn(*args, torch._C._cuda_getCurrentRawStream(index))
-    if status != ARC_OK:
-        check(status, what)
+_ops = None
 
 
-@functools.lru_cache(maxsize=1024)
-def workspace_bytes(name: str, *sizes: int) -> int:
-    """What the library's workspace query `name` says for these sizes."""
-    size = ctypes.c_size_t(0)
-    check(getattr(lib(), name)(*sizes, ctypes.byref(size)), name)
-    return size.value
+def torch_ops():
+    """The PyTorch side of the linear and grouped operators, bound to the loaded library."""
+    global _ops
+    if _ops is None:
+        handle = lib()
+        with _lock:
+            if _ops is None:
+                if not TORCH_OPS_PATH.exists():
+                    raise RuntimeError(f"{TORCH_OPS_PATH} is not built; the arc operators have no fallback. "
+                                       "Build it with `python -m arc.build`.")
+                import torch  # noqa: F401  (its libraries are what the module links against)
+
+                from . import _torch_ops
+
+                _torch_ops.bind({name: ctypes.cast(getattr(handle, name), ctypes.c_void_p).value
+                                 for name in SIGNATURES}, ArcError)
+                _ops = _torch_ops
+    return _ops
 
 
 def describe_plan(M: int, N: int, K: int, num_sms: int = 148) -> dict:

@@ -24,6 +24,9 @@ LIB_PATH = PKG_DIR / "libarcb200.so"
 PROBE_LIB_PATH = PKG_DIR / "libarcb200_probe.so"
 TVM_FFI_LIB_PATH = PKG_DIR / "libarcb200_tvm_ffi.so"
 TVM_FFI_SOURCE = "tvm_ffi_shim.cc"
+TORCH_OPS_NAME = "_torch_ops"
+TORCH_OPS_PATH = PKG_DIR / f"{TORCH_OPS_NAME}.so"
+TORCH_OPS_SOURCE = "torch_ops.cc"
 STAMP = ROOT / "_build" / "libarcb200.hash"
 
 SOURCES = ["api.cu"]
@@ -135,8 +138,45 @@ def build_tvm_ffi(force: bool = False) -> Path | None:
     return TVM_FFI_LIB_PATH
 
 
+def build_torch_ops(force: bool = False) -> Path:
+    """Compile _torch_ops.so: the linear and grouped operators' PyTorch side (checks, tensors,
+    autograd) over the C ABI. Host C++ only (g++), against the headers of the torch that is
+    installed; the C ABI's functions are handed to it by address when the package loads it.
+    """
+    import sysconfig
+
+    import torch
+
+    src = CSRC / TORCH_OPS_SOURCE
+    stamp = STAMP.with_name("torch_ops.hash")
+    h = hashlib.sha256(src.read_bytes() + (INCLUDE / "arc_b200.h").read_bytes() + torch.__version__.encode()).hexdigest()
+    if not force and TORCH_OPS_PATH.exists() and stamp.exists() and stamp.read_text().strip() == h:
+        return TORCH_OPS_PATH
+    cxx = shutil.which("g++") or shutil.which("c++")
+    if cxx is None:
+        raise RuntimeError("no C++ compiler for the PyTorch operators")
+    cuda_home = Path(find_nvcc()).resolve().parent.parent
+    tmp = TORCH_OPS_PATH.with_suffix(".so.tmp")
+    torch_dir = Path(torch.__file__).resolve().parent
+    includes = [torch_dir / "include", torch_dir / "include" / "torch" / "csrc" / "api" / "include",
+                cuda_home / "include", Path(sysconfig.get_paths()["include"])]
+    cmd = [cxx, "-std=c++17", "-O2", "-fPIC", "-shared", "-o", str(tmp), str(src), "-I", str(INCLUDE),
+           *[a for p in includes for a in ("-isystem", str(p))],
+           f"-DTORCH_EXTENSION_NAME={TORCH_OPS_NAME}", "-DTORCH_API_INCLUDE_EXTENSION_H",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch.compiled_with_cxx11_abi())}",
+           "-L", str(torch_dir / "lib"), "-ltorch", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-ltorch_python"]
+    res = subprocess.run(cmd, capture_output=True, text=True)
+    if res.returncode != 0:
+        raise RuntimeError(f"PyTorch operators: build failed ({res.returncode}):\n{res.stdout}\n{res.stderr}")
+    tmp.replace(TORCH_OPS_PATH)
+    stamp.parent.mkdir(parents=True, exist_ok=True)
+    stamp.write_text(h)
+    return TORCH_OPS_PATH
+
+
 if __name__ == "__main__":
     import sys
 
     print(build(force=True, verbose=True, probe="--probe" in sys.argv))
     print(build_tvm_ffi(force=True))
+    print(build_torch_ops(force=True))

@@ -11,18 +11,17 @@ namespace GQ = arcb::a8w4;
 namespace GR = arcb::rows;
 
 // The grouped int32 kernel by token tile.
-template <uint32_t BT, uint32_t EWG, uint32_t LSN, uint32_t UWG, uint32_t UNP, uint32_t OCC>
+template <uint32_t BT, uint32_t EWG, uint32_t LSN, uint32_t UWG, uint32_t UNP>
 struct A8w4Grouped {
-  static constexpr uint32_t kPerSm = OCC;
-  using Cfg = GQ::Cfg<BT, EWG, LSN, UWG, UNP, OCC>;
+  using Cfg = GQ::Cfg<BT, EWG, LSN, UWG, UNP>;
   static constexpr size_t kSmem = sizeof(GQ::GroupedSmem<BT, EWG, LSN, UWG, UNP>) + 1024;
-  static_assert(kSmem + 1024 <= 228 * 1024 / OCC, "OCC blocks fit in an SM's 228 KB");
-  static constexpr auto kKernel = GQ::gemm_a8w4_grouped_kernel<BT, EWG, LSN, UWG, UNP, OCC>;
+  static_assert(kSmem <= 232448, "shared memory fits in 227 KB");
+  static constexpr auto kKernel = GQ::gemm_a8w4_grouped_kernel<BT, EWG, LSN, UWG, UNP>;
 };
-using A8w4Grouped16 = A8w4Grouped<16, 1, 2, 1, 2, 2>;
-using A8w4Grouped32 = A8w4Grouped<32, 1, 4, 2, 3, 1>;
-using A8w4Grouped64 = A8w4Grouped<64, 1, 4, 2, 2, 1>;
-using A8w4Grouped128 = A8w4Grouped<128, 2, 3, 1, 2, 1>;
+using A8w4Grouped16 = A8w4Grouped<16, 1, 6, 2, 3>;
+using A8w4Grouped32 = A8w4Grouped<32, 2, 5, 2, 3>;
+using A8w4Grouped64 = A8w4Grouped<64, 2, 4, 2, 2>;
+using A8w4Grouped128 = A8w4Grouped<128, 2, 3, 1, 2>;
 
 // The register moves between warpgroups need exactly the launch count they were sized for.
 template <typename V>
@@ -78,8 +77,7 @@ bool a8w4_grouped_wide(uint32_t T, uint32_t E) {
 
 template <typename V>
 cudaError_t launch_a8w4_grouped(const GQ::GroupedParams& p, uint64_t tiles, uint32_t sms, cudaStream_t stream) {
-  const uint32_t slots = sms * V::kPerSm;
-  const uint32_t grid = tiles < slots ? static_cast<uint32_t>(tiles) : slots;
+  const uint32_t grid = tiles < sms ? static_cast<uint32_t>(tiles) : sms;
   return launch_ex(V::kKernel, p, grid, V::Cfg::kThreads, V::kSmem, 1, stream);
 }
 

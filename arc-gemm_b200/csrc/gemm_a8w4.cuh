@@ -106,30 +106,39 @@ struct GroupedParams : Params {
   uint32_t zero_others;  // zero the output rows of no group
 };
 
-// UWG: unpack warpgroups (on alternate steps), UNP: unpacked stages, OCC: CTAs per SM.
-template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG = 1, uint32_t UNP = kUnpacked, uint32_t OCC = 1>
+// UWG: unpack warpgroups (on alternate steps), UNP: unpacked stages.
+template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG = 1, uint32_t UNP = kUnpacked>
 struct Cfg {
   static_assert(BT == 16 || BT == 32 || BT == 64 || BT == 128, "token tile");
   static_assert(EWG == 1 || EWG == 2, "epilogue warpgroups");
   static_assert(LS >= 2 && LS <= kDoneRing && UNP <= kDoneRing && kAccPairs < kDoneRing,
                 "each waiter must stay within one phase of its completion barrier");
-  static_assert(UWG == 1 || (UWG == 2 && EWG == 1), "unpack warpgroups");
-  static_assert(OCC == 1 || (OCC == 2 && UWG == 1 && EWG == 1), "CTAs per SM");
+  static_assert(UWG == 1 || (UWG + EWG <= 4 && UNP >= UWG), "unpack warpgroups");
   static constexpr uint32_t kEpiWarp = 4 + 4 * UWG;  // first epilogue warp
   static constexpr uint32_t kThreads = 128 + 128 * UWG + 128 * EWG;
   static constexpr uint32_t kCols = BT / EWG;               // columns per epilogue thread
   static constexpr uint32_t kChunk = kCols < 32 ? kCols : 32;  // TMEM columns per load
-  static constexpr uint32_t kTmemCols = kAccPairs * kGps * BT;  // 64 to 512
+  // Few columns leave TMEM for more steps in flight: with two, a step's products wait for the
+  // epilogue of the step before last.
+  static constexpr uint32_t kAcc = UWG > 1 && BT <= 32 ? 4 : kAccPairs;
+  // A small UMMA costs its issuing thread about 61 cycles and the pipe 73, or 95 in a chain on one
+  // accumulator: at eight per step that, and not the weight stream, would set the pace. Two
+  // issuers take alternate steps, and a step's two groups are issued in turn.
+  static constexpr uint32_t kIssuers = UWG > 1 ? 2 : 1;
+  // The epilogue of a small tile is a chain of waits (for the barrier, TMEM loads, TMEM stores)
+  // around little work, so it takes two steps at a time; larger tiles group by group.
+  static constexpr uint32_t kAtOnce = UWG > 1 && kCols <= 16 ? 2 : 1;
+  static constexpr uint32_t kTmemCols = kAcc * kGps * BT;  // 64 to 512
   static constexpr uint32_t kTokBytes = BT * kGroupK;       // one group's token box
   static constexpr uint32_t kWpBytes = kRows * kPackedRow * kGps;
   static constexpr uint32_t kWBytes = kRows * kGroupK;      // one group's unpacked tile
   // Register budget: the producer/UMMA and unpack warpgroups drop to kRegsLow and
   // the epilogue warpgroup(s) rise to kRegsHigh, out of kLaunchRegs per thread at
   // launch (the most 1 CTA/SM allows; the host checks the compiled count).
-  static constexpr uint32_t kLaunchRegs = OCC == 2 ? 80 : EWG + UWG == 3 ? 128 : 168;
+  static constexpr uint32_t kLaunchRegs = EWG + UWG == 4 ? 96 : EWG + UWG == 3 ? 128 : 168;
   static constexpr bool kSplitRegs = true;
-  static constexpr uint32_t kRegsLow = OCC == 2 ? 72 : EWG == 2 ? 80 : UWG == 2 ? 96 : 112;
-  static constexpr uint32_t kRegsHigh = OCC == 2 ? 96 : EWG == 2 ? 176 : UWG == 2 ? 224 : 232;
+  static constexpr uint32_t kRegsLow = EWG == 2 || UWG == 3 ? 80 : UWG == 2 ? 96 : 112;
+  static constexpr uint32_t kRegsHigh = UWG == 3 ? 160 : EWG == 2 ? (UWG == 2 ? 120 : 176) : UWG == 2 ? 224 : 232;
   static_assert((128 + 128 * UWG) * kRegsLow + 128 * EWG * kRegsHigh <= kThreads * kLaunchRegs,
                 "register shares exceed the launch budget");
   static_assert(kCols % kChunk == 0, "epilogue column split");
@@ -144,7 +153,7 @@ struct alignas(1024) Smem {
   uint64_t load_full[LS];                       // TMA bytes landed (tokens + packed W)
   uint64_t w_full[UNP];                         // 4 unpack warps wrote w[u]
   uint64_t mma_done[kDoneRing];                 // the UMMAs of step si retired
-  uint64_t tmem_empty[kAccPairs];               // epilogue read accumulator pair a
+  uint64_t tmem_empty[C::kAcc];                 // epilogue read accumulator pair a
   uint32_t tmem_base;
   uint32_t abort;
 };
@@ -249,10 +258,10 @@ __device__ __forceinline__ void expand_piece(const uint4& x, uint32_t split, uin
 // Kernel
 // ---------------------------------------------------------------------------------
 // P: Params (one weight matrix) or GroupedParams (row groups, each with its own).
-template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG, uint32_t UNP, uint32_t OCC, typename P>
+template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG, uint32_t UNP, typename P>
 __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
   constexpr bool kGrouped = std::is_same<P, GroupedParams>::value;
-  using C = Cfg<BT, EWG, LS, UWG, UNP, OCC>;
+  using C = Cfg<BT, EWG, LS, UWG, UNP>;
   using S_t =
       typename std::conditional<kGrouped, GroupedSmem<BT, EWG, LS, UWG, UNP>, Smem<BT, EWG, LS, UWG, UNP>>::type;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -274,7 +283,7 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
     for (uint32_t i = 0; i < LS; ++i) mbar_init(&s.load_full[i], 1);
     for (uint32_t i = 0; i < UNP; ++i) mbar_init(&s.w_full[i], 4);  // one per unpack warp
     for (uint32_t i = 0; i < kDoneRing; ++i) mbar_init(&s.mma_done[i], 1);  // UMMA commit
-    for (uint32_t i = 0; i < kAccPairs; ++i) mbar_init(&s.tmem_empty[i], 4 * EWG);
+    for (uint32_t i = 0; i < C::kAcc; ++i) mbar_init(&s.tmem_empty[i], 4 * EWG);
     s.abort = 0;
     fence_barrier_init();
   }
@@ -291,7 +300,7 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
     const uint32_t ew = warp - C::kEpiWarp;
     const uint32_t row = tmem_base + (((ew & 3u) * 32u) << 16) + (ew >> 2) * C::kCols;
 #pragma unroll
-    for (uint32_t b = 0; b < kAccPairs * kGps; ++b) {
+    for (uint32_t b = 0; b < C::kAcc * kGps; ++b) {
 #pragma unroll
       for (uint32_t c = 0; c < C::kCols; c += 8) tmem_st_32x32b_x8_fill(row + b * BT + c, kBiasBits);
     }
@@ -360,47 +369,65 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
         mbar_drain(&s.load_full[i % LS], (i / LS) & 1u);
       }
     }
-  } else if (warp == 1) {
+  } else if (warp == 1 || (C::kIssuers == 2 && warp == 3)) {
     // ------------------------------------------------------------ UMMA issuer
     if constexpr (C::kSplitRegs) regs_release<C::kRegsLow>();
     if (lane == 0) {
       constexpr uint32_t idesc = idesc_s8_s32(kRows, BT);
       uint32_t stage = 0, phase = 0, us = 0, uphase = 0, si = 0, cursor = 0;
+      uint32_t issued = 0;  // steps up to this thread's last one
       Work w;
       bool ok = true;
       while (ok && next(cursor, w)) {
         for (uint32_t t = 0; t < steps_per_tile; ++t, ++si) {
-          const uint32_t pair = si % kAccPairs;
-          const uint32_t acc_parity = (si / kAccPairs - 1u) & 1u;
-          // Test all three first (their latencies overlap), block only on the others.
-          const uint32_t t_acc = si >= kAccPairs ? mbar_test(&s.tmem_empty[pair], acc_parity) : 1u;
-          const uint32_t t_w = mbar_test(&s.w_full[us], uphase);
-          const uint32_t t_ld = mbar_test(&s.load_full[stage], phase);
-          if ((t_acc == 0u && !mbar_wait(&s.tmem_empty[pair], acc_parity, abort, kStatusTimeoutMma)) ||
-              (t_w == 0u && !mbar_wait(&s.w_full[us], uphase, abort, kStatusTimeoutMma)) ||
-              (t_ld == 0u && !mbar_wait(&s.load_full[stage], phase, abort, kStatusTimeoutMma))) {
-            ok = false;
-            break;
-          }
-          if (si - 4u < 8u) probe_mark(si - 4u);
-          tc_fence_after_sync();
-          // A group past K (odd group count) is skipped: its accumulator keeps the bias
-          // for the next tile, and the epilogue skips it too.
-          const uint32_t real = min(kGps, w.g_end - (w.g_begin + t * kGps));
-#pragma unroll
-          for (uint32_t h = 0; h < kGps; ++h) {
-            if (h >= real) break;
-            const uint64_t adesc = make_sw128_kmajor_desc(s.w[us][h]);
-            const uint64_t bdesc = make_sw128_kmajor_desc(s.tok[stage][h]);
-            const uint32_t d_tmem = tmem_base + (pair * kGps + h) * BT;
-            // Every UMMA accumulates: the group starts from the bias the epilogue left.
-#pragma unroll
-            for (uint32_t k = 0; k < kGroupK / kUmmaK; ++k) {
-              umma_s8(d_tmem, desc_advance(adesc, k * kUmmaK), desc_advance(bdesc, k * kUmmaK),
-                      idesc, 1u);
+          if (C::kIssuers == 1 || (si & 1u) == warp / 2u) {  // alternate steps
+            const uint32_t pair = si % C::kAcc;
+            const uint32_t acc_parity = (si / C::kAcc - 1u) & 1u;
+            // Test all three first (their latencies overlap), block only on the others.
+            const uint32_t t_acc = si >= C::kAcc ? mbar_test(&s.tmem_empty[pair], acc_parity) : 1u;
+            const uint32_t t_w = mbar_test(&s.w_full[us], uphase);
+            const uint32_t t_ld = mbar_test(&s.load_full[stage], phase);
+            if ((t_acc == 0u && !mbar_wait(&s.tmem_empty[pair], acc_parity, abort, kStatusTimeoutMma)) ||
+                (t_w == 0u && !mbar_wait(&s.w_full[us], uphase, abort, kStatusTimeoutMma)) ||
+                (t_ld == 0u && !mbar_wait(&s.load_full[stage], phase, abort, kStatusTimeoutMma))) {
+              ok = false;
+              break;
             }
+            if (si - 4u < 8u) probe_mark(si - 4u);
+            tc_fence_after_sync();
+            // A group past K (odd group count) is skipped: its accumulator keeps the bias
+            // for the next tile, and the epilogue skips it too.
+            const uint32_t real = min(kGps, w.g_end - (w.g_begin + t * kGps));
+            if constexpr (C::kIssuers == 2) {
+#pragma unroll
+              for (uint32_t k = 0; k < kGroupK / kUmmaK; ++k) {
+#pragma unroll
+                for (uint32_t h = 0; h < kGps; ++h) {
+                  if (h < real) {
+                    umma_s8(tmem_base + (pair * kGps + h) * BT,
+                            desc_advance(make_sw128_kmajor_desc(s.w[us][h]), k * kUmmaK),
+                            desc_advance(make_sw128_kmajor_desc(s.tok[stage][h]), k * kUmmaK), idesc, 1u);
+                  }
+                }
+              }
+            } else {
+#pragma unroll
+              for (uint32_t h = 0; h < kGps; ++h) {
+                if (h >= real) break;
+                const uint64_t adesc = make_sw128_kmajor_desc(s.w[us][h]);
+                const uint64_t bdesc = make_sw128_kmajor_desc(s.tok[stage][h]);
+                const uint32_t d_tmem = tmem_base + (pair * kGps + h) * BT;
+                // Every UMMA accumulates: the group starts from the bias the epilogue left.
+#pragma unroll
+                for (uint32_t k = 0; k < kGroupK / kUmmaK; ++k) {
+                  umma_s8(d_tmem, desc_advance(adesc, k * kUmmaK), desc_advance(bdesc, k * kUmmaK),
+                          idesc, 1u);
+                }
+              }
+            }
+            umma_commit(&s.mma_done[si % kDoneRing]);
+            issued = si + 1u;
           }
-          umma_commit(&s.mma_done[si % kDoneRing]);
           if (++stage == LS) {
             stage = 0;
             phase ^= 1u;
@@ -412,7 +439,7 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
         }
       }
       // The last commit covers every UMMA this thread issued.
-      if (si > 0u) mbar_drain(&s.mma_done[(si - 1u) % kDoneRing], done_parity(si - 1u));
+      if (issued > 0u) mbar_drain(&s.mma_done[(issued - 1u) % kDoneRing], done_parity(issued - 1u));
     }
   } else if (warp >= 4 && warp < C::kEpiWarp) {
     // ------------------------------------------------------------ unpack warpgroup
@@ -491,7 +518,8 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
     const bool vec_sb = (p.G % 8u == 0u) && (p.ldsb % 8u == 0u) &&
                         ((reinterpret_cast<uintptr_t>(p.sb) & 15u) == 0u);
     uint32_t si = 0, cursor = 0;
-    uint32_t pre = 0;  // step si's partials seen complete by an early test
+    uint32_t pre = 0, pre2 = 0;  // step si's (si + 1's) partials seen complete by an early test
+    (void)pre2;
     Work w;
     bool ok = true;
     while (ok && next(cursor, w)) {
@@ -517,86 +545,153 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
           s_next = bf16_bits_to_float(__ldg(sb_row + w.g_begin));
         }
       }
-      for (uint32_t t = 0; t < steps_per_tile; ++t, ++si) {
-        const uint32_t pair = si % kAccPairs;
-        if (!mbar_wait_all2(&s.mma_done[si % kDoneRing], done_parity(si), pre,
-                             &s.mma_done[si % kDoneRing], done_parity(si), 1u, abort,
-                             kStatusTimeoutEpilogue)) {
-          ok = false;
-          break;
+      // The scale of group g (called once per group, in order).
+      const auto next_scale = [&](uint32_t g) {
+        float s_g;
+        if (vec_sb) {
+          s_g = __uint_as_float(win0.x << 16) * 0.0625f;  // 1/16: high-nibble placement
+          win0.x = __funnelshift_r(win0.x, win0.y, 16);
+          win0.y = __funnelshift_r(win0.y, win0.z, 16);
+          win0.z = __funnelshift_r(win0.z, win0.w, 16);
+          win0.w >>= 16;
+          if (((g - w.g_begin) & 7u) == 7u) {
+            win0 = win1;
+            if (n_valid && g + 9u < w.g_end) {
+              win1 = __ldg(reinterpret_cast<const uint4*>(sb_row + g + 9u));
+            }
+          }
+        } else {
+          s_g = s_next * 0.0625f;
+          if (n_valid && g + 1 < w.g_end) s_next = bf16_bits_to_float(__ldg(sb_row + g + 1));
         }
-        if (et == 0 && si - 4u < 8u) probe_mark(8 + si - 4u);
-        tc_fence_after_sync();
+        return s_g;
+      };
+      if constexpr (C::kAtOnce == 2) {
+        for (uint32_t t = 0; t < steps_per_tile && ok; t += C::kAtOnce) {
+          const uint32_t num = min(C::kAtOnce, steps_per_tile - t);
+          ok = mbar_wait_all2(&s.mma_done[si % kDoneRing], done_parity(si), pre, &s.mma_done[(si + 1u) % kDoneRing],
+                              done_parity(si + 1u), num < 2u ? 1u : pre2, abort, kStatusTimeoutEpilogue);
+          if (!ok) break;
+          if (et == 0 && si - 4u < 8u) probe_mark(8 + si - 4u);
+          tc_fence_after_sync();
+          // A group past K (odd group count) reads and keeps the bias, which nobody uses.
+          uint32_t r[C::kAtOnce][kGps][C::kCols];
 #pragma unroll
-        for (uint32_t h = 0; h < kGps; ++h) {
-          const uint32_t g = w.g_begin + t * kGps + h;
-          if (g >= w.g_end) break;  // past K: uniform across the CTA
-          float s_g;
-          if (vec_sb) {
-            s_g = __uint_as_float(win0.x << 16) * 0.0625f;  // 1/16: high-nibble placement
-            win0.x = __funnelshift_r(win0.x, win0.y, 16);
-            win0.y = __funnelshift_r(win0.y, win0.z, 16);
-            win0.z = __funnelshift_r(win0.z, win0.w, 16);
-            win0.w >>= 16;
-            if (((g - w.g_begin) & 7u) == 7u) {
-              win0 = win1;
-              if (n_valid && g + 9u < w.g_end) {
-                win1 = __ldg(reinterpret_cast<const uint4*>(sb_row + g + 9u));
-              }
-            }
-          } else {
-            s_g = s_next * 0.0625f;
-            if (n_valid && g + 1 < w.g_end) s_next = bf16_bits_to_float(__ldg(sb_row + g + 1));
-          }
-          const uint64_t s2 = f32x2_pack(s_g, s_g);
-          const uint32_t t_row = tmem_base + ((q * 32u) << 16) + (pair * kGps + h) * BT + col0;
-          // All of this thread's columns of the group in one wait; the bias re-arm is
-          // issued right away and overlaps the arithmetic.
-          uint32_t r[C::kCols];
+          for (uint32_t b = 0; b < C::kAtOnce; ++b) {
+            const uint32_t t_row = tmem_base + ((q * 32u) << 16) + (si + b) % C::kAcc * kGps * BT + col0;
 #pragma unroll
-          for (uint32_t c0 = 0; c0 < C::kCols; c0 += C::kChunk) {
-            if constexpr (C::kChunk == 16) {
-              tmem_ld_32x32b_x16(t_row + c0, *reinterpret_cast<uint32_t(*)[16]>(r + c0));
-            } else {
-              tmem_ld_32x32b_x32(t_row + c0, *reinterpret_cast<uint32_t(*)[32]>(r + c0));
+            for (uint32_t h = 0; h < kGps; ++h) {
+              if (b < num) tmem_ld_32x32b_x16(t_row + h * BT, *reinterpret_cast<uint32_t(*)[16]>(r[b][h]));
             }
           }
-          // Ask early whether the next step's partials are ready; the answer arrives
-          // while the loads are in flight.
-          if (h == 0) pre = mbar_test(&s.mma_done[(si + 1u) % kDoneRing], done_parity(si + 1u));
+          // Ask early whether the next steps' partials are ready.
+          pre = mbar_test(&s.mma_done[(si + num) % kDoneRing], done_parity(si + num));
+          pre2 = mbar_test(&s.mma_done[(si + num + 1u) % kDoneRing], done_parity(si + num + 1u));
           tmem_ld_wait();
 #pragma unroll
-          for (uint32_t c = 0; c < C::kCols; c += 8) tmem_st_32x32b_x8_fill(t_row + c, kBiasBits);
+          for (uint32_t b = 0; b < C::kAtOnce; ++b) {
+            const uint32_t t_row = tmem_base + ((q * 32u) << 16) + (si + b) % C::kAcc * kGps * BT + col0;
 #pragma unroll
-          for (uint32_t j = 0; j < C::kCols; j += 2) {
-            acc[j / 2] = f32x2_fma(f32x2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), s2,
-                                   acc[j / 2]);
+            for (uint32_t c = 0; c < kGps * C::kCols; c += 8) {
+              if (b < num) tmem_st_32x32b_x8_fill(t_row + c / C::kCols * BT + c % C::kCols, kBiasBits);
+            }
           }
-          if (p.partials != nullptr && n_valid) {
 #pragma unroll
-            for (uint32_t j = 0; j < C::kCols; ++j) {
-              const uint32_t m = w.m0 + col0 + j;
-              if (m < w.m_end) {
-                p.partials[(size_t(m) * p.N + n) * p.G + g] =
-                    static_cast<int32_t>(r[j] - kBiasBits) >> 4;
+          for (uint32_t b = 0; b < C::kAtOnce; ++b) {
+#pragma unroll
+            for (uint32_t h = 0; h < kGps; ++h) {
+              const uint32_t g = w.g_begin + (t + b) * kGps + h;
+              if (b < num && g < w.g_end) {
+                const float s_g = next_scale(g);
+                const uint64_t s2 = f32x2_pack(s_g, s_g);
+#pragma unroll
+                for (uint32_t j = 0; j < C::kCols; j += 2) {
+                  acc[j / 2] = f32x2_fma(
+                      f32x2_pack(__uint_as_float(r[b][h][j]), __uint_as_float(r[b][h][j + 1])), s2, acc[j / 2]);
+                }
+                bias_sum += s_g * kBiasF;  // exact: 8 significant bits times 2
               }
             }
           }
-          bias_sum += s_g * kBiasF;  // exact: 8 significant bits times 2
-        }
-        // Both accumulators of the pair are read and re-armed: hand them back.
-        tmem_st_wait();
-        tc_fence_before_sync();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.tmem_empty[pair]);
-        if (et == 0 && si - 4u < 8u) probe_mark(16 + si - 4u);
-        if ((t * kGps) % kBiasFlush == kBiasFlush - kGps || t + 1 == steps_per_tile) {
+          // The accumulators are read and re-armed: hand them back.
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane < num) mbar_arrive(&s.tmem_empty[(si + lane) % C::kAcc]);
+          if (et == 0 && si - 4u < 8u) probe_mark(16 + si - 4u);
+          static_assert(C::kAtOnce == 1 || kBiasFlush == 2 * kGps, "flush every two steps");
           const uint64_t nb = f32x2_pack(-bias_sum, -bias_sum);
 #pragma unroll
           for (uint32_t j = 0; j < kPairs; ++j) acc[j] = f32x2_add(acc[j], nb);
           bias_sum = 0.f;
+          si += num;
         }
-        if (et == 0 && si - 4u < 8u) probe_mark(48 + si - 4u);
+      } else {
+        for (uint32_t t = 0; t < steps_per_tile; ++t, ++si) {
+          const uint32_t pair = si % C::kAcc;
+          if (!mbar_wait_all2(&s.mma_done[si % kDoneRing], done_parity(si), pre,
+                               &s.mma_done[si % kDoneRing], done_parity(si), 1u, abort,
+                               kStatusTimeoutEpilogue)) {
+            ok = false;
+            break;
+          }
+          if (et == 0 && si - 4u < 8u) probe_mark(8 + si - 4u);
+          tc_fence_after_sync();
+#pragma unroll
+          for (uint32_t h = 0; h < kGps; ++h) {
+            const uint32_t g = w.g_begin + t * kGps + h;
+            if (g >= w.g_end) break;  // past K: uniform across the CTA
+            const float s_g = next_scale(g);
+            const uint64_t s2 = f32x2_pack(s_g, s_g);
+            const uint32_t t_row = tmem_base + ((q * 32u) << 16) + (pair * kGps + h) * BT + col0;
+            // All of this thread's columns of the group in one wait; the bias re-arm is
+            // issued right away and overlaps the arithmetic.
+            uint32_t r[C::kCols];
+#pragma unroll
+            for (uint32_t c0 = 0; c0 < C::kCols; c0 += C::kChunk) {
+              if constexpr (C::kChunk == 16) {
+                tmem_ld_32x32b_x16(t_row + c0, *reinterpret_cast<uint32_t(*)[16]>(r + c0));
+              } else {
+                tmem_ld_32x32b_x32(t_row + c0, *reinterpret_cast<uint32_t(*)[32]>(r + c0));
+              }
+            }
+            // Ask early whether the next step's partials are ready; the answer arrives
+            // while the loads are in flight.
+            if (h == 0) pre = mbar_test(&s.mma_done[(si + 1u) % kDoneRing], done_parity(si + 1u));
+            tmem_ld_wait();
+#pragma unroll
+            for (uint32_t c = 0; c < C::kCols; c += 8) tmem_st_32x32b_x8_fill(t_row + c, kBiasBits);
+#pragma unroll
+            for (uint32_t j = 0; j < C::kCols; j += 2) {
+              acc[j / 2] = f32x2_fma(f32x2_pack(__uint_as_float(r[j]), __uint_as_float(r[j + 1])), s2,
+                                     acc[j / 2]);
+            }
+            if (p.partials != nullptr && n_valid) {
+#pragma unroll
+              for (uint32_t j = 0; j < C::kCols; ++j) {
+                const uint32_t m = w.m0 + col0 + j;
+                if (m < w.m_end) {
+                  p.partials[(size_t(m) * p.N + n) * p.G + g] =
+                      static_cast<int32_t>(r[j] - kBiasBits) >> 4;
+                }
+              }
+            }
+            bias_sum += s_g * kBiasF;  // exact: 8 significant bits times 2
+          }
+          // Both accumulators of the pair are read and re-armed: hand them back.
+          tmem_st_wait();
+          tc_fence_before_sync();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(&s.tmem_empty[pair]);
+          if (et == 0 && si - 4u < 8u) probe_mark(16 + si - 4u);
+          if ((t * kGps) % kBiasFlush == kBiasFlush - kGps || t + 1 == steps_per_tile) {
+            const uint64_t nb = f32x2_pack(-bias_sum, -bias_sum);
+#pragma unroll
+            for (uint32_t j = 0; j < kPairs; ++j) acc[j] = f32x2_add(acc[j], nb);
+            bias_sum = 0.f;
+          }
+          if (et == 0 && si - 4u < 8u) probe_mark(48 + si - 4u);
+        }
       }
       if (!ok) break;
 
@@ -636,13 +731,13 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
 template <uint32_t BT, uint32_t EWG, uint32_t LS>
 __global__ void __launch_bounds__(Cfg<BT, EWG, LS>::kThreads, 1)
     gemm_a8w4_kernel(const __grid_constant__ Params p) {
-  gemm_a8w4_body<BT, EWG, LS, 1, kUnpacked, 1>(p);
+  gemm_a8w4_body<BT, EWG, LS, 1, kUnpacked>(p);
 }
 
-template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG, uint32_t UNP, uint32_t OCC>
-__global__ void __launch_bounds__(Cfg<BT, EWG, LS, UWG, UNP, OCC>::kThreads, OCC)
+template <uint32_t BT, uint32_t EWG, uint32_t LS, uint32_t UWG, uint32_t UNP>
+__global__ void __launch_bounds__(Cfg<BT, EWG, LS, UWG, UNP>::kThreads, 1)
     gemm_a8w4_grouped_kernel(const __grid_constant__ GroupedParams p) {
-  gemm_a8w4_body<BT, EWG, LS, UWG, UNP, OCC>(p);
+  gemm_a8w4_body<BT, EWG, LS, UWG, UNP>(p);
 }
 
 }  // namespace a8w4

@@ -5,7 +5,6 @@ import pytest
 import torch
 
 import arc
-from arc import _lib
 from arc._lib import STATUS_BAD_OFFSETS
 from linear_bounds import H, SUM, assert_within, normal
 
@@ -163,9 +162,7 @@ def _a8w4(sizes, behind, n, k, seed=0):
 def a8w4_kernel(request, monkeypatch):
     """Both kernels on every size: int32 partial sums, or scales in the fp16 operand."""
     monkeypatch.setenv("ARC_A8W4_GROUPED", request.param)
-    _lib.workspace_bytes.cache_clear()
-    yield request.param
-    _lib.workspace_bytes.cache_clear()
+    return request.param
 
 
 def _check_a8w4(kernel, a, b, sizes, offsets, prepacked=False):

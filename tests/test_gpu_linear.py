@@ -217,6 +217,33 @@ def test_two_streams_at_once(cuda_device):
         assert torch.equal(t, want[i % 2])
 
 
+def test_second_derivatives_are_refused(cuda_device):
+    x, w, b, _ = _inputs(4, 24, 16, residual=False)
+    lx, lw, lb = _leaves(x, w, b)
+    dy = torch.ones(4, 24, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    (dx,) = torch.autograd.grad(arc.linear(lx, lw, lb, activation="gelu"), [lx], dy, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        dx.sum().backward()
+
+
+def test_unused_gradients_and_no_grad(cuda_device):
+    x, w, b, r = _inputs(4, 24, 16)
+    lx, lw = _leaves(x, w)
+    with torch.no_grad():
+        assert not arc.linear(lx, lw, b, r).requires_grad
+    out = torch.empty_like(r)
+    with torch.no_grad():
+        arc.linear(lx, lw, b, r, out=out)
+    lr = r.clone().requires_grad_()
+    arc.linear(x, w, b, lr).backward(r)  # only the residual's
+    assert torch.equal(lr.grad, r)
+    # twice through the same leaves accumulates
+    arc.linear(lx, lw, b).backward(r)
+    first = lw.grad.clone()
+    arc.linear(lx, lw, b).backward(r)
+    assert torch.equal(lw.grad, first + first)
+
+
 def test_refusals(cuda_device):
     x, w, b, r = _inputs(4, 24, 16)
     with pytest.raises(ValueError, match="activation"):

@@ -111,7 +111,16 @@ def test_group_rows_checks(native_lib, p):
     assert call(slots=1 << 20) == BAD  # no workspace
 
 
-def test_python_refuses_cpu_tensors():
+@pytest.fixture(scope="session")
+def torch_ops(native_lib):
+    """The built PyTorch operators (built here if missing; the build is CPU-only)."""
+    from arc import build
+
+    build.build_torch_ops()
+    return _lib.torch_ops()
+
+
+def test_python_refuses_cpu_tensors(torch_ops):
     x, w = torch.zeros(2, 8, dtype=torch.bfloat16), torch.zeros(3, 8, dtype=torch.bfloat16)
     off = torch.zeros(3, dtype=torch.int32)
     with pytest.raises(ValueError, match="CUDA"):
