@@ -19,7 +19,7 @@ struct A8w4Grouped {
   static constexpr auto kKernel = GQ::gemm_a8w4_grouped_kernel<BT, EWG, LSN, UWG, UNP>;
 };
 using A8w4Grouped16 = A8w4Grouped<16, 1, 6, 2, 3>;
-using A8w4Grouped32 = A8w4Grouped<32, 2, 5, 2, 3>;
+using A8w4Grouped32 = A8w4Grouped<32, 2, 4, 2, 3>;
 using A8w4Grouped64 = A8w4Grouped<64, 2, 4, 2, 2>;
 using A8w4Grouped128 = A8w4Grouped<128, 2, 3, 1, 2>;
 

@@ -114,6 +114,10 @@ struct Cfg {
   static_assert(LS >= 2 && LS <= kDoneRing && UNP <= kDoneRing && kAccPairs < kDoneRing,
                 "each waiter must stay within one phase of its completion barrier");
   static_assert(UWG == 1 || (UWG + EWG <= 4 && UNP >= UWG), "unpack warpgroups");
+  // A parity wait tells a barrier's phase only from the one before, so whoever takes every n-th
+  // step must meet the same ring slots each time round (the unpacked ring, which may be odd, is
+  // waited for through the completions of the steps: see the issuer).
+  static_assert(LS % UWG == 0 && kDoneRing % UWG == 0, "rings and unpack warpgroups");
   static constexpr uint32_t kEpiWarp = 4 + 4 * UWG;  // first epilogue warp
   static constexpr uint32_t kThreads = 128 + 128 * UWG + 128 * EWG;
   static constexpr uint32_t kCols = BT / EWG;               // columns per epilogue thread
@@ -125,6 +129,7 @@ struct Cfg {
   // accumulator: at eight per step that, and not the weight stream, would set the pace. Two
   // issuers take alternate steps, and a step's two groups are issued in turn.
   static constexpr uint32_t kIssuers = UWG > 1 ? 2 : 1;
+  static_assert(LS % kIssuers == 0 && kDoneRing % kIssuers == 0 && kAcc % kIssuers == 0, "rings and issuers");
   // The epilogue of a small tile is a chain of waits (for the barrier, TMEM loads, TMEM stores)
   // around little work, so it takes two steps at a time; larger tiles group by group.
   static constexpr uint32_t kAtOnce = UWG > 1 && kCols <= 16 ? 2 : 1;
@@ -383,6 +388,13 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
           if (C::kIssuers == 1 || (si & 1u) == warp / 2u) {  // alternate steps
             const uint32_t pair = si % C::kAcc;
             const uint32_t acc_parity = (si / C::kAcc - 1u) & 1u;
+            // With an odd ring this issuer has not seen the slot's last use (the other one has):
+            // once that step's products are done, w_full's parity is this step's.
+            if (UNP % C::kIssuers != 0u && si >= UNP &&
+                !mbar_wait(&s.mma_done[(si - UNP) % kDoneRing], done_parity(si - UNP), abort, kStatusTimeoutMma)) {
+              ok = false;
+              break;
+            }
             // Test all three first (their latencies overlap), block only on the others.
             const uint32_t t_acc = si >= C::kAcc ? mbar_test(&s.tmem_empty[pair], acc_parity) : 1u;
             const uint32_t t_w = mbar_test(&s.w_full[us], uphase);

@@ -195,6 +195,7 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_add
 template <bool W_MN, bool W4>
 __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(const __grid_constant__ Params p) {
   static_assert(!(W_MN && W4), "codes are K-major");
+  static_assert(kStages % kExpandSets == 0, "a set returns to the same operand slots");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem<W4>& s = *reinterpret_cast<Smem<W4>*>(smem_raw + smem_align_pad(smem_raw));
   const uint32_t warp = warp_idx_sync();
@@ -464,7 +465,10 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
       const uint16_t* sb_row[2];
       float up[2];
       uint32_t next[2];
-      uint32_t kb = (set - c0) % kExpandSets;
+      // The set's first stage of this tile. A set must take every kExpandSets-th stage of the whole
+      // walk (and so the same operand slots each time round): a parity wait tells a barrier's
+      // phase only from the one before, which its waiter must have seen.
+      uint32_t kb = (set + kExpandSets - c0 % kExpandSets) % kExpandSets;
 #pragma unroll
       for (uint32_t i = 0; i < 2; ++i) {
         const uint32_t f = w.f0 + rank * kRowsPerCta + row + 64u * i;
@@ -486,6 +490,8 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
         const uint8_t* src = s.codes[slot] + row * (kScaleGroup / 2) + (c & 1u) * 32u + low * 16u;
         const uint4 x[2] = {*reinterpret_cast<const uint4*>(src),
                             *reinterpret_cast<const uint4*>(src + 64u * (kScaleGroup / 2))};
+        // The slot's next codes arrive by TMA: order this warp's reads before the release.
+        fence_proxy_async_smem();
         __syncwarp();
         if (lane == 0) mbar_arrive(&s.codes_empty[slot]);
         // The products that read this operand slot last have retired.

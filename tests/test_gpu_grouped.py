@@ -229,6 +229,61 @@ def test_a8w4_kernels_are_chosen_by_rows(cuda_device):
         _check_a8w4("wide" if sum(sizes) > 128 * len(sizes) else "narrow", a, b, sizes, offsets)
 
 
+def _a8w4_on_gpu(a, b, offsets):
+    """The product in fp64 on the GPU, group by group, and the magnitude of its terms."""
+    (x, sa), (wp, sb) = a, b
+    ends = offsets.tolist()
+    want = torch.zeros(x.shape[0], wp.shape[1], dtype=torch.float64, device="cuda")
+    mag = torch.zeros_like(want)
+    for i, (r0, r1) in enumerate(zip(ends, ends[1:])):
+        codes = torch.stack((wp[i] & 15, wp[i] >> 4), -1).flatten(-2).to(torch.int16)
+        w = torch.where(codes >= 8, codes - 16, codes).double() * sb[i].double().repeat_interleave(128, 1)
+        xe = x[r0:r1].double() * sa[r0:r1].double()[:, None]
+        want[r0:r1], mag[r0:r1] = xe @ w.T, xe.abs() @ w.abs().T
+    return want, mag
+
+
+@pytest.mark.parametrize("sizes,n,k", [([763, 578, 517, 684, 346, 455, 153, 597], 4096, 1024),
+                                       ([300] * 24, 2056, 640), ([900, 100], 14336, 128), ([257] * 16, 1024, 2048),
+                                       ([2] * 32, 4096, 1152), ([20] * 32, 4096, 1152), ([40] * 32, 4096, 1152),
+                                       ([80, 1, 0, 128] * 8, 2048, 1152), ([1] * 512, 512, 256)])
+def test_a8w4_many_tiles_per_block(cuda_device, a8w4_kernel, sizes, n, k):
+    """Every block walks several tiles: the pipelines run on from tile to tile. The result is the
+    same each time, bit for bit, and right."""
+    g = torch.Generator(device="cuda").manual_seed(k)
+    t, e = sum(sizes), len(sizes)
+    a = (torch.randint(-127, 128, (t, k), generator=g, device="cuda").to(torch.int8),
+         torch.rand(t, generator=g, device="cuda") + 0.5)
+    b = (torch.randint(0, 256, (e, n, k // 2), generator=g, device="cuda").to(torch.uint8),
+         (torch.rand(e, n, k // 128, generator=g, device="cuda") + 0.1).to(torch.bfloat16))
+    offsets = _offsets(sizes)
+    first = arc.a8w4_grouped_matmul(a, b, offsets)
+    want, mag = _a8w4_on_gpu(a, b, offsets)
+    err = (k + 8) * SUM * mag  # covers both kernels' sums
+    assert_within(first, want, err + H * (want.abs() + err), "first")
+    for _ in range(12):
+        assert torch.equal(arc.a8w4_grouped_matmul(a, b, offsets), first)
+    assert arc.device_status(0) == 0
+
+
+@pytest.mark.parametrize("sizes,n,k", [([763, 578, 517, 684, 0, 455, 153, 597], 2048, 1024), ([300] * 24, 1032, 520),
+                                       ([17, 3, 9, 30] * 16, 2048, 1024)])
+def test_grouped_many_tiles_per_block(cuda_device, sizes, n, k):
+    x, w, dy, offsets = _inputs(sizes, 0, n, k)
+    want = _reference(x, w, dy, sizes)
+    first = None
+    for _ in range(8):
+        lx, lw = x.clone().requires_grad_(), w.clone().requires_grad_()
+        y = arc.grouped_matmul(lx, lw, offsets)
+        got = (y.detach(), *torch.autograd.grad(y, [lx, lw], dy))
+        if first is None:
+            first = got
+            for v, name in zip(got, ("y", "dx", "dw")):
+                assert_within(v, *want[name], name)
+        for a, b in zip(got, first):
+            assert torch.equal(a, b)
+
+
 def test_a8w4_one_group_is_a8w4_matmul(cuda_device):
     a, (wp, sb), offsets = _a8w4([100], 0, 256, 512)
     assert torch.equal(arc.a8w4_grouped_matmul(a, (wp, sb), offsets), arc.a8w4_matmul(a, (wp[0], sb[0])))
