@@ -40,12 +40,23 @@ uint32_t row_vec(const void* p, uint64_t ld, uint64_t group_stride = 0) {
   return (bits & 31u) == 0 ? 2u : (bits & 15u) == 0 ? 1u : 0u;
 }
 
+// Whether column pairs of a row-major bf16 matrix can be moved as 4-byte words.
+uint32_t column_pairs(const void* p, uint64_t ld, uint32_t cols) {
+  return cols % 2 == 0 && ld % 2 == 0 && (reinterpret_cast<uintptr_t>(p) & 3u) == 0 ? 1u : 0u;
+}
+
 // The kernel for a product of rows, in one group or several.
 //
-// Pairs (256 x 256 tiles) when the groups' rows fill half such a tile and there are tiles for
-// half of the pairs; else the streaming kernel, its row tile the smallest that holds an
-// average group's rows, with the contraction split over a cluster until the two block slots
-// of every SM have work (at least kStreamMinKb blocks of 64 each).
+// One group: pairs (256 x 256 tiles) when the rows fill half such a tile and there are tiles for
+// half of the pairs. Several groups: the pair kernel's row tile fits itself to the group, so it
+// takes all but the smallest groups (more than 16 rows on average; 64 groups, 2048 x 1024: at 32
+// rows 51 us against the streaming kernel's 70, at 128 57 against 116; 16 groups of 8 rows,
+// 4096 x 4096: 93 against 85).
+//
+// Else the streaming kernel: the row tile is the smallest that holds an average group's rows and
+// the contraction is split over a cluster until the two block slots of every SM have work (at
+// least kStreamMinKb blocks of 64 each). Where that leaves SMs without work (a short
+// contraction), smaller row tiles fill them (1796 x 111 x 448 with a residual: STREAM_FILL).
 //
 // ARC_LINEAR_PLAN="pair" | "BN:S" (tests and tuning) forces the choice where it is valid.
 struct LinearPlan {
@@ -60,7 +71,7 @@ int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t
   const uint32_t live = groups < rows ? groups : rows;  // groups that can have rows
   const uint32_t avg = ceil_div(rows, live);
   const uint64_t pair_tiles = uint64_t(ceil_div(avg, LP::kTile)) * live * ceil_div(cols, LP::kTile);
-  plan->pair = max_pairs > 0 && avg > 128 && pair_tiles * 2 > max_pairs;
+  plan->pair = max_pairs > 0 && avg > (groups == 1 ? 128u : 16u) && pair_tiles * 2 > max_pairs;
   plan->bn = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
   uint32_t forced = 0;
   if (const char* env = getenv("ARC_LINEAR_PLAN")) {
@@ -76,15 +87,18 @@ int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t
       return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_LINEAR_PLAN must be 'pair' or 'BN:S' (got '%s')", env);
     }
   }
-  // With groups the host knows only a bound: a group of c rows has at most c / bn + 1 tiles.
-  plan->row_tiles = groups == 1 ? ceil_div(rows, plan->bn) : live + rows / plan->bn;
-  const uint64_t tiles = uint64_t(plan->row_tiles) * ceil_div(cols, LS::kRows);
-  plan->splits = 1;
-  for (uint32_t s : {8u, 4u, 2u}) {
-    if (forced != 0 ? (s == forced && s <= num_kb) : (tiles * s <= 2 * sms && num_kb >= s * kStreamMinKb)) {
-      plan->splits = s;
-      break;
+  for (;; plan->bn /= 2) {
+    // With groups the host knows only a bound: a group of c rows has at most c / bn + 1 tiles.
+    plan->row_tiles = groups == 1 ? ceil_div(rows, plan->bn) : live + rows / plan->bn;
+    const uint64_t tiles = uint64_t(plan->row_tiles) * ceil_div(cols, LS::kRows);
+    plan->splits = 1;
+    for (uint32_t s : {8u, 4u, 2u}) {
+      if (forced != 0 ? (s == forced && s <= num_kb) : (tiles * s <= 2 * sms && num_kb >= s * kStreamMinKb)) {
+        plan->splits = s;
+        break;
+      }
     }
+    if (forced != 0 || plan->bn == 16 || tiles * plan->splits >= sms) break;
   }
   return ARC_OK;
 }
@@ -146,7 +160,7 @@ cudaError_t grouped_pair_launch(GP::Params& p, const arcb::lin::Groups& groups, 
   p.groups = groups;
   p.cols = cols;
   p.tiles_f = ceil_div(cols, GP::kTileF);
-  p.pair_store = cols % 2 == 0 && ldo % 2 == 0 && (reinterpret_cast<uintptr_t>(out) & 3u) == 0;
+  p.pair_store = column_pairs(out, ldo, cols);
   p.zero_others = zero_others ? 1u : 0u;
   // The host knows only a bound: a group of c rows has at most c / kTileT + 1 row tiles.
   const uint64_t tiles = uint64_t((groups.num < groups.rows ? groups.num : groups.rows) + groups.rows / GP::kTileT) *
@@ -202,6 +216,9 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
     p.out = out;
     p.ldo = ldo;
     p.epi = epi;
+    p.epi.vec_bias = row_vec(epi.bias, 0);
+    p.epi.vec_residual = row_vec(epi.residual, epi.ldr);
+    p.epi.vec_z = row_vec(epi.z, epi.ldz);
     p.epi.vec_out = row_vec(out, ldo);
     p.M = groups.rows;
     p.N = cols;
@@ -231,6 +248,9 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
   p.ldo = ldo;
   p.groups = groups;
   p.epi = epi;
+  p.epi.pair_residual = column_pairs(epi.residual, epi.ldr, cols);
+  p.epi.pair_z = column_pairs(epi.z, epi.ldz, cols);
+  p.epi.pair_out = column_pairs(out, ldo, cols);
   p.cols = cols;
   p.tiles_n = ceil_div(cols, LS::kRows);
   p.num_kb = num_kb;
@@ -357,9 +377,6 @@ int arc_linear_bf16(const uint16_t* x, const uint16_t* w, const uint16_t* bias, 
   epi.ldr = residual != nullptr ? ldr : 0;
   epi.ldz = z != nullptr ? ldz : 0;
   epi.act = static_cast<uint32_t>(activation);
-  epi.vec_bias = row_vec(bias, 0);
-  epi.vec_residual = row_vec(residual, epi.ldr);
-  epi.vec_z = row_vec(z, epi.ldz);
   const arcb::lin::Groups groups = {nullptr, 1u, static_cast<uint32_t>(M)};
   return linear_rows(x, w, groups, out, N, K, ldx, ldw, uint64_t(N) * ldw, ldo, epi, false, false, stream);
 }

@@ -183,15 +183,6 @@ __device__ __forceinline__ void expand_codes(const uint4& x, uint32_t split, uin
   }
 }
 
-// Arrive on a barrier of the other CTA without ordering memory at cluster scope: a release there
-// holds the thread up for about 1700 cycles, three times a stage's products. What the arrival
-// announces needs no more: the expanded weights lie in this CTA's shared memory, where only this
-// SM's tensor core reads them, and the expanding threads have made them visible to it
-// (fence.proxy.async) before the arrival that this thread has waited for.
-__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
-  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
-}
-
 template <bool W_MN, bool W4>
 __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(const __grid_constant__ Params p) {
   static_assert(!(W_MN && W4), "codes are K-major");
@@ -379,6 +370,8 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
       for (uint32_t t = pair; ok && tile_at(p, s.prefix, t, w); t += num_pairs) {
         for (uint32_t kb = 0; kb < p.num_kb && ok; ++kb) {
           ok = mbar_wait_poll(&s.expanded[stage], phase, abort, kStatusTimeoutUnpack);
+          // The expanded weights lie in this CTA's shared memory, where only this SM's tensor core
+          // reads them, and were made visible to it (fence.proxy.async) before "expanded".
           if (ok) mbar_arrive_cluster_relaxed(map_to_rank(&s.full[stage], 0));
           if (++stage == kStages) {
             stage = 0;
@@ -406,7 +399,7 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
       tc_fence_after_sync();
       const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * kTileT;
 #pragma unroll 1
-      for (uint32_t c0 = wg * 32u; c0 < w.n; c0 += 64u) {
+      for (uint32_t c0 = wg * 32u; c0 < w.rows; c0 += 64u) {
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_row + c0, r);
         tmem_ld_wait();
@@ -418,35 +411,15 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
             r[j] = __float_as_uint(__uint_as_float(r[j]) * (__shfl_sync(0xffffffffu, sa, j) * unscale));
           }
         }
-        uint16_t* o = p.out + size_t(w.row0 + c0) * p.ldo + f;
-        if (p.pair_store) {
-          // Neighbouring lanes exchange values so that each stores two columns of one row: the
-          // even lane's rows are the even ones. The output's columns come in whole pairs here.
-          const uint32_t odd = lane & 1u;
-          uint16_t* o2 = o - odd + odd * p.ldo;
+        float v[32];
 #pragma unroll
-          for (uint32_t j = 0; j < 32; j += 2) {
-            const uint32_t give = odd ? r[j] : r[j + 1];
-            const uint32_t got = __shfl_xor_sync(0xffffffffu, give, 1);
-            const uint32_t lo = odd ? got : r[j], hi = odd ? r[j + 1] : got;
-            if (valid && c0 + j + odd < w.rows) {
-              *reinterpret_cast<uint32_t*>(o2 + size_t(j) * p.ldo) =
-                  pack_bf16x2(__uint_as_float(lo), __uint_as_float(hi));
-            }
-          }
-        } else {
-#pragma unroll
-          for (uint32_t j = 0; j < 32; ++j) {
-            if (valid && c0 + j < w.rows) {
-              o[size_t(j) * p.ldo] = __bfloat16_as_ushort(__float2bfloat16_rn(__uint_as_float(r[j])));
-            }
-          }
-        }
+        for (uint32_t j = 0; j < 32; ++j) v[j] = __uint_as_float(r[j]);
+        lin::store_columns(p.out + size_t(w.row0 + c0) * p.ldo + f, p.ldo, v, w.rows - c0, valid, p.pair_store);
         __syncwarp();
       }
       tc_fence_before_sync();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(empty0[acc]);
+      if (lane == 0) mbar_arrive_cluster_relaxed(empty0[acc]);
     }
   } else if (W4 && warp >= 4 + kEpiWarps && (warp & 3u) != 1u) {
     // ------------------------------------------------------------ codes -> fp16 weights

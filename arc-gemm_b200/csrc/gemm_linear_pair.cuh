@@ -343,7 +343,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
         if (c + 2u >= kTile / 32u) {
           tc_fence_before_sync();
           __syncwarp();
-          if (lane == 0) mbar_arrive_cluster(empty0[acc]);
+          if (lane == 0) mbar_arrive_cluster_relaxed(empty0[acc]);
         }
         if (live) {
           uint32_t packed[16];
@@ -364,20 +364,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
               }
               lin::store_row32(p.epi.z + size_t(m) * p.epi.ldz + n, packed, cols, p.epi.vec_z);
             }
-            switch (p.epi.act) {  // one uniform branch per 32 columns
-#define ARC_ACT_CASE(A)                                                                            \
-    case A:                                                                                          \
-      _Pragma("unroll") for (uint32_t i = 0; i < 32; ++i) r[i] =                                     \
-          __float_as_uint(lin::act_value(__uint_as_float(r[i]), A));                                 \
-      break;
-              ARC_ACT_CASE(lin::kActRelu)
-              ARC_ACT_CASE(lin::kActGelu)
-              ARC_ACT_CASE(lin::kActGeluTanh)
-              ARC_ACT_CASE(lin::kActSilu)
-#undef ARC_ACT_CASE
-              default:
-                break;
-            }
+            float v[32];
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+            lin::activate(v, p.epi.act);
+#pragma unroll
+            for (uint32_t i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
             if (with_residual) {
 #pragma unroll
               for (uint32_t i = 0; i < 16; ++i) {

@@ -224,31 +224,28 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_linear_stream_kernel(const _
     if (ok) {
 #pragma unroll 1
       for (uint32_t c0 = 0; c0 < rows; c0 += 16u) {
-        uint32_t r[16];
+        const size_t row = row0 + c0;
+        uint32_t r[16], res[16];
         tmem_ld_32x32b_x16(t_row + c0, r);
-        float res[16];
         if (p.epi.residual != nullptr) {
-#pragma unroll
-          for (uint32_t j = 0; j < 16; ++j) {
-            res[j] = mine && c0 + j < rows
-                         ? bf16_bits_to_float(p.epi.residual[size_t(row0 + c0 + j) * p.epi.ldr + f])
-                         : 0.f;
-          }
+          lin::load_columns_start(p.epi.residual + row * p.epi.ldr + f, p.epi.ldr, res, rows - c0, mine, p.epi.pair_residual);
         }
         tmem_ld_wait();
-        if (mine) {
+        float v[16];
 #pragma unroll
-          for (uint32_t j = 0; j < 16; ++j) {
-            if (c0 + j < rows) {
-              const float z = __uint_as_float(r[j]) + bias;
-              const size_t row = row0 + c0 + j;
-              if (p.epi.z != nullptr) p.epi.z[row * p.epi.ldz + f] = __bfloat16_as_ushort(__float2bfloat16_rn(z));
-              float y = lin::act_value(z, p.epi.act);
-              if (p.epi.residual != nullptr) y += res[j];
-              p.out[row * p.ldo + f] = __bfloat16_as_ushort(__float2bfloat16_rn(y));
-            }
-          }
+        for (uint32_t j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) + bias;
+        if (p.epi.z != nullptr) {
+          lin::store_columns(p.epi.z + row * p.epi.ldz + f, p.epi.ldz, v, rows - c0, mine, p.epi.pair_z);
         }
+        lin::activate(v, p.epi.act);
+        if (p.epi.residual != nullptr) {
+          float add[16];
+          lin::load_columns_finish(res, add, p.epi.pair_residual);
+#pragma unroll
+          for (uint32_t j = 0; j < 16; ++j) v[j] += add[j];
+        }
+        lin::store_columns(p.out + row * p.ldo + f, p.ldo, v, rows - c0, mine, p.epi.pair_out);
+        __syncwarp();
       }
     }
   } else {

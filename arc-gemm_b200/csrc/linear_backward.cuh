@@ -26,7 +26,36 @@ struct Params {
   uint32_t M, N, act, rows_per_block;
 };
 
+// v *= act'(z), one branch for eight values.
+__device__ __forceinline__ void times_slope8(float (&v)[8], const float (&z)[8], uint32_t act) {
+  switch (act) {
+#define ARC_SLOPE_CASE(A)                                                              \
+  case A:                                                                              \
+    _Pragma("unroll") for (uint32_t j = 0; j < 8; ++j) v[j] *= lin::act_slope(z[j], A); \
+    break;
+    ARC_SLOPE_CASE(lin::kActRelu)
+    ARC_SLOPE_CASE(lin::kActGelu)
+    ARC_SLOPE_CASE(lin::kActGeluTanh)
+    ARC_SLOPE_CASE(lin::kActSilu)
+#undef ARC_SLOPE_CASE
+    default:
+      break;
+  }
+}
+
+__device__ __forceinline__ void unpack8(const uint4& x, float (&v)[8]) {
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    v[2 * j] = __uint_as_float(w[j] << 16);
+    v[2 * j + 1] = __uint_as_float(w[j] & 0xFFFF0000u);
+  }
+}
+
 // VEC: every row of dy, z and dz is 16-byte aligned and N is a multiple of 8.
+// A thread keeps kAhead rows' loads in flight: the loads of a round come before its stores.
+constexpr uint32_t kAhead = 4;
+
 template <bool VEC>
 __global__ void __launch_bounds__(kThreads) linear_dz_kernel(const Params p) {
   __shared__ float sums[kRowLanes][kColsPerBlock];
@@ -42,42 +71,55 @@ __global__ void __launch_bounds__(kThreads) linear_dz_kernel(const Params p) {
   if (VEC) {
     const uint32_t n = n0 + tx * 8u;
     if (n < p.N) {
-#pragma unroll 4
-      for (uint32_t m = m_begin + ty; m < m_end; m += kRowLanes) {
-        const uint4 g = __ldg(reinterpret_cast<const uint4*>(p.dy + size_t(m) * p.lddy + n));
-        float v[8] = {__uint_as_float(g.x << 16), __uint_as_float(g.x & 0xFFFF0000u),
-                      __uint_as_float(g.y << 16), __uint_as_float(g.y & 0xFFFF0000u),
-                      __uint_as_float(g.z << 16), __uint_as_float(g.z & 0xFFFF0000u),
-                      __uint_as_float(g.w << 16), __uint_as_float(g.w & 0xFFFF0000u)};
-        if (p.z != nullptr) {
-          const uint4 a = __ldg(reinterpret_cast<const uint4*>(p.z + size_t(m) * p.ldz + n));
-          const float zv[8] = {__uint_as_float(a.x << 16), __uint_as_float(a.x & 0xFFFF0000u),
-                               __uint_as_float(a.y << 16), __uint_as_float(a.y & 0xFFFF0000u),
-                               __uint_as_float(a.z << 16), __uint_as_float(a.z & 0xFFFF0000u),
-                               __uint_as_float(a.w << 16), __uint_as_float(a.w & 0xFFFF0000u)};
+      for (uint32_t m0 = m_begin + ty; m0 < m_end; m0 += kAhead * kRowLanes) {
+        uint4 g[kAhead], a[kAhead];
 #pragma unroll
-          for (uint32_t j = 0; j < 8; ++j) v[j] *= lin::act_slope(zv[j], p.act);
-        }
-        if (p.dz != nullptr) {
-          *reinterpret_cast<uint4*>(p.dz + size_t(m) * p.lddz + n) =
-              make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
-                         pack_bf16x2(v[6], v[7]));
+        for (uint32_t i = 0; i < kAhead; ++i) {
+          const uint32_t m = m0 + i * kRowLanes;
+          if (m < m_end) {
+            g[i] = __ldg(reinterpret_cast<const uint4*>(p.dy + size_t(m) * p.lddy + n));
+            if (p.z != nullptr) a[i] = __ldg(reinterpret_cast<const uint4*>(p.z + size_t(m) * p.ldz + n));
+          }
         }
 #pragma unroll
-        for (uint32_t j = 0; j < 8; ++j) acc[j] += v[j];
+        for (uint32_t i = 0; i < kAhead; ++i) {
+          const uint32_t m = m0 + i * kRowLanes;
+          if (m >= m_end) break;
+          float v[8];
+          unpack8(g[i], v);
+          if (p.z != nullptr) {
+            float z[8];
+            unpack8(a[i], z);
+            times_slope8(v, z, p.act);
+          }
+          if (p.dz != nullptr) {
+            *reinterpret_cast<uint4*>(p.dz + size_t(m) * p.lddz + n) =
+                make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]),
+                           pack_bf16x2(v[6], v[7]));
+          }
+#pragma unroll
+          for (uint32_t j = 0; j < 8; ++j) acc[j] += v[j];
+        }
       }
     }
   } else {
+    // Lanes take neighbouring columns, eight of them 32 apart.
     for (uint32_t m = m_begin + ty; m < m_end; m += kRowLanes) {
+      float v[8], z[8];
 #pragma unroll
       for (uint32_t j = 0; j < 8; ++j) {
         const uint32_t n = n0 + j * 32u + tx;
-        if (n < p.N) {
-          float v = bf16_bits_to_float(__ldg(p.dy + size_t(m) * p.lddy + n));
-          if (p.z != nullptr) v *= lin::act_slope(bf16_bits_to_float(__ldg(p.z + size_t(m) * p.ldz + n)), p.act);
-          if (p.dz != nullptr) p.dz[size_t(m) * p.lddz + n] = __bfloat16_as_ushort(__float2bfloat16_rn(v));
-          acc[j] += v;
+        v[j] = n < p.N ? bf16_bits_to_float(__ldg(p.dy + size_t(m) * p.lddy + n)) : 0.f;
+        z[j] = n < p.N && p.z != nullptr ? bf16_bits_to_float(__ldg(p.z + size_t(m) * p.ldz + n)) : 0.f;
+      }
+      if (p.z != nullptr) times_slope8(v, z, p.act);
+#pragma unroll
+      for (uint32_t j = 0; j < 8; ++j) {
+        const uint32_t n = n0 + j * 32u + tx;
+        if (n < p.N && p.dz != nullptr) {
+          p.dz[size_t(m) * p.lddz + n] = __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
         }
+        acc[j] += v[j];
       }
     }
   }

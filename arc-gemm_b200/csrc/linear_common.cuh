@@ -161,6 +161,86 @@ __device__ __forceinline__ float act_slope(float z, uint32_t act) {
   }
 }
 
+// The activation of N values, one branch for all.
+template <uint32_t N>
+__device__ __forceinline__ void activate(float (&v)[N], uint32_t act) {
+  switch (act) {
+#define ARC_ACT_CASE(A)                                                             \
+  case A:                                                                           \
+    _Pragma("unroll") for (uint32_t i = 0; i < N; ++i) v[i] = act_value(v[i], A);    \
+    break;
+    ARC_ACT_CASE(kActRelu)
+    ARC_ACT_CASE(kActGelu)
+    ARC_ACT_CASE(kActGeluTanh)
+    ARC_ACT_CASE(kActSilu)
+#undef ARC_ACT_CASE
+    default:
+      break;
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// Row-major access from the transposed side: a lane holds one column (lane l of the warp column
+// f = f0 + l) of N consecutive rows, of which `rows` exist. With `paired` (whole column pairs,
+// 4-byte aligned rows) neighbouring lanes exchange values, so that each moves two columns of
+// every second row. All lanes of the warp take part; `valid` says whether this lane's column
+// exists.
+// ---------------------------------------------------------------------------------
+template <uint32_t N>
+__device__ __forceinline__ void store_columns(uint16_t* p, uint64_t ld, const float (&v)[N], uint32_t rows, bool valid,
+                                              uint32_t paired) {
+  if (paired) {
+    const uint32_t odd = threadIdx.x & 1u;
+    uint16_t* p2 = p - odd + odd * ld;
+#pragma unroll
+    for (uint32_t j = 0; j < N; j += 2) {
+      const float got = __shfl_xor_sync(0xffffffffu, odd ? v[j] : v[j + 1], 1);
+      if (valid && j + odd < rows) {
+        *reinterpret_cast<uint32_t*>(p2 + size_t(j) * ld) = odd ? pack_bf16x2(got, v[j + 1]) : pack_bf16x2(v[j], got);
+      }
+    }
+  } else {
+#pragma unroll
+    for (uint32_t j = 0; j < N; ++j) {
+      if (valid && j < rows) p[size_t(j) * ld] = __bfloat16_as_ushort(__float2bfloat16_rn(v[j]));
+    }
+  }
+}
+
+// The raw words of a paired load, for load_columns_finish (so that other work can come between).
+template <uint32_t N>
+__device__ __forceinline__ void load_columns_start(const uint16_t* p, uint64_t ld, uint32_t (&raw)[N], uint32_t rows,
+                                                   bool valid, uint32_t paired) {
+  const uint32_t odd = threadIdx.x & 1u;
+  const uint16_t* p2 = p - odd + odd * ld;
+#pragma unroll
+  for (uint32_t j = 0; j < N; ++j) {
+    raw[j] = 0u;
+    if (paired) {
+      if ((j & 1u) == 0u && valid && j + odd < rows) raw[j] = *reinterpret_cast<const uint32_t*>(p2 + size_t(j) * ld);
+    } else if (valid && j < rows) {
+      raw[j] = p[size_t(j) * ld];
+    }
+  }
+}
+
+template <uint32_t N>
+__device__ __forceinline__ void load_columns_finish(const uint32_t (&raw)[N], float (&v)[N], uint32_t paired) {
+  const uint32_t odd = threadIdx.x & 1u;
+#pragma unroll
+  for (uint32_t j = 0; j < N; j += 2) {
+    if (paired) {
+      const uint32_t other = __shfl_xor_sync(0xffffffffu, raw[j], 1);
+      const uint32_t even_row = odd ? other : raw[j], odd_row = odd ? raw[j] : other;
+      v[j] = odd ? __uint_as_float(even_row & 0xFFFF0000u) : __uint_as_float(even_row << 16);
+      v[j + 1] = odd ? __uint_as_float(odd_row & 0xFFFF0000u) : __uint_as_float(odd_row << 16);
+    } else {
+      v[j] = __uint_as_float(raw[j] << 16);
+      v[j + 1] = __uint_as_float(raw[j + 1] << 16);
+    }
+  }
+}
+
 // ---------------------------------------------------------------------------------
 // 32 consecutive bf16 columns of one row, of which `cols` are in range. `vec` is the widest
 // access every row allows: 2 = 32 bytes, 1 = 16 bytes, 0 = single elements (the host derives
@@ -229,7 +309,8 @@ struct Epilogue {
   uint16_t* z;               // [M][ldz] or null: x w^T + bias, bf16
   uint64_t ldr, ldz;
   uint32_t act;
-  uint32_t vec_bias, vec_residual, vec_z, vec_out;
+  uint32_t vec_bias, vec_residual, vec_z, vec_out;      // row-wise access (store_row32)
+  uint32_t pair_residual, pair_z, pair_out;             // column-wise access (store_columns)
 };
 
 // Shared-memory descriptor of an MN-major operand as a TMA load with the 128-byte swizzle

@@ -636,6 +636,14 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
                : "memory");
 }
 
+// The same without ordering memory at cluster scope: a release there holds the arriving thread up
+// for about 1700 cycles, and longer while stores of its own are in flight. For announcements that
+// need no such order: accumulators read (the reads have completed, tcgen05.wait::ld), or operands
+// that only this SM's tensor core reads and that were made visible to it before.
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
+}
+
 // 2-D tiled load into this CTA's shared memory whose completion is signalled on an
 // mbarrier of either CTA of the pair (`bar` is a shared::cluster address).
 __device__ __forceinline__ void tma_load_2d_pair(const CUtensorMap* map, uint32_t bar, void* dst,
