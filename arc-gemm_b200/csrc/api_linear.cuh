@@ -333,12 +333,13 @@ int output_check(const char* what, const char* name, const void* p, int64_t ld, 
   return ARC_OK;
 }
 
-// Row blocks of the dz pass: enough blocks to fill the GPU several times over, at least 16
-// rows each.
-constexpr uint32_t kDzBlocks = 6 * 148;  // of the whole grid; the workspace size must not depend on the device
+// Row blocks of the dz pass: the grid fills the GPU's block slots once, without a rest (a rest of
+// a few blocks costs a whole round: 59 against DZ_US us at 4096 x 8192), at least 16 rows each.
+// The workspace size must not depend on the device.
+constexpr uint32_t kDzBlocks = 148 * LB::kBlocksPerSm;
 uint32_t dz_row_blocks(uint32_t M, uint32_t N) {
-  const uint32_t want = ceil_div(kDzBlocks, ceil_div(N, LB::kColsPerBlock)), most = ceil_div(M, 16);
-  return want < most ? want : most;
+  const uint32_t want = kDzBlocks / ceil_div(N, LB::kColsPerBlock), most = ceil_div(M, 16);
+  return want < 1 ? 1 : want < most ? want : most;
 }
 // dz lies in the workspace with rows that TMA can read.
 uint64_t dz_ld(uint32_t N) { return (uint64_t(N) + 7) / 8 * 8; }

@@ -59,7 +59,18 @@ __global__ void __launch_bounds__(kThreads) count_rows_kernel(const Params p) {
   __syncthreads();
   pdl_wait();
   const uint32_t begin = blockIdx.x * p.per_block, end = min(p.slots, begin + p.per_block);
-  for (uint32_t i = begin + threadIdx.x; i < end; i += kThreads) atomicAdd(&hist[bucket_of<Id>(p, i)], 1u);
+  for (uint32_t i0 = begin + threadIdx.x; i0 < end; i0 += kThreads * kKept) {
+    uint32_t b[kKept];  // loads first
+#pragma unroll
+    for (uint32_t j = 0; j < kKept; ++j) {
+      const uint32_t i = i0 + j * kThreads;
+      b[j] = i < end ? bucket_of<Id>(p, i) : kNone;
+    }
+#pragma unroll
+    for (uint32_t j = 0; j < kKept; ++j) {
+      if (b[j] != kNone) atomicAdd(&hist[b[j]], 1u);
+    }
+  }
   __syncthreads();
   const uint32_t ld = counts_ld(p.blocks);
   for (uint32_t i = threadIdx.x; i < buckets; i += kThreads) {
@@ -114,7 +125,7 @@ __global__ void __launch_bounds__(kThreads) place_rows_kernel(const Params p) {
     }
   } else {
     const uint32_t vecs = counts_ld(p.blocks) / 4u;
-#pragma unroll 4
+#pragma unroll 8
     for (uint32_t b = warp; b < buckets; b += kWarps) {
       const uint4* column = reinterpret_cast<const uint4*>(p.counts) + size_t(b) * vecs;
       uint32_t total = 0, earlier = 0;

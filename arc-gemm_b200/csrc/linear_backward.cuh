@@ -16,6 +16,7 @@ namespace linbwd {
 constexpr uint32_t kThreads = 256;
 constexpr uint32_t kColsPerBlock = 256;  // 32 threads x 8 columns
 constexpr uint32_t kRowLanes = 8;
+constexpr uint32_t kBlocksPerSm = 3;
 
 struct Params {
   const uint16_t* dy;  // [M][lddy]
@@ -57,7 +58,7 @@ __device__ __forceinline__ void unpack8(const uint4& x, float (&v)[8]) {
 constexpr uint32_t kAhead = 4;
 
 template <bool VEC>
-__global__ void __launch_bounds__(kThreads) linear_dz_kernel(const Params p) {
+__global__ void __launch_bounds__(kThreads, kBlocksPerSm) linear_dz_kernel(const Params p) {
   __shared__ float sums[kRowLanes][kColsPerBlock];
   pdl_launch_dependents();
   pdl_wait();
