@@ -22,7 +22,7 @@ int encode_groups_3d(CUtensorMap* map, const void* ptr, uint64_t cols, uint64_t 
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[3] = {cols, rows, groups};
-  const cuuint64_t strides[2] = {ld * 2, group_stride * 2};
+  const cuuint64_t strides[2] = {ld * 2, (groups > 1 ? group_stride : ld) * 2};  // one group: never used
   const cuuint32_t box[3] = {box_cols, box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, estr,
@@ -205,8 +205,7 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
   }
   if (plan.pair) {
     LP::Params p = {};
-    if (int st = encode_groups_3d(&p.tm_a, a, inner, groups.rows, 1, lda, uint64_t(groups.rows) * lda, 64,
-                                  LP::kRowsPerCta, "rows")) {
+    if (int st = encode_groups_3d(&p.tm_a, a, inner, groups.rows, 1, lda, 0, 64, LP::kRowsPerCta, "rows")) {
       return st;
     }
     if (int st = encode_groups_3d(&p.tm_b, w, w_cols, w_rows, 1, ldw, w_stride, 64, grad ? 64 : LP::kRowsPerCta,
@@ -273,8 +272,8 @@ int linear_dw(const char* what, const uint16_t* dy, const uint16_t* x, const arc
   const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
   if (max_pairs == 0) return fail(ARC_ERR_UNSUPPORTED, "%s: no CTA pair fits on this device", what);
   LP::Params p = {};
-  if (int st = encode_groups_3d(&p.tm_a, dy, N, groups.rows, 1, lddy, uint64_t(groups.rows) * lddy, 64, 64, "dy")) return st;
-  if (int st = encode_groups_3d(&p.tm_b, x, K, groups.rows, 1, ldx, uint64_t(groups.rows) * ldx, 64, 64, "x")) return st;
+  if (int st = encode_groups_3d(&p.tm_a, dy, N, groups.rows, 1, lddy, 0, 64, 64, "dy")) return st;
+  if (int st = encode_groups_3d(&p.tm_b, x, K, groups.rows, 1, ldx, 0, 64, 64, "x")) return st;
   p.out = dw;
   p.ldo = lddw;
   p.out_group = dw_stride;

@@ -42,6 +42,7 @@ constexpr uint32_t kTileT = 256;       // most rows of a group per tile
 constexpr uint32_t kSubK = 64;         // one 128-byte swizzle row
 constexpr uint32_t kSubBytes = kRowsPerCta * kSubK * 2;
 constexpr uint32_t kEpiWarps = 8;
+constexpr uint32_t kBandF = 8;  // weight tiles per raster band
 // W4: the expanding warps work in sets of four on alternate stages: what a stage costs a warp is
 // mostly waiting (for the slot, for its stores to be visible to the tensor core), about twice a
 // stage's products. None of them shares a scheduler with the UMMA issuer (warp 1, and so every
@@ -119,10 +120,13 @@ __device__ __forceinline__ bool tile_at(const Params& p, const uint32_t* prefix,
   w.e = lin::group_of_tile(prefix, p.groups.num, t / p.tiles_f);
   const uint32_t own = prefix[w.e + 1] - prefix[w.e];
   const uint32_t rem = t - prefix[w.e] * p.tiles_f;
-  // A group's row tiles side by side: they read the same weights.
-  const uint32_t ft = rem / own;
-  w.f0 = ft * kTileF;
-  const uint32_t at = (rem - ft * own) * kTileT;
+  // Bands of eight weight tiles: the pairs that run together share both operands in L2 (one group
+  // of 8192 rows, 4096 x 4096: 191 us with a group's row tiles first, 177 in bands).
+  const uint32_t band = rem / (kBandF * own);
+  const uint32_t in_band = rem - band * kBandF * own;
+  const uint32_t width = min(kBandF, p.tiles_f - band * kBandF);
+  w.f0 = (band * kBandF + in_band % width) * kTileF;
+  const uint32_t at = in_band / width * kTileT;
   w.row0 = lin::group_begin(p.groups, w.e) + at;
   w.rows = min(kTileT, lin::group_count(p.groups, w.e) - at);
   w.n = (w.rows + 31u) & ~31u;

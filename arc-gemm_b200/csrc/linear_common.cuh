@@ -83,9 +83,14 @@ __device__ __forceinline__ void zero_other_rows(const Groups& g, uint16_t* out, 
                                                 uint32_t block, uint32_t num_blocks) {
   const uint32_t first = group_bound(g, 0), last = group_bound(g, g.num);
   const uint32_t behind = last < g.rows ? g.rows - last : 0u;
+  const bool wide = ((reinterpret_cast<uintptr_t>(out) | (ldo * 2)) & 15u) == 0u;
   for (uint32_t i = block; i < first + behind; i += num_blocks) {
     uint16_t* row = out + size_t(i < first ? i : last + (i - first)) * ldo;
-    for (uint32_t c = threadIdx.x; c < cols; c += blockDim.x) row[c] = 0;
+    const uint32_t vecs = wide ? cols / 8u : 0u;
+    for (uint32_t c = threadIdx.x; c < vecs; c += blockDim.x) {
+      reinterpret_cast<uint4*>(row)[c] = make_uint4(0u, 0u, 0u, 0u);
+    }
+    for (uint32_t c = vecs * 8u + threadIdx.x; c < cols; c += blockDim.x) row[c] = 0;
   }
 }
 

@@ -130,10 +130,13 @@ Tensor unit_rows(const Tensor& t) {
   return t.stride(1) == 1 && t.stride(0) >= t.size(1) ? t : t.contiguous();
 }
 
+// Their leading dimension (a single row may have any stride).
+int64_t row_ld(const Tensor& t) { return t.size(0) == 1 ? std::max(t.stride(0), t.size(1)) : t.stride(0); }
+
 void expect_out(const Tensor& out, int64_t rows, int64_t cols, const at::Device& dev) {
   expect_bf16(out, "out", 2);
   if (out.size(0) != rows || out.size(1) != cols || out.device() != dev || out.stride(1) != 1 ||
-      out.stride(0) < cols) {
+      (rows > 1 && out.stride(0) < cols)) {
     bad_value("out must be a row-major bf16 [", rows, ", ", cols, "] tensor on ", dev.str());
   }
 }
@@ -160,7 +163,7 @@ void linear_call(const Tensor& x, const Tensor& w, const OptTensor& bias, const 
                  const Tensor& z, int act) {
   check(g_api.linear(u16(x), u16(w), bias ? u16(*bias) : nullptr, residual ? u16(*residual) : nullptr, u16_mut(out),
                      z.defined() ? u16_mut(z) : nullptr, x.size(0), w.size(0), x.size(1), x.stride(0), w.stride(0),
-                     residual ? residual->stride(0) : 0, out.stride(0), z.defined() ? z.stride(0) : 0, act,
+                     residual ? row_ld(*residual) : 0, row_ld(out), z.defined() ? z.stride(0) : 0, act,
                      stream_of(x)),
         "arc.linear");
 }
@@ -208,7 +211,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     if (need_w) out[1] = m > 0 ? at::empty({n, k}, options) : at::zeros({n, k}, options);
     if (need_bias) out[2] = m > 0 ? at::empty({n}, options) : at::zeros({n}, options);
     if (m > 0) {
-      const bool need_dz = (need_x || need_w) && (z.defined() || dy.stride(0) % 8 != 0 || !aligned16(dy));
+      const bool need_dz = (need_x || need_w) && (z.defined() || row_ld(dy) % 8 != 0 || !aligned16(dy));
       size_t bytes = 0;
       check(g_api.linear_backward_ws(m, n, need_dz, need_bias, &bytes), "arc.linear backward");
       Tensor workspace;
@@ -216,7 +219,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       check(g_api.linear_backward(u16(dy), u16(x), u16(w), z.defined() ? u16(z) : nullptr,
                                   need_x ? u16_mut(out[0]) : nullptr, need_w ? u16_mut(out[1]) : nullptr,
                                   need_bias ? u16_mut(out[2]) : nullptr, bytes > 0 ? workspace.data_ptr() : nullptr,
-                                  bytes, m, n, k, dy.stride(0), x.stride(0), w.stride(0), z.defined() ? z.stride(0) : 0,
+                                  bytes, m, n, k, row_ld(dy), x.stride(0), w.stride(0), z.defined() ? z.stride(0) : 0,
                                   k, k, static_cast<int>(ctx->saved_data["act"].toInt()), stream_of(x)),
             "arc.linear backward");
     }
@@ -273,7 +276,7 @@ void expect_offsets(const Tensor& offsets, int64_t groups, const at::Device& dev
 
 void grouped_call(const Tensor& x, const Tensor& w, const Tensor& offsets, const Tensor& out, bool zero_others) {
   check(g_api.grouped(u16(x), u16(w), offsets.const_data_ptr<int32_t>(), u16_mut(out), x.size(0), w.size(0), w.size(1),
-                      x.size(1), x.stride(0), w.stride(1), w.stride(0), out.stride(0),
+                      x.size(1), x.stride(0), w.stride(1), w.stride(0), row_ld(out),
                       zero_others ? ARC_GROUPED_ZERO_OTHERS : 0u, stream_of(x)),
         "arc.grouped_matmul");
 }

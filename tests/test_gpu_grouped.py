@@ -135,6 +135,25 @@ def test_grouped_layouts(cuda_device):
     assert arc.grouped_matmul(x[:0], w, torch.zeros(4, dtype=torch.int32, device="cuda")).shape == (0, 37)
 
 
+@pytest.mark.parametrize("plan", [None, "pair", "16:1"])
+@pytest.mark.parametrize("n", [96, 33])
+def test_mostly_padding(cuda_device, monkeypatch, plan, n):
+    """A buffer of which the groups fill little: the rest is zeroed, or left alone."""
+    if plan:
+        monkeypatch.setenv("ARC_LINEAR_PLAN", plan)
+    g = torch.Generator().manual_seed(1)
+    x, w = normal(g, 3000, 64), normal(g, 4, n, 64)
+    offsets = torch.tensor([7, 10, 10, 40, 41], dtype=torch.int32, device="cuda")
+    y = arc.grouped_matmul(x, w, offsets)
+    assert (y[:7] == 0).all() and (y[41:] == 0).all() and (y[7:41] != 0).any(1).all()
+    out = torch.full_like(y, 4.0)
+    arc.grouped_matmul(x, w, offsets, out=out)
+    assert (out[:7] == 4).all() and (out[41:] == 4).all() and torch.equal(out[7:41], y[7:41])
+    lx, lw = x.clone().requires_grad_(), w.clone().requires_grad_()
+    dx, dw = torch.autograd.grad(arc.grouped_matmul(lx, lw, offsets), [lx, lw], torch.ones_like(y))
+    assert (dx[:7] == 0).all() and (dx[41:] == 0).all() and (dw[1] == 0).all()
+
+
 def test_bad_offsets_are_reported(cuda_device):
     """Offsets outside the rows stay in bounds and set the status bit."""
     x, w, _, _ = _inputs([40], 0, 64, 64)

@@ -161,6 +161,24 @@ def test_partial_gradients_and_layouts(cuda_device):
         assert_within(v, *want[name], name)
 
 
+def test_single_row_and_column_layouts(cuda_device):
+    """One row or one column: the other stride may be anything."""
+    x, w, b, r = _inputs(1, 24, 64)
+    y, bound, _, _ = linear_forward(x, w, b, r, "relu")
+    odd = [t.as_strided(t.shape, (3, 1)) for t in (x, r)]
+    assert_within(arc.linear(odd[0], w, b, odd[1], activation="relu"), y, bound, "row")
+    out = torch.empty(24, dtype=torch.bfloat16, device="cuda").as_strided((1, 24), (5, 1))
+    assert_within(arc.linear(x, w, b, r, activation="relu", out=out), y, bound, "out")
+    lx, lw, lb = _leaves(x, w, b)
+    arc.linear(lx, lw, lb).backward(odd[1])
+    _, _, z, zerr = linear_forward(x, w, b, None, None)
+    for leaf, name in ((lx, "dx"), (lw, "dw"), (lb, "dbias")):
+        assert_within(leaf.grad, *linear_gradients(x, w, z, zerr, r, None)[name], name)
+    x, w, b, r = _inputs(9, 1, 64)
+    y, bound, _, _ = linear_forward(x, w, b, r, None)
+    assert_within(arc.linear(x, w, b, r.t().contiguous().t()), y, bound, "column")
+
+
 def test_no_rows(cuda_device):
     x, w, b, _ = _inputs(4, 24, 16, residual=False)
     assert arc.linear(x[:0], w, b).shape == (0, 24)
