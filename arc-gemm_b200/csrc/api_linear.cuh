@@ -18,7 +18,8 @@ namespace LB = arcb::linbwd;
 // Row-major matrices [groups][rows][cols] (bf16), `ld` elements between rows and
 // `group_stride` between groups.
 int encode_groups_3d(CUtensorMap* map, const void* ptr, uint64_t cols, uint64_t rows, uint64_t groups, uint64_t ld,
-                     uint64_t group_stride, uint32_t box_cols, uint32_t box_rows, const char* what) {
+                     uint64_t group_stride, uint32_t box_cols, uint32_t box_rows, const char* what,
+                     CUtensorMapSwizzle swizzle = CU_TENSOR_MAP_SWIZZLE_128B) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[3] = {cols, rows, groups};
@@ -26,7 +27,7 @@ int encode_groups_3d(CUtensorMap* map, const void* ptr, uint64_t cols, uint64_t 
   const cuuint32_t box[3] = {box_cols, box_rows, 1};
   const cuuint32_t estr[3] = {1, 1, 1};
   const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), dims, strides, box, estr,
-                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
                         CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled(%s) failed with CUresult %d", what, static_cast<int>(r));
@@ -34,10 +35,17 @@ int encode_groups_3d(CUtensorMap* map, const void* ptr, uint64_t cols, uint64_t 
   return ARC_OK;
 }
 
-// Widest vector that every row of a bf16 matrix allows (lin::store_row32).
-uint32_t row_vec(const void* p, uint64_t ld, uint64_t group_stride = 0) {
-  const uint64_t bits = reinterpret_cast<uintptr_t>(p) | (ld * 2) | (group_stride * 2);
-  return (bits & 31u) == 0 ? 2u : (bits & 15u) == 0 ? 1u : 0u;
+// Whether TMA (or a 16-byte access) reaches every row of a bf16 matrix.
+bool rows_aligned16(const void* p, uint64_t ld, uint64_t group_stride = 0) {
+  return ((reinterpret_cast<uintptr_t>(p) | (ld * 2) | (group_stride * 2)) & 15u) == 0;
+}
+
+// The map of an epilogue matrix's 32 x 32 pieces, where TMA reaches it.
+int encode_pieces(CUtensorMap* map, uint32_t* tma, const void* ptr, uint64_t cols, uint64_t rows, uint64_t groups,
+                  uint64_t ld, uint64_t group_stride, const char* what) {
+  *tma = ptr != nullptr && rows_aligned16(ptr, ld, groups > 1 ? group_stride : 0) ? 1u : 0u;
+  if (!*tma) return ARC_OK;
+  return encode_groups_3d(map, ptr, cols, rows, groups, ld, group_stride, 32, 32, what, CU_TENSOR_MAP_SWIZZLE_64B);
 }
 
 // Whether column pairs of a row-major bf16 matrix can be moved as 4-byte words.
@@ -58,11 +66,33 @@ uint32_t column_pairs(const void* p, uint64_t ld, uint32_t cols) {
 // least kStreamMinKb blocks of 64 each). Where that leaves SMs without work (a short
 // contraction), smaller row tiles fill them (1796 x 111 x 448 with a residual: STREAM_FILL).
 //
-// ARC_LINEAR_PLAN="pair" | "BN:S" (tests and tuning) forces the choice where it is valid.
+// ARC_LINEAR_PLAN="pair:S" | "BN:S" (tests and tuning) forces the choice where it is valid.
 struct LinearPlan {
   bool pair;
+  uint32_t pair_splits;
   uint32_t bn, splits, row_tiles;
 };
+
+// Parts of the contraction for `tiles` pair tiles: two where there are pairs for both, with at
+// least kPairMinKb blocks of 64 each. (Four would take clusters of eight CTAs, of which too few
+// fit at once: 512 x 4096 x 4096 25 us whole, 20 in two parts, 48 in four.)
+constexpr uint32_t kPairMinKb = 4;
+uint32_t pair_splits(uint64_t tiles, uint32_t num_kb, uint32_t max_pairs) {
+  return tiles * 2 <= max_pairs && num_kb >= 2 * kPairMinKb ? 2 : 1;
+}
+
+// The pair kernel, one cluster per tile if the contraction is split.
+template <bool A_MN, bool B_MN, bool ALONG_K>
+cudaError_t launch_linear_pair(LP::Params& p, uint64_t tiles, uint32_t splits, uint32_t max_pairs, cudaStream_t stream) {
+  p.splits = splits;
+  if (splits > 1) {
+    return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, true>, p, static_cast<uint32_t>(tiles) * 2 * splits,
+                     LP::kThreads, LP::kSmemBytes, 2 * splits, stream);
+  }
+  const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
+  return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, false>, p, grid, LP::kThreads, LP::kSmemBytes, 2,
+                   stream);
+}
 constexpr uint32_t kStreamMinKb = 4;
 
 int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t num_kb, LinearPlan* plan) {
@@ -72,19 +102,21 @@ int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t
   const uint32_t avg = ceil_div(rows, live);
   const uint64_t pair_tiles = uint64_t(ceil_div(avg, LP::kTile)) * live * ceil_div(cols, LP::kTile);
   plan->pair = max_pairs > 0 && avg > (groups == 1 ? 128u : 16u) && pair_tiles * 2 > max_pairs;
+  plan->pair_splits = groups == 1 ? pair_splits(pair_tiles, num_kb, max_pairs) : 1;
   plan->bn = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
   uint32_t forced = 0;
   if (const char* env = getenv("ARC_LINEAR_PLAN")) {
     unsigned bn = 0, s = 0;
-    if (strcmp(env, "pair") == 0 && max_pairs > 0) {
+    if (sscanf(env, "pair:%u", &s) == 1 && max_pairs > 0 && (s == 1 || s == 2)) {
       plan->pair = true;
+      plan->pair_splits = s <= num_kb ? s : 1;
     } else if (sscanf(env, "%u:%u", &bn, &s) == 2 && (bn == 16 || bn == 32 || bn == 64 || bn == 128) &&
                (s == 1 || s == 2 || s == 4 || s == 8)) {
       plan->pair = false;
       plan->bn = bn;
       forced = s;
     } else {
-      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_LINEAR_PLAN must be 'pair' or 'BN:S' (got '%s')", env);
+      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_LINEAR_PLAN must be 'pair:S' or 'BN:S' (got '%s')", env);
     }
   }
   for (;; plan->bn /= 2) {
@@ -126,9 +158,13 @@ cudaError_t linear_init(DeviceState& st) {
   if (e == cudaSuccess) e = allow_smem(LS::gemm_linear_stream_kernel<BN, MN>, LS::smem_bytes<BN>());
   ARC_LINEAR_STREAM_VARIANTS(ARC_SET_ATTR)
 #undef ARC_SET_ATTR
-  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, false, false>, LP::kSmemBytes);
-  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, true, false>, LP::kSmemBytes);
-  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<true, true, true>, LP::kSmemBytes);
+#define ARC_SET_ATTR(SPLIT)                                                                                         \
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, false, false, SPLIT>, LP::kSmemBytes);    \
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, true, false, SPLIT>, LP::kSmemBytes);     \
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<true, true, true, SPLIT>, LP::kSmemBytes);
+  ARC_SET_ATTR(false)
+  ARC_SET_ATTR(true)
+#undef ARC_SET_ATTR
   if (e == cudaSuccess) e = allow_smem(GP::gemm_grouped_pair_kernel<false, false>, GP::smem_bytes<false>());
   if (e == cudaSuccess) e = allow_smem(GP::gemm_grouped_pair_kernel<true, false>, GP::smem_bytes<false>());
   if (e == cudaSuccess) e = allow_smem(GP::gemm_grouped_pair_kernel<false, true>, GP::smem_bytes<true>());
@@ -215,10 +251,10 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
     p.out = out;
     p.ldo = ldo;
     p.epi = epi;
-    p.epi.vec_bias = row_vec(epi.bias, 0);
-    p.epi.vec_residual = row_vec(epi.residual, epi.ldr);
-    p.epi.vec_z = row_vec(epi.z, epi.ldz);
-    p.epi.vec_out = row_vec(out, ldo);
+    p.epi.wide_bias = aligned16(epi.bias) ? 1u : 0u;
+    if (int st = encode_pieces(&p.tm_out, &p.tma_out, out, cols, groups.rows, 1, ldo, 0, "out")) return st;
+    if (int st = encode_pieces(&p.tm_z, &p.tma_z, epi.z, cols, groups.rows, 1, epi.ldz, 0, "z")) return st;
+    if (int st = encode_pieces(&p.tm_res, &p.tma_res, epi.residual, cols, groups.rows, 1, epi.ldr, 0, "residual")) return st;
     p.M = groups.rows;
     p.N = cols;
     p.tiles_m = ceil_div(groups.rows, LP::kTile);
@@ -226,11 +262,8 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
     p.num_kb = num_kb;
     const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
     if (tiles > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
-    const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
-    e = grad ? launch_ex(LP::gemm_linear_pair_kernel<false, true, false>, p, grid, LP::kThreads, LP::kSmemBytes, 2,
-                         stream)
-             : launch_ex(LP::gemm_linear_pair_kernel<false, false, false>, p, grid, LP::kThreads, LP::kSmemBytes, 2,
-                         stream);
+    e = grad ? launch_linear_pair<false, true, false>(p, tiles, plan.pair_splits, max_pairs, stream)
+             : launch_linear_pair<false, false, false>(p, tiles, plan.pair_splits, max_pairs, stream);
     if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
     return ARC_OK;
   }
@@ -278,16 +311,17 @@ int linear_dw(const char* what, const uint16_t* dy, const uint16_t* x, const arc
   p.ldo = lddw;
   p.out_group = dw_stride;
   p.groups = groups;
-  p.epi.vec_out = row_vec(dw, lddw, dw_stride);
+  if (int st = encode_pieces(&p.tm_out, &p.tma_out, dw, K, N, groups.num, lddw, dw_stride, "dw")) return st;
   p.M = N;
   p.N = K;
   p.tiles_m = ceil_div(N, LP::kTile);
   p.tiles_n = ceil_div(K, LP::kTile);
   const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n * groups.num;
   if (tiles > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "%s: too many tiles for one launch", what);
-  const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
-  const cudaError_t e = launch_ex(LP::gemm_linear_pair_kernel<true, true, true>, p, grid, LP::kThreads, LP::kSmemBytes,
-                                  2, stream);
+  // The host knows the contraction's length only for one group of all rows.
+  const uint32_t splits =
+      groups.offsets == nullptr ? pair_splits(tiles, ceil_div(groups.rows, arcb::lin::BK), max_pairs) : 1;
+  const cudaError_t e = launch_linear_pair<true, true, true>(p, tiles, splits, max_pairs, stream);
   if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
   return ARC_OK;
 }
@@ -448,7 +482,7 @@ int arc_linear_backward(const uint16_t* dy, const uint16_t* x, const uint16_t* w
     p.N = N;
     p.act = static_cast<uint32_t>(activation);
     p.rows_per_block = ceil_div(M, row_blocks);
-    const bool vec = N % 8 == 0 && row_vec(dy, lddy) != 0 && (z == nullptr || row_vec(z, ldz) != 0);
+    const bool vec = N % 8 == 0 && rows_aligned16(dy, lddy) && (z == nullptr || rows_aligned16(z, ldz));
     const dim3 grid(ceil_div(N, LB::kColsPerBlock), row_blocks, 1);
     cudaError_t e = vec ? launch_grid(LB::linear_dz_kernel<true>, grid, LB::kThreads, 0, stream, p)
                         : launch_grid(LB::linear_dz_kernel<false>, grid, LB::kThreads, 0, stream, p);

@@ -19,9 +19,15 @@
 // inside the last step are overwritten with zeros in shared memory, in both operands, by a warp
 // of each CTA between the load's arrival and the product.
 //
+// SPLIT: problems with fewer tiles than pairs. A cluster of two pairs (or more) takes one tile, its pairs
+// the contraction in equal parts; each CTA then leaves its sums in its ring's shared memory, and
+// pair i finishes the i-th part of the columns, adding the parts in order through distributed
+// shared memory (the result does not depend on timing).
+//
 // Roles (384 threads per CTA): warp 0 TMA producer, warp 1 UMMA issuer (rank 0), warp 2 TMEM
 // owner, warp 3 zeroes a group's tail, warps 4-11 epilogue: two warpgroups take 32 columns in
-// turn, a thread owns one output row and stores 32 columns as two 32-byte sectors.
+// turn; a thread owns one output row, and a warp's 32 x 32 piece goes out by TMA through shared
+// memory (the residual comes in the same way, one piece ahead).
 #pragma once
 
 #include "gemm_bf16_pair.cuh"
@@ -46,6 +52,7 @@ constexpr uint32_t kStageBytes = 2 * kOperandBytes;  // A + B of one CTA
 struct alignas(1024) Smem {
   uint8_t a[kStages][kOperandBytes];
   uint8_t b[kStages][kOperandBytes];
+  uint8_t piece[kEpiWarps][2][lin::kWarpTileBytes];
   uint64_t full[kStages];        // rank 0: both CTAs' bytes of a stage
   uint64_t empty[kStages];       // each CTA: the pair's UMMAs consumed its stage
   uint64_t tail_full[kStages];   // each CTA: its own bytes of a group's tail block
@@ -53,15 +60,20 @@ struct alignas(1024) Smem {
   uint64_t tmem_full[2];
   uint64_t tmem_empty[2];
   uint64_t drain;
+  uint64_t piece_in[kEpiWarps][2];  // a residual piece landed
   uint32_t tmem_base;
   uint32_t abort;
 };
 constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
+static_assert(kStages * kOperandBytes * 2 >= kTile * kRowsPerCta * 4, "a CTA's sums fit in its ring");
 static_assert(kSmemBytes <= 232448, "shared memory fits in 227 KB");
 
 struct Params {
   CUtensorMap tm_a;  // 3-D, SW128: K-major {K, M, E} box {64, 128, 1}; MN-major {M, K, E} box {64, 64, 1}
   CUtensorMap tm_b;  // likewise, with N in the place of M
+  // Pieces of 32 x 32, 3-D {N, M, E}, SW64, where tma_* says so.
+  CUtensorMap tm_out, tm_z, tm_res;
+  uint32_t tma_out, tma_z, tma_res;
   uint16_t* out;
   uint64_t ldo;        // elements between output rows
   uint64_t out_group;  // contraction mode: elements between the groups' outputs
@@ -69,6 +81,7 @@ struct Params {
   lin::Epilogue epi;
   uint32_t M, N;       // output rows (of a group) and columns
   uint32_t tiles_m, tiles_n, num_kb;
+  uint32_t splits;     // SPLIT: pairs per cluster
 };
 
 // One tile of the walk.
@@ -77,12 +90,14 @@ struct Tile {
   uint32_t m0, n0;
   uint32_t k0;          // first contraction row
   uint32_t num_kb;      // blocks of 64
+  uint32_t kb0, kb1;    // this pair's
   uint32_t last_steps;  // UMMA steps of the last block (4 unless a group ends inside it)
   uint32_t tail_rows;   // valid rows of the last block if it needs zeroing, else 0
 };
 
-template <bool ALONG_K>
-__device__ __forceinline__ bool tile_at(const Params& p, uint32_t t, Tile& w) {
+// `part`: this pair's part of the contraction (SPLIT).
+template <bool ALONG_K, bool SPLIT>
+__device__ __forceinline__ bool tile_at(const Params& p, uint32_t t, uint32_t part, Tile& w) {
   const uint32_t per = p.tiles_m * p.tiles_n;
   w.e = 0;
   w.k0 = 0;
@@ -109,17 +124,125 @@ __device__ __forceinline__ bool tile_at(const Params& p, uint32_t t, Tile& w) {
   const uint32_t m_cnt = min(kBandM, p.tiles_m - m_first);
   w.m0 = (m_first + rem % m_cnt) * kTile;
   w.n0 = rem / m_cnt * kTile;
+  w.kb0 = SPLIT ? w.num_kb * part / p.splits : 0u;
+  w.kb1 = SPLIT ? w.num_kb * (part + 1u) / p.splits : w.num_kb;
   return true;
 }
 
-template <bool A_MN, bool B_MN, bool ALONG_K>
+// One warp's way to memory: its two pieces in turn.
+struct Pieces {
+  uint8_t (*buf)[lin::kWarpTileBytes];
+  uint64_t* in;     // barriers of residual loads
+  uint32_t next;    // piece to use next
+  uint32_t phases;  // parity of each piece's next residual load
+  bool asked;       // the residual's piece is on its way into `next`
+};
+
+// The piece to use next is free once all stores but the last have read theirs.
+__device__ __forceinline__ void piece_claim(uint32_t lane) {
+  if (lane == 0) tma_store_wait_read<1>();
+  __syncwarp();
+}
+
+// A 32 x 32 piece (row `lane` in v) from the registers to rows m.., columns n.. of a matrix.
+__device__ __forceinline__ void piece_store(Pieces& b, const float (&v)[32], const CUtensorMap* map, uint32_t tma,
+                                            uint16_t* p, uint64_t ld, uint32_t rows, uint32_t cols, uint32_t n,
+                                            uint32_t m, uint32_t e, uint32_t lane) {
+  uint32_t packed[16];
+#pragma unroll
+  for (uint32_t i = 0; i < 16; ++i) packed[i] = pack_bf16x2(v[2 * i], v[2 * i + 1]);
+  uint8_t* tile = b.buf[b.next];
+  lin::warp_tile_put(tile, packed);
+  if (tma) {
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) {
+      tma_store_3d(map, tile, int32_t(n), int32_t(m), int32_t(e));
+      tma_store_commit();
+    }
+  } else {
+    __syncwarp();
+    lin::warp_tile_to_rows(tile, p, ld, rows, cols);
+    fence_proxy_async_smem();  // a residual's load may be the next to write here
+    __syncwarp();
+    if (lane == 0) tma_store_commit();  // an empty group: every piece counts as one
+  }
+  b.next ^= 1u;
+}
+
+// Ask for the residual's piece at (m, n), which the piece to use next will hold.
+__device__ __forceinline__ void piece_ask(const Params& p, Pieces& b, uint32_t n, uint32_t m, uint32_t lane) {
+  piece_claim(lane);
+  if (lane == 0) {
+    mbar_arrive_expect_tx(&b.in[b.next], lin::kWarpTileBytes);
+    tma_load_3d(&p.tm_res, &b.in[b.next], b.buf[b.next], int32_t(n), int32_t(m), 0, kCacheEvictNormal);
+  }
+  b.asked = true;
+}
+
+// 32 x 32 sums of a warp (lane = output row m + lane) from column n on, through the epilogue and
+// out. False if a wait was abandoned.
+template <bool ALONG_K>
+__device__ __forceinline__ bool finish_piece(const Params& p, Pieces& b, float (&v)[32], uint32_t m, uint32_t n,
+                                             uint32_t e, volatile uint32_t* abort, uint32_t lane) {
+  const uint32_t rows = min(32u, p.M - m), cols = min(32u, p.N - n);
+  if (!ALONG_K) {
+    if (p.epi.bias != nullptr) {
+      uint32_t c[16];
+      lin::load_row32(p.epi.bias + n, c, cols, p.epi.wide_bias);
+#pragma unroll
+      for (uint32_t i = 0; i < 16; ++i) {
+        v[2 * i] += __uint_as_float(c[i] << 16);
+        v[2 * i + 1] += __uint_as_float(c[i] & 0xFFFF0000u);
+      }
+    }
+    if (p.epi.z != nullptr) {
+      piece_claim(lane);
+      piece_store(b, v, &p.tm_z, p.tma_z, p.epi.z + size_t(m) * p.epi.ldz + n, p.epi.ldz, rows, cols, n, m, 0, lane);
+    }
+    lin::activate(v, p.epi.act);
+  }
+  if (!ALONG_K && p.epi.residual != nullptr) {
+    uint32_t c[16];
+    if (p.tma_res) {
+      if (!b.asked) piece_ask(p, b, n, m, lane);
+      if (!__all_sync(0xffffffffu, mbar_wait(&b.in[b.next], (b.phases >> b.next) & 1u, abort, kStatusTimeoutEpilogue))) {
+        return false;
+      }
+      b.asked = false;
+      b.phases ^= 1u << b.next;
+    } else {
+      piece_claim(lane);
+      lin::warp_tile_from_rows(b.buf[b.next], p.epi.residual + size_t(m) * p.epi.ldr + n, p.epi.ldr, rows, cols);
+      __syncwarp();
+    }
+    lin::warp_tile_get(b.buf[b.next], c);
+#pragma unroll
+    for (uint32_t i = 0; i < 16; ++i) {
+      v[2 * i] += __uint_as_float(c[i] << 16);
+      v[2 * i + 1] += __uint_as_float(c[i] & 0xFFFF0000u);
+    }
+  } else {
+    piece_claim(lane);
+  }
+  piece_store(b, v, &p.tm_out, p.tma_out, p.out + (ALONG_K ? size_t(e) * p.out_group : 0u) + size_t(m) * p.ldo + n,
+              p.ldo, rows, cols, n, m, e, lane);
+  return true;
+}
+
+template <bool A_MN, bool B_MN, bool ALONG_K, bool SPLIT>
 __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __grid_constant__ Params p) {
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem& s = *reinterpret_cast<Smem*>(smem_raw + smem_align_pad(smem_raw));
   const uint32_t warp = warp_idx_sync();
   const uint32_t lane = threadIdx.x & 31u;
-  const uint32_t rank = cluster_ctarank();
-  const uint32_t pair = blockIdx.x >> 1, num_pairs = gridDim.x >> 1;
+  // rank: CTA of the pair; lead: the pair's first CTA in the cluster. Without SPLIT a cluster is a pair
+  // that walks over tiles, with it a cluster takes one tile.
+  const uint32_t rank = cluster_ctarank() & 1u;
+  const uint32_t lead = SPLIT ? cluster_ctarank() - rank : 0u, part = lead >> 1;
+  const uint32_t per_cluster = SPLIT ? 2u * p.splits : 2u;
+  const uint32_t pair = blockIdx.x / per_cluster, num_pairs = gridDim.x / per_cluster;
+  const uint16_t both = static_cast<uint16_t>(0x3u << lead);
   volatile uint32_t* abort = &s.abort;
 
   if (warp == 0 && lane == 0) {
@@ -136,6 +259,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       mbar_init(&s.tmem_empty[i], 2 * kEpiWarps);  // of both CTAs
     }
     mbar_init(&s.drain, 1);
+    for (uint32_t i = 0; i < 2 * kEpiWarps; ++i) mbar_init(&s.piece_in[i >> 1][i & 1u], 1);
     s.abort = 0;
     fence_barrier_init();
   }
@@ -153,6 +277,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
   pdl_launch_dependents();
   const uint32_t tmem_base = s.tmem_base;
 
+  const uint32_t epi_warp = warp >= 4 ? warp - 4u : 0u;
+  Pieces pieces = {s.piece[epi_warp], s.piece_in[epi_warp], 0u, 0u, false};
   if (warp == 0) {
     // ------------------------------------------------------------ TMA producer
     if (lane == 0) {
@@ -161,8 +287,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       const uint32_t row0 = rank * kRowsPerCta;
       Tile w;
       bool ok = true;
-      for (uint32_t t = pair; ok && tile_at<ALONG_K>(p, t, w); t += num_pairs) {
-        for (uint32_t kb = 0; kb < w.num_kb; ++kb) {
+      for (uint32_t t = pair; ok && (tile_at<ALONG_K, SPLIT>(p, t, part, w)); t += num_pairs) {
+        for (uint32_t kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait(&s.empty[stage], phase ^ 1u, abort, kStatusTimeoutProducer)) {
             ok = false;
             break;
@@ -170,12 +296,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
           const bool tail = ALONG_K && w.tail_rows != 0u && kb + 1u == w.num_kb;
           uint32_t bar;
           if (tail) {
-            bar = map_to_rank(&s.tail_full[stage], rank);
+            bar = map_to_rank(&s.tail_full[stage], lead + rank);
             mbar_arrive_expect_tx(&s.tail_full[stage], kStageBytes);
             is_tail |= 1u << stage;
             tail_parity ^= 1u << stage;
           } else {
-            bar = map_to_rank(&s.full[stage], 0);
+            bar = map_to_rank(&s.full[stage], lead);
             if (rank == 0) mbar_arrive_expect_tx(&s.full[stage], 2 * kStageBytes);
             is_tail &= ~(1u << stage);
           }
@@ -222,15 +348,15 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       uint32_t stage = 0, phase = 0, local = 0;
       bool ok = true;
       Tile w;
-      for (uint32_t t = pair; ok && tile_at<ALONG_K>(p, t, w); t += num_pairs) {
-        if (w.num_kb == 0u) continue;  // a group without rows: the epilogue stores zeros
+      for (uint32_t t = pair; ok && (tile_at<ALONG_K, SPLIT>(p, t, part, w)); t += num_pairs) {
+        if (w.kb0 == w.kb1) continue;  // nothing to multiply: the epilogue takes zeros
         const uint32_t acc = local & 1u;
         const uint32_t acc_phase = (local >> 1) & 1u;
         ++local;
         if (!__all_sync(0xffffffffu, mbar_wait(&s.tmem_empty[acc], acc_phase ^ 1u, abort, kStatusTimeoutMma))) break;
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + acc * kTile;
-        for (uint32_t kb = 0; kb < w.num_kb; ++kb) {
+        for (uint32_t kb = w.kb0; kb < w.kb1; ++kb) {
           if (!__all_sync(0xffffffffu, mbar_wait(&s.full[stage], phase, abort, kStatusTimeoutMma))) {
             ok = false;
             break;
@@ -243,20 +369,20 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
           for (uint32_t k = 0; k < BK / kUmmaK; ++k) {
             if (leader && (!ALONG_K || k < steps)) {
               umma_bf16_pair(d_tmem, desc_advance(adesc, k * lin::operand_step<A_MN>()),
-                             desc_advance(bdesc, k * lin::operand_step<B_MN>()), idesc, (kb | k) != 0u ? 1u : 0u);
+                             desc_advance(bdesc, k * lin::operand_step<B_MN>()), idesc, kb != w.kb0 || k != 0u ? 1u : 0u);
             }
           }
-          if (leader) umma_commit_pair(&s.empty[stage], 0x3);
+          if (leader) umma_commit_pair(&s.empty[stage], both);
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
           }
         }
-        if (ok && leader) umma_commit_pair(&s.tmem_full[acc], 0x3);
+        if (ok && leader) umma_commit_pair(&s.tmem_full[acc], both);
       }
       // Every pair UMMA must retire before either CTA releases TMEM or exits.
       if (leader) {
-        umma_commit_pair(&s.drain, 0x1);
+        umma_commit_pair(&s.drain, static_cast<uint16_t>(0x1u << lead));
         mbar_drain(&s.drain, 0);
       }
       __syncwarp();
@@ -267,11 +393,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       uint32_t stage = 0, parity = 0;  // parity: per stage, of its next tail
       Tile w;
       bool ok = true;
-      for (uint32_t t = pair; ok && tile_at<ALONG_K>(p, t, w); t += num_pairs) {
-        if (w.num_kb == 0u) continue;
-        const uint32_t st = (stage + w.num_kb - 1u) % kStages;
-        stage = (stage + w.num_kb) % kStages;
-        if (w.tail_rows == 0u) continue;
+      for (uint32_t t = pair; ok && (tile_at<ALONG_K, SPLIT>(p, t, part, w)); t += num_pairs) {
+        if (w.kb0 == w.kb1) continue;
+        const uint32_t st = (stage + w.kb1 - w.kb0 - 1u) % kStages;
+        stage = (stage + w.kb1 - w.kb0) % kStages;
+        if (w.tail_rows == 0u || w.kb1 != w.num_kb) continue;
         const uint32_t par = (parity >> st) & 1u;
         ok = __all_sync(0xffffffffu, mbar_wait(&s.tail_full[st], par, abort, kStatusTimeoutScales));
         if (!ok) break;
@@ -288,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
         __syncwarp();
         if (lane == 0) {
           if (rank == 1) {
-            mbar_arrive_cluster(map_to_rank(&s.tail_fixed[st], 0));
+            mbar_arrive_cluster(map_to_rank(&s.tail_fixed[st], lead));
           } else if (mbar_wait_cluster(&s.tail_fixed[st], par, abort, kStatusTimeoutScales)) {
             mbar_arrive(&s.full[st]);
           }
@@ -302,97 +428,110 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     const uint32_t q = warp & 3u;
     const uint32_t wg = (warp - 4u) >> 2;
     const uint32_t row = q * 32 + lane;
-    const uint32_t empty0[2] = {map_to_rank(&s.tmem_empty[0], 0), map_to_rank(&s.tmem_empty[1], 0)};
+    const uint32_t empty0[2] = {map_to_rank(&s.tmem_empty[0], lead), map_to_rank(&s.tmem_empty[1], lead)};
     uint32_t local = 0;
+    bool ok = true;
     Tile w;
-    for (uint32_t t = pair; tile_at<ALONG_K>(p, t, w); t += num_pairs) {
-      const uint32_t m = w.m0 + rank * kRowsPerCta + row;
-      const bool valid = m < p.M;
-      uint16_t* out = p.out + (ALONG_K ? size_t(w.e) * p.out_group : 0u) + size_t(valid ? m : 0u) * p.ldo;
-      if (ALONG_K && w.num_kb == 0u) {
-        const uint32_t zero[16] = {0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u, 0u};
-#pragma unroll 1
-        for (uint32_t n = w.n0 + wg * 32u; n < min(w.n0 + kTile, p.N) && valid; n += 64u) {
-          lin::store_row32(out + n, zero, p.N - n, p.epi.vec_out);
-        }
-        __syncwarp();
-        continue;
-      }
+    for (uint32_t t = pair; (tile_at<ALONG_K, SPLIT>(p, t, part, w)); t += num_pairs) {
+      const bool any = w.kb0 != w.kb1;
       const uint32_t acc = local & 1u;
       const uint32_t acc_phase = (local >> 1) & 1u;
-      ++local;
-      // The residual comes from memory: its first columns are asked for before the wait, the
-      // next ones while the present are worked on.
-      const bool with_residual = !ALONG_K && p.epi.residual != nullptr && valid;
-      const uint16_t* residual = p.epi.residual + (with_residual ? size_t(m) * p.epi.ldr : 0u);
-      uint32_t res[16];
-      if (with_residual && w.n0 + wg * 32u < p.N) {
-        lin::load_row32(residual + w.n0 + wg * 32u, res, p.N - (w.n0 + wg * 32u), p.epi.vec_residual);
-      }
-      if (!__all_sync(0xffffffffu, mbar_wait(&s.tmem_full[acc], acc_phase, abort, kStatusTimeoutEpilogue))) break;
-      tc_fence_after_sync();
+      if (any) ++local;
       const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * kTile;
+      if constexpr (SPLIT) {
+        // This CTA's sums, column by column, into its ring: every load and product has ended.
+        if (any) {
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.tmem_full[acc], acc_phase, abort, kStatusTimeoutEpilogue));
+          if (!ok) break;
+          tc_fence_after_sync();
+        }
+        float* sums = reinterpret_cast<float*>(s.a[0]) + row;
+#pragma unroll 1
+        for (uint32_t c = wg; c < kTile / 32u; c += 2u) {
+          uint32_t r[32];
+          if (any) {
+            tmem_ld_32x32b_x32(t_row + c * 32u, r);
+            tmem_ld_wait();
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < 32; ++i) sums[(c * 32u + i) * kRowsPerCta] = any ? __uint_as_float(r[i]) : 0.f;
+        }
+        continue;
+      }
+      const uint32_t m = w.m0 + rank * kRowsPerCta + q * 32u;  // the warp's first row
+      if (ALONG_K && !any) {  // a group without rows
+        float zero[32];
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i) zero[i] = 0.f;
+        for (uint32_t n = w.n0 + wg * 32u; m < p.M && n < min(w.n0 + kTile, p.N); n += 64u) {
+          finish_piece<ALONG_K>(p, pieces, zero, m, n, w.e, abort, lane);
+        }
+        continue;
+      }
+      // The residual comes from memory: its first piece is asked for before the wait, the next
+      // ones while the present is worked on (a pre-activation that also goes out takes turns on
+      // the same pieces, which leaves none to ask ahead for).
+      const bool ahead = !ALONG_K && p.epi.residual != nullptr && p.tma_res && p.epi.z == nullptr && m < p.M;
+      if (ahead && w.n0 + wg * 32u < p.N) piece_ask(p, pieces, w.n0 + wg * 32u, m, lane);
+      ok = __all_sync(0xffffffffu, mbar_wait(&s.tmem_full[acc], acc_phase, abort, kStatusTimeoutEpilogue));
+      if (!ok) break;
+      tc_fence_after_sync();
 #pragma unroll 1
       for (uint32_t c = wg; c < kTile / 32u; c += 2u) {
         const uint32_t n = w.n0 + c * 32u;
-        const uint32_t cols = n < p.N ? p.N - n : 0u;  // columns in range (more than 32: all)
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_row + c * 32u, r);
-        const bool live = valid && cols != 0u;
         tmem_ld_wait();
         if (c + 2u >= kTile / 32u) {
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(empty0[acc]);
         }
-        if (live) {
-          uint32_t packed[16];
-          if (!ALONG_K) {
-            if (p.epi.bias != nullptr) {
-              uint32_t b[16];
-              lin::load_row32(p.epi.bias + n, b, cols, p.epi.vec_bias);
+        if (m < p.M && n < p.N && ok) {
+          float v[32];
 #pragma unroll
-              for (uint32_t i = 0; i < 16; ++i) {
-                r[2 * i] = __float_as_uint(__uint_as_float(r[2 * i]) + __uint_as_float(b[i] << 16));
-                r[2 * i + 1] = __float_as_uint(__uint_as_float(r[2 * i + 1]) + __uint_as_float(b[i] & 0xFFFF0000u));
-              }
-            }
-            if (p.epi.z != nullptr) {
-#pragma unroll
-              for (uint32_t i = 0; i < 16; ++i) {
-                packed[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-              }
-              lin::store_row32(p.epi.z + size_t(m) * p.epi.ldz + n, packed, cols, p.epi.vec_z);
-            }
-            float v[32];
-#pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
-            lin::activate(v, p.epi.act);
-#pragma unroll
-            for (uint32_t i = 0; i < 32; ++i) r[i] = __float_as_uint(v[i]);
-            if (with_residual) {
-#pragma unroll
-              for (uint32_t i = 0; i < 16; ++i) {
-                r[2 * i] = __float_as_uint(__uint_as_float(r[2 * i]) + __uint_as_float(res[i] << 16));
-                r[2 * i + 1] = __float_as_uint(__uint_as_float(r[2 * i + 1]) + __uint_as_float(res[i] & 0xFFFF0000u));
-              }
-              const uint32_t n2 = n + 64u;
-              if (c + 2u < kTile / 32u && n2 < p.N) {
-                lin::load_row32(residual + n2, res, p.N - n2, p.epi.vec_residual);
-              }
-            }
-          }
-#pragma unroll
-          for (uint32_t i = 0; i < 16; ++i) {
-            packed[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
-          }
-          lin::store_row32(out + n, packed, cols, p.epi.vec_out);
+          for (uint32_t i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
+          ok = finish_piece<ALONG_K>(p, pieces, v, m, n, w.e, abort, lane);
+          if (ok && ahead && c + 2u < kTile / 32u && n + 64u < p.N) piece_ask(p, pieces, n + 64u, m, lane);
         }
-        __syncwarp();
       }
+      if (!ok) break;
     }
   }
 
+  if constexpr (SPLIT) {
+    __syncwarp();
+    cluster_sync_all();  // every part's sums are in its shared memory
+    Tile w;
+    if (warp >= 4 && (tile_at<ALONG_K, SPLIT>(p, pair, part, w)) && *abort == 0u) {
+      const uint32_t row = (warp & 3u) * 32u + lane;
+      const uint32_t m = w.m0 + rank * kRowsPerCta + (warp & 3u) * 32u;  // the warp's first row
+      const uint32_t first = kTile / p.splits * part, last = first + kTile / p.splits;
+      bool ok = m < p.M;
+#pragma unroll 1
+      for (uint32_t c = first + ((warp - 4u) >> 2) * 32u; c < last && w.n0 + c < p.N && ok; c += 64u) {
+        float v[32];
+#pragma unroll
+        for (uint32_t i = 0; i < 32; ++i) v[i] = 0.f;
+        const float* sums = reinterpret_cast<const float*>(s.a[0]) + c * kRowsPerCta + row;
+        for (uint32_t j = 0; j < p.splits; ++j) {
+          const uint32_t from = map_to_rank(sums, 2u * j + rank);
+#pragma unroll
+          for (uint32_t i = 0; i < 32; ++i) v[i] += ld_dsmem_f32(from + i * (kRowsPerCta * 4u));
+        }
+        ok = finish_piece<ALONG_K>(p, pieces, v, m, w.n0 + c, w.e, abort, lane);
+      }
+    }
+    __syncwarp();
+  }
+
+  // Pieces on their way in have landed and those on their way out are written before the CTA may
+  // exit (a load is under way here only if a wait was abandoned).
+  if (warp >= 4 && lane == 0) {
+    if (pieces.asked) mbar_drain(&pieces.in[pieces.next], (pieces.phases >> pieces.next) & 1u);
+    tma_store_wait_all<0>();
+  }
+  __syncwarp();
   // Both CTAs stay resident until the pair's last UMMA retired (rank 0's drain) and both
   // epilogues finished with TMEM; then each frees its TMEM columns.
   tc_fence_before_sync();

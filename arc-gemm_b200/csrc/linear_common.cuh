@@ -246,51 +246,12 @@ __device__ __forceinline__ void load_columns_finish(const uint32_t (&raw)[N], fl
   }
 }
 
-// ---------------------------------------------------------------------------------
-// 32 consecutive bf16 columns of one row, of which `cols` are in range. `vec` is the widest
-// access every row allows: 2 = 32 bytes, 1 = 16 bytes, 0 = single elements (the host derives
-// it from the base address and the leading dimension). Full vectors go out wide, the ragged
-// end element by element.
-// ---------------------------------------------------------------------------------
-__device__ __forceinline__ void st_global_32b(void* p, const uint32_t* v) {
-  asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(p), "r"(v[0]), "r"(v[1]),
-               "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
-               : "memory");
-}
-
-__device__ __forceinline__ void ld_global_32b(const void* p, uint32_t* v) {
-  asm volatile("ld.global.v8.b32 {%0, %1, %2, %3, %4, %5, %6, %7}, [%8];"
-               : "=r"(v[0]), "=r"(v[1]), "=r"(v[2]), "=r"(v[3]), "=r"(v[4]), "=r"(v[5]), "=r"(v[6]),
-                 "=r"(v[7])
-               : "l"(p)
-               : "memory");
-}
-
-__device__ __forceinline__ void store_row32(uint16_t* p, const uint32_t (&v)[16], uint32_t cols, uint32_t vec) {
-  if (vec == 2u && cols >= 32u) {
-    st_global_32b(p, v);
-    st_global_32b(p + 16, v + 8);
-  } else if (vec != 0u && cols >= 32u) {
+// 32 consecutive bf16 values, the same for all lanes, of which `cols` exist; `wide`: 16-byte aligned.
+__device__ __forceinline__ void load_row32(const uint16_t* p, uint32_t (&v)[16], uint32_t cols, uint32_t wide) {
+  if (wide != 0u && cols >= 32u) {
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
-      *reinterpret_cast<uint4*>(p + 8 * j) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
-    }
-  } else {
-#pragma unroll
-    for (uint32_t j = 0; j < 32; ++j) {
-      if (j < cols) p[j] = static_cast<uint16_t>(v[j >> 1] >> ((j & 1u) * 16u));
-    }
-  }
-}
-
-__device__ __forceinline__ void load_row32(const uint16_t* p, uint32_t (&v)[16], uint32_t cols, uint32_t vec) {
-  if (vec == 2u && cols >= 32u) {
-    ld_global_32b(p, v);
-    ld_global_32b(p + 16, v + 8);
-  } else if (vec != 0u && cols >= 32u) {
-#pragma unroll
-    for (uint32_t j = 0; j < 4; ++j) {
-      const uint4 x = *reinterpret_cast<const uint4*>(p + 8 * j);
+      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p + 8 * j));
       v[4 * j] = x.x;
       v[4 * j + 1] = x.y;
       v[4 * j + 2] = x.z;
@@ -301,8 +262,62 @@ __device__ __forceinline__ void load_row32(const uint16_t* p, uint32_t (&v)[16],
     for (uint32_t j = 0; j < 16; ++j) v[j] = 0u;
 #pragma unroll
     for (uint32_t j = 0; j < 32; ++j) {
-      if (j < cols) v[j >> 1] |= static_cast<uint32_t>(p[j]) << ((j & 1u) * 16u);
+      if (j < cols) v[j >> 1] |= static_cast<uint32_t>(__ldg(p + j)) << ((j & 1u) * 16u);
     }
+  }
+}
+
+// ---------------------------------------------------------------------------------
+// A warp's 32 x 32 bf16 tile in shared memory (2 KB, 64-byte rows in the 64-byte swizzle of a
+// TMA box {32, 32}): lane = row on the side of the registers; on the side of memory TMA moves
+// it whole, or the warp row by row where the matrix has no 16-byte aligned rows. Straight from
+// registers every lane would touch a line of its own, and the load-store unit would take longer
+// than a short contraction's products.
+// ---------------------------------------------------------------------------------
+constexpr uint32_t kWarpTileBytes = 32 * 64;
+
+__device__ __forceinline__ uint8_t* warp_tile_piece(uint8_t* tile, uint32_t row, uint32_t j) {
+  return tile + row * 64u + ((j ^ ((row >> 1) & 3u)) << 4);
+}
+
+__device__ __forceinline__ void warp_tile_put(uint8_t* tile, const uint32_t (&v)[16]) {
+  const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    *reinterpret_cast<uint4*>(warp_tile_piece(tile, lane, j)) = make_uint4(v[4 * j], v[4 * j + 1], v[4 * j + 2], v[4 * j + 3]);
+  }
+}
+
+__device__ __forceinline__ void warp_tile_get(const uint8_t* tile, uint32_t (&v)[16]) {
+  const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll
+  for (uint32_t j = 0; j < 4; ++j) {
+    const uint4 x = *reinterpret_cast<const uint4*>(warp_tile_piece(const_cast<uint8_t*>(tile), lane, j));
+    v[4 * j] = x.x;
+    v[4 * j + 1] = x.y;
+    v[4 * j + 2] = x.z;
+    v[4 * j + 3] = x.w;
+  }
+}
+
+// Row by row, a lane per column; `rows` and `cols` of the tile lie in the matrix.
+__device__ __forceinline__ void warp_tile_to_rows(const uint8_t* tile, uint16_t* p, uint64_t ld, uint32_t rows,
+                                                  uint32_t cols) {
+  const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll 8
+  for (uint32_t r = 0; r < 32u; ++r) {
+    const uint8_t* at = warp_tile_piece(const_cast<uint8_t*>(tile), r, lane >> 3) + (lane & 7u) * 2u;
+    if (r < rows && lane < cols) p[size_t(r) * ld + lane] = *reinterpret_cast<const uint16_t*>(at);
+  }
+}
+
+__device__ __forceinline__ void warp_tile_from_rows(uint8_t* tile, const uint16_t* p, uint64_t ld, uint32_t rows,
+                                                    uint32_t cols) {
+  const uint32_t lane = threadIdx.x & 31u;
+#pragma unroll 8
+  for (uint32_t r = 0; r < 32u; ++r) {
+    const uint16_t v = r < rows && lane < cols ? p[size_t(r) * ld + lane] : uint16_t(0);
+    *reinterpret_cast<uint16_t*>(warp_tile_piece(tile, r, lane >> 3) + (lane & 7u) * 2u) = v;
   }
 }
 
@@ -314,8 +329,8 @@ struct Epilogue {
   uint16_t* z;               // [M][ldz] or null: x w^T + bias, bf16
   uint64_t ldr, ldz;
   uint32_t act;
-  uint32_t vec_bias, vec_residual, vec_z, vec_out;      // row-wise access (store_row32)
-  uint32_t pair_residual, pair_z, pair_out;             // column-wise access (store_columns)
+  uint32_t wide_bias;                           // 16-byte aligned
+  uint32_t pair_residual, pair_z, pair_out;     // column-wise access (store_columns)
 };
 
 // Shared-memory descriptor of an MN-major operand as a TMA load with the 128-byte swizzle

@@ -13,7 +13,7 @@ pytestmark = pytest.mark.gpu
 # Rows of each group, rows behind the last one.
 SPLITS = [([5], 0), ([0, 0, 0], 4), ([1, 0, 1], 0), ([16, 17, 0, 15, 33], 3), ([0, 130, 300, 1, 0], 9),
           ([64, 64, 64, 64], 0), ([257, 63, 16, 48, 15, 1], 2)]
-PLANS = ["pair", "16:1", "16:2", "32:1", "64:4", "128:1", "128:8"]
+PLANS = ["pair:1", "16:1", "16:2", "32:1", "64:4", "128:1", "128:8"]
 
 
 def _offsets(sizes):
@@ -67,7 +67,7 @@ def test_grouped_forward(cuda_device, monkeypatch, plan, sizes, behind, n, k):
     assert arc.device_status(0) == 0
 
 
-@pytest.mark.parametrize("plan", [None, "pair", "16:2", "64:1"])
+@pytest.mark.parametrize("plan", [None, "pair:1", "16:2", "64:1"])
 @pytest.mark.parametrize("sizes,behind", SPLITS)
 @pytest.mark.parametrize("n,k", [(136, 200), (77, 320)])
 def test_grouped_gradients(cuda_device, monkeypatch, plan, sizes, behind, n, k):
@@ -135,7 +135,7 @@ def test_grouped_layouts(cuda_device):
     assert arc.grouped_matmul(x[:0], w, torch.zeros(4, dtype=torch.int32, device="cuda")).shape == (0, 37)
 
 
-@pytest.mark.parametrize("plan", [None, "pair", "16:1"])
+@pytest.mark.parametrize("plan", [None, "pair:1", "16:1"])
 @pytest.mark.parametrize("n", [96, 33])
 def test_mostly_padding(cuda_device, monkeypatch, plan, n):
     """A buffer of which the groups fill little: the rest is zeroed, or left alone."""

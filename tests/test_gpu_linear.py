@@ -10,7 +10,7 @@ from linear_bounds import act64, assert_within, linear_forward, linear_gradients
 pytestmark = pytest.mark.gpu
 
 ACTS = [None, "relu", "gelu", "gelu_tanh", "silu"]
-PLANS = ["pair", "16:1", "16:4", "32:2", "64:1", "128:8", "128:1"]
+PLANS = ["pair:1", "pair:2", "16:1", "16:4", "32:2", "64:1", "128:8", "128:1"]
 
 
 def _inputs(m, n, k, seed=0, bias=True, residual=True):
@@ -48,7 +48,7 @@ def test_real_sizes(cuda_device, m, n, k):
     _check(m, n, k, "silu")
 
 
-@pytest.mark.parametrize("plan", ["pair", "16:4", "128:1"])
+@pytest.mark.parametrize("plan", ["pair:1", "pair:2", "16:4", "128:1"])
 def test_strided_operands(cuda_device, monkeypatch, plan):
     """Column slices of wider matrices; an output whose rows are not 16-byte aligned."""
     monkeypatch.setenv("ARC_LINEAR_PLAN", plan)
@@ -109,6 +109,28 @@ def test_gradients(cuda_device, m, n, k, act):
     for name, leaf in (("dx", lx), ("dw", lw), ("dbias", lb)):
         assert_within(leaf.grad, *grads[name], f"{name} {act}")
     assert torch.equal(lr.grad, dy)
+    assert arc.device_status(0) == 0
+
+
+@pytest.mark.parametrize("m,n,k", [(300, 264, 136), (1000, 260, 520), (4100, 72, 64), (520, 300, 2056)])
+def test_split_contractions(cuda_device, m, n, k):
+    """Few tiles and long contractions, in every product of a training step; the same bits each time."""
+    x, w, b, _ = _inputs(m, n, k, seed=m, residual=False)
+    dy = normal(torch.Generator().manual_seed(9), m, n)
+    first = None
+    for _ in range(4):
+        leaves = _leaves(x, w, b)
+        y = arc.linear(*leaves, activation="silu")
+        got = (y.detach(), *torch.autograd.grad(y, leaves, dy))
+        if first is None:
+            first = got
+            want, bound, z, zerr = linear_forward(x, w, b, None, "silu")
+            assert_within(got[0], want, bound, "y")
+            grads = linear_gradients(x, w, z, zerr, dy, "silu")
+            for v, name in zip(got[1:], ("dx", "dw", "dbias")):
+                assert_within(v, *grads[name], name)
+        for a, c in zip(got, first):
+            assert torch.equal(a, c)
     assert arc.device_status(0) == 0
 
 
