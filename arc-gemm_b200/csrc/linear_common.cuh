@@ -104,7 +104,10 @@ constexpr float kSqrt2OverPi = 0.79788456080286536f;
 constexpr float kInvSqrt2Pi = 0.39894228040143268f;
 constexpr float kGeluCubic = 0.044715f;
 
-__device__ __forceinline__ float sigmoidf(float z) { return __fdividef(1.f, 1.f + __expf(-z)); }
+constexpr float kLog2E = 1.4426950408889634f;
+
+// 1 / (1 + e^-z); e^-z overflows to infinity, whose reciprocal is the right 0.
+__device__ __forceinline__ float sigmoidf(float z) { return rcp_ftz(1.f + ex2_ftz(-kLog2E * z)); }
 
 // The tanh form's argument. 1 + tanh(u) = 2 sigmoid(2u), which keeps its relative accuracy
 // in the lower tail, where 1 + tanh(u) would cancel.
@@ -112,27 +115,40 @@ __device__ __forceinline__ float gelu_tanh_arg(float z) {
   return 2.f * kSqrt2OverPi * (z + kGeluCubic * z * z * z);
 }
 
-// e = exp(-x^2) and q = 1 - erf(x) for x = |z| / sqrt(2), by formula 7.1.26 of Abramowitz and
-// Stegun (Handbook of Mathematical Functions): q = (a1 t + ... + a5 t^5) e with t = 1 / (1 + p x),
-// off by at most 1.5e-7. The erf form's value and slope need both, and 2 Phi(z) = 1 + erf is q
-// itself below zero, so nothing cancels in the lower tail.
-__device__ __forceinline__ float erfc_of(float z, float& e) {
-  const float x = fabsf(z) * kSqrtHalf;
-  const float t = __fdividef(1.f, fmaf(0.3275911f, x, 1.f));
-  e = __expf(-x * x);
-  const float poly =
-      t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f);
-  return poly * e;
+// The erf form, two values at once: z Phi(z) = max(z, 0) - |z| q / 2 with q = 1 - erf(|z| / sqrt 2),
+// where nothing cancels. q = (1 + a1 x + ... + a6 x^6)^-16 by formula 7.1.28 of Abramowitz and
+// Stegun (Handbook of Mathematical Functions), off by at most 3e-7 (and by 3e-6 of itself in fp32,
+// through the 16th power): one reciprocal and packed products, where the special-function unit
+// would bound a formula with an exponential. x stops at 16, where q has long been 0.
+__device__ __forceinline__ void gelu_pair(float& z0, float& z1) {
+  constexpr float r = kSqrtHalf;  // the formula's argument is |z| r: powers of r go into its factors
+  const float x0 = fminf(fabsf(z0), 16.f), x1 = fminf(fabsf(z1), 16.f);
+  const uint64_t x = f32x2_pack(x0, x1);
+  const auto both = [](float c) { return f32x2_pack(c, c); };
+  uint64_t t = f32x2_fma(x, both(0.0000430638f * r * r * r * r * r * r), both(0.0002765672f * r * r * r * r * r));
+  t = f32x2_fma(x, t, both(0.0001520143f * r * r * r * r));
+  t = f32x2_fma(x, t, both(0.0092705272f * r * r * r));
+  t = f32x2_fma(x, t, both(0.0422820123f * r * r));
+  t = f32x2_fma(x, t, both(0.0705230784f * r));
+  t = f32x2_fma(x, t, both(1.f));
+  t = f32x2_mul(t, t);
+  t = f32x2_mul(t, t);
+  t = f32x2_mul(t, t);
+  t = f32x2_mul(t, t);
+  float p0, p1;
+  f32x2_unpack(t, p0, p1);
+  const uint64_t h = f32x2_mul(x, f32x2_pack(rcp_ftz(p0), rcp_ftz(p1)));
+  f32x2_unpack(f32x2_fma(h, both(-0.5f), f32x2_pack(relu_nan(z0), relu_nan(z1))), z0, z1);
 }
 
 __device__ __forceinline__ float act_value(float z, uint32_t act) {
   switch (act) {
     case kActRelu:
-      return z > 0.f ? z : (z != z ? z : 0.f);
+      return relu_nan(z);
     case kActGelu: {
-      float e;
-      const float q = erfc_of(z, e);
-      return 0.5f * z * (z < 0.f ? q : 2.f - q);
+      float other = 0.f;
+      gelu_pair(z, other);
+      return z;
     }
     case kActGeluTanh:
       return z * sigmoidf(gelu_tanh_arg(z));
@@ -143,15 +159,18 @@ __device__ __forceinline__ float act_value(float z, uint32_t act) {
   }
 }
 
-// d act / d z.
+// d act / d z. The erf form: Phi(z) + z phi(z) with e = exp(-z^2 / 2) and, by formula 7.1.26 of
+// the same book, 1 - erf(x) = (a1 t + ... + a5 t^5) e, t = 1 / (1 + p x), off by at most 1.5e-7.
 __device__ __forceinline__ float act_slope(float z, uint32_t act) {
   switch (act) {
     case kActRelu:
       return z > 0.f ? 1.f : 0.f;
     case kActGelu: {
-      float e;
-      const float q = erfc_of(z, e);
-      return 0.5f * (z < 0.f ? q : 2.f - q) + z * kInvSqrt2Pi * e;
+      const float t = rcp_ftz(fmaf(0.3275911f * kSqrtHalf, fabsf(z), 1.f));
+      const float e = ex2_ftz(-0.5f * kLog2E * z * z);
+      const float q =
+          t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * e;
+      return (z < 0.f ? 0.5f * q : fmaf(-0.5f, q, 1.f)) + z * kInvSqrt2Pi * e;
     }
     case kActGeluTanh: {
       const float s = sigmoidf(gelu_tanh_arg(z));
@@ -174,8 +193,11 @@ __device__ __forceinline__ void activate(float (&v)[N], uint32_t act) {
   case A:                                                                           \
     _Pragma("unroll") for (uint32_t i = 0; i < N; ++i) v[i] = act_value(v[i], A);    \
     break;
+    case kActGelu:
+#pragma unroll
+      for (uint32_t i = 0; i < N; i += 2) gelu_pair(v[i], v[i + 1]);
+      break;
     ARC_ACT_CASE(kActRelu)
-    ARC_ACT_CASE(kActGelu)
     ARC_ACT_CASE(kActGeluTanh)
     ARC_ACT_CASE(kActSilu)
 #undef ARC_ACT_CASE
