@@ -6,6 +6,7 @@
 // errors are returned (never exit()), tensor maps take explicit leading dimensions,
 // and the tile/stage configuration is chosen per shape instead of being fixed at
 // (128,128,128)x3 (arc/mm.py:64).
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>

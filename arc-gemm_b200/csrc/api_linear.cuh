@@ -53,35 +53,116 @@ uint32_t column_pairs(const void* p, uint64_t ld, uint32_t cols) {
   return cols % 2 == 0 && ld % 2 == 0 && (reinterpret_cast<uintptr_t>(p) & 3u) == 0 ? 1u : 0u;
 }
 
-// The kernel for a product of rows, in one group or several.
-//
-// One group: pairs (256 x 256 tiles) when the rows fill half such a tile and there are tiles for
-// half of the pairs. Several groups: the pair kernel's row tile fits itself to the group, so it
-// takes all but the smallest groups (more than 16 rows on average; 64 groups, 2048 x 1024: at 32
-// rows 51 us against the streaming kernel's 70, at 128 57 against 116; 16 groups of 8 rows,
-// 4096 x 4096: 93 against 85).
-//
-// Else the streaming kernel: the row tile is the smallest that holds an average group's rows and
-// the contraction is split over a cluster until the two block slots of every SM have work (at
-// least kStreamMinKb blocks of 64 each). Where that leaves SMs without work (a short
-// contraction), smaller row tiles fill them (1796 x 111 x 448 with a residual: STREAM_FILL).
-//
-// ARC_LINEAR_PLAN="pair:S" | "BN:S" (tests and tuning) forces the choice where it is valid.
-struct LinearPlan {
-  bool pair;
-  uint32_t pair_splits;
-  uint32_t bn, splits, row_tiles;
-};
-
-// Parts of the contraction for `tiles` pair tiles: two where there are pairs for both, with at
-// least kPairMinKb blocks of 64 each. (Four would take clusters of eight CTAs, of which too few
-// fit at once: 512 x 4096 x 4096 25 us whole, 20 in two parts, 48 in four.)
-constexpr uint32_t kPairMinKb = 4;
+// The pair kernel's parts of the contraction: two where there are pairs for both halves of every
+// tile. (Four would take clusters of eight CTAs, of which too few fit at once: 512 x 4096 x 4096
+// 25 us whole, 20 in two parts, 48 in four.)
 uint32_t pair_splits(uint64_t tiles, uint32_t num_kb, uint32_t max_pairs) {
-  return tiles * 2 <= max_pairs && num_kb >= 2 * kPairMinKb ? 2 : 1;
+  return tiles * 2 <= max_pairs && num_kb >= 8 ? 2 : 1;
 }
 
-// The pair kernel, one cluster per tile if the contraction is split.
+// The kernel for a product of rows, in one group or several.
+struct LinearPlan {
+  bool pair;
+  uint32_t pair_splits;            // pair kernel: 1 or 2
+  uint32_t bn, splits, row_tiles;  // streaming kernel: row tile, parts of the contraction
+};
+
+// Estimated time of one group's product: what a launch costs, and per round of blocks what a
+// tile costs besides its contraction blocks of 64 and with them. Only the order of the plans
+// counts; the constants are a fit to the measured times of all plans of 500 products (1 to 4096
+// rows, 64 to 8192 columns, contractions of 64 to 6400). The plan it picks is 2 % behind the best
+// one, geometric mean over those and over 200 others; fixed thresholds on rows and tiles were 14 %.
+double stream_cost(uint32_t rows, uint32_t cols, uint32_t num_kb, uint32_t bn, uint32_t splits, uint32_t sms) {
+  // Two blocks fit on an SM; clusters of four and eight leave some slots empty, and two blocks of
+  // a cluster of two come to lie on one SM.
+  const double slots = 2.0 * sms * (splits == 8 ? 256.0 / 296 : splits == 4 ? 280.0 / 296 : 1.0);
+  const double cluster = splits == 8 ? 0.1 : splits == 4 ? 0.8 : splits == 2 ? 2.44 : 0.0;
+  const double blocks = static_cast<double>(ceil_div(rows, bn)) * ceil_div(cols, LS::kRows) * splits;
+  const double load = blocks < 2.0 * sms ? blocks / (2.0 * sms) : 1.0;
+  const double per_kb = 0.0724 + 0.0033 * (16 + bn / 8.0) * load;  // latency, and a share of the bandwidth
+  const double epilogue = bn / 16.0 * (0.693 / splits + 0.45) + 1.16;
+  return 0.95 + ceil(blocks / slots) * (ceil_div(num_kb, splits) * per_kb + epilogue) + cluster;
+}
+
+double pair_cost(uint32_t rows, uint32_t cols, uint32_t num_kb, uint32_t splits, bool aligned, uint32_t max_pairs) {
+  const double tiles = static_cast<double>(ceil_div(rows, LP::kTile)) * ceil_div(cols, LP::kTile);
+  const double products = ceil_div(num_kb, splits) * 0.0442 + 0.51;
+  const double epilogue = aligned ? 3.17 : 8.78;  // output rows by TMA, or element by element
+  return 4.0 + ceil(tiles * splits / max_pairs) * (products > epilogue ? products : epilogue) + epilogue / splits +
+         (splits > 1 ? 1.37 : 0.0);
+}
+
+// One group: the plan of the least estimated time. Several groups, of which the host knows only the
+// average: the pair kernel's row tile fits itself to the group, so it takes all but the smallest
+// groups (more than 16 rows; 64 groups, 2048 x 1024: at 32 rows 51 us against the streaming
+// kernel's 70, at 128 57 against 116; 16 groups of 8 rows, 4096 x 4096: 93 against 85) where
+// there are tiles for half of the pairs. Else the streaming kernel, its row tile the smallest that
+// holds an average group's rows, with the contraction split over a cluster until the two block
+// slots of every SM have work (four blocks of 64 each at least).
+//
+// ARC_LINEAR_PLAN="pair:S" | "BN:S" (tests and tuning) forces the choice where it is valid.
+int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t num_kb, bool aligned, LinearPlan* plan) {
+  const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
+  const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
+  const uint32_t live = groups < rows ? groups : rows;  // groups that can have rows
+  const uint32_t avg = ceil_div(rows, live);
+  *plan = {false, 1, 16, 1, 0};
+  if (const char* env = getenv("ARC_LINEAR_PLAN")) {
+    unsigned bn = 0, s = 0;
+    if (sscanf(env, "pair:%u", &s) == 1 && max_pairs > 0 && (s == 1 || s == 2)) {
+      plan->pair = true;
+      plan->pair_splits = s <= num_kb ? s : 1;
+    } else if (sscanf(env, "%u:%u", &bn, &s) == 2 && (bn == 16 || bn == 32 || bn == 64 || bn == 128) &&
+               (s == 1 || s == 2 || s == 4 || s == 8)) {
+      plan->bn = bn;
+      plan->splits = s <= num_kb ? s : 1;
+    } else {
+      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_LINEAR_PLAN must be 'pair:S' or 'BN:S' (got '%s')", env);
+    }
+  } else if (groups == 1) {
+    double best = 1e30;
+    for (uint32_t bn : {16u, 32u, 64u, 128u}) {
+      for (uint32_t s : {1u, 2u, 4u, 8u}) {
+        if (s > num_kb) break;
+        const double t = stream_cost(rows, cols, num_kb, bn, s, sms);
+        if (t < best) {
+          best = t;
+          plan->bn = bn;
+          plan->splits = s;
+        }
+      }
+    }
+    for (uint32_t s : {1u, 2u}) {
+      if (max_pairs == 0 || s > num_kb) break;
+      const double t = pair_cost(rows, cols, num_kb, s, aligned, max_pairs);
+      if (t < best) {
+        best = t;
+        plan->pair = true;
+        plan->pair_splits = s;
+      }
+    }
+  } else {
+    const uint64_t pair_tiles = uint64_t(ceil_div(avg, GP::kTileT)) * live * ceil_div(cols, GP::kTileF);
+    plan->pair = max_pairs > 0 && avg > 16 && pair_tiles * 2 > max_pairs;
+    plan->bn = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
+    for (;; plan->bn /= 2) {
+      const uint64_t tiles = uint64_t(live + rows / plan->bn) * ceil_div(cols, LS::kRows);
+      plan->splits = 1;
+      for (uint32_t s : {8u, 4u, 2u}) {
+        if (tiles * s <= 2 * sms && num_kb >= 4 * s) {
+          plan->splits = s;
+          break;
+        }
+      }
+      if (plan->bn == 16 || tiles * plan->splits >= sms) break;
+    }
+  }
+  // With several groups the host knows only a bound: a group of c rows has at most c / bn + 1 tiles.
+  plan->row_tiles = groups == 1 ? ceil_div(rows, plan->bn) : live + rows / plan->bn;
+  return ARC_OK;
+}
+
+// The pair kernel, one cluster of two pairs per tile if the contraction is split.
 template <bool A_MN, bool B_MN, bool ALONG_K>
 cudaError_t launch_linear_pair(LP::Params& p, uint64_t tiles, uint32_t splits, uint32_t max_pairs, cudaStream_t stream) {
   p.splits = splits;
@@ -92,47 +173,6 @@ cudaError_t launch_linear_pair(LP::Params& p, uint64_t tiles, uint32_t splits, u
   const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
   return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, false>, p, grid, LP::kThreads, LP::kSmemBytes, 2,
                    stream);
-}
-constexpr uint32_t kStreamMinKb = 4;
-
-int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t num_kb, LinearPlan* plan) {
-  const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
-  const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
-  const uint32_t live = groups < rows ? groups : rows;  // groups that can have rows
-  const uint32_t avg = ceil_div(rows, live);
-  const uint64_t pair_tiles = uint64_t(ceil_div(avg, LP::kTile)) * live * ceil_div(cols, LP::kTile);
-  plan->pair = max_pairs > 0 && avg > (groups == 1 ? 128u : 16u) && pair_tiles * 2 > max_pairs;
-  plan->pair_splits = groups == 1 ? pair_splits(pair_tiles, num_kb, max_pairs) : 1;
-  plan->bn = avg <= 16 ? 16 : avg <= 32 ? 32 : avg <= 64 ? 64 : 128;
-  uint32_t forced = 0;
-  if (const char* env = getenv("ARC_LINEAR_PLAN")) {
-    unsigned bn = 0, s = 0;
-    if (sscanf(env, "pair:%u", &s) == 1 && max_pairs > 0 && (s == 1 || s == 2)) {
-      plan->pair = true;
-      plan->pair_splits = s <= num_kb ? s : 1;
-    } else if (sscanf(env, "%u:%u", &bn, &s) == 2 && (bn == 16 || bn == 32 || bn == 64 || bn == 128) &&
-               (s == 1 || s == 2 || s == 4 || s == 8)) {
-      plan->pair = false;
-      plan->bn = bn;
-      forced = s;
-    } else {
-      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_LINEAR_PLAN must be 'pair:S' or 'BN:S' (got '%s')", env);
-    }
-  }
-  for (;; plan->bn /= 2) {
-    // With groups the host knows only a bound: a group of c rows has at most c / bn + 1 tiles.
-    plan->row_tiles = groups == 1 ? ceil_div(rows, plan->bn) : live + rows / plan->bn;
-    const uint64_t tiles = uint64_t(plan->row_tiles) * ceil_div(cols, LS::kRows);
-    plan->splits = 1;
-    for (uint32_t s : {8u, 4u, 2u}) {
-      if (forced != 0 ? (s == forced && s <= num_kb) : (tiles * s <= 2 * sms && num_kb >= s * kStreamMinKb)) {
-        plan->splits = s;
-        break;
-      }
-    }
-    if (forced != 0 || plan->bn == 16 || tiles * plan->splits >= sms) break;
-  }
-  return ARC_OK;
 }
 
 template <uint32_t BN, bool W_MN>
@@ -214,7 +254,7 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
   if (int st = current_device(&dev)) return st;
   const uint32_t num_kb = ceil_div(inner, arcb::lin::BK);
   LinearPlan plan;
-  if (int st = linear_plan(dev, groups.rows, groups.num, cols, num_kb, &plan)) return st;
+  if (int st = linear_plan(dev, groups.rows, groups.num, cols, num_kb, rows_aligned16(out, ldo), &plan)) return st;
   const uint64_t w_rows = grad ? inner : cols, w_cols = grad ? cols : inner;
   cudaError_t e;
   const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
@@ -261,7 +301,7 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
     p.tiles_n = ceil_div(cols, LP::kTile);
     p.num_kb = num_kb;
     const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
-    if (tiles > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
+    if (tiles * 4 > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
     e = grad ? launch_linear_pair<false, true, false>(p, tiles, plan.pair_splits, max_pairs, stream)
              : launch_linear_pair<false, false, false>(p, tiles, plan.pair_splits, max_pairs, stream);
     if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
@@ -317,7 +357,7 @@ int linear_dw(const char* what, const uint16_t* dy, const uint16_t* x, const arc
   p.tiles_m = ceil_div(N, LP::kTile);
   p.tiles_n = ceil_div(K, LP::kTile);
   const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n * groups.num;
-  if (tiles > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "%s: too many tiles for one launch", what);
+  if (tiles * 4 > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "%s: too many tiles for one launch", what);
   // The host knows the contraction's length only for one group of all rows.
   const uint32_t splits =
       groups.offsets == nullptr ? pair_splits(tiles, ceil_div(groups.rows, arcb::lin::BK), max_pairs) : 1;
