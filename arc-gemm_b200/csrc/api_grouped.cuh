@@ -144,11 +144,11 @@ int arc_a8w4_grouped_gemm(const int8_t* A, const float* sa, const uint8_t* Wp, c
     const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
     if (max_pairs == 0) return fail(ARC_ERR_UNSUPPORTED, "%s: no CTA pair fits on this device", what);
     const uint64_t pieces = uint64_t(T) * K / 16;
-    const uint64_t want = (pieces + GP::kWidenThreads - 1) / GP::kWidenThreads;
-    const uint64_t cap = uint64_t(g_dev[dev].sms) * 8;
-    cudaError_t e = launch_grid(GP::widen_rows_kernel, dim3(static_cast<uint32_t>(want < cap ? want : cap)),
-                                GP::kWidenThreads, 0, stream, reinterpret_cast<const uint4*>(A),
-                                static_cast<uint4*>(workspace), pieces);
+    const uint64_t per_block = uint64_t(GP::kWidenThreads) * GP::kWidenAhead;
+    const uint64_t blocks = (pieces + per_block - 1) / per_block;
+    if (blocks > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "%s: too many rows for one launch", what);
+    cudaError_t e = launch_grid(GP::widen_rows_kernel, dim3(static_cast<uint32_t>(blocks)), GP::kWidenThreads, 0, stream,
+                                reinterpret_cast<const uint4*>(A), static_cast<uint4*>(workspace), pieces);
     if (e != cudaSuccess) return cuda_fail(e, "widen_rows_kernel launch");
     GP::Params p = {};
     if (int st = encode_codes_3d(&p.tm_w, Wp, K / 2, N, E)) return st;

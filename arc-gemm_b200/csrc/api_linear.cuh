@@ -132,8 +132,8 @@ int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t
         }
       }
     }
-    for (uint32_t s : {1u, 2u}) {
-      if (max_pairs == 0 || s > num_kb) break;
+    const uint64_t tiles = uint64_t(ceil_div(rows, LP::kTile)) * ceil_div(cols, LP::kTile);
+    for (uint32_t s = 1; max_pairs > 0 && s <= pair_splits(tiles, num_kb, max_pairs); ++s) {
       const double t = pair_cost(rows, cols, num_kb, s, aligned, max_pairs);
       if (t < best) {
         best = t;

@@ -504,15 +504,26 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
   }
 }
 
-// int8 rows -> fp16 (exact), the W4 kernel's N operand. HBM-bound: 3 bytes per element.
+// int8 rows -> fp16 (exact), the W4 kernel's N operand. HBM-bound: 3 bytes per element (the result
+// mostly stays in L2 for the product). A thread has kWidenAhead 16-byte loads in flight and stores
+// whole 32-byte sectors.
 constexpr uint32_t kWidenThreads = 256;
+constexpr uint32_t kWidenAhead = 4;
 __global__ void __launch_bounds__(kWidenThreads) widen_rows_kernel(const uint4* src, uint4* dst, uint64_t pieces) {
   pdl_launch_dependents();
   pdl_wait();
-  for (uint64_t i = uint64_t(blockIdx.x) * kWidenThreads + threadIdx.x; i < pieces;
-       i += uint64_t(gridDim.x) * kWidenThreads) {
-    const uint4 x = __ldg(src + i);
-    const uint32_t w[4] = {x.x ^ 0x80808080u, x.y ^ 0x80808080u, x.z ^ 0x80808080u, x.w ^ 0x80808080u};
+  const uint64_t first = uint64_t(blockIdx.x) * (kWidenThreads * kWidenAhead) + threadIdx.x;
+  uint4 x[kWidenAhead];
+#pragma unroll
+  for (uint32_t u = 0; u < kWidenAhead; ++u) {
+    const uint64_t i = first + u * kWidenThreads;
+    if (i < pieces) x[u] = __ldg(src + i);
+  }
+#pragma unroll
+  for (uint32_t u = 0; u < kWidenAhead; ++u) {
+    const uint64_t i = first + u * kWidenThreads;
+    if (i >= pieces) break;
+    const uint32_t w[4] = {x[u].x ^ 0x80808080u, x[u].y ^ 0x80808080u, x[u].z ^ 0x80808080u, x[u].w ^ 0x80808080u};
     uint32_t v[8];
 #pragma unroll
     for (uint32_t j = 0; j < 8; ++j) {
@@ -520,8 +531,14 @@ __global__ void __launch_bounds__(kWidenThreads) widen_rows_kernel(const uint4* 
       const uint32_t h = __byte_perm(w[j >> 1], 0x64646464u, (j & 1u) ? 0x4342u : 0x4140u);
       asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(v[j]) : "r"(h), "r"(0x64806480u));
     }
-    dst[2 * i] = make_uint4(v[0], v[1], v[2], v[3]);
-    dst[2 * i + 1] = make_uint4(v[4], v[5], v[6], v[7]);
+    if ((reinterpret_cast<uintptr_t>(dst) & 31u) == 0u) {
+      asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst + 2 * i), "r"(v[0]), "r"(v[1]),
+                   "r"(v[2]), "r"(v[3]), "r"(v[4]), "r"(v[5]), "r"(v[6]), "r"(v[7])
+                   : "memory");
+    } else {
+      dst[2 * i] = make_uint4(v[0], v[1], v[2], v[3]);
+      dst[2 * i + 1] = make_uint4(v[4], v[5], v[6], v[7]);
+    }
   }
 }
 
