@@ -30,8 +30,8 @@ def linear(x: torch.Tensor, w: torch.Tensor, bias: torch.Tensor | None = None,
 
     x [M, K], w [N, K], bias [N], residual [M, N], all bf16 on one CUDA device.
     activation: None, "relu", "gelu" (erf), "gelu_tanh" or "silu".
-    `out` receives the result (it may be `residual`); it cannot be combined with inputs that
-    require gradients.
+    `out` receives the result. It may be `residual` itself and must not overlap x, w or bias; it
+    cannot be combined with inputs that require gradients.
     """
     code = ACTIVATIONS.get(activation)
     if code is None:

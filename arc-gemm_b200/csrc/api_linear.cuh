@@ -407,7 +407,7 @@ int output_check(const char* what, const char* name, const void* p, int64_t ld, 
 }
 
 // Row blocks of the dz pass: the grid fills the GPU's block slots once, without a rest (a rest of
-// a few blocks costs a whole round: 59 against DZ_US us at 4096 x 8192), at least 16 rows each.
+// a few blocks costs a whole round: 59 against 43 us at 4096 x 8192), at least 16 rows each.
 // The workspace size must not depend on the device.
 constexpr uint32_t kDzBlocks = 148 * LB::kBlocksPerSm;
 uint32_t dz_row_blocks(uint32_t M, uint32_t N) {

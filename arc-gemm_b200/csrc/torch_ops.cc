@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -141,14 +142,27 @@ void expect_out(const Tensor& out, int64_t rows, int64_t cols, const at::Device&
   }
 }
 
+// An `out` that is about to be written: not a tensor whose gradient is recorded, not one of the
+// operands that other blocks still read, and a new version for whoever has saved it.
+void claim_out(const OptTensor& out, std::initializer_list<const Tensor*> operands) {
+  if (!out) return;
+  if (at::GradMode::is_enabled() && out->requires_grad()) bad_value("out must not require a gradient");
+  for (const Tensor* t : operands) {
+    const at::MemOverlapStatus s = at::get_overlap_status(*out, *t);
+    if (s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial) bad_value("out must not overlap an operand");
+  }
+  if (!out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
+}
+
 cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream(t.get_device()).stream(); }
 
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 
-// The gradients are not differentiable themselves: a second derivative raises.
-torch::autograd::variable_list once(torch::autograd::variable_list grads, const Tensor& dy) {
-  if (!at::GradMode::is_enabled() || !dy.requires_grad()) return grads;
+// The gradients are not differentiable themselves: a second derivative raises, by dy or by the
+// operands (grad mode is on in a backward pass only for create_graph).
+torch::autograd::variable_list once(torch::autograd::variable_list grads) {
+  if (!at::GradMode::is_enabled()) return grads;
   auto node = std::make_shared<torch::autograd::DelayedError>(
       "the gradients of arc's operators cannot be differentiated again", static_cast<int64_t>(grads.size()));
   torch::autograd::variable_list tracked;
@@ -223,7 +237,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
                                   k, k, static_cast<int>(ctx->saved_data["act"].toInt()), stream_of(x)),
             "arc.linear backward");
     }
-    return once(std::move(out), dy_in);
+    return once(std::move(out));
   }
 };
 
@@ -254,6 +268,10 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptTensor& bias, const Opt
   }
   const c10::cuda::CUDAGuard guard(dev);
   if (out) expect_out(*out, m, n, dev);
+  if (out && residual && at::get_overlap_status(*out, *residual) == at::MemOverlapStatus::Partial) {
+    bad_value("out must be residual itself or not overlap it");
+  }
+  claim_out(out, {&x, &w, bias ? &*bias : &w});
   const Tensor y = out ? *out : at::empty({m, n}, x.options().requires_grad(false));
   if (m > 0) {
     linear_call(product_rows(x), product_rows(w), bias ? OptTensor(bias->contiguous()) : bias,
@@ -323,7 +341,7 @@ struct GroupedFunction : torch::autograd::Function<GroupedFunction> {
                              dy.stride(0), x.stride(0), k, n * k, stream_of(x)),
             what);
     }
-    return once(std::move(out), dy_in);
+    return once(std::move(out));
   }
 };
 
@@ -343,6 +361,7 @@ Tensor grouped_matmul(const Tensor& x, const Tensor& w, const Tensor& offsets, c
   }
   const c10::cuda::CUDAGuard guard(dev);
   if (out) expect_out(*out, t, n, dev);
+  claim_out(out, {&x, &w});
   const Tensor y = out ? *out : at::empty({t, n}, x.options().requires_grad(false));
   if (t > 0) grouped_call(product_rows(x), product_rows(w), offsets, y, !out);
   return y;
@@ -372,6 +391,7 @@ Tensor a8w4_grouped_matmul(const Tensor& x, const Tensor& sa_in, const Tensor& w
   expect_offsets(offsets, e, dev);
   const c10::cuda::CUDAGuard guard(dev);
   if (out) expect(*out, "out", at::kBFloat16, {t, n}, dev);
+  claim_out(out, {&x, &sa, &wp, &sb});
   const Tensor y = out ? *out : at::empty({t, n}, x.options().dtype(at::kBFloat16));
   if (t == 0) return y;
   size_t bytes = 0;

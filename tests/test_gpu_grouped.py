@@ -422,3 +422,46 @@ def test_refusals(cuda_device):
         arc.a8w4_grouped_matmul(a, (b[0][:1], b[1]), off)
     with pytest.raises(TypeError):
         arc.a8w4_grouped_matmul((a[0].float(), a[1]), b, off)
+
+
+def test_out_is_refused_where_it_would_be_wrong(cuda_device):
+    x, w, _, offsets = _inputs([20, 12], 0, 32, 32)
+    with pytest.raises(ValueError, match="overlap"):
+        arc.grouped_matmul(x, w, offsets, out=x)
+    with pytest.raises(ValueError, match="gradient"):
+        arc.grouped_matmul(x, w, offsets, out=x.clone().requires_grad_())
+
+
+@pytest.mark.parametrize("rows", [2, 40])
+def test_weights_past_two_to_the_31st_element(cuda_device, rows):
+    """Weights and their gradient of more than 2^31 elements, by the streaming and the pair kernel."""
+    e, n, k = 33, 8192, 8200
+    g = torch.Generator(device="cuda").manual_seed(rows)
+    x, dy = (torch.randn(e * rows, c, generator=g, device="cuda").to(torch.bfloat16) for c in (k, n))
+    w = torch.empty(e, n, k, dtype=torch.bfloat16, device="cuda").normal_(generator=g).requires_grad_()
+    lx = x.clone().requires_grad_()
+    y = arc.grouped_matmul(lx, w, _offsets([rows] * e))
+    dx, dw = torch.autograd.grad(y, [lx, w], dy)
+    for i in (0, 15, e - 1):
+        at = slice(i * rows, (i + 1) * rows)
+        want = _reference(x[at], w.detach()[i:i + 1], dy[at], [rows])
+        assert_within(y.detach()[at], *want["y"], "y")
+        assert_within(dx[at], *want["dx"], "dx")
+        assert_within(dw[i:i + 1], *want["dw"], "dw")
+    assert arc.device_status(0) == 0
+
+
+def test_a8w4_codes_past_two_to_the_31st_byte(cuda_device, a8w4_kernel):
+    e, n, k, rows = 65, 8192, 8192, 3
+    g = torch.Generator(device="cuda").manual_seed(k)
+    x = torch.randint(-127, 128, (e * rows, k), generator=g, device="cuda").to(torch.int8)
+    sa = torch.rand(e * rows, generator=g, device="cuda") + 0.5
+    wp = torch.empty(e, n, k // 2, dtype=torch.uint8, device="cuda").random_(0, 256, generator=g)
+    sb = (torch.rand(e, n, k // 128, generator=g, device="cuda") + 0.1).to(torch.bfloat16)
+    got = arc.a8w4_grouped_matmul((x, sa), (wp, sb), _offsets([rows] * e))
+    for i in (0, 31, e - 1):
+        at = slice(i * rows, (i + 1) * rows)
+        want, mag = _a8w4_on_gpu((x[at], sa[at]), (wp[i:i + 1], sb[i:i + 1]), _offsets([rows]))
+        err = (k + 8) * SUM * mag
+        assert_within(got[at], want, err + H * (want.abs() + err), f"group {i}")
+    assert arc.device_status(0) == 0

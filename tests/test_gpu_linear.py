@@ -316,3 +316,57 @@ def test_any_contraction_size(cuda_device):
         want = linear_gradients(x, w, z, zerr, dy, "gelu")
         for v, name in zip(got, ("dx", "dw", "dbias")):
             assert_within(v, *want[name], name)
+
+
+def test_second_derivatives_by_operands_are_refused(cuda_device):
+    """dx depends on w and dw on x, also where dy is a constant."""
+    x, w, _, _ = _inputs(4, 24, 16, bias=False, residual=False)
+    lx, lw = _leaves(x, w)
+    (dx,) = torch.autograd.grad(arc.linear(lx, lw).sum(), [lx], create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiated again"):
+        (dx * dx).sum().backward()
+
+
+def test_out_is_refused_where_it_would_be_wrong(cuda_device):
+    x, w, b, r = _inputs(32, 32, 32)
+    for bad in (x, w, x.view(-1).view(32, 32)):  # views included
+        with pytest.raises(ValueError, match="overlap"):
+            arc.linear(x, w, b, out=bad)
+    buf = torch.zeros(33 * 32, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="residual"):
+        arc.linear(x, w, b, buf[:1024].view(32, 32), out=buf[32:].view(32, 32))
+    with pytest.raises(ValueError, match="gradient"):
+        arc.linear(x, w, b, out=r.clone().requires_grad_())
+    # Side by side in one buffer is no overlap.
+    both = torch.zeros(32, 64, dtype=torch.bfloat16, device="cuda")
+    both[:, :32] = x
+    arc.linear(both[:, :32], w, b, out=both[:, 32:])
+    y, bound, _, _ = linear_forward(x, w, b, None, None)
+    assert_within(both[:, 32:], y, bound, "side by side")
+    # A tensor that a graph has saved is not overwritten unnoticed.
+    h = x.clone()
+    y = arc.linear(h, w.clone().requires_grad_())
+    arc.linear(x, w, out=h)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
+@pytest.mark.parametrize("m,n", [(70_001, 32_776), (32_776, 70_001)])
+def test_past_two_to_the_31st_element(cuda_device, m, n):
+    """Outputs, z and dz of more than 2^31 elements; dy is zero but for a few rows."""
+    k = 64
+    x, w, b, _ = _inputs(m, n, k, residual=False)
+    rows = torch.tensor([0, 1, m // 2, m - 2, m - 1], device="cuda")
+    leaves = _leaves(x, w, b)
+    y = arc.linear(*leaves, activation="silu")
+    want, bound, z, zerr = linear_forward(x[rows], w, b, None, "silu")
+    assert_within(y.detach()[rows], want, bound, "y")
+    some = normal(torch.Generator().manual_seed(1), 5, n)
+    dy = torch.zeros_like(y).index_copy_(0, rows, some)
+    dx, dw, db = torch.autograd.grad(y, leaves, dy)
+    grads = linear_gradients(x[rows], w, z, zerr, some, "silu")
+    assert_within(dx[rows], *grads["dx"], "dx")
+    assert_within(dw, *grads["dw"], "dw")
+    assert_within(db, *grads["dbias"], "dbias")
+    assert dx.count_nonzero() == dx[rows].count_nonzero()
+    assert arc.device_status(0) == 0
