@@ -96,7 +96,7 @@ A8W4_STATIC_WEIGHTS = 2
 ACTIVATIONS = {None: 0, "relu": 1, "gelu": 2, "gelu_tanh": 3, "silu": 4}
 
 # Operation codes of arc_kernel_name (include/arc_b200.h).
-OP_MATMUL_BF16, OP_A8W4, OP_FP8_FP4 = 0, 1, 2
+OP_MATMUL_BF16, OP_A8W4, OP_FP8_FP4, OP_LINEAR = 0, 1, 2, 3
 
 
 def probe_enabled() -> bool:

@@ -191,6 +191,7 @@ bool decode_stream(int G, int S, int num_items, int grid) {
   X(128, 2, 3)
 
 cudaError_t linear_init(DeviceState& st);          // api_linear.cuh
+int linear_kernel_name(int dev, uint32_t M, uint32_t N, uint32_t K, char* name, int len);
 cudaError_t grouped_init(DeviceState& st, bool* regs_ok);  // api_grouped.cuh
 
 int init_device(int dev) {
@@ -709,6 +710,8 @@ int arc_kernel_name(int op, int M, int N, int K, char* name, int len) {
     if (int st = choose_fp8fp4(dev, M, N, K, true, &variant)) return st;
     kernel = variant == 2 ? "gemm_fp8fp4_pair_kernel"
                           : (variant == 1 ? "gemm_fp8fp4_kernel<2>" : "gemm_fp8fp4_kernel<1>");
+  } else if (op == ARC_OP_LINEAR) {
+    return linear_kernel_name(dev, M, N, K, name, len);
   } else {
     return fail(ARC_ERR_INVALID_ARGUMENT, "arc_kernel_name: unknown op %d", op);
   }

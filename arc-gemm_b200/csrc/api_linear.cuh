@@ -162,6 +162,18 @@ int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t
   return ARC_OK;
 }
 
+// The kernel of arc_linear_bf16 as ncu lists it (16-byte aligned output rows assumed).
+int linear_kernel_name(int dev, uint32_t M, uint32_t N, uint32_t K, char* name, int len) {
+  LinearPlan plan;
+  if (int st = linear_plan(dev, M, 1, N, ceil_div(K, arcb::lin::BK), true, &plan)) return st;
+  if (plan.pair) {
+    snprintf(name, static_cast<size_t>(len), "gemm_linear_pair_kernel<0, 0, 0, %d>", plan.pair_splits > 1 ? 1 : 0);
+  } else {
+    snprintf(name, static_cast<size_t>(len), "gemm_linear_stream_kernel<%u, 0>", plan.bn);
+  }
+  return ARC_OK;
+}
+
 // The pair kernel, one cluster of two pairs per tile if the contraction is split.
 template <bool A_MN, bool B_MN, bool ALONG_K>
 cudaError_t launch_linear_pair(LP::Params& p, uint64_t tiles, uint32_t splits, uint32_t max_pairs, cudaStream_t stream) {

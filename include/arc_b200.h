@@ -393,15 +393,17 @@ int arc_probe_attach(void *buffer, size_t bytes);
 
 /*
  * Name of the kernel the library launches for an operation of this shape on the
- * current device (op: ARC_OP_MATMUL_BF16, ARC_OP_A8W4 or ARC_OP_FP8_FP4; the FP8 x FP4
- * answer assumes a 16-byte aligned sfa), e.g. "gemm_bf16_pair_kernel", written into
- * name[0..len). The shape is not checked beyond what the choice needs; the
- * ARC_BF16_CTAS / ARC_FP8FP4_KERNEL overrides apply. The reference has one kernel per
- * operation, so it has no counterpart; this serves profiling (matching ncu launch lists).
+ * current device (op: ARC_OP_MATMUL_BF16, ARC_OP_A8W4, ARC_OP_FP8_FP4 or ARC_OP_LINEAR;
+ * the FP8 x FP4 answer assumes a 16-byte aligned sfa, the linear layer's aligned rows),
+ * e.g. "gemm_bf16_pair_kernel", written into name[0..len). The shape is not checked beyond
+ * what the choice needs; the ARC_BF16_CTAS / ARC_FP8FP4_KERNEL / ARC_LINEAR_PLAN overrides
+ * apply. The reference has one kernel per operation, so it has no counterpart; this serves
+ * profiling (matching ncu launch lists).
  */
 #define ARC_OP_MATMUL_BF16 0
 #define ARC_OP_A8W4 1
 #define ARC_OP_FP8_FP4 2
+#define ARC_OP_LINEAR 3
 int arc_kernel_name(int op, int M, int N, int K, char *name, int len);
 
 /*

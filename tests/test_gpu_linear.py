@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import arc
+from arc import _lib
 from linear_bounds import act64, assert_within, linear_forward, linear_gradients, normal
 
 pytestmark = pytest.mark.gpu
@@ -370,3 +371,11 @@ def test_past_two_to_the_31st_element(cuda_device, m, n):
     assert_within(db, *grads["dbias"], "dbias")
     assert dx.count_nonzero() == dx[rows].count_nonzero()
     assert arc.device_status(0) == 0
+
+
+def test_kernel_name(cuda_device, monkeypatch):
+    name = lambda *s: arc.kernel_name(_lib.OP_LINEAR, *s)  # noqa: E731
+    assert name(4096, 14336, 4096) == "gemm_linear_pair_kernel<0, 0, 0, 0>"
+    assert name(16, 14336, 4096) == "gemm_linear_stream_kernel<16, 0>"
+    monkeypatch.setenv("ARC_LINEAR_PLAN", "pair:2")
+    assert name(16, 14336, 4096) == "gemm_linear_pair_kernel<0, 0, 0, 1>"
