@@ -145,6 +145,7 @@ struct DeviceState {
   int max_bf16_pairs = 0;  // co-resident CTA pairs of the bf16 pair kernel
   int max_fp8fp4_pairs = 0;  // co-resident CTA pairs of the FP8 x FP4 pair kernel
   int max_linear_pairs = 0;  // co-resident CTA pairs of the linear pair kernel
+  int max_linear_quads = 0;  // co-resident clusters of two pairs (contraction in two parts)
 };
 DeviceState g_dev[kMaxDevices];
 

@@ -53,11 +53,12 @@ uint32_t column_pairs(const void* p, uint64_t ld, uint32_t cols) {
   return cols % 2 == 0 && ld % 2 == 0 && (reinterpret_cast<uintptr_t>(p) & 3u) == 0 ? 1u : 0u;
 }
 
-// The pair kernel's parts of the contraction: two where there are pairs for both halves of every
-// tile. (Four would take clusters of eight CTAs, of which too few fit at once: 512 x 4096 x 4096
-// 25 us whole, 20 in two parts, 48 in four.)
-uint32_t pair_splits(uint64_t tiles, uint32_t num_kb, uint32_t max_pairs) {
-  return tiles * 2 <= max_pairs && num_kb >= 8 ? 2 : 1;
+// The pair kernel's parts of the contraction: two where the clusters of all tiles run at once, which
+// are fewer than half the pairs (32 tiles: 512 x 4096 x 4096 29 us whole, 21 in two parts; 36 tiles:
+// 512 x 4608 x 4096 29 and 39). Of the clusters of eight CTAs that four parts would take, 15 fit: 256
+// x 3840 x 4096 20 us in two parts, 18.6 in four, but 256 x 4096 x 4096 20 and 33.
+uint32_t pair_splits(uint64_t tiles, uint32_t num_kb, int dev) {
+  return tiles <= static_cast<uint64_t>(g_dev[dev].max_linear_quads) && num_kb >= 8 ? 2 : 1;
 }
 
 // The kernel for a product of rows, in one group or several.
@@ -133,7 +134,7 @@ int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t
       }
     }
     const uint64_t tiles = uint64_t(ceil_div(rows, LP::kTile)) * ceil_div(cols, LP::kTile);
-    for (uint32_t s = 1; max_pairs > 0 && s <= pair_splits(tiles, num_kb, max_pairs); ++s) {
+    for (uint32_t s = 1; max_pairs > 0 && s <= pair_splits(tiles, num_kb, dev); ++s) {
       const double t = pair_cost(rows, cols, num_kb, s, aligned, max_pairs);
       if (t < best) {
         best = t;
@@ -236,6 +237,14 @@ cudaError_t linear_init(DeviceState& st) {
   int n = 0;
   e = cudaOccupancyMaxActiveClusters(&n, GP::gemm_grouped_pair_kernel<false, true>, &cfg);
   st.max_linear_pairs = e == cudaSuccess ? n : 0;
+  if (e != cudaSuccess) return e;
+  // And how many clusters of two pairs of the linear one.
+  cfg.blockDim = dim3(LP::kThreads, 1, 1);
+  cfg.dynamicSmemBytes = LP::kSmemBytes;
+  cfg.gridDim = dim3(4 * (st.sms / 4), 1, 1);
+  attr[0].val.clusterDim.x = 4;
+  e = cudaOccupancyMaxActiveClusters(&n, LP::gemm_linear_pair_kernel<false, false, false, true>, &cfg);
+  st.max_linear_quads = e == cudaSuccess ? n : 0;
   return e;
 }
 
@@ -372,7 +381,7 @@ int linear_dw(const char* what, const uint16_t* dy, const uint16_t* x, const arc
   if (tiles * 4 > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "%s: too many tiles for one launch", what);
   // The host knows the contraction's length only for one group of all rows.
   const uint32_t splits =
-      groups.offsets == nullptr ? pair_splits(tiles, ceil_div(groups.rows, arcb::lin::BK), max_pairs) : 1;
+      groups.offsets == nullptr ? pair_splits(tiles, ceil_div(groups.rows, arcb::lin::BK), dev) : 1;
   const cudaError_t e = launch_linear_pair<true, true, true>(p, tiles, splits, max_pairs, stream);
   if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
   return ARC_OK;
