@@ -65,32 +65,33 @@ uint32_t pair_splits(uint64_t tiles, uint32_t num_kb, int dev) {
 struct LinearPlan {
   bool pair;
   uint32_t pair_splits;            // pair kernel: 1 or 2
+  uint32_t pair_cols;              // its tile's columns: 256 or 128
   uint32_t bn, splits, row_tiles;  // streaming kernel: row tile, parts of the contraction
 };
 
-// Estimated time of one group's product: what a launch costs, and per round of blocks what a
-// tile costs besides its contraction blocks of 64 and with them. Only the order of the plans
-// counts; the constants are a fit to the measured times of all plans of 500 products (1 to 4096
-// rows, 64 to 8192 columns, contractions of 64 to 6400). The plan it picks is 2 % behind the best
-// one, geometric mean over those and over 200 others; fixed thresholds on rows and tiles were 14 %.
+// Estimated time of one group's product in microseconds: what a launch costs, and per round of
+// blocks what a tile costs besides its contraction blocks of 64 and with them. The constants are a
+// fit to the measured times of all plans of 500 products (1 to 4096 rows, 64 to 8192 columns,
+// contractions of 64 to 6400). The plan it picks is 1.1 % behind the best one, geometric mean over
+// those, and 1.4 % over 200 others; fixed thresholds on rows and tiles were 14 %.
 double stream_cost(uint32_t rows, uint32_t cols, uint32_t num_kb, uint32_t bn, uint32_t splits, uint32_t sms) {
-  // Two blocks fit on an SM; clusters of four and eight leave some slots empty, and two blocks of
-  // a cluster of two come to lie on one SM.
-  const double slots = 2.0 * sms * (splits == 8 ? 256.0 / 296 : splits == 4 ? 280.0 / 296 : 1.0);
-  const double cluster = splits == 8 ? 0.1 : splits == 4 ? 0.8 : splits == 2 ? 2.44 : 0.0;
+  // Two blocks fit on an SM; clusters of four and eight leave some slots empty.
+  const double slots = 2.0 * sms * (splits == 8 ? 240.0 / 296 : splits == 4 ? 280.0 / 296 : 1.0);
+  const double cluster = splits > 1 ? 1.36 : 0.0;
   const double blocks = static_cast<double>(ceil_div(rows, bn)) * ceil_div(cols, LS::kRows) * splits;
   const double load = blocks < 2.0 * sms ? blocks / (2.0 * sms) : 1.0;
-  const double per_kb = 0.0724 + 0.0033 * (16 + bn / 8.0) * load;  // latency, and a share of the bandwidth
-  const double epilogue = bn / 16.0 * (0.693 / splits + 0.45) + 1.16;
-  return 0.95 + ceil(blocks / slots) * (ceil_div(num_kb, splits) * per_kb + epilogue) + cluster;
+  const double per_kb = 0.16 + 0.008 * (16 + bn / 8.0) * load;  // latency, and a share of the bandwidth
+  const double epilogue = bn / 16.0 * (1.035 / splits + 0.48) + 0.95;
+  return 1.3 + ceil(blocks / slots) * (ceil_div(num_kb, splits) * per_kb + epilogue) + cluster;
 }
 
-double pair_cost(uint32_t rows, uint32_t cols, uint32_t num_kb, uint32_t splits, bool aligned, uint32_t max_pairs) {
-  const double tiles = static_cast<double>(ceil_div(rows, LP::kTile)) * ceil_div(cols, LP::kTile);
-  const double products = ceil_div(num_kb, splits) * 0.0442 + 0.51;
-  const double epilogue = aligned ? 3.17 : 8.78;  // output rows by TMA, or element by element
-  return 4.0 + ceil(tiles * splits / max_pairs) * (products > epilogue ? products : epilogue) + epilogue / splits +
-         (splits > 1 ? 1.37 : 0.0);
+double pair_cost(uint32_t rows, uint32_t cols, uint32_t num_kb, uint32_t tile_cols, uint32_t splits, bool aligned,
+                 uint32_t max_pairs) {
+  const double tiles = static_cast<double>(ceil_div(rows, LP::kTile)) * ceil_div(cols, tile_cols);
+  const double products = ceil_div(num_kb, splits) * (tile_cols == 128 ? 0.185 : 0.265) + 0.53;
+  const double epilogue = (aligned ? 3.4 : 9.5) * tile_cols / 256;  // output rows by TMA, or element by element
+  return 5.9 + ceil(tiles * splits / max_pairs) * (products > epilogue ? products : epilogue) + epilogue / splits +
+         (splits > 1 ? 1.5 : 0.0);
 }
 
 // One group: the plan of the least estimated time. Several groups, of which the host knows only the
@@ -101,24 +102,26 @@ double pair_cost(uint32_t rows, uint32_t cols, uint32_t num_kb, uint32_t splits,
 // holds an average group's rows, with the contraction split over a cluster until the two block
 // slots of every SM have work (four blocks of 64 each at least).
 //
-// ARC_LINEAR_PLAN="pair:S" | "BN:S" (tests and tuning) forces the choice where it is valid.
+// ARC_LINEAR_PLAN="pair:S" | "pair128:S" | "BN:S" (tests and tuning) forces the choice where it is valid.
 int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t num_kb, bool aligned, LinearPlan* plan) {
   const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
   const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
   const uint32_t live = groups < rows ? groups : rows;  // groups that can have rows
   const uint32_t avg = ceil_div(rows, live);
-  *plan = {false, 1, 16, 1, 0};
+  *plan = {false, 1, LP::kTile, 16, 1, 0};
   if (const char* env = getenv("ARC_LINEAR_PLAN")) {
     unsigned bn = 0, s = 0;
-    if (sscanf(env, "pair:%u", &s) == 1 && max_pairs > 0 && (s == 1 || s == 2)) {
+    const bool narrow = sscanf(env, "pair128:%u", &s) == 1;
+    if ((narrow || sscanf(env, "pair:%u", &s) == 1) && max_pairs > 0 && (s == 1 || s == 2)) {
       plan->pair = true;
+      if (narrow) plan->pair_cols = 128;
       plan->pair_splits = s <= num_kb ? s : 1;
     } else if (sscanf(env, "%u:%u", &bn, &s) == 2 && (bn == 16 || bn == 32 || bn == 64 || bn == 128) &&
                (s == 1 || s == 2 || s == 4 || s == 8)) {
       plan->bn = bn;
       plan->splits = s <= num_kb ? s : 1;
     } else {
-      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_LINEAR_PLAN must be 'pair:S' or 'BN:S' (got '%s')", env);
+      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_LINEAR_PLAN must be 'pair:S', 'pair128:S' or 'BN:S' (got '%s')", env);
     }
   } else if (groups == 1) {
     double best = 1e30;
@@ -133,13 +136,16 @@ int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t
         }
       }
     }
-    const uint64_t tiles = uint64_t(ceil_div(rows, LP::kTile)) * ceil_div(cols, LP::kTile);
-    for (uint32_t s = 1; max_pairs > 0 && s <= pair_splits(tiles, num_kb, dev); ++s) {
-      const double t = pair_cost(rows, cols, num_kb, s, aligned, max_pairs);
-      if (t < best) {
-        best = t;
-        plan->pair = true;
-        plan->pair_splits = s;
+    for (uint32_t tile_cols : {256u, 128u}) {
+      const uint64_t tiles = uint64_t(ceil_div(rows, LP::kTile)) * ceil_div(cols, tile_cols);
+      for (uint32_t s = 1; max_pairs > 0 && s <= pair_splits(tiles, num_kb, dev); ++s) {
+        const double t = pair_cost(rows, cols, num_kb, tile_cols, s, aligned, max_pairs);
+        if (t < best) {
+          best = t;
+          plan->pair = true;
+          plan->pair_splits = s;
+          plan->pair_cols = tile_cols;
+        }
       }
     }
   } else {
@@ -168,7 +174,8 @@ int linear_kernel_name(int dev, uint32_t M, uint32_t N, uint32_t K, char* name, 
   LinearPlan plan;
   if (int st = linear_plan(dev, M, 1, N, ceil_div(K, arcb::lin::BK), true, &plan)) return st;
   if (plan.pair) {
-    snprintf(name, static_cast<size_t>(len), "gemm_linear_pair_kernel<0, 0, 0, %d>", plan.pair_splits > 1 ? 1 : 0);
+    snprintf(name, static_cast<size_t>(len), "gemm_linear_pair_kernel<0, 0, 0, %d, %u>",
+             plan.pair_splits > 1 ? 1 : 0, plan.pair_cols);
   } else {
     snprintf(name, static_cast<size_t>(len), "gemm_linear_stream_kernel<%u, 0>", plan.bn);
   }
@@ -176,15 +183,15 @@ int linear_kernel_name(int dev, uint32_t M, uint32_t N, uint32_t K, char* name, 
 }
 
 // The pair kernel, one cluster of two pairs per tile if the contraction is split.
-template <bool A_MN, bool B_MN, bool ALONG_K>
+template <bool A_MN, bool B_MN, bool ALONG_K, uint32_t TN>
 cudaError_t launch_linear_pair(LP::Params& p, uint64_t tiles, uint32_t splits, uint32_t max_pairs, cudaStream_t stream) {
   p.splits = splits;
   if (splits > 1) {
-    return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, true>, p, static_cast<uint32_t>(tiles) * 2 * splits,
-                     LP::kThreads, LP::kSmemBytes, 2 * splits, stream);
+    return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, true, TN>, p, static_cast<uint32_t>(tiles) * 2 * splits,
+                     LP::kThreads, LP::kSmemBytes<TN>, 2 * splits, stream);
   }
   const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
-  return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, false>, p, grid, LP::kThreads, LP::kSmemBytes, 2,
+  return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, false, TN>, p, grid, LP::kThreads, LP::kSmemBytes<TN>, 2,
                    stream);
 }
 
@@ -212,9 +219,11 @@ cudaError_t linear_init(DeviceState& st) {
   ARC_LINEAR_STREAM_VARIANTS(ARC_SET_ATTR)
 #undef ARC_SET_ATTR
 #define ARC_SET_ATTR(SPLIT)                                                                                         \
-  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, false, false, SPLIT>, LP::kSmemBytes);    \
-  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, true, false, SPLIT>, LP::kSmemBytes);     \
-  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<true, true, true, SPLIT>, LP::kSmemBytes);
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, false, false, SPLIT, 256>, LP::kSmemBytes<256>); \
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, true, false, SPLIT, 256>, LP::kSmemBytes<256>);  \
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, false, false, SPLIT, 128>, LP::kSmemBytes<128>); \
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<false, true, false, SPLIT, 128>, LP::kSmemBytes<128>);  \
+  if (e == cudaSuccess) e = allow_smem(LP::gemm_linear_pair_kernel<true, true, true, SPLIT, 256>, LP::kSmemBytes<256>);
   ARC_SET_ATTR(false)
   ARC_SET_ATTR(true)
 #undef ARC_SET_ATTR
@@ -240,10 +249,10 @@ cudaError_t linear_init(DeviceState& st) {
   if (e != cudaSuccess) return e;
   // And how many clusters of two pairs of the linear one.
   cfg.blockDim = dim3(LP::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = LP::kSmemBytes;
+  cfg.dynamicSmemBytes = LP::kSmemBytes<256>;
   cfg.gridDim = dim3(4 * (st.sms / 4), 1, 1);
   attr[0].val.clusterDim.x = 4;
-  e = cudaOccupancyMaxActiveClusters(&n, LP::gemm_linear_pair_kernel<false, false, false, true>, &cfg);
+  e = cudaOccupancyMaxActiveClusters(&n, LP::gemm_linear_pair_kernel<false, false, false, true, 256>, &cfg);
   st.max_linear_quads = e == cudaSuccess ? n : 0;
   return e;
 }
@@ -305,7 +314,8 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
     if (int st = encode_groups_3d(&p.tm_a, a, inner, groups.rows, 1, lda, 0, 64, LP::kRowsPerCta, "rows")) {
       return st;
     }
-    if (int st = encode_groups_3d(&p.tm_b, w, w_cols, w_rows, 1, ldw, w_stride, 64, grad ? 64 : LP::kRowsPerCta,
+    if (int st = encode_groups_3d(&p.tm_b, w, w_cols, w_rows, 1, ldw, w_stride, 64,
+                                  grad ? 64 : plan.pair_cols / 2,
                                   "weights")) {
       return st;
     }
@@ -319,12 +329,14 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
     p.M = groups.rows;
     p.N = cols;
     p.tiles_m = ceil_div(groups.rows, LP::kTile);
-    p.tiles_n = ceil_div(cols, LP::kTile);
+    p.tiles_n = ceil_div(cols, plan.pair_cols);
     p.num_kb = num_kb;
     const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
     if (tiles * 4 > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
-    e = grad ? launch_linear_pair<false, true, false>(p, tiles, plan.pair_splits, max_pairs, stream)
-             : launch_linear_pair<false, false, false>(p, tiles, plan.pair_splits, max_pairs, stream);
+    const bool narrow = plan.pair_cols == 128;
+    const auto launch = grad ? (narrow ? launch_linear_pair<false, true, false, 128> : launch_linear_pair<false, true, false, 256>)
+                             : (narrow ? launch_linear_pair<false, false, false, 128> : launch_linear_pair<false, false, false, 256>);
+    e = launch(p, tiles, plan.pair_splits, max_pairs, stream);
     if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
     return ARC_OK;
   }
@@ -382,7 +394,7 @@ int linear_dw(const char* what, const uint16_t* dy, const uint16_t* x, const arc
   // The host knows the contraction's length only for one group of all rows.
   const uint32_t splits =
       groups.offsets == nullptr ? pair_splits(tiles, ceil_div(groups.rows, arcb::lin::BK), dev) : 1;
-  const cudaError_t e = launch_linear_pair<true, true, true>(p, tiles, splits, max_pairs, stream);
+  const cudaError_t e = launch_linear_pair<true, true, true, 256>(p, tiles, splits, max_pairs, stream);
   if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_pair_kernel launch");
   return ARC_OK;
 }

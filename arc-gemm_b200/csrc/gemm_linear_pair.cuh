@@ -22,10 +22,14 @@
 // inside the last step are overwritten with zeros in shared memory, in both operands, by a warp
 // of each CTA between the load's arrival and the product.
 //
-// SPLIT: problems with fewer tiles than pairs. A cluster of two pairs (or more) takes one tile, its pairs
+// SPLIT: problems with fewer tiles than pairs. A cluster of two pairs takes one tile, its pairs
 // the contraction in equal parts; each CTA then leaves its sums in its ring's shared memory, and
 // pair i finishes the i-th part of the columns, adding the parts in order through distributed
 // shared memory (the result does not depend on timing).
+//
+// TN: columns of a tile. 128 where tiles of 256 leave pairs without work or a last round mostly
+// empty (256 x 4096 x 4096: 20.1 us with 256, 15.9 with 128; 512 x 4608 x 4096 29 and 22; but 1024 x
+// 4096 x 4096 30 and 37, since a stage's products then hardly cover its hand-offs).
 //
 // Roles (384 threads per CTA): warp 0 TMA producer, warp 1 UMMA issuer (rank 0), warp 2 TMEM
 // owner, warp 3 zeroes a group's tail, warps 4-11 epilogue: two warpgroups take 32 columns in
@@ -43,18 +47,27 @@ using lin::BK;
 using lin::kUmmaK;
 
 constexpr uint32_t kRowsPerCta = 128;
-constexpr uint32_t kTile = 256;  // pair tile, both directions
-constexpr uint32_t kStages = 6;
+constexpr uint32_t kTile = 256;  // pair tile, rows; and columns unless TN is 128
 constexpr uint32_t kEpiWarps = 8;
 constexpr uint32_t kThreads = 32 * (4 + kEpiWarps);
 constexpr uint32_t kTmemCols = 512;
 constexpr uint32_t kBandM = 8;  // row tiles per raster band (L2 reuse)
 constexpr uint32_t kOperandBytes = kRowsPerCta * BK * 2;
-constexpr uint32_t kStageBytes = 2 * kOperandBytes;  // A + B of one CTA
+// A and B of one CTA, in as many stages as shared memory holds: narrow tiles are short of loads in
+// flight rather than of tensor time (256 x 4096 x 14336 in two parts: 36.4 us with six stages, 34.8 with eight).
+template <uint32_t TN>
+struct Cfg {
+  static constexpr uint32_t kStages = TN == 256 ? 6 : 8;
+  static constexpr uint32_t kBBytes = TN / 2 * BK * 2;
+  static constexpr uint32_t kStageBytes = kOperandBytes + kBBytes;
+  static_assert(kStages * kStageBytes >= TN * kRowsPerCta * 4, "a CTA's sums fit in its ring");
+};
 
+template <uint32_t TN>
 struct alignas(1024) Smem {
+  static constexpr uint32_t kStages = Cfg<TN>::kStages;
   uint8_t a[kStages][kOperandBytes];
-  uint8_t b[kStages][kOperandBytes];
+  uint8_t b[kStages][Cfg<TN>::kBBytes];
   uint8_t piece[kEpiWarps][2][lin::kWarpTileBytes];
   uint64_t full[kStages];        // rank 0: both CTAs' bytes of a stage
   uint64_t empty[kStages];       // each CTA: the pair's UMMAs consumed its stage
@@ -67,9 +80,9 @@ struct alignas(1024) Smem {
   uint32_t tmem_base;
   uint32_t abort;
 };
-constexpr size_t kSmemBytes = sizeof(Smem) + 1024;
-static_assert(kStages * kOperandBytes * 2 >= kTile * kRowsPerCta * 4, "a CTA's sums fit in its ring");
-static_assert(kSmemBytes <= 232448, "shared memory fits in 227 KB");
+template <uint32_t TN>
+constexpr size_t kSmemBytes = sizeof(Smem<TN>) + 1024;
+static_assert(kSmemBytes<256> <= 232448 && kSmemBytes<128> <= 232448, "shared memory fits in 227 KB");
 
 struct Params {
   CUtensorMap tm_a;  // 3-D, SW128: K-major {K, M, E} box {64, 128, 1}; MN-major {M, K, E} box {64, 64, 1}
@@ -99,7 +112,7 @@ struct Tile {
 };
 
 // `part`: this pair's part of the contraction (SPLIT).
-template <bool ALONG_K, bool SPLIT>
+template <bool ALONG_K, bool SPLIT, uint32_t TN>
 __device__ __forceinline__ bool tile_at(const Params& p, uint32_t t, uint32_t part, Tile& w) {
   const uint32_t per = p.tiles_m * p.tiles_n;
   w.e = 0;
@@ -126,7 +139,7 @@ __device__ __forceinline__ bool tile_at(const Params& p, uint32_t t, uint32_t pa
   const uint32_t m_first = band * kBandM;
   const uint32_t m_cnt = min(kBandM, p.tiles_m - m_first);
   w.m0 = (m_first + rem % m_cnt) * kTile;
-  w.n0 = rem / m_cnt * kTile;
+  w.n0 = rem / m_cnt * TN;
   w.kb0 = SPLIT ? w.num_kb * part / p.splits : 0u;
   w.kb1 = SPLIT ? w.num_kb * (part + 1u) / p.splits : w.num_kb;
   return true;
@@ -233,10 +246,12 @@ __device__ __forceinline__ bool finish_piece(const Params& p, Pieces& b, float (
   return true;
 }
 
-template <bool A_MN, bool B_MN, bool ALONG_K, bool SPLIT>
+template <bool A_MN, bool B_MN, bool ALONG_K, bool SPLIT, uint32_t TN>
 __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __grid_constant__ Params p) {
+  static_assert(TN == 256 || (TN == 128 && !ALONG_K), "columns of a tile");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  Smem& s = *reinterpret_cast<Smem*>(smem_raw + smem_align_pad(smem_raw));
+  constexpr uint32_t kStages = Cfg<TN>::kStages;
+  Smem<TN>& s = *reinterpret_cast<Smem<TN>*>(smem_raw + smem_align_pad(smem_raw));
   const uint32_t warp = warp_idx_sync();
   const uint32_t lane = threadIdx.x & 31u;
   // rank: CTA of the pair; lead: the pair's first CTA in the cluster. Without SPLIT a cluster is a pair
@@ -290,7 +305,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       const uint32_t row0 = rank * kRowsPerCta;
       Tile w;
       bool ok = true;
-      for (uint32_t t = pair; ok && (tile_at<ALONG_K, SPLIT>(p, t, part, w)); t += num_pairs) {
+      for (uint32_t t = pair; ok && (tile_at<ALONG_K, SPLIT, TN>(p, t, part, w)); t += num_pairs) {
         for (uint32_t kb = w.kb0; kb < w.kb1; ++kb) {
           if (!mbar_wait(&s.empty[stage], phase ^ 1u, abort, kStatusTimeoutProducer)) {
             ok = false;
@@ -300,15 +315,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
           uint32_t bar;
           if (tail) {
             bar = map_to_rank(&s.tail_full[stage], lead + rank);
-            mbar_arrive_expect_tx(&s.tail_full[stage], kStageBytes);
+            mbar_arrive_expect_tx(&s.tail_full[stage], Cfg<TN>::kStageBytes);
             is_tail |= 1u << stage;
             tail_parity ^= 1u << stage;
           } else {
             bar = map_to_rank(&s.full[stage], lead);
-            if (rank == 0) mbar_arrive_expect_tx(&s.full[stage], 2 * kStageBytes);
+            if (rank == 0) mbar_arrive_expect_tx(&s.full[stage], 2 * Cfg<TN>::kStageBytes);
             is_tail &= ~(1u << stage);
           }
-          const int32_t k = int32_t(w.k0 + kb * BK), m = int32_t(w.m0 + row0), n = int32_t(w.n0 + row0);
+          const int32_t k = int32_t(w.k0 + kb * BK), m = int32_t(w.m0 + row0),
+                        n = int32_t(w.n0 + rank * (TN / 2u));
           if (A_MN) {
             tma_load_3d_pair(&p.tm_a, bar, s.a[stage], m, k, 0, kCacheEvictNormal);
             tma_load_3d_pair(&p.tm_a, bar, s.a[stage] + lin::kMnChunkBytes, m + 64, k, 0, kCacheEvictNormal);
@@ -317,7 +333,9 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
           }
           if (B_MN) {
             tma_load_3d_pair(&p.tm_b, bar, s.b[stage], n, k, 0, kCacheEvictNormal);
-            tma_load_3d_pair(&p.tm_b, bar, s.b[stage] + lin::kMnChunkBytes, n + 64, k, 0, kCacheEvictNormal);
+            if (TN == 256) {
+              tma_load_3d_pair(&p.tm_b, bar, s.b[stage] + lin::kMnChunkBytes, n + 64, k, 0, kCacheEvictNormal);
+            }
           } else {
             tma_load_3d_pair(&p.tm_b, bar, s.b[stage], k, n, 0, kCacheEvictNormal);
           }
@@ -347,18 +365,18 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     // stage), one lane issues.
     if (rank == 0) {
       const bool leader = elect_one();
-      constexpr uint32_t idesc = lin::idesc_of<A_MN, B_MN>(kTile, kTile);
+      constexpr uint32_t idesc = lin::idesc_of<A_MN, B_MN>(kTile, TN);
       uint32_t stage = 0, phase = 0, local = 0;
       bool ok = true;
       Tile w;
-      for (uint32_t t = pair; ok && (tile_at<ALONG_K, SPLIT>(p, t, part, w)); t += num_pairs) {
+      for (uint32_t t = pair; ok && (tile_at<ALONG_K, SPLIT, TN>(p, t, part, w)); t += num_pairs) {
         if (w.kb0 == w.kb1) continue;  // nothing to multiply: the epilogue takes zeros
         const uint32_t acc = local & 1u;
         const uint32_t acc_phase = (local >> 1) & 1u;
         ++local;
         if (!__all_sync(0xffffffffu, mbar_wait(&s.tmem_empty[acc], acc_phase ^ 1u, abort, kStatusTimeoutMma))) break;
         tc_fence_after_sync();
-        const uint32_t d_tmem = tmem_base + acc * kTile;
+        const uint32_t d_tmem = tmem_base + acc * TN;
         for (uint32_t kb = w.kb0; kb < w.kb1; ++kb) {
           if (!__all_sync(0xffffffffu, mbar_wait(&s.full[stage], phase, abort, kStatusTimeoutMma))) {
             ok = false;
@@ -396,7 +414,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       uint32_t stage = 0, parity = 0;  // parity: per stage, of its next tail
       Tile w;
       bool ok = true;
-      for (uint32_t t = pair; ok && (tile_at<ALONG_K, SPLIT>(p, t, part, w)); t += num_pairs) {
+      for (uint32_t t = pair; ok && (tile_at<ALONG_K, SPLIT, TN>(p, t, part, w)); t += num_pairs) {
         if (w.kb0 == w.kb1) continue;
         const uint32_t st = (stage + w.kb1 - w.kb0 - 1u) % kStages;
         stage = (stage + w.kb1 - w.kb0) % kStages;
@@ -435,12 +453,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     uint32_t local = 0;
     bool ok = true;
     Tile w;
-    for (uint32_t t = pair; (tile_at<ALONG_K, SPLIT>(p, t, part, w)); t += num_pairs) {
+    for (uint32_t t = pair; (tile_at<ALONG_K, SPLIT, TN>(p, t, part, w)); t += num_pairs) {
       const bool any = w.kb0 != w.kb1;
       const uint32_t acc = local & 1u;
       const uint32_t acc_phase = (local >> 1) & 1u;
       if (any) ++local;
-      const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * kTile;
+      const uint32_t t_row = tmem_base + ((q * 32u) << 16) + acc * TN;
       if constexpr (SPLIT) {
         // This CTA's sums, column by column, into its ring: every load and product has ended.
         if (any) {
@@ -450,7 +468,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
         }
         float* sums = reinterpret_cast<float*>(s.a[0]) + row;
 #pragma unroll 1
-        for (uint32_t c = wg; c < kTile / 32u; c += 2u) {
+        for (uint32_t c = wg; c < TN / 32u; c += 2u) {
           uint32_t r[32];
           if (any) {
             tmem_ld_32x32b_x32(t_row + c * 32u, r);
@@ -466,7 +484,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
         float zero[32];
 #pragma unroll
         for (uint32_t i = 0; i < 32; ++i) zero[i] = 0.f;
-        for (uint32_t n = w.n0 + wg * 32u; m < p.M && n < min(w.n0 + kTile, p.N); n += 64u) {
+        for (uint32_t n = w.n0 + wg * 32u; m < p.M && n < min(w.n0 + TN, p.N); n += 64u) {
           finish_piece<ALONG_K>(p, pieces, zero, m, n, w.e, abort, lane);
         }
         continue;
@@ -480,12 +498,12 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       if (!ok) break;
       tc_fence_after_sync();
 #pragma unroll 1
-      for (uint32_t c = wg; c < kTile / 32u; c += 2u) {
+      for (uint32_t c = wg; c < TN / 32u; c += 2u) {
         const uint32_t n = w.n0 + c * 32u;
         uint32_t r[32];
         tmem_ld_32x32b_x32(t_row + c * 32u, r);
         tmem_ld_wait();
-        if (c + 2u >= kTile / 32u) {
+        if (c + 2u >= TN / 32u) {
           tc_fence_before_sync();
           __syncwarp();
           if (lane == 0) mbar_arrive_cluster_relaxed(empty0[acc]);
@@ -495,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
 #pragma unroll
           for (uint32_t i = 0; i < 32; ++i) v[i] = __uint_as_float(r[i]);
           ok = finish_piece<ALONG_K>(p, pieces, v, m, n, w.e, abort, lane);
-          if (ok && ahead && c + 2u < kTile / 32u && n + 64u < p.N) piece_ask(p, pieces, n + 64u, m, lane);
+          if (ok && ahead && c + 2u < TN / 32u && n + 64u < p.N) piece_ask(p, pieces, n + 64u, m, lane);
         }
       }
       if (!ok) break;
@@ -506,10 +524,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     __syncwarp();
     cluster_sync_all();  // every part's sums are in its shared memory
     Tile w;
-    if (warp >= 4 && (tile_at<ALONG_K, SPLIT>(p, pair, part, w)) && *abort == 0u) {
+    if (warp >= 4 && (tile_at<ALONG_K, SPLIT, TN>(p, pair, part, w)) && *abort == 0u) {
       const uint32_t row = (warp & 3u) * 32u + lane;
       const uint32_t m = w.m0 + rank * kRowsPerCta + (warp & 3u) * 32u;  // the warp's first row
-      const uint32_t first = kTile / p.splits * part, last = first + kTile / p.splits;
+      const uint32_t first = TN / p.splits * part, last = first + TN / p.splits;
       bool ok = m < p.M;
 #pragma unroll 1
       for (uint32_t c = first + ((warp - 4u) >> 2) * 32u; c < last && w.n0 + c < p.N && ok; c += 64u) {

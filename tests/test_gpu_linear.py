@@ -11,7 +11,7 @@ from linear_bounds import act64, assert_within, linear_forward, linear_gradients
 pytestmark = pytest.mark.gpu
 
 ACTS = [None, "relu", "gelu", "gelu_tanh", "silu"]
-PLANS = ["pair:1", "pair:2", "16:1", "16:4", "32:2", "64:1", "128:8", "128:1"]
+PLANS = ["pair:1", "pair:2", "pair128:1", "pair128:2", "16:1", "16:4", "32:2", "64:1", "128:8", "128:1"]
 
 
 def _inputs(m, n, k, seed=0, bias=True, residual=True):
@@ -49,7 +49,7 @@ def test_real_sizes(cuda_device, m, n, k):
     _check(m, n, k, "silu")
 
 
-@pytest.mark.parametrize("plan", ["pair:1", "pair:2", "16:4", "128:1"])
+@pytest.mark.parametrize("plan", ["pair:1", "pair:2", "pair128:1", "pair128:2", "16:4", "128:1"])
 def test_strided_operands(cuda_device, monkeypatch, plan):
     """Column slices of wider matrices; an output whose rows are not 16-byte aligned."""
     monkeypatch.setenv("ARC_LINEAR_PLAN", plan)
@@ -375,7 +375,23 @@ def test_past_two_to_the_31st_element(cuda_device, m, n):
 
 def test_kernel_name(cuda_device, monkeypatch):
     name = lambda *s: arc.kernel_name(_lib.OP_LINEAR, *s)  # noqa: E731
-    assert name(4096, 14336, 4096) == "gemm_linear_pair_kernel<0, 0, 0, 0>"
+    assert name(4096, 14336, 4096) == "gemm_linear_pair_kernel<0, 0, 0, 0, 256>"
     assert name(16, 14336, 4096) == "gemm_linear_stream_kernel<16, 0>"
     monkeypatch.setenv("ARC_LINEAR_PLAN", "pair:2")
-    assert name(16, 14336, 4096) == "gemm_linear_pair_kernel<0, 0, 0, 1>"
+    assert name(16, 14336, 4096) == "gemm_linear_pair_kernel<0, 0, 0, 1, 256>"
+
+
+@pytest.mark.parametrize("plan", ["pair:1", "pair:2", "pair128:1", "pair128:2", "32:2"])
+@pytest.mark.parametrize("m,n,k", [(300, 264, 136), (1000, 1500, 520), (2600, 2056, 264)])
+def test_row_gradient_by_every_plan(cuda_device, monkeypatch, plan, m, n, k):
+    """The row gradient takes the forward product's kernels with w read MN-major; several tiles per pair."""
+    monkeypatch.setenv("ARC_LINEAR_PLAN", plan)
+    x, w, _, _ = _inputs(m, k, n, bias=False, residual=False)
+    dy = normal(torch.Generator().manual_seed(2), m, k)
+    lx = x.clone().requires_grad_()
+    (dx,) = torch.autograd.grad(arc.linear(lx, w), [lx], dy)
+    z = x.double() @ w.double().T
+    want = linear_gradients(x, w, z, torch.zeros_like(z), dy, None)
+    assert_within(dx, *want["dx"], "dx")
+    _check(m, n, k, "silu")
+    assert arc.device_status(0) == 0
