@@ -72,11 +72,11 @@ struct LinearPlan {
 // Estimated time of one group's product in microseconds: what a launch costs, and per round of
 // blocks what a tile costs besides its contraction blocks of 64 and with them. The constants are a
 // fit to the measured times of all plans of 500 products (1 to 4096 rows, 64 to 8192 columns,
-// contractions of 64 to 6400). The plan it picks is 1.1 % behind the best one, geometric mean over
+// contractions of 64 to 6400). The plan it picks is 1.2 % behind the best one, geometric mean over
 // those, and 1.4 % over 200 others; fixed thresholds on rows and tiles were 14 %.
 double stream_cost(uint32_t rows, uint32_t cols, uint32_t num_kb, uint32_t bn, uint32_t splits, uint32_t sms) {
   // Two blocks fit on an SM; clusters of four and eight leave some slots empty.
-  const double slots = 2.0 * sms * (splits == 8 ? 240.0 / 296 : splits == 4 ? 280.0 / 296 : 1.0);
+  const double slots = 2.0 * sms * (splits == 8 ? 256.0 / 296 : splits == 4 ? 280.0 / 296 : 1.0);
   const double cluster = splits > 1 ? 1.36 : 0.0;
   const double blocks = static_cast<double>(ceil_div(rows, bn)) * ceil_div(cols, LS::kRows) * splits;
   const double load = blocks < 2.0 * sms ? blocks / (2.0 * sms) : 1.0;
