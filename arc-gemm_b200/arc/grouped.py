@@ -28,7 +28,7 @@ def grouped_matmul(x: torch.Tensor, w: torch.Tensor, offsets: torch.Tensor,
 
     x [T, K] and w [E, N, K] bf16, offsets int32 [E+1] on the same device, E <= 1024. Rows that
     are not contiguous and 16-byte aligned (strides multiples of 8) are copied first. `out`
-    must not overlap x or w and cannot be combined with inputs that require gradients.
+    must not overlap x, w or offsets and cannot be combined with inputs that require gradients.
     """
     return torch_ops().grouped_matmul(x, w, offsets, out)
 

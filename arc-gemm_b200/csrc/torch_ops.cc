@@ -10,13 +10,15 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
-#include <ATen/MemoryOverlap.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
+#include <algorithm>
 #include <optional>
 #include <string>
 #include <unordered_map>
+#include <utility>
+#include <vector>
 
 #include "arc_b200.h"
 
@@ -142,14 +144,78 @@ void expect_out(const Tensor& out, int64_t rows, int64_t cols, const at::Device&
   }
 }
 
+// The bytes of a tensor, as runs of `width` bytes: `rows` of them `pitch` apart, `blocks` of those rows
+// `step` apart (at most three dimensions, none of negative stride).
+struct Runs {
+  int64_t at = 0, width = 0, rows = 1, pitch = 0, blocks = 1, step = 0;
+  int64_t end() const { return at + width + (rows - 1) * pitch + (blocks - 1) * step; }
+};
+
+Runs runs_of(const Tensor& t) {
+  const int64_t item = t.element_size();
+  std::vector<std::pair<int64_t, int64_t>> dims;  // stride in bytes, size; smallest stride first
+  for (int64_t d = 0; d < t.dim(); ++d) {
+    if (t.size(d) > 1 && t.stride(d) > 0) dims.emplace_back(t.stride(d) * item, t.size(d));
+  }
+  std::sort(dims.begin(), dims.end());
+  Runs r;
+  r.at = reinterpret_cast<intptr_t>(t.const_data_ptr());
+  r.width = item;
+  size_t d = 0;
+  for (; d < dims.size() && dims[d].first <= r.width; ++d) r.width += (dims[d].second - 1) * dims[d].first;
+  if (dims.size() > d + 2) {  // no dimension without gaps: everything from the first byte to the last
+    for (; d < dims.size(); ++d) r.width += (dims[d].second - 1) * dims[d].first;
+  }
+  if (d < dims.size()) r.pitch = dims[d].first, r.rows = dims[d].second, ++d;
+  if (d < dims.size()) r.step = dims[d].first, r.blocks = dims[d].second;
+  return r;
+}
+
+// Whether a run of [at, at + width) meets one of `rows` runs of `own` bytes from byte 0 on, `pitch`
+// apart; the run itself may stand for `also` ones of the same pitch.
+bool meets(int64_t at, int64_t width, int64_t also, int64_t own, int64_t rows, int64_t pitch) {
+  // Rows i and j meet if at - own < (i - j) pitch < at + width.
+  if (pitch == 0) return at < own && at + width > 0;
+  const int64_t below = at - own;
+  int64_t m = below >= 0 ? below / pitch + 1 : -((-below - 1) / pitch);  // the least multiple above `below`
+  m = std::max(m, 1 - also);
+  return m <= rows - 1 && m * pitch < at + width;
+}
+
+// Whether two tensors (`a` of two dimensions at most) share a byte. Decided by addresses and strides,
+// exactly (but for operands of three dimensions that all have gaps): column slices of one buffer that
+// lie side by side share none. One look for tensors of one pitch, else one per row of `b`.
+bool share_bytes(const Tensor& ta, const Tensor& tb) {
+  if (ta.numel() == 0 || tb.numel() == 0) return false;
+  const Runs a = runs_of(ta), b = runs_of(tb);
+  if (a.end() <= b.at || b.end() <= a.at) return false;
+  const bool together = a.rows == 1 || b.rows == 1 || a.pitch == b.pitch;
+  const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
+  for (int64_t k = 0; k < b.blocks; ++k) {
+    for (int64_t j = 0; j < (together ? 1 : b.rows); ++j) {
+      const int64_t at = b.at + k * b.step + j * b.pitch - a.at;
+      if (meets(at, b.width, together ? b.rows : 1, a.width, a.rows, pitch)) return true;
+    }
+  }
+  return false;
+}
+
+// The same elements in the same order.
+bool same_view(const Tensor& a, const Tensor& b) {
+  if (a.const_data_ptr() != b.const_data_ptr() || a.sizes() != b.sizes()) return false;
+  for (int64_t d = 0; d < a.dim(); ++d) {
+    if (a.size(d) > 1 && a.stride(d) != b.stride(d)) return false;
+  }
+  return true;
+}
+
 // An `out` that is about to be written: not a tensor whose gradient is recorded, not one of the
 // operands that other blocks still read, and a new version for whoever has saved it.
 void claim_out(const OptTensor& out, std::initializer_list<const Tensor*> operands) {
   if (!out) return;
   if (at::GradMode::is_enabled() && out->requires_grad()) bad_value("out must not require a gradient");
   for (const Tensor* t : operands) {
-    const at::MemOverlapStatus s = at::get_overlap_status(*out, *t);
-    if (s == at::MemOverlapStatus::Full || s == at::MemOverlapStatus::Partial) bad_value("out must not overlap an operand");
+    if (share_bytes(*out, *t)) bad_value("out must not overlap an operand");
   }
   if (!out->is_inference()) out->unsafeGetTensorImpl()->bump_version();
 }
@@ -268,7 +334,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptTensor& bias, const Opt
   }
   const c10::cuda::CUDAGuard guard(dev);
   if (out) expect_out(*out, m, n, dev);
-  if (out && residual && at::get_overlap_status(*out, *residual) == at::MemOverlapStatus::Partial) {
+  if (out && residual && !same_view(*out, *residual) && share_bytes(*out, *residual)) {
     bad_value("out must be residual itself or not overlap it");
   }
   claim_out(out, {&x, &w, bias ? &*bias : &w});
@@ -361,7 +427,7 @@ Tensor grouped_matmul(const Tensor& x, const Tensor& w, const Tensor& offsets, c
   }
   const c10::cuda::CUDAGuard guard(dev);
   if (out) expect_out(*out, t, n, dev);
-  claim_out(out, {&x, &w});
+  claim_out(out, {&x, &w, &offsets});
   const Tensor y = out ? *out : at::empty({t, n}, x.options().requires_grad(false));
   if (t > 0) grouped_call(product_rows(x), product_rows(w), offsets, y, !out);
   return y;
@@ -391,7 +457,7 @@ Tensor a8w4_grouped_matmul(const Tensor& x, const Tensor& sa_in, const Tensor& w
   expect_offsets(offsets, e, dev);
   const c10::cuda::CUDAGuard guard(dev);
   if (out) expect(*out, "out", at::kBFloat16, {t, n}, dev);
-  claim_out(out, {&x, &sa, &wp, &sb});
+  claim_out(out, {&x, &sa, &wp, &sb, &offsets});
   const Tensor y = out ? *out : at::empty({t, n}, x.options().dtype(at::kBFloat16));
   if (t == 0) return y;
   size_t bytes = 0;

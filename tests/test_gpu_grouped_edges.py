@@ -1,0 +1,47 @@
+"""Edges of the grouped products on the B200: extreme scales, offsets that are not offsets."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import arc
+from linear_bounds import normal
+
+pytestmark = pytest.mark.gpu
+
+
+def _offsets(*values):
+    return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def test_out_that_overlaps_is_refused(cuda_device):
+    """Slices of one buffer, weights between the rows of out, and the offsets themselves."""
+    g = torch.Generator().manual_seed(0)
+    buf, w, offsets = normal(g, 32, 96), normal(g, 2, 32, 32), _offsets(0, 20, 32)
+    for c in (0, 8, 31):
+        with pytest.raises(ValueError, match="overlap"):
+            arc.grouped_matmul(buf[:, :32], w, offsets, out=buf[:, c:c + 32])
+    want = arc.grouped_matmul(buf[:, :32].clone(), w, offsets)
+    assert torch.equal(arc.grouped_matmul(buf[:, :32], w, offsets, out=buf[:, 32:64]), want)
+    flat = torch.zeros(2 * 40 * 96, dtype=torch.bfloat16, device="cuda")
+    x = normal(g, 32, 32)
+    weights = flat.view(2, 40, 96)[:, :32, :32]
+    for bad in (flat.view(80, 96)[8:40, 24:56], flat.view(80, 96)[40:72, 31:63]):
+        with pytest.raises(ValueError, match="overlap"):
+            arc.grouped_matmul(x, weights, offsets, out=bad)
+    weights.copy_(w)
+    want = arc.grouped_matmul(x, w, offsets)
+    for good in (flat.view(80, 96)[8:40, 32:64], flat.view(80, 96)[32:40, :32]):
+        off = _offsets(0, 3, good.shape[0])
+        want = arc.grouped_matmul(x[:good.shape[0]], w, off)
+        assert torch.equal(arc.grouped_matmul(x[:good.shape[0]], weights, off, out=good), want)
+    words = torch.zeros(8, 32, dtype=torch.bfloat16, device="cuda")
+    words.view(torch.int32).view(-1)[:3] = torch.tensor([0, 4, 8], dtype=torch.int32)
+    inside = words.view(torch.int32).view(-1)[:3]
+    with pytest.raises(ValueError, match="overlap"):
+        arc.grouped_matmul(x[:8], w, inside, out=words)
+    q, sa = torch.zeros(8, 128, dtype=torch.int8, device="cuda"), torch.ones(8, device="cuda")
+    wp = torch.zeros(2, 32, 64, dtype=torch.uint8, device="cuda")
+    sb = torch.ones(2, 32, 1, dtype=torch.bfloat16, device="cuda")
+    with pytest.raises(ValueError, match="overlap"):
+        arc.a8w4_grouped_matmul((q, sa), (wp, sb), inside, out=words)

@@ -1,0 +1,65 @@
+"""Edges of the linear layer on the B200: far tails of the activations, what a graph keeps, derivatives that
+are not offered."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import arc
+from linear_bounds import normal
+
+pytestmark = pytest.mark.gpu
+
+
+def _views(buf, *where):
+    """Row-major views of one buffer: (rows, columns) slices."""
+    return [buf[r, c] for r, c in where]
+
+
+def test_out_that_overlaps_inside_wider_rows_is_refused(cuda_device):
+    """Column slices of one buffer: refused where they share an element, taken where they lie side by side."""
+    s = slice
+    g = torch.Generator().manual_seed(0)
+    buf = normal(g, 40, 96)
+    w, b, r = normal(g, 32, 32, scale=0.2), normal(g, 32), normal(g, 32, 32)
+    for at_x, at_out in (((s(0, 32), s(0, 32)), (s(0, 32), s(16, 48))),    # columns meet
+                         ((s(0, 32), s(0, 32)), (s(0, 32), s(0, 32))),     # two views of one slice
+                         ((s(0, 32), s(32, 64)), (s(8, 40), s(56, 88))),   # a corner
+                         ((s(0, 32), s(0, 32)), (s(0, 32), s(31, 63))),    # one column
+                         ((s(31, 40), s(64, 96)), (s(23, 32), s(64, 96)))):  # one row
+        x, out = _views(buf, at_x, at_out)
+        with pytest.raises(ValueError, match="overlap"):
+            arc.linear(x, w, b, out=out)
+        wx, = _views(buf, (s(0, 32), s(0, 32)))
+        with pytest.raises(ValueError, match="overlap"):
+            arc.linear(normal(g, 32, 32), wx, out=_views(buf, (s(0, 32), s(24, 56)))[0])
+    # residual: itself or nothing of it
+    for at_r, at_out in (((s(0, 32), s(0, 32)), (s(0, 32), s(8, 40))), ((s(0, 32), s(0, 32)), (s(1, 33), s(0, 32))),
+                         ((s(0, 32), s(64, 96)), (s(0, 32), s(63, 95)))):
+        res, out = _views(buf, at_r, at_out)
+        with pytest.raises(ValueError, match="residual"):
+            arc.linear(normal(g, 32, 32), w, b, res, out=out)
+    # other pitches, one row, a bias inside out, transposed operands
+    flat = torch.zeros(40 * 96, dtype=torch.bfloat16, device="cuda")
+    out = flat.view(40, 96)[:32, 8:40]
+    for bad in (flat[1000:1000 + 1024].view(32, 32), flat.as_strided((32, 32), (64, 1), 100),
+                flat.as_strided((32, 32), (1, 96), 8)):
+        with pytest.raises(ValueError, match="overlap"):
+            arc.linear(bad, w, b, out=out)
+    for bad in (flat[96 * 3 + 8:96 * 3 + 40], flat[96 * 3 + 39:96 * 3 + 71]):
+        with pytest.raises(ValueError, match="overlap"):
+            arc.linear(r, w, bad, out=out)
+    # What shares nothing is taken, and right.
+    base = buf.clone()
+    for at_x, at_out in (((s(0, 32), s(0, 32)), (s(0, 32), s(32, 64))), ((s(0, 32), s(64, 96)), (s(8, 40), s(32, 64))),
+                         ((s(0, 20), s(0, 32)), (s(20, 40), s(0, 32))), ((s(0, 1), s(0, 32)), (s(1, 2), s(0, 32)))):
+        buf.copy_(base)
+        x, out = _views(buf, at_x, at_out)
+        want = arc.linear(x.clone(), w, b)
+        assert torch.equal(arc.linear(x, w, b, out=out), want)
+    gap = flat[96 * 3 + 40:96 * 3 + 72].copy_(b)  # a bias in the columns beside out
+    out = flat.view(40, 96)[:32, 8:40]
+    assert torch.equal(arc.linear(r, w, gap, out=out), arc.linear(r, w, b))
+    res, = _views(buf, (s(0, 32), s(5, 37)))
+    want = arc.linear(r, w, b, res.clone())
+    assert torch.equal(arc.linear(r, w, b, buf[0:32, 5:37], out=res), want)  # two views of the same slice: in place
