@@ -10,7 +10,8 @@ there, so no call waits for the host. Rows of no group (behind the last one, whe
 places the choices of ids outside [0, E)) never reach a result, whatever they hold; their
 output rows are left as they are when `out` is given and are zero otherwise.
 
-`grouped_matmul` is differentiable in x and w; `a8w4_grouped_matmul` is the serving form on
+`grouped_matmul` is differentiable in x and w (once, in reverse mode; a second derivative or a
+forward-mode tangent is refused); `a8w4_grouped_matmul` is the serving form on
 int8 activations and int4 weights, with the operands of `arc.a8w4_matmul`. Offsets that
 decrease or leave the rows give unspecified values and set bit 7 of `arc.device_status`.
 """

@@ -4,7 +4,8 @@
 
 `linear` is one launch of `arc_linear_bf16` (include/arc_b200.h) on the caller's stream: the product accumulates in
 fp32, bias, activation and residual are applied to the fp32 value and the result is rounded
-to bf16 once. It is differentiable in x, w, bias and residual:
+to bf16 once. It is differentiable in x, w, bias and residual
+(once, in reverse mode; a second derivative or a forward-mode tangent is refused):
 
     dz = dout * act'(z)   z = x . w^T + bias
     dx = dz . w           dw = dz^T . x         dbias = sum_m dz         dresidual = dout

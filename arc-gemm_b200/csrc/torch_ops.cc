@@ -10,6 +10,7 @@
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/extension.h>
 
+#include <c10/core/AutogradState.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 
@@ -225,6 +226,17 @@ cudaStream_t stream_of(const Tensor& t) { return c10::cuda::getCurrentCUDAStream
 bool wants_grad(const Tensor& t) { return t.requires_grad(); }
 bool wants_grad(const OptTensor& t) { return t.has_value() && t->requires_grad(); }
 
+// Forward-mode derivatives are not offered. A tangent must not be dropped unnoticed, whatever the grad
+// mode: the result would pass for a constant.
+bool has_tangent(const Tensor& t) { return t._fw_grad(/*level=*/0).defined(); }
+bool has_tangent(const OptTensor& t) { return t.has_value() && has_tangent(*t); }
+template <typename... Ts>
+void refuse_tangents(const Ts&... ts) {
+  if (c10::AutogradState::get_tls_state().get_fw_grad_mode() && (has_tangent(ts) || ...)) {
+    throw std::runtime_error("arc's operators have no forward-mode derivative, and an argument carries a tangent");
+  }
+}
+
 // The gradients are not differentiable themselves: a second derivative raises, by dy or by the
 // operands (grad mode is on in a backward pass only for create_graph).
 torch::autograd::variable_list once(torch::autograd::variable_list grads) {
@@ -328,6 +340,7 @@ Tensor linear(const Tensor& x, const Tensor& w, const OptTensor& bias, const Opt
     expect_shape(*residual, "residual", {m, n});
     expect_device(*residual, "residual", dev);
   }
+  refuse_tangents(x, w, bias, residual, out);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w) || wants_grad(bias) || wants_grad(residual))) {
     if (out) bad_value("out cannot be given when an input requires a gradient");
     return LinearFunction::apply(x, w, bias, residual, act);
@@ -421,6 +434,7 @@ Tensor grouped_matmul(const Tensor& x, const Tensor& w, const Tensor& offsets, c
   if (n == 0 || k == 0) bad_value("w must not be empty, got shape ", shape_of(w));
   as_int(t, "T"), as_int(n, "N"), as_int(k, "K");
   expect_offsets(offsets, w.size(0), dev);
+  refuse_tangents(x, w, out);
   if (at::GradMode::is_enabled() && (wants_grad(x) || wants_grad(w))) {
     if (out) bad_value("out cannot be given when an input requires a gradient");
     return GroupedFunction::apply(x, w, offsets);
@@ -455,6 +469,7 @@ Tensor a8w4_grouped_matmul(const Tensor& x, const Tensor& sa_in, const Tensor& w
   expect(wp, "b[0]", at::kByte, {e, n, k / 2}, dev);
   expect(sb, "b[1]", at::kBFloat16, {e, n, k / kScaleGroup}, dev);
   expect_offsets(offsets, e, dev);
+  refuse_tangents(sa, sb, out);
   const c10::cuda::CUDAGuard guard(dev);
   if (out) expect(*out, "out", at::kBFloat16, {t, n}, dev);
   claim_out(out, {&x, &sa, &wp, &sb, &offsets});

@@ -3,6 +3,7 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import arc
 from linear_bounds import normal
@@ -12,6 +13,24 @@ pytestmark = pytest.mark.gpu
 
 def _offsets(*values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+def test_forward_gradients_are_refused(cuda_device):
+    g = torch.Generator().manual_seed(0)
+    x, w, offsets = normal(g, 8, 16), normal(g, 2, 24, 16), _offsets(0, 4, 8)
+    with forward_ad.dual_level():
+        for args in ((forward_ad.make_dual(x, torch.ones_like(x)), w), (x, forward_ad.make_dual(w, torch.ones_like(w)))):
+            for no_grad in (False, True):
+                with torch.set_grad_enabled(not no_grad), pytest.raises(RuntimeError, match="forward"):
+                    arc.grouped_matmul(*args, offsets)
+        sa = forward_ad.make_dual(torch.ones(8, device="cuda"), torch.ones(8, device="cuda"))
+        q = torch.zeros(8, 128, dtype=torch.int8, device="cuda")
+        wp = torch.zeros(2, 8, 64, dtype=torch.uint8, device="cuda")
+        sb = torch.ones(2, 8, 1, dtype=torch.bfloat16, device="cuda")
+        with pytest.raises(RuntimeError, match="forward"):
+            arc.a8w4_grouped_matmul((q, sa), (wp, sb), offsets)
+        with pytest.raises(RuntimeError, match="forward"):
+            arc.a8w4_grouped_matmul((q, torch.ones(8, device="cuda")), (wp, forward_ad.make_dual(sb, sb)), offsets)
 
 
 def test_out_that_overlaps_is_refused(cuda_device):

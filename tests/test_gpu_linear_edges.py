@@ -4,11 +4,29 @@ from __future__ import annotations
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 import arc
 from linear_bounds import normal
 
 pytestmark = pytest.mark.gpu
+
+
+def test_forward_gradients_are_refused(cuda_device):
+    """A forward-mode derivative is not offered; it must not be dropped unnoticed."""
+    g = torch.Generator().manual_seed(0)
+    x, w, b, r = normal(g, 4, 16), normal(g, 24, 16), normal(g, 24), normal(g, 4, 24)
+    with forward_ad.dual_level():
+        for i in range(4):
+            args = [x, w, b, r]
+            args[i] = forward_ad.make_dual(args[i], torch.ones_like(args[i]))
+            for no_grad in (False, True):
+                with torch.set_grad_enabled(not no_grad), pytest.raises(RuntimeError, match="forward"):
+                    arc.linear(*args)
+        out = forward_ad.make_dual(r.clone(), torch.ones_like(r))
+        with pytest.raises(RuntimeError, match="forward"):
+            arc.linear(x, w, b, out=out)
+    assert arc.linear(x, w, b, r).shape == (4, 24)
 
 
 def _views(buf, *where):
