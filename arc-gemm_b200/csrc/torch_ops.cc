@@ -275,7 +275,11 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       linear_call(x, w, bias ? OptTensor(bias->contiguous()) : bias, residual ? OptTensor(unit_rows(*residual)) : residual,
                   out, z, static_cast<int>(act));
     }
-    ctx->save_for_backward({x, w, z});
+    // Only what a gradient will read: the rest may change or be freed.
+    ctx->save_for_backward({wants_grad(w_in) ? x : Tensor(), wants_grad(x_in) ? w : Tensor(), z});
+    ctx->saved_data["m"] = m;
+    ctx->saved_data["n"] = n;
+    ctx->saved_data["k"] = x.size(1);
     ctx->saved_data["act"] = act;
     ctx->saved_data["bias"] = wants_grad(bias);
     ctx->saved_data["residual"] = wants_grad(residual);
@@ -291,12 +295,12 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     const Tensor& dy_in = grads[0];
     const bool need_x = ctx->saved_data["x"].toBool(), need_w = ctx->saved_data["w"].toBool(),
                need_bias = ctx->saved_data["bias"].toBool(), need_residual = ctx->saved_data["residual"].toBool();
-    const int64_t m = x.size(0), n = w.size(0), k = x.size(1);
+    const int64_t m = ctx->saved_data["m"].toInt(), n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
     torch::autograd::variable_list out(5);
     if (!dy_in.defined()) return out;
     if (need_residual) out[3] = dy_in;
     if (!(need_x || need_w || need_bias)) return out;
-    const c10::cuda::CUDAGuard guard(x.device());
+    const c10::cuda::CUDAGuard guard(dy_in.device());
     const Tensor dy = unit_rows(dy_in.detach());
     const auto options = dy.options();
     if (need_x) out[0] = at::empty({m, k}, options);
@@ -308,11 +312,13 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       check(g_api.linear_backward_ws(m, n, need_dz, need_bias, &bytes), "arc.linear backward");
       Tensor workspace;
       if (bytes > 0) workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
-      check(g_api.linear_backward(u16(dy), u16(x), u16(w), z.defined() ? u16(z) : nullptr,
+      check(g_api.linear_backward(u16(dy), need_w ? u16(x) : nullptr, need_x ? u16(w) : nullptr,
+                                  z.defined() ? u16(z) : nullptr,
                                   need_x ? u16_mut(out[0]) : nullptr, need_w ? u16_mut(out[1]) : nullptr,
                                   need_bias ? u16_mut(out[2]) : nullptr, bytes > 0 ? workspace.data_ptr() : nullptr,
-                                  bytes, m, n, k, row_ld(dy), x.stride(0), w.stride(0), z.defined() ? z.stride(0) : 0,
-                                  k, k, static_cast<int>(ctx->saved_data["act"].toInt()), stream_of(x)),
+                                  bytes, m, n, k, row_ld(dy), need_w ? x.stride(0) : 0, need_x ? w.stride(0) : 0,
+                                  z.defined() ? z.stride(0) : 0, k, k,
+                                  static_cast<int>(ctx->saved_data["act"].toInt()), stream_of(dy)),
             "arc.linear backward");
     }
     return once(std::move(out));
@@ -385,9 +391,14 @@ struct GroupedFunction : torch::autograd::Function<GroupedFunction> {
     const Tensor x = product_rows(x_in), w = product_rows(w_in);
     Tensor out = at::empty({x.size(0), w.size(1)}, x.options().requires_grad(false));
     if (x.size(0) > 0) grouped_call(x, w, offsets, out, true);
-    ctx->save_for_backward({x, w, offsets});
+    // Only what a gradient will read: the rest may change or be freed.
+    ctx->save_for_backward({wants_grad(w_in) ? x : Tensor(), wants_grad(x_in) ? w : Tensor(), offsets});
     ctx->saved_data["x"] = wants_grad(x_in);
     ctx->saved_data["w"] = wants_grad(w_in);
+    ctx->saved_data["t"] = x.size(0);
+    ctx->saved_data["e"] = w.size(0);
+    ctx->saved_data["n"] = w.size(1);
+    ctx->saved_data["k"] = w.size(2);
     return out;
   }
 
@@ -396,10 +407,11 @@ struct GroupedFunction : torch::autograd::Function<GroupedFunction> {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
     const Tensor& dy_in = grads[0];
-    const int64_t t = x.size(0), k = x.size(1), e = w.size(0), n = w.size(1);
+    const int64_t t = ctx->saved_data["t"].toInt(), e = ctx->saved_data["e"].toInt(), n = ctx->saved_data["n"].toInt(),
+                  k = ctx->saved_data["k"].toInt();
     torch::autograd::variable_list out(3);
     if (!dy_in.defined()) return out;
-    const c10::cuda::CUDAGuard guard(x.device());
+    const c10::cuda::CUDAGuard guard(dy_in.device());
     const char* what = "arc.grouped_matmul backward";
     const auto options = dy_in.options().requires_grad(false);
     if (t == 0) {
@@ -411,13 +423,13 @@ struct GroupedFunction : torch::autograd::Function<GroupedFunction> {
     if (ctx->saved_data["x"].toBool()) {
       out[0] = at::empty({t, k}, options);
       check(g_api.grouped_dx(u16(dy), u16(w), offsets.const_data_ptr<int32_t>(), u16_mut(out[0]), t, e, n, k,
-                             dy.stride(0), w.stride(1), w.stride(0), k, ARC_GROUPED_ZERO_OTHERS, stream_of(x)),
+                             dy.stride(0), w.stride(1), w.stride(0), k, ARC_GROUPED_ZERO_OTHERS, stream_of(dy)),
             what);
     }
     if (ctx->saved_data["w"].toBool()) {
       out[1] = at::empty({e, n, k}, options);
       check(g_api.grouped_dw(u16(dy), u16(x), offsets.const_data_ptr<int32_t>(), u16_mut(out[1]), t, e, n, k,
-                             dy.stride(0), x.stride(0), k, n * k, stream_of(x)),
+                             dy.stride(0), x.stride(0), k, n * k, stream_of(dy)),
             what);
     }
     return once(std::move(out));

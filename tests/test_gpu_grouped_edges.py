@@ -6,7 +6,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import arc
-from linear_bounds import normal
+from linear_bounds import H, normal
 
 pytestmark = pytest.mark.gpu
 
@@ -31,6 +31,30 @@ def test_forward_gradients_are_refused(cuda_device):
             arc.a8w4_grouped_matmul((q, sa), (wp, sb), offsets)
         with pytest.raises(RuntimeError, match="forward"):
             arc.a8w4_grouped_matmul((q, torch.ones(8, device="cuda")), (wp, forward_ad.make_dual(sb, sb)), offsets)
+
+
+def test_operands_that_no_gradient_needs_may_change(cuda_device):
+    g = torch.Generator().manual_seed(0)
+    x, w, dy, offsets = normal(g, 8, 16), normal(g, 2, 24, 16), normal(g, 8, 24), _offsets(0, 5, 8)
+    lx, frozen = x.clone().requires_grad_(), w.clone()
+    y = arc.grouped_matmul(lx, frozen, offsets)
+    with torch.no_grad():
+        lx.mul_(2)  # dx does not need x
+    (dx,) = torch.autograd.grad(y, [lx], dy)
+    want = torch.cat((dy[:5].double() @ w[0].double(), dy[5:].double() @ w[1].double()))
+    assert (dx.double() - want).norm() <= 2 * H * want.norm()
+    lw, data = w.clone().requires_grad_(), x.clone()
+    y = arc.grouped_matmul(data, lw, offsets)
+    with torch.no_grad():
+        lw.mul_(2)  # dw does not need w
+    (dw,) = torch.autograd.grad(y, [lw], dy)
+    want = torch.stack((dy[:5].double().T @ x[:5].double(), dy[5:].double().T @ x[5:].double()))
+    assert (dw.double() - want).norm() <= 2 * H * want.norm()
+    for changed in (data, offsets):
+        y = arc.grouped_matmul(data, lw, offsets)
+        changed.mul_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, [lw], dy)
 
 
 def test_out_that_overlaps_is_refused(cuda_device):

@@ -7,7 +7,7 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import arc
-from linear_bounds import normal
+from linear_bounds import H, normal, slope64
 
 pytestmark = pytest.mark.gpu
 
@@ -27,6 +27,48 @@ def test_forward_gradients_are_refused(cuda_device):
         with pytest.raises(RuntimeError, match="forward"):
             arc.linear(x, w, b, out=out)
     assert arc.linear(x, w, b, r).shape == (4, 24)
+
+
+def test_operands_that_no_gradient_needs_may_change(cuda_device):
+    """The graph keeps what its gradients need: x for dw, w for dx. The other one may be written."""
+    g = torch.Generator().manual_seed(0)
+    x, w, dy = normal(g, 4, 16), normal(g, 24, 16), normal(g, 4, 24)
+    for act in (None, "silu"):
+        slope = slope64(x.double() @ w.double().T, act)
+        lx = x.clone().requires_grad_()
+        frozen = w.clone()
+        y = arc.linear(lx, frozen, activation=act)
+        h = lx.detach()
+        with torch.no_grad():
+            h.mul_(2)  # dx does not need x
+        (dx,) = torch.autograd.grad(y, [lx], dy)
+        want = (dy.double() * slope) @ w.double()
+        assert (dx.double() - want).norm() <= 4 * H * want.norm()
+        lw, data = w.clone().requires_grad_(), x.clone()
+        y = arc.linear(data, lw, activation=act)
+        with torch.no_grad():
+            lw.mul_(2)  # dw does not need w
+        (dw,) = torch.autograd.grad(y, [lw], dy)
+        want = (dy.double() * slope).T @ x.double()
+        assert (dw.double() - want).norm() <= 4 * H * want.norm()
+        # What a gradient does need is still watched.
+        y = arc.linear(data, lw, activation=act)
+        data.mul_(2)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(y, [lw], dy)
+
+
+def test_frozen_operands_are_not_kept_alive(cuda_device):
+    """Activations in front of a frozen layer are freed as soon as their own graph lets them go."""
+    w = torch.zeros(64, 4096, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    lx = torch.zeros(4096, 4096, dtype=torch.bfloat16, device="cuda", requires_grad=True)
+    h = lx * 1.0
+    before = torch.cuda.memory_allocated()
+    y = arc.linear(h, w)
+    del h
+    assert torch.cuda.memory_allocated() <= before - 4096 * 4096 * 2 + 2 * y.numel() * 2
+    y.sum().backward()
 
 
 def _views(buf, *where):
