@@ -298,8 +298,10 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
     const int64_t m = ctx->saved_data["m"].toInt(), n = ctx->saved_data["n"].toInt(), k = ctx->saved_data["k"].toInt();
     torch::autograd::variable_list out(5);
     if (!dy_in.defined()) return out;
-    if (need_residual) out[3] = dy_in;
-    if (!(need_x || need_w || need_bias)) return out;
+    if (!(need_x || need_w || need_bias)) {
+      if (need_residual) out[3] = dy_in;
+      return out;
+    }
     const c10::cuda::CUDAGuard guard(dy_in.device());
     const Tensor dy = unit_rows(dy_in.detach());
     const auto options = dy.options();
@@ -321,7 +323,9 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
                                   static_cast<int>(ctx->saved_data["act"].toInt()), stream_of(dy)),
             "arc.linear backward");
     }
-    return once(std::move(out));
+    out = once(std::move(out));
+    if (need_residual) out[3] = dy_in;  // the identity, which can be differentiated again
+    return out;
   }
 };
 

@@ -71,6 +71,18 @@ def test_frozen_operands_are_not_kept_alive(cuda_device):
     y.sum().backward()
 
 
+def test_residual_gradient_can_be_differentiated(cuda_device):
+    """dresidual is dy itself, with other gradients asked for or without."""
+    g = torch.Generator().manual_seed(0)
+    x, w, r = normal(g, 4, 16), normal(g, 24, 16), normal(g, 4, 24)
+    for frozen in (True, False):
+        lr, lx = r.clone().requires_grad_(), x.clone().requires_grad_(not frozen)
+        dy = normal(g, 4, 24).requires_grad_()
+        (dr,) = torch.autograd.grad(arc.linear(lx, w, None, lr), [lr], dy, create_graph=True)
+        (ddy,) = torch.autograd.grad(dr.sum(), [dy])
+        assert (ddy == 1).all()
+
+
 def _views(buf, *where):
     """Row-major views of one buffer: (rows, columns) slices."""
     return [buf[r, c] for r, c in where]
