@@ -306,8 +306,15 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
         tc_fence_after_sync();
         const uint32_t d_tmem = tmem_base + acc * kTileT;
         for (uint32_t kb = 0; kb < p.num_kb; ++kb) {
-          ok = mbar_wait_all2(&s.full[stage], phase, full, &s.expanded[stage], phase, W4 ? expanded : 1u, abort,
-                              kStatusTimeoutMma);
+          if constexpr (W4) {
+            // `full` also stands for the weights that rank 1 has expanded into its shared memory.
+            ok = __all_sync(0xffffffffu,
+                            (full != 0u || mbar_wait_relaxed(&s.full[stage], phase, abort, kStatusTimeoutMma)) &&
+                                (expanded != 0u || mbar_wait(&s.expanded[stage], phase, abort, kStatusTimeoutMma)));
+            fence_acquire_cluster_smem();
+          } else {
+            ok = __all_sync(0xffffffffu, full != 0u || mbar_wait(&s.full[stage], phase, abort, kStatusTimeoutMma));
+          }
           if (!ok) break;
           tc_fence_after_sync();
           const uint64_t adesc = lin::operand_desc<W_MN>(s.a[stage]);
@@ -326,7 +333,7 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
           }
           // A test takes about 180 cycles to answer, a third of a stage's products: the next
           // stage's are asked together, and early.
-          full = mbar_test(&s.full[stage], phase);
+          full = W4 ? mbar_test_relaxed(&s.full[stage], phase) : mbar_test(&s.full[stage], phase);
           if (W4) expanded = mbar_test(&s.expanded[stage], phase);
           if (kb == 0u) more = tile_at(p, s.prefix, t + num_pairs, next);
         }
@@ -377,9 +384,12 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
       for (uint32_t t = pair; ok && tile_at(p, s.prefix, t, w); t += num_pairs) {
         for (uint32_t kb = 0; kb < p.num_kb && ok; ++kb) {
           ok = mbar_wait_poll(&s.expanded[stage], phase, abort, kStatusTimeoutUnpack);
-          // The expanded weights lie in this CTA's shared memory, where only this SM's tensor core
-          // reads them, and were made visible to it (fence.proxy.async) before "expanded".
-          if (ok) mbar_arrive_cluster_relaxed(map_to_rank(&s.full[stage], 0));
+          // The expanding warps made their writes visible to the tensor core (fence.proxy.async) in front
+          // of "expanded"; this passes them on to the thread of rank 0 that issues the product.
+          if (ok) {
+            fence_release_cluster_smem();
+            mbar_arrive_cluster_relaxed(map_to_rank(&s.full[stage], 0));
+          }
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;

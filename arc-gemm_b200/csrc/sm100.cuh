@@ -251,6 +251,56 @@ __device__ __forceinline__ uint32_t mbar_test(uint64_t* bar, uint32_t parity) {
   return ok;
 }
 
+// A hand-off between CTAs of a cluster through shared memory alone. The thread that announces its CTA's
+// writes (its own, or ones it has waited for) releases them with the first fence in front of
+// mbar_arrive_cluster_relaxed; the waiter sees the phase with the relaxed forms below and acquires with
+// the second fence. Restricted to shared memory the fences cost nothing measurable, where a release of
+// all memory at cluster scope holds the announcing thread up for some 1700 cycles.
+__device__ __forceinline__ void fence_release_cluster_smem() {
+  asm volatile("fence.release.sync_restrict::shared::cta.cluster;" ::: "memory");
+}
+__device__ __forceinline__ void fence_acquire_cluster_smem() {
+  asm volatile("fence.acquire.sync_restrict::shared::cluster.cluster;" ::: "memory");
+}
+
+__device__ __forceinline__ uint32_t mbar_test_relaxed(uint64_t* bar, uint32_t parity) {
+  uint32_t ok;
+  asm volatile(
+      "{\n\t.reg .pred P;\n\t"
+      "mbarrier.test_wait.parity.relaxed.cluster.shared::cta.b64 P, [%1], %2;\n\t"
+      "selp.u32 %0, 1, 0, P;\n\t}"
+      : "=r"(ok)
+      : "r"(smem_u32(bar)), "r"(parity)
+      : "memory");
+  return ok;
+}
+
+__device__ __forceinline__ bool mbar_wait_relaxed(uint64_t* bar, uint32_t parity, volatile uint32_t* abort,
+                                                  uint32_t err_bit) {
+  const uint32_t addr = smem_u32(bar);
+  const uint64_t start = globaltimer_ns();
+#pragma unroll 1
+  for (uint32_t it = 1;; ++it) {
+    uint32_t ok;
+    asm volatile(
+        "{\n\t.reg .pred P;\n\t"
+        "mbarrier.try_wait.parity.relaxed.cluster.shared::cta.b64 P, [%1], %2, %3;\n\t"
+        "selp.u32 %0, 1, 0, P;\n\t}"
+        : "=r"(ok)
+        : "r"(addr), "r"(parity), "r"(20000u)
+        : "memory");
+    if (ok) return true;
+    if ((it & 15u) == 0u) {
+      if (*abort) return false;
+      if (globaltimer_ns() - start > kWaitTimeoutNs) {
+        *abort = 1u;
+        atomicOr(&g_arc_status, err_bit);
+        return false;
+      }
+    }
+  }
+}
+
 // Warp-wide bounded wait on up to two barriers. Every lane tests and waits for
 // itself (each lane's wait is its own acquire), skipping a barrier whose completion
 // it already saw in an earlier mbar_test (`pre1`, `pre2`; pass 1 for "no wait"),
@@ -648,8 +698,8 @@ __device__ __forceinline__ void mbar_arrive_cluster(uint32_t cluster_addr) {
 
 // The same without ordering memory at cluster scope: a release there holds the arriving thread up
 // for about 1700 cycles, and longer while stores of its own are in flight. For announcements that
-// need no such order: accumulators read (the reads have completed, tcgen05.wait::ld), or operands
-// that only this SM's tensor core reads and that were made visible to it before.
+// need no such order (accumulators read: the reads have completed, tcgen05.wait::ld), or whose order
+// fence_release_cluster_smem gives.
 __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t cluster_addr) {
   asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(cluster_addr) : "memory");
 }
