@@ -286,7 +286,7 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
   //   pair released   24-31 unpack waits passed   32-39 stage unpacked   40-47 loads
   //   issued   48-55 step accumulated   56 entry   57 prologue done   59 exit
   if (threadIdx.x == 0) probe_mark(56);
-  pdl_launch_dependents();
+  if constexpr (!kGrouped) pdl_launch_dependents();
   if (warp == 0 && lane == 0) {
     tma_prefetch_desc(&p.tm_tok);
     tma_prefetch_desc(&p.tm_wp);
@@ -297,6 +297,9 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
     s.abort = 0;
     fence_barrier_init();
   }
+  // Grouped: TMEM is taken only after the preceding grid has ended, and the next grid is let in only
+  // after it is taken (see gemm_linear_stream.cuh).
+  if constexpr (kGrouped) pdl_wait();
   if (warp == 2) {
     tmem_alloc(&s.tmem_base, C::kTmemCols);
     tmem_relinquish();
@@ -304,6 +307,10 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  if constexpr (kGrouped) {
+    pdl_launch_dependents();
+    if (warp == 2) lin::group_tiles_prefix(p.groups, BT, s.prefix);
+  }
   const uint32_t tmem_base = s.tmem_base;
   if (warp >= C::kEpiWarp) {
     // Arm every accumulator with the bias before the first UMMA may touch it.
@@ -321,12 +328,10 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
   tc_fence_after_sync();
   // The prologue above may overlap the previous grid in the stream (programmatic
   // dependent launch); global memory is only touched after it has completed.
-  pdl_wait();
+  if constexpr (!kGrouped) pdl_wait();
   if (threadIdx.x == 0) probe_mark(57);
   if constexpr (kGrouped) {
-    if (warp == 2) lin::group_tiles_prefix(p.groups, BT, s.prefix);
     if (p.zero_others) lin::zero_other_rows(p.groups, p.out, p.ldc, p.N, blockIdx.x, gridDim.x);
-    __syncthreads();
   }
   const auto next = [&](uint32_t& cursor, Work& w) {
     if constexpr (kGrouped) {

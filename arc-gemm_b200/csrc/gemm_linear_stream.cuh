@@ -152,21 +152,19 @@ __global__ void __launch_bounds__(kThreads, 2) gemm_linear_stream_kernel(const _
     s.abort = 0;
     fence_barrier_init();
   }
+  // TMEM is taken only after the preceding grid has ended, and the next grid is let in only after it
+  // is taken: whatever kernels stand beside this one on the stream, none waits for columns that are
+  // held by one that waits for it.
+  pdl_wait();
   if (warp == 1) {
     tmem_alloc(&s.tmem_base, C::kTmemCols);
     tmem_relinquish();
   }
-  // The next grid is let in only after TMEM is taken. Taking it before the preceding grid has
-  // ended cannot hold that one up either: this kernel's blocks, and all others of the library
-  // that use TMEM, need so much shared memory that an SM holds at most two, of at most 256
-  // columns each.
-  __syncthreads();
-  pdl_launch_dependents();
-  pdl_wait();
   if (warp == 2 && p.groups.offsets != nullptr) lin::group_tiles_prefix(p.groups, BN, s.prefix);
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
+  pdl_launch_dependents();
   const uint32_t tmem_base = s.tmem_base;
   if (p.zero_others) lin::zero_other_rows(p.groups, p.out, p.ldo, p.cols, blockIdx.x, gridDim.x);
 
