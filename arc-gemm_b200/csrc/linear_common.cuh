@@ -115,29 +115,34 @@ __device__ __forceinline__ float gelu_tanh_arg(float z) {
   return 2.f * kSqrt2OverPi * (z + kGeluCubic * z * z * z);
 }
 
-// The erf form, two values at once: z Phi(z) = max(z, 0) - |z| q / 2 with q = 1 - erf(|z| / sqrt 2),
-// where nothing cancels. q = (1 + a1 x + ... + a6 x^6)^-16 by formula 7.1.28 of Abramowitz and
-// Stegun (Handbook of Mathematical Functions), off by at most 3e-7 (and by 3e-6 of itself in fp32,
-// through the 16th power): one reciprocal and packed products, where the special-function unit
-// would bound a formula with an exponential. x stops at 16, where q has long been 0.
+// q(y) = 1 - erf(y / sqrt 2) = t R(t) exp(-y^2 / 2), t = 1 / (1 + p y): the form of formula 7.1.26 of
+// Abramowitz and Stegun (Handbook of Mathematical Functions) with seven terms, fitted here for the
+// least relative error (minimax by linear programming on 0 <= y <= 13.5, where q leaves fp32: 6e-7,
+// and 9e-6 in fp32, through the exponential's argument). q's own accuracy is what the lower tail of
+// the activation needs: with a formula of an absolute bound (7.1.28, 3e-7) gelu(-5) was off by 5 %.
+constexpr float kTailP = 0.265f;
+__device__ __forceinline__ constexpr float tail_term(int i) {
+  constexpr float c[7] = {0.21120048617f, 0.21566298207f, 0.16594652836f, 0.28485278664f,
+                          -0.13254834990f, 0.39042731883f, -0.13554236419f};
+  return c[i];
+}
+
+// The erf form, two values at once: z Phi(z) = max(z, 0) - |z| q(|z|) / 2, where nothing cancels. The
+// pair shares one reciprocal; the rest are packed products and an exponential each. |z| stops at 16,
+// where q is 0 in fp32.
 __device__ __forceinline__ void gelu_pair(float& z0, float& z1) {
-  constexpr float r = kSqrtHalf;  // the formula's argument is |z| r: powers of r go into its factors
-  const float x0 = fminf(fabsf(z0), 16.f), x1 = fminf(fabsf(z1), 16.f);
-  const uint64_t x = f32x2_pack(x0, x1);
+  const float y0 = fminf(fabsf(z0), 16.f), y1 = fminf(fabsf(z1), 16.f);
+  const uint64_t y = f32x2_pack(y0, y1);
   const auto both = [](float c) { return f32x2_pack(c, c); };
-  uint64_t t = f32x2_fma(x, both(0.0000430638f * r * r * r * r * r * r), both(0.0002765672f * r * r * r * r * r));
-  t = f32x2_fma(x, t, both(0.0001520143f * r * r * r * r));
-  t = f32x2_fma(x, t, both(0.0092705272f * r * r * r));
-  t = f32x2_fma(x, t, both(0.0422820123f * r * r));
-  t = f32x2_fma(x, t, both(0.0705230784f * r));
-  t = f32x2_fma(x, t, both(1.f));
-  t = f32x2_mul(t, t);
-  t = f32x2_mul(t, t);
-  t = f32x2_mul(t, t);
-  t = f32x2_mul(t, t);
-  float p0, p1;
-  f32x2_unpack(t, p0, p1);
-  const uint64_t h = f32x2_mul(x, f32x2_pack(rcp_ftz(p0), rcp_ftz(p1)));
+  float d0, d1, e0, e1;
+  f32x2_unpack(f32x2_fma(y, both(kTailP), both(1.f)), d0, d1);
+  f32x2_unpack(f32x2_mul(f32x2_mul(y, both(-0.5f * kLog2E)), y), e0, e1);
+  const float r = rcp_ftz(d0 * d1);
+  const uint64_t t = f32x2_pack(r * d1, r * d0);
+  uint64_t q = f32x2_fma(t, both(tail_term(6)), both(tail_term(5)));
+#pragma unroll
+  for (int i = 4; i >= 0; --i) q = f32x2_fma(t, q, both(tail_term(i)));
+  const uint64_t h = f32x2_mul(f32x2_mul(f32x2_mul(t, q), y), f32x2_pack(ex2_ftz(e0), ex2_ftz(e1)));
   f32x2_unpack(f32x2_fma(h, both(-0.5f), f32x2_pack(relu_nan(z0), relu_nan(z1))), z0, z1);
 }
 
@@ -159,17 +164,18 @@ __device__ __forceinline__ float act_value(float z, uint32_t act) {
   }
 }
 
-// d act / d z. The erf form: Phi(z) + z phi(z) with e = exp(-z^2 / 2) and, by formula 7.1.26 of
-// the same book, 1 - erf(x) = (a1 t + ... + a5 t^5) e, t = 1 / (1 + p x), off by at most 1.5e-7.
+// d act / d z. The erf form: Phi(z) + z phi(z), with q as above.
 __device__ __forceinline__ float act_slope(float z, uint32_t act) {
   switch (act) {
     case kActRelu:
       return z > 0.f ? 1.f : 0.f;
     case kActGelu: {
-      const float t = rcp_ftz(fmaf(0.3275911f * kSqrtHalf, fabsf(z), 1.f));
+      const float t = rcp_ftz(fmaf(kTailP, fminf(fabsf(z), 16.f), 1.f));
       const float e = ex2_ftz(-0.5f * kLog2E * z * z);
-      const float q =
-          t * fmaf(t, fmaf(t, fmaf(t, fmaf(t, 1.061405429f, -1.453152027f), 1.421413741f), -0.284496736f), 0.254829592f) * e;
+      float q = tail_term(6);
+#pragma unroll
+      for (int i = 5; i >= 0; --i) q = fmaf(t, q, tail_term(i));
+      q *= t * e;
       return (z < 0.f ? 0.5f * q : fmaf(-0.5f, q, 1.f)) + z * kInvSqrt2Pi * e;
     }
     case kActGeluTanh: {

@@ -7,9 +7,41 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import arc
-from linear_bounds import H, normal, slope64
+from linear_bounds import H, act64, normal, slope64
 
 pytestmark = pytest.mark.gpu
+
+
+def _on_a_grid(values, act):
+    """arc.linear with z = the given bf16 values exactly: x is zero and the bias holds them."""
+    b = torch.tensor(values, dtype=torch.float64).to(torch.bfloat16).cuda()
+    x = torch.zeros(3, 8, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(b.numel(), 8, dtype=torch.bfloat16, device="cuda")
+    return b, arc.linear(x, w, b, activation=act)
+
+
+@pytest.mark.parametrize("act", ["gelu", "gelu_tanh", "silu"])
+def test_lower_tails_are_relatively_accurate(cuda_device, act):
+    """Where an activation is small it is still right relative to itself, as long as it is a normal number.
+
+    The exponential's argument is at most 128 in powers of two and has up to six roundings of 2^-24
+    behind it: 6 * 128 * ln 2 * 2^-24 = 2^-15 of the result. The approximations are within 2^-19, the
+    products behind them 2^-22. 2^-14 is allowed for all, beside the rounding to bf16.
+    """
+    z = torch.linspace(-13, 4, 1400).tolist()
+    b, got = _on_a_grid(z, act)
+    if act == "gelu":  # erfc, not 1 + erf, which cancels in 64 bits too
+        want = 0.5 * b.double() * torch.special.erfc(-b.double() * 0.5 ** 0.5)
+    elif act == "gelu_tanh":
+        u = (2 / torch.pi) ** 0.5 * (b.double() + 0.044715 * b.double() ** 3)
+        want = b.double() / (1 + torch.exp(-2 * u))
+    else:
+        want = act64(b.double(), act)
+    normal_range = want.abs() > 2.0 ** -120
+    assert normal_range.sum() > 1000
+    off = (got.double() - want).abs() / want.abs().clamp_min(2.0 ** -120)
+    assert off[:, normal_range].max() <= (H + 2.0 ** -14) * 1.001, off[:, normal_range].max()
+    assert (got.double().abs()[:, ~normal_range] <= 2.0 ** -119).all()
 
 
 def test_forward_gradients_are_refused(cuda_device):
