@@ -180,7 +180,8 @@ __device__ __forceinline__ float act_slope(float z, uint32_t act) {
     }
     case kActGeluTanh: {
       const float s = sigmoidf(gelu_tanh_arg(z));
-      return s + z * s * (1.f - s) * (2.f * kSqrt2OverPi) * (1.f + 3.f * kGeluCubic * z * z);
+      // z^2 stops where s (1 - s) has long been 0: infinity times that 0 would be NaN.
+      return s + z * s * (1.f - s) * (2.f * kSqrt2OverPi) * (1.f + 3.f * kGeluCubic * fminf(z * z, 1e8f));
     }
     case kActSilu: {
       const float s = sigmoidf(z);

@@ -44,6 +44,17 @@ def test_lower_tails_are_relatively_accurate(cuda_device, act):
     assert (got.double().abs()[:, ~normal_range] <= 2.0 ** -119).all()
 
 
+@pytest.mark.parametrize("act", [None, "relu", "gelu", "gelu_tanh", "silu"])
+def test_slopes_of_far_values(cuda_device, act):
+    """d act / dz of the largest finite values is 0 or 1, not NaN."""
+    b = torch.tensor([3e38, 1e30, 1e20, 1e19, 1e6, -1e6, -1e19, -1e20, -1e30, -3e38]).to(torch.bfloat16).cuda()
+    x = torch.zeros(1, 8, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(10, 8, dtype=torch.bfloat16, device="cuda")
+    lb = b.clone().requires_grad_()
+    (db,) = torch.autograd.grad(arc.linear(x, w, lb, activation=act), [lb], torch.ones_like(b)[None])
+    assert torch.equal(db.double(), (b > 0).double() if act else torch.ones(10, dtype=torch.float64, device="cuda"))
+
+
 def test_forward_gradients_are_refused(cuda_device):
     """A forward-mode derivative is not offered; it must not be dropped unnoticed."""
     g = torch.Generator().manual_seed(0)
