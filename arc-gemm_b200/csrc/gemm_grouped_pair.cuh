@@ -425,7 +425,8 @@ __global__ void __launch_bounds__(threads<W4>(), 1) gemm_grouped_pair_kernel(con
           const float sa = c0 + lane < w.rows ? __ldg(p.sa + row + lane) : 0.f;
 #pragma unroll
           for (uint32_t j = 0; j < 32; ++j) {
-            r[j] = __float_as_uint(__uint_as_float(r[j]) * (__shfl_sync(0xffffffffu, sa, j) * unscale));
+            // In this order: the two scales' product may leave fp32 where the result does not.
+            r[j] = __float_as_uint(__uint_as_float(r[j]) * unscale * __shfl_sync(0xffffffffu, sa, j));
           }
         }
         float v[32];

@@ -6,13 +6,40 @@ import torch
 import torch.autograd.forward_ad as forward_ad
 
 import arc
-from linear_bounds import H, normal
+from linear_bounds import H, SUM, assert_within, normal
 
 pytestmark = pytest.mark.gpu
 
 
 def _offsets(*values):
     return torch.tensor(values, dtype=torch.int32, device="cuda")
+
+
+@pytest.mark.parametrize("kernel", ["narrow", "wide"])
+@pytest.mark.parametrize("token,weight", [(-100, 100), (100, -100), (-30, -90), (-25, -108), (-20, -118)])
+def test_a8w4_scales_far_apart(cuda_device, monkeypatch, kernel, token, weight):
+    """Token scales of 2^token and weight scales of 2^weight: each alone fits fp32, and so does the result.
+
+    Scaling by powers of two is exact, so the bounds are those of scales around one: an fp32 sum over K
+    (k + 8 roundings of at most 2^-23 of the terms) and the rounding to bf16, whose last step is 2^-133;
+    the sum before the token's scale is a normal number in every case.
+    """
+    monkeypatch.setenv("ARC_A8W4_GROUPED", kernel)
+    g = torch.Generator().manual_seed(1)
+    t, e, n, k = 40, 2, 24, 256
+    x = torch.randint(-127, 128, (t, k), generator=g).to(torch.int8).cuda()
+    wp = torch.randint(0, 256, (e, n, k // 2), generator=g).to(torch.uint8).cuda()
+    sa = ((torch.rand(t, generator=g) + 0.5).double() * 2.0 ** token).float().cuda()
+    sb = ((torch.rand(e, n, k // 128, generator=g) + 0.5).double() * 2.0 ** weight).to(torch.bfloat16).cuda()
+    got = arc.a8w4_grouped_matmul((x, sa), (wp, sb), _offsets(0, 25, 40))
+    codes = torch.stack((wp & 15, wp >> 4), -1).flatten(-2).to(torch.int16)
+    w = torch.where(codes >= 8, codes - 16, codes).double() * sb.double().repeat_interleave(128, 2)
+    xe = x.double() * sa.double()[:, None]
+    want = torch.cat((xe[:25] @ w[0].T, xe[25:] @ w[1].T))
+    mag = torch.cat((xe[:25].abs() @ w[0].abs().T, xe[25:].abs() @ w[1].abs().T))
+    err = (k + 8) * SUM * mag
+    assert_within(got, want, err + H * (want.abs() + err) + 2.0 ** -133, f"{kernel} {token} {weight}")
+    assert arc.device_status(0) == 0
 
 
 def test_forward_gradients_are_refused(cuda_device):
