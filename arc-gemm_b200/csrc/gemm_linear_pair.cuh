@@ -408,6 +408,11 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       }
       __syncwarp();
     }
+  } else if (warp == 2) {
+    if (ALONG_K && p.groups.offsets != nullptr && blockIdx.x == 0) {
+      for (uint32_t e = lane; e < p.groups.num; e += 32u) lin::group_check(p.groups, e);
+    }
+    __syncwarp();
   } else if (warp == 3) {
     // ------------------------------------------------------------ a group's tail
     if (ALONG_K) {

@@ -34,9 +34,14 @@ __device__ __forceinline__ uint32_t group_count(const Groups& g, uint32_t e) {
   return b > a ? b - a : 0u;
 }
 
+// Offsets that decrease or leave [0, rows] set the status bit that arc_device_status reports.
+__device__ __forceinline__ void group_check(const Groups& g, uint32_t e) {
+  const int32_t a = __ldg(g.offsets + e), b = __ldg(g.offsets + e + 1u);
+  if (a < 0 || b < a || static_cast<uint32_t>(b) > g.rows) atomicOr(&g_arc_status, kStatusBadOffsets);
+}
+
 // One warp: prefix[e] = tiles of the groups before e (each group has ceil(count / tile)
-// row tiles), prefix[num] = all of them. Offsets that decrease or leave [0, rows] set the
-// status bit that arc_device_status reports.
+// row tiles), prefix[num] = all of them. Checks the offsets.
 __device__ __forceinline__ void group_tiles_prefix(const Groups& g, uint32_t tile, uint32_t* prefix) {
   const uint32_t lane = threadIdx.x & 31u;
   uint32_t base = 0;
@@ -44,10 +49,7 @@ __device__ __forceinline__ void group_tiles_prefix(const Groups& g, uint32_t til
     const uint32_t e = e0 + lane;
     uint32_t c = 0;
     if (e < g.num) {
-      if (g.offsets != nullptr) {
-        const int32_t a = __ldg(g.offsets + e), b = __ldg(g.offsets + e + 1u);
-        if (a < 0 || b < a || static_cast<uint32_t>(b) > g.rows) atomicOr(&g_arc_status, kStatusBadOffsets);
-      }
+      if (g.offsets != nullptr) group_check(g, e);
       c = (group_count(g, e) + tile - 1u) / tile;
     }
     uint32_t incl = c;

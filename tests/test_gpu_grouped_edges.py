@@ -1,11 +1,14 @@
 """Edges of the grouped products on the B200: extreme scales, offsets that are not offsets."""
 from __future__ import annotations
 
+import ctypes
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
 import arc
+from arc._lib import STATUS_BAD_OFFSETS
 from linear_bounds import H, SUM, assert_within, normal
 
 pytestmark = pytest.mark.gpu
@@ -40,6 +43,23 @@ def test_a8w4_scales_far_apart(cuda_device, monkeypatch, kernel, token, weight):
     err = (k + 8) * SUM * mag
     assert_within(got, want, err + H * (want.abs() + err) + 2.0 ** -133, f"{kernel} {token} {weight}")
     assert arc.device_status(0) == 0
+
+
+def test_bad_offsets_of_a_weight_gradient_are_reported(cuda_device):
+    """The C entry point for dw alone reads the offsets too, and says when they are none."""
+    from arc._lib import lib
+
+    g = torch.Generator().manual_seed(0)
+    t, e, n, k = 40, 3, 24, 16
+    dy, x = normal(g, t, n), normal(g, t, k)
+    dw = torch.empty(e, n, k, dtype=torch.bfloat16, device="cuda")
+    for bad in ((0, 30, 10, 40), (-5, 10, 20, 40), (0, 10, 20, 4000), (0, 10, 20, 40)):
+        off = _offsets(*bad)
+        stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+        status = lib().arc_grouped_matmul_dw(dy.data_ptr(), x.data_ptr(), off.data_ptr(), dw.data_ptr(), t, e, n, k,
+                                             n, k, k, n * k, stream)
+        assert status == 0
+        assert arc.device_status(0) == (STATUS_BAD_OFFSETS if bad != (0, 10, 20, 40) else 0)
 
 
 def test_forward_gradients_are_refused(cuda_device):
