@@ -66,6 +66,23 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// Whether the calling thread has a context.
+bool has_context() {
+  using Fn = CUresult (*)(CUcontext*);
+  static Fn fn = nullptr;
+  static std::once_flag once;
+  std::call_once(once, [] {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuCtxGetCurrent", &p, cudaEnableDefault, &q) == cudaSuccess &&
+        q == cudaDriverEntryPointSuccess) {
+      fn = reinterpret_cast<Fn>(p);
+    }
+  });
+  CUcontext ctx = nullptr;
+  return fn != nullptr && fn(&ctx) == CUDA_SUCCESS && ctx != nullptr;
+}
+
 // 2-D row-major matrix [rows][cols] with `ld` elements between rows.
 int encode_2d(CUtensorMap* map, CUtensorMapDataType dtype, uint32_t elem_bytes, const void* ptr,
               uint64_t cols, uint64_t rows, uint64_t ld, uint32_t box_cols, uint32_t box_rows,
@@ -369,12 +386,11 @@ int current_device(int* dev) {
   if (e != cudaSuccess) return cuda_fail(e, "cudaGetDevice");
   if (*dev < 0 || *dev >= kMaxDevices) return fail(ARC_ERR_NO_DEVICE, "device %d out of range", *dev);
   // A thread that has not launched anything yet (an autograd thread, say) has no context
-  // bound, and encoding a tensor map, a driver call, needs one.
-  thread_local int bound = -1;
-  if (bound != *dev) {
+  // bound, and encoding a tensor map, a driver call, needs one. A context that the caller has
+  // made current stays, the device's primary one or not.
+  if (!has_context()) {
     const cudaError_t s = cudaSetDevice(*dev);
     if (s != cudaSuccess) return cuda_fail(s, "cudaSetDevice");
-    bound = *dev;
   }
   return init_device(*dev);
 }
