@@ -163,6 +163,9 @@ struct DeviceState {
   int max_fp8fp4_pairs = 0;  // co-resident CTA pairs of the FP8 x FP4 pair kernel
   int max_linear_pairs = 0;  // co-resident CTA pairs of the linear pair kernel
   int max_linear_quads = 0;  // co-resident clusters of two pairs (contraction in two parts)
+  // The linear layer's and the grouped operators' kernels: what fails there leaves the rest alone.
+  int linear_status = ARC_OK;
+  int grouped_status = ARC_OK;
 };
 DeviceState g_dev[kMaxDevices];
 
@@ -208,9 +211,9 @@ bool decode_stream(int G, int S, int num_items, int grid) {
   X(64, 1, 4)                \
   X(128, 2, 3)
 
-cudaError_t linear_init(DeviceState& st);          // api_linear.cuh
+int linear_init(DeviceState& st);  // api_linear.cuh
 int linear_kernel_name(int dev, uint32_t M, uint32_t N, uint32_t K, char* name, int len);
-cudaError_t grouped_init(DeviceState& st, bool* regs_ok);  // api_grouped.cuh
+int grouped_init();  // api_grouped.cuh
 
 int init_device(int dev) {
   DeviceState& st = g_dev[dev];
@@ -303,13 +306,6 @@ int init_device(int dev) {
         return;
       }
     }
-    if (e == cudaSuccess) e = linear_init(st);
-    if (e == cudaSuccess) e = grouped_init(st, &regs_ok);
-    if (e == cudaSuccess && !regs_ok) {
-      st.status = fail(ARC_ERR_UNSUPPORTED,
-                       "gemm_a8w4_grouped_kernel was compiled with an unexpected register count");
-      return;
-    }
     if (e != cudaSuccess) {
       st.status = cuda_fail(e, "cudaFuncSetAttribute");
       return;
@@ -373,6 +369,8 @@ int init_device(int dev) {
       }
       st.max_fp8fp4_pairs = n;
     }
+    st.linear_status = linear_init(st);
+    st.grouped_status = grouped_init();
   });
   if (st.status != ARC_OK) {
     // Re-state the stored failure for this thread.
@@ -393,6 +391,15 @@ int current_device(int* dev) {
     if (s != cudaSuccess) return cuda_fail(s, "cudaSetDevice");
   }
   return init_device(*dev);
+}
+
+// The same for the linear layer's and the grouped operators' kernels (`status` of the two).
+int current_device(int* dev, int DeviceState::*status) {
+  if (int st = current_device(dev)) return st;
+  if (int st = g_dev[*dev].*status) {
+    return fail(st, "device %d failed to initialise these kernels (first error reported earlier)", *dev);
+  }
+  return ARC_OK;
 }
 
 bool aligned16(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }

@@ -33,18 +33,25 @@ cudaError_t a8w4_grouped_attr(bool* regs_ok) {
   return e;
 }
 
-cudaError_t grouped_init(DeviceState&, bool* regs_ok) {
-  cudaError_t e = cudaSuccess;
-  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped16>(regs_ok);
-  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped32>(regs_ok);
-  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped64>(regs_ok);
-  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped128>(regs_ok);
+int grouped_init() {
+  bool regs_ok = true;
+  cudaError_t e = a8w4_grouped_attr<A8w4Grouped16>(&regs_ok);
+  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped32>(&regs_ok);
+  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped64>(&regs_ok);
+  if (e == cudaSuccess) e = a8w4_grouped_attr<A8w4Grouped128>(&regs_ok);
   const int most = static_cast<int>(GR::smem_bytes(GR::kMaxBuckets - 1));
   for (const void* k : {reinterpret_cast<const void*>(GR::place_rows_kernel<int32_t>),
                         reinterpret_cast<const void*>(GR::place_rows_kernel<int64_t>)}) {
     if (e == cudaSuccess) e = cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, most);
   }
-  return e;
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // clear
+    return cuda_fail(e, "cudaFuncSetAttribute (grouped A8W4 and row grouping kernels)");
+  }
+  if (!regs_ok) {
+    return fail(ARC_ERR_UNSUPPORTED, "gemm_a8w4_grouped_kernel was compiled with an unexpected register count");
+  }
+  return ARC_OK;
 }
 
 // Int4 codes [groups][rows][bytes].
@@ -131,13 +138,14 @@ int arc_a8w4_grouped_gemm(const int8_t* A, const float* sa, const uint8_t* Wp, c
   }
   if (int64_t(E) * N > 0x7FFFFFFF) return fail(ARC_ERR_UNSUPPORTED, "%s: E * N must be below 2^31", what);
   int dev = 0;
-  if (int st = current_device(&dev)) return st;
+  if (int st = current_device(&dev, &DeviceState::grouped_status)) return st;
   const uint32_t live = E < T ? E : T;  // groups that can have rows
   const uint32_t avg = ceil_div(T, live);
   const uint32_t BT = avg <= 16 ? 16u : avg <= 32 ? 32u : avg <= 64 ? 64u : 128u;
   const arcb::lin::Groups groups = {offsets, static_cast<uint32_t>(E), static_cast<uint32_t>(T)};
   const bool zero_others = (flags & ARC_GROUPED_ZERO_OTHERS) != 0;
   if (a8w4_grouped_wide(T, E)) {
+    if (int st = current_device(&dev, &DeviceState::linear_status)) return st;
     if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < size_t(T) * K * 2) {
       return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what,
                   size_t(T) * K * 2);
@@ -243,7 +251,7 @@ int arc_group_rows(const void* ids, int id_bytes, int32_t* offsets, int32_t* row
     return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
   }
   int dev = 0;
-  if (int st = current_device(&dev)) return st;
+  if (int st = current_device(&dev, &DeviceState::grouped_status)) return st;
   GR::Params p = {};
   p.ids = ids;
   p.offsets = offsets;

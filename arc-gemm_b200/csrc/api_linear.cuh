@@ -171,6 +171,7 @@ int linear_plan(int dev, uint32_t rows, uint32_t groups, uint32_t cols, uint32_t
 
 // The kernel of arc_linear_bf16 as ncu lists it (16-byte aligned output rows assumed).
 int linear_kernel_name(int dev, uint32_t M, uint32_t N, uint32_t K, char* name, int len) {
+  if (int st = current_device(&dev, &DeviceState::linear_status)) return st;
   LinearPlan plan;
   if (int st = linear_plan(dev, M, 1, N, ceil_div(K, arcb::lin::BK), true, &plan)) return st;
   if (plan.pair) {
@@ -212,7 +213,29 @@ cudaError_t launch_stream_bn(const LS::Params& p, uint32_t bn, uint32_t grid, cu
 #define ARC_LINEAR_STREAM_VARIANTS(X) X(16, false) X(32, false) X(64, false) X(128, false) \
   X(16, true) X(32, true) X(64, true) X(128, true)
 
-cudaError_t linear_init(DeviceState& st) {
+// How many clusters of `size` CTAs of a kernel fit at once (0 where the query fails: no plan uses them).
+template <typename Kern>
+int clusters_at_once(Kern kernel, const DeviceState& st, uint32_t size, uint32_t threads, size_t smem) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3(size * (st.sms / size), 1, 1);
+  cfg.blockDim = dim3(threads, 1, 1);
+  cfg.dynamicSmemBytes = smem;
+  cudaLaunchAttribute attr[1];
+  attr[0].id = cudaLaunchAttributeClusterDimension;
+  attr[0].val.clusterDim.x = size;
+  attr[0].val.clusterDim.y = 1;
+  attr[0].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = 1;
+  int n = 0;
+  if (cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+    cudaGetLastError();  // clear
+    n = 0;
+  }
+  return n;
+}
+
+int linear_init(DeviceState& st) {
   cudaError_t e = cudaSuccess;
 #define ARC_SET_ATTR(BN, MN) \
   if (e == cudaSuccess) e = allow_smem(LS::gemm_linear_stream_kernel<BN, MN>, LS::smem_bytes<BN>());
@@ -230,31 +253,16 @@ cudaError_t linear_init(DeviceState& st) {
   if (e == cudaSuccess) e = allow_smem(GP::gemm_grouped_pair_kernel<false, false>, GP::smem_bytes<false>());
   if (e == cudaSuccess) e = allow_smem(GP::gemm_grouped_pair_kernel<true, false>, GP::smem_bytes<false>());
   if (e == cudaSuccess) e = allow_smem(GP::gemm_grouped_pair_kernel<false, true>, GP::smem_bytes<true>());
-  if (e != cudaSuccess) return e;
-  // How many pairs of the largest of these kernels fit at once.
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3(st.sms, 1, 1);
-  cfg.blockDim = dim3(GP::threads<true>(), 1, 1);
-  cfg.dynamicSmemBytes = GP::smem_bytes<true>();
-  cudaLaunchAttribute attr[1];
-  attr[0].id = cudaLaunchAttributeClusterDimension;
-  attr[0].val.clusterDim.x = 2;
-  attr[0].val.clusterDim.y = 1;
-  attr[0].val.clusterDim.z = 1;
-  cfg.attrs = attr;
-  cfg.numAttrs = 1;
-  int n = 0;
-  e = cudaOccupancyMaxActiveClusters(&n, GP::gemm_grouped_pair_kernel<false, true>, &cfg);
-  st.max_linear_pairs = e == cudaSuccess ? n : 0;
-  if (e != cudaSuccess) return e;
-  // And how many clusters of two pairs of the linear one.
-  cfg.blockDim = dim3(LP::kThreads, 1, 1);
-  cfg.dynamicSmemBytes = LP::kSmemBytes<256>;
-  cfg.gridDim = dim3(4 * (st.sms / 4), 1, 1);
-  attr[0].val.clusterDim.x = 4;
-  e = cudaOccupancyMaxActiveClusters(&n, LP::gemm_linear_pair_kernel<false, false, false, true, 256>, &cfg);
-  st.max_linear_quads = e == cudaSuccess ? n : 0;
-  return e;
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // clear
+    return cuda_fail(e, "cudaFuncSetAttribute (linear and grouped kernels)");
+  }
+  // Pairs of the largest of these kernels, and clusters of two pairs of the linear one.
+  st.max_linear_pairs =
+      clusters_at_once(GP::gemm_grouped_pair_kernel<false, true>, st, 2, GP::threads<true>(), GP::smem_bytes<true>());
+  st.max_linear_quads = clusters_at_once(LP::gemm_linear_pair_kernel<false, false, false, true, 256>, st, 4, LP::kThreads,
+                                         LP::kSmemBytes<256>);
+  return ARC_OK;
 }
 
 // The walk's fields and the launch of the grouped pair kernel (its maps are set by the caller).
@@ -281,7 +289,7 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
                 uint32_t inner, uint64_t lda, uint64_t ldw, uint64_t w_stride, uint64_t ldo,
                 const arcb::lin::Epilogue& epi, bool grad, bool zero_others, cudaStream_t stream) {
   int dev = 0;
-  if (int st = current_device(&dev)) return st;
+  if (int st = current_device(&dev, &DeviceState::linear_status)) return st;
   const uint32_t num_kb = ceil_div(inner, arcb::lin::BK);
   LinearPlan plan;
   if (int st = linear_plan(dev, groups.rows, groups.num, cols, num_kb, rows_aligned16(out, ldo), &plan)) return st;
@@ -374,7 +382,7 @@ int linear_dw(const char* what, const uint16_t* dy, const uint16_t* x, const arc
               uint32_t N, uint32_t K, uint64_t lddy, uint64_t ldx, uint64_t lddw, uint64_t dw_stride,
               cudaStream_t stream) {
   int dev = 0;
-  if (int st = current_device(&dev)) return st;
+  if (int st = current_device(&dev, &DeviceState::linear_status)) return st;
   const uint32_t max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
   if (max_pairs == 0) return fail(ARC_ERR_UNSUPPORTED, "%s: no CTA pair fits on this device", what);
   LP::Params p = {};
@@ -541,7 +549,7 @@ int arc_linear_backward(const uint16_t* dy, const uint16_t* x, const uint16_t* w
     return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
   }
   int dev = 0;
-  if (int st = current_device(&dev)) return st;
+  if (int st = current_device(&dev, &DeviceState::linear_status)) return st;
   if (need_dz || dbias != nullptr) {
     LB::Params p = {};
     p.dy = dy;
