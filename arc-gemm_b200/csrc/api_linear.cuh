@@ -185,11 +185,10 @@ int linear_kernel_name(int dev, uint32_t M, uint32_t N, uint32_t K, char* name, 
 
 // The pair kernel, one cluster of two pairs per tile if the contraction is split.
 template <bool A_MN, bool B_MN, bool ALONG_K, uint32_t TN>
-cudaError_t launch_linear_pair(LP::Params& p, uint64_t tiles, uint32_t splits, uint32_t max_pairs, cudaStream_t stream) {
-  p.splits = splits;
+cudaError_t launch_linear_pair(const LP::Params& p, uint64_t tiles, uint32_t splits, uint32_t max_pairs, cudaStream_t stream) {
   if (splits > 1) {
-    return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, true, TN>, p, static_cast<uint32_t>(tiles) * 2 * splits,
-                     LP::kThreads, LP::kSmemBytes<TN>, 2 * splits, stream);
+    return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, true, TN>, p, static_cast<uint32_t>(tiles) * 4,
+                     LP::kThreads, LP::kSmemBytes<TN>, 4, stream);
   }
   const uint32_t grid = 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
   return launch_ex(LP::gemm_linear_pair_kernel<A_MN, B_MN, ALONG_K, false, TN>, p, grid, LP::kThreads, LP::kSmemBytes<TN>, 2,

@@ -118,7 +118,7 @@ struct Cfg {
   static_assert(EWG == 1 || EWG == 2, "epilogue warpgroups");
   static_assert(LS >= 2 && LS <= kDoneRing && UNP <= kDoneRing && kAccPairs < kDoneRing,
                 "each waiter must stay within one phase of its completion barrier");
-  static_assert(UWG == 1 || (UWG + EWG <= 4 && UNP >= UWG), "unpack warpgroups");
+  static_assert(UWG == 1 || (UWG == 2 && UNP >= UWG), "unpack warpgroups");
   // A parity wait tells a barrier's phase only from the one before, so whoever takes every n-th
   // step must meet the same ring slots each time round (the unpacked ring, which may be odd, is
   // waited for through the completions of the steps: see the issuer).
@@ -147,8 +147,8 @@ struct Cfg {
   // launch (the most 1 CTA/SM allows; the host checks the compiled count).
   static constexpr uint32_t kLaunchRegs = EWG + UWG == 4 ? 96 : EWG + UWG == 3 ? 128 : 168;
   static constexpr bool kSplitRegs = true;
-  static constexpr uint32_t kRegsLow = EWG == 2 || UWG == 3 ? 80 : UWG == 2 ? 96 : 112;
-  static constexpr uint32_t kRegsHigh = UWG == 3 ? 160 : EWG == 2 ? (UWG == 2 ? 120 : 176) : UWG == 2 ? 224 : 232;
+  static constexpr uint32_t kRegsLow = EWG == 2 ? 80 : UWG == 2 ? 96 : 112;
+  static constexpr uint32_t kRegsHigh = EWG == 2 ? (UWG == 2 ? 120 : 176) : UWG == 2 ? 224 : 232;
   static_assert((128 + 128 * UWG) * kRegsLow + 128 * EWG * kRegsHigh <= kThreads * kLaunchRegs,
                 "register shares exceed the launch budget");
   static_assert(kCols % kChunk == 0, "epilogue column split");

@@ -23,8 +23,8 @@
 // of each CTA between the load's arrival and the product.
 //
 // SPLIT: problems with fewer tiles than pairs. A cluster of two pairs takes one tile, its pairs
-// the contraction in equal parts; each CTA then leaves its sums in its ring's shared memory, and
-// pair i finishes the i-th part of the columns, adding the parts in order through distributed
+// half of the contraction each; each CTA then leaves its sums in its ring's shared memory, and
+// pair i finishes the i-th half of the columns, adding the halves in order through distributed
 // shared memory (the result does not depend on timing).
 //
 // TN: columns of a tile. 128 where tiles of 256 leave pairs without work or a last round mostly
@@ -97,7 +97,6 @@ struct Params {
   lin::Epilogue epi;
   uint32_t M, N;       // output rows (of a group) and columns
   uint32_t tiles_m, tiles_n, num_kb;
-  uint32_t splits;     // SPLIT: pairs per cluster
 };
 
 // One tile of the walk.
@@ -111,7 +110,7 @@ struct Tile {
   uint32_t tail_rows;   // valid rows of the last block if it needs zeroing, else 0
 };
 
-// `part`: this pair's part of the contraction (SPLIT).
+// `part`: this pair's half of the contraction (SPLIT).
 template <bool ALONG_K, bool SPLIT, uint32_t TN>
 __device__ __forceinline__ bool tile_at(const Params& p, uint32_t t, uint32_t part, Tile& w) {
   const uint32_t per = p.tiles_m * p.tiles_n;
@@ -140,8 +139,8 @@ __device__ __forceinline__ bool tile_at(const Params& p, uint32_t t, uint32_t pa
   const uint32_t m_cnt = min(kBandM, p.tiles_m - m_first);
   w.m0 = (m_first + rem % m_cnt) * kTile;
   w.n0 = rem / m_cnt * TN;
-  w.kb0 = SPLIT ? w.num_kb * part / p.splits : 0u;
-  w.kb1 = SPLIT ? w.num_kb * (part + 1u) / p.splits : w.num_kb;
+  w.kb0 = SPLIT && part == 1u ? w.num_kb / 2u : 0u;
+  w.kb1 = SPLIT && part == 0u ? w.num_kb / 2u : w.num_kb;
   return true;
 }
 
@@ -258,7 +257,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
   // that walks over tiles, with it a cluster takes one tile.
   const uint32_t rank = cluster_ctarank() & 1u;
   const uint32_t lead = SPLIT ? cluster_ctarank() - rank : 0u, part = lead >> 1;
-  const uint32_t per_cluster = SPLIT ? 2u * p.splits : 2u;
+  constexpr uint32_t per_cluster = SPLIT ? 4u : 2u;
   const uint32_t pair = blockIdx.x / per_cluster, num_pairs = gridDim.x / per_cluster;
   const uint16_t both = static_cast<uint16_t>(0x3u << lead);
   volatile uint32_t* abort = &s.abort;
@@ -532,7 +531,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     if (warp >= 4 && (tile_at<ALONG_K, SPLIT, TN>(p, pair, part, w)) && *abort == 0u) {
       const uint32_t row = (warp & 3u) * 32u + lane;
       const uint32_t m = w.m0 + rank * kRowsPerCta + (warp & 3u) * 32u;  // the warp's first row
-      const uint32_t first = TN / p.splits * part, last = first + TN / p.splits;
+      const uint32_t first = TN / 2u * part, last = first + TN / 2u;
       bool ok = m < p.M;
 #pragma unroll 1
       for (uint32_t c = first + ((warp - 4u) >> 2) * 32u; c < last && w.n0 + c < p.N && ok; c += 64u) {
@@ -540,7 +539,8 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
 #pragma unroll
         for (uint32_t i = 0; i < 32; ++i) v[i] = 0.f;
         const float* sums = reinterpret_cast<const float*>(s.a[0]) + c * kRowsPerCta + row;
-        for (uint32_t j = 0; j < p.splits; ++j) {
+#pragma unroll 1
+        for (uint32_t j = 0; j < 2u; ++j) {
           const uint32_t from = map_to_rank(sums, 2u * j + rank);
 #pragma unroll
           for (uint32_t i = 0; i < 32; ++i) v[i] += ld_dsmem_f32(from + i * (kRowsPerCta * 4u));
