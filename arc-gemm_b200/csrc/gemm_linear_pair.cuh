@@ -144,6 +144,12 @@ __device__ __forceinline__ bool tile_at(const Params& p, uint32_t t, uint32_t pa
   return true;
 }
 
+// The limit of a wait for a tile's whole contraction, which the rows of a weight gradient can make
+// long: 2^23 blocks of 64 rows take 2.2 s. A block takes 0.27 us; 2 are allowed.
+__device__ __forceinline__ uint64_t products_limit(const Tile& w) {
+  return kWaitTimeoutNs + uint64_t(w.kb1 - w.kb0) * 2000u;
+}
+
 // One warp's way to memory: its two pieces in turn.
 struct Pieces {
   uint8_t (*buf)[lin::kWarpTileBytes];
@@ -424,7 +430,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
         stage = (stage + w.kb1 - w.kb0) % kStages;
         if (w.tail_rows == 0u || w.kb1 != w.num_kb) continue;
         const uint32_t par = (parity >> st) & 1u;
-        ok = __all_sync(0xffffffffu, mbar_wait(&s.tail_full[st], par, abort, kStatusTimeoutScales));
+        ok = __all_sync(0xffffffffu, mbar_wait(&s.tail_full[st], par, abort, kStatusTimeoutScales, products_limit(w)));
         if (!ok) break;
         // Rows tail_rows .. end of their step, both chunks of both operands; a row of a chunk
         // is one 128-byte line whatever the swizzle does inside it.
@@ -466,7 +472,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       if constexpr (SPLIT) {
         // This CTA's sums, column by column, into its ring: every load and product has ended.
         if (any) {
-          ok = __all_sync(0xffffffffu, mbar_wait(&s.tmem_full[acc], acc_phase, abort, kStatusTimeoutEpilogue));
+          ok = __all_sync(0xffffffffu, mbar_wait(&s.tmem_full[acc], acc_phase, abort, kStatusTimeoutEpilogue, products_limit(w)));
           if (!ok) break;
           tc_fence_after_sync();
         }
@@ -498,7 +504,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
       // the same pieces, which leaves none to ask ahead for).
       const bool ahead = !ALONG_K && p.epi.residual != nullptr && p.tma_res && p.epi.z == nullptr && m < p.M;
       if (ahead && w.n0 + wg * 32u < p.N) piece_ask(p, pieces, w.n0 + wg * 32u, m, lane);
-      ok = __all_sync(0xffffffffu, mbar_wait(&s.tmem_full[acc], acc_phase, abort, kStatusTimeoutEpilogue));
+      ok = __all_sync(0xffffffffu, mbar_wait(&s.tmem_full[acc], acc_phase, abort, kStatusTimeoutEpilogue, products_limit(w)));
       if (!ok) break;
       tc_fence_after_sync();
 #pragma unroll 1

@@ -155,7 +155,8 @@ __device__ __forceinline__ bool mbar_try_wait_sleep(uint32_t bar, uint32_t parit
 // raises *abort and ORs `err_bit` into the device status word) or another role of
 // the CTA already raised *abort.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
-                                          volatile uint32_t* abort, uint32_t err_bit) {
+                                          volatile uint32_t* abort, uint32_t err_bit,
+                                          uint64_t limit_ns = kWaitTimeoutNs) {
   const uint32_t addr = smem_u32(bar);
   if (mbar_try_wait(addr, parity)) return true;
   const uint64_t start = globaltimer_ns();
@@ -164,7 +165,7 @@ __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity,
     if (mbar_try_wait_sleep(addr, parity, 20000u)) return true;
     if ((it & 15u) == 0u) {
       if (*abort) return false;
-      if (globaltimer_ns() - start > kWaitTimeoutNs) {
+      if (globaltimer_ns() - start > limit_ns) {
         *abort = 1u;
         atomicOr(&g_arc_status, err_bit);
         return false;

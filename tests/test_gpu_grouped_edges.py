@@ -135,3 +135,24 @@ def test_out_that_overlaps_is_refused(cuda_device):
     sb = torch.ones(2, 32, 1, dtype=torch.bfloat16, device="cuda")
     with pytest.raises(ValueError, match="overlap"):
         arc.a8w4_grouped_matmul((q, sa), (wp, sb), inside, out=words)
+
+
+def test_weight_gradient_of_very_many_rows(cuda_device):
+    """A contraction of 2^29 rows takes longer than the limit of an ordinary wait (2 s) and is no fault."""
+    from arc._lib import lib
+
+    t, n, k = 2 ** 29 + 37, 8, 8
+    dy, x = (torch.zeros(t, c, dtype=torch.bfloat16, device="cuda") for c in (n, k))
+    rows = torch.tensor([0, 1, 2 ** 28 + 3, t - 7, t - 6], device="cuda")
+    g = torch.Generator().manual_seed(0)
+    dy[rows], x[rows] = normal(g, 5, n), normal(g, 5, k)
+    dy[t - 5:], x[t - 5:] = float("nan"), float("inf")  # behind the group
+    dw = torch.empty(1, n, k, dtype=torch.bfloat16, device="cuda")
+    stream = ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
+    off = _offsets(0, t - 5)
+    assert lib().arc_grouped_matmul_dw(dy.data_ptr(), x.data_ptr(), off.data_ptr(), dw.data_ptr(), t, 1, n, k,
+                                       n, k, k, n * k, stream) == 0
+    assert arc.device_status(0) == 0
+    want = dy[rows].double().T @ x[rows].double()
+    err = 5 * SUM * (dy[rows].double().abs().T @ x[rows].double().abs())  # all other terms are zero
+    assert_within(dw[0], want, err + H * (want.abs() + err), "dw")
