@@ -207,6 +207,9 @@ template <bool ALONG_K>
 __device__ __forceinline__ bool finish_piece(const Params& p, Pieces& b, float (&v)[32], uint32_t m, uint32_t n,
                                              uint32_t e, volatile uint32_t* abort, uint32_t lane) {
   const uint32_t rows = min(32u, p.M - m), cols = min(32u, p.N - n);
+  // A TMA store writes whole 16-byte pieces, zeros behind a matrix's last column: where that column
+  // ends inside one, the piece goes out element by element and what lies beside the matrix stays.
+  const uint32_t whole = cols % 8u == 0u ? 1u : 0u;
   if (!ALONG_K) {
     if (p.epi.bias != nullptr) {
       uint32_t c[16];
@@ -219,7 +222,7 @@ __device__ __forceinline__ bool finish_piece(const Params& p, Pieces& b, float (
     }
     if (p.epi.z != nullptr) {
       piece_claim(lane);
-      piece_store(b, v, &p.tm_z, p.tma_z, p.epi.z + size_t(m) * p.epi.ldz + n, p.epi.ldz, rows, cols, n, m, 0, lane);
+      piece_store(b, v, &p.tm_z, p.tma_z & whole, p.epi.z + size_t(m) * p.epi.ldz + n, p.epi.ldz, rows, cols, n, m, 0, lane);
     }
     lin::activate(v, p.epi.act);
   }
@@ -246,7 +249,7 @@ __device__ __forceinline__ bool finish_piece(const Params& p, Pieces& b, float (
   } else {
     piece_claim(lane);
   }
-  piece_store(b, v, &p.tm_out, p.tma_out, p.out + (ALONG_K ? size_t(e) * p.out_group : 0u) + size_t(m) * p.ldo + n,
+  piece_store(b, v, &p.tm_out, p.tma_out & whole, p.out + (ALONG_K ? size_t(e) * p.out_group : 0u) + size_t(m) * p.ldo + n,
               p.ldo, rows, cols, n, m, e, lane);
   return true;
 }

@@ -178,3 +178,40 @@ def test_out_that_overlaps_inside_wider_rows_is_refused(cuda_device):
     res, = _views(buf, (s(0, 32), s(5, 37)))
     want = arc.linear(r, w, b, res.clone())
     assert torch.equal(arc.linear(r, w, b, buf[0:32, 5:37], out=res), want)  # two views of the same slice: in place
+
+
+@pytest.mark.parametrize("plan", ["pair:1", "pair:2", "pair128:1", "pair128:2", "16:1", "32:4"])
+def test_nothing_beside_out_is_written(cuda_device, monkeypatch, plan):
+    """Columns beside a slice of a wider buffer keep what they hold, whatever the slice's width."""
+    monkeypatch.setenv("ARC_LINEAR_PLAN", plan)
+    g = torch.Generator().manual_seed(0)
+    for n in (*range(1, 42), 255, 257, 513):
+        x, w, r = normal(g, 37, 72), normal(g, n, 72), normal(g, 37, n)
+        for lead in (0, 8, 3):
+            buf = torch.full((40, (n + lead + 15) // 8 * 8), 7.0, dtype=torch.bfloat16, device="cuda")
+            out = buf[1:38, lead:lead + n]
+            arc.linear(x, w, None, r, out=out)
+            assert torch.equal(out, arc.linear(x, w, None, r)), (n, lead)
+            out.fill_(7.0)
+            assert (buf == 7).all(), (n, lead)
+
+
+@pytest.mark.parametrize("n,k", [(33, 40), (24, 37), (129, 261)])
+def test_nothing_beside_z_and_dw_is_written(cuda_device, monkeypatch, n, k):
+    """The same for the pre-activation and the weight gradient of the C entry points."""
+    from arc._lib import lib
+
+    monkeypatch.setenv("ARC_LINEAR_PLAN", "pair:1")
+    g = torch.Generator().manual_seed(0)
+    m, wide = 50, 272
+    x, w, dy = normal(g, m, wide)[:, :k], normal(g, n, wide)[:, :k], normal(g, m, wide)[:, :n]
+    stream = torch.cuda.current_stream().cuda_stream
+    z, dw = (torch.full((rows, wide), 7.0, dtype=torch.bfloat16, device="cuda") for rows in (m, n))
+    out = torch.empty(m, wide, dtype=torch.bfloat16, device="cuda")
+    assert lib().arc_linear_bf16(x.data_ptr(), w.data_ptr(), None, None, out.data_ptr(), z.data_ptr(), m, n, k,
+                                 wide, wide, 0, wide, wide, 4, stream) == 0
+    assert (z[:, n:] == 7).all() and (z[:, :n] != 7).any(1).all()
+    assert lib().arc_linear_backward(dy.data_ptr(), x.data_ptr(), None, None, None, dw.data_ptr(), None, None, 0, m, n, k,
+                                     wide, wide, 0, 0, 0, wide, 0, stream) == 0
+    assert (dw[:, k:] == 7).all() and (dw[:, :k] != 7).any(1).all()
+    assert arc.device_status(0) == 0
