@@ -784,6 +784,8 @@ int arc_matmul_bf16(const void* A, const void* B, void* C, int M, int N, int K, 
                            P2::kEpiCols, P2::kRowsPerCta, CU_TENSOR_MAP_SWIZZLE_64B, "C")) {
       return st;
     }
+    p.c = static_cast<uint16_t*>(C);
+    p.ldc = ldc;
     p.M = M;
     p.N = N;
     p.K = K;
@@ -812,6 +814,8 @@ int arc_matmul_bf16(const void* A, const void* B, void* C, int M, int N, int K, 
                          B16::kEpiCols, B16::BM, CU_TENSOR_MAP_SWIZZLE_64B, "C")) {
     return st;
   }
+  p.c = static_cast<uint16_t*>(C);
+  p.ldc = ldc;
   p.M = M;
   p.N = N;
   p.K = K;

@@ -61,6 +61,8 @@ struct Params {
   CUtensorMap tm_a;  // [M][K] bf16, box {64, 128}, SW128
   CUtensorMap tm_b;  // [N][K] bf16, box {64, 128}, SW128
   CUtensorMap tm_c;  // [M][N] bf16, box {32, 128}, SW64
+  uint16_t* c;       // the same, for a chunk that ends inside 16 bytes
+  uint32_t ldc;
   uint32_t M, N, K;
   uint32_t tiles_m, tiles_n, num_tiles, num_kb;  // pair tiles of 256 x 256
 };
@@ -221,6 +223,21 @@ __global__ void __launch_bounds__(kNumThreads, 1) gemm_bf16_pair_kernel(const __
         for (uint32_t i = 0; i < 16; ++i) {
           packed[i] = pack_bf16x2(__uint_as_float(r[2 * i]), __uint_as_float(r[2 * i + 1]));
         }
+        const uint32_t n0 = nb * kTileN + c * kEpiCols;
+        const uint32_t cols = n0 < p.N ? min(kEpiCols, p.N - n0) : 0u;
+        if (cols % 8u != 0u) {
+          // A TMA store writes whole 16-byte pieces, zeros behind C's last column: where that column
+          // ends inside one, element by element, so that what lies beside C stays.
+          if (m0 + row < p.M) {
+            uint16_t* at = p.c + size_t(m0 + row) * p.ldc + n0;
+#pragma unroll
+            for (uint32_t i = 0; i < kEpiCols; ++i) {
+              if (i < cols) at[i] = static_cast<uint16_t>(packed[i / 2u] >> (i % 2u * 16u));
+            }
+          }
+          if (et == 0) tma_store_commit();  // an empty group: every chunk counts as one
+          continue;
+        }
         const uint32_t buf = chunk_ctr & 1u;
         if (et == 0) tma_store_wait_read<1>();
         named_barrier_sync(1, 128);
@@ -233,7 +250,6 @@ __global__ void __launch_bounds__(kNumThreads, 1) gemm_bf16_pair_kernel(const __
         }
         fence_proxy_async_smem();
         named_barrier_sync(1, 128);
-        const uint32_t n0 = nb * kTileN + c * kEpiCols;
         // Boxes wholly past M or N (a pair tile's second half at the edge) are skipped.
         if (et == 0 && m0 < p.M && n0 < p.N) {
           tma_store_2d(&p.tm_c, s.cd[buf], int32_t(n0), int32_t(m0));
