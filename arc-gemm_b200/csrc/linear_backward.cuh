@@ -27,15 +27,22 @@ struct Params {
   uint32_t M, N, act, rows_per_block;
 };
 
-// v *= act'(z), one branch for eight values.
-__device__ __forceinline__ void times_slope8(float (&v)[8], const float (&z)[8], uint32_t act) {
+// v *= act'(z), one branch for eight values (z is used up).
+__device__ __forceinline__ void times_slope8(float (&v)[8], float (&z)[8], uint32_t act) {
   switch (act) {
 #define ARC_SLOPE_CASE(A)                                                              \
   case A:                                                                              \
     _Pragma("unroll") for (uint32_t j = 0; j < 8; ++j) v[j] *= lin::act_slope(z[j], A); \
     break;
+    case lin::kActGelu:
+#pragma unroll
+      for (uint32_t j = 0; j < 8; j += 2) {
+        lin::gelu_slope_pair(z[j], z[j + 1]);
+        v[j] *= z[j];
+        v[j + 1] *= z[j + 1];
+      }
+      break;
     ARC_SLOPE_CASE(lin::kActRelu)
-    ARC_SLOPE_CASE(lin::kActGelu)
     ARC_SLOPE_CASE(lin::kActGeluTanh)
     ARC_SLOPE_CASE(lin::kActSilu)
 #undef ARC_SLOPE_CASE

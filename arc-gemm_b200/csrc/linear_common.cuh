@@ -129,34 +129,53 @@ __device__ __forceinline__ constexpr float tail_term(int i) {
   return c[i];
 }
 
-// The erf form, two values at once: z Phi(z) = max(z, 0) - |z| q(|z|) / 2, where nothing cancels. The
-// pair shares one reciprocal; the rest are packed products and an exponential each. |z| stops at 16,
-// where q is 0 in fp32.
-__device__ __forceinline__ void gelu_pair(float& z0, float& z1) {
-  const float y0 = fminf(fabsf(z0), 16.f), y1 = fminf(fabsf(z1), 16.f);
-  const uint64_t y = f32x2_pack(y0, y1);
+// t R(t) of two values, with one reciprocal for both and packed products.
+__device__ __forceinline__ uint64_t gelu_tail_pair(uint64_t y) {
   const auto both = [](float c) { return f32x2_pack(c, c); };
-  float d0, d1, e0, e1;
+  float d0, d1;
   f32x2_unpack(f32x2_fma(y, both(kTailP), both(1.f)), d0, d1);
-  f32x2_unpack(f32x2_mul(f32x2_mul(y, both(-0.5f * kLog2E)), y), e0, e1);
   const float r = rcp_ftz(d0 * d1);
   const uint64_t t = f32x2_pack(r * d1, r * d0);
   uint64_t q = f32x2_fma(t, both(tail_term(6)), both(tail_term(5)));
 #pragma unroll
   for (int i = 4; i >= 0; --i) q = f32x2_fma(t, q, both(tail_term(i)));
-  const uint64_t h = f32x2_mul(f32x2_mul(f32x2_mul(t, q), y), f32x2_pack(ex2_ftz(e0), ex2_ftz(e1)));
-  f32x2_unpack(f32x2_fma(h, both(-0.5f), f32x2_pack(relu_nan(z0), relu_nan(z1))), z0, z1);
+  return f32x2_mul(t, q);
 }
 
+// exp(-y^2 / 2) of two values.
+__device__ __forceinline__ uint64_t gauss_pair(uint64_t y) {
+  float e0, e1;
+  f32x2_unpack(f32x2_mul(f32x2_mul(y, f32x2_pack(-0.5f * kLog2E, -0.5f * kLog2E)), y), e0, e1);
+  return f32x2_pack(ex2_ftz(e0), ex2_ftz(e1));
+}
+
+// The erf form, two values at once: z Phi(z) = max(z, 0) - |z| q(|z|) / 2, where nothing cancels.
+// |z| stops at 16, where q is 0 in fp32.
+__device__ __forceinline__ void gelu_pair(float& z0, float& z1) {
+  const uint64_t y = f32x2_pack(fminf(fabsf(z0), 16.f), fminf(fabsf(z1), 16.f));
+  const uint64_t h = f32x2_mul(f32x2_mul(gelu_tail_pair(y), y), gauss_pair(y));
+  f32x2_unpack(f32x2_fma(h, f32x2_pack(-0.5f, -0.5f), f32x2_pack(relu_nan(z0), relu_nan(z1))), z0, z1);
+}
+
+// Its slope Phi(z) + z phi(z), two values at once (in their place): with e = exp(-z^2 / 2) and
+// h = t R(t) / 2 it is e (h + z / sqrt(2 pi)) below zero and 1 - e (h - z / sqrt(2 pi)) above.
+__device__ __forceinline__ void gelu_slope_pair(float& z0, float& z1) {
+  const uint64_t y = f32x2_pack(fminf(fabsf(z0), 16.f), fminf(fabsf(z1), 16.f));
+  const uint64_t e = gauss_pair(f32x2_pack(z0, z1));  // not y: a NaN stays one
+  // |slope - (z > 0)| = e (h - |z| / sqrt(2 pi))
+  const uint64_t d = f32x2_mul(e, f32x2_fma(gelu_tail_pair(y), f32x2_pack(0.5f, 0.5f),
+                                            f32x2_mul(y, f32x2_pack(-kInvSqrt2Pi, -kInvSqrt2Pi))));
+  float d0, d1;
+  f32x2_unpack(d, d0, d1);
+  z0 = z0 < 0.f ? d0 : 1.f - d0;
+  z1 = z1 < 0.f ? d1 : 1.f - d1;
+}
+
+// The others, one value.
 __device__ __forceinline__ float act_value(float z, uint32_t act) {
   switch (act) {
     case kActRelu:
       return relu_nan(z);
-    case kActGelu: {
-      float other = 0.f;
-      gelu_pair(z, other);
-      return z;
-    }
     case kActGeluTanh:
       return z * sigmoidf(gelu_tanh_arg(z));
     case kActSilu:
@@ -166,20 +185,11 @@ __device__ __forceinline__ float act_value(float z, uint32_t act) {
   }
 }
 
-// d act / d z. The erf form: Phi(z) + z phi(z), with q as above.
+// d act / d z.
 __device__ __forceinline__ float act_slope(float z, uint32_t act) {
   switch (act) {
     case kActRelu:
       return z > 0.f ? 1.f : 0.f;
-    case kActGelu: {
-      const float t = rcp_ftz(fmaf(kTailP, fminf(fabsf(z), 16.f), 1.f));
-      const float e = ex2_ftz(-0.5f * kLog2E * z * z);
-      float q = tail_term(6);
-#pragma unroll
-      for (int i = 5; i >= 0; --i) q = fmaf(t, q, tail_term(i));
-      q *= t * e;
-      return (z < 0.f ? 0.5f * q : fmaf(-0.5f, q, 1.f)) + z * kInvSqrt2Pi * e;
-    }
     case kActGeluTanh: {
       const float s = sigmoidf(gelu_tanh_arg(z));
       // z^2 stops where s (1 - s) has long been 0: infinity times that 0 would be NaN.

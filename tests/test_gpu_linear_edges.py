@@ -215,3 +215,17 @@ def test_nothing_beside_z_and_dw_is_written(cuda_device, monkeypatch, n, k):
                                      wide, wide, 0, 0, 0, wide, 0, stream) == 0
     assert (dw[:, k:] == 7).all() and (dw[:, :k] != 7).any(1).all()
     assert arc.device_status(0) == 0
+
+
+def test_slope_of_gelu_on_a_grid(cuda_device):
+    """The slope over the whole range, relative to itself in the tail too (bounds as for the tail above;
+    2^-20 beside the slope's zero at -0.75, where its two terms of 0.3 cancel)."""
+    b = torch.linspace(-13, 13, 1700, dtype=torch.float64).to(torch.bfloat16).cuda()
+    x = torch.zeros(1, 8, dtype=torch.bfloat16, device="cuda")
+    w = torch.zeros(b.numel(), 8, dtype=torch.bfloat16, device="cuda")
+    lb = b.clone().requires_grad_()
+    (db,) = torch.autograd.grad(arc.linear(x, w, lb, activation="gelu"), [lb], torch.ones_like(b)[None])
+    z = b.double()
+    want = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5) + z * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
+    near = torch.where((z + 0.75).abs() < 1, 2.0 ** -20, 2.0 ** -120)
+    assert ((db.double() - want).abs() <= (H + 2.0 ** -14) * want.abs() + near).all()
