@@ -8,7 +8,9 @@
 Group e owns the rows [offsets[e], offsets[e+1]); offsets is int32 [E+1] on the GPU and is read
 there, so no call waits for the host. Rows of no group (behind the last one, where `group_rows`
 places the choices of ids outside [0, E)) never reach a result, whatever they hold; their
-output rows are left as they are when `out` is given and are zero otherwise.
+output rows are left as they are when `out` is given and are zero otherwise. The kernel and its row
+tile are chosen by the rows per group on average, since the sizes are on the GPU: a batch of which
+one expert has most rows is as right, but slower than an even one.
 
 `grouped_matmul` is differentiable in x and w (once, in reverse mode; a second derivative or a
 forward-mode tangent is refused); `a8w4_grouped_matmul` is the serving form on
@@ -39,12 +41,13 @@ def a8w4_grouped_matmul(a: TensorPair, b: TensorPair, offsets: torch.Tensor, out
     """A8W4 GEMM of each row group with its own weights. See the module docstring.
 
     a = (x int8 [T, K], sa float32 [T]); b = (wp uint8 [E, N, K/2], sb bfloat16 [E, N, K/128]),
-    the operands of `arc.a8w4_matmul` with a leading group dimension. `prepacked=True` says that
+    the operands of `arc.a8w4_matmul` with a leading group dimension, contiguous and 16-byte aligned. `prepacked=True` says that
     wp is in the layout of `arc.prepack_weights` (of wp viewed as [E*N, K/2]).
 
     Up to 128 rows per group on average the int32 group partials are exact, as in
     `arc.a8w4_matmul`; above, code times scale is an exact fp16 operand and the sum over K runs
-    in fp32 (scales below 2^-24 of their weight row's largest may round).
+    in fp32 (scales below 2^-24 of their weight row's largest may round). So the last bits of a
+    token's result depend on how many rows and groups share the call.
     """
     x, sa = a
     wp, sb = b

@@ -54,9 +54,8 @@ uint32_t column_pairs(const void* p, uint64_t ld, uint32_t cols) {
 }
 
 // The pair kernel's parts of the contraction: two where the clusters of all tiles run at once, which
-// are fewer than half the pairs (32 tiles: 512 x 4096 x 4096 29 us whole, 21 in two parts; 36 tiles:
-// 512 x 4608 x 4096 29 and 39). Of the clusters of eight CTAs that four parts would take, 15 fit: 256
-// x 3840 x 4096 20 us in two parts, 18.6 in four, but 256 x 4096 x 4096 20 and 33.
+// are fewer than half the pairs (32 tiles: 512 x 4096 x 4096 30 us whole, 22 in two parts; 36 tiles:
+// 512 x 4608 x 4096 30 and 41).
 uint32_t pair_splits(uint64_t tiles, uint32_t num_kb, int dev) {
   return tiles <= static_cast<uint64_t>(g_dev[dev].max_linear_quads) && num_kb >= 8 ? 2 : 1;
 }
@@ -75,7 +74,10 @@ struct LinearPlan {
 // contractions of 64 to 6400). The plan it picks is 1.2 % behind the best one, geometric mean over
 // those, and 1.4 % over 200 others; fixed thresholds on rows and tiles were 14 %.
 double stream_cost(uint32_t rows, uint32_t cols, uint32_t num_kb, uint32_t bn, uint32_t splits, uint32_t sms) {
-  // Two blocks fit on an SM; clusters of four and eight leave some slots empty.
+  // Two blocks fit on an SM; clusters of four and eight leave some slots empty. Counted on one B200,
+  // by the blocks of a long launch that began before any ended: 296, 296, 284 and 264 blocks in
+  // clusters of 1, 2, 4 and 8; a little less is assumed, since it depends on which SMs a part has.
+  // (The driver's own count says one block per SM for any kernel that takes TMEM.)
   const double slots = 2.0 * sms * (splits == 8 ? 256.0 / 296 : splits == 4 ? 280.0 / 296 : 1.0);
   const double cluster = splits > 1 ? 1.36 : 0.0;
   const double blocks = static_cast<double>(ceil_div(rows, bn)) * ceil_div(cols, LS::kRows) * splits;

@@ -8,9 +8,10 @@
 // would cost a full 256 (at 512 rows per group a quarter of all work). Bound by the tensor pipe.
 // The accumulator is double buffered in TMEM (2 x 256 columns), the epilogue of a tile runs
 // under the next tile's products. Measured: 8190 rows in 16 groups of 113 to 1101, 4096 x 4096,
-// 233 us (1180 TFLOP/s), 275 under the power cap; 16 groups of 512 take 202. Row tiles of equal
+// 233 us in a short run (1180 TFLOP/s), 274 to 281 under the power cap; 16 groups of 512 take 203. Row tiles of equal
 // size within a group (200 + 200 for 256 + 144) measured the same there, 1 to 2 % slower with W_MN.
-// W4: 4093 rows in 8 groups of 106 to 1255, 14336 x 4096, 398 us (1208 TFLOP/s), 468 under the cap.
+// W4: 4093 rows in 8 groups of 106 to 1255, 14336 x 4096, 400 to 410 us (1190 TFLOP/s), 455 to 485 under
+// the cap.
 //
 // W_MN: w is read MN-major ([E][contraction][features]): the gradient of the rows.
 //

@@ -8,9 +8,10 @@
 // written and read 32 KB each for 128 x 256 x 64 MACs (a single CTA with the same tile would
 // move half as much again and stop near 70 % of the tensor peak). The accumulator is double
 // buffered in TMEM; a tile's epilogue runs under the next tile's products. Measured: 4096 x 14336
-// x 4096 with bias, GELU and residual 335 us (1436 TFLOP/s), 380 under the power cap; the gradient
-// of 4096 x 8192 x 4096: rows 185, weights 195 us (both operands MN-major: each 64-row piece of
-// them is two boxes, and the tensor pipe is busy 78 % against 91 % of the forward product's time).
+// x 4096 with bias, GELU and residual 332 us in a short run (1450 TFLOP/s), 382 to 391 under the power
+// cap; the gradient of 4096 x 8192 x 4096, from cold: rows 187, weights 195 us (both operands MN-major:
+// each 64-row piece of them is two boxes, and the tensor pipe is busy 78 % against 90 % of the forward
+// product's time).
 //
 // Operands are read as they lie in memory. A K-major operand has the contraction contiguous
 // (the forward product); an MN-major one has the output index contiguous: w in the gradient
@@ -28,8 +29,9 @@
 // shared memory (the result does not depend on timing).
 //
 // TN: columns of a tile. 128 where tiles of 256 leave pairs without work or a last round mostly
-// empty (256 x 4096 x 4096: 20.1 us with 256, 15.9 with 128; 512 x 4608 x 4096 29 and 22; but 1024 x
-// 4096 x 4096 30 and 37, since a stage's products then hardly cover its hand-offs).
+// empty (with bias and GELU 256 x 4096 x 4096: 21.3 us with 256, 16.8 with 128; 512 x 4608 x 4096 30
+// and 23; but 1024 x 4096 x 4096 31 to 35 and 43, since a stage's products then hardly cover its
+// hand-offs).
 //
 // Roles (384 threads per CTA): warp 0 TMA producer, warp 1 UMMA issuer (rank 0), warp 2 TMEM
 // owner, warp 3 zeroes a group's tail, warps 4-11 epilogue: two warpgroups take 32 columns in

@@ -9,9 +9,10 @@
 //
 // Bound by: HBM (weights, 2 bytes each, read once). Two blocks fit on an SM (about 110 KB of
 // shared memory each), so one block's prologue and epilogue run under the other's stream and
-// about 200 KB of loads are in flight per SM. Measured: 16 rows, 14336 x 4096 with bias, GELU and
-// residual 24.9 us, 4.7 TB/s of weights (one wave of blocks: some 7 us are the first bytes' way,
-// the reduction and the epilogue); one row, 4096 x 4096 9.3 us.
+// about 200 KB of loads are in flight per SM. Measured, one call after another on several sets of
+// inputs: 16 rows, 14336 x 4096 with bias, GELU and residual 25.3 us, 4.6 TB/s of weights (one wave
+// of blocks: some 7 us are the first bytes' way, the reduction and the epilogue); one row, 4096 x
+// 4096 8.5 us.
 //
 // W_MN = false: w is [E][N][K], K contiguous: the forward product.
 // W_MN = true:  the roles of N and K are exchanged: out[t, f] = sum_n dy[t, n] w[e, n, f], the
@@ -86,8 +87,8 @@ struct Params {
 
 // The rows rank, rank + S, ... of one output column: the cluster's partial sums in rank order, then
 // the epilogue. 16 sums are on their way at once: row by row, each row waits for a round trip
-// through the cluster (128 x 4096 x 4096 19.3 us against 14.8; 333 x 1003 x 2056 13.9 against
-// 11.8); with 32 they come in no faster (64 x 4096 x 4096 11.9 and 12.2).
+// through the cluster (128 x 4096 x 4096 19.3 us against 14.8 without an epilogue); with 32 they
+// come in no faster (64 x 4096 x 4096 11.9 and 12.2).
 template <uint32_t BN, uint32_t S>
 __device__ __forceinline__ void finish_rows(const Params& p, const float* part, uint32_t rank, uint32_t row0,
                                             uint32_t rows, uint32_t f, float bias) {

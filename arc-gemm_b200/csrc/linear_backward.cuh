@@ -5,7 +5,7 @@
 // One pass over dy and z writes dz (bf16: it is the next two products' tensor-core operand)
 // and sums the unrounded dz by column in fp32, each block its own rows; a second, small kernel
 // adds the blocks' sums in order, so the result does not depend on timing. HBM-bound: 6 bytes
-// per element with an activation. Measured: 4096 x 8192 42 us from cold, 4.8 TB/s.
+// per element with an activation. Measured: 4096 x 8192 with GELU 39 us from cold, 5.2 TB/s.
 #pragma once
 
 #include "linear_common.cuh"

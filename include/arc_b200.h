@@ -298,7 +298,9 @@ int arc_quantize_int8(const void *x, int8_t *q, float *sa, int M, int K, int ldx
  *   z [M][ldz] or NULL: receives x w^T + bias in bf16, what arc_linear_backward needs later
  * Requirements: M, N, K >= 1 (any sizes); x and w 16-byte aligned with leading dimensions
  * that are multiples of 8; the others need 2-byte alignment only (aligned rows are
- * faster). residual may be out itself.
+ * faster). residual may be out itself; otherwise out and z overlap no operand. Only the N columns of
+ * out and z are written, whatever their leading dimension. The activations are off by less than
+ * 2^-14 of themselves before the rounding, in their lower tails too (down to 2^-118).
  */
 #define ARC_ACT_NONE 0
 #define ARC_ACT_RELU 1
@@ -358,7 +360,8 @@ int arc_grouped_matmul_dw(const uint16_t *dy, const uint16_t *x, const int32_t *
  * K % 128 == 0, N % 8 == 0, E <= 1024, E * N < 2^31; A, Wp and C 16-byte aligned.
  * Few rows per group: the int32 partials are exact and the scales multiply them in fp32. Many
  * (more than 128 on average): code times scale is the tensor cores' fp16 operand, exactly, and
- * the sum over K runs in fp32; scales below 2^-24 of their weight row's largest may round.
+ * the sum over K runs in fp32; scales below 2^-24 of their weight row's largest may round. A
+ * token's last bits therefore depend on how many rows and groups share the call.
  * workspace: 16-byte aligned, arc_a8w4_grouped_workspace_bytes (0 for few rows per group), no
  * initialisation needed.
  */
