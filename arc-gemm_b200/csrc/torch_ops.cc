@@ -291,7 +291,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &z = saved[2];
+    Tensor x = saved[0], w = saved[1], z = saved[2];
     const Tensor& dy_in = grads[0];
     const bool need_x = ctx->saved_data["x"].toBool(), need_w = ctx->saved_data["w"].toBool(),
                need_bias = ctx->saved_data["bias"].toBool(), need_residual = ctx->saved_data["residual"].toBool();
@@ -303,6 +303,10 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
       return out;
     }
     const c10::cuda::CUDAGuard guard(dy_in.device());
+    // Hooks on saved tensors may bring them back in a layout of their own.
+    if (need_w) x = product_rows(x);
+    if (need_x) w = product_rows(w);
+    if (z.defined()) z = unit_rows(z);
     const Tensor dy = unit_rows(dy_in.detach());
     const auto options = dy.options();
     if (need_x) out[0] = at::empty({m, k}, options);
@@ -319,7 +323,7 @@ struct LinearFunction : torch::autograd::Function<LinearFunction> {
                                   need_x ? u16_mut(out[0]) : nullptr, need_w ? u16_mut(out[1]) : nullptr,
                                   need_bias ? u16_mut(out[2]) : nullptr, bytes > 0 ? workspace.data_ptr() : nullptr,
                                   bytes, m, n, k, row_ld(dy), need_w ? x.stride(0) : 0, need_x ? w.stride(0) : 0,
-                                  z.defined() ? z.stride(0) : 0, k, k,
+                                  z.defined() ? row_ld(z) : 0, k, k,
                                   static_cast<int>(ctx->saved_data["act"].toInt()), stream_of(dy)),
             "arc.linear backward");
     }
@@ -409,7 +413,8 @@ struct GroupedFunction : torch::autograd::Function<GroupedFunction> {
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
     const auto saved = ctx->get_saved_variables();
-    const Tensor &x = saved[0], &w = saved[1], &offsets = saved[2];
+    Tensor x = saved[0], w = saved[1];
+    const Tensor offsets = saved[2].contiguous();
     const Tensor& dy_in = grads[0];
     const int64_t t = ctx->saved_data["t"].toInt(), e = ctx->saved_data["e"].toInt(), n = ctx->saved_data["n"].toInt(),
                   k = ctx->saved_data["k"].toInt();
@@ -423,6 +428,9 @@ struct GroupedFunction : torch::autograd::Function<GroupedFunction> {
       if (ctx->saved_data["w"].toBool()) out[1] = at::zeros({e, n, k}, options);
       return out;
     }
+    // Hooks on saved tensors may bring them back in a layout of their own.
+    if (ctx->saved_data["w"].toBool()) x = product_rows(x);
+    if (ctx->saved_data["x"].toBool()) w = product_rows(w);
     const Tensor dy = product_rows(dy_in.detach());
     if (ctx->saved_data["x"].toBool()) {
       out[0] = at::empty({t, k}, options);

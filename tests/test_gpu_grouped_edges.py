@@ -156,3 +156,16 @@ def test_weight_gradient_of_very_many_rows(cuda_device):
     want = dy[rows].double().T @ x[rows].double()
     err = 5 * SUM * (dy[rows].double().abs().T @ x[rows].double().abs())  # all other terms are zero
     assert_within(dw[0], want, err + H * (want.abs() + err), "dw")
+
+
+@pytest.mark.parametrize("n,k", [(33, 131), (24, 64)])
+def test_saved_tensors_may_move(cuda_device, n, k):
+    """torch.autograd.graph.save_on_cpu brings the saved tensors back in a layout of its own."""
+    g = torch.Generator().manual_seed(0)
+    x, w, dy, offsets = normal(g, 40, k), normal(g, 2, n, k, scale=k ** -0.5), normal(g, 40, n), _offsets(0, 25, 40)
+    leaves = [t.requires_grad_() for t in (x, w)]
+    want = torch.autograd.grad(arc.grouped_matmul(*leaves, offsets), leaves, dy)
+    with torch.autograd.graph.save_on_cpu():
+        y = arc.grouped_matmul(*leaves, offsets)
+    for got, ref in zip(torch.autograd.grad(y, leaves, dy), want):
+        assert torch.equal(got, ref)

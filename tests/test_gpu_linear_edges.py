@@ -229,3 +229,18 @@ def test_slope_of_gelu_on_a_grid(cuda_device):
     want = 0.5 * torch.special.erfc(-z * 0.5 ** 0.5) + z * torch.exp(-z * z / 2) / (2 * torch.pi) ** 0.5
     near = torch.where((z + 0.75).abs() < 1, 2.0 ** -20, 2.0 ** -120)
     assert ((db.double() - want).abs() <= (H + 2.0 ** -14) * want.abs() + near).all()
+
+
+@pytest.mark.parametrize("m,n,k", [(9, 33, 131), (300, 77, 44), (40, 24, 64)])
+def test_saved_tensors_may_move(cuda_device, m, n, k):
+    """torch.autograd.graph.save_on_cpu brings the saved tensors back in a layout of its own."""
+    g = torch.Generator().manual_seed(0)
+    x, w, b, dy = normal(g, m, k), normal(g, n, k, scale=k ** -0.5), normal(g, n), normal(g, m, n)
+    for wide in (False, True):  # rows that are 16-byte aligned only as the slice they are
+        x = torch.nn.functional.pad(x, (0, 16 - k % 8))[:, :k] if wide else x
+        leaves = [t.detach().requires_grad_() for t in (x, w, b)]
+        want = torch.autograd.grad(arc.linear(*leaves, activation="silu"), leaves, dy)
+        with torch.autograd.graph.save_on_cpu():
+            y = arc.linear(*leaves, activation="silu")
+        for got, ref in zip(torch.autograd.grad(y, leaves, dy), want):
+            assert torch.equal(got, ref)
