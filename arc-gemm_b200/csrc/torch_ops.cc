@@ -149,8 +149,15 @@ void expect_out(const Tensor& out, int64_t rows, int64_t cols, const at::Device&
 // `step` apart (at most three dimensions, none of negative stride).
 struct Runs {
   int64_t at = 0, width = 0, rows = 1, pitch = 0, blocks = 1, step = 0;
-  int64_t end() const { return at + width + (rows - 1) * pitch + (blocks - 1) * step; }
 };
+
+// The bytes from a tensor's first to behind its last one.
+std::pair<int64_t, int64_t> span_of(const Tensor& t) {
+  int64_t last = 0;
+  for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+  const int64_t at = reinterpret_cast<intptr_t>(t.const_data_ptr());
+  return {at, at + (last + 1) * static_cast<int64_t>(t.element_size())};
+}
 
 Runs runs_of(const Tensor& t) {
   const int64_t item = t.element_size();
@@ -188,8 +195,9 @@ bool meets(int64_t at, int64_t width, int64_t also, int64_t own, int64_t rows, i
 // lie side by side share none. One look for tensors of one pitch, else one per row of `b`.
 bool share_bytes(const Tensor& ta, const Tensor& tb) {
   if (ta.numel() == 0 || tb.numel() == 0) return false;
+  const auto sa = span_of(ta), sb = span_of(tb);
+  if (sa.second <= sb.first || sb.second <= sa.first) return false;
   const Runs a = runs_of(ta), b = runs_of(tb);
-  if (a.end() <= b.at || b.end() <= a.at) return false;
   const bool together = a.rows == 1 || b.rows == 1 || a.pitch == b.pitch;
   const int64_t pitch = a.rows > 1 ? a.pitch : b.pitch;
   for (int64_t k = 0; k < b.blocks; ++k) {
