@@ -299,7 +299,10 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
   }
   // Grouped: TMEM is taken only after the preceding grid has ended, and the next grid is let in only
   // after it is taken (see gemm_linear_stream.cuh).
-  if constexpr (kGrouped) pdl_wait();
+  if constexpr (kGrouped) {
+    pdl_wait();
+    if (warp == 3) lin::group_tiles_prefix(p.groups, BT, s.prefix);
+  }
   if (warp == 2) {
     tmem_alloc(&s.tmem_base, C::kTmemCols);
     tmem_relinquish();
@@ -307,10 +310,7 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
   tc_fence_before_sync();
   __syncthreads();
   tc_fence_after_sync();
-  if constexpr (kGrouped) {
-    pdl_launch_dependents();
-    if (warp == 2) lin::group_tiles_prefix(p.groups, BT, s.prefix);
-  }
+  if constexpr (kGrouped) pdl_launch_dependents();
   const uint32_t tmem_base = s.tmem_base;
   if (warp >= C::kEpiWarp) {
     // Arm every accumulator with the bias before the first UMMA may touch it.
@@ -324,7 +324,14 @@ __device__ __forceinline__ void gemm_a8w4_body(const P& p) {
     tmem_st_wait();
   }
   tc_fence_before_sync();
-  __syncthreads();
+  if constexpr (kGrouped) {
+    // Loads and unpacking need not wait for the accumulators: only issuers and epilogue meet here.
+    if (warp >= C::kEpiWarp || warp == 1 || (C::kIssuers == 2 && warp == 3)) {
+      named_barrier_sync(1, 128 * EWG + 32 * C::kIssuers);
+    }
+  } else {
+    __syncthreads();
+  }
   tc_fence_after_sync();
   // The prologue above may overlap the previous grid in the stream (programmatic
   // dependent launch); global memory is only touched after it has completed.
