@@ -1,0 +1,40 @@
+"""The expert layer of a few tokens: a decode batch through the experts it has chosen, in two launches.
+
+    h[t, j] = act(x[t] . g_e^T) * (x[t] . u_e^T)      e = ids[t, j]; w_in[e] holds g_e, then u_e
+    y[t]    = sum_j weights[t, j] (h[t, j] . w_out[e]^T)
+
+`moe` does what `group_rows`, two `grouped_matmul` and the steps between them do, for batches whose cost
+is reading the chosen experts' weights: nothing is sorted or gathered in memory, and the second
+product's weights are on their way before the first has ended. Above ARC_MOE_MAX_TOKENS tokens the products are
+worth `grouped_matmul`'s tensor-core tiles; `moe` refuses them.
+
+Sums are fp32; h is rounded to bf16 as operand of the second product, the result is rounded once. It is the serving
+form: there is no gradient, and inputs that require one are refused (outside torch.no_grad()).
+"""
+from __future__ import annotations
+
+import torch
+
+from ._lib import ACTIVATIONS, torch_ops
+from .quant import TensorPair
+
+
+def moe(x: torch.Tensor, w_in: torch.Tensor | TensorPair, w_out: torch.Tensor | TensorPair, ids: torch.Tensor,
+        weights: torch.Tensor, *, activation: str | None = "silu", out: torch.Tensor | None = None) -> torch.Tensor:
+    """y[t] = sum_j weights[t, j] expert_{ids[t, j]}(x[t]). See the module docstring.
+
+    x [T, K] bf16. w_in [E, 2I, K] bf16 with gate and up rows, or [E, I, K] for experts without a gate
+    (h = act(x . w_in^T)); w_out [E, N, I] bf16. Or both int4, as pairs (packed uint8 [E, rows, K/2], scales
+    bfloat16 [E, rows, K/128]) in the packing of `arc.a8w4_matmul` (not pre-packed), with K and I multiples
+    of 128; the activations stay bf16.
+    ids [T, top], int32 or int64, and weights [T, top], float32 or bfloat16: a router's choices. An id outside
+    [0, E) chooses nobody; an expert chosen twice counts with the sum of its weights. T <= 256, T * top <= 4096,
+    E <= 1024. activation: as for `arc.linear`. bf16 operands whose rows are not contiguous and
+    16-byte aligned are copied first, on every call. `out` [T, N] receives the result and must not overlap an operand.
+    """
+    code = ACTIVATIONS.get(activation)
+    if code is None:
+        raise ValueError(f"activation must be one of {list(ACTIVATIONS)}, got {activation!r}")
+    w_in, s_in = w_in if isinstance(w_in, (tuple, list)) else (w_in, None)
+    w_out, s_out = w_out if isinstance(w_out, (tuple, list)) else (w_out, None)
+    return torch_ops().moe(x, w_in, s_in, w_out, s_out, ids, weights, code, out)

@@ -45,6 +45,8 @@ struct Api {
   decltype(&arc_a8w4_grouped_gemm) a8w4_grouped = nullptr;
   decltype(&arc_group_rows_workspace_bytes) group_rows_ws = nullptr;
   decltype(&arc_group_rows) group_rows = nullptr;
+  decltype(&arc_moe_workspace_bytes) moe_ws = nullptr;
+  decltype(&arc_moe) moe = nullptr;
 };
 Api g_api;
 
@@ -550,6 +552,102 @@ std::tuple<Tensor, Tensor, Tensor> group_rows(const Tensor& ids_in, int64_t grou
 }
 
 // ---------------------------------------------------------------------------------
+// moe
+// ---------------------------------------------------------------------------------
+// Operators without a gradient refuse inputs that ask for one.
+template <typename... Ts>
+void refuse_gradients(const char* what, const Ts&... ts) {
+  if (at::GradMode::is_enabled() && (wants_grad(ts) || ...)) {
+    throw std::runtime_error(std::string(what) + " has no gradient, and an input requires one");
+  }
+}
+
+// Weights of experts: bf16 [E, rows, inner], or packed int4 [E, rows, inner/2] with scales [E, rows, inner/128].
+struct ExpertWeights {
+  const Tensor& data;
+  const OptTensor& scales;
+  const char* name;
+
+  int64_t inner() const { return scales ? 2 * data.size(2) : data.size(2); }
+  void check(const at::Device& dev) const {
+    expect_cuda(data, name);
+    expect_device(data, name, dev);
+    expect_dtype(data, name, scales ? at::kByte : at::kBFloat16);
+    if (data.size(1) == 0 || data.size(2) == 0) bad_value(name, " must not be empty, got shape ", shape_of(data));
+    if (!scales) return;
+    if (inner() % kScaleGroup != 0) {
+      bad_value(name, ": the contraction (", inner(), ") must be a multiple of ", kScaleGroup);
+    }
+    if (!data.is_contiguous()) bad_value(name, " must be contiguous");
+    if (!aligned16(data)) bad_value(name, " must be 16-byte aligned");
+    expect(*scales, name, at::kBFloat16, {data.size(0), data.size(1), inner() / kScaleGroup}, dev);
+  }
+};
+
+Tensor moe(const Tensor& x_in, const Tensor& w_in, const OptTensor& s_in, const Tensor& w_out, const OptTensor& s_out,
+           const Tensor& ids_in, const Tensor& weights_in, int64_t act, const OptTensor& out) {
+  expect_bf16(x_in, "x", 2);
+  expect_dims(w_in, "w_in", 3);
+  expect_dims(w_out, "w_out", 3);
+  const at::Device dev = x_in.device();
+  const ExpertWeights in{w_in, s_in, "w_in"}, last{w_out, s_out, "w_out"};
+  if (s_in.has_value() != s_out.has_value()) bad_value("w_in and w_out must both be bf16 or both be int4 with scales");
+  in.check(dev);
+  last.check(dev);
+  const int64_t t = x_in.size(0), k = x_in.size(1), e = w_in.size(0), i = last.inner(), n = w_out.size(1);
+  if (k != in.inner()) bad_value("Inner dimensions must match: ", k, " vs ", in.inner());
+  if (w_out.size(0) != e) bad_value("w_in and w_out must have as many experts: ", e, " vs ", w_out.size(0));
+  if (e < 1 || e > kMaxGroups) bad_value("between 1 and ", kMaxGroups, " experts are supported, got ", e);
+  const bool gated = w_in.size(1) == 2 * i;
+  if (!gated && w_in.size(1) != i) {
+    bad_value("w_in must have ", 2 * i, " rows (gate and up) or ", i, " per expert, got ", w_in.size(1));
+  }
+  as_int(n, "N"), as_int(k, "K"), as_int(2 * i, "I");
+  expect_cuda(ids_in, "ids");
+  expect_device(ids_in, "ids", dev);
+  if (ids_in.scalar_type() != at::kInt && ids_in.scalar_type() != at::kLong) {
+    bad_type("ids must be int32 or int64, got ", ids_in.scalar_type());
+  }
+  expect_dims(ids_in, "ids", 2);
+  const int64_t top = ids_in.size(1);
+  expect_shape(ids_in, "ids", {t, top});
+  expect_cuda(weights_in, "weights");
+  expect_device(weights_in, "weights", dev);
+  if (weights_in.scalar_type() != at::kFloat && weights_in.scalar_type() != at::kBFloat16) {
+    bad_type("weights must be float32 or bfloat16, got ", weights_in.scalar_type());
+  }
+  expect_shape(weights_in, "weights", {t, top});
+  if (t > ARC_MOE_MAX_TOKENS || t * top > ARC_MOE_MAX_CHOICES) {
+    bad_value("at most ", ARC_MOE_MAX_TOKENS, " tokens and ", ARC_MOE_MAX_CHOICES, " choices are supported, got ", t,
+              " x ", top, " (for more: group_rows and grouped_matmul)");
+  }
+  refuse_tangents(x_in, w_in, s_in, w_out, s_out, weights_in, out);
+  refuse_gradients("arc.moe", x_in, w_in, s_in, w_out, s_out, weights_in);
+  const c10::cuda::CUDAGuard guard(dev);
+  if (out) expect_out(*out, t, n, dev);
+  claim_out(out, {&x_in, &w_in, &w_out, &ids_in, &weights_in, s_in ? &*s_in : &x_in, s_out ? &*s_out : &x_in});
+  const Tensor y = out ? *out : at::empty({t, n}, x_in.options().requires_grad(false));
+  if (t == 0) return y;
+  if (top == 0) {
+    Tensor all = y;
+    all.zero_();
+    return y;
+  }
+  const Tensor x = product_rows(x_in), wi = s_in ? w_in : product_rows(w_in), wo = s_out ? w_out : product_rows(w_out);
+  const Tensor ids = ids_in.contiguous(), weights = weights_in.contiguous();
+  size_t bytes = 0;
+  check(g_api.moe_ws(t, top, i, &bytes), "arc.moe");
+  const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte).requires_grad(false));
+  check(g_api.moe(u16(x), wi.const_data_ptr(), s_in ? u16(*s_in) : nullptr, wo.const_data_ptr(),
+                  s_out ? u16(*s_out) : nullptr, ids.const_data_ptr(), static_cast<int>(ids.element_size()),
+                  weights.const_data_ptr(), static_cast<int>(weights.element_size()), u16_mut(y), workspace.data_ptr(),
+                  bytes, t, top, e, k, i, n, x.stride(0), wi.stride(1), wi.stride(0), wo.stride(1), wo.stride(0),
+                  row_ld(y), gated ? 1 : 0, static_cast<int>(act), stream_of(x)),
+        "arc.moe");
+  return y;
+}
+
+// ---------------------------------------------------------------------------------
 // Module
 // ---------------------------------------------------------------------------------
 PyObject* g_arc_error = nullptr;  // arc.ArcError, one reference for the life of the process
@@ -570,6 +668,8 @@ void bind(const std::unordered_map<std::string, uintptr_t>& addresses, py::objec
   set(g_api.a8w4_grouped, "arc_a8w4_grouped_gemm");
   set(g_api.group_rows_ws, "arc_group_rows_workspace_bytes");
   set(g_api.group_rows, "arc_group_rows");
+  set(g_api.moe_ws, "arc_moe_workspace_bytes");
+  set(g_api.moe, "arc_moe");
   g_arc_error = arc_error.release().ptr();
 }
 
@@ -589,4 +689,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("grouped_matmul", &grouped_matmul);
   m.def("a8w4_grouped_matmul", &a8w4_grouped_matmul);
   m.def("group_rows", &group_rows);
+  m.def("moe", &moe);
 }

@@ -384,6 +384,33 @@ int arc_group_rows(const void *ids, int id_bytes, int32_t *offsets, int32_t *row
                    size_t workspace_bytes, int slots, int top, int E, cudaStream_t stream);
 
 /*
+ * Expert layer of a few tokens (a decode batch), in two launches:
+ *   h[t,j] = act(x[t] g_e^T) * (x[t] u_e^T)   gated: w_in [E][2I][K] holds g (rows 0 .. I-1), then u
+ *   h[t,j] = act(x[t] w_in[e]^T)              not gated: w_in [E][I][K]
+ *   out[t] = sum_j weights[t,j] h[t,j] w_out[e]^T,   e = ids[t,j], w_out [E][N][I]
+ * bf16 with fp32 sums; h is rounded to bf16. An id outside [0, E) chooses nobody (a token without choices
+ * gets zeros); an expert chosen twice by a token counts with the sum of its weights. Only the
+ * weights of chosen experts are read.
+ *   s_in, s_out   NULL: bf16 weights with leading dimensions ld_* and strides stride_* between experts
+ *                 (elements). Else scales [E][rows][K/128] and [E][N][I/128], bf16: the weights are packed int4
+ *                 as in arc_a8w4_gemm, contiguous (ld_* and stride_* are not used), K and I multiples of 128
+ *   ids           [T][top] signed integers of id_bytes 4 or 8
+ *   weights       [T][top] of weight_bytes 4 (fp32) or 2 (bf16)
+ *   workspace     16-byte aligned, arc_moe_workspace_bytes, no initialisation needed
+ * Requirements: T <= ARC_MOE_MAX_TOKENS, T * top <= ARC_MOE_MAX_CHOICES, E <= 1024; x and the weights 16-byte
+ * aligned, their leading dimensions and strides multiples of 8. out overlaps no operand. The result does not
+ * depend on timing, nor a token's on the other tokens of a call of the same plan.
+ */
+#define ARC_MOE_MAX_TOKENS 256
+#define ARC_MOE_MAX_CHOICES 4096
+int arc_moe_workspace_bytes(int T, int top, int I, size_t *bytes);
+int arc_moe(const uint16_t *x, const void *w_in, const uint16_t *s_in, const void *w_out, const uint16_t *s_out,
+            const void *ids, int id_bytes, const void *weights, int weight_bytes, uint16_t *out, void *workspace,
+            size_t workspace_bytes, int T, int top, int E, int K, int I, int N, int64_t ldx, int64_t ld_in,
+            int64_t stride_in, int64_t ld_out, int64_t stride_out, int64_t ldo, int gated, int activation,
+            cudaStream_t stream);
+
+/*
  * Probe builds only (libarcb200_probe.so, compiled with -DARC_PROBE and loaded by the
  * Python package when the ARC_PROBE environment variable is set). Attaches a device
  * buffer of at least 64 uint64 per CTA; every kernel launched afterwards on the
