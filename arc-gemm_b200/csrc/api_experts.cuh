@@ -9,24 +9,26 @@ namespace {
 
 namespace EX = arcb::experts;
 
-// The instantiations the plan can choose: columns of a pass and row groups of a tile.
-#define ARC_EXPERT_VARIANTS(X) X(8, 1) X(8, 2) X(16, 2) X(16, 4) X(32, 2) X(32, 4)
+// The instantiations the plan can choose: columns of a pass, blocks of 16 rows and row groups of a tile.
+#define ARC_EXPERT_VARIANTS(X) X(8, 2, 1) X(8, 2, 2) X(8, 4, 1) X(8, 4, 2) X(16, 2, 2) X(16, 2, 4) X(16, 4, 1) X(16, 4, 2) X(32, 2, 2) X(32, 2, 4)
 
 using ExpertKernel = void (*)(EX::Params);
 
 struct ExpertVariant {
-  uint32_t nt, wr;
+  uint32_t nt, mr, wr;
   ExpertKernel kernel[2][2];  // [int4][second]
-  uint32_t stage_bytes[2], sum_bytes;
+  uint32_t stage_bytes[2], sum_bytes, rows;
 };
 constexpr ExpertVariant kExpertVariants[] = {
-#define ARC_EXPERT_ENTRY(NT, WR)                                                                         \
-  {NT,                                                                                                   \
-   WR,                                                                                                   \
-   {{EX::expert_layer_kernel<NT, WR, false, false>, EX::expert_layer_kernel<NT, WR, false, true>},       \
-    {EX::expert_layer_kernel<NT, WR, true, false>, EX::expert_layer_kernel<NT, WR, true, true>}},        \
-   {EX::Cfg<NT, WR, false>::kStageBytes, EX::Cfg<NT, WR, true>::kStageBytes},                            \
-   EX::Cfg<NT, WR, false>::kSumBytes},
+#define ARC_EXPERT_ENTRY(NT, MR, WR)                                                                             \
+  {NT,                                                                                                           \
+   MR,                                                                                                           \
+   WR,                                                                                                           \
+   {{EX::expert_layer_kernel<NT, MR, WR, false, false>, EX::expert_layer_kernel<NT, MR, WR, false, true>},       \
+    {EX::expert_layer_kernel<NT, MR, WR, true, false>, EX::expert_layer_kernel<NT, MR, WR, true, true>}},        \
+   {EX::Cfg<NT, MR, WR, false>::kStageBytes, EX::Cfg<NT, MR, WR, true>::kStageBytes},                            \
+   EX::Cfg<NT, MR, WR, false>::kSumBytes,                                                                        \
+   EX::Cfg<NT, MR, WR, false>::kRows},
     ARC_EXPERT_VARIANTS(ARC_EXPERT_ENTRY)
 #undef ARC_EXPERT_ENTRY
 };
@@ -50,11 +52,12 @@ int experts_init() {
 struct ExpertPlan {
   const ExpertVariant* v;
   uint32_t stages, smem, blocks_per_sm;
+  bool own_y;
 };
 
-const ExpertVariant* expert_variant(uint32_t nt, uint32_t wr) {
+const ExpertVariant* expert_variant(uint32_t nt, uint32_t mr, uint32_t wr) {
   for (const ExpertVariant& v : kExpertVariants) {
-    if (v.nt == nt && v.wr == wr) return &v;
+    if (v.nt == nt && v.mr == mr && v.wr == wr) return &v;
   }
   return nullptr;
 }
@@ -64,16 +67,19 @@ const ExpertVariant* expert_variant(uint32_t nt, uint32_t wr) {
 void expert_ring(const ExpertVariant& v, bool int4, bool second, uint32_t tokens, uint32_t slots, uint32_t experts,
                  ExpertPlan* plan) {
   const uint32_t parts = EX::kConsumers / v.wr;
-  const uint32_t rest = EX::layout_of(v.sum_bytes, 32 * v.wr, v.nt, tokens, slots, experts, second).total + 1024;
   const uint32_t stage = v.stage_bytes[int4 ? 1 : 0];
+  plan->v = &v;
+  plan->own_y = second && parts * v.rows * tokens * 4 <= 32 * 1024;
+  const uint32_t rest =
+      EX::layout_of(v.sum_bytes, parts, v.rows, v.nt, tokens, slots, experts, second, plan->own_y).total + 1024;
+  const uint32_t unit = parts < 4 ? 4 : parts;  // a whole number of parts and of batches
   const auto stages = [&](uint32_t budget) {
     const uint32_t n = budget > rest ? (budget - rest) / stage : 0;
-    return (n < EX::kMaxStages ? n : EX::kMaxStages) / parts * parts;
+    return (n < EX::kMaxStages ? n : EX::kMaxStages) / unit * unit;
   };
-  plan->v = &v;
   plan->blocks_per_sm = 2;
   plan->stages = stages(kExpertSmemHalf);
-  if (plan->stages * 32 * v.wr * EX::kRowBytes < 32 * 1024) {
+  if (plan->stages * v.rows * EX::kRowBytes < 32 * 1024) {
     plan->blocks_per_sm = 1;
     plan->stages = stages(kExpertSmemWhole);
   }
@@ -82,12 +88,12 @@ void expert_ring(const ExpertVariant& v, bool int4, bool second, uint32_t tokens
 
 // Weights of E experts as {bytes or elements of a row, rows, 2 (gate and up) or 1, E}.
 int encode_expert_weights(CUtensorMap* map, const void* w, bool int4, uint64_t inner, uint64_t cols, bool gated,
-                          uint64_t experts, uint64_t ld_bytes, uint64_t stride_bytes, uint32_t wr) {
+                          uint64_t experts, uint64_t ld_bytes, uint64_t stride_bytes, uint32_t rows) {
   EncodeTiledFn fn = encode_fn();
   if (fn == nullptr) return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[4] = {inner, cols, gated ? 2u : 1u, experts};
   const cuuint64_t strides[3] = {ld_bytes, ld_bytes * cols, experts > 1 ? stride_bytes : ld_bytes * cols};
-  const cuuint32_t box[4] = {int4 ? EX::kRowBytes : EX::kRowBytes / 2, gated ? 16 * wr : 32 * wr, gated ? 2u : 1u, 1};
+  const cuuint32_t box[4] = {int4 ? EX::kRowBytes : EX::kRowBytes / 2, gated ? rows / 2 : rows, gated ? 2u : 1u, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = fn(map, int4 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                         const_cast<void*>(w), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
@@ -188,17 +194,18 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   if (int st = current_device(&dev, &DeviceState::experts_status)) return st;
   const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
 
-  uint32_t nt = expert_columns(T, slots, E), wr1 = nt == 8 ? 1 : nt == 16 ? 2 : 4, wr2 = nt == 8 ? 1 : 2, splits = 0;
-  uint32_t per_sm = 2;
+  uint32_t nt = expert_columns(T, slots, E), mr1 = int4 && nt < 32 ? 4 : 2, mr2 = mr1, splits = 0, per_sm = 2;
+  uint32_t wr1 = nt == 8 ? 2 : 4 * 2 / mr1, wr2 = 2;
   if (const char* env = getenv("ARC_EXPERT_PLAN")) {
-    if (sscanf(env, "%u:%u:%u:%u:%u", &nt, &wr1, &wr2, &splits, &per_sm) < 3 || expert_variant(nt, wr1) == nullptr ||
-        expert_variant(nt, wr2) == nullptr || (splits & (splits - 1)) != 0 || splits > 8) {
-      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_EXPERT_PLAN must be 'columns:groups:groups[:S]' (got '%s')", env);
+    if (sscanf(env, "%u:%u:%u:%u:%u:%u:%u", &nt, &mr1, &wr1, &mr2, &wr2, &splits, &per_sm) < 5 ||
+        expert_variant(nt, mr1, wr1) == nullptr || expert_variant(nt, mr2, wr2) == nullptr ||
+        (splits & (splits - 1)) != 0 || splits > 8) {
+      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_EXPERT_PLAN must be 'NT:MR:WR:MR:WR[:S]' (got '%s')", env);
     }
   }
   ExpertPlan first, second;
-  expert_ring(*expert_variant(nt, wr1), int4, false, T, slots, E, &first);
-  expert_ring(*expert_variant(nt, wr2), int4, true, T, slots, E, &second);
+  expert_ring(*expert_variant(nt, mr1, wr1), int4, false, T, slots, E, &first);
+  expert_ring(*expert_variant(nt, mr2, wr2), int4, true, T, slots, E, &second);
   if (first.stages == 0 || second.stages == 0) return fail(ARC_ERR_UNSUPPORTED, "%s: does not fit in shared memory", what);
 
   EX::Params p = {};
@@ -208,13 +215,14 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   p.weights_bf16 = weight_bytes == 2;
   p.tokens = T;
   p.top = top;
+  p.top_inverse = top == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + top - 1) / top);
   p.experts = E;
   p.slots = slots;
   const uint32_t elem = int4 ? 1 : 2;
 
   // FIRST: h [slots][I].
   const uint32_t box_k = int4 ? 2 * EX::kRowBytes : EX::kRowBytes / 2;
-  if (int st = encode_expert_weights(&p.tm_w, w_in, int4, int4 ? K / 2 : K, I, gated, E, ld_in * elem, stride_in * elem, wr1)) {
+  if (int st = encode_expert_weights(&p.tm_w, w_in, int4, int4 ? K / 2 : K, I, gated, E, ld_in * elem, stride_in * elem, first.v->rows)) {
     return st;
   }
   if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, K, T, ldx, 64, 1, CU_TENSOR_MAP_SWIZZLE_128B, "x")) {
@@ -224,7 +232,7 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   p.out = static_cast<uint16_t*>(workspace);
   p.ldo = ldh;
   p.cols = I;
-  p.tiles = ceil_div(I, (gated ? 16 : 32) * wr1);
+  p.tiles = ceil_div(I, gated ? first.v->rows / 2 : first.v->rows);
   p.num_kb = ceil_div(K, box_k);
   p.groups = K / group;
   p.gated = gated ? 1 : 0;
@@ -238,7 +246,7 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   if (e != cudaSuccess) return cuda_fail(e, "expert_layer_kernel launch");
 
   // SECOND: y [T][N].
-  if (int st = encode_expert_weights(&p.tm_w, w_out, int4, int4 ? I / 2 : I, N, false, E, ld_out * elem, stride_out * elem, wr2)) {
+  if (int st = encode_expert_weights(&p.tm_w, w_out, int4, int4 ? I / 2 : I, N, false, E, ld_out * elem, stride_out * elem, second.v->rows)) {
     return st;
   }
   if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, workspace, I, slots, ldh, 64, 1,
@@ -249,7 +257,7 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   p.out = out;
   p.ldo = ldo;
   p.cols = N;
-  p.tiles = ceil_div(N, 32 * wr2);
+  p.tiles = ceil_div(N, second.v->rows);
   p.num_kb = ceil_div(I, box_k);
   p.groups = I / group;
   p.gated = 0;
@@ -257,10 +265,10 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   p.stages = second.stages;
   if (splits == 0) {
     splits = 1;
-    while (splits < 8 && p.tiles * splits * 2 <= sms * second.blocks_per_sm && p.num_kb >= splits * 2) splits *= 2;
+    while (splits < 8 && p.tiles * splits * 2 <= sms * second.blocks_per_sm) splits *= 2;
   }
-  while (splits > p.num_kb) splits /= 2;
   p.splits = splits;
+  p.own_y = second.own_y ? 1 : 0;
   e = launch_ex(second.v->kernel[int4][1], p, p.tiles * splits, EX::kThreads, second.smem, splits, stream);
   if (e != cudaSuccess) return cuda_fail(e, "expert_layer_kernel launch");
   return ARC_OK;

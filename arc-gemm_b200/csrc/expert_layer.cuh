@@ -51,25 +51,30 @@ struct Params {
   uint64_t ldo;
   uint32_t ids_wide, weights_bf16;  // int64 ids; bf16 weights
   uint32_t tokens, top, experts, slots;
+  uint32_t top_inverse;  // ceil(2^32 / top), for choices below 2^16; 0 for one choice a token
   uint32_t cols, tiles;  // output columns, tiles of them
   uint32_t num_kb;       // boxes along the contraction
   uint32_t groups;       // scale groups along it
   uint32_t gated, act;
   uint32_t stages;       // of the ring, a multiple of WK
-  uint32_t splits;       // SECOND: blocks of a cluster, which share the contraction
+  uint32_t splits;       // SECOND: blocks of a cluster, which share the passes' boxes
+  uint32_t own_y;        // SECOND: see Layout
 };
 
-template <uint32_t NT, uint32_t WR, bool INT4>
+// NT columns of a pass; a tile is WR groups of MR blocks of 16 weight rows.
+template <uint32_t NT, uint32_t MR, uint32_t WR, bool INT4>
 struct Cfg {
   static_assert(NT == 8 || NT == 16 || NT == 32, "columns of a pass");
+  static_assert(MR == 2 || MR == 4, "blocks of rows: half of them gate, half of them up");
   static constexpr uint32_t kParts = kConsumers / WR;  // WK
   static_assert(kParts >= 2, "parts of the contraction");
-  static constexpr uint32_t kRows = 32 * WR;
+  static constexpr uint32_t kRows = 16 * MR * WR;
   static constexpr uint32_t kSub = INT4 ? 4 : 1;  // boxes of tokens per box of weights
   static constexpr uint32_t kWBytes = kRows * kRowBytes;
   static constexpr uint32_t kXBytes = NT * kRowBytes;  // a box of tokens
   static constexpr uint32_t kStageBytes = kWBytes + kSub * kXBytes;
   static constexpr uint32_t kSumBytes = kParts * kRows * NT * 4;
+  static constexpr uint32_t kBatch = kParts < 4 ? kParts : 4;  // boxes loaded at a time
 };
 
 // One pass over an expert's weights, for up to NT of its choices.
@@ -77,17 +82,18 @@ struct Pass {
   uint16_t expert, first, count, unused;
 };
 
-// Shared memory behind the ring, in bytes from its end.
+// Shared memory behind the ring, in bytes from its end. SECOND with `own_y`: every part of the contraction adds
+// to sums of y of its own, and the parts' sums of an item are not exchanged.
 struct Layout {
   uint32_t sums, y, passes, list, ids, share, total;
 };
-__host__ __device__ inline Layout layout_of(uint32_t sum_bytes, uint32_t rows, uint32_t nt, uint32_t tokens,
-                                            uint32_t slots, uint32_t experts, bool second) {
+__host__ __device__ inline Layout layout_of(uint32_t sum_bytes, uint32_t parts, uint32_t rows, uint32_t nt,
+                                            uint32_t tokens, uint32_t slots, uint32_t experts, bool second, bool own_y) {
   const auto up = [](uint32_t v) { return (v + 15u) & ~15u; };
   Layout l;
   l.sums = 0;
-  l.y = l.sums + sum_bytes;
-  l.passes = l.y + (second ? tokens * rows * 4u : 0u);
+  l.y = l.sums + (own_y ? 0u : sum_bytes);
+  l.passes = l.y + (second ? tokens * rows * 4u * (own_y ? parts : 1u) : 0u);
   const uint32_t live = experts < slots ? experts : slots;
   l.list = l.passes + up((live + slots / nt) * 8u);
   l.ids = l.list + up(slots * 2u);
@@ -228,6 +234,10 @@ __device__ __forceinline__ uint32_t sort_choices(const Params& p, Pass* passes, 
   return *totals;
 }
 
+__device__ __forceinline__ uint32_t token_of(const Params& p, uint32_t s) {
+  return p.top_inverse == 0u ? s : __umulhi(s, p.top_inverse);
+}
+
 // The weight of choice s: with those of its token's later choices of the same expert.
 __device__ __forceinline__ float share_of(const Params& p, uint32_t s) {
   float sum = 0.f;
@@ -245,9 +255,9 @@ __device__ __forceinline__ float share_of(const Params& p, uint32_t s) {
   return sum;
 }
 
-template <uint32_t NT, uint32_t WR, bool INT4, bool SECOND>
+template <uint32_t NT, uint32_t MR, uint32_t WR, bool INT4, bool SECOND>
 __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_constant__ Params p) {
-  using C = Cfg<NT, WR, INT4>;
+  using C = Cfg<NT, MR, WR, INT4>;
   constexpr uint32_t WK = C::kParts;
   constexpr uint32_t kTiles8 = NT / 8;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
@@ -255,9 +265,10 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
   __shared__ uint32_t abort_flag, num_passes;
   uint8_t* ring = smem_raw + smem_align_pad(smem_raw);
   uint8_t* rest = ring + p.stages * C::kStageBytes;
-  const Layout l = layout_of(C::kSumBytes, C::kRows, NT, p.tokens, p.slots, p.experts, SECOND);
+  const Layout l =
+      layout_of(C::kSumBytes, WK, C::kRows, NT, p.tokens, p.slots, p.experts, SECOND, SECOND && p.own_y != 0u);
   float* sums = reinterpret_cast<float*>(rest + l.sums);  // [WK][kTiles8][kRows][8]
-  float* y = reinterpret_cast<float*>(rest + l.y);        // SECOND: [tokens][kRows]
+  float* y = reinterpret_cast<float*>(rest + l.y);        // SECOND: [own_y ? WK : 1][tokens][kRows]
   Pass* passes = reinterpret_cast<Pass*>(rest + l.passes);
   uint16_t* list = reinterpret_cast<uint16_t*>(rest + l.list);
   uint16_t* ids = reinterpret_cast<uint16_t*>(rest + l.ids);
@@ -283,8 +294,9 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
     pdl_launch_dependents();
   }
   const uint32_t passes_n = sort_choices<NT>(p, passes, list, ids, reinterpret_cast<uint16_t*>(ring), &num_passes);
+  const uint32_t y_size = p.tokens * C::kRows;
   if (SECOND) {
-    for (uint32_t i = threadIdx.x; i < p.tokens * C::kRows; i += kThreads) y[i] = 0.f;
+    for (uint32_t i = threadIdx.x; i < y_size * (p.own_y ? WK : 1u); i += kThreads) y[i] = 0.f;
     const uint32_t listed = passes_n == 0u ? 0u : passes[passes_n - 1u].first + passes[passes_n - 1u].count;
     for (uint32_t i = threadIdx.x; i < listed; i += kThreads) share[i] = share_of(p, list[i]);
   }
@@ -292,95 +304,119 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
   fence_proxy_async_smem();
   __syncthreads();
 
-  // This block's walk: items of (pass, column tile), each a run of boxes along the contraction.
+  // This block's walk: items of (pass, column tile), each a run of boxes along the contraction. FIRST: tiles of a
+  // pass side by side over the blocks, whole items. SECOND: one tile, all passes; the blocks of a cluster share
+  // the passes' boxes evenly, so an item may be cut at either end.
   const uint32_t rank = SECOND && p.splits > 1u ? cluster_ctarank() : 0u;
-  const uint32_t kb0 = SECOND ? p.num_kb * rank / p.splits : 0u;
-  const uint32_t nkb = SECOND ? p.num_kb * (rank + 1u) / p.splits - kb0 : p.num_kb;
+  const uint32_t nkb = p.num_kb;
   const uint32_t tile_cols = p.gated ? C::kRows / 2u : C::kRows;
-  uint32_t item0, item_step, item_end;
-  if (SECOND) {  // one tile, every pass
-    item0 = 0;
-    item_step = 1;
-    item_end = passes_n;
-  } else {  // tiles of a pass side by side
-    item0 = blockIdx.x;
-    item_step = gridDim.x;
-    item_end = passes_n * p.tiles;
-  }
   const uint32_t my_tile = SECOND ? blockIdx.x / p.splits : 0u;
+  const uint32_t item_step = SECOND ? 1u : gridDim.x;
+  uint32_t item0, kb_first, boxes;
+  if (SECOND) {
+    const uint32_t all = passes_n * nkb;
+    const uint32_t from = static_cast<uint32_t>(uint64_t(all) * rank / p.splits);
+    boxes = static_cast<uint32_t>(uint64_t(all) * (rank + 1u) / p.splits) - from;
+    item0 = from / nkb;
+    kb_first = from - item0 * nkb;
+  } else {
+    const uint32_t items = passes_n * p.tiles;
+    item0 = blockIdx.x;
+    kb_first = 0;
+    boxes = item0 < items ? (items - item0 + item_step - 1u) / item_step * nkb : 0u;
+  }
 
   if (warp == kConsumers) {
     // ------------------------------------------------------------ producer
-    uint32_t stage = 0, phase = 0, issued = 0;
-    bool ok = true;
-    const auto coords = [&](uint32_t item, Pass& ps, uint32_t& f0) {
+    // kBatch boxes at a time, lane i for the weights of the i-th: their waits, and the issue of their loads,
+    // run side by side (box by box a block fetched 4 KB per 780 cycles, whatever was in flight).
+    constexpr uint32_t kBatch = C::kBatch;
+    uint32_t item = item0, kb = kb_first + lane;  // of this lane's box
+    Pass ps = {0, 0, 1, 0};
+    uint32_t f0 = 0;
+    const auto locate = [&]() {
+      while (kb >= nkb) {
+        kb -= nkb;
+        item += item_step;
+      }
       const uint32_t pi = SECOND ? item : item / p.tiles;
       ps = passes[pi];
       f0 = (SECOND ? my_tile : item - pi * p.tiles) * tile_cols;
     };
-    const auto load_weights = [&](const Pass& ps, uint32_t f0, uint32_t kb, uint32_t st) {
-      const uint32_t quads = (ps.count + 3u) / 4u;
-      mbar_arrive_expect_tx(&full[st], C::kWBytes + C::kSub * quads * 4u * kRowBytes);
+    const auto load_weights = [&](uint32_t st) {
+      mbar_arrive_expect_tx(&full[st], C::kWBytes + C::kSub * ((ps.count + 3u) / 4u) * 4u * kRowBytes);
       tma_load_4d(&p.tm_w, &full[st], ring + st * C::kStageBytes, int32_t(kb * (INT4 ? kRowBytes : kRowBytes / 2u)),
                   int32_t(f0), 0, ps.expert, kCacheEvictNormal);
-    };
-    const auto load_rows = [&](const Pass& ps, uint32_t kb, uint32_t st) {
-      const uint32_t quads = (ps.count + 3u) / 4u;
-      for (uint32_t g = lane; g < quads * C::kSub; g += 32u) {
-        const uint32_t sub = g / quads, quad = g - sub * quads;
-        int32_t r[4];
-#pragma unroll
-        for (uint32_t i = 0; i < 4; ++i) {
-          const uint32_t c = quad * 4u + i;
-          const uint32_t s = list[ps.first + min(c, ps.count - 1u)];
-          r[i] = c < ps.count ? int32_t(SECOND ? s : s / p.top) : int32_t(SECOND ? p.slots : p.tokens);
-        }
-        tma_gather4(&p.tm_x, &full[st], ring + st * C::kStageBytes + C::kWBytes + sub * C::kXBytes + quad * 4u * kRowBytes,
-                    int32_t((kb * C::kSub + sub) * 64u), r[0], r[1], r[2], r[3], kCacheEvictLast);
-      }
     };
     uint32_t ahead = 0;  // boxes whose weights are on their way
     if (SECOND) {
       // The first weights do not wait for the first launch.
-      ahead = min(p.stages, item_end * nkb);
-      if (lane == 0) {
-        for (uint32_t b = 0; b < ahead; ++b) {
-          Pass ps;
-          uint32_t f0;
-          coords(b / nkb, ps, f0);
-          load_weights(ps, f0, kb0 + b % nkb, b);
+      ahead = min(p.stages, boxes);
+      if (lane < kBatch) {
+        for (uint32_t b = lane; b < ahead; b += kBatch) {
+          locate();
+          load_weights(b);
+          kb += kBatch;
         }
       }
+      item = item0, kb = kb_first + lane;
       __syncwarp();
       pdl_wait();
       pdl_launch_dependents();
     }
-    for (uint32_t item = item0; ok && item < item_end; item += item_step) {
-      Pass ps;
-      uint32_t f0;
-      coords(item, ps, f0);
-      for (uint32_t kb = 0; kb < nkb; ++kb) {
-        if (issued >= ahead) {
-          if (lane == 0) {
-            ok = mbar_wait(&empty[stage], phase ^ 1u, abort, kStatusTimeoutProducer);
-            if (ok) load_weights(ps, f0, kb0 + kb, stage);
-          }
-          ok = __shfl_sync(0xffffffffu, ok ? 1u : 0u, 0) != 0u;
-          if (!ok) break;
+    uint32_t stage = lane % kBatch, phase = 0, issued = 0;  // of this lane's box; boxes it has loaded
+    for (uint32_t b0 = 0; b0 < boxes; b0 += kBatch) {
+      const bool mine = lane < kBatch && b0 + lane < boxes;
+      bool go = mine;
+      if (mine) {
+        locate();
+        if (b0 + lane >= ahead) {
+          go = mbar_wait(&empty[stage], phase ^ 1u, abort, kStatusTimeoutProducer);
+          if (go) load_weights(stage);
         }
-        load_rows(ps, kb0 + kb, stage);
+      }
+      const uint32_t going = __ballot_sync(0xffffffffu, go);
+      // Rows of all boxes that go, four a gather.
+      constexpr uint32_t kQuads = NT / 4u, kPerBox = kQuads * C::kSub;
+#pragma unroll
+      for (uint32_t g0 = 0; g0 < kBatch * kPerBox; g0 += 32u) {
+        const uint32_t g = g0 + lane, box = g / kPerBox, sub = g % kPerBox / kQuads, quad = g % kQuads;
+        const uint32_t from = box < kBatch ? box : 0u;
+        const uint32_t first = __shfl_sync(0xffffffffu, uint32_t(ps.first), from);
+        const uint32_t count = __shfl_sync(0xffffffffu, uint32_t(ps.count), from);
+        const uint32_t k = __shfl_sync(0xffffffffu, kb, from);
+        const uint32_t st = __shfl_sync(0xffffffffu, stage, from);
+        if (box < kBatch && ((going >> box) & 1u) != 0u && quad * 4u < count) {
+          int32_t r[4];
+#pragma unroll
+          for (uint32_t i = 0; i < 4; ++i) {
+            const uint32_t c = quad * 4u + i;
+            const uint32_t s = list[first + min(c, count - 1u)];
+            r[i] = int32_t(SECOND ? (c < count ? s : p.slots) : (c < count ? token_of(p, s) : p.tokens));
+          }
+          tma_gather4(&p.tm_x, &full[st],
+                      ring + st * C::kStageBytes + C::kWBytes + sub * C::kXBytes + quad * 4u * kRowBytes,
+                      int32_t((k * C::kSub + sub) * 64u), r[0], r[1], r[2], r[3], kCacheEvictLast);
+        }
+      }
+      if (go) {
         ++issued;
-        if (++stage == p.stages) {
-          stage = 0;
+        kb += kBatch;
+        stage += kBatch;
+        if (stage >= p.stages) {
+          stage -= p.stages;
           phase ^= 1u;
         }
       }
+      if (__any_sync(0xffffffffu, mine && !go)) break;
     }
-    // Copies in flight land before the block may exit (of every box both parts are on their way: the
-    // only wait that can be abandoned comes behind the boxes loaded ahead).
-    if (lane == 0) {
-      const uint32_t n = min(issued, p.stages);
-      for (uint32_t i = issued - n; i < issued; ++i) mbar_drain(&full[i % p.stages], (i / p.stages) & 1u);
+    // Copies in flight land before the block may exit.
+    if (lane < kBatch) {
+      const uint32_t per_lane = p.stages / kBatch;
+      for (uint32_t i = issued - min(issued, per_lane); i < issued; ++i) {
+        const uint32_t b = i * kBatch + lane;
+        mbar_drain(&full[b % p.stages], (b / p.stages) & 1u);
+      }
     }
     __syncwarp();
   } else {
@@ -388,42 +424,79 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
     if (SECOND) pdl_wait();
     const uint32_t wr = warp % WR, part = warp / WR;
     const uint32_t g8 = lane >> 2, q = lane & 3u;
-    uint32_t stage = part, phase = 0;  // of this part's next box
-    uint32_t done = 0;                 // boxes of the items before
+    // Lanes of a quarter warp take the rows r and r + 4, whose halves of 128 swizzled bytes lie in different
+    // banks: a 16-byte read of four lanes a row meets no conflict. So column n of a product is row perm(n).
+    const uint32_t perm = (g8 >> 1) | (g8 & 1u) << 2;
+    uint32_t stage = part, phase = 0;             // of this part's next box
+    uint32_t box = part;                          // its running number
+    uint32_t item = item0, kb = kb_first + part;  // and where it lies
     bool ok = true;
-    for (uint32_t item = item0; item < item_end; item += item_step) {
-      const uint32_t pi = SECOND ? item : item / p.tiles;
-      const Pass ps = passes[pi];
-      const uint32_t f0 = (SECOND ? my_tile : item - pi * p.tiles) * tile_cols;
-      float acc[2][kTiles8][4];
+
+    // int4: the scales of a box, two groups a weight row, on their way a box ahead. Lane l has row l (and l + 32) of
+    // this warp's rows.
+    constexpr uint32_t kScaleRegs = MR / 2;
+    uint32_t scales[kScaleRegs];
+    const auto fetch_scales = [&]() {
+      if constexpr (INT4) {
+        const uint32_t pi = SECOND ? item : item / p.tiles;
+        const uint32_t f0 = (SECOND ? my_tile : item - pi * p.tiles) * tile_cols;
+        const uint32_t rows = p.gated ? 2u * p.cols : p.cols;
+        const uint32_t g0 = kb * 2u;
 #pragma unroll
-      for (uint32_t m = 0; m < 2; ++m) {
+        for (uint32_t i = 0; i < kScaleRegs; ++i) {
+          const uint32_t m = i * 2u + (lane >> 4);
+          const bool up = p.gated && m >= MR / 2;
+          const uint32_t f = f0 + ((up ? m - MR / 2 : m) * WR + wr) * 16u + (lane & 15u);
+          uint32_t bits = 0;
+          if (f < p.cols) {
+            const uint16_t* at = p.sb + (size_t(passes[pi].expert) * rows + f + (up ? p.cols : 0u)) * p.groups + g0;
+            if ((p.groups & 1u) == 0u && (reinterpret_cast<uintptr_t>(p.sb) & 3u) == 0u) {
+              bits = __ldg(reinterpret_cast<const uint32_t*>(at));
+            } else {
+              bits = __ldg(at);
+              if (g0 + 1u < p.groups) bits |= static_cast<uint32_t>(__ldg(at + 1)) << 16;
+            }
+          }
+          scales[i] = bits;
+        }
+      }
+    };
+    const auto locate = [&]() {
+      while (kb >= nkb) {
+        kb -= nkb;
+        item += item_step;
+      }
+    };
+    if (box < boxes) {
+      locate();
+      fetch_scales();
+    }
+
+    const uint32_t last = boxes == 0u ? 0u : kb_first + boxes;  // boxes from the first item's start to this block's last one
+    for (uint32_t at = item0, before = 0; before < last; at += item_step, before += nkb) {
+      const uint32_t pi = SECOND ? at : at / p.tiles;
+      const Pass ps = passes[pi];
+      const uint32_t f0 = (SECOND ? my_tile : at - pi * p.tiles) * tile_cols;
+      float acc[MR][kTiles8][4];
+#pragma unroll
+      for (uint32_t m = 0; m < MR; ++m) {
 #pragma unroll
         for (uint32_t j = 0; j < kTiles8; ++j) {
 #pragma unroll
           for (uint32_t i = 0; i < 4; ++i) acc[m][j][i] = 0.f;
         }
       }
-      // The boxes whose running number is `part` modulo WK.
-      for (uint32_t kb = (part + WK - done % WK) % WK; kb < nkb; kb += WK) {
-        uint32_t scale_bits[2][2];  // int4: of the box's two groups, per block of rows: rows g8 and g8 + 8
-        if constexpr (INT4) {
-          const uint32_t g0 = (kb0 + kb) * 2u;
+      bool any = false;
+      while (box < boxes && item == at) {
+        any = true;
+        uint32_t sc[kScaleRegs];
 #pragma unroll
-          for (uint32_t m = 0; m < 2; ++m) {
-#pragma unroll
-            for (uint32_t i = 0; i < 2; ++i) {
-              const uint32_t f = f0 + (p.gated ? wr * 16u : (m * WR + wr) * 16u) + i * 8u + g8;
-              const uint32_t row = f + (p.gated ? m * p.cols : 0u);
-              uint32_t bits = 0;
-              if (f < p.cols) {
-                const uint16_t* at = p.sb + (size_t(ps.expert) * (p.gated ? 2u * p.cols : p.cols) + row) * p.groups + g0;
-                bits = __ldg(at);
-                if (g0 + 1u < p.groups) bits |= static_cast<uint32_t>(__ldg(at + 1)) << 16;
-              }
-              scale_bits[m][i] = bits;
-            }
-          }
+        for (uint32_t i = 0; i < kScaleRegs; ++i) sc[i] = scales[i];
+        box += WK;
+        kb += WK;
+        if (box < boxes) {
+          locate();
+          fetch_scales();
         }
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort, kStatusTimeoutMma));
         const uint32_t w_at = smem_u32(ring + stage * C::kStageBytes), x_at = w_at + C::kWBytes;
@@ -440,7 +513,7 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
                 }
               }
 #pragma unroll
-              for (uint32_t m = 0; m < 2; ++m) {
+              for (uint32_t m = 0; m < MR; ++m) {
 #pragma unroll
                 for (uint32_t k = 0; k < 2; ++k) {
                   uint32_t a[4];
@@ -456,9 +529,9 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
           } else {
 #pragma unroll
             for (uint32_t g = 0; g < 2; ++g) {  // scale groups
-              float part_sum[2][kTiles8][4];
+              float part_sum[MR][kTiles8][4];
 #pragma unroll
-              for (uint32_t m = 0; m < 2; ++m) {
+              for (uint32_t m = 0; m < MR; ++m) {
 #pragma unroll
                 for (uint32_t j = 0; j < kTiles8; ++j) {
 #pragma unroll
@@ -468,35 +541,45 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
 #pragma unroll
               for (uint32_t c4 = 0; c4 < 4; ++c4) {  // 32 codes of a row, 16 bytes
                 const uint32_t c = g * 4u + c4;
-                uint32_t a[4];  // rows 0-7 and 8-15 of the two blocks of rows
-                {
-                  const uint32_t row = ((lane >> 4) * WR + wr) * 16u + (lane & 15u);
-                  ldmatrix_x4(w_at + row * kRowBytes + ((c ^ (row & 7u)) << 4), a);
-                }
-                uint32_t v[4][4];
-#pragma unroll
-                for (uint32_t i = 0; i < 4; ++i) codes_to_bf16(a[i], v[i]);
+                // Pairs of k: (0, 4), (1, 5), (2, 6), (3, 7) of a lane's eight, as the codes come.
+                uint32_t b[kTiles8][4];
 #pragma unroll
                 for (uint32_t j = 0; j < kTiles8; ++j) {
                   if (j * 8u < ps.count) {
-                    // Lanes of column n take row n / 2 + 4 (n % 2), so that a quarter of a warp reads all banks.
-                    const uint32_t row = (g8 >> 1) | (g8 & 1u) << 2, chunk = (c & 1u) * 4u + q;
                     uint32_t x[4];  // k = 8 q .. 8 q + 7 of the 32
-                    lds_128(x_at + (c >> 1) * C::kXBytes + (j * 8u + row) * kRowBytes + ((chunk ^ row) << 4), x);
-                    const uint32_t b0 = __byte_perm(x[0], x[2], 0x5410), b1 = __byte_perm(x[0], x[2], 0x7632);
-                    const uint32_t b2 = __byte_perm(x[1], x[3], 0x5410), b3 = __byte_perm(x[1], x[3], 0x7632);
+                    lds_128(x_at + (c >> 1) * C::kXBytes + (j * 8u + perm) * kRowBytes + ((((c & 1u) * 4u + q) ^ perm) << 4), x);
+                    b[j][0] = __byte_perm(x[0], x[2], 0x5410);
+                    b[j][1] = __byte_perm(x[0], x[2], 0x7632);
+                    b[j][2] = __byte_perm(x[1], x[3], 0x5410);
+                    b[j][3] = __byte_perm(x[1], x[3], 0x7632);
+                  }
+                }
 #pragma unroll
-                    for (uint32_t m = 0; m < 2; ++m) {
-                      mma_bf16(part_sum[m][j], v[2 * m][0], v[2 * m + 1][0], v[2 * m][1], v[2 * m + 1][1], b0, b1);
-                      mma_bf16(part_sum[m][j], v[2 * m][2], v[2 * m + 1][2], v[2 * m][3], v[2 * m + 1][3], b2, b3);
+                for (uint32_t m2 = 0; m2 < MR; m2 += 2) {
+                  uint32_t a[4];  // rows 0-7 and 8-15 of two blocks of rows
+                  const uint32_t row = ((m2 + (lane >> 4)) * WR + wr) * 16u + (lane & 15u);
+                  ldmatrix_x4(w_at + row * kRowBytes + ((c ^ (row & 7u)) << 4), a);
+#pragma unroll
+                  for (uint32_t m = 0; m < 2; ++m) {
+                    uint32_t lo[4], hi[4];
+                    codes_to_bf16(a[2 * m], lo);
+                    codes_to_bf16(a[2 * m + 1], hi);
+#pragma unroll
+                    for (uint32_t j = 0; j < kTiles8; ++j) {
+                      if (j * 8u < ps.count) {
+                        mma_bf16(part_sum[m2 + m][j], lo[0], hi[0], lo[1], hi[1], b[j][0], b[j][1]);
+                        mma_bf16(part_sum[m2 + m][j], lo[2], hi[2], lo[3], hi[3], b[j][2], b[j][3]);
+                      }
                     }
                   }
                 }
               }
 #pragma unroll
-              for (uint32_t m = 0; m < 2; ++m) {
-                const float s0 = __uint_as_float(g == 0 ? scale_bits[m][0] << 16 : scale_bits[m][0] & 0xFFFF0000u);
-                const float s1 = __uint_as_float(g == 0 ? scale_bits[m][1] << 16 : scale_bits[m][1] & 0xFFFF0000u);
+              for (uint32_t m = 0; m < MR; ++m) {
+                const uint32_t s_lo = __shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + g8);
+                const uint32_t s_hi = __shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + 8u + g8);
+                const float s0 = __uint_as_float(g == 0 ? s_lo << 16 : s_lo & 0xFFFF0000u);
+                const float s1 = __uint_as_float(g == 0 ? s_hi << 16 : s_hi & 0xFFFF0000u);
 #pragma unroll
                 for (uint32_t j = 0; j < kTiles8; ++j) {
                   if (j * 8u < ps.count) {
@@ -518,24 +601,48 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
           phase ^= 1u;
         }
       }
-      done += nkb;
 
+      // Columns of a product that this lane holds.
+      const uint32_t col[2] = {INT4 ? q : 2u * q, INT4 ? q + 4u : 2u * q + 1u};
+      if (SECOND && p.own_y) {
+        // Into this part's own sums of y: a pass holds a token once, so no two lanes meet.
+        if (any) {
+#pragma unroll
+          for (uint32_t j = 0; j < kTiles8; ++j) {
+#pragma unroll
+            for (uint32_t i = 0; i < 2; ++i) {
+              const uint32_t c = j * 8u + col[i];
+              if (c < ps.count) {
+                const float w = share[ps.first + c];
+                float* to = y + part * y_size + token_of(p, list[ps.first + c]) * C::kRows + wr * 16u + g8;
+#pragma unroll
+                for (uint32_t m = 0; m < MR; ++m) {
+                  to[m * WR * 16u] = fmaf(w, acc[m][j][i], to[m * WR * 16u]);
+                  to[m * WR * 16u + 8u] = fmaf(w, acc[m][j][2 + i], to[m * WR * 16u + 8u]);
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();  // another lane may hold the token in the next pass
+        continue;
+      }
       // The parts' sums meet in shared memory.
       named_barrier_sync(1, kConsumers * 32);  // the last item's have been read
 #pragma unroll
       for (uint32_t j = 0; j < kTiles8; ++j) {
         if (j * 8u < ps.count) {
 #pragma unroll
-          for (uint32_t m = 0; m < 2; ++m) {
-            float* at = sums + ((part * kTiles8 + j) * C::kRows + (m * WR + wr) * 16u + g8) * 8u;
+          for (uint32_t m = 0; m < MR; ++m) {
+            float* to = sums + ((part * kTiles8 + j) * C::kRows + (m * WR + wr) * 16u + g8) * 8u;
             if constexpr (INT4) {
-              at[q] = acc[m][j][0];
-              at[q + 4] = acc[m][j][1];
-              at[64 + q] = acc[m][j][2];
-              at[64 + q + 4] = acc[m][j][3];
+              to[q] = acc[m][j][0];
+              to[q + 4] = acc[m][j][1];
+              to[64 + q] = acc[m][j][2];
+              to[64 + q + 4] = acc[m][j][3];
             } else {
-              *reinterpret_cast<float2*>(at + 2 * q) = make_float2(acc[m][j][0], acc[m][j][1]);
-              *reinterpret_cast<float2*>(at + 64 + 2 * q) = make_float2(acc[m][j][2], acc[m][j][3]);
+              *reinterpret_cast<float2*>(to + 2 * q) = make_float2(acc[m][j][0], acc[m][j][1]);
+              *reinterpret_cast<float2*>(to + 64 + 2 * q) = make_float2(acc[m][j][2], acc[m][j][3]);
             }
           }
         }
@@ -552,8 +659,8 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
         if (f0 + f >= p.cols) continue;
         const uint32_t s = list[ps.first + c];
         if (SECOND) {
-          float* at = y + (s / p.top) * C::kRows + f;
-          *at = fmaf(share[ps.first + c], total(f, c), *at);
+          float* to = y + token_of(p, s) * C::kRows + f;
+          *to = fmaf(share[ps.first + c], total(f, c), *to);
         } else {
           float v[2] = {total(f, c), 0.f};
           lin::activate(v, p.act);
@@ -567,11 +674,21 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
 
   if (SECOND) {
     const uint32_t f0 = my_tile * C::kRows, cols = min(C::kRows, p.cols - f0);
+    const auto part_total = [&](uint32_t o) {
+      float v = y[o];
+      if (p.own_y) {
+        for (uint32_t k = 1; k < WK; ++k) v += y[k * y_size + o];
+      }
+      return v;
+    };
     if (p.splits > 1u) {
       __syncthreads();
+      if (p.own_y) {
+        for (uint32_t o = threadIdx.x; o < y_size; o += kThreads) y[o] = part_total(o);
+      }
       cluster_sync_all();
       // Block r of the cluster finishes the tokens r, r + S, ...
-      for (uint32_t o = threadIdx.x; o < p.tokens * C::kRows; o += kThreads) {
+      for (uint32_t o = threadIdx.x; o < y_size; o += kThreads) {
         const uint32_t f = o % C::kRows, t = o / C::kRows;
         if (t % p.splits != rank || f >= cols) continue;
         float v = 0.f;
@@ -580,9 +697,9 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
       }
       cluster_sync_all();
     } else if (warp < kConsumers) {
-      for (uint32_t o = threadIdx.x; o < p.tokens * C::kRows; o += kConsumers * 32u) {
+      for (uint32_t o = threadIdx.x; o < y_size; o += kConsumers * 32u) {
         const uint32_t f = o % C::kRows, t = o / C::kRows;
-        if (f < cols) p.out[size_t(t) * p.ldo + f0 + f] = __bfloat16_as_ushort(__float2bfloat16_rn(y[o]));
+        if (f < cols) p.out[size_t(t) * p.ldo + f0 + f] = __bfloat16_as_ushort(__float2bfloat16_rn(part_total(o)));
       }
     }
   }

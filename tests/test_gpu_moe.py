@@ -65,7 +65,8 @@ def test_int4(cuda_device, shape, gated):
 
 
 @pytest.mark.parametrize("kind", ["bf16", "int4"])
-@pytest.mark.parametrize("plan", ["8:1:1:1", "8:2:1:2", "8:1:2:4", "16:2:2:8", "16:4:4:2", "32:4:2:1", "32:2:4:2"])
+@pytest.mark.parametrize("plan", ["8:2:1:2:1:1", "8:2:2:2:1:2", "8:2:1:2:2:4", "8:4:1:4:2:2", "8:4:2:4:1:4", "16:2:2:2:4:8", "16:2:4:2:2:2", "16:4:1:4:2:1", "16:4:2:4:1:2", "32:2:4:2:2:1",
+                                  "32:2:2:2:4:2"])
 def test_plans(cuda_device, monkeypatch, plan, kind):
     """Every instantiation and cluster size, with experts of more choices than a pass holds."""
     monkeypatch.setenv("ARC_EXPERT_PLAN", plan)
