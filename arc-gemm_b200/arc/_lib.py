@@ -86,7 +86,7 @@ SIGNATURES = {
     "arc_a8w4_grouped_gemm": ([_P] * 7 + [ctypes.c_size_t] + [_I] * 5 + [ctypes.c_uint, _P], _I),
     "arc_group_rows_workspace_bytes": ([_I, _I, ctypes.POINTER(ctypes.c_size_t)], _I),
     "arc_group_rows": ([_P, _I, _P, _P, _P, _P, ctypes.c_size_t, _I, _I, _I, _P], _I),
-    "arc_moe_workspace_bytes": ([_I] * 3 + [ctypes.POINTER(ctypes.c_size_t)], _I),
+    "arc_moe_workspace_bytes": ([_I] * 5 + [ctypes.POINTER(ctypes.c_size_t)], _I),
     "arc_moe": ([_P] * 6 + [_I, _P, _I, _P, _P, ctypes.c_size_t] + [_I] * 6 + [_L] * 6 + [_I, _I, _P], _I),
     "arc_a8w4_gemm_gather_sync": ([_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_uint, _P], _I),
 }

@@ -9,37 +9,40 @@ namespace {
 
 namespace EX = arcb::experts;
 
-// The instantiations the plan can choose: columns of a pass, blocks of 16 rows and row groups of a tile.
-#define ARC_EXPERT_VARIANTS(X) X(8, 2, 1) X(8, 2, 2) X(8, 4, 1) X(8, 4, 2) X(16, 2, 2) X(16, 2, 4) X(16, 4, 1) X(16, 4, 2) X(32, 2, 2) X(32, 2, 4)
-
+// The kernels by weights and columns of a pass. Tiles (blocks of 16 rows x row groups) as measured best, 4096 x 2048
+// experts, microseconds: bf16 16 tokens of 64 experts (8 columns) 2x2 334, 2x1 389, 4x2 366; 64 tokens (16 columns)
+// 2x4 both 495, 2x2 both 512; 128 tokens (32 columns) 2x4 and 2x2 659, 2x2 both 699; int4 32 tokens (8
+// columns) 4x2 222, 2x2 272, 4x1 264; 64 tokens (16 columns) 2x4 and 2x2 338, 2x2 both 348.
 using ExpertKernel = void (*)(EX::Params);
-
 struct ExpertVariant {
-  uint32_t nt, mr, wr;
-  ExpertKernel kernel[2][2];  // [int4][second]
-  uint32_t stage_bytes[2], sum_bytes, rows;
+  ExpertKernel kernel;
+  uint32_t rows, parts, stage_bytes, weight_bytes, sum_bytes;
 };
-constexpr ExpertVariant kExpertVariants[] = {
-#define ARC_EXPERT_ENTRY(NT, MR, WR)                                                                             \
-  {NT,                                                                                                           \
-   MR,                                                                                                           \
-   WR,                                                                                                           \
-   {{EX::expert_layer_kernel<NT, MR, WR, false, false>, EX::expert_layer_kernel<NT, MR, WR, false, true>},       \
-    {EX::expert_layer_kernel<NT, MR, WR, true, false>, EX::expert_layer_kernel<NT, MR, WR, true, true>}},        \
-   {EX::Cfg<NT, MR, WR, false>::kStageBytes, EX::Cfg<NT, MR, WR, true>::kStageBytes},                            \
-   EX::Cfg<NT, MR, WR, false>::kSumBytes,                                                                        \
-   EX::Cfg<NT, MR, WR, false>::kRows},
-    ARC_EXPERT_VARIANTS(ARC_EXPERT_ENTRY)
-#undef ARC_EXPERT_ENTRY
+template <uint32_t NT, uint32_t MR, uint32_t WR, bool INT4, bool SECOND>
+constexpr ExpertVariant expert_variant() {
+  using C = EX::Cfg<NT, MR, WR, INT4>;
+  return {EX::expert_layer_kernel<NT, MR, WR, INT4, SECOND>, C::kRows, C::kParts, C::kStageBytes, C::kWBytes, C::kSumBytes};
+}
+struct ExpertForm {
+  bool int4;
+  uint32_t columns;
+  ExpertVariant first, second;
+};
+constexpr ExpertForm kExpertForms[] = {
+    {false, 8, expert_variant<8, 2, 2, false, false>(), expert_variant<8, 2, 2, false, true>()},
+    {false, 16, expert_variant<16, 2, 4, false, false>(), expert_variant<16, 2, 4, false, true>()},
+    {false, 32, expert_variant<32, 2, 4, false, false>(), expert_variant<32, 2, 2, false, true>()},
+    {true, 8, expert_variant<8, 4, 2, true, false>(), expert_variant<8, 4, 2, true, true>()},
+    {true, 16, expert_variant<16, 2, 4, true, false>(), expert_variant<16, 2, 2, true, true>()},
 };
 
 // Dynamic shared memory of a block: what the system and the kernel's own barriers take is off.
 constexpr uint32_t kExpertSmemHalf = 112 * 1024, kExpertSmemWhole = 226 * 1024;
 
 int experts_init() {
-  for (const ExpertVariant& v : kExpertVariants) {
-    for (int i = 0; i < 4; ++i) {
-      const cudaError_t e = allow_smem(v.kernel[i >> 1][i & 1], kExpertSmemWhole);
+  for (const ExpertForm& f : kExpertForms) {
+    for (const ExpertVariant* v : {&f.first, &f.second}) {
+      const cudaError_t e = allow_smem(v->kernel, kExpertSmemWhole);
       if (e != cudaSuccess) {
         cudaGetLastError();  // clear
         return cuda_fail(e, "cudaFuncSetAttribute (expert layer)");
@@ -49,41 +52,66 @@ int experts_init() {
   return ARC_OK;
 }
 
+// How a call runs: columns of a pass, blocks of a cluster of the second launch (0: as many as fit), and whether the
+// rows of x are put in the sorted order first.
 struct ExpertPlan {
-  const ExpertVariant* v;
+  const ExpertForm* form;
+  uint32_t splits;
+  bool sorted;
+};
+
+// An expert's choices fill a pass on average half: they are uneven, and a second pass reads the weights again, while
+// columns that stay empty cost shared memory. int4 weights stop at 16: the registers of 32 do not fit. Sorted rows
+// pay from 8 choices an expert (8 experts of 4096 x 7168, two a token, 32 tokens: 240 us with gathers, 224 sorted;
+// 64 experts of 4096 x 2048, 16 tokens of two choices an expert: 338 and 339).
+//
+// ARC_EXPERT_PLAN="columns:S:sorted" (tests and tuning) forces them.
+int expert_plan(bool int4, uint32_t tokens, uint32_t slots, uint32_t experts, ExpertPlan* plan) {
+  const uint32_t live = experts < slots ? experts : slots;
+  uint32_t want = 2 * ceil_div(slots, live);
+  if (want > tokens) want = tokens;
+  uint32_t columns = want <= 8 ? 8 : want <= 16 || int4 ? 16 : 32, sorted = slots >= 8 * experts ? 1 : 0;
+  plan->splits = 0;
+  if (const char* env = getenv("ARC_EXPERT_PLAN")) {
+    uint32_t s = 0;
+    if (sscanf(env, "%u:%u:%u", &columns, &s, &sorted) != 3 || (s != 1 && s != 2 && s != 4 && s != 8) || sorted > 1) {
+      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_EXPERT_PLAN must be 'columns:S:sorted' (got '%s')", env);
+    }
+    plan->splits = s;
+  }
+  plan->sorted = sorted != 0;
+  for (const ExpertForm& f : kExpertForms) {
+    plan->form = &f;
+    if (f.int4 == int4 && f.columns == columns) return ARC_OK;
+  }
+  return fail(ARC_ERR_INVALID_ARGUMENT, "the expert layer has no form of %u columns", columns);
+}
+
+// The ring of a launch: as many stages as half an SM holds if that keeps 32 KB of weights in flight, else as many as
+// a whole one does. In the second launch every part of the contraction has its own sums of y where they take 32 KB
+// at most.
+struct ExpertRing {
   uint32_t stages, smem, blocks_per_sm;
   bool own_y;
 };
-
-const ExpertVariant* expert_variant(uint32_t nt, uint32_t mr, uint32_t wr) {
-  for (const ExpertVariant& v : kExpertVariants) {
-    if (v.nt == nt && v.mr == mr && v.wr == wr) return &v;
-  }
-  return nullptr;
-}
-
-// The ring of a launch: as many stages as half an SM holds if that keeps 48 KB of weights in flight, else
-// as many as a whole one does.
-void expert_ring(const ExpertVariant& v, bool int4, bool second, uint32_t tokens, uint32_t slots, uint32_t experts,
-                 ExpertPlan* plan) {
-  const uint32_t parts = EX::kConsumers / v.wr;
-  const uint32_t stage = v.stage_bytes[int4 ? 1 : 0];
-  plan->v = &v;
-  plan->own_y = second && parts * v.rows * tokens * 4 <= 32 * 1024;
+int expert_ring(const char* what, const ExpertVariant& v, bool second, uint32_t columns, uint32_t tokens, uint32_t slots,
+                uint32_t experts, ExpertRing* ring) {
+  ring->own_y = second && v.parts * v.rows * tokens * 4 <= 32 * 1024;
   const uint32_t rest =
-      EX::layout_of(v.sum_bytes, parts, v.rows, v.nt, tokens, slots, experts, second, plan->own_y).total + 1024;
-  const uint32_t unit = parts < 4 ? 4 : parts;  // a whole number of parts and of batches
+      EX::layout_of(v.sum_bytes, v.parts, v.rows, columns, tokens, slots, experts, second, ring->own_y).total + 1024;
+  const uint32_t unit = v.parts < 4 ? 4 : v.parts;  // a whole number of parts and of batches
   const auto stages = [&](uint32_t budget) {
-    const uint32_t n = budget > rest ? (budget - rest) / stage : 0;
+    const uint32_t n = budget > rest ? (budget - rest) / v.stage_bytes : 0;
     return (n < EX::kMaxStages ? n : EX::kMaxStages) / unit * unit;
   };
-  plan->blocks_per_sm = 2;
-  plan->stages = stages(kExpertSmemHalf);
-  if (plan->stages * v.rows * EX::kRowBytes < 32 * 1024) {
-    plan->blocks_per_sm = 1;
-    plan->stages = stages(kExpertSmemWhole);
+  ring->blocks_per_sm = 2;
+  ring->stages = stages(kExpertSmemHalf);
+  if (ring->stages * v.weight_bytes < 32 * 1024) {
+    ring->blocks_per_sm = 1;
+    ring->stages = stages(kExpertSmemWhole);
   }
-  plan->smem = rest + plan->stages * stage;
+  ring->smem = rest + ring->stages * v.stage_bytes;
+  return ring->stages > 0 ? ARC_OK : fail(ARC_ERR_UNSUPPORTED, "%s: does not fit in shared memory", what);
 }
 
 // Weights of E experts as {bytes or elements of a row, rows, 2 (gate and up) or 1, E}.
@@ -93,38 +121,36 @@ int encode_expert_weights(CUtensorMap* map, const void* w, bool int4, uint64_t i
   if (fn == nullptr) return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled is unavailable");
   const cuuint64_t dims[4] = {inner, cols, gated ? 2u : 1u, experts};
   const cuuint64_t strides[3] = {ld_bytes, ld_bytes * cols, experts > 1 ? stride_bytes : ld_bytes * cols};
-  const cuuint32_t box[4] = {int4 ? EX::kRowBytes : EX::kRowBytes / 2, gated ? rows / 2 : rows, gated ? 2u : 1u, 1};
+  const cuuint32_t box[4] = {64, gated ? rows / 2 : rows, gated ? 2u : 1u, 1};
   const cuuint32_t estr[4] = {1, 1, 1, 1};
   const CUresult r = fn(map, int4 ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 4,
                         const_cast<void*>(w), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                        CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                        int4 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_128B,
+                        CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
   if (r != CUDA_SUCCESS) {
     return fail(ARC_ERR_CUDA, "cuTensorMapEncodeTiled(expert weights) failed with CUresult %d", static_cast<int>(r));
   }
   return ARC_OK;
 }
 
-// Columns of a pass: those that an expert's choices fill on average, doubled, since they are uneven.
-uint32_t expert_columns(uint32_t tokens, uint32_t slots, uint32_t experts) {
-  const uint32_t live = experts < slots ? experts : slots;
-  uint32_t want = 2 * ceil_div(slots, live);
-  if (want > tokens) want = tokens;
-  return want <= 8 ? 8 : want <= 16 ? 16 : 32;
+// h, and the sorted rows of x, lie in the workspace with rows that TMA can read.
+uint64_t expert_ld(uint32_t inner) { return (uint64_t(inner) + 7) / 8 * 8; }
+size_t expert_workspace(size_t slots, uint32_t inner_in, uint32_t inner_out, bool sorted) {
+  return slots * 2 * (expert_ld(inner_out) + (sorted ? expert_ld(inner_in) : 0));
 }
-
-// h lies in the workspace with rows that TMA can read.
-uint64_t expert_ldh(uint32_t inner) { return (uint64_t(inner) + 7) / 8 * 8; }
 
 }  // namespace
 
 extern "C" {
 
-int arc_moe_workspace_bytes(int T, int top, int I, size_t* bytes) {
-  if (bytes == nullptr || T <= 0 || top <= 0 || I <= 0) {
+int arc_moe_workspace_bytes(int T, int top, int E, int K, int I, size_t* bytes) {
+  if (bytes == nullptr || T <= 0 || top <= 0 || E <= 0 || K <= 0 || I <= 0 ||
+      T > ARC_MOE_MAX_TOKENS || int64_t(T) * top > ARC_MOE_MAX_CHOICES) {
     return fail(ARC_ERR_INVALID_ARGUMENT, "arc_moe_workspace_bytes: bad argument");
   }
-  *bytes = size_t(T) * top * expert_ldh(I) * 2;
+  ExpertPlan plan;
+  if (int st = expert_plan(false, T, static_cast<uint32_t>(T) * top, E, &plan)) return st;
+  *bytes = expert_workspace(size_t(T) * top, K, I, plan.sorted);
   return ARC_OK;
 }
 
@@ -185,8 +211,10 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
     return fail(ARC_ERR_UNSUPPORTED, "%s: ids or weights are misaligned", what);
   }
   const uint32_t slots = static_cast<uint32_t>(T) * top;
-  const uint64_t ldh = expert_ldh(I);
-  const size_t need = size_t(slots) * ldh * 2;
+  const uint64_t ldh = expert_ld(I);
+  ExpertPlan plan;
+  if (int st = expert_plan(int4, T, slots, E, &plan)) return st;
+  const size_t need = expert_workspace(slots, K, I, plan.sorted);
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need) {
     return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
   }
@@ -194,19 +222,11 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   if (int st = current_device(&dev, &DeviceState::experts_status)) return st;
   const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
 
-  uint32_t nt = expert_columns(T, slots, E), mr1 = int4 && nt < 32 ? 4 : 2, mr2 = mr1, splits = 0, per_sm = 2;
-  uint32_t wr1 = nt == 8 ? 2 : 4 * 2 / mr1, wr2 = 2;
-  if (const char* env = getenv("ARC_EXPERT_PLAN")) {
-    if (sscanf(env, "%u:%u:%u:%u:%u:%u:%u", &nt, &mr1, &wr1, &mr2, &wr2, &splits, &per_sm) < 5 ||
-        expert_variant(nt, mr1, wr1) == nullptr || expert_variant(nt, mr2, wr2) == nullptr ||
-        (splits & (splits - 1)) != 0 || splits > 8) {
-      return fail(ARC_ERR_INVALID_ARGUMENT, "ARC_EXPERT_PLAN must be 'NT:MR:WR:MR:WR[:S]' (got '%s')", env);
-    }
-  }
-  ExpertPlan first, second;
-  expert_ring(*expert_variant(nt, mr1, wr1), int4, false, T, slots, E, &first);
-  expert_ring(*expert_variant(nt, mr2, wr2), int4, true, T, slots, E, &second);
-  if (first.stages == 0 || second.stages == 0) return fail(ARC_ERR_UNSUPPORTED, "%s: does not fit in shared memory", what);
+  const ExpertVariant &v1 = plan.form->first, &v2 = plan.form->second;
+  const uint32_t columns = plan.form->columns;
+  ExpertRing first, second;
+  if (int st = expert_ring(what, v1, false, columns, T, slots, E, &first)) return st;
+  if (int st = expert_ring(what, v2, true, columns, T, slots, E, &second)) return st;
 
   EX::Params p = {};
   p.ids = ids;
@@ -215,41 +235,56 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   p.weights_bf16 = weight_bytes == 2;
   p.tokens = T;
   p.top = top;
+  p.sorted = plan.sorted ? 1 : 0;
   p.top_inverse = top == 1 ? 0 : static_cast<uint32_t>(((1ull << 32) + top - 1) / top);
   p.experts = E;
   p.slots = slots;
   const uint32_t elem = int4 ? 1 : 2;
 
   // FIRST: h [slots][I].
-  const uint32_t box_k = int4 ? 2 * EX::kRowBytes : EX::kRowBytes / 2;
-  if (int st = encode_expert_weights(&p.tm_w, w_in, int4, int4 ? K / 2 : K, I, gated, E, ld_in * elem, stride_in * elem, first.v->rows)) {
+  const uint32_t box_k = int4 ? group : 64;
+  if (int st = encode_expert_weights(&p.tm_w, w_in, int4, int4 ? K / 2 : K, I, gated, E, ld_in * elem, stride_in * elem, v1.rows)) {
     return st;
   }
-  if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, K, T, ldx, 64, 1, CU_TENSOR_MAP_SWIZZLE_128B, "x")) {
+  cudaError_t e;
+  if (p.sorted) {
+    uint16_t* xs = static_cast<uint16_t*>(workspace) + slots * ldh;
+    const uint64_t ldxs = expert_ld(K);
+    const uint32_t smem = EX::layout_of(0, 1, 0, columns, T, slots, E, false, true).total + 2 * E;
+    e = launch_grid(columns == 8    ? EX::expert_rows_kernel<8>
+                    : columns == 16 ? EX::expert_rows_kernel<16>
+                                    : EX::expert_rows_kernel<32>,
+                    dim3(slots < sms ? slots : sms), EX::kThreads, smem, stream, p, xs, ldxs, x, ldx, uint32_t(K));
+    if (e != cudaSuccess) return cuda_fail(e, "expert_rows_kernel launch");
+    if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, xs, K, slots, ldxs, 64, 8,
+                           CU_TENSOR_MAP_SWIZZLE_128B, "sorted x")) {
+      return st;
+    }
+  } else if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, K, T, ldx, 64, 1,
+                                CU_TENSOR_MAP_SWIZZLE_128B, "x")) {
     return st;
   }
   p.sb = s_in;
   p.out = static_cast<uint16_t*>(workspace);
   p.ldo = ldh;
   p.cols = I;
-  p.tiles = ceil_div(I, gated ? first.v->rows / 2 : first.v->rows);
+  p.tiles = ceil_div(I, gated ? v1.rows / 2 : v1.rows);
   p.num_kb = ceil_div(K, box_k);
   p.groups = K / group;
   p.gated = gated ? 1 : 0;
   p.act = activation;
   p.stages = first.stages;
   p.splits = 1;
-  const uint64_t items = uint64_t((uint32_t(E) < slots ? E : slots) + slots / nt) * p.tiles;
-  const uint64_t most = uint64_t(sms) * (first.blocks_per_sm < per_sm ? first.blocks_per_sm : per_sm);
-  cudaError_t e = launch_ex(first.v->kernel[int4][0], p, static_cast<uint32_t>(items < most ? items : most), EX::kThreads,
-                            first.smem, 1, stream);
+  const uint64_t items = uint64_t((uint32_t(E) < slots ? E : slots) + slots / columns) * p.tiles;
+  const uint64_t most = uint64_t(sms) * first.blocks_per_sm;
+  e = launch_ex(v1.kernel, p, static_cast<uint32_t>(items < most ? items : most), EX::kThreads, first.smem, 1, stream);
   if (e != cudaSuccess) return cuda_fail(e, "expert_layer_kernel launch");
 
   // SECOND: y [T][N].
-  if (int st = encode_expert_weights(&p.tm_w, w_out, int4, int4 ? I / 2 : I, N, false, E, ld_out * elem, stride_out * elem, second.v->rows)) {
+  if (int st = encode_expert_weights(&p.tm_w, w_out, int4, int4 ? I / 2 : I, N, false, E, ld_out * elem, stride_out * elem, v2.rows)) {
     return st;
   }
-  if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, workspace, I, slots, ldh, 64, 1,
+  if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, workspace, I, slots, ldh, 64, 8,
                          CU_TENSOR_MAP_SWIZZLE_128B, "h")) {
     return st;
   }
@@ -257,19 +292,21 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   p.out = out;
   p.ldo = ldo;
   p.cols = N;
-  p.tiles = ceil_div(N, second.v->rows);
+  p.tiles = ceil_div(N, v2.rows);
   p.num_kb = ceil_div(I, box_k);
   p.groups = I / group;
   p.gated = 0;
   p.act = ARC_ACT_NONE;
   p.stages = second.stages;
+  // The cluster shares a tile's boxes until both block slots of every SM have work.
+  uint32_t splits = plan.splits;
   if (splits == 0) {
     splits = 1;
     while (splits < 8 && p.tiles * splits * 2 <= sms * second.blocks_per_sm) splits *= 2;
   }
   p.splits = splits;
   p.own_y = second.own_y ? 1 : 0;
-  e = launch_ex(second.v->kernel[int4][1], p, p.tiles * splits, EX::kThreads, second.smem, splits, stream);
+  e = launch_ex(v2.kernel, p, p.tiles * splits, EX::kThreads, second.smem, splits, stream);
   if (e != cudaSuccess) return cuda_fail(e, "expert_layer_kernel launch");
   return ARC_OK;
 }

@@ -10,7 +10,9 @@
 //
 // * No sorting launch, no gathered copies. Every block sorts the choices in shared memory by itself (a
 //   microsecond, in SECOND under the first launch), and the rows of x and h that belong to an expert
-//   come by TMA gather, four rows an instruction.
+//   come by TMA gather, four rows an instruction. Where experts have many rows gathers hold the stream up (128
+//   tokens, 64 experts of 2048 x 4096: loads alone 711 us, 508 without the rows), so h lies in the sorted order,
+//   eight rows a load, and a small launch in front puts the rows of x there as well.
 // * Blocks walk over (expert, column tile) and their ring of loads runs on from one to the next, so the
 //   stream of weights pauses only at a launch's ends. SECOND loads its first weights under FIRST's last tiles.
 // * A tile is 32 WR weight rows; the eight warps are WR groups of rows times WK = 8 / WR parts of the
@@ -25,8 +27,9 @@
 //   its blocks' sums in rank order. The result does not depend on timing.
 //
 // Sums are fp32. h is rounded to bf16, the tensor cores' operand type, and the weights of the choices multiply
-// fp32 sums. Codes of int4 weights are exact bf16; a group of 128 products is summed before its scale is
-// applied in fp32.
+// fp32 sums. Codes of int4 weights enter as code + 136, which is what a nibble costs fewest instructions as, and
+// 136 times the group's sum of x, which the tensor cores give beside it, is taken off in fp32 before the scale: at
+// most 2^-14 of the group's largest |x| goes to the tensor cores' fp32 sums that way, where 2^-8 of h is rounded.
 #pragma once
 
 #include "linear_common.cuh"
@@ -36,18 +39,18 @@ namespace experts {
 
 constexpr uint32_t kConsumers = 8;  // warps
 constexpr uint32_t kThreads = 32 * (kConsumers + 1);
-constexpr uint32_t kRowBytes = 128;  // of a box: 64 bf16 or 256 codes
+constexpr uint32_t kRowBytes = 128;  // of a box of 64 bf16; one of 128 codes, a scale group, has 64
 constexpr uint32_t kScaleGroup = 128;
-constexpr uint32_t kMaxStages = 24;
+constexpr uint32_t kMaxStages = 32;
 constexpr uint16_t kNoExpert = 0xFFFFu;
 
 struct Params {
   CUtensorMap tm_w;  // {K, columns, 2 or 1, E}, box {128 bytes, 16 WR, 2, 1} with a gate, else {.., 32 WR, 1, 1}; SW128
-  CUtensorMap tm_x;  // {K, rows}, box {64, 1}, SW128
+  CUtensorMap tm_x;  // {K, rows}, SW128, box {64, 8}, of rows in the sorted order; else, of tokens, {64, 1}
   const uint16_t* sb;   // int4: scales [E][weight rows][groups]
   const void* ids;      // [tokens][top]
   const void* weights;  // SECOND: [tokens][top], fp32 or bf16
-  uint16_t* out;        // FIRST: h [slots][ldo]; SECOND: y [tokens][ldo]
+  uint16_t* out;        // FIRST: h [slots][ldo], sorted by expert; SECOND: y [tokens][ldo]
   uint64_t ldo;
   uint32_t ids_wide, weights_bf16;  // int64 ids; bf16 weights
   uint32_t tokens, top, experts, slots;
@@ -56,6 +59,7 @@ struct Params {
   uint32_t num_kb;       // boxes along the contraction
   uint32_t groups;       // scale groups along it
   uint32_t gated, act;
+  uint32_t sorted;       // FIRST: rows of x lie in the order of the sorted choices
   uint32_t stages;       // of the ring, a multiple of WK
   uint32_t splits;       // SECOND: blocks of a cluster, which share the passes' boxes
   uint32_t own_y;        // SECOND: see Layout
@@ -69,8 +73,9 @@ struct Cfg {
   static constexpr uint32_t kParts = kConsumers / WR;  // WK
   static_assert(kParts >= 2, "parts of the contraction");
   static constexpr uint32_t kRows = 16 * MR * WR;
-  static constexpr uint32_t kSub = INT4 ? 4 : 1;  // boxes of tokens per box of weights
-  static constexpr uint32_t kWBytes = kRows * kRowBytes;
+  static constexpr uint32_t kSub = INT4 ? 2 : 1;  // boxes of tokens per box of weights
+  static constexpr uint32_t kWRow = INT4 ? 64 : kRowBytes;
+  static constexpr uint32_t kWBytes = kRows * kWRow;
   static constexpr uint32_t kXBytes = NT * kRowBytes;  // a box of tokens
   static constexpr uint32_t kStageBytes = kWBytes + kSub * kXBytes;
   static constexpr uint32_t kSumBytes = kParts * kRows * NT * 4;
@@ -119,7 +124,7 @@ __device__ __forceinline__ void lds_128(uint32_t addr, uint32_t (&r)[4]) {
 }
 __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                          uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -128,7 +133,7 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
 // Four rows of a matrix, 128 bytes each from column x on; a row outside it comes as zeros.
 __device__ __forceinline__ void tma_gather4(const CUtensorMap* map, uint64_t* bar, void* dst, int32_t x, int32_t r0,
                                             int32_t r1, int32_t r2, int32_t r3, uint64_t cache_hint) {
-  asm volatile(
+  asm(
       "cp.async.bulk.tensor.2d.shared::cta.global.tile::gather4.mbarrier::complete_tx::bytes.L2::cache_hint "
       "[%0], [%1, {%3, %4, %5, %6, %7}], [%2], %8;" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(r0), "r"(r1), "r"(r2), "r"(r3),
@@ -137,23 +142,33 @@ __device__ __forceinline__ void tma_gather4(const CUtensorMap* map, uint64_t* ba
 }
 __device__ __forceinline__ void tma_load_4d(const CUtensorMap* map, uint64_t* bar, void* dst, int32_t x, int32_t y,
                                             int32_t z, int32_t w, uint64_t cache_hint) {
-  asm volatile(
+  asm(
       "cp.async.bulk.tensor.4d.shared::cta.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint "
       "[%0], [%1, {%3, %4, %5, %6}], [%2], %7;" ::"r"(smem_u32(dst)),
       "l"(reinterpret_cast<uint64_t>(map)), "r"(smem_u32(bar)), "r"(x), "r"(y), "r"(z), "r"(w), "l"(cache_hint)
       : "memory");
 }
 
-// Eight int4 codes (k = 0..7 from the low nibble up) as bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7). 0x4300 | m is
-// the bf16 128 + m; a code's nibble with its sign bit turned over is code + 8, so 136 is taken off again, exactly.
+// The same with sums that start from zero.
+__device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
+                                               uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %10, %10, %10};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
+}
+
+// Eight int4 codes (k = 0..7 from the low nibble up) as bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7) of code + 136:
+// 0x4300 | m is the bf16 128 + m, and a code's nibble with its sign bit turned over is code + 8.
 __device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t (&v)[4]) {
 #pragma unroll
   for (uint32_t i = 0; i < 4; ++i) {
-    uint32_t m;
-    asm("lop3.b32 %0, %1, 0x000F000F, 0x43084308, 0x6A;" : "=r"(m) : "r"(w >> (4 * i)));  // (a & b) ^ c
-    asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(v[i]) : "r"(m), "r"(0x43084308u));
+    asm("lop3.b32 %0, %1, 0x000F000F, 0x43084308, 0x6A;" : "=r"(v[i]) : "r"(w >> (4 * i)));  // (a & b) ^ c
   }
 }
+constexpr float kCodeBias = 136.f;
+constexpr uint32_t kOnes = 0x3F803F80u;  // two bf16 ones
 
 // ---------------------------------------------------------------------------------
 // The choices, sorted by expert in shared memory by the whole block: `list` holds the choices of
@@ -255,6 +270,118 @@ __device__ __forceinline__ float share_of(const Params& p, uint32_t s) {
   return sum;
 }
 
+// One warp's share of a box of weights times the J tiles of eight columns of its rows of x.
+template <uint32_t MR, uint32_t WR, uint32_t XBYTES, bool INT4, uint32_t J, uint32_t N>
+__device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_at, uint32_t x_at,
+                                             const uint32_t (&sc)[MR / 2], uint32_t wr, uint32_t lane) {
+  if constexpr (!INT4) {
+#pragma unroll
+    for (uint32_t half = 0; half < 2; ++half) {  // 32 of the contraction
+      uint32_t b[J][4];
+#pragma unroll
+      for (uint32_t j = 0; j < J; ++j) {
+        const uint32_t row = lane & 7u, chunk = half * 4u + (lane >> 3);
+        ldmatrix_x4(x_at + (j * 8u + row) * kRowBytes + ((chunk ^ row) << 4), b[j]);
+      }
+#pragma unroll
+      for (uint32_t m = 0; m < MR; ++m) {
+#pragma unroll
+        for (uint32_t k = 0; k < 2; ++k) {
+          uint32_t a[4];
+          const uint32_t row = (m * WR + wr) * 16u + (lane & 15u), chunk = half * 4u + k * 2u + (lane >> 4);
+          ldmatrix_x4(w_at + row * kRowBytes + ((chunk ^ (row & 7u)) << 4), a);
+#pragma unroll
+          for (uint32_t j = 0; j < J; ++j) mma_bf16(acc[m][j], a[0], a[1], a[2], a[3], b[j][2 * k], b[j][2 * k + 1]);
+        }
+      }
+    }
+  } else {
+    const uint32_t g8 = lane >> 2, q = lane & 3u;
+    // A lane's codes are k = 8 q .. 8 q + 7 of 32, so it takes the same of x, 16 bytes of a row. Lanes of a quarter warp
+    // take the rows r and r + 4, whose halves of 128 swizzled bytes lie in different banks; so column n of a
+    // product is row perm(n).
+    const uint32_t perm = (g8 >> 1) | (g8 & 1u) << 2;
+    float part_sum[MR][J][4], x_sum[J][4];  // over the group: of (code + 136) x, and of x
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) {  // 32 codes of a row, 16 bytes
+      uint32_t b[J][4];  // pairs of k: (0, 4), (1, 5), (2, 6), (3, 7) of a lane's eight, as the codes come
+#pragma unroll
+      for (uint32_t j = 0; j < J; ++j) {
+        uint32_t x[4];
+        lds_128(x_at + (c >> 1) * XBYTES + (j * 8u + perm) * kRowBytes + ((((c & 1u) * 4u + q) ^ perm) << 4), x);
+        b[j][0] = __byte_perm(x[0], x[2], 0x5410);
+        b[j][1] = __byte_perm(x[0], x[2], 0x7632);
+        b[j][2] = __byte_perm(x[1], x[3], 0x5410);
+        b[j][3] = __byte_perm(x[1], x[3], 0x7632);
+        if (c == 0) {
+          mma_bf16_first(x_sum[j], kOnes, kOnes, kOnes, kOnes, b[j][0], b[j][1]);
+        } else {
+          mma_bf16(x_sum[j], kOnes, kOnes, kOnes, kOnes, b[j][0], b[j][1]);
+        }
+        mma_bf16(x_sum[j], kOnes, kOnes, kOnes, kOnes, b[j][2], b[j][3]);
+      }
+#pragma unroll
+      for (uint32_t m2 = 0; m2 < MR; m2 += 2) {
+        uint32_t a[4];  // rows 0-7 and 8-15 of two blocks of rows
+        const uint32_t row = ((m2 + (lane >> 4)) * WR + wr) * 16u + (lane & 15u);
+        ldmatrix_x4(w_at + row * 64u + ((c ^ ((row >> 1) & 3u)) << 4), a);
+#pragma unroll
+        for (uint32_t m = 0; m < 2; ++m) {
+          uint32_t lo[4], hi[4];
+          codes_to_bf16(a[2 * m], lo);
+          codes_to_bf16(a[2 * m + 1], hi);
+#pragma unroll
+          for (uint32_t j = 0; j < J; ++j) {
+            if (c == 0) {
+              mma_bf16_first(part_sum[m2 + m][j], lo[0], hi[0], lo[1], hi[1], b[j][0], b[j][1]);
+            } else {
+              mma_bf16(part_sum[m2 + m][j], lo[0], hi[0], lo[1], hi[1], b[j][0], b[j][1]);
+            }
+            mma_bf16(part_sum[m2 + m][j], lo[2], hi[2], lo[3], hi[3], b[j][2], b[j][3]);
+          }
+        }
+      }
+    }
+#pragma unroll
+    for (uint32_t m = 0; m < MR; ++m) {
+      const float s0 = __uint_as_float(__shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + g8) << 16);
+      const float s1 = __uint_as_float(__shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + 8u + g8) << 16);
+#pragma unroll
+      for (uint32_t j = 0; j < J; ++j) {
+#pragma unroll
+        for (uint32_t i = 0; i < 4; ++i) {
+          const float v = fmaf(-kCodeBias, x_sum[j][i & 1u], part_sum[m][j][i]);
+          acc[m][j][i] = fmaf(i < 2 ? s0 : s1, v, acc[m][j][i]);
+        }
+      }
+    }
+  }
+}
+
+// The rows of x in the order of the sorted choices, for batches whose experts have many: xs [choices][ldxs].
+template <uint32_t NT>
+__global__ void __launch_bounds__(kThreads) expert_rows_kernel(const __grid_constant__ Params p, uint16_t* xs, uint64_t ldxs,
+                                                               const uint16_t* x, uint64_t ldx, uint32_t inner) {
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ uint32_t num_passes;
+  const Layout l = layout_of(0, 1, 0, NT, p.tokens, p.slots, p.experts, false, true);
+  Pass* passes = reinterpret_cast<Pass*>(smem_raw + l.passes);
+  uint16_t* list = reinterpret_cast<uint16_t*>(smem_raw + l.list);
+  pdl_wait();
+  pdl_launch_dependents();
+  const uint32_t n = sort_choices<NT>(p, passes, list, reinterpret_cast<uint16_t*>(smem_raw + l.ids),
+                                      reinterpret_cast<uint16_t*>(smem_raw + l.total), &num_passes);
+  const uint32_t listed = n == 0u ? 0u : passes[n - 1u].first + passes[n - 1u].count;
+  for (uint32_t i = blockIdx.x; i < listed; i += gridDim.x) {
+    const uint16_t* from = x + token_of(p, list[i]) * ldx;
+    uint16_t* to = xs + i * ldxs;
+    for (uint32_t v = threadIdx.x; v < inner / 8u; v += kThreads) {
+      reinterpret_cast<uint4*>(to)[v] = __ldg(reinterpret_cast<const uint4*>(from) + v);
+    }
+    for (uint32_t k = inner / 8u * 8u + threadIdx.x; k < inner; k += kThreads) to[k] = __ldg(from + k);
+  }
+}
+
 template <uint32_t NT, uint32_t MR, uint32_t WR, bool INT4, bool SECOND>
 __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_constant__ Params p) {
   using C = Cfg<NT, MR, WR, INT4>;
@@ -287,9 +414,10 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
     abort_flag = 0;
     fence_barrier_init();
   }
-  // The choices and their weights are older than the first launch, which has waited for them before it
-  // lets the second one in.
-  if (!SECOND) {
+  // A launch of this layer in front of this one has waited for the choices and their weights before it let
+  // this one in: they and the layer's weights can be read at once, its results (`tm_x`'s) after the wait.
+  const bool early = SECOND || p.sorted != 0u;
+  if (!early) {
     pdl_wait();
     pdl_launch_dependents();
   }
@@ -344,13 +472,14 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
       f0 = (SECOND ? my_tile : item - pi * p.tiles) * tile_cols;
     };
     const auto load_weights = [&](uint32_t st) {
-      mbar_arrive_expect_tx(&full[st], C::kWBytes + C::kSub * ((ps.count + 3u) / 4u) * 4u * kRowBytes);
-      tma_load_4d(&p.tm_w, &full[st], ring + st * C::kStageBytes, int32_t(kb * (INT4 ? kRowBytes : kRowBytes / 2u)),
+      const uint32_t rows = early ? (ps.count + 7u) & ~7u : (ps.count + 3u) & ~3u;
+      mbar_arrive_expect_tx(&full[st], C::kWBytes + C::kSub * rows * kRowBytes);
+      tma_load_4d(&p.tm_w, &full[st], ring + st * C::kStageBytes, int32_t(kb * 64u),
                   int32_t(f0), 0, ps.expert, kCacheEvictNormal);
     };
     uint32_t ahead = 0;  // boxes whose weights are on their way
-    if (SECOND) {
-      // The first weights do not wait for the first launch.
+    if (early) {
+      // The first weights do not wait for the launch in front.
       ahead = min(p.stages, boxes);
       if (lane < kBatch) {
         for (uint32_t b = lane; b < ahead; b += kBatch) {
@@ -376,7 +505,7 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
         }
       }
       const uint32_t going = __ballot_sync(0xffffffffu, go);
-      // Rows of all boxes that go, four a gather.
+      // Rows of all boxes that go: eight a load where they lie in the order of `list`, else four a gather.
       constexpr uint32_t kQuads = NT / 4u, kPerBox = kQuads * C::kSub;
 #pragma unroll
       for (uint32_t g0 = 0; g0 < kBatch * kPerBox; g0 += 32u) {
@@ -387,16 +516,19 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
         const uint32_t k = __shfl_sync(0xffffffffu, kb, from);
         const uint32_t st = __shfl_sync(0xffffffffu, stage, from);
         if (box < kBatch && ((going >> box) & 1u) != 0u && quad * 4u < count) {
-          int32_t r[4];
+          uint8_t* to = ring + st * C::kStageBytes + C::kWBytes + sub * C::kXBytes + quad * 4u * kRowBytes;
+          const int32_t x = int32_t((k * C::kSub + sub) * 64u);
+          if (early) {
+            if ((quad & 1u) == 0u) tma_load_2d(&p.tm_x, &full[st], to, x, int32_t(first + quad * 4u), kCacheEvictLast);
+          } else {
+            int32_t r[4];
 #pragma unroll
-          for (uint32_t i = 0; i < 4; ++i) {
-            const uint32_t c = quad * 4u + i;
-            const uint32_t s = list[first + min(c, count - 1u)];
-            r[i] = int32_t(SECOND ? (c < count ? s : p.slots) : (c < count ? token_of(p, s) : p.tokens));
+            for (uint32_t i = 0; i < 4; ++i) {
+              const uint32_t c = quad * 4u + i;
+              r[i] = int32_t(c < count ? token_of(p, list[first + c]) : p.tokens);
+            }
+            tma_gather4(&p.tm_x, &full[st], to, x, r[0], r[1], r[2], r[3], kCacheEvictLast);
           }
-          tma_gather4(&p.tm_x, &full[st],
-                      ring + st * C::kStageBytes + C::kWBytes + sub * C::kXBytes + quad * 4u * kRowBytes,
-                      int32_t((k * C::kSub + sub) * 64u), r[0], r[1], r[2], r[3], kCacheEvictLast);
         }
       }
       if (go) {
@@ -421,18 +553,15 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
     __syncwarp();
   } else {
     // ------------------------------------------------------------ consumers
-    if (SECOND) pdl_wait();
+    if (early) pdl_wait();
     const uint32_t wr = warp % WR, part = warp / WR;
     const uint32_t g8 = lane >> 2, q = lane & 3u;
-    // Lanes of a quarter warp take the rows r and r + 4, whose halves of 128 swizzled bytes lie in different
-    // banks: a 16-byte read of four lanes a row meets no conflict. So column n of a product is row perm(n).
-    const uint32_t perm = (g8 >> 1) | (g8 & 1u) << 2;
     uint32_t stage = part, phase = 0;             // of this part's next box
     uint32_t box = part;                          // its running number
     uint32_t item = item0, kb = kb_first + part;  // and where it lies
     bool ok = true;
 
-    // int4: the scales of a box, two groups a weight row, on their way a box ahead. Lane l has row l (and l + 32) of
+    // int4: the scales of a box, one a weight row, on their way a box ahead. Lane l has row l (and l + 32) of
     // this warp's rows.
     constexpr uint32_t kScaleRegs = MR / 2;
     uint32_t scales[kScaleRegs];
@@ -441,22 +570,13 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
         const uint32_t pi = SECOND ? item : item / p.tiles;
         const uint32_t f0 = (SECOND ? my_tile : item - pi * p.tiles) * tile_cols;
         const uint32_t rows = p.gated ? 2u * p.cols : p.cols;
-        const uint32_t g0 = kb * 2u;
 #pragma unroll
         for (uint32_t i = 0; i < kScaleRegs; ++i) {
           const uint32_t m = i * 2u + (lane >> 4);
           const bool up = p.gated && m >= MR / 2;
           const uint32_t f = f0 + ((up ? m - MR / 2 : m) * WR + wr) * 16u + (lane & 15u);
           uint32_t bits = 0;
-          if (f < p.cols) {
-            const uint16_t* at = p.sb + (size_t(passes[pi].expert) * rows + f + (up ? p.cols : 0u)) * p.groups + g0;
-            if ((p.groups & 1u) == 0u && (reinterpret_cast<uintptr_t>(p.sb) & 3u) == 0u) {
-              bits = __ldg(reinterpret_cast<const uint32_t*>(at));
-            } else {
-              bits = __ldg(at);
-              if (g0 + 1u < p.groups) bits |= static_cast<uint32_t>(__ldg(at + 1)) << 16;
-            }
-          }
+          if (f < p.cols) bits = __ldg(p.sb + (size_t(passes[pi].expert) * rows + f + (up ? p.cols : 0u)) * p.groups + kb);
           scales[i] = bits;
         }
       }
@@ -501,96 +621,13 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort, kStatusTimeoutMma));
         const uint32_t w_at = smem_u32(ring + stage * C::kStageBytes), x_at = w_at + C::kWBytes;
         if (ok) {
-          if constexpr (!INT4) {
-#pragma unroll
-            for (uint32_t half = 0; half < 2; ++half) {  // 32 of the contraction
-              uint32_t b[kTiles8][4];
-#pragma unroll
-              for (uint32_t j = 0; j < kTiles8; ++j) {
-                if (j * 8u < ps.count) {
-                  const uint32_t row = lane & 7u, chunk = half * 4u + (lane >> 3);
-                  ldmatrix_x4(x_at + (j * 8u + row) * kRowBytes + ((chunk ^ row) << 4), b[j]);
-                }
-              }
-#pragma unroll
-              for (uint32_t m = 0; m < MR; ++m) {
-#pragma unroll
-                for (uint32_t k = 0; k < 2; ++k) {
-                  uint32_t a[4];
-                  const uint32_t row = (m * WR + wr) * 16u + (lane & 15u), chunk = half * 4u + k * 2u + (lane >> 4);
-                  ldmatrix_x4(w_at + row * kRowBytes + ((chunk ^ (row & 7u)) << 4), a);
-#pragma unroll
-                  for (uint32_t j = 0; j < kTiles8; ++j) {
-                    if (j * 8u < ps.count) mma_bf16(acc[m][j], a[0], a[1], a[2], a[3], b[j][2 * k], b[j][2 * k + 1]);
-                  }
-                }
-              }
-            }
+          // As many tiles of eight columns as the pass has (in steps of two above two).
+          if (NT == 8 || ps.count <= 8u) {
+            multiply_box<MR, WR, C::kXBytes, INT4, (1 < kTiles8 ? 1 : kTiles8)>(acc, w_at, x_at, sc, wr, lane);
+          } else if (NT == 16 || ps.count <= 16u) {
+            multiply_box<MR, WR, C::kXBytes, INT4, (2 < kTiles8 ? 2 : kTiles8)>(acc, w_at, x_at, sc, wr, lane);
           } else {
-#pragma unroll
-            for (uint32_t g = 0; g < 2; ++g) {  // scale groups
-              float part_sum[MR][kTiles8][4];
-#pragma unroll
-              for (uint32_t m = 0; m < MR; ++m) {
-#pragma unroll
-                for (uint32_t j = 0; j < kTiles8; ++j) {
-#pragma unroll
-                  for (uint32_t i = 0; i < 4; ++i) part_sum[m][j][i] = 0.f;
-                }
-              }
-#pragma unroll
-              for (uint32_t c4 = 0; c4 < 4; ++c4) {  // 32 codes of a row, 16 bytes
-                const uint32_t c = g * 4u + c4;
-                // Pairs of k: (0, 4), (1, 5), (2, 6), (3, 7) of a lane's eight, as the codes come.
-                uint32_t b[kTiles8][4];
-#pragma unroll
-                for (uint32_t j = 0; j < kTiles8; ++j) {
-                  if (j * 8u < ps.count) {
-                    uint32_t x[4];  // k = 8 q .. 8 q + 7 of the 32
-                    lds_128(x_at + (c >> 1) * C::kXBytes + (j * 8u + perm) * kRowBytes + ((((c & 1u) * 4u + q) ^ perm) << 4), x);
-                    b[j][0] = __byte_perm(x[0], x[2], 0x5410);
-                    b[j][1] = __byte_perm(x[0], x[2], 0x7632);
-                    b[j][2] = __byte_perm(x[1], x[3], 0x5410);
-                    b[j][3] = __byte_perm(x[1], x[3], 0x7632);
-                  }
-                }
-#pragma unroll
-                for (uint32_t m2 = 0; m2 < MR; m2 += 2) {
-                  uint32_t a[4];  // rows 0-7 and 8-15 of two blocks of rows
-                  const uint32_t row = ((m2 + (lane >> 4)) * WR + wr) * 16u + (lane & 15u);
-                  ldmatrix_x4(w_at + row * kRowBytes + ((c ^ (row & 7u)) << 4), a);
-#pragma unroll
-                  for (uint32_t m = 0; m < 2; ++m) {
-                    uint32_t lo[4], hi[4];
-                    codes_to_bf16(a[2 * m], lo);
-                    codes_to_bf16(a[2 * m + 1], hi);
-#pragma unroll
-                    for (uint32_t j = 0; j < kTiles8; ++j) {
-                      if (j * 8u < ps.count) {
-                        mma_bf16(part_sum[m2 + m][j], lo[0], hi[0], lo[1], hi[1], b[j][0], b[j][1]);
-                        mma_bf16(part_sum[m2 + m][j], lo[2], hi[2], lo[3], hi[3], b[j][2], b[j][3]);
-                      }
-                    }
-                  }
-                }
-              }
-#pragma unroll
-              for (uint32_t m = 0; m < MR; ++m) {
-                const uint32_t s_lo = __shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + g8);
-                const uint32_t s_hi = __shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + 8u + g8);
-                const float s0 = __uint_as_float(g == 0 ? s_lo << 16 : s_lo & 0xFFFF0000u);
-                const float s1 = __uint_as_float(g == 0 ? s_hi << 16 : s_hi & 0xFFFF0000u);
-#pragma unroll
-                for (uint32_t j = 0; j < kTiles8; ++j) {
-                  if (j * 8u < ps.count) {
-                    acc[m][j][0] = fmaf(s0, part_sum[m][j][0], acc[m][j][0]);
-                    acc[m][j][1] = fmaf(s0, part_sum[m][j][1], acc[m][j][1]);
-                    acc[m][j][2] = fmaf(s1, part_sum[m][j][2], acc[m][j][2]);
-                    acc[m][j][3] = fmaf(s1, part_sum[m][j][3], acc[m][j][3]);
-                  }
-                }
-              }
-            }
+            multiply_box<MR, WR, C::kXBytes, INT4, (4 < kTiles8 ? 4 : kTiles8)>(acc, w_at, x_at, sc, wr, lane);
           }
           __syncwarp();
           if (lane == 0) mbar_arrive(&empty[stage]);
@@ -657,15 +694,14 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
       for (uint32_t o = threadIdx.x; o < tile_cols * ps.count; o += kConsumers * 32u) {
         const uint32_t f = o % tile_cols, c = o / tile_cols;
         if (f0 + f >= p.cols) continue;
-        const uint32_t s = list[ps.first + c];
         if (SECOND) {
-          float* to = y + token_of(p, s) * C::kRows + f;
+          float* to = y + token_of(p, list[ps.first + c]) * C::kRows + f;
           *to = fmaf(share[ps.first + c], total(f, c), *to);
         } else {
           float v[2] = {total(f, c), 0.f};
           lin::activate(v, p.act);
           if (p.gated) v[0] *= total(C::kRows / 2u + f, c);
-          p.out[size_t(s) * p.ldo + f0 + f] = __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
+          p.out[size_t(ps.first + c) * p.ldo + f0 + f] = __bfloat16_as_ushort(__float2bfloat16_rn(v[0]));
         }
       }
     }

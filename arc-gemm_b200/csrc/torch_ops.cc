@@ -636,7 +636,7 @@ Tensor moe(const Tensor& x_in, const Tensor& w_in, const OptTensor& s_in, const 
   const Tensor x = product_rows(x_in), wi = s_in ? w_in : product_rows(w_in), wo = s_out ? w_out : product_rows(w_out);
   const Tensor ids = ids_in.contiguous(), weights = weights_in.contiguous();
   size_t bytes = 0;
-  check(g_api.moe_ws(t, top, i, &bytes), "arc.moe");
+  check(g_api.moe_ws(t, top, e, k, i, &bytes), "arc.moe");
   const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, x.options().dtype(at::kByte).requires_grad(false));
   check(g_api.moe(u16(x), wi.const_data_ptr(), s_in ? u16(*s_in) : nullptr, wo.const_data_ptr(),
                   s_out ? u16(*s_out) : nullptr, ids.const_data_ptr(), static_cast<int>(ids.element_size()),

@@ -403,7 +403,7 @@ int arc_group_rows(const void *ids, int id_bytes, int32_t *offsets, int32_t *row
  */
 #define ARC_MOE_MAX_TOKENS 256
 #define ARC_MOE_MAX_CHOICES 4096
-int arc_moe_workspace_bytes(int T, int top, int I, size_t *bytes);
+int arc_moe_workspace_bytes(int T, int top, int E, int K, int I, size_t *bytes);
 int arc_moe(const uint16_t *x, const void *w_in, const uint16_t *s_in, const void *w_out, const uint16_t *s_out,
             const void *ids, int id_bytes, const void *weights, int weight_bytes, uint16_t *out, void *workspace,
             size_t workspace_bytes, int T, int top, int E, int K, int I, int N, int64_t ldx, int64_t ld_in,

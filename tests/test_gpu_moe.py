@@ -64,14 +64,16 @@ def test_int4(cuda_device, shape, gated):
     _check(_inputs(*shape, kind="int4", gated=gated), "silu")
 
 
-@pytest.mark.parametrize("kind", ["bf16", "int4"])
-@pytest.mark.parametrize("plan", ["8:2:1:2:1:1", "8:2:2:2:1:2", "8:2:1:2:2:4", "8:4:1:4:2:2", "8:4:2:4:1:4", "16:2:2:2:4:8", "16:2:4:2:2:2", "16:4:1:4:2:1", "16:4:2:4:1:2", "32:2:4:2:2:1",
-                                  "32:2:2:2:4:2"])
-def test_plans(cuda_device, monkeypatch, plan, kind):
+@pytest.mark.parametrize("kind,columns", [("bf16", 8), ("bf16", 16), ("bf16", 32), ("int4", 8), ("int4", 16)])
+@pytest.mark.parametrize("splits,ordered", [(1, 0), (2, 1), (4, 0), (8, 1)])
+def test_plans(cuda_device, monkeypatch, kind, columns, splits, ordered):
     """Every instantiation and cluster size, with experts of more choices than a pass holds."""
-    monkeypatch.setenv("ARC_EXPERT_PLAN", plan)
+    monkeypatch.setenv("ARC_EXPERT_PLAN", f"{columns}:{splits}:{ordered}")
     for t in (3, 70):
-        _check(_inputs(t, 2, 5, 640, 512, n=456, kind=kind, seed=t), "gelu", plan)
+        _check(_inputs(t, 2, 5, 640, 512, n=456, kind=kind, seed=t), "gelu", t)
+    x, w_in, w_out, ids, weights = _inputs(40, 6, 4, 128, 256, kind=kind, repeat=True, seed=5)
+    ids[3], ids[4, 1:] = -1, 7
+    _check((x, w_in, w_out, ids, weights), "silu", "absent and repeated")
 
 
 @pytest.mark.parametrize("act", ACTS)
