@@ -19,6 +19,7 @@ the GEMM path is what this package covers):
 * `a8w4_grouped_matmul((x, sa), (wp, sb), offsets)`  the same on int8 x int4
 * `group_rows(ids, num_groups)`       a router's choices -> (offsets, rows, positions)
 * `moe(x, w_in, w_out, ids, weights)`  the expert layer of a few tokens, bf16 or int4 weights
+* `lora_linear(x, w, a, b, ids, bias, residual)`  the linear layer with an adapter of its own in every row
 * `quant`, `math`, `parallel`, `testing` helpers
 
 The kernels are AOT-built into libarcb200.so for sm_100a (`python -m arc.build`).
@@ -29,6 +30,7 @@ from .a8w4 import (a8w4_gemm_nt, a8w4_matmul, a8w4_matmul_bf16, fp8_fp4_gemm_nt,
                    quantize_int8)
 from .grouped import a8w4_grouped_matmul, group_rows, grouped_matmul
 from .linear import linear
+from .lora import lora_linear
 from .mm import matmul
 from .moe import moe
 
@@ -45,6 +47,7 @@ __all__ = [
     "a8w4_grouped_matmul",
     "group_rows",
     "moe",
+    "lora_linear",
     "ArcError",
     "describe_plan",
     "device_status",

@@ -167,6 +167,7 @@ struct DeviceState {
   int linear_status = ARC_OK;
   int grouped_status = ARC_OK;
   int experts_status = ARC_OK;
+  int lora_status = ARC_OK;
 };
 DeviceState g_dev[kMaxDevices];
 
@@ -216,6 +217,7 @@ int linear_init(DeviceState& st);  // api_linear.cuh
 int linear_kernel_name(int dev, uint32_t M, uint32_t N, uint32_t K, char* name, int len);
 int grouped_init();  // api_grouped.cuh
 int experts_init();  // api_experts.cuh
+int lora_init();  // api_lora.cuh
 
 int init_device(int dev) {
   DeviceState& st = g_dev[dev];
@@ -374,6 +376,7 @@ int init_device(int dev) {
     st.linear_status = linear_init(st);
     st.grouped_status = grouped_init();
     st.experts_status = experts_init();
+    st.lora_status = lora_init();
   });
   if (st.status != ARC_OK) {
     // Re-state the stored failure for this thread.
@@ -1447,3 +1450,4 @@ int arc_device_status(int device, uint32_t* status, int clear) {
 #include "api_linear.cuh"
 #include "api_grouped.cuh"
 #include "api_experts.cuh"
+#include "api_lora.cuh"

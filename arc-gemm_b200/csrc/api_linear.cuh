@@ -284,6 +284,63 @@ cudaError_t grouped_pair_launch(GP::Params& p, const arcb::lin::Groups& groups, 
   return launch_ex(kernel, p, grid, threads, smem, 2, stream);
 }
 
+// The pair kernel's operands, epilogue and walk for one group of rows.
+int linear_pair_params(LP::Params& p, const uint16_t* a, const uint16_t* w, uint32_t rows, uint16_t* out, uint32_t cols,
+                       uint32_t inner, uint64_t lda, uint64_t ldw, uint64_t w_stride, uint64_t ldo,
+                       const arcb::lin::Epilogue& epi, bool grad, uint32_t tile_cols) {
+  const uint64_t w_rows = grad ? inner : cols, w_cols = grad ? cols : inner;
+  if (int st = encode_groups_3d(&p.tm_a, a, inner, rows, 1, lda, 0, 64, LP::kRowsPerCta, "rows")) return st;
+  if (int st = encode_groups_3d(&p.tm_b, w, w_cols, w_rows, 1, ldw, w_stride, 64, grad ? 64 : tile_cols / 2, "weights")) {
+    return st;
+  }
+  p.out = out;
+  p.ldo = ldo;
+  p.epi = epi;
+  p.epi.wide_bias = aligned16(epi.bias) ? 1u : 0u;
+  if (int st = encode_pieces(&p.tm_out, &p.tma_out, out, cols, rows, 1, ldo, 0, "out")) return st;
+  if (int st = encode_pieces(&p.tm_z, &p.tma_z, epi.z, cols, rows, 1, epi.ldz, 0, "z")) return st;
+  if (int st = encode_pieces(&p.tm_res, &p.tma_res, epi.residual, cols, rows, 1, epi.ldr, 0, "residual")) return st;
+  p.M = rows;
+  p.N = cols;
+  p.tiles_m = ceil_div(rows, LP::kTile);
+  p.tiles_n = ceil_div(cols, tile_cols);
+  p.num_kb = ceil_div(inner, arcb::lin::BK);
+  if (uint64_t(p.tiles_m) * p.tiles_n * 4 > 0x7FFFFFFFu) {
+    return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
+  }
+  return ARC_OK;
+}
+
+// The same of the streaming kernel, and its grid.
+int linear_stream_params(LS::Params& p, const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& groups,
+                         uint16_t* out, uint32_t cols, uint32_t inner, uint64_t lda, uint64_t ldw, uint64_t w_stride,
+                         uint64_t ldo, const arcb::lin::Epilogue& epi, bool grad, const LinearPlan& plan, uint32_t* grid) {
+  const uint64_t w_rows = grad ? inner : cols, w_cols = grad ? cols : inner;
+  if (int st = encode_groups_3d(&p.tm_w, w, w_cols, w_rows, groups.num, ldw, w_stride, 64, grad ? 64 : LS::kRows,
+                                "weights")) {
+    return st;
+  }
+  if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a, inner, groups.rows, lda, 64, plan.bn,
+                         CU_TENSOR_MAP_SWIZZLE_128B, "rows")) {
+    return st;
+  }
+  p.out = out;
+  p.ldo = ldo;
+  p.groups = groups;
+  p.epi = epi;
+  p.epi.pair_residual = column_pairs(epi.residual, epi.ldr, cols);
+  p.epi.pair_z = column_pairs(epi.z, epi.ldz, cols);
+  p.epi.pair_out = column_pairs(out, ldo, cols);
+  p.cols = cols;
+  p.tiles_n = ceil_div(cols, LS::kRows);
+  p.num_kb = ceil_div(inner, arcb::lin::BK);
+  p.splits = plan.splits;
+  const uint64_t blocks = uint64_t(plan.row_tiles) * p.tiles_n * plan.splits;
+  if (blocks > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
+  *grid = static_cast<uint32_t>(blocks);
+  return ARC_OK;
+}
+
 // out[rows][cols] = epilogue of a [rows][inner] times w, per group. grad = false: w is
 // [E][cols][inner]; grad = true: w is [E][inner][cols] (the gradient of the rows).
 int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& groups, uint16_t* out, uint32_t cols,
@@ -320,28 +377,11 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
   }
   if (plan.pair) {
     LP::Params p = {};
-    if (int st = encode_groups_3d(&p.tm_a, a, inner, groups.rows, 1, lda, 0, 64, LP::kRowsPerCta, "rows")) {
+    if (int st = linear_pair_params(p, a, w, groups.rows, out, cols, inner, lda, ldw, w_stride, ldo, epi, grad,
+                                    plan.pair_cols)) {
       return st;
     }
-    if (int st = encode_groups_3d(&p.tm_b, w, w_cols, w_rows, 1, ldw, w_stride, 64,
-                                  grad ? 64 : plan.pair_cols / 2,
-                                  "weights")) {
-      return st;
-    }
-    p.out = out;
-    p.ldo = ldo;
-    p.epi = epi;
-    p.epi.wide_bias = aligned16(epi.bias) ? 1u : 0u;
-    if (int st = encode_pieces(&p.tm_out, &p.tma_out, out, cols, groups.rows, 1, ldo, 0, "out")) return st;
-    if (int st = encode_pieces(&p.tm_z, &p.tma_z, epi.z, cols, groups.rows, 1, epi.ldz, 0, "z")) return st;
-    if (int st = encode_pieces(&p.tm_res, &p.tma_res, epi.residual, cols, groups.rows, 1, epi.ldr, 0, "residual")) return st;
-    p.M = groups.rows;
-    p.N = cols;
-    p.tiles_m = ceil_div(groups.rows, LP::kTile);
-    p.tiles_n = ceil_div(cols, plan.pair_cols);
-    p.num_kb = num_kb;
     const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
-    if (tiles * 4 > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
     const bool narrow = plan.pair_cols == 128;
     const auto launch = grad ? (narrow ? launch_linear_pair<false, true, false, 128> : launch_linear_pair<false, true, false, 256>)
                              : (narrow ? launch_linear_pair<false, false, false, 128> : launch_linear_pair<false, false, false, 256>);
@@ -350,30 +390,12 @@ int linear_rows(const uint16_t* a, const uint16_t* w, const arcb::lin::Groups& g
     return ARC_OK;
   }
   LS::Params p = {};
-  if (int st = encode_groups_3d(&p.tm_w, w, w_cols, w_rows, groups.num, ldw, w_stride, 64, grad ? 64 : LS::kRows,
-                                "weights")) {
+  uint32_t grid = 0;
+  if (int st = linear_stream_params(p, a, w, groups, out, cols, inner, lda, ldw, w_stride, ldo, epi, grad, plan, &grid)) {
     return st;
   }
-  if (int st = encode_2d(&p.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, a, inner, groups.rows, lda, 64, plan.bn,
-                         CU_TENSOR_MAP_SWIZZLE_128B, "rows")) {
-    return st;
-  }
-  p.out = out;
-  p.ldo = ldo;
-  p.groups = groups;
-  p.epi = epi;
-  p.epi.pair_residual = column_pairs(epi.residual, epi.ldr, cols);
-  p.epi.pair_z = column_pairs(epi.z, epi.ldz, cols);
-  p.epi.pair_out = column_pairs(out, ldo, cols);
-  p.cols = cols;
-  p.tiles_n = ceil_div(cols, LS::kRows);
-  p.num_kb = num_kb;
-  p.splits = plan.splits;
   p.zero_others = zero_others ? 1u : 0u;
-  const uint64_t grid = uint64_t(plan.row_tiles) * p.tiles_n * plan.splits;
-  if (grid > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "the product has too many tiles for one launch");
-  e = grad ? launch_stream_bn<true>(p, plan.bn, static_cast<uint32_t>(grid), stream)
-           : launch_stream_bn<false>(p, plan.bn, static_cast<uint32_t>(grid), stream);
+  e = grad ? launch_stream_bn<true>(p, plan.bn, grid, stream) : launch_stream_bn<false>(p, plan.bn, grid, stream);
   if (e != cudaSuccess) return cuda_fail(e, "gemm_linear_stream_kernel launch");
   return ARC_OK;
 }

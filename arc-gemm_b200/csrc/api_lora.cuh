@@ -1,0 +1,215 @@
+// api_lora.cuh — host side of the linear layer with adapters: argument checks, launches. Included by api.cu, whose
+// helpers it uses.
+#pragma once
+
+#include "api_linear.cuh"
+
+namespace {
+
+namespace LO = arcb::lora;
+
+int lora_init() {
+  cudaError_t e = allow_smem(LP::lora_linear_pair_kernel<false, 256>, LP::kSmemBytes<256>);
+  if (e == cudaSuccess) e = allow_smem(LP::lora_linear_pair_kernel<true, 256>, LP::kSmemBytes<256>);
+  if (e == cudaSuccess) e = allow_smem(LP::lora_linear_pair_kernel<false, 128>, LP::kSmemBytes<128>);
+  if (e == cudaSuccess) e = allow_smem(LP::lora_linear_pair_kernel<true, 128>, LP::kSmemBytes<128>);
+  if (e == cudaSuccess) e = allow_smem(LS::lora_linear_stream_kernel<16>, LS::smem_bytes<16>());
+  if (e == cudaSuccess) e = allow_smem(LS::lora_linear_stream_kernel<32>, LS::smem_bytes<32>());
+  if (e == cudaSuccess) e = allow_smem(LS::lora_linear_stream_kernel<64>, LS::smem_bytes<64>());
+  if (e == cudaSuccess) e = allow_smem(LS::lora_linear_stream_kernel<128>, LS::smem_bytes<128>());
+  if (e != cudaSuccess) {
+    cudaGetLastError();  // clear
+    return cuda_fail(e, "cudaFuncSetAttribute (linear layer with adapters)");
+  }
+  return ARC_OK;
+}
+
+// The workspace: u [M][ldu], the number of adapters of each row tile, and their lists. Row tiles have 16 rows at
+// least, and of a list's places none is used beyond the rows of a tile and the adapters.
+struct LoraWorkspace {
+  uint64_t ldu;
+  size_t counts, lists, bytes;  // offsets
+};
+LoraWorkspace lora_workspace(uint32_t M, uint32_t rank) {
+  LoraWorkspace w;
+  w.ldu = (uint64_t(rank) + 7) / 8 * 8;
+  w.counts = (size_t(M) * w.ldu * 2 + 15) / 16 * 16;
+  const size_t tiles = ceil_div(M, 16);
+  w.lists = w.counts + (tiles * 2 + 15) / 16 * 16;
+  w.bytes = w.lists + (size_t(M) + 256) * 2;  // row tiles x rows of a tile
+  return w;
+}
+
+template <uint32_t RT, uint32_t NW>
+cudaError_t launch_lora_down(const LO::DownParams& p, uint32_t grid, cudaStream_t stream) {
+  return launch_ex(LO::lora_down_kernel<RT, NW>, p, grid, LO::kDownThreads, 0, p.splits, stream);
+}
+
+// u and the row tiles' lists. The contraction is split until the blocks fill the GPU or a warp has one round of
+// loads; then clusters share a block's adapters, of which there are 32 at most and in a prompt one or two.
+int lora_down(LO::DownParams& p, uint32_t sms, cudaStream_t stream) {
+  const uint32_t cols = p.rank <= 16 ? 16 : p.rank <= 32 ? 32 : 64;
+  p.row_blocks = ceil_div(p.M, LO::kDownRows);
+  p.rank_parts = ceil_div(p.rank, cols);
+  const uint32_t items = p.row_blocks * p.rank_parts, most = 2 * sms;
+  const uint32_t adapters = p.adapters < p.M ? p.adapters : p.M;
+  const uint32_t rounds = ceil_div(ceil_div(p.K, 32), LO::kDownWarps);  // chunks of a warp, unsplit
+  p.splits = 1;
+  while (p.splits < 8 && items * p.splits * 2 <= most && rounds >= p.splits * 2) p.splits *= 2;
+  if (p.row_blocks > 4 && p.splits > 4) p.splits = 4;  // leave some for a mixed batch's adapters
+  p.sets = most / (items * p.splits);
+  const uint32_t bound = adapters < LO::kDownRows ? adapters : LO::kDownRows;
+  p.sets = p.sets < 1 ? 1 : p.sets < bound ? p.sets : bound;
+  const uint64_t grid = uint64_t(items) * p.sets * p.splits;
+  if (grid > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "too many rows for one launch");
+  const cudaError_t e = cols == 16   ? launch_lora_down<2, 1>(p, static_cast<uint32_t>(grid), stream)
+                        : cols == 32 ? launch_lora_down<4, 1>(p, static_cast<uint32_t>(grid), stream)
+                                     : launch_lora_down<4, 2>(p, static_cast<uint32_t>(grid), stream);
+  if (e != cudaSuccess) return cuda_fail(e, "lora_down_kernel launch");
+  return ARC_OK;
+}
+
+template <bool SPLIT, uint32_t TN>
+cudaError_t launch_lora_pair(const LP::LoraParams& p, uint64_t tiles, uint32_t max_pairs, cudaStream_t stream) {
+  const uint32_t grid = SPLIT ? static_cast<uint32_t>(tiles) * 4 : 2 * static_cast<uint32_t>(tiles < max_pairs ? tiles : max_pairs);
+  return launch_ex(LP::lora_linear_pair_kernel<SPLIT, TN>, p, grid, LP::kThreads, LP::kSmemBytes<TN>, SPLIT ? 4 : 2, stream);
+}
+
+template <uint32_t BN>
+cudaError_t launch_lora_stream(const LS::LoraParams& p, uint32_t grid, cudaStream_t stream) {
+  return launch_ex(LS::lora_linear_stream_kernel<BN>, p, grid, LS::kThreads, LS::smem_bytes<BN>(), p.splits, stream);
+}
+
+}  // namespace
+
+extern "C" {
+
+int arc_lora_linear_workspace_bytes(int M, int R, size_t* bytes) {
+  if (bytes == nullptr || M <= 0 || R <= 0) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "arc_lora_linear_workspace_bytes: bad argument");
+  }
+  *bytes = lora_workspace(M, R).bytes;
+  return ARC_OK;
+}
+
+int arc_lora_linear(const uint16_t* x, const uint16_t* w, const uint16_t* a, const uint16_t* b, const void* ids,
+                    int id_bytes, const float* scales, const uint16_t* bias, const uint16_t* residual, uint16_t* out,
+                    void* workspace, size_t workspace_bytes, int M, int N, int K, int R, int L, int64_t ldx, int64_t ldw,
+                    int64_t lda, int64_t a_stride, int64_t ldb, int64_t b_stride, int64_t ldr, int64_t ldo, int activation,
+                    cudaStream_t stream) {
+  const char* what = "arc_lora_linear";
+  g_last_error[0] = '\0';
+  if (x == nullptr || w == nullptr || a == nullptr || b == nullptr || ids == nullptr || out == nullptr) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: null pointer", what);
+  }
+  if (M <= 0 || N <= 0 || K <= 0 || R <= 0 || L <= 0) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: sizes must be positive (M=%d N=%d K=%d R=%d L=%d)", what, M, N, K, R, L);
+  }
+  if (R > static_cast<int>(LO::kMaxRank) || L > static_cast<int>(LO::kMaxAdapters)) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: at most %u adapters of rank %u (got %d and %d)", what, LO::kMaxAdapters,
+                LO::kMaxRank, L, R);
+  }
+  if (activation < ARC_ACT_NONE || activation > ARC_ACT_SILU) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: unknown activation %d", what, activation);
+  }
+  if (id_bytes != 4 && id_bytes != 8) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: ids are 4- or 8-byte integers (got %d bytes)", what, id_bytes);
+  }
+  if (int st = operand_check(what, "x", x, ldx, K)) return st;
+  if (int st = operand_check(what, "w", w, ldw, K)) return st;
+  if (int st = operand_check(what, "a", a, lda, K)) return st;
+  if (int st = operand_check(what, "a's adapters", a, a_stride, int64_t(R - 1) * lda + K)) return st;
+  if (int st = operand_check(what, "b", b, ldb, R)) return st;
+  if (int st = operand_check(what, "b's adapters", b, b_stride, int64_t(N - 1) * ldb + R)) return st;
+  if (int st = output_check(what, "out", out, ldo, N)) return st;
+  if (residual != nullptr) {
+    if (int st = output_check(what, "residual", residual, ldr, N)) return st;
+  }
+  if ((reinterpret_cast<uintptr_t>(bias) & 1u) || (reinterpret_cast<uintptr_t>(scales) & 3u) ||
+      (reinterpret_cast<uintptr_t>(ids) & (id_bytes - 1))) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: bias, scales or ids are misaligned", what);
+  }
+  const LoraWorkspace ws = lora_workspace(M, R);
+  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < ws.bytes) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what, ws.bytes);
+  }
+  int dev = 0;
+  if (int st = current_device(&dev, &DeviceState::linear_status)) return st;
+  if (int st = current_device(&dev, &DeviceState::lora_status)) return st;
+  const uint32_t num_kb = ceil_div(K, arcb::lin::BK), max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
+  LinearPlan plan;
+  if (int st = linear_plan(dev, M, 1, N, num_kb, rows_aligned16(out, ldo), &plan)) return st;
+  const uint32_t tile_rows = plan.pair ? LP::kTile : plan.bn;
+
+  uint8_t* const base = static_cast<uint8_t*>(workspace);
+  LO::DownParams d = {};
+  d.x = x;
+  d.a = a;
+  d.scales = scales;
+  d.ids = ids;
+  d.u = static_cast<uint16_t*>(workspace);
+  d.counts = reinterpret_cast<uint16_t*>(base + ws.counts);
+  d.lists = reinterpret_cast<uint16_t*>(base + ws.lists);
+  d.ldx = ldx;
+  d.lda = lda;
+  d.a_stride = a_stride;
+  d.ldu = ws.ldu;
+  d.ids_wide = id_bytes == 8 ? 1 : 0;
+  d.adapters = L;
+  d.M = M;
+  d.K = K;
+  d.rank = R;
+  d.tile_rows = tile_rows;
+  d.tiles = ceil_div(M, tile_rows);
+  d.cap = tile_rows;
+  LO::Extra extra = {};
+  if (int st = encode_groups_3d(&extra.tm_u, workspace, R, M, 1, ws.ldu, 0, 64, plan.pair ? LP::kRowsPerCta : plan.bn, "u")) {
+    return st;
+  }
+  if (int st = encode_groups_3d(&extra.tm_b, b, R, N, L, ldb, b_stride, 64, plan.pair ? plan.pair_cols / 2 : LS::kRows, "b")) {
+    return st;
+  }
+  extra.counts = d.counts;
+  extra.lists = d.lists;
+  extra.ids = ids;
+  extra.ids_wide = d.ids_wide;
+  extra.adapters = L;
+  extra.rows = M;
+  extra.rank = R;
+  extra.cap = d.cap;
+  arcb::lin::Epilogue epi = {};
+  epi.bias = bias;
+  epi.residual = residual;
+  epi.ldr = residual != nullptr ? ldr : 0;
+  epi.act = static_cast<uint32_t>(activation);
+  const uint64_t w_stride = uint64_t(N) * ldw;
+
+  if (plan.pair) {
+    LP::LoraParams p = {};
+    if (int st = linear_pair_params(p, x, w, M, out, N, K, ldx, ldw, w_stride, ldo, epi, false, plan.pair_cols)) return st;
+    p.extra = extra;
+    if (int st = lora_down(d, static_cast<uint32_t>(g_dev[dev].sms), stream)) return st;
+    const uint64_t tiles = uint64_t(p.tiles_m) * p.tiles_n;
+    const bool narrow = plan.pair_cols == 128, split = plan.pair_splits > 1;
+    const cudaError_t e = narrow ? (split ? launch_lora_pair<true, 128>(p, tiles, max_pairs, stream)
+                                          : launch_lora_pair<false, 128>(p, tiles, max_pairs, stream))
+                                 : (split ? launch_lora_pair<true, 256>(p, tiles, max_pairs, stream)
+                                          : launch_lora_pair<false, 256>(p, tiles, max_pairs, stream));
+    if (e != cudaSuccess) return cuda_fail(e, "lora_linear_pair_kernel launch");
+    return ARC_OK;
+  }
+  LS::LoraParams p = {};
+  uint32_t grid = 0;
+  const arcb::lin::Groups groups = {nullptr, 1u, static_cast<uint32_t>(M)};
+  if (int st = linear_stream_params(p, x, w, groups, out, N, K, ldx, ldw, w_stride, ldo, epi, false, plan, &grid)) return st;
+  p.extra = extra;
+  if (int st = lora_down(d, static_cast<uint32_t>(g_dev[dev].sms), stream)) return st;
+  const cudaError_t e = plan.bn == 16   ? launch_lora_stream<16>(p, grid, stream)
+                        : plan.bn == 32 ? launch_lora_stream<32>(p, grid, stream)
+                        : plan.bn == 64 ? launch_lora_stream<64>(p, grid, stream)
+                                        : launch_lora_stream<128>(p, grid, stream);
+  if (e != cudaSuccess) return cuda_fail(e, "lora_linear_stream_kernel launch");
+  return ARC_OK;
+}
+
+}  // extern "C"

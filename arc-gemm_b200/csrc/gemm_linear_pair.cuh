@@ -33,6 +33,9 @@
 // and 23; but 1024 x 4096 x 4096 31 to 35 and 43, since a stage's products then hardly cover its
 // hand-offs).
 //
+// LORA: the blocks of a tile's adapters come behind the contraction's, as products that leave the rows of other
+// adapters as they are.
+//
 // Roles (384 threads per CTA): warp 0 TMA producer, warp 1 UMMA issuer (rank 0), warp 2 TMEM
 // owner, warp 3 zeroes a group's tail, warps 4-11 epilogue: two warpgroups take 32 columns in
 // turn; a thread owns one output row, and a warp's 32 x 32 piece goes out by TMA through shared
@@ -41,6 +44,7 @@
 
 #include "gemm_bf16_pair.cuh"
 #include "linear_common.cuh"
+#include "lora.cuh"
 
 namespace arcb {
 namespace linpair {
@@ -99,6 +103,11 @@ struct Params {
   lin::Epilogue epi;
   uint32_t M, N;       // output rows (of a group) and columns
   uint32_t tiles_m, tiles_n, num_kb;
+};
+
+// With adapters (LORA): see lora.cuh. The blocks of the tile's adapters follow those of the contraction.
+struct LoraParams : Params {
+  lora::Extra extra;
 };
 
 // One tile of the walk.
@@ -256,9 +265,10 @@ __device__ __forceinline__ bool finish_piece(const Params& p, Pieces& b, float (
   return true;
 }
 
-template <bool A_MN, bool B_MN, bool ALONG_K, bool SPLIT, uint32_t TN>
-__global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __grid_constant__ Params p) {
+template <bool A_MN, bool B_MN, bool ALONG_K, bool SPLIT, uint32_t TN, bool LORA, typename P>
+__device__ __forceinline__ void linear_pair(const P& p) {
   static_assert(TN == 256 || (TN == 128 && !ALONG_K), "columns of a tile");
+  static_assert(!LORA || (!A_MN && !B_MN && !ALONG_K), "adapters belong to the forward product");
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   constexpr uint32_t kStages = Cfg<TN>::kStages;
   Smem<TN>& s = *reinterpret_cast<Smem<TN>*>(smem_raw + smem_align_pad(smem_raw));
@@ -292,8 +302,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     fence_barrier_init();
   }
   // TMEM is taken only after the preceding grid has ended, and the next grid is let in only
-  // after it is taken: two grids of the stream never hold each other's columns up.
-  pdl_wait();
+  // after it is taken: two grids of the stream never hold each other's columns up. With adapters the preceding
+  // grid is lora_down_kernel, which uses no TMEM and has waited for what came before it: only what it
+  // writes, and the output, wait for its end.
+  if (!LORA) pdl_wait();
   if (warp == 2) {
     tmem_alloc_pair(&s.tmem_base, kTmemCols);
     tmem_relinquish_pair();
@@ -302,7 +314,7 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
   __syncthreads();
   cluster_sync_all();  // both CTAs' barriers exist before any remote arrive or TMA
   tc_fence_after_sync();
-  pdl_launch_dependents();
+  if (!LORA) pdl_launch_dependents();
   const uint32_t tmem_base = s.tmem_base;
 
   const uint32_t epi_warp = warp >= 4 ? warp - 4u : 0u;
@@ -353,6 +365,28 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
+          }
+        }
+        if constexpr (LORA) {
+          if (SPLIT && part == 0u) continue;
+          pdl_wait();
+          const lora::TileList list(p.extra, w.m0 / kTile);
+          for (uint32_t i = 0; ok && i < list.blocks; ++i) {
+            if (!mbar_wait(&s.empty[stage], phase ^ 1u, abort, kStatusTimeoutProducer)) {
+              ok = false;
+              break;
+            }
+            const uint32_t bar = map_to_rank(&s.full[stage], lead);
+            if (rank == 0) mbar_arrive_expect_tx(&s.full[stage], 2 * Cfg<TN>::kStageBytes);
+            const int32_t r = int32_t(list.column(i));
+            tma_load_3d_pair(&p.extra.tm_u, bar, s.a[stage], r, int32_t(w.m0 + row0), 0, kCacheEvictNormal);
+            tma_load_3d_pair(&p.extra.tm_b, bar, s.b[stage], r, int32_t(w.n0 + rank * (TN / 2u)), int32_t(list.adapter(i)),
+                             kCacheEvictNormal);
+            ++issued;
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
         }
       }
@@ -407,6 +441,34 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
           if (++stage == kStages) {
             stage = 0;
             phase ^= 1u;
+          }
+        }
+        if constexpr (LORA) {
+          pdl_wait();
+          const lora::TileList list(p.extra, w.m0 / kTile);
+          const lora::RowAdapters<kTile> rows(p.extra, w.m0, lane);
+          const uint32_t blocks = !SPLIT || part == 1u ? list.blocks : 0u;
+          for (uint32_t i = 0; ok && i < blocks; ++i) {
+            uint32_t keep[kTile / 32];
+            rows.others(list.adapter(i), keep);
+            ok = __all_sync(0xffffffffu, mbar_wait(&s.full[stage], phase, abort, kStatusTimeoutMma));
+            if (!ok) break;
+            tc_fence_after_sync();
+            const uint64_t adesc = lin::operand_desc<A_MN>(s.a[stage]);
+            const uint64_t bdesc = lin::operand_desc<B_MN>(s.b[stage]);
+            const uint32_t steps = lora::steps_of(p.extra, i);
+#pragma unroll
+            for (uint32_t k = 0; k < BK / kUmmaK; ++k) {
+              if (leader && k < steps) {
+                umma_bf16_pair_masked(d_tmem, desc_advance(adesc, k * lin::operand_step<A_MN>()),
+                                      desc_advance(bdesc, k * lin::operand_step<B_MN>()), idesc, 1u, keep);
+              }
+            }
+            if (leader) umma_commit_pair(&s.empty[stage], both);
+            if (++stage == kStages) {
+              stage = 0;
+              phase ^= 1u;
+            }
           }
         }
         if (ok && leader) umma_commit_pair(&s.tmem_full[acc], both);
@@ -465,6 +527,10 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     const uint32_t wg = (warp - 4u) >> 2;
     const uint32_t row = q * 32 + lane;
     const uint32_t empty0[2] = {map_to_rank(&s.tmem_empty[0], lead), map_to_rank(&s.tmem_empty[1], lead)};
+    if (LORA) {
+      pdl_wait();
+      pdl_launch_dependents();
+    }
     uint32_t local = 0;
     bool ok = true;
     Tile w;
@@ -577,6 +643,16 @@ __global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __g
     tc_fence_after_sync();
     tmem_dealloc_pair(tmem_base, kTmemCols);
   }
+}
+
+template <bool A_MN, bool B_MN, bool ALONG_K, bool SPLIT, uint32_t TN>
+__global__ void __launch_bounds__(kThreads, 1) gemm_linear_pair_kernel(const __grid_constant__ Params p) {
+  linear_pair<A_MN, B_MN, ALONG_K, SPLIT, TN, false>(p);
+}
+
+template <bool SPLIT, uint32_t TN>
+__global__ void __launch_bounds__(kThreads, 1) lora_linear_pair_kernel(const __grid_constant__ LoraParams p) {
+  linear_pair<false, false, false, SPLIT, TN, true>(p);
 }
 
 }  // namespace linpair

@@ -752,6 +752,18 @@ __device__ __forceinline__ void umma_bf16_pair(uint32_t d_tmem, uint64_t a_desc,
       : "memory");
 }
 
+// The same, leaving rows of D as they are: bit r of `keep` (rows 0-127 in rank 0's TMEM, 128-255 in rank 1's).
+__device__ __forceinline__ void umma_bf16_pair_masked(uint32_t d_tmem, uint64_t a_desc, uint64_t b_desc, uint32_t idesc,
+                                                      uint32_t accumulate, const uint32_t (&keep)[8]) {
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "setp.ne.b32 p, %4, 0;\n\t"
+      "tcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, {%5, %6, %7, %8, %9, %10, %11, %12}, p;\n\t}" ::"r"(d_tmem),
+      "l"(a_desc), "l"(b_desc), "r"(idesc), "r"(accumulate), "r"(keep[0]), "r"(keep[1]), "r"(keep[2]), "r"(keep[3]),
+      "r"(keep[4]), "r"(keep[5]), "r"(keep[6]), "r"(keep[7])
+      : "memory");
+}
+
 // Arrive once on the mbarrier at `bar`'s offset in every CTA of `cta_mask` when all
 // pair tcgen05 operations issued so far by this thread have completed. (This is the
 // completion signal of tcgen05, not a memory load.)

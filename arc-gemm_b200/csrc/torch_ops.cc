@@ -47,6 +47,8 @@ struct Api {
   decltype(&arc_group_rows) group_rows = nullptr;
   decltype(&arc_moe_workspace_bytes) moe_ws = nullptr;
   decltype(&arc_moe) moe = nullptr;
+  decltype(&arc_lora_linear_workspace_bytes) lora_linear_ws = nullptr;
+  decltype(&arc_lora_linear) lora_linear = nullptr;
 };
 Api g_api;
 
@@ -648,6 +650,81 @@ Tensor moe(const Tensor& x_in, const Tensor& w_in, const OptTensor& s_in, const 
 }
 
 // ---------------------------------------------------------------------------------
+// lora_linear
+// ---------------------------------------------------------------------------------
+constexpr int64_t kMaxAdapters = 1024, kMaxRank = 256;
+
+Tensor lora_linear(const Tensor& x_in, const Tensor& w_in, const Tensor& a_in, const Tensor& b_in, const Tensor& ids_in,
+                   const OptTensor& bias, const OptTensor& residual, const OptTensor& scales, int64_t act,
+                   const OptTensor& out) {
+  expect_bf16(x_in, "x", 2);
+  expect_bf16(w_in, "w", 2);
+  expect_bf16(a_in, "a", 3);
+  expect_bf16(b_in, "b", 3);
+  const at::Device dev = x_in.device();
+  expect_device(w_in, "w", dev);
+  expect_device(a_in, "a", dev);
+  expect_device(b_in, "b", dev);
+  const int64_t m = x_in.size(0), n = w_in.size(0), k = x_in.size(1), l = a_in.size(0), r = a_in.size(1);
+  if (k != w_in.size(1)) bad_value("Inner dimensions must match: ", k, " vs ", w_in.size(1));
+  if (n == 0 || k == 0) bad_value("w must not be empty, got shape ", shape_of(w_in));
+  if (l < 1 || l > kMaxAdapters || r < 1 || r > kMaxRank) {
+    bad_value("between 1 and ", kMaxAdapters, " adapters of rank 1 to ", kMaxRank, " are supported, got ", l, " of ", r);
+  }
+  expect_shape(a_in, "a", {l, r, k});
+  expect_shape(b_in, "b", {l, n, r});
+  as_int(m, "M"), as_int(n, "N"), as_int(k, "K");
+  expect_cuda(ids_in, "ids");
+  expect_device(ids_in, "ids", dev);
+  if (ids_in.scalar_type() != at::kInt && ids_in.scalar_type() != at::kLong) {
+    bad_type("ids must be int32 or int64, got ", ids_in.scalar_type());
+  }
+  expect_shape(ids_in, "ids", {m});
+  if (bias) {
+    if (bias->scalar_type() != at::kBFloat16 || bias->dim() != 1 || bias->size(0) != n) {
+      bad_value("bias must be bfloat16 of shape [", n, "], got ", bias->scalar_type(), " ", shape_of(*bias));
+    }
+    expect_device(*bias, "bias", dev);
+  }
+  if (residual) {
+    expect_bf16(*residual, "residual", 2);
+    expect_shape(*residual, "residual", {m, n});
+    expect_device(*residual, "residual", dev);
+  }
+  if (scales) {
+    expect_cuda(*scales, "scales");
+    expect_device(*scales, "scales", dev);
+    expect_dtype(*scales, "scales", at::kFloat);
+    expect_shape(*scales, "scales", {l});
+  }
+  refuse_tangents(x_in, w_in, a_in, b_in, bias, residual, scales, out);
+  refuse_gradients("arc.lora_linear", x_in, w_in, a_in, b_in, bias, residual, scales);
+  const c10::cuda::CUDAGuard guard(dev);
+  if (out) expect_out(*out, m, n, dev);
+  if (out && residual && !same_view(*out, *residual) && share_bytes(*out, *residual)) {
+    bad_value("out must be residual itself or not overlap it");
+  }
+  claim_out(out, {&x_in, &w_in, &a_in, &b_in, &ids_in, bias ? &*bias : &w_in, scales ? &*scales : &w_in});
+  const auto options = x_in.options().requires_grad(false);
+  const Tensor y = out ? *out : at::empty({m, n}, options);
+  if (m == 0) return y;
+  const Tensor x = product_rows(x_in), w = product_rows(w_in), a = product_rows(a_in), b = product_rows(b_in);
+  const Tensor ids = ids_in.contiguous();
+  const OptTensor bias_c = bias ? OptTensor(bias->contiguous()) : bias, scales_c = scales ? OptTensor(scales->contiguous()) : scales,
+                  rows = residual ? OptTensor(unit_rows(*residual)) : residual;
+  size_t bytes = 0;
+  check(g_api.lora_linear_ws(m, r, &bytes), "arc.lora_linear");
+  const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
+  check(g_api.lora_linear(u16(x), u16(w), u16(a), u16(b), ids.const_data_ptr(), static_cast<int>(ids.element_size()),
+                          scales_c ? scales_c->const_data_ptr<float>() : nullptr, bias_c ? u16(*bias_c) : nullptr,
+                          rows ? u16(*rows) : nullptr, u16_mut(y), workspace.data_ptr(), bytes, m, n, k, r, l, x.stride(0),
+                          w.stride(0), a.stride(1), a.stride(0), b.stride(1), b.stride(0), rows ? row_ld(*rows) : 0, row_ld(y),
+                          static_cast<int>(act), stream_of(x)),
+        "arc.lora_linear");
+  return y;
+}
+
+// ---------------------------------------------------------------------------------
 // Module
 // ---------------------------------------------------------------------------------
 PyObject* g_arc_error = nullptr;  // arc.ArcError, one reference for the life of the process
@@ -670,6 +747,8 @@ void bind(const std::unordered_map<std::string, uintptr_t>& addresses, py::objec
   set(g_api.group_rows, "arc_group_rows");
   set(g_api.moe_ws, "arc_moe_workspace_bytes");
   set(g_api.moe, "arc_moe");
+  set(g_api.lora_linear_ws, "arc_lora_linear_workspace_bytes");
+  set(g_api.lora_linear, "arc_lora_linear");
   g_arc_error = arc_error.release().ptr();
 }
 
@@ -690,4 +769,5 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("a8w4_grouped_matmul", &a8w4_grouped_matmul);
   m.def("group_rows", &group_rows);
   m.def("moe", &moe);
+  m.def("lora_linear", &lora_linear);
 }
