@@ -88,7 +88,7 @@ SIGNATURES = {
     "arc_group_rows": ([_P, _I, _P, _P, _P, _P, ctypes.c_size_t, _I, _I, _I, _P], _I),
     "arc_moe_workspace_bytes": ([_I] * 5 + [ctypes.POINTER(ctypes.c_size_t)], _I),
     "arc_moe": ([_P] * 6 + [_I, _P, _I, _P, _P, ctypes.c_size_t] + [_I] * 6 + [_L] * 6 + [_I, _I, _P], _I),
-    "arc_lora_linear_workspace_bytes": ([_I, _I, ctypes.POINTER(ctypes.c_size_t)], _I),
+    "arc_lora_linear_workspace_bytes": ([_I] * 4 + [ctypes.POINTER(ctypes.c_size_t)], _I),
     "arc_lora_linear": ([_P] * 5 + [_I] + [_P] * 5 + [ctypes.c_size_t] + [_I] * 5 + [_L] * 8 + [_I, _P], _I),
     "arc_a8w4_gemm_gather_sync": ([_P, _P, _P, _P, _P, _P, _I, _I, _I, _I, _I, ctypes.c_uint, _P], _I),
 }

@@ -17,6 +17,9 @@ int lora_init() {
   if (e == cudaSuccess) e = allow_smem(LS::lora_linear_stream_kernel<32>, LS::smem_bytes<32>());
   if (e == cudaSuccess) e = allow_smem(LS::lora_linear_stream_kernel<64>, LS::smem_bytes<64>());
   if (e == cudaSuccess) e = allow_smem(LS::lora_linear_stream_kernel<128>, LS::smem_bytes<128>());
+  if (e == cudaSuccess) e = allow_smem(LO::lora_down_kernel<16>, LO::kDownSmem);
+  if (e == cudaSuccess) e = allow_smem(LO::lora_down_kernel<32>, LO::kDownSmem);
+  if (e == cudaSuccess) e = allow_smem(LO::lora_down_kernel<64>, LO::kDownSmem);
   if (e != cudaSuccess) {
     cudaGetLastError();  // clear
     return cuda_fail(e, "cudaFuncSetAttribute (linear layer with adapters)");
@@ -24,47 +27,44 @@ int lora_init() {
   return ARC_OK;
 }
 
-// The workspace: u [M][ldu], the number of adapters of each row tile, and their lists. Row tiles have 16 rows at
-// least, and of a list's places none is used beyond the rows of a tile and the adapters.
+// The workspace: u [M][ldu], the number of adapters of each row tile, their lists, and where the product streams the
+// adapters' sums [M][N]. Row tiles have 16 rows at least, and a list has a place for each row of its tile.
 struct LoraWorkspace {
   uint64_t ldu;
-  size_t counts, lists, bytes;  // offsets
+  size_t counts, lists, sums, bytes;  // offsets
 };
-LoraWorkspace lora_workspace(uint32_t M, uint32_t rank) {
+LoraWorkspace lora_workspace(uint32_t M, uint32_t N, uint32_t rank, const LinearPlan& plan) {
   LoraWorkspace w;
   w.ldu = (uint64_t(rank) + 7) / 8 * 8;
   w.counts = (size_t(M) * w.ldu * 2 + 15) / 16 * 16;
   const size_t tiles = ceil_div(M, 16);
   w.lists = w.counts + (tiles * 2 + 15) / 16 * 16;
-  w.bytes = w.lists + (size_t(M) + 256) * 2;  // row tiles x rows of a tile
+  w.sums = (w.lists + (size_t(M) + 256) * 2 + 15) / 16 * 16;  // row tiles x rows of a tile
+  w.bytes = w.sums + (plan.pair ? 0 : size_t(M) * N * sizeof(float));
   return w;
 }
 
-template <uint32_t RT, uint32_t NW>
-cudaError_t launch_lora_down(const LO::DownParams& p, uint32_t grid, cudaStream_t stream) {
-  return launch_ex(LO::lora_down_kernel<RT, NW>, p, grid, LO::kDownThreads, 0, p.splits, stream);
-}
+// Rows that an adapter has among the 64 of an item.
+uint32_t lora_rows(uint32_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 
-// u and the row tiles' lists. The contraction is split until the blocks fill the GPU or a warp has one round of
-// loads; then clusters share a block's adapters, of which there are 32 at most and in a prompt one or two.
+// u and the row tiles' lists. The contraction is split until the blocks fill the GPU or a warp has one box; then
+// clusters share a block's adapters, of which there are 32 at most and in a prompt one or two.
 int lora_down(LO::DownParams& p, uint32_t sms, cudaStream_t stream) {
-  const uint32_t cols = p.rank <= 16 ? 16 : p.rank <= 32 ? 32 : 64;
+  const uint32_t rows = lora_rows(p.rank), group = LO::kDownCols / rows;
   p.row_blocks = ceil_div(p.M, LO::kDownRows);
-  p.rank_parts = ceil_div(p.rank, cols);
-  const uint32_t items = p.row_blocks * p.rank_parts, most = 2 * sms;
+  p.rank_parts = ceil_div(p.rank, LO::kDownCols);
   const uint32_t adapters = p.adapters < p.M ? p.adapters : p.M;
-  const uint32_t rounds = ceil_div(ceil_div(p.K, 32), LO::kDownWarps);  // chunks of a warp, unsplit
+  const uint32_t bound = ceil_div(adapters < LO::kDownRows ? adapters : LO::kDownRows, group);  // items of a block
+  const uint32_t items = p.row_blocks * p.rank_parts, most = 2 * sms, boxes = ceil_div(p.K, 64);
   p.splits = 1;
-  while (p.splits < 8 && items * p.splits * 2 <= most && rounds >= p.splits * 2) p.splits *= 2;
-  if (p.row_blocks > 4 && p.splits > 4) p.splits = 4;  // leave some for a mixed batch's adapters
+  while (p.splits < 8 && items * p.splits * 2 <= most && boxes >= LO::kDownWarps * p.splits * 2) p.splits *= 2;
   p.sets = most / (items * p.splits);
-  const uint32_t bound = adapters < LO::kDownRows ? adapters : LO::kDownRows;
   p.sets = p.sets < 1 ? 1 : p.sets < bound ? p.sets : bound;
   const uint64_t grid = uint64_t(items) * p.sets * p.splits;
   if (grid > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "too many rows for one launch");
-  const cudaError_t e = cols == 16   ? launch_lora_down<2, 1>(p, static_cast<uint32_t>(grid), stream)
-                        : cols == 32 ? launch_lora_down<4, 1>(p, static_cast<uint32_t>(grid), stream)
-                                     : launch_lora_down<4, 2>(p, static_cast<uint32_t>(grid), stream);
+  const auto kernel = rows == 16 ? LO::lora_down_kernel<16> : rows == 32 ? LO::lora_down_kernel<32> : LO::lora_down_kernel<64>;
+  const cudaError_t e =
+      launch_ex(kernel, p, static_cast<uint32_t>(grid), LO::kDownThreads, LO::kDownSmem, p.splits, stream);
   if (e != cudaSuccess) return cuda_fail(e, "lora_down_kernel launch");
   return ARC_OK;
 }
@@ -84,11 +84,20 @@ cudaError_t launch_lora_stream(const LS::LoraParams& p, uint32_t grid, cudaStrea
 
 extern "C" {
 
-int arc_lora_linear_workspace_bytes(int M, int R, size_t* bytes) {
-  if (bytes == nullptr || M <= 0 || R <= 0) {
+int arc_lora_linear_workspace_bytes(int M, int N, int K, int R, size_t* bytes) {
+  if (bytes == nullptr || M <= 0 || N <= 0 || K <= 0 || R <= 0) {
     return fail(ARC_ERR_INVALID_ARGUMENT, "arc_lora_linear_workspace_bytes: bad argument");
   }
-  *bytes = lora_workspace(M, R).bytes;
+  // The larger of the plans for aligned and for other output rows.
+  *bytes = 0;
+  int dev = 0;
+  if (int st = current_device(&dev, &DeviceState::linear_status)) return st;
+  for (bool aligned : {false, true}) {
+    LinearPlan plan;
+    if (int st = linear_plan(dev, M, 1, N, ceil_div(K, arcb::lin::BK), aligned, &plan)) return st;
+    const size_t need = lora_workspace(M, N, R, plan).bytes;
+    if (need > *bytes) *bytes = need;
+  }
   return ARC_OK;
 }
 
@@ -129,9 +138,8 @@ int arc_lora_linear(const uint16_t* x, const uint16_t* w, const uint16_t* a, con
       (reinterpret_cast<uintptr_t>(ids) & (id_bytes - 1))) {
     return fail(ARC_ERR_UNSUPPORTED, "%s: bias, scales or ids are misaligned", what);
   }
-  const LoraWorkspace ws = lora_workspace(M, R);
-  if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < ws.bytes) {
-    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what, ws.bytes);
+  if (workspace == nullptr || !aligned16(workspace)) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace", what);
   }
   int dev = 0;
   if (int st = current_device(&dev, &DeviceState::linear_status)) return st;
@@ -139,20 +147,26 @@ int arc_lora_linear(const uint16_t* x, const uint16_t* w, const uint16_t* a, con
   const uint32_t num_kb = ceil_div(K, arcb::lin::BK), max_pairs = static_cast<uint32_t>(g_dev[dev].max_linear_pairs);
   LinearPlan plan;
   if (int st = linear_plan(dev, M, 1, N, num_kb, rows_aligned16(out, ldo), &plan)) return st;
+  const LoraWorkspace ws = lora_workspace(M, N, R, plan);
+  if (workspace_bytes < ws.bytes) {
+    return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a workspace of %zu bytes", what, ws.bytes);
+  }
   const uint32_t tile_rows = plan.pair ? LP::kTile : plan.bn;
 
   uint8_t* const base = static_cast<uint8_t*>(workspace);
   LO::DownParams d = {};
-  d.x = x;
-  d.a = a;
+  if (int st = encode_2d(&d.tm_x, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, x, K, M, ldx, 64, LO::kDownRows,
+                         CU_TENSOR_MAP_SWIZZLE_128B, "x")) {
+    return st;
+  }
+  if (int st = encode_groups_3d(&d.tm_a, a, K, R, L, lda, a_stride, 64, lora_rows(R), "a")) return st;
   d.scales = scales;
   d.ids = ids;
   d.u = static_cast<uint16_t*>(workspace);
-  d.counts = reinterpret_cast<uint16_t*>(base + ws.counts);
-  d.lists = reinterpret_cast<uint16_t*>(base + ws.lists);
-  d.ldx = ldx;
-  d.lda = lda;
-  d.a_stride = a_stride;
+  if (plan.pair) {
+    d.counts = reinterpret_cast<uint16_t*>(base + ws.counts);
+    d.lists = reinterpret_cast<uint16_t*>(base + ws.lists);
+  }
   d.ldu = ws.ldu;
   d.ids_wide = id_bytes == 8 ? 1 : 0;
   d.adapters = L;
@@ -163,12 +177,16 @@ int arc_lora_linear(const uint16_t* x, const uint16_t* w, const uint16_t* a, con
   d.tiles = ceil_div(M, tile_rows);
   d.cap = tile_rows;
   LO::Extra extra = {};
-  if (int st = encode_groups_3d(&extra.tm_u, workspace, R, M, 1, ws.ldu, 0, 64, plan.pair ? LP::kRowsPerCta : plan.bn, "u")) {
-    return st;
+  if (plan.pair) {
+    if (int st = encode_groups_3d(&extra.tm_u, workspace, R, M, 1, ws.ldu, 0, 64, LP::kRowsPerCta, "u")) return st;
+    if (int st = encode_groups_3d(&extra.tm_b, b, R, N, L, ldb, b_stride, 64, plan.pair_cols / 2, "b")) return st;
   }
-  if (int st = encode_groups_3d(&extra.tm_b, b, R, N, L, ldb, b_stride, 64, plan.pair ? plan.pair_cols / 2 : LS::kRows, "b")) {
-    return st;
-  }
+  extra.u = d.u;
+  extra.b = b;
+  extra.sums = reinterpret_cast<float*>(base + ws.sums);
+  extra.ldu = ws.ldu;
+  extra.ldb = ldb;
+  extra.b_stride = b_stride;
   extra.counts = d.counts;
   extra.lists = d.lists;
   extra.ids = ids;

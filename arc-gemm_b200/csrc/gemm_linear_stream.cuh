@@ -86,9 +86,9 @@ struct Params {
   uint32_t zero_others;  // zero the output rows of no group
 };
 
-// With adapters (LORA): see lora.cuh. The blocks of the tile's adapters follow those of the contraction, shared out
-// over the cluster as those are; warp 2 zeroes the rows of other adapters in shared memory, and what is not finite in
-// the adapter, for which its own rows get NaN.
+// With adapters (LORA): see lora.cuh. The epilogue's warps compute the adapters' part of the tile while the weights
+// stream, an adapter of the tile's list each in turn (a block of a cluster has every S-th), and leave it in memory,
+// from where the block that has computed a row adds it to its own sums.
 struct LoraParams : Params {
   lora::Extra extra;
 };
@@ -144,10 +144,6 @@ template <uint32_t BN, bool W_MN, bool LORA, typename P>
 __device__ __forceinline__ void linear_stream(const P& p) {
   static_assert(!LORA || !W_MN, "adapters belong to the forward product");
   using C = Cfg<BN>;
-  constexpr uint32_t kRowWords = (BN + 31u) / 32u;
-  __shared__ uint64_t landed[LORA ? C::kStages : 1];  // LORA: an adapter's block is in, its rows not yet zeroed
-  __shared__ uint32_t spoilt[LORA ? kRows : 1][kRowWords];  // LORA: rows whose adapter is not finite in a column
-  __shared__ uint32_t any_spoilt;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   Smem<BN>& s = *reinterpret_cast<Smem<BN>*>(smem_raw + smem_align_pad(smem_raw));
   const uint32_t warp = warp_idx_sync();
@@ -161,7 +157,6 @@ __device__ __forceinline__ void linear_stream(const P& p) {
     for (uint32_t i = 0; i < C::kStages; ++i) {
       mbar_init(&s.full[i], 1);
       mbar_init(&s.empty[i], 1);
-      if (LORA) mbar_init(&landed[i], 1);
     }
     mbar_init(&s.done, 1);
     s.abort = 0;
@@ -249,37 +244,9 @@ __device__ __forceinline__ void linear_stream(const P& p) {
           phase ^= 1u;
         }
       }
-      uint32_t is_extra = 0, extra_parity = 0;  // per stage: last block was an adapter's; its barrier's next parity
-      if constexpr (LORA) {
-        const uint32_t plain = issued;
-        if (plain == kb1 - kb0) {
-          pdl_wait();
-          const lora::TileList list(p.extra, row0 / BN);
-          const uint32_t i1 = list.blocks * (rank + 1u) / p.splits;
-          for (uint32_t i = list.blocks * rank / p.splits; i < i1; ++i) {
-            if (!mbar_wait(&s.empty[stage], phase ^ 1u, abort, kStatusTimeoutProducer)) break;
-            mbar_arrive_expect_tx(&landed[stage], kWBytes + C::kXBytes);
-            is_extra |= 1u << stage;
-            extra_parity ^= 1u << stage;
-            const int32_t r = int32_t(list.column(i));
-            tma_load_3d(&p.extra.tm_b, &landed[stage], s.w[stage], r, int32_t(f0), int32_t(list.adapter(i)), kCacheEvictNormal);
-            tma_load_3d(&p.extra.tm_u, &landed[stage], s.x[stage], r, int32_t(row0), 0, kCacheEvictNormal);
-            ++issued;
-            if (++stage == C::kStages) {
-              stage = 0;
-              phase ^= 1u;
-            }
-          }
-        }
-      }
       const uint32_t n_drain = issued < C::kStages ? issued : C::kStages;
       for (uint32_t i = issued - n_drain; i < issued; ++i) {
-        const uint32_t st = i % C::kStages;
-        if (LORA && ((is_extra >> st) & 1u) != 0u) {
-          mbar_drain(&landed[st], ((extra_parity >> st) & 1u) ^ 1u);
-        } else {
-          mbar_drain(&s.full[st], (i / C::kStages) & 1u);
-        }
+        mbar_drain(&s.full[i % C::kStages], (i / C::kStages) & 1u);
       }
     }
   } else if (warp == 1) {
@@ -303,77 +270,40 @@ __device__ __forceinline__ void linear_stream(const P& p) {
           phase ^= 1u;
         }
       }
-      if constexpr (LORA) {
-        pdl_wait();
-        const uint32_t blocks = lora::TileList(p.extra, row0 / BN).blocks;
-        const uint32_t i1 = blocks * (rank + 1u) / p.splits;
-        for (uint32_t i = blocks * rank / p.splits; i < i1; ++i) {
-          if (!mbar_wait(&s.full[stage], phase, abort, kStatusTimeoutMma)) break;
-          tc_fence_after_sync();
-          const uint64_t adesc = lin::operand_desc<W_MN>(s.w[stage]);
-          const uint64_t bdesc = make_sw128_kmajor_desc(s.x[stage]);
-          const uint32_t steps = lora::steps_of(p.extra, i);
-          for (uint32_t k = 0; k < steps; ++k) {
-            umma_bf16(tmem_base, desc_advance(adesc, k * lin::operand_step<W_MN>()),
-                      desc_advance(bdesc, k * kUmmaK * 2), idesc, 1u);
-          }
-          umma_commit(&s.empty[stage]);
-          if (++stage == C::kStages) {
-            stage = 0;
-            phase ^= 1u;
-          }
-        }
-      }
       // Covers every UMMA above: the accumulator is complete, the ring is free.
       umma_commit(&s.done);
       mbar_drain(&s.done, 0);
     }
-  } else if (LORA && warp == 2) {
-    // ------------------------------------------------------------ the adapters' rows
-    if constexpr (LORA) {
-      pdl_wait();
-      const lora::TileList list(p.extra, row0 / BN);
-      const lora::RowAdapters<BN> rows(p.extra, row0, lane);
-      const uint32_t i1 = list.blocks * (rank + 1u) / p.splits;
-      uint32_t stage = (kb1 - kb0) % C::kStages, parity = 0;
-      for (uint32_t i = lane; i < kRows * kRowWords; i += 32u) (&spoilt[0][0])[i] = 0u;
-      __syncwarp();
-      bool any = false;
-      for (uint32_t i = list.blocks * rank / p.splits; i < i1; ++i) {
-        if (!__all_sync(0xffffffffu, mbar_wait(&landed[stage], (parity >> stage) & 1u, abort, kStatusTimeoutScales))) break;
-        uint32_t others[kRowWords], own[kRowWords];
-        rows.others(list.adapter(i), others);
-#pragma unroll
-        for (uint32_t k = 0; k < kRowWords; ++k) own[k] = ~others[k];
-        lora::zero_rows<BN>(s.x[stage], others, lane);
-        any |= lora::take_out_nonfinite(s.w[stage], min(kRows, p.cols - f0), min(64u, p.extra.rank - list.column(i)), spoilt,
-                                        own, lane);
-        fence_proxy_async_smem();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&s.full[stage]);
-        parity ^= 1u << stage;
-        stage = stage + 1u == C::kStages ? 0u : stage + 1u;
-      }
-      if (lane == 0) any_spoilt = any ? 1u : 0u;
-    }
   }
   __syncwarp();
-  const auto spoil = [&](float* v, uint32_t c0, uint32_t col) {  // 16 rows from c0 on
+
+  // LORA: which rows' adapters this block has computed.
+  constexpr uint32_t kRowWords = (BN + 31u) / 32u;
+  [[maybe_unused]] uint32_t added[kRowWords] = {};
+  if constexpr (LORA) {
+    if (warp >= 2u) {
+      lora::adapter_sums<BN, kRows>(p.extra, row0, f0, p.cols, rank, p.splits, warp - 2u, lane, added);
+      pdl_launch_dependents();
+      named_barrier_sync(2, 128);
+    }
+  }
+  // Adds what lora::adapter_sums has left to 16 rows from c0 on.
+  [[maybe_unused]] const auto add_adapters = [&](float (&v)[16], uint32_t c0, uint32_t f, bool valid) {
     if constexpr (LORA) {
-      const uint32_t word = spoilt[col][c0 / 32u] >> (c0 % 32u);
+      uint32_t word = added[0];
+#pragma unroll
+      for (uint32_t k = 1; k < kRowWords; ++k) word = c0 / 32u == k ? added[k] : word;
+      word = word >> (c0 % 32u) & 0xFFFFu;
+      if (word == 0u) return;
+      float d[16];
 #pragma unroll
       for (uint32_t j = 0; j < 16; ++j) {
-        if ((word >> j) & 1u) v[j] = __uint_as_float(0x7FC00000u);
+        d[j] = valid && ((word >> j) & 1u) != 0u ? __ldcg(p.extra.sums + size_t(row0 + c0 + j) * p.cols + f) : 0.f;
       }
+#pragma unroll
+      for (uint32_t j = 0; j < 16; ++j) v[j] += d[j];
     }
   };
-  bool spoiling = false;
-  if (LORA && warp >= 2u) {
-    pdl_wait();
-    pdl_launch_dependents();
-    named_barrier_sync(2, 128);  // warp 2's notes are complete
-    spoiling = any_spoilt != 0u;
-  }
 
   // ------------------------------------------------------------ epilogue
   const uint32_t q = warp & 3u;
@@ -403,7 +333,7 @@ __device__ __forceinline__ void linear_stream(const P& p) {
         float v[16];
 #pragma unroll
         for (uint32_t j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]) + bias;
-        if (LORA && spoiling) spoil(v, c0, fl);
+        add_adapters(v, c0, f, mine);
         if (p.epi.z != nullptr) {
           lin::store_columns(p.epi.z + row * p.epi.ldz + f, p.epi.ldz, v, rows - c0, mine, p.epi.pair_z);
         }
@@ -427,16 +357,12 @@ __device__ __forceinline__ void linear_stream(const P& p) {
         uint32_t r[16];
         tmem_ld_32x32b_x16(t_row + c0, r);
         tmem_ld_wait();
+        float v[16];
 #pragma unroll
-        for (uint32_t j = 0; j < 16; ++j) s.part[c0 + j][fl] = __uint_as_float(r[j]);
-        if (LORA && spoiling) {
-          float v[16];
+        for (uint32_t j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
+        add_adapters(v, c0, f, mine);
 #pragma unroll
-          for (uint32_t j = 0; j < 16; ++j) v[j] = __uint_as_float(r[j]);
-          spoil(v, c0, fl);
-#pragma unroll
-          for (uint32_t j = 0; j < 16; ++j) s.part[c0 + j][fl] = v[j];
-        }
+        for (uint32_t j = 0; j < 16; ++j) s.part[c0 + j][fl] = v[j];
       }
     }
     cluster_sync_all();

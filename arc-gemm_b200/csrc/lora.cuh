@@ -2,20 +2,23 @@
 //
 //   y[t] = act( x[t] w^T + bias + s_i (x[t] a_i^T) b_i^T ) + residual[t],   i = ids[t]
 //
-// The adapters' part is a longer contraction: row t's u[t] = s_i (x[t] a_i^T) follows x[t], and b_i's rows follow w's.
-// lora_down_kernel writes u, in bf16 (the tensor cores' operand type, one rounding), and for every row tile of
-// the product which adapters occur in it; the product (gemm_linear_stream.cuh, gemm_linear_pair.cuh) appends a block of
-// up to 64 of the rank per such adapter, which leaves the rows of other adapters alone (the pair kernel's by
-// tcgen05.mma's mask of output lanes, the streaming kernel's, whose lanes are columns, as zeros). So bias,
-// activation and residual stay where they are, nothing of the output's size is written twice, and the price of a
-// tile is its own adapters (a prompt's tile has one or two).
+// lora_down_kernel writes u[t] = s_i (x[t] a_i^T), in bf16 (the tensor cores' operand type, one rounding), and for every
+// row tile of the product which adapters occur in it. Then the product, with bias, activation and residual where they
+// were; nothing of the output's size passes through memory twice.
 //
-// lora_down_kernel. An item is one adapter of a block of 32 rows, the contraction split over a cluster of S
-// blocks and eight warps each. The rows that have the adapter are packed into tiles of 16 (a decode batch has one or
-// two per adapter), and both operands go from memory straight into the registers of mma.sync: a lane takes 16
-// bytes of a row, the same 8 of 32 of the contraction for rows and adapter, so no layout has to be met
-// in shared memory. Bound by the latency of those loads: a warp has one or two rounds of them. The partial sums
-// are added over warps, then over the cluster in rank order.
+// * Many rows (gemm_linear_pair.cuh): the adapters' part is a longer contraction. u follows x and b's rows follow w's, a
+//   block of up to 64 of the rank for each adapter of a tile, whose products leave the rows of other adapters as they
+//   are (tcgen05.mma's mask of output lanes). A prompt's tile has one adapter or two, which is what it pays.
+// * Few rows (gemm_linear_stream.cuh), where rows bring an adapter each and the output's lanes are columns: warps
+//   that wait for the stream of weights compute u b^T, adapter by adapter. As blocks of the contraction 25 rows
+//   with 21 adapters cost 38 us beside the stream's 25.
+//
+// lora_down_kernel. An item is a block of 32 rows times as many of its adapters as have 64 rows together, the contraction
+// split over a cluster of S blocks and eight warps each: warp i takes every eighth box of 64 by a ring slot
+// of its own. All 32 rows are multiplied by all the adapters (the pipe idles either way) and a row's own part kept.
+// Bound by latency for few rows, by the loads of x and the adapters from L2 for many. The partial sums are added over
+// warps, then over the cluster in rank order. (Straight from memory into registers, without the ring, 4096 rows of 4096
+// by rank 64 took 59 us.)
 #pragma once
 
 #include "sm100.cuh"
@@ -41,6 +44,10 @@ struct Extra {
   const uint16_t* lists;  // [row tiles][cap]: which, in the order of their first rows
   const void* ids;        // [rows]
   uint32_t ids_wide, adapters, rows, rank, cap;
+  // The streaming kernel's: u and b themselves, and where it leaves the adapters' sums.
+  const uint16_t *u, *b;
+  float* sums;  // [rows][N]
+  uint64_t ldu, ldb, b_stride;
 };
 
 // The adapters of a row tile, as blocks of 64 of the rank. For use behind griddepcontrol.wait.
@@ -81,72 +88,6 @@ struct RowAdapters {
   }
 };
 
-// One warp: zeros in the rows (128-byte lines) of an operand whose bit is set, whatever lies there.
-template <uint32_t ROWS>
-__device__ __forceinline__ void zero_rows(uint8_t* operand, const uint32_t (&mask)[(ROWS + 31u) / 32u], uint32_t lane) {
-#pragma unroll
-  for (uint32_t i = 0; i < (ROWS + 31u) / 32u; ++i) {
-#pragma unroll
-    for (uint32_t j = 0; j < 32u; j += 4u) {
-      const uint32_t r = j + (lane >> 3);
-      if (i * 32u + r < ROWS && ((mask[i] >> r) & 1u) != 0u) {
-        *reinterpret_cast<uint4*>(operand + (i * 32u + r) * 128u + (lane & 7u) * 16u) = make_uint4(0u, 0u, 0u, 0u);
-      }
-    }
-  }
-}
-
-// Rows of zeros keep other adapters' rows out of a product only if the adapter is finite: 0 times infinity is NaN, in
-// rows of requests that have nothing to do with it. One warp looks through `rows` rows of an adapter's block (swizzled
-// 128-byte lines, `cols` elements of each), sets what is not finite to zero, and notes in `spoilt` [row][words] that
-// the rows of x in `own` get NaN there. Returns whether there was any.
-template <uint32_t WORDS>
-__device__ __forceinline__ bool take_out_nonfinite(uint8_t* operand, uint32_t rows, uint32_t cols, uint32_t (*spoilt)[WORDS],
-                                                   const uint32_t (&own)[WORDS], uint32_t lane) {
-  const uint32_t pieces = (cols + 7u) / 8u;  // 16 bytes each
-  bool found = false;
-  for (uint32_t i = lane; i < rows * pieces; i += 32u) {
-    const uint32_t r = i / pieces, c = i % pieces;
-    uint4* at = reinterpret_cast<uint4*>(operand + r * 128u + ((c ^ (r & 7u)) << 4));
-    const uint4 v = *at;
-    uint32_t word[4] = {v.x, v.y, v.z, v.w};
-    bool bad = false;
-#pragma unroll
-    for (uint32_t k = 0; k < 4; ++k) {
-      if ((word[k] & 0x7F80u) == 0x7F80u) word[k] &= 0xFFFF0000u, bad = true;
-      if ((word[k] & 0x7F800000u) == 0x7F800000u) word[k] &= 0x0000FFFFu, bad = true;
-    }
-    if (bad) {
-      *at = make_uint4(word[0], word[1], word[2], word[3]);
-#pragma unroll
-      for (uint32_t k = 0; k < WORDS; ++k) atomicOr(&spoilt[r][k], own[k]);
-      found = true;
-    }
-  }
-  return __any_sync(0xffffffffu, found);
-}
-
-// ---------------------------------------------------------------------------------
-// lora_down_kernel
-// ---------------------------------------------------------------------------------
-constexpr uint32_t kDownWarps = 8;
-constexpr uint32_t kDownThreads = 32 * kDownWarps;
-constexpr uint32_t kDownRows = 32;  // rows of a block: one a lane
-
-struct DownParams {
-  const uint16_t* x;    // [M][ldx], 16-byte aligned rows
-  const uint16_t* a;    // [adapters] x a_stride, [rank][lda], 16-byte aligned rows
-  const float* scales;  // [adapters] or null
-  const void* ids;      // [M]
-  uint16_t* u;          // [M][ldu]
-  uint16_t *counts, *lists;
-  uint64_t ldx, lda, a_stride, ldu;
-  uint32_t ids_wide, adapters, M, K, rank;
-  uint32_t row_blocks, sets;       // blocks of rows; clusters that share a block's adapters
-  uint32_t rank_parts, splits;     // parts of 8 RT of the rank; blocks of a cluster
-  uint32_t tile_rows, tiles, cap;  // row tiles of the product
-};
-
 __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                             uint32_t b0, uint32_t b1) {
   asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
@@ -172,6 +113,153 @@ __device__ __forceinline__ uint32_t nth_bit(uint32_t mask, uint32_t n) {
   return mask == 0xFFFFFFFFu ? n : __fns(mask, 0, int(n) + 1);
 }
 
+// u b^T of a tile of ROWS rows and COLS columns, fp32, to `sums`, by four warps: an adapter each in turn, of the
+// adapters in the order of their first rows those with index `part` modulo `parts`. The rows of one adapter are
+// packed into tiles of 8, the columns are the 16 of mma.sync; operands go from memory straight into the registers, a
+// lane takes 16 bytes of a row, the same 8 of 32 of the rank for both. Beside a stream of weights a load takes
+// microseconds, so what does not depend on u is under way before u is there. Contains griddepcontrol.wait. `added`: the
+// rows that were written, a bit each.
+template <uint32_t ROWS, uint32_t COLS>
+__device__ __forceinline__ void adapter_sums(const Extra& e, uint32_t row0, uint32_t f0, uint32_t cols, uint32_t part,
+                                             uint32_t parts, uint32_t warp, uint32_t lane, uint32_t (&added)[(ROWS + 31u) / 32u]) {
+  constexpr uint32_t kSets = (ROWS + 31u) / 32u, kBlocks = COLS / 16u;
+  const uint32_t g8 = lane >> 2, q = lane & 3u;
+  const RowAdapters<ROWS> rows(e, row0, lane);
+  // Rows that are the first with their adapter, a bit each.
+  uint32_t firsts[kSets], n = 0;
+#pragma unroll
+  for (uint32_t k = 0; k < kSets; ++k) {
+    const uint32_t same = __match_any_sync(0xffffffffu, rows.id[k]);  // of all lanes, those without an adapter too
+    bool first = rows.id[k] != kNone && (same & ((1u << lane) - 1u)) == 0u;
+    if (k > 0) {
+#pragma unroll 1
+      for (uint32_t l = 0; l < 32u; ++l) {
+#pragma unroll
+        for (uint32_t j = 0; j < k; ++j) {
+          const uint32_t earlier = __shfl_sync(0xffffffffu, rows.id[j], l);  // of all lanes, whatever `first` is
+          if (earlier == rows.id[k]) first = false;
+        }
+      }
+    }
+    firsts[k] = __ballot_sync(0xffffffffu, first);
+    n += __popc(firsts[k]);
+  }
+  // The adapter with index i, and its rows.
+  const auto adapter_at = [&](uint32_t i, uint32_t (&own)[kSets]) {
+    uint32_t adapter = 0, left = i;
+#pragma unroll
+    for (uint32_t k = 0; k < kSets; ++k) {
+      const uint32_t here = __popc(firsts[k]);
+      if (left < here) adapter = __shfl_sync(0xffffffffu, rows.id[k], nth_bit(firsts[k], left));
+      left = left < here ? kNone : left == kNone ? kNone : left - here;
+    }
+    rows.others(adapter, own);
+#pragma unroll
+    for (uint32_t k = 0; k < kSets; ++k) own[k] = ~own[k];
+    return adapter;
+  };
+  for (uint32_t i = part; i < n; i += parts) {
+    uint32_t own[kSets];
+    const uint32_t adapter = adapter_at(i, own);
+#pragma unroll
+    for (uint32_t k = 0; k < kSets; ++k) added[k] |= own[k];
+    if ((i - part) / parts % 4u != warp) continue;
+    for (uint32_t f = lane; f < COLS && f0 + f < cols; f += 32u) {
+      const uint16_t* row = e.b + adapter * e.b_stride + size_t(f0 + f) * e.ldb;
+      for (uint32_t r = 0; r < e.rank; r += 64u) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + r));
+    }
+  }
+  bool waited = false;
+  for (uint32_t i = part + parts * warp; i < n; i += parts * 4u) {
+    uint32_t own[kSets], count = 0;
+    const uint16_t* b = e.b + adapter_at(i, own) * e.b_stride;
+#pragma unroll
+    for (uint32_t k = 0; k < kSets; ++k) count += __popc(own[k]);
+    const auto row_of = [&](uint32_t c) {
+      uint32_t r = 0, left = c;
+#pragma unroll
+      for (uint32_t k = 0; k < kSets; ++k) {
+        const uint32_t here = __popc(own[k]);
+        if (left < here) r = k * 32u + nth_bit(own[k], left);
+        left = left < here ? kNone : left == kNone ? kNone : left - here;
+      }
+      return row0 + r;
+    };
+    for (uint32_t c0 = 0; c0 < count; c0 += 8u) {
+      // This lane's row as an operand; later the two whose sums it holds.
+      const uint16_t* u = c0 + g8 < count ? e.u + size_t(row_of(c0 + g8)) * e.ldu : nullptr;
+      float acc[kBlocks][4];
+#pragma unroll
+      for (uint32_t m = 0; m < kBlocks; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+      for (uint32_t k = 0; k < e.rank; k += 32u) {
+        uint4 lo[kBlocks], hi[kBlocks];
+#pragma unroll
+        for (uint32_t m = 0; m < kBlocks; ++m) {
+          const uint32_t f = f0 + m * 16u + g8;
+          lo[m] = load8(f < cols ? b + size_t(f) * e.ldb : nullptr, k + q * 8u, e.rank);
+          hi[m] = load8(f + 8u < cols ? b + size_t(f + 8u) * e.ldb : nullptr, k + q * 8u, e.rank);
+        }
+        if (!waited) {
+          pdl_wait();
+          waited = true;
+        }
+        uint4 v = make_uint4(0u, 0u, 0u, 0u);
+        // Rows of u are padded to 16 bytes with zeros.
+        if (u != nullptr && k + q * 8u < e.rank) v = __ldcg(reinterpret_cast<const uint4*>(u + k + q * 8u));
+#pragma unroll
+        for (uint32_t m = 0; m < kBlocks; ++m) {
+          mma_16x8x16(acc[m], lo[m].x, hi[m].x, lo[m].y, hi[m].y, v.x, v.y);
+          mma_16x8x16(acc[m], lo[m].z, hi[m].z, lo[m].w, hi[m].w, v.z, v.w);
+        }
+      }
+#pragma unroll
+      for (uint32_t j = 0; j < 2; ++j) {
+        const uint32_t c = c0 + 2u * q + j;
+        if (c >= count) continue;
+        float* to = e.sums + size_t(row_of(c)) * cols + f0 + g8;
+#pragma unroll
+        for (uint32_t m = 0; m < kBlocks; ++m) {
+          if (f0 + m * 16u + g8 < cols) to[m * 16u] = acc[m][j];
+          if (f0 + m * 16u + g8 + 8u < cols) to[m * 16u + 8u] = acc[m][2 + j];
+        }
+      }
+    }
+  }
+  if (!waited) pdl_wait();
+}
+
+// ---------------------------------------------------------------------------------
+// lora_down_kernel
+// ---------------------------------------------------------------------------------
+constexpr uint32_t kDownWarps = 8;  // and one for the loads
+constexpr uint32_t kDownThreads = 32 * (kDownWarps + 1);
+constexpr uint32_t kDownRows = 32;  // rows of a block: one a lane
+constexpr uint32_t kDownCols = 64;  // rows of adapters
+constexpr uint32_t kDownXBytes = kDownRows * 128, kDownSlotBytes = kDownXBytes + kDownCols * 128;
+constexpr uint32_t kDownSmem = kDownWarps * kDownSlotBytes + 1024;
+static_assert(kDownWarps * kDownRows * kDownCols * 4 <= kDownWarps * kDownSlotBytes, "the sums reuse the ring");
+
+struct DownParams {
+  CUtensorMap tm_x;     // {K, M}, box {64, 32}, SW128
+  CUtensorMap tm_a;     // {K, rank, adapters}, box {64, RS, 1}, SW128
+  const float* scales;  // [adapters] or null
+  const void* ids;      // [M]
+  uint16_t* u;          // [M][ldu]
+  uint16_t *counts, *lists;  // null where the product streams
+  uint64_t ldu;
+  uint32_t ids_wide, adapters, M, K, rank;
+  uint32_t row_blocks, sets;       // blocks of rows; clusters that share a block's adapters
+  uint32_t rank_parts, splits;     // parts of 64 of the rank; blocks of a cluster
+  uint32_t tile_rows, tiles, cap;  // row tiles of the product
+};
+
+__device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3])
+               : "r"(addr)
+               : "memory");
+}
+
 // Which adapters occur in row tile t, in the order of their first rows. One warp; `seen` has a bit an adapter.
 __device__ __forceinline__ void list_tile(const DownParams& p, uint32_t t, uint32_t* seen, uint32_t lane) {
   seen[lane] = 0u;
@@ -193,18 +281,29 @@ __device__ __forceinline__ void list_tile(const DownParams& p, uint32_t t, uint3
   if (lane == 0) p.counts[t] = static_cast<uint16_t>(n);
 }
 
-// RT: tiles of 8 of the rank that a warp has; NW: groups of warps that share them out.
-template <uint32_t RT, uint32_t NW>
-__global__ void __launch_bounds__(kDownThreads) lora_down_kernel(const __grid_constant__ DownParams p) {
-  constexpr uint32_t KW = kDownWarps / NW;   // warps along the contraction
-  constexpr uint32_t kCols = RT * NW * 8;    // of the rank
-  constexpr uint32_t kAhead = RT >= 4 ? 2 : 4;  // chunks of 32 whose loads are under way together
-  __shared__ float sums[KW][kDownRows][kCols];
+// RS: rows that an adapter has among the 64.
+template <uint32_t RS>
+__global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid_constant__ DownParams p) {
+  constexpr uint32_t kGroup = kDownCols / RS;  // adapters of an item
+  extern __shared__ __align__(1024) uint8_t smem_raw[];
+  __shared__ uint64_t full[kDownWarps], empty[kDownWarps];
   __shared__ uint32_t seen[kMaxAdapters / 32];
-  const uint32_t warp = threadIdx.x >> 5, lane = threadIdx.x & 31u;
-  const uint32_t g8 = lane >> 2, q = lane & 3u;
-  const uint32_t kw = warp % KW, nw = warp / KW;
+  __shared__ uint32_t abort_flag;
+  uint8_t* ring = smem_raw + smem_align_pad(smem_raw);
+  const uint32_t warp = warp_idx_sync(), lane = threadIdx.x & 31u;
   const uint32_t rank = p.splits > 1u ? cluster_ctarank() : 0u;
+  volatile uint32_t* abort = &abort_flag;
+  if (threadIdx.x == 0) {
+    tma_prefetch_desc(&p.tm_x);
+    tma_prefetch_desc(&p.tm_a);
+    for (uint32_t i = 0; i < kDownWarps; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    abort_flag = 0;
+    fence_barrier_init();
+  }
+  __syncthreads();
   // The product's weights do not wait for this grid, so it lets the product in at once, but only after what
   // precedes it has ended.
   pdl_wait();
@@ -212,104 +311,158 @@ __global__ void __launch_bounds__(kDownThreads) lora_down_kernel(const __grid_co
 
   const uint32_t cluster = blockIdx.x / p.splits;
   const uint32_t set = cluster % p.sets, rest = cluster / p.sets;
-  const uint32_t r0 = rest % p.rank_parts * kCols, row0 = rest / p.rank_parts * kDownRows;
+  const uint32_t r0 = rest % p.rank_parts * kDownCols, row0 = rest / p.rank_parts * kDownRows;
   const uint32_t id = row0 + lane < p.M ? id_at(p.ids, p.ids_wide, p.adapters, row0 + lane) : kNone;
   const uint32_t same = __match_any_sync(0xffffffffu, id);
   const uint32_t leaders = __ballot_sync(0xffffffffu, id != kNone && (same & ((1u << lane) - 1u)) == 0u);
-  const uint32_t chunks = (p.K + 31u) / 32u;
-  const uint32_t c0 = chunks * rank / p.splits, c1 = chunks * (rank + 1u) / p.splits;
+  // This lane's row: the place of its adapter among the block's.
+  const uint32_t place = id == kNone ? kNone : __popc(leaders & ((1u << (__ffs(same) - 1)) - 1u));
+  const uint32_t distinct = __popc(leaders), boxes = (p.K + 63u) / 64u;
+  const uint32_t b0 = boxes * rank / p.splits, own = boxes * (rank + 1u) / p.splits - b0;
+  float* sums = reinterpret_cast<float*>(ring);  // [kDownWarps][kDownRows][kDownCols]
 
-  for (uint32_t n = set; n < uint32_t(__popc(leaders)); n += p.sets) {
-    const uint32_t lead = nth_bit(leaders, n);
-    const uint32_t adapter = __shfl_sync(0xffffffffu, id, lead), mask = __shfl_sync(0xffffffffu, same, lead);
-    const uint32_t count = __popc(mask);
-    // This lane's rows of x (g8 and 8 + g8 of up to two tiles) and of the adapter.
-    const uint16_t *xr[4], *ar[RT];
+  uint32_t uses = 0;  // of the ring slot: a consumer's by its warp, a loader's by its lane
+  bool ok = true;
+  for (uint32_t g = set * kGroup; g < distinct; g += p.sets * kGroup) {
+    const uint32_t adapters = min(kGroup, distinct - g);
+    float acc[2][kDownCols / 8][4];
+    if (warp == kDownWarps) {
+      // ---------------------------------------------------------- loads: lane i for warp i
+      uint32_t adapter[kGroup];
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) {
-      const uint32_t c = i * 8u + g8;
-      xr[i] = c < count ? p.x + (row0 + nth_bit(mask, c)) * p.ldx : nullptr;
-    }
-#pragma unroll
-    for (uint32_t i = 0; i < RT; ++i) {
-      const uint32_t r = r0 + (nw * RT + i) * 8u + g8;
-      ar[i] = r < p.rank ? p.a + adapter * p.a_stride + r * p.lda : nullptr;
-    }
-    float acc[2][RT][4];
-#pragma unroll
-    for (uint32_t m = 0; m < 2; ++m) {
-#pragma unroll
-      for (uint32_t i = 0; i < RT; ++i) acc[m][i][0] = acc[m][i][1] = acc[m][i][2] = acc[m][i][3] = 0.f;
-    }
-    const bool two = count > 16u;
-    for (uint32_t c = c0 + kw; c < c1; c += KW * kAhead) {
-      uint4 xv[kAhead][4], av[kAhead][RT];
-#pragma unroll
-      for (uint32_t h = 0; h < kAhead; ++h) {
-        const uint32_t k = c + h * KW < c1 ? (c + h * KW) * 32u + q * 8u : p.K;
-#pragma unroll
-        for (uint32_t i = 0; i < RT; ++i) av[h][i] = load8(ar[i], k, p.K);
-        xv[h][0] = load8(xr[0], k, p.K);
-        xv[h][1] = load8(xr[1], k, p.K);
-        xv[h][2] = two ? load8(xr[2], k, p.K) : make_uint4(0u, 0u, 0u, 0u);
-        xv[h][3] = two ? load8(xr[3], k, p.K) : make_uint4(0u, 0u, 0u, 0u);
+      for (uint32_t i = 0; i < kGroup; ++i) {
+        adapter[i] = __shfl_sync(0xffffffffu, id, i < adapters ? nth_bit(leaders, g + i) : 0u);
       }
+      if (lane < kDownWarps) {
+        uint8_t* slot = ring + lane * kDownSlotBytes;
+        for (uint32_t b = lane; ok && b < own; b += kDownWarps) {
+          ok = mbar_wait(&empty[lane], (uses & 1u) ^ 1u, abort, kStatusTimeoutProducer);
+          if (!ok) break;
+          mbar_arrive_expect_tx(&full[lane], kDownXBytes + adapters * RS * 128u);
+          const int32_t k = int32_t((b0 + b) * 64u);
+          tma_load_2d(&p.tm_x, &full[lane], slot, k, int32_t(row0), kCacheEvictNormal);
 #pragma unroll
-      for (uint32_t h = 0; h < kAhead; ++h) {
+          for (uint32_t i = 0; i < kGroup; ++i) {
+            if (i < adapters) {
+              tma_load_3d(&p.tm_a, &full[lane], slot + kDownXBytes + i * RS * 128u, k, int32_t(r0), int32_t(adapter[i]),
+                          kCacheEvictNormal);
+            }
+          }
+          ++uses;
+        }
+        // Loads land before the ring is used for the sums, and before the block may exit.
+        if (uses > 0u) mbar_drain(&full[lane], (uses - 1u) & 1u);
+      }
+      __syncwarp();
+    } else {
+      // ---------------------------------------------------------- products
 #pragma unroll
-        for (uint32_t m = 0; m < 2; ++m) {
-          if (m == 1 && !two) continue;
-          const uint4 lo = xv[h][2 * m], hi = xv[h][2 * m + 1];
+      for (uint32_t m = 0; m < 2; ++m) {
 #pragma unroll
-          for (uint32_t i = 0; i < RT; ++i) {
-            mma_16x8x16(acc[m][i], lo.x, hi.x, lo.y, hi.y, av[h][i].x, av[h][i].y);
-            mma_16x8x16(acc[m][i], lo.z, hi.z, lo.w, hi.w, av[h][i].z, av[h][i].w);
+        for (uint32_t j = 0; j < kDownCols / 8; ++j) acc[m][j][0] = acc[m][j][1] = acc[m][j][2] = acc[m][j][3] = 0.f;
+      }
+      const uint32_t x_at = smem_u32(ring + warp * kDownSlotBytes), a_at = x_at + kDownXBytes;
+      for (uint32_t b = warp; b < own; b += kDownWarps) {
+        if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[warp], uses & 1u, abort, kStatusTimeoutMma));
+        ++uses;
+        if (!ok) continue;
+#pragma unroll
+        for (uint32_t half = 0; half < 2; ++half) {  // 32 of the contraction
+          uint32_t xa[2][2][4];
+#pragma unroll
+          for (uint32_t m = 0; m < 2; ++m) {
+#pragma unroll
+            for (uint32_t k = 0; k < 2; ++k) {
+              const uint32_t row = m * 16u + (lane & 15u), chunk = half * 4u + k * 2u + (lane >> 4);
+              ldmatrix_x4(x_at + row * 128u + ((chunk ^ (row & 7u)) << 4), xa[m][k]);
+            }
+          }
+#pragma unroll
+          for (uint32_t i = 0; i < kGroup; ++i) {
+            if (i < adapters) {
+#pragma unroll
+              for (uint32_t j8 = 0; j8 < RS / 8; ++j8) {
+                const uint32_t j = i * (RS / 8) + j8;
+                uint32_t v[4];
+                const uint32_t row = lane & 7u, chunk = half * 4u + (lane >> 3);
+                ldmatrix_x4(a_at + (j * 8u + row) * 128u + ((chunk ^ row) << 4), v);
+#pragma unroll
+                for (uint32_t m = 0; m < 2; ++m) {
+#pragma unroll
+                  for (uint32_t k = 0; k < 2; ++k) {
+                    mma_16x8x16(acc[m][j], xa[m][k][0], xa[m][k][1], xa[m][k][2], xa[m][k][3], v[2 * k], v[2 * k + 1]);
+                  }
+                }
+              }
+            }
+          }
+        }
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&empty[warp]);
+      }
+    }
+    __syncthreads();  // the ring is free
+    if (warp < kDownWarps) {
+#pragma unroll
+      for (uint32_t m = 0; m < 2; ++m) {
+#pragma unroll
+        for (uint32_t j = 0; j < kDownCols / 8; ++j) {
+          if (j < adapters * (RS / 8)) {
+            float* to = sums + (warp * kDownRows + m * 16u + (lane >> 2)) * kDownCols + j * 8u + 2u * (lane & 3u);
+            *reinterpret_cast<float2*>(to) = make_float2(acc[m][j][0], acc[m][j][1]);
+            *reinterpret_cast<float2*>(to + 8 * kDownCols) = make_float2(acc[m][j][2], acc[m][j][3]);
           }
         }
       }
     }
-    // Warps, then blocks, in order.
-#pragma unroll
-    for (uint32_t m = 0; m < 2; ++m) {
-#pragma unroll
-      for (uint32_t i = 0; i < RT; ++i) {
-        float* to = &sums[kw][m * 16u + g8][(nw * RT + i) * 8u + 2u * q];
-        *reinterpret_cast<float2*>(to) = make_float2(acc[m][i][0], acc[m][i][1]);
-        *reinterpret_cast<float2*>(to + 8 * kCols) = make_float2(acc[m][i][2], acc[m][i][3]);
-      }
-    }
     __syncthreads();
-    float* mine = &sums[0][0][0];
-    for (uint32_t o = threadIdx.x; o < count * kCols; o += kDownThreads) {
-      float v = mine[o];
+    // A row's own adapter, over the warps, then over the blocks, in order. A warp has a row at a time.
+    for (uint32_t row = warp; row < kDownRows; row += kDownWarps + 1u) {
+      const uint32_t at = __shfl_sync(0xffffffffu, place, row) - g;  // wraps around for rows of other items
+      if (at >= adapters) continue;
+      for (uint32_t r = lane; r < RS; r += 32u) {
+        float* to = sums + row * kDownCols + at * RS + r;
+        float v = to[0];
 #pragma unroll
-      for (uint32_t k = 1; k < KW; ++k) v += mine[k * kDownRows * kCols + o];
-      mine[o] = v;
-    }
-    if (p.splits > 1u) {
-      cluster_sync_all();
-    } else {
-      __syncthreads();
-    }
-    const float scale = p.scales != nullptr ? __ldg(p.scales + adapter) : 1.f;
-    for (uint32_t o = threadIdx.x; o < count * kCols; o += kDownThreads) {
-      const uint32_t row = o / kCols, r = r0 + o % kCols;
-      if (row % p.splits != rank || r >= p.rank) continue;
-      float v = 0.f;
-      if (p.splits > 1u) {
-        for (uint32_t i = 0; i < p.splits; ++i) v += ld_dsmem_f32(map_to_rank(mine + o, i));
-      } else {
-        v = mine[o];
+        for (uint32_t k = 1; k < kDownWarps; ++k) v += to[k * kDownRows * kDownCols];
+        to[0] = v;
       }
-      p.u[(row0 + nth_bit(mask, row)) * p.ldu + r] = __bfloat16_as_ushort(__float2bfloat16_rn(scale * v));
     }
+    __syncwarp();
+    if (p.splits > 1u) cluster_sync_all();
+    for (uint32_t row = warp; row < kDownRows; row += kDownWarps + 1u) {
+      const uint32_t at = __shfl_sync(0xffffffffu, place, row) - g;
+      if (at >= adapters || row % p.splits != rank) continue;
+      const uint32_t adapter = __shfl_sync(0xffffffffu, id, row);
+      const float scale = p.scales != nullptr ? __ldg(p.scales + adapter) : 1.f;
+      for (uint32_t r = lane; r < RS; r += 32u) {
+        const float* from = sums + row * kDownCols + at * RS + r;
+        float v = 0.f;
+        if (p.splits > 1u) {
+          float all[8];  // on their way together
+#pragma unroll
+          for (uint32_t i = 0; i < 8; ++i) all[i] = ld_dsmem_f32(map_to_rank(from, min(i, p.splits - 1u)));
+#pragma unroll
+          for (uint32_t i = 0; i < 8; ++i) v += i < p.splits ? all[i] : 0.f;
+        } else {
+          v = *from;
+        }
+        // Zeros behind the rank, up to 16 bytes.
+        if (r0 + r < p.ldu) {
+          p.u[(row0 + row) * p.ldu + r0 + r] = __bfloat16_as_ushort(__float2bfloat16_rn(r0 + r < p.rank ? scale * v : 0.f));
+        }
+      }
+    }
+    fence_proxy_async_smem();  // the next item's loads come behind these accesses
     if (p.splits > 1u) {
-      cluster_sync_all();  // a peer may still be reading these sums
+      cluster_sync_all();  // a peer may still be reading this block's sums
     } else {
       __syncthreads();
     }
   }
-  for (uint32_t t = blockIdx.x; warp == 0 && t < p.tiles; t += gridDim.x) list_tile(p, t, seen, lane);
+  if (warp == 0 && p.lists != nullptr) {
+    for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x) list_tile(p, t, seen, lane);
+  }
 }
 
 }  // namespace lora

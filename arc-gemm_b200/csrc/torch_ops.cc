@@ -713,7 +713,7 @@ Tensor lora_linear(const Tensor& x_in, const Tensor& w_in, const Tensor& a_in, c
   const OptTensor bias_c = bias ? OptTensor(bias->contiguous()) : bias, scales_c = scales ? OptTensor(scales->contiguous()) : scales,
                   rows = residual ? OptTensor(unit_rows(*residual)) : residual;
   size_t bytes = 0;
-  check(g_api.lora_linear_ws(m, r, &bytes), "arc.lora_linear");
+  check(g_api.lora_linear_ws(m, n, k, r, &bytes), "arc.lora_linear");
   const Tensor workspace = at::empty({static_cast<int64_t>(bytes)}, options.dtype(at::kByte));
   check(g_api.lora_linear(u16(x), u16(w), u16(a), u16(b), ids.const_data_ptr(), static_cast<int>(ids.element_size()),
                           scales_c ? scales_c->const_data_ptr<float>() : nullptr, bias_c ? u16(*bias_c) : nullptr,

@@ -415,7 +415,7 @@ int arc_moe(const uint16_t *x, const void *w_in, const uint16_t *s_in, const voi
  *   out[m] = act( x[m] w^T + bias + s_i (x[m] a_i^T) b_i^T ) + residual[m],   i = ids[m]
  * bf16 with fp32 sums; s_i (x[m] a_i^T) is rounded to bf16 once, as an operand. A row whose id lies
  * outside [0, L) has no adapter. Only the adapters that occur are read, and what is not finite in one stays in
- * its own rows (where b has infinities they may come as NaN).
+ * its own rows.
  *   ids [M] signed integers of id_bytes 4 or 8;  a [L][R][lda], b [L][N][ldb], a_stride and b_stride elements
  *   between adapters;  scales [L] fp32 or NULL (all one);  the others as in arc_linear_bf16
  *   workspace    16-byte aligned, arc_lora_linear_workspace_bytes, no initialisation needed
@@ -423,7 +423,7 @@ int arc_moe(const uint16_t *x, const void *w_in, const uint16_t *s_in, const voi
  * are multiples of 8. Overlap as in arc_linear_bf16. Rows of one request side by side are fastest: a row
  * tile's time grows with the adapters in it.
  */
-int arc_lora_linear_workspace_bytes(int M, int R, size_t *bytes);
+int arc_lora_linear_workspace_bytes(int M, int N, int K, int R, size_t *bytes);
 int arc_lora_linear(const uint16_t *x, const uint16_t *w, const uint16_t *a, const uint16_t *b, const void *ids,
                     int id_bytes, const float *scales, const uint16_t *bias, const uint16_t *residual, uint16_t *out,
                     void *workspace, size_t workspace_bytes, int M, int N, int K, int R, int L, int64_t ldx, int64_t ldw,
