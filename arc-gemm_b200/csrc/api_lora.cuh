@@ -47,8 +47,10 @@ LoraWorkspace lora_workspace(uint32_t M, uint32_t N, uint32_t rank, const Linear
 // Rows that an adapter has among the 64 of an item.
 uint32_t lora_rows(uint32_t rank) { return rank <= 16 ? 16 : rank <= 32 ? 32 : 64; }
 
-// u and the row tiles' lists. The contraction is split until the blocks fill the GPU or a warp has one box; then
-// clusters share a block's adapters, of which there are 32 at most and in a prompt one or two.
+// u and the row tiles' lists. Clusters share a block's adapters, of which a mixed batch has up to 32 and a prompt one, two
+// where the next one begins: one cluster for both would make everyone wait for it (4096 rows of nine prompts, rank 64:
+// 33 us). The contraction is split until the blocks fill the GPU or a warp has one box, but only in four
+// from 5 blocks of rows on, so that a mixed batch finds clusters for its adapters.
 int lora_down(LO::DownParams& p, uint32_t sms, cudaStream_t stream) {
   const uint32_t rows = lora_rows(p.rank), group = LO::kDownCols / rows;
   p.row_blocks = ceil_div(p.M, LO::kDownRows);
@@ -56,10 +58,12 @@ int lora_down(LO::DownParams& p, uint32_t sms, cudaStream_t stream) {
   const uint32_t adapters = p.adapters < p.M ? p.adapters : p.M;
   const uint32_t bound = ceil_div(adapters < LO::kDownRows ? adapters : LO::kDownRows, group);  // items of a block
   const uint32_t items = p.row_blocks * p.rank_parts, most = 2 * sms, boxes = ceil_div(p.K, 64);
+  const uint32_t most_splits = p.row_blocks > 4 ? 4 : 8;
   p.splits = 1;
-  while (p.splits < 8 && items * p.splits * 2 <= most && boxes >= LO::kDownWarps * p.splits * 2) p.splits *= 2;
+  while (p.splits < most_splits && items * p.splits * 2 <= most && boxes >= LO::kDownWarps * p.splits * 2) p.splits *= 2;
   p.sets = most / (items * p.splits);
-  p.sets = p.sets < 1 ? 1 : p.sets < bound ? p.sets : bound;
+  p.sets = p.sets < 2 ? 2 : p.sets;
+  p.sets = p.sets < bound ? p.sets : bound;
   const uint64_t grid = uint64_t(items) * p.sets * p.splits;
   if (grid > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "too many rows for one launch");
   const auto kernel = rows == 16 ? LO::lora_down_kernel<16> : rows == 32 ? LO::lora_down_kernel<32> : LO::lora_down_kernel<64>;

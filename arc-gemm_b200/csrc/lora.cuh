@@ -96,16 +96,28 @@ __device__ __forceinline__ void mma_16x8x16(float (&d)[4], uint32_t a0, uint32_t
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// Eight elements of a row from k on, zeros behind the row's end and where there is no row.
-__device__ __forceinline__ uint4 load8(const uint16_t* row, uint32_t k, uint32_t K) {
-  if (row == nullptr || k >= K) return make_uint4(0u, 0u, 0u, 0u);
-  if (k + 8u <= K) return __ldg(reinterpret_cast<const uint4*>(row + k));
-  uint32_t v[4] = {0u, 0u, 0u, 0u};
+// Elements of a row by aligned vectors: where the row ends inside one, `keep` takes what lies behind it out (the vector
+// itself has an element of the row, so it is there to be read).
+template <uint32_t WORDS>
+struct Keep {
+  uint32_t mask[WORDS];
+  __device__ __forceinline__ Keep(uint32_t k, uint32_t end) {
 #pragma unroll
-  for (uint32_t i = 0; i < 8; ++i) {
-    if (k + i < K) v[i >> 1] |= static_cast<uint32_t>(__ldg(row + k + i)) << ((i & 1u) * 16u);
+    for (uint32_t i = 0; i < WORDS; ++i) {
+      mask[i] = (k + 2u * i < end ? 0x0000FFFFu : 0u) | (k + 2u * i + 1u < end ? 0xFFFF0000u : 0u);
+    }
   }
-  return make_uint4(v[0], v[1], v[2], v[3]);
+};
+__device__ __forceinline__ uint4 load8(const uint16_t* p, bool there, const Keep<4>& keep) {
+  uint4 v = make_uint4(0u, 0u, 0u, 0u);
+  // volatile: not to be moved behind a wait that it is meant to pass
+  if (there) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return make_uint4(v.x & keep.mask[0], v.y & keep.mask[1], v.z & keep.mask[2], v.w & keep.mask[3]);
+}
+__device__ __forceinline__ uint2 load4(const uint16_t* p, bool there, const Keep<2>& keep) {
+  uint2 v = make_uint2(0u, 0u);
+  if (there) asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return make_uint2(v.x & keep.mask[0], v.y & keep.mask[1]);
 }
 
 // The lane of the n-th set bit (n < popc).
@@ -116,7 +128,7 @@ __device__ __forceinline__ uint32_t nth_bit(uint32_t mask, uint32_t n) {
 // u b^T of a tile of ROWS rows and COLS columns, fp32, to `sums`, by four warps: an adapter each in turn, of the
 // adapters in the order of their first rows those with index `part` modulo `parts`. The rows of one adapter are
 // packed into tiles of 8, the columns are the 16 of mma.sync; operands go from memory straight into the registers, a
-// lane takes 16 bytes of a row, the same 8 of 32 of the rank for both. Beside a stream of weights a load takes
+// lane takes 16 bytes of a row (8 where the rank is 16), the same elements for both. Beside a stream of weights a load takes
 // microseconds, so what does not depend on u is under way before u is there. Contains griddepcontrol.wait. `added`: the
 // rows that were written, a bit each.
 template <uint32_t ROWS, uint32_t COLS>
@@ -132,7 +144,7 @@ __device__ __forceinline__ void adapter_sums(const Extra& e, uint32_t row0, uint
     const uint32_t same = __match_any_sync(0xffffffffu, rows.id[k]);  // of all lanes, those without an adapter too
     bool first = rows.id[k] != kNone && (same & ((1u << lane) - 1u)) == 0u;
     if (k > 0) {
-#pragma unroll 1
+#pragma unroll 1  // (an instruction that is not in the cache yet costs a short launch more than a loop does)
       for (uint32_t l = 0; l < 32u; ++l) {
 #pragma unroll
         for (uint32_t j = 0; j < k; ++j) {
@@ -169,59 +181,118 @@ __device__ __forceinline__ void adapter_sums(const Extra& e, uint32_t row0, uint
       for (uint32_t r = 0; r < e.rank; r += 64u) asm volatile("prefetch.global.L2 [%0];" ::"l"(row + r));
     }
   }
-  bool waited = false;
-  for (uint32_t i = part + parts * warp; i < n; i += parts * 4u) {
-    uint32_t own[kSets], count = 0;
-    const uint16_t* b = e.b + adapter_at(i, own) * e.b_stride;
+  const auto row_of = [&](const uint32_t (&own)[kSets], uint32_t c) {
+    uint32_t r = 0, left = c;
 #pragma unroll
-    for (uint32_t k = 0; k < kSets; ++k) count += __popc(own[k]);
-    const auto row_of = [&](uint32_t c) {
-      uint32_t r = 0, left = c;
+    for (uint32_t k = 0; k < kSets; ++k) {
+      const uint32_t here = __popc(own[k]);
+      if (left < here) r = k * 32u + nth_bit(own[k], left);
+      left = left < here ? kNone : left == kNone ? kNone : left - here;
+    }
+    return row0 + r;
+  };
+  // Sums of 8 rows from c0 on: this lane has two of them, in columns g8 and g8 + 8 of every 16.
+  const auto store = [&](const uint32_t (&own)[kSets], uint32_t c0, uint32_t count, const float (&acc)[kBlocks][4]) {
 #pragma unroll
-      for (uint32_t k = 0; k < kSets; ++k) {
-        const uint32_t here = __popc(own[k]);
-        if (left < here) r = k * 32u + nth_bit(own[k], left);
-        left = left < here ? kNone : left == kNone ? kNone : left - here;
+    for (uint32_t j = 0; j < 2; ++j) {
+      const uint32_t c = c0 + 2u * q + j;
+      if (c >= count) continue;
+      float* to = e.sums + size_t(row_of(own, c)) * cols + f0 + g8;
+#pragma unroll
+      for (uint32_t m = 0; m < kBlocks; ++m) {
+        if (f0 + m * 16u + g8 < cols) to[m * 16u] = acc[m][j];
+        if (f0 + m * 16u + g8 + 8u < cols) to[m * 16u + 8u] = acc[m][2 + j];
       }
-      return row0 + r;
-    };
-    for (uint32_t c0 = 0; c0 < count; c0 += 8u) {
-      // This lane's row as an operand; later the two whose sums it holds.
-      const uint16_t* u = c0 + g8 < count ? e.u + size_t(row_of(c0 + g8)) * e.ldu : nullptr;
-      float acc[kBlocks][4];
+    }
+  };
+  bool waited = false;
+  if (e.rank <= 16u && n > 4u * parts) {
+    // A rank of 16 is one step with four elements a lane, so that three adapters fit in the registers at once (32
+    // rows by 14336 x 4096, 21 adapters: 33.2 us one by one, 28.7 so).
+    constexpr uint32_t kAtOnce = 3;
+    const Keep<2> keep(q * 4u, e.rank);
+    const bool k_there = q * 4u < e.rank;
+    for (uint32_t i0 = part + parts * warp; i0 < n; i0 += parts * 4u * kAtOnce) {
+      uint32_t own[kAtOnce][kSets], count[kAtOnce];
+      uint2 lo[kAtOnce][kBlocks], hi[kAtOnce][kBlocks];
 #pragma unroll
-      for (uint32_t m = 0; m < kBlocks; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-      for (uint32_t k = 0; k < e.rank; k += 32u) {
-        uint4 lo[kBlocks], hi[kBlocks];
+      for (uint32_t h = 0; h < kAtOnce; ++h) {
+        const uint32_t i = i0 + h * parts * 4u;
+        count[h] = 0;
+        if (i >= n) continue;
+        const uint16_t* b = e.b + adapter_at(i, own[h]) * e.b_stride;
+#pragma unroll
+        for (uint32_t k = 0; k < kSets; ++k) count[h] += __popc(own[h][k]);
 #pragma unroll
         for (uint32_t m = 0; m < kBlocks; ++m) {
           const uint32_t f = f0 + m * 16u + g8;
-          lo[m] = load8(f < cols ? b + size_t(f) * e.ldb : nullptr, k + q * 8u, e.rank);
-          hi[m] = load8(f + 8u < cols ? b + size_t(f + 8u) * e.ldb : nullptr, k + q * 8u, e.rank);
-        }
-        if (!waited) {
-          pdl_wait();
-          waited = true;
-        }
-        uint4 v = make_uint4(0u, 0u, 0u, 0u);
-        // Rows of u are padded to 16 bytes with zeros.
-        if (u != nullptr && k + q * 8u < e.rank) v = __ldcg(reinterpret_cast<const uint4*>(u + k + q * 8u));
-#pragma unroll
-        for (uint32_t m = 0; m < kBlocks; ++m) {
-          mma_16x8x16(acc[m], lo[m].x, hi[m].x, lo[m].y, hi[m].y, v.x, v.y);
-          mma_16x8x16(acc[m], lo[m].z, hi[m].z, lo[m].w, hi[m].w, v.z, v.w);
+          lo[h][m] = load4(b + size_t(f) * e.ldb + q * 4u, k_there && f < cols, keep);
+          hi[h][m] = load4(b + size_t(f + 8u) * e.ldb + q * 4u, k_there && f + 8u < cols, keep);
         }
       }
-#pragma unroll
-      for (uint32_t j = 0; j < 2; ++j) {
-        const uint32_t c = c0 + 2u * q + j;
-        if (c >= count) continue;
-        float* to = e.sums + size_t(row_of(c)) * cols + f0 + g8;
-#pragma unroll
-        for (uint32_t m = 0; m < kBlocks; ++m) {
-          if (f0 + m * 16u + g8 < cols) to[m * 16u] = acc[m][j];
-          if (f0 + m * 16u + g8 + 8u < cols) to[m * 16u + 8u] = acc[m][2 + j];
+      if (!waited) {
+        pdl_wait();
+        waited = true;
+      }
+      uint2 v[kAtOnce];  // of the first 8 rows
+      const auto load_u = [&](uint32_t h, uint32_t c0) {
+        uint2 r = make_uint2(0u, 0u);
+        if (c0 + g8 < count[h] && q * 4u < e.ldu) {
+          r = __ldcg(reinterpret_cast<const uint2*>(e.u + size_t(row_of(own[h], c0 + g8)) * e.ldu + q * 4u));
         }
+        return r;
+      };
+#pragma unroll
+      for (uint32_t h = 0; h < kAtOnce; ++h) v[h] = load_u(h, 0u);
+#pragma unroll
+      for (uint32_t h = 0; h < kAtOnce; ++h) {
+        for (uint32_t c0 = 0; c0 < count[h]; c0 += 8u) {
+          if (c0 > 0u) v[h] = load_u(h, c0);
+          float acc[kBlocks][4];
+#pragma unroll
+          for (uint32_t m = 0; m < kBlocks; ++m) {
+            acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+            mma_16x8x16(acc[m], lo[h][m].x, hi[h][m].x, lo[h][m].y, hi[h][m].y, v[h].x, v[h].y);
+          }
+          store(own[h], c0, count[h], acc);
+        }
+      }
+    }
+  } else {
+    for (uint32_t i = part + parts * warp; i < n; i += parts * 4u) {
+      uint32_t own[kSets], count = 0;
+      const uint16_t* b = e.b + adapter_at(i, own) * e.b_stride;
+#pragma unroll
+      for (uint32_t k = 0; k < kSets; ++k) count += __popc(own[k]);
+      for (uint32_t c0 = 0; c0 < count; c0 += 8u) {
+        const uint16_t* u = c0 + g8 < count ? e.u + size_t(row_of(own, c0 + g8)) * e.ldu : nullptr;
+        float acc[kBlocks][4];
+#pragma unroll
+        for (uint32_t m = 0; m < kBlocks; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
+        for (uint32_t k = 0; k < e.rank; k += 32u) {
+          uint4 lo[kBlocks], hi[kBlocks];
+          const uint32_t kq = k + q * 8u;
+          const Keep<4> keep(kq, e.rank);
+#pragma unroll
+          for (uint32_t m = 0; m < kBlocks; ++m) {
+            const uint32_t f = f0 + m * 16u + g8;
+            lo[m] = load8(b + size_t(f) * e.ldb + kq, kq < e.rank && f < cols, keep);
+            hi[m] = load8(b + size_t(f + 8u) * e.ldb + kq, kq < e.rank && f + 8u < cols, keep);
+          }
+          if (!waited) {
+            pdl_wait();
+            waited = true;
+          }
+          uint4 v = make_uint4(0u, 0u, 0u, 0u);
+          // Rows of u are padded to 16 bytes with zeros.
+          if (u != nullptr && kq < e.rank) v = __ldcg(reinterpret_cast<const uint4*>(u + kq));
+#pragma unroll
+          for (uint32_t m = 0; m < kBlocks; ++m) {
+            mma_16x8x16(acc[m], lo[m].x, hi[m].x, lo[m].y, hi[m].y, v.x, v.y);
+            mma_16x8x16(acc[m], lo[m].z, hi[m].z, lo[m].w, hi[m].w, v.z, v.w);
+          }
+        }
+        store(own, c0, count, acc);
       }
     }
   }
@@ -262,20 +333,28 @@ __device__ __forceinline__ void ldmatrix_x4(uint32_t addr, uint32_t (&r)[4]) {
 
 // Which adapters occur in row tile t, in the order of their first rows. One warp; `seen` has a bit an adapter.
 __device__ __forceinline__ void list_tile(const DownParams& p, uint32_t t, uint32_t* seen, uint32_t lane) {
+  constexpr uint32_t kSets = 8;  // tiles have 256 rows at most; their ids are loaded together
+  const uint32_t first = t * p.tile_rows, end = min(p.M, first + p.tile_rows);
+  uint32_t ids[kSets];
+#pragma unroll
+  for (uint32_t i = 0; i < kSets; ++i) {
+    const uint32_t r = first + i * 32u + lane;
+    ids[i] = r < end ? id_at(p.ids, p.ids_wide, p.adapters, r) : kNone;
+  }
   seen[lane] = 0u;
   __syncwarp();
   uint32_t n = 0;
-  const uint32_t end = min(p.M, (t + 1u) * p.tile_rows);
-  for (uint32_t r0 = t * p.tile_rows; r0 < end; r0 += 32u) {
-    const uint32_t id = r0 + lane < end ? id_at(p.ids, p.ids_wide, p.adapters, r0 + lane) : kNone;
+#pragma unroll
+  for (uint32_t i = 0; i < kSets; ++i) {
+    const uint32_t id = ids[i];
     const uint32_t same = __match_any_sync(0xffffffffu, id);
-    const bool first = id != kNone && (same & ((1u << lane) - 1u)) == 0u && ((seen[id >> 5] >> (id & 31u)) & 1u) == 0u;
-    const uint32_t firsts = __ballot_sync(0xffffffffu, first);
-    if (first) {
-      p.lists[size_t(t) * p.cap + n + __popc(firsts & ((1u << lane) - 1u))] = static_cast<uint16_t>(id);
+    const bool is_new = id != kNone && (same & ((1u << lane) - 1u)) == 0u && ((seen[id >> 5] >> (id & 31u)) & 1u) == 0u;
+    const uint32_t news = __ballot_sync(0xffffffffu, is_new);
+    if (is_new) {
+      p.lists[size_t(t) * p.cap + n + __popc(news & ((1u << lane) - 1u))] = static_cast<uint16_t>(id);
       atomicOr(&seen[id >> 5], 1u << (id & 31u));
     }
-    n += __popc(firsts);
+    n += __popc(news);
     __syncwarp();
   }
   if (lane == 0) p.counts[t] = static_cast<uint16_t>(n);
@@ -321,6 +400,11 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
   const uint32_t b0 = boxes * rank / p.splits, own = boxes * (rank + 1u) / p.splits - b0;
   float* sums = reinterpret_cast<float*>(ring);  // [kDownWarps][kDownRows][kDownCols]
 
+  bool lists = p.lists != nullptr && warp == kDownWarps;  // still to be made
+  const auto make_lists = [&]() {
+    for (uint32_t t = blockIdx.x; lists && t < p.tiles; t += gridDim.x) list_tile(p, t, seen, lane);
+    lists = false;
+  };
   uint32_t uses = 0;  // of the ring slot: a consumer's by its warp, a loader's by its lane
   bool ok = true;
   for (uint32_t g = set * kGroup; g < distinct; g += p.sets * kGroup) {
@@ -350,9 +434,11 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
           }
           ++uses;
         }
-        // Loads land before the ring is used for the sums, and before the block may exit.
-        if (uses > 0u) mbar_drain(&full[lane], (uses - 1u) & 1u);
       }
+      __syncwarp();
+      make_lists();  // while the loads are on their way
+      // Loads land before the ring is used for the sums, and before the block may exit.
+      if (lane < kDownWarps && uses > 0u) mbar_drain(&full[lane], (uses - 1u) & 1u);
       __syncwarp();
     } else {
       // ---------------------------------------------------------- products
@@ -460,9 +546,7 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
       __syncthreads();
     }
   }
-  if (warp == 0 && p.lists != nullptr) {
-    for (uint32_t t = blockIdx.x; t < p.tiles; t += gridDim.x) list_tile(p, t, seen, lane);
-  }
+  make_lists();  // where a block had no adapters
 }
 
 }  // namespace lora
