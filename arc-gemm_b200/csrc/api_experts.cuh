@@ -27,13 +27,19 @@ struct ExpertForm {
   bool int4;
   uint32_t columns;
   ExpertVariant first, second;
+  ExpertVariant second_narrow;  // where the second's sums of all tokens do not fit
 };
 constexpr ExpertForm kExpertForms[] = {
-    {false, 8, expert_variant<8, 2, 2, false, false>(), expert_variant<8, 2, 2, false, true>()},
-    {false, 16, expert_variant<16, 2, 4, false, false>(), expert_variant<16, 2, 4, false, true>()},
-    {false, 32, expert_variant<32, 2, 4, false, false>(), expert_variant<32, 2, 2, false, true>()},
-    {true, 8, expert_variant<8, 4, 2, true, false>(), expert_variant<8, 4, 2, true, true>()},
-    {true, 16, expert_variant<16, 2, 4, true, false>(), expert_variant<16, 2, 2, true, true>()},
+    {false, 8, expert_variant<8, 2, 2, false, false>(), expert_variant<8, 2, 2, false, true>(),
+     expert_variant<8, 2, 2, false, true>()},
+    {false, 16, expert_variant<16, 2, 4, false, false>(), expert_variant<16, 2, 4, false, true>(),
+     expert_variant<16, 2, 2, false, true>()},
+    {false, 32, expert_variant<32, 2, 4, false, false>(), expert_variant<32, 2, 2, false, true>(),
+     expert_variant<32, 2, 2, false, true>()},
+    {true, 8, expert_variant<8, 4, 2, true, false>(), expert_variant<8, 4, 2, true, true>(),
+     expert_variant<8, 2, 2, true, true>()},
+    {true, 16, expert_variant<16, 2, 4, true, false>(), expert_variant<16, 2, 2, true, true>(),
+     expert_variant<16, 2, 2, true, true>()},
 };
 
 // Dynamic shared memory of a block: what the system and the kernel's own barriers take is off.
@@ -41,7 +47,7 @@ constexpr uint32_t kExpertSmemHalf = 112 * 1024, kExpertSmemWhole = 226 * 1024;
 
 int experts_init() {
   for (const ExpertForm& f : kExpertForms) {
-    for (const ExpertVariant* v : {&f.first, &f.second}) {
+    for (const ExpertVariant* v : {&f.first, &f.second, &f.second_narrow}) {
       const cudaError_t e = allow_smem(v->kernel, kExpertSmemWhole);
       if (e != cudaSuccess) {
         cudaGetLastError();  // clear
@@ -94,8 +100,8 @@ struct ExpertRing {
   uint32_t stages, smem, blocks_per_sm;
   bool own_y;
 };
-int expert_ring(const char* what, const ExpertVariant& v, bool second, uint32_t columns, uint32_t tokens, uint32_t slots,
-                uint32_t experts, ExpertRing* ring) {
+bool expert_ring(const ExpertVariant& v, bool second, uint32_t columns, uint32_t tokens, uint32_t slots, uint32_t experts,
+                 ExpertRing* ring) {
   ring->own_y = second && v.parts * v.rows * tokens * 4 <= 32 * 1024;
   const uint32_t rest =
       EX::layout_of(v.sum_bytes, v.parts, v.rows, columns, tokens, slots, experts, second, ring->own_y).total + 1024;
@@ -111,7 +117,7 @@ int expert_ring(const char* what, const ExpertVariant& v, bool second, uint32_t 
     ring->stages = stages(kExpertSmemWhole);
   }
   ring->smem = rest + ring->stages * v.stage_bytes;
-  return ring->stages > 0 ? ARC_OK : fail(ARC_ERR_UNSUPPORTED, "%s: does not fit in shared memory", what);
+  return ring->stages > 0;
 }
 
 // Weights of E experts as {bytes or elements of a row, rows, 2 (gate and up) or 1, E}.
@@ -218,15 +224,18 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   if (workspace == nullptr || !aligned16(workspace) || workspace_bytes < need) {
     return fail(ARC_ERR_INVALID_ARGUMENT, "%s: needs a 16-byte aligned workspace of %zu bytes", what, need);
   }
+  const ExpertVariant& v1 = plan.form->first;
+  const uint32_t columns = plan.form->columns;
+  ExpertRing first, second;
+  const bool narrow = !expert_ring(plan.form->second, true, columns, T, slots, E, &second);
+  const ExpertVariant& v2 = narrow ? plan.form->second_narrow : plan.form->second;
+  if ((narrow && !expert_ring(v2, true, columns, T, slots, E, &second)) ||
+      !expert_ring(v1, false, columns, T, slots, E, &first)) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: does not fit in shared memory", what);  // no sizes within the limits get here
+  }
   int dev = 0;
   if (int st = current_device(&dev, &DeviceState::experts_status)) return st;
   const uint32_t sms = static_cast<uint32_t>(g_dev[dev].sms);
-
-  const ExpertVariant &v1 = plan.form->first, &v2 = plan.form->second;
-  const uint32_t columns = plan.form->columns;
-  ExpertRing first, second;
-  if (int st = expert_ring(what, v1, false, columns, T, slots, E, &first)) return st;
-  if (int st = expert_ring(what, v2, true, columns, T, slots, E, &second)) return st;
 
   EX::Params p = {};
   p.ids = ids;

@@ -47,9 +47,9 @@ def _check(args, act, what="", **kw):
 # tokens, top, experts, K, I: one token and many, odd sizes, one expert, passes of an expert that run over,
 # contractions shorter than a box and no multiple of one.
 SHAPES = [(1, 1, 1, 64, 64), (1, 8, 64, 512, 256), (2, 2, 4, 8, 8), (5, 3, 10, 136, 72), (16, 8, 64, 256, 128),
-          (7, 1, 3, 1032, 520), (33, 4, 8, 200, 104), (100, 2, 3, 264, 136), (256, 8, 16, 128, 64), (3, 16, 1024, 72, 40)]
+          (7, 1, 3, 1032, 520), (33, 4, 8, 200, 104), (100, 2, 3, 264, 136), (256, 8, 16, 128, 64), (3, 16, 1024, 72, 40), (256, 16, 1024, 64, 32), (256, 8, 200, 136, 72)]
 SHAPES4 = [(1, 1, 1, 128, 128), (1, 8, 64, 512, 256), (5, 3, 10, 384, 128), (16, 8, 64, 256, 384), (33, 4, 8, 640, 128),
-           (100, 2, 3, 256, 128), (256, 8, 16, 128, 256)]
+           (100, 2, 3, 256, 128), (256, 8, 16, 128, 256), (256, 16, 600, 128, 128), (250, 4, 100, 256, 128)]
 
 
 @pytest.mark.parametrize("gated", [True, False])
