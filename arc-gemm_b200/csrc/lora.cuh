@@ -17,7 +17,8 @@
 // split over a cluster of S blocks and eight warps each: warp i takes every eighth box of 64 by a ring slot
 // of its own. All 32 rows are multiplied by all the adapters (the pipe idles either way) and a row's own part kept.
 // Bound by latency for few rows, by the loads of x and the adapters from L2 for many. The partial sums are added over
-// warps, then over the cluster in rank order. (Straight from memory into registers, without the ring, 4096 rows of 4096
+// warps, then sent to the block of the cluster that owns the row, which adds them in rank order (with cluster barriers
+// around reads of the peers' sums that took 4.3 us of the 8 of one token; sent, 1.5). (Straight from memory into registers, without the ring, 4096 rows of 4096
 // by rank 64 took 59 us.)
 #pragma once
 
@@ -307,7 +308,8 @@ constexpr uint32_t kDownThreads = 32 * (kDownWarps + 1);
 constexpr uint32_t kDownRows = 32;  // rows of a block: one a lane
 constexpr uint32_t kDownCols = 64;  // rows of adapters
 constexpr uint32_t kDownXBytes = kDownRows * 128, kDownSlotBytes = kDownXBytes + kDownCols * 128;
-constexpr uint32_t kDownSmem = kDownWarps * kDownSlotBytes + 1024;
+constexpr uint32_t kDownGotBytes = kDownRows * kDownCols * 4;
+constexpr uint32_t kDownSmem = kDownWarps * kDownSlotBytes + kDownGotBytes + 1024;
 static_assert(kDownWarps * kDownRows * kDownCols * 4 <= kDownWarps * kDownSlotBytes, "the sums reuse the ring");
 
 struct DownParams {
@@ -360,12 +362,17 @@ __device__ __forceinline__ void list_tile(const DownParams& p, uint32_t t, uint3
   if (lane == 0) p.counts[t] = static_cast<uint16_t>(n);
 }
 
+// One element of u, and zeros behind the rank, up to 16 bytes.
+__device__ __forceinline__ void store_u(const DownParams& p, uint32_t row, uint32_t r, float v) {
+  if (r < p.ldu) p.u[row * p.ldu + r] = __bfloat16_as_ushort(__float2bfloat16_rn(r < p.rank ? v : 0.f));
+}
+
 // RS: rows that an adapter has among the 64.
 template <uint32_t RS>
 __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid_constant__ DownParams p) {
   constexpr uint32_t kGroup = kDownCols / RS;  // adapters of an item
   extern __shared__ __align__(1024) uint8_t smem_raw[];
-  __shared__ uint64_t full[kDownWarps], empty[kDownWarps];
+  __shared__ uint64_t full[kDownWarps], empty[kDownWarps], got_all;
   __shared__ uint32_t seen[kMaxAdapters / 32];
   __shared__ uint32_t abort_flag;
   uint8_t* ring = smem_raw + smem_align_pad(smem_raw);
@@ -379,10 +386,12 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
+    mbar_init(&got_all, 1);
     abort_flag = 0;
     fence_barrier_init();
   }
   __syncthreads();
+  if (p.splits > 1u) cluster_arrive();  // this block is there, and its barriers
   // The product's weights do not wait for this grid, so it lets the product in at once, but only after what
   // precedes it has ended.
   pdl_wait();
@@ -399,12 +408,17 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
   const uint32_t distinct = __popc(leaders), boxes = (p.K + 63u) / 64u;
   const uint32_t b0 = boxes * rank / p.splits, own = boxes * (rank + 1u) / p.splits - b0;
   float* sums = reinterpret_cast<float*>(ring);  // [kDownWarps][kDownRows][kDownCols]
+  // What the cluster's blocks send this one, for the rows rank, rank + S, ...: [S][kDownRows / S][kDownCols].
+  float* got = reinterpret_cast<float*>(ring + kDownWarps * kDownSlotBytes);
+  // A scale is on its way before it is needed.
+  const float scale = id != kNone && p.scales != nullptr ? __ldg(p.scales + id) : 1.f;
 
   bool lists = p.lists != nullptr && warp == kDownWarps;  // still to be made
   const auto make_lists = [&]() {
     for (uint32_t t = blockIdx.x; lists && t < p.tiles; t += gridDim.x) list_tile(p, t, seen, lane);
     lists = false;
   };
+  uint32_t parity = 0;
   uint32_t uses = 0;  // of the ring slot: a consumer's by its warp, a loader's by its lane
   bool ok = true;
   for (uint32_t g = set * kGroup; g < distinct; g += p.sets * kGroup) {
@@ -502,50 +516,60 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
       }
     }
     __syncthreads();
-    // A row's own adapter, over the warps, then over the blocks, in order. A warp has a row at a time.
+    // A row's own adapter: a warp has a row at a time and adds the warps' sums.
+    const bool last = g + p.sets * kGroup >= distinct;
+    const uint32_t per = kDownRows / p.splits;
+    uint32_t mine = 0;  // rows of this block that others send sums for
+    if (p.splits > 1u) {
+      if (g == set * kGroup) cluster_wait();
+      for (uint32_t row = rank; row < kDownRows; row += p.splits) {
+        if (__shfl_sync(0xffffffffu, place, row) - g < adapters) ++mine;
+      }
+      if (threadIdx.x == 0) mbar_arrive_expect_tx(&got_all, mine * RS * 4u * p.splits);
+    }
     for (uint32_t row = warp; row < kDownRows; row += kDownWarps + 1u) {
       const uint32_t at = __shfl_sync(0xffffffffu, place, row) - g;  // wraps around for rows of other items
+      const float row_scale = __shfl_sync(0xffffffffu, scale, row);
       if (at >= adapters) continue;
       for (uint32_t r = lane; r < RS; r += 32u) {
-        float* to = sums + row * kDownCols + at * RS + r;
-        float v = to[0];
-#pragma unroll
-        for (uint32_t k = 1; k < kDownWarps; ++k) v += to[k * kDownRows * kDownCols];
-        to[0] = v;
-      }
-    }
-    __syncwarp();
-    if (p.splits > 1u) cluster_sync_all();
-    for (uint32_t row = warp; row < kDownRows; row += kDownWarps + 1u) {
-      const uint32_t at = __shfl_sync(0xffffffffu, place, row) - g;
-      if (at >= adapters || row % p.splits != rank) continue;
-      const uint32_t adapter = __shfl_sync(0xffffffffu, id, row);
-      const float scale = p.scales != nullptr ? __ldg(p.scales + adapter) : 1.f;
-      for (uint32_t r = lane; r < RS; r += 32u) {
         const float* from = sums + row * kDownCols + at * RS + r;
-        float v = 0.f;
+        float v = from[0];
+#pragma unroll
+        for (uint32_t k = 1; k < kDownWarps; ++k) v += from[k * kDownRows * kDownCols];
         if (p.splits > 1u) {
-          float all[8];  // on their way together
-#pragma unroll
-          for (uint32_t i = 0; i < 8; ++i) all[i] = ld_dsmem_f32(map_to_rank(from, min(i, p.splits - 1u)));
-#pragma unroll
-          for (uint32_t i = 0; i < 8; ++i) v += i < p.splits ? all[i] : 0.f;
+          const uint32_t owner = row % p.splits;
+          store_async(map_to_rank(got + (rank * per + row / p.splits) * kDownCols + r, owner), v, map_to_rank(&got_all, owner));
         } else {
-          v = *from;
-        }
-        // Zeros behind the rank, up to 16 bytes.
-        if (r0 + r < p.ldu) {
-          p.u[(row0 + row) * p.ldu + r0 + r] = __bfloat16_as_ushort(__float2bfloat16_rn(r0 + r < p.rank ? scale * v : 0.f));
+          store_u(p, row0 + row, r0 + r, row_scale * v);
         }
       }
     }
-    fence_proxy_async_smem();  // the next item's loads come behind these accesses
     if (p.splits > 1u) {
-      cluster_sync_all();  // a peer may still be reading this block's sums
-    } else {
-      __syncthreads();
+      // All that is sent here lands before this block may exit, whatever has been abandoned: a peer's sums may come after
+      // the limits of its own waits.
+      if (mine > 0u || !last) mbar_drain(&got_all, parity, 4u * kWaitTimeoutNs);
+      parity ^= 1u;
+      for (uint32_t row = warp * p.splits + rank; row < kDownRows; row += (kDownWarps + 1u) * p.splits) {
+        const uint32_t at = __shfl_sync(0xffffffffu, place, row) - g;
+        const float row_scale = __shfl_sync(0xffffffffu, scale, row);
+        if (at >= adapters) continue;
+        for (uint32_t r = lane; r < RS; r += 32u) {
+          float v = 0.f;
+          for (uint32_t i = 0; i < p.splits; ++i) v += got[(i * per + row / p.splits) * kDownCols + r];
+          store_u(p, row0 + row, r0 + r, row_scale * v);
+        }
+      }
+    }
+    if (!last) {
+      fence_proxy_async_smem();  // the next item's loads come behind these accesses
+      if (p.splits > 1u) {
+        cluster_sync_all();  // and its sums behind the reads of these
+      } else {
+        __syncthreads();
+      }
     }
   }
+  if (p.splits > 1u && set * kGroup >= distinct) cluster_wait();  // of the arrival above
   make_lists();  // where a block had no adapters
 }
 

@@ -331,12 +331,12 @@ __device__ __forceinline__ void regs_claim() {
 
 // Bounded wait that ignores the abort flag: used on the teardown path to let
 // copies already in flight land before the CTA exits.
-__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity) {
+__device__ __forceinline__ bool mbar_drain(uint64_t* bar, uint32_t parity, uint64_t limit_ns = kWaitTimeoutNs) {
   const uint32_t addr = smem_u32(bar);
   const uint64_t start = globaltimer_ns();
 #pragma unroll 1
   while (!mbar_try_wait(addr, parity)) {
-    if (globaltimer_ns() - start > kWaitTimeoutNs) {
+    if (globaltimer_ns() - start > limit_ns) {
       atomicOr(&g_arc_status, kStatusTimeoutDrain);
       return false;
     }
@@ -664,6 +664,14 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
   float v;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
   return v;
+}
+
+// One float into the shared memory of a CTA of the cluster, whose barrier there counts its four bytes (both addresses from
+// map_to_rank, of the same CTA).
+__device__ __forceinline__ void store_async(uint32_t dst, float v, uint32_t remote_bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(dst),
+               "r"(__float_as_uint(v)), "r"(remote_bar)
+               : "memory");
 }
 
 // Bulk copy of `bytes` (a multiple of 16) from this CTA's shared memory into the
