@@ -58,12 +58,13 @@ int lora_down(LO::DownParams& p, uint32_t sms, cudaStream_t stream) {
   const uint32_t adapters = p.adapters < p.M ? p.adapters : p.M;
   const uint32_t bound = ceil_div(adapters < LO::kDownRows ? adapters : LO::kDownRows, group);  // items of a block
   const uint32_t items = p.row_blocks * p.rank_parts, most = 2 * sms, boxes = ceil_div(p.K, 64);
-  const uint32_t most_splits = p.row_blocks > 4 ? 4 : 8;
+  const uint32_t most_splits = p.row_blocks > 4 ? 4 : 8, least_sets = bound < 2 ? bound : 2;
   p.splits = 1;
-  while (p.splits < most_splits && items * p.splits * 2 <= most && boxes >= LO::kDownWarps * p.splits * 2) p.splits *= 2;
+  while (p.splits < most_splits && items * least_sets * p.splits * 2 <= most && boxes >= LO::kDownWarps * p.splits * 2) {
+    p.splits *= 2;
+  }
   p.sets = most / (items * p.splits);
-  p.sets = p.sets < 2 ? 2 : p.sets;
-  p.sets = p.sets < bound ? p.sets : bound;
+  p.sets = p.sets < least_sets ? least_sets : p.sets < bound ? p.sets : bound;
   const uint64_t grid = uint64_t(items) * p.sets * p.splits;
   if (grid > 0x7FFFFFFFu) return fail(ARC_ERR_UNSUPPORTED, "too many rows for one launch");
   const auto kernel = rows == 16 ? LO::lora_down_kernel<16> : rows == 32 ? LO::lora_down_kernel<32> : LO::lora_down_kernel<64>;

@@ -362,9 +362,13 @@ __device__ __forceinline__ void list_tile(const DownParams& p, uint32_t t, uint3
   if (lane == 0) p.counts[t] = static_cast<uint16_t>(n);
 }
 
-// One element of u, and zeros behind the rank, up to 16 bytes.
-__device__ __forceinline__ void store_u(const DownParams& p, uint32_t row, uint32_t r, float v) {
-  if (r < p.ldu) p.u[row * p.ldu + r] = __bfloat16_as_ushort(__float2bfloat16_rn(r < p.rank ? v : 0.f));
+// Four elements of u, zeros behind the rank.
+__device__ __forceinline__ void store_u(const DownParams& p, uint32_t row, uint32_t r, float scale, const float4& v) {
+  if (r >= p.ldu) return;
+  uint2 w;
+  w.x = pack_bf16x2(r < p.rank ? scale * v.x : 0.f, r + 1u < p.rank ? scale * v.y : 0.f);
+  w.y = pack_bf16x2(r + 2u < p.rank ? scale * v.z : 0.f, r + 3u < p.rank ? scale * v.w : 0.f);
+  *reinterpret_cast<uint2*>(p.u + row * p.ldu + r) = w;
 }
 
 // RS: rows that an adapter has among the 64.
@@ -413,9 +417,10 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
   // A scale is on its way before it is needed.
   const float scale = id != kNone && p.scales != nullptr ? __ldg(p.scales + id) : 1.f;
 
-  bool lists = p.lists != nullptr && warp == kDownWarps;  // still to be made
+  // The row tiles' lists are made by blocks that seldom have an adapter to work on.
+  bool lists = p.lists != nullptr && warp == kDownWarps && rank == 0u && set + 1u == p.sets;
   const auto make_lists = [&]() {
-    for (uint32_t t = blockIdx.x; lists && t < p.tiles; t += gridDim.x) list_tile(p, t, seen, lane);
+    for (uint32_t t = rest; lists && t < p.tiles; t += p.row_blocks * p.rank_parts) list_tile(p, t, seen, lane);
     lists = false;
   };
   uint32_t parity = 0;
@@ -516,31 +521,34 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
       }
     }
     __syncthreads();
-    // A row's own adapter: a warp has a row at a time and adds the warps' sums.
+    // A row's own adapter, four of its rank a lane: the warps' sums are added and sent to the row's owner.
+    constexpr uint32_t kLanes = RS / 4u, kRowsAtOnce = 32u / kLanes;
+    const uint32_t r4 = lane % kLanes * 4u;
     const bool last = g + p.sets * kGroup >= distinct;
     const uint32_t per = kDownRows / p.splits;
     uint32_t mine = 0;  // rows of this block that others send sums for
     if (p.splits > 1u) {
       if (g == set * kGroup) cluster_wait();
-      for (uint32_t row = rank; row < kDownRows; row += p.splits) {
-        if (__shfl_sync(0xffffffffu, place, row) - g < adapters) ++mine;
-      }
+      mine = __popc(__ballot_sync(0xffffffffu, place - g < adapters && lane % p.splits == rank));
       if (threadIdx.x == 0) mbar_arrive_expect_tx(&got_all, mine * RS * 4u * p.splits);
     }
-    for (uint32_t row = warp; row < kDownRows; row += kDownWarps + 1u) {
+    for (uint32_t first = warp * kRowsAtOnce; first < kDownRows; first += (kDownWarps + 1u) * kRowsAtOnce) {
+      const uint32_t row = first + lane / kLanes;
       const uint32_t at = __shfl_sync(0xffffffffu, place, row) - g;  // wraps around for rows of other items
       const float row_scale = __shfl_sync(0xffffffffu, scale, row);
-      if (at >= adapters) continue;
-      for (uint32_t r = lane; r < RS; r += 32u) {
-        const float* from = sums + row * kDownCols + at * RS + r;
-        float v = from[0];
+      if (at < adapters) {
+        const float* from = sums + row * kDownCols + at * RS + r4;
+        float4 v = *reinterpret_cast<const float4*>(from);
 #pragma unroll
-        for (uint32_t k = 1; k < kDownWarps; ++k) v += from[k * kDownRows * kDownCols];
+        for (uint32_t k = 1; k < kDownWarps; ++k) {
+          const float4 o = *reinterpret_cast<const float4*>(from + k * kDownRows * kDownCols);
+          v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+        }
         if (p.splits > 1u) {
           const uint32_t owner = row % p.splits;
-          store_async(map_to_rank(got + (rank * per + row / p.splits) * kDownCols + r, owner), v, map_to_rank(&got_all, owner));
+          store_async(map_to_rank(got + (rank * per + row / p.splits) * kDownCols + r4, owner), v, map_to_rank(&got_all, owner));
         } else {
-          store_u(p, row0 + row, r0 + r, row_scale * v);
+          store_u(p, row0 + row, r0 + r4, row_scale, v);
         }
       }
     }
@@ -549,14 +557,17 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
       // the limits of its own waits.
       if (mine > 0u || !last) mbar_drain(&got_all, parity, 4u * kWaitTimeoutNs);
       parity ^= 1u;
-      for (uint32_t row = warp * p.splits + rank; row < kDownRows; row += (kDownWarps + 1u) * p.splits) {
+      for (uint32_t first = warp * kRowsAtOnce; first < per; first += (kDownWarps + 1u) * kRowsAtOnce) {
+        const uint32_t i = first + lane / kLanes, row = i < per ? i * p.splits + rank : 0u;
         const uint32_t at = __shfl_sync(0xffffffffu, place, row) - g;
         const float row_scale = __shfl_sync(0xffffffffu, scale, row);
-        if (at >= adapters) continue;
-        for (uint32_t r = lane; r < RS; r += 32u) {
-          float v = 0.f;
-          for (uint32_t i = 0; i < p.splits; ++i) v += got[(i * per + row / p.splits) * kDownCols + r];
-          store_u(p, row0 + row, r0 + r, row_scale * v);
+        if (i < per && at < adapters) {
+          float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+          for (uint32_t k = 0; k < p.splits; ++k) {
+            const float4 o = *reinterpret_cast<const float4*>(got + (k * per + i) * kDownCols + r4);
+            v = make_float4(v.x + o.x, v.y + o.y, v.z + o.z, v.w + o.w);
+          }
+          store_u(p, row0 + row, r0 + r4, row_scale, v);
         }
       }
     }

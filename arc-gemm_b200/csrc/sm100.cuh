@@ -666,11 +666,12 @@ __device__ __forceinline__ float ld_dsmem_f32(uint32_t addr) {
   return v;
 }
 
-// One float into the shared memory of a CTA of the cluster, whose barrier there counts its four bytes (both addresses from
+// Four floats into the shared memory of a CTA of the cluster, whose barrier there counts the 16 bytes (both addresses from
 // map_to_rank, of the same CTA).
-__device__ __forceinline__ void store_async(uint32_t dst, float v, uint32_t remote_bar) {
-  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.b32 [%0], %1, [%2];" ::"r"(dst),
-               "r"(__float_as_uint(v)), "r"(remote_bar)
+__device__ __forceinline__ void store_async(uint32_t dst, const float4& v, uint32_t remote_bar) {
+  asm volatile("st.async.weak.shared::cluster.mbarrier::complete_tx::bytes.v4.b32 [%0], {%1, %2, %3, %4}, [%5];" ::"r"(dst),
+               "r"(__float_as_uint(v.x)), "r"(__float_as_uint(v.y)), "r"(__float_as_uint(v.z)), "r"(__float_as_uint(v.w)),
+               "r"(remote_bar)
                : "memory");
 }
 
