@@ -27,9 +27,8 @@
 //   its blocks' sums in rank order. The result does not depend on timing.
 //
 // Sums are fp32. h is rounded to bf16, the tensor cores' operand type, and the weights of the choices multiply
-// fp32 sums. Codes of int4 weights enter as code + 136, which is what a nibble costs fewest instructions as, and
-// 136 times the group's sum of x, which the tensor cores give beside it, is taken off in fp32 before the scale: at
-// most 2^-14 of the group's largest |x| goes to the tensor cores' fp32 sums that way, where 2^-8 of h is rounded.
+// fp32 sums. Codes of int4 weights enter as code + 8, exactly, and 8 times the group's sum of x, which the tensor cores give
+// beside it, is taken off in fp32 before the scale is applied.
 #pragma once
 
 #include "linear_common.cuh"
@@ -159,16 +158,29 @@ __device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint3
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(0.f));
 }
 
-// Eight int4 codes (k = 0..7 from the low nibble up) as bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7) of code + 136:
-// 0x4300 | m is the bf16 128 + m, and a code's nibble with its sign bit turned over is code + 8.
+// Eight int4 codes (k = 0..7 from the low nibble up) as bf16 pairs (0, 4), (1, 5), (2, 6), (3, 7). A nibble with its sign
+// bit turned over is code + 8, and as the lowest bits of a bf16 it is that many units of 2^-133: below 2^-125 the bits
+// of a bf16 are an integer. So a mask is all that the even pairs cost; the odd ones, four bits further up, come as 16 times as
+// much, for which their x is 16 times smaller. (Nibbles moved to a place of their own in the mantissa of 128 + n took two
+// instructions more for eight codes, 7 instead of 5, on the pipe that bounds the kernel.)
 __device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t (&v)[4]) {
-#pragma unroll
-  for (uint32_t i = 0; i < 4; ++i) {
-    asm("lop3.b32 %0, %1, 0x000F000F, 0x43084308, 0x6A;" : "=r"(v[i]) : "r"(w >> (4 * i)));  // (a & b) ^ c
-  }
+  const uint32_t u = w >> 8;
+  asm("lop3.b32 %0, %1, 0x000F000F, 0x00080008, 0x6A;" : "=r"(v[0]) : "r"(w));  // (a & b) ^ c
+  asm("lop3.b32 %0, %1, 0x00F000F0, 0x00800080, 0x6A;" : "=r"(v[1]) : "r"(w));
+  asm("lop3.b32 %0, %1, 0x000F000F, 0x00080008, 0x6A;" : "=r"(v[2]) : "r"(u));
+  asm("lop3.b32 %0, %1, 0x00F000F0, 0x00800080, 0x6A;" : "=r"(v[3]) : "r"(u));
 }
-constexpr float kCodeBias = 136.f;
-constexpr uint32_t kOnes = 0x3F803F80u;  // two bf16 ones
+// The eights that come with the codes, as codes of zero: what they add is taken off again.
+constexpr uint32_t kEightEven = 0x00080008u, kEightOdd = 0x00800080u;
+// x is multiplied by 2^64 (even pairs) and 2^60, so that products of codes are normal fp32 numbers, and the sums are in
+// units of 2^-69. |x| must be below 2^63.
+constexpr uint32_t kScaleEven = 0x5F805F80u, kScaleOdd = 0x5D805D80u;  // two bf16 each
+constexpr float kCodeUnit = 590295810358705651712.f;                   // 2^69
+__device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
 
 // ---------------------------------------------------------------------------------
 // The choices, sorted by expert in shared memory by the whole block: `list` holds the choices of
@@ -301,7 +313,7 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
     // take the rows r and r + 4, whose halves of 128 swizzled bytes lie in different banks; so column n of a
     // product is row perm(n).
     const uint32_t perm = (g8 >> 1) | (g8 & 1u) << 2;
-    float part_sum[MR][J][4], x_sum[J][4];  // over the group: of (code + 136) x, and of x
+    float part_sum[MR][J][4], x_sum[J][4];  // over the group: of (code + 8) x, and of 8 x
 #pragma unroll
     for (uint32_t c = 0; c < 4; ++c) {  // 32 codes of a row, 16 bytes
       uint32_t b[J][4];  // pairs of k: (0, 4), (1, 5), (2, 6), (3, 7) of a lane's eight, as the codes come
@@ -309,16 +321,16 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
       for (uint32_t j = 0; j < J; ++j) {
         uint32_t x[4];
         lds_128(x_at + (c >> 1) * XBYTES + (j * 8u + perm) * kRowBytes + ((((c & 1u) * 4u + q) ^ perm) << 4), x);
-        b[j][0] = __byte_perm(x[0], x[2], 0x5410);
-        b[j][1] = __byte_perm(x[0], x[2], 0x7632);
-        b[j][2] = __byte_perm(x[1], x[3], 0x5410);
-        b[j][3] = __byte_perm(x[1], x[3], 0x7632);
+        b[j][0] = mul_bf16x2(__byte_perm(x[0], x[2], 0x5410), kScaleEven);
+        b[j][1] = mul_bf16x2(__byte_perm(x[0], x[2], 0x7632), kScaleOdd);
+        b[j][2] = mul_bf16x2(__byte_perm(x[1], x[3], 0x5410), kScaleEven);
+        b[j][3] = mul_bf16x2(__byte_perm(x[1], x[3], 0x7632), kScaleOdd);
         if (c == 0) {
-          mma_bf16_first(x_sum[j], kOnes, kOnes, kOnes, kOnes, b[j][0], b[j][1]);
+          mma_bf16_first(x_sum[j], kEightEven, kEightEven, kEightOdd, kEightOdd, b[j][0], b[j][1]);
         } else {
-          mma_bf16(x_sum[j], kOnes, kOnes, kOnes, kOnes, b[j][0], b[j][1]);
+          mma_bf16(x_sum[j], kEightEven, kEightEven, kEightOdd, kEightOdd, b[j][0], b[j][1]);
         }
-        mma_bf16(x_sum[j], kOnes, kOnes, kOnes, kOnes, b[j][2], b[j][3]);
+        mma_bf16(x_sum[j], kEightEven, kEightEven, kEightOdd, kEightOdd, b[j][2], b[j][3]);
       }
 #pragma unroll
       for (uint32_t m2 = 0; m2 < MR; m2 += 2) {
@@ -350,8 +362,7 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
       for (uint32_t j = 0; j < J; ++j) {
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-          const float v = fmaf(-kCodeBias, x_sum[j][i & 1u], part_sum[m][j][i]);
-          acc[m][j][i] = fmaf(i < 2 ? s0 : s1, v, acc[m][j][i]);
+          acc[m][j][i] = fmaf(i < 2 ? s0 : s1, part_sum[m][j][i] - x_sum[j][i & 1u], acc[m][j][i]);
         }
       }
     }
@@ -641,6 +652,16 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
 
       // Columns of a product that this lane holds.
       const uint32_t col[2] = {INT4 ? q : 2u * q, INT4 ? q + 4u : 2u * q + 1u};
+      if constexpr (INT4) {
+#pragma unroll
+        for (uint32_t m = 0; m < MR; ++m) {
+#pragma unroll
+          for (uint32_t j = 0; j < kTiles8; ++j) {
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) acc[m][j][i] *= kCodeUnit;
+          }
+        }
+      }
       if (SECOND && p.own_y) {
         // Into this part's own sums of y: a pass holds a token once, so no two lanes meet.
         if (any) {
