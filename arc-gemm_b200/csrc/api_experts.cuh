@@ -259,7 +259,7 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   if (p.sorted) {
     uint16_t* xs = static_cast<uint16_t*>(workspace) + slots * ldh;
     const uint64_t ldxs = expert_ld(K);
-    const uint32_t smem = EX::layout_of(0, 1, 0, columns, T, slots, E, false, true).total + 2 * E;
+    const uint32_t smem = EX::layout_of(0, 1, 0, columns, T, slots, E, false, true).total + EX::sort_scratch(E);
     e = launch_grid(columns == 8    ? EX::expert_rows_kernel<8>
                     : columns == 16 ? EX::expert_rows_kernel<16>
                                     : EX::expert_rows_kernel<32>,
