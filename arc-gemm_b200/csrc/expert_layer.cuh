@@ -195,17 +195,43 @@ template <uint32_t NT>
 __device__ __forceinline__ uint32_t sort_choices(const Params& p, Pass* passes, uint16_t* list, uint16_t* ids,
                                                  uint16_t* counts /* [kSortWarps][experts], scratch */, uint32_t* totals) {
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
-  for (uint32_t s = tid; s < p.slots; s += kThreads) {
-    uint16_t id = kNoExpert;
-    if (p.ids_wide) {
-      const int64_t v = __ldg(static_cast<const long long*>(p.ids) + s);
-      if (v >= 0 && v < static_cast<int64_t>(p.experts)) id = static_cast<uint16_t>(v);
-    } else {
-      const int32_t v = __ldg(static_cast<const int32_t*>(p.ids) + s);
-      if (v >= 0 && v < static_cast<int32_t>(p.experts)) id = static_cast<uint16_t>(v);
+  const auto id_of = [&](uint32_t s) {
+    const int64_t v = p.ids_wide ? static_cast<int64_t>(__ldg(static_cast<const long long*>(p.ids) + s))
+                                 : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p.ids) + s));
+    return v >= 0 && v < static_cast<int64_t>(p.experts) ? static_cast<uint16_t>(v) : kNoExpert;
+  };
+  if (p.slots <= 32u) {
+    // A choice a lane, experts in the order of their first choices, one barrier (one token of 8 experts, 4096 x 2048: 73.3 us
+    // with the general way, 69.2 so).
+    if (warp == 0u) {
+      uint32_t id = lane < p.slots ? id_of(lane) : kNoExpert;
+      const uint32_t below = (1u << lane) - 1u;
+      const uint32_t first_of_token = lane - lane % p.top;
+      const uint32_t repeats = __match_any_sync(0xffffffffu, id) & below & ~((1u << first_of_token) - 1u);
+      if (repeats != 0u) id = kNoExpert;
+      const uint32_t same = __match_any_sync(0xffffffffu, id);
+      const bool first = id != kNoExpert && (same & below) == 0u;
+      const uint32_t c = first ? __popc(same) : 0u;
+      uint32_t incl = c | (c + NT - 1u) / NT << 16;
+      const uint32_t own = incl;
+#pragma unroll
+      for (uint32_t d = 1; d < 32u; d <<= 1) {
+        const uint32_t o = __shfl_up_sync(0xffffffffu, incl, d);
+        if (lane >= d) incl += o;
+      }
+      const uint32_t at = incl - own;
+      for (uint32_t i = 0; i * NT < c; ++i) {
+        passes[(at >> 16) + i] = {static_cast<uint16_t>(id), static_cast<uint16_t>((at & 0xFFFFu) + i * NT),
+                                  static_cast<uint16_t>(min(NT, c - i * NT)), 0};
+      }
+      const uint32_t begin = __shfl_sync(0xffffffffu, at & 0xFFFFu, __ffs(same) - 1);  // of this lane's expert
+      if (id != kNoExpert) list[begin + __popc(same & below)] = static_cast<uint16_t>(lane);
+      if (lane == 31u) *totals = incl >> 16;
     }
-    ids[s] = id;
+    __syncthreads();
+    return *totals;
   }
+  for (uint32_t s = tid; s < p.slots; s += kThreads) ids[s] = id_of(s);
   for (uint32_t i = tid; i < kSortWarps * p.experts; i += kThreads) counts[i] = 0;
   __syncthreads();
   // A choice that repeats an earlier one of its token adds nothing of its own. `list` notes it for now.
