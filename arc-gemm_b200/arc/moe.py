@@ -4,8 +4,8 @@
     y[t]    = sum_j weights[t, j] (h[t, j] . w_out[e]^T)
 
 `moe` does what `group_rows`, two `grouped_matmul` and the steps between them do, for batches whose cost
-is reading the chosen experts' weights: nothing is sorted or gathered in memory, and the second
-product's weights are on their way before the first has ended. Above ARC_MOE_MAX_TOKENS tokens the products are
+is reading the chosen experts' weights: nothing is sorted in memory, rows are gathered there only where
+an expert has many, and the second product's weights are on their way before the first has ended. Above 256 tokens the products are
 worth `grouped_matmul`'s tensor-core tiles; `moe` refuses them.
 
 Sums are fp32; h is rounded to bf16 as operand of the second product, the result is rounded once. It is the serving
@@ -26,7 +26,8 @@ def moe(x: torch.Tensor, w_in: torch.Tensor | TensorPair, w_out: torch.Tensor | 
     x [T, K] bf16. w_in [E, 2I, K] bf16 with gate and up rows, or [E, I, K] for experts without a gate
     (h = act(x . w_in^T)); w_out [E, N, I] bf16. Or both int4, as pairs (packed uint8 [E, rows, K/2], scales
     bfloat16 [E, rows, K/128]) in the packing of `arc.a8w4_matmul` (not pre-packed), with K and I multiples
-    of 128; the activations stay bf16.
+    of 128; the activations stay bf16, and those of 2^63 and more in magnitude (infinities among them) give
+    infinities or NaN in their token's result.
     ids [T, top], int32 or int64, and weights [T, top], float32 or bfloat16: a router's choices. An id outside
     [0, E) chooses nobody; an expert chosen twice counts with the sum of its weights. T <= 256, T * top <= 4096,
     E <= 1024. activation: as for `arc.linear`. bf16 operands whose rows are not contiguous and

@@ -11,8 +11,8 @@ namespace EX = arcb::experts;
 
 // The kernels by weights and columns of a pass. Tiles (blocks of 16 rows x row groups) as measured best, 4096 x 2048
 // experts, microseconds: bf16 16 tokens of 64 experts (8 columns) 2x2 334, 2x1 389, 4x2 366; 64 tokens (16 columns)
-// 2x4 both 495, 2x2 both 512; 128 tokens (32 columns) 2x4 and 2x2 659, 2x2 both 699; int4 32 tokens (8
-// columns) 4x2 222, 2x2 272, 4x1 264; 64 tokens (16 columns) 2x4 and 2x2 338, 2x2 both 348.
+// 2x4 both 495, 2x2 both 512; 128 tokens (32 columns) 2x4 and 2x2 659, 2x2 both 699; int4, with an earlier unpacking, 32
+// tokens (8 columns) 4x2 222, 2x2 272, 4x1 264; 64 tokens (16 columns) 2x4 and 2x2 338, 2x2 both 348.
 using ExpertKernel = void (*)(EX::Params);
 struct ExpertVariant {
   ExpertKernel kernel;

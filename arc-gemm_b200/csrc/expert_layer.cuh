@@ -8,23 +8,26 @@
 // A few tokens choose most of the experts with a few rows each: the weights are the traffic, each read
 // once, and everything else has to stay out of their way.
 //
-// * No sorting launch, no gathered copies. Every block sorts the choices in shared memory by itself (a
-//   microsecond, in SECOND under the first launch), and the rows of x and h that belong to an expert
-//   come by TMA gather, four rows an instruction. Where experts have many rows gathers hold the stream up (128
-//   tokens, 64 experts of 2048 x 4096: loads alone 711 us, 508 without the rows), so h lies in the sorted order,
-//   eight rows a load, and a small launch in front puts the rows of x there as well.
+// * No sorting launch. Every block sorts the choices in shared memory by itself (a microsecond or two, in SECOND under the
+//   first launch), and the rows of x and h that belong to an expert come by TMA gather, four rows an instruction. Where
+//   experts have many rows gathers hold the stream up (128 tokens, 64 experts of 2048 x 4096: loads alone 711 us,
+//   508 without the rows), so h lies in the sorted order, eight rows a load, and a small launch in front puts the
+//   rows of x there as well (expert_rows_kernel).
 // * Blocks walk over (expert, column tile) and their ring of loads runs on from one to the next, so the
 //   stream of weights pauses only at a launch's ends. SECOND loads its first weights under FIRST's last tiles.
-// * A tile is 32 WR weight rows; the eight warps are WR groups of rows times WK = 8 / WR parts of the
-//   contraction. 32 rows make tiles fine enough to share evenly (one token, 8 experts, 2048 columns: 1024
+// * A tile is WR groups of MR blocks of 16 weight rows; the eight warps are the WR groups times WK = 8 / WR parts of the
+//   contraction. 64 rows make tiles fine enough to share evenly (one token, 8 experts, 2048 gated columns: 512
 //   tiles); wider tiles read the tokens' rows less often, which counts once an expert has many.
 // * Products are mma.sync from registers: with at most 32 columns an operand byte is used for so little
 //   arithmetic that the pipe idles either way, int4 codes pass through registers in any case, and
 //   accumulators of 16 x 8 fit tiles of 16 columns, where UMMA's 128 lanes would cut the work into
 //   pieces too coarse to share out.
 // * SECOND keeps a column tile's sums of all tokens in shared memory and adds the experts in their order:
-//   no atomics, no partial results in memory; where tiles are few a cluster shares the contraction and adds
+//   no atomics, no partial results in memory; where tiles are few a cluster shares the passes' boxes and adds
 //   its blocks' sums in rank order. The result does not depend on timing.
+//
+// Bound by HBM with bf16 weights (16 tokens, 64 experts of 4096 x 2048, 8 a token: 334 us for 339 at the measured copy
+// rate; one token 69 for 62), by the ALU pipe with int4 ones (32 tokens 201 us for 96: 34 instructions for 16 x 32 codes).
 //
 // Sums are fp32. h is rounded to bf16, the tensor cores' operand type, and the weights of the choices multiply
 // fp32 sums. Codes of int4 weights enter as code + 8, exactly, and 8 times the group's sum of x, which the tensor cores give

@@ -393,7 +393,8 @@ int arc_group_rows(const void *ids, int id_bytes, int32_t *offsets, int32_t *row
  * weights of chosen experts are read.
  *   s_in, s_out   NULL: bf16 weights with leading dimensions ld_* and strides stride_* between experts
  *                 (elements). Else scales [E][rows][K/128] and [E][N][I/128], bf16: the weights are packed int4
- *                 as in arc_a8w4_gemm, contiguous (ld_* and stride_* are not used), K and I multiples of 128
+ *                 as in arc_a8w4_gemm, contiguous (ld_* and stride_* are not used), K and I multiples of 128, and
+ *                 |x| and |h| must be below 2^63 (a token beyond gets infinities or NaN)
  *   ids           [T][top] signed integers of id_bytes 4 or 8
  *   weights       [T][top] of weight_bytes 4 (fp32) or 2 (bf16)
  *   workspace     16-byte aligned, arc_moe_workspace_bytes, no initialisation needed
