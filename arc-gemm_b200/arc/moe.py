@@ -30,7 +30,7 @@ def moe(x: torch.Tensor, w_in: torch.Tensor | TensorPair, w_out: torch.Tensor | 
     infinities or NaN in their token's result.
     ids [T, top], int32 or int64, and weights [T, top], float32 or bfloat16: a router's choices. An id outside
     [0, E) chooses nobody; an expert chosen twice counts with the sum of its weights. T <= 256, T * top <= 4096,
-    E <= 1024. activation: as for `arc.linear`. bf16 operands whose rows are not contiguous and
+    E <= 1024; K, I and N at most 2^20. activation: as for `arc.linear`. bf16 operands whose rows are not contiguous and
     16-byte aligned are copied first, on every call. `out` [T, N] receives the result and must not overlap an operand.
     """
     code = ACTIVATIONS.get(activation)

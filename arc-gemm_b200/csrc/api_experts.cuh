@@ -194,7 +194,10 @@ int arc_moe(const uint16_t* x, const void* w_in, const uint16_t* s_in, const voi
   if (int4 && (K % group != 0 || I % group != 0)) {
     return fail(ARC_ERR_UNSUPPORTED, "%s: int4 weights need K and I to be multiples of %u (K=%d I=%d)", what, group, K, I);
   }
-  if (K > (1 << 30) || I > (1 << 29) || N > (1 << 30)) return fail(ARC_ERR_UNSUPPORTED, "%s: sizes too large", what);
+  // (The kernel counts a block's boxes in 32 bits.)
+  if (K > ARC_MOE_MAX_WIDTH || I > ARC_MOE_MAX_WIDTH || N > ARC_MOE_MAX_WIDTH) {
+    return fail(ARC_ERR_UNSUPPORTED, "%s: K, I and N are at most %d (got %d, %d, %d)", what, ARC_MOE_MAX_WIDTH, K, I, N);
+  }
   const int rows_in = gated ? 2 * I : I;
   if (int st = operand_check(what, "x", x, ldx, K)) return st;
   if (int4) {

@@ -45,9 +45,12 @@ constexpr uint32_t kRowBytes = 128;  // of a box of 64 bf16; one of 128 codes, a
 constexpr uint32_t kScaleGroup = 128;
 constexpr uint32_t kMaxStages = 32;
 constexpr uint16_t kNoExpert = 0xFFFFu;
+constexpr uint16_t kRepeat = 0x8000u;  // beside an id: an earlier choice of the token is the same
 
 struct Params {
-  CUtensorMap tm_w;  // {K, columns, 2 or 1, E}, box {128 bytes, 16 WR, 2, 1} with a gate, else {.., 32 WR, 1, 1}; SW128
+  // {K or K / 2 bytes, columns, 2 or 1, E}: a box is 64 of a row (bf16 SW128, codes SW64) of a tile's rows, with a gate
+  // half of them gate and half up.
+  CUtensorMap tm_w;
   CUtensorMap tm_x;  // {K, rows}, SW128, box {64, 8}, of rows in the sorted order; else, of tokens, {64, 1}
   const uint16_t* sb;   // int4: scales [E][weight rows][groups]
   const void* ids;      // [tokens][top]
@@ -173,10 +176,10 @@ __device__ __forceinline__ void codes_to_bf16(uint32_t w, uint32_t (&v)[4]) {
   asm("lop3.b32 %0, %1, 0x000F000F, 0x00080008, 0x6A;" : "=r"(v[2]) : "r"(u));
   asm("lop3.b32 %0, %1, 0x00F000F0, 0x00800080, 0x6A;" : "=r"(v[3]) : "r"(u));
 }
-// The eights that come with the codes, as codes of zero: what they add is taken off again.
-constexpr uint32_t kEightEven = 0x00080008u, kEightOdd = 0x00800080u;
+// Minus the eights that come with the codes.
+constexpr uint32_t kEightEven = 0x80088008u, kEightOdd = 0x80808080u;  // -8 and -128 units
 // x is multiplied by 2^64 (even pairs) and 2^60, so that products of codes are normal fp32 numbers, and the sums are in
-// units of 2^-69. |x| must be below 2^63.
+// units of 2^-69. |x| must be below 2^63; what a group's sum loses to the end of fp32's range is below 2^-80 a product.
 constexpr uint32_t kScaleEven = 0x5F805F80u, kScaleOdd = 0x5D805D80u;  // two bf16 each
 constexpr float kCodeUnit = 590295810358705651712.f;                   // 2^69
 __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
@@ -189,18 +192,25 @@ __device__ __forceinline__ uint32_t mul_bf16x2(uint32_t a, uint32_t b) {
 // The choices, sorted by expert in shared memory by the whole block: `list` holds the choices of
 // every expert in their order, `passes` which of them a pass takes. Returns the number of passes.
 // Every block must find the same, so the order is that of the choices: eight warps have a contiguous share each, which
-// they count, and place behind the shares before, 32 choices at a time (one warp alone took 15 us for 1024).
+// they count, and place behind the shares before, 32 choices at a time (one warp alone took 15 us for 1024). `ids` keeps
+// all choices' experts, repeats marked.
 // ---------------------------------------------------------------------------------
 constexpr uint32_t kSortWarps = 8;
 __host__ __device__ constexpr uint32_t sort_scratch(uint32_t experts) { return kSortWarps * experts * 2u; }
+
+// Choices and their weights are read past the L1 cache: a block that does not wait for the launch in front may start
+// beside lines that are older than they are.
+__device__ __forceinline__ int64_t id_at(const Params& p, uint32_t s) {
+  return p.ids_wide ? static_cast<int64_t>(__ldcg(static_cast<const long long*>(p.ids) + s))
+                    : static_cast<int64_t>(__ldcg(static_cast<const int32_t*>(p.ids) + s));
+}
 
 template <uint32_t NT>
 __device__ __forceinline__ uint32_t sort_choices(const Params& p, Pass* passes, uint16_t* list, uint16_t* ids,
                                                  uint16_t* counts /* [kSortWarps][experts], scratch */, uint32_t* totals) {
   const uint32_t tid = threadIdx.x, warp = tid >> 5, lane = tid & 31u;
   const auto id_of = [&](uint32_t s) {
-    const int64_t v = p.ids_wide ? static_cast<int64_t>(__ldg(static_cast<const long long*>(p.ids) + s))
-                                 : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p.ids) + s));
+    const int64_t v = id_at(p, s);
     return v >= 0 && v < static_cast<int64_t>(p.experts) ? static_cast<uint16_t>(v) : kNoExpert;
   };
   if (p.slots <= 32u) {
@@ -208,6 +218,7 @@ __device__ __forceinline__ uint32_t sort_choices(const Params& p, Pass* passes, 
     // with the general way, 69.2 so).
     if (warp == 0u) {
       uint32_t id = lane < p.slots ? id_of(lane) : kNoExpert;
+      if (lane < p.slots) ids[lane] = static_cast<uint16_t>(id);
       const uint32_t below = (1u << lane) - 1u;
       const uint32_t first_of_token = lane - lane % p.top;
       const uint32_t repeats = __match_any_sync(0xffffffffu, id) & below & ~((1u << first_of_token) - 1u);
@@ -237,12 +248,12 @@ __device__ __forceinline__ uint32_t sort_choices(const Params& p, Pass* passes, 
   for (uint32_t s = tid; s < p.slots; s += kThreads) ids[s] = id_of(s);
   for (uint32_t i = tid; i < kSortWarps * p.experts; i += kThreads) counts[i] = 0;
   __syncthreads();
-  // A choice that repeats an earlier one of its token adds nothing of its own. `list` notes it for now.
+  // A choice that repeats an earlier one of its token has no place of its own. `list` notes it for now.
   for (uint32_t s = tid; s < p.slots; s += kThreads) {
     uint16_t id = ids[s];
-    for (uint32_t i = s - s % p.top; i < s; ++i) {
-      if (ids[i] == id) id = kNoExpert;
-    }
+    bool repeats = false;
+    for (uint32_t i = s - s % p.top; i < s; ++i) repeats |= ids[i] == id;
+    if (repeats && id != kNoExpert) id |= kRepeat;
     list[s] = id;
   }
   __syncthreads();
@@ -253,7 +264,7 @@ __device__ __forceinline__ uint32_t sort_choices(const Params& p, Pass* passes, 
     const uint32_t s = s0 + lane, id = s < end ? list[s] : kNoExpert;
     if (s < end) ids[s] = static_cast<uint16_t>(id);
     const uint32_t same = __match_any_sync(0xffffffffu, id);
-    if (id != kNoExpert && (same >> lane) == 1u) mine[id] = static_cast<uint16_t>(mine[id] + __popc(same));
+    if ((id & kRepeat) == 0u && (same >> lane) == 1u) mine[id] = static_cast<uint16_t>(mine[id] + __popc(same));
     __syncwarp();
   }
   __syncthreads();
@@ -296,9 +307,9 @@ __device__ __forceinline__ uint32_t sort_choices(const Params& p, Pass* passes, 
     const uint32_t s = s0 + lane, id = s < end ? ids[s] : kNoExpert;
     const uint32_t same = __match_any_sync(0xffffffffu, id);
     const uint32_t before = __popc(same & ((1u << lane) - 1u));
-    if (id != kNoExpert) list[mine[id] + before] = static_cast<uint16_t>(s);
+    if ((id & kRepeat) == 0u) list[mine[id] + before] = static_cast<uint16_t>(s);
     __syncwarp();
-    if (id != kNoExpert && (same >> lane) == 1u) mine[id] = static_cast<uint16_t>(mine[id] + before + 1u);
+    if ((id & kRepeat) == 0u && (same >> lane) == 1u) mine[id] = static_cast<uint16_t>(mine[id] + before + 1u);
     __syncwarp();
   }
   __syncthreads();
@@ -309,18 +320,14 @@ __device__ __forceinline__ uint32_t token_of(const Params& p, uint32_t s) {
   return p.top_inverse == 0u ? s : __umulhi(s, p.top_inverse);
 }
 
-// The weight of choice s: with those of its token's later choices of the same expert.
-__device__ __forceinline__ float share_of(const Params& p, uint32_t s) {
+// The weight of choice s, the first of its expert: with those of its token's later choices of the same.
+__device__ __forceinline__ float share_of(const Params& p, const uint16_t* ids, uint32_t s) {
   float sum = 0.f;
-  const uint32_t end = s - s % p.top + p.top;
-  int64_t own = 0;
+  const uint32_t end = s - s % p.top + p.top, own = ids[s];
   for (uint32_t i = s; i < end; ++i) {
-    const int64_t id = p.ids_wide ? static_cast<int64_t>(__ldg(static_cast<const long long*>(p.ids) + i))
-                                  : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(p.ids) + i));
-    if (i == s) own = id;
-    if (id == own) {
-      sum += p.weights_bf16 ? bf16_bits_to_float(__ldg(static_cast<const uint16_t*>(p.weights) + i))
-                            : __ldg(static_cast<const float*>(p.weights) + i);
+    if ((ids[i] & ~uint32_t(kRepeat)) == own) {
+      sum += p.weights_bf16 ? bf16_bits_to_float(__ldcg(static_cast<const uint16_t*>(p.weights) + i))
+                            : __ldcg(static_cast<const float*>(p.weights) + i);
     }
   }
   return sum;
@@ -357,25 +364,34 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
     // take the rows r and r + 4, whose halves of 128 swizzled bytes lie in different banks; so column n of a
     // product is row perm(n).
     const uint32_t perm = (g8 >> 1) | (g8 & 1u) << 2;
-    float part_sum[MR][J][4], x_sum[J][4];  // over the group: of (code + 8) x, and of 8 x
+    // Pairs of k: (0, 4), (1, 5), (2, 6), (3, 7) of a lane's eight, as the codes come; 32 codes of a row are 16 bytes.
+    const auto load_x = [&](uint32_t c, uint32_t j, uint32_t (&b)[4]) {
+      uint32_t x[4];
+      lds_128(x_at + (c >> 1) * XBYTES + (j * 8u + perm) * kRowBytes + ((((c & 1u) * 4u + q) ^ perm) << 4), x);
+      b[0] = mul_bf16x2(__byte_perm(x[0], x[2], 0x5410), kScaleEven);
+      b[1] = mul_bf16x2(__byte_perm(x[0], x[2], 0x7632), kScaleOdd);
+      b[2] = mul_bf16x2(__byte_perm(x[1], x[3], 0x5410), kScaleEven);
+      b[3] = mul_bf16x2(__byte_perm(x[1], x[3], 0x7632), kScaleOdd);
+    };
+    // Over the group: -8 x, which the sums of (code + 8) x start from (32 tokens 198 us; sums from zero and -8 x added
+    // to each 204).
+    float part_sum[MR][J][4], x_sum[J][4];
+    uint32_t b[4][J][4];
 #pragma unroll
-    for (uint32_t c = 0; c < 4; ++c) {  // 32 codes of a row, 16 bytes
-      uint32_t b[J][4];  // pairs of k: (0, 4), (1, 5), (2, 6), (3, 7) of a lane's eight, as the codes come
+    for (uint32_t j = 0; j < J; ++j) {
 #pragma unroll
-      for (uint32_t j = 0; j < J; ++j) {
-        uint32_t x[4];
-        lds_128(x_at + (c >> 1) * XBYTES + (j * 8u + perm) * kRowBytes + ((((c & 1u) * 4u + q) ^ perm) << 4), x);
-        b[j][0] = mul_bf16x2(__byte_perm(x[0], x[2], 0x5410), kScaleEven);
-        b[j][1] = mul_bf16x2(__byte_perm(x[0], x[2], 0x7632), kScaleOdd);
-        b[j][2] = mul_bf16x2(__byte_perm(x[1], x[3], 0x5410), kScaleEven);
-        b[j][3] = mul_bf16x2(__byte_perm(x[1], x[3], 0x7632), kScaleOdd);
+      for (uint32_t c = 0; c < 4; ++c) {
+        load_x(c, j, b[c][j]);
         if (c == 0) {
-          mma_bf16_first(x_sum[j], kEightEven, kEightEven, kEightOdd, kEightOdd, b[j][0], b[j][1]);
+          mma_bf16_first(x_sum[j], kEightEven, kEightEven, kEightOdd, kEightOdd, b[c][j][0], b[c][j][1]);
         } else {
-          mma_bf16(x_sum[j], kEightEven, kEightEven, kEightOdd, kEightOdd, b[j][0], b[j][1]);
+          mma_bf16(x_sum[j], kEightEven, kEightEven, kEightOdd, kEightOdd, b[c][j][0], b[c][j][1]);
         }
-        mma_bf16(x_sum[j], kEightEven, kEightEven, kEightOdd, kEightOdd, b[j][2], b[j][3]);
+        mma_bf16(x_sum[j], kEightEven, kEightEven, kEightOdd, kEightOdd, b[c][j][2], b[c][j][3]);
       }
+    }
+#pragma unroll
+    for (uint32_t c = 0; c < 4; ++c) {
 #pragma unroll
       for (uint32_t m2 = 0; m2 < MR; m2 += 2) {
         uint32_t a[4];  // rows 0-7 and 8-15 of two blocks of rows
@@ -389,11 +405,11 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
 #pragma unroll
           for (uint32_t j = 0; j < J; ++j) {
             if (c == 0) {
-              mma_bf16_first(part_sum[m2 + m][j], lo[0], hi[0], lo[1], hi[1], b[j][0], b[j][1]);
-            } else {
-              mma_bf16(part_sum[m2 + m][j], lo[0], hi[0], lo[1], hi[1], b[j][0], b[j][1]);
+#pragma unroll
+              for (uint32_t i = 0; i < 4; ++i) part_sum[m2 + m][j][i] = x_sum[j][i];
             }
-            mma_bf16(part_sum[m2 + m][j], lo[2], hi[2], lo[3], hi[3], b[j][2], b[j][3]);
+            mma_bf16(part_sum[m2 + m][j], lo[0], hi[0], lo[1], hi[1], b[c][j][0], b[c][j][1]);
+            mma_bf16(part_sum[m2 + m][j], lo[2], hi[2], lo[3], hi[3], b[c][j][2], b[c][j][3]);
           }
         }
       }
@@ -406,7 +422,7 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
       for (uint32_t j = 0; j < J; ++j) {
 #pragma unroll
         for (uint32_t i = 0; i < 4; ++i) {
-          acc[m][j][i] = fmaf(i < 2 ? s0 : s1, part_sum[m][j][i] - x_sum[j][i & 1u], acc[m][j][i]);
+          acc[m][j][i] = fmaf(i < 2 ? s0 : s1, part_sum[m][j][i], acc[m][j][i]);
         }
       }
     }
@@ -481,7 +497,7 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
   if (SECOND) {
     for (uint32_t i = threadIdx.x; i < y_size * (p.own_y ? WK : 1u); i += kThreads) y[i] = 0.f;
     const uint32_t listed = passes_n == 0u ? 0u : passes[passes_n - 1u].first + passes[passes_n - 1u].count;
-    for (uint32_t i = threadIdx.x; i < listed; i += kThreads) share[i] = share_of(p, list[i]);
+    for (uint32_t i = threadIdx.x; i < listed; i += kThreads) share[i] = share_of(p, ids, list[i]);
   }
   // The ring held scratch of the sorting: order its writes before the loads.
   fence_proxy_async_smem();

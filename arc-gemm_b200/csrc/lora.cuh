@@ -31,9 +31,11 @@ constexpr uint32_t kMaxAdapters = 1024;
 constexpr uint32_t kMaxRank = 256;
 constexpr uint32_t kNone = 0xFFFFFFFFu;
 
+// The product's blocks start beside lora_down_kernel's, so what they read before they wait for it, ids and b, comes past
+// the L1 cache, whose lines may be older.
 __device__ __forceinline__ uint32_t id_at(const void* ids, uint32_t wide, uint32_t adapters, uint32_t row) {
-  const int64_t v = wide ? static_cast<int64_t>(__ldg(static_cast<const long long*>(ids) + row))
-                         : static_cast<int64_t>(__ldg(static_cast<const int32_t*>(ids) + row));
+  const int64_t v = wide ? static_cast<int64_t>(__ldcg(static_cast<const long long*>(ids) + row))
+                         : static_cast<int64_t>(__ldcg(static_cast<const int32_t*>(ids) + row));
   return v < 0 || v >= static_cast<int64_t>(adapters) ? kNone : static_cast<uint32_t>(v);
 }
 
@@ -112,12 +114,12 @@ struct Keep {
 __device__ __forceinline__ uint4 load8(const uint16_t* p, bool there, const Keep<4>& keep) {
   uint4 v = make_uint4(0u, 0u, 0u, 0u);
   // volatile: not to be moved behind a wait that it is meant to pass
-  if (there) asm volatile("ld.global.nc.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  if (there) asm volatile("ld.global.cg.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
   return make_uint4(v.x & keep.mask[0], v.y & keep.mask[1], v.z & keep.mask[2], v.w & keep.mask[3]);
 }
 __device__ __forceinline__ uint2 load4(const uint16_t* p, bool there, const Keep<2>& keep) {
   uint2 v = make_uint2(0u, 0u);
-  if (there) asm volatile("ld.global.nc.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  if (there) asm volatile("ld.global.cg.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return make_uint2(v.x & keep.mask[0], v.y & keep.mask[1]);
 }
 

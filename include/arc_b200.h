@@ -398,12 +398,13 @@ int arc_group_rows(const void *ids, int id_bytes, int32_t *offsets, int32_t *row
  *   ids           [T][top] signed integers of id_bytes 4 or 8
  *   weights       [T][top] of weight_bytes 4 (fp32) or 2 (bf16)
  *   workspace     16-byte aligned, arc_moe_workspace_bytes, no initialisation needed
- * Requirements: T <= ARC_MOE_MAX_TOKENS, T * top <= ARC_MOE_MAX_CHOICES, E <= 1024; x and the weights 16-byte
- * aligned, their leading dimensions and strides multiples of 8. out overlaps no operand. The result does not
+ * Requirements: T <= ARC_MOE_MAX_TOKENS, T * top <= ARC_MOE_MAX_CHOICES, E <= 1024; K, I and N <=
+ * ARC_MOE_MAX_WIDTH; x and the weights 16-byte aligned, their leading dimensions and strides multiples of 8. out overlaps no operand. The result does not
  * depend on timing, nor a token's on the other tokens of a call of the same plan.
  */
 #define ARC_MOE_MAX_TOKENS 256
 #define ARC_MOE_MAX_CHOICES 4096
+#define ARC_MOE_MAX_WIDTH (1 << 20)
 int arc_moe_workspace_bytes(int T, int top, int E, int K, int I, size_t *bytes);
 int arc_moe(const uint16_t *x, const void *w_in, const uint16_t *s_in, const void *w_out, const uint16_t *s_out,
             const void *ids, int id_bytes, const void *weights, int weight_bytes, uint16_t *out, void *workspace,

@@ -122,6 +122,62 @@ def test_nan_stays_in_its_rows(cuda_device):
         assert got[ids == 2].isnan().all() and not got[ids == 3].isfinite().all()
 
 
+@pytest.mark.parametrize("plan", PLANS)
+def test_nan_stays_in_its_rows_whatever_the_plan(cuda_device, monkeypatch, plan):
+    """Adapters of NaN and infinities, and a row of NaN, beside the others of their tile; the rank passes one block of 64."""
+    monkeypatch.setenv("ARC_LINEAR_PLAN", plan)
+    for r in (16, 72):
+        x, w, a, b, ids, bias, residual, scales = _inputs(150, 136, 520, r, 9, seed=r, without=0.1)
+        want, bound = reference(x, w, a, b, ids, bias, residual, scales, None)
+        a[2], b[3], scales[4] = float("nan"), float("inf"), float("inf")
+        x[70] = float("nan")
+        got = arc.lora_linear(x, w, a, b, ids, bias, residual, scales=scales)
+        keep = (ids < 2) | (ids > 4)
+        keep[70] = False
+        assert_within(got[keep], want[keep], bound[keep], plan)
+        assert got[70].isnan().all() and got[ids == 2].isnan().all() and not got[ids == 3].isfinite().all()
+
+
+def test_adapters_beyond_32_bits_of_elements(cuda_device):
+    """The last adapters of a and b lie more than 2^32 elements behind the first."""
+    n, k, r, count = 32768, 32768, 136, 1024
+    a = torch.empty(count, r, k, dtype=torch.bfloat16, device="cuda")
+    b = torch.empty(count, n, r, dtype=torch.bfloat16, device="cuda")
+    g = torch.Generator().manual_seed(3)
+    last_a, last_b = normal(g, 1, r, 8), normal(g, 1, n, r, scale=r ** -0.5)
+    a[-1].zero_()
+    a[-1, :, -8:] = last_a[0]
+    b[-1] = last_b[0]
+    w = torch.zeros(n, 1, dtype=torch.bfloat16, device="cuda").expand(n, k).contiguous()
+    for m in (3, 300):
+        x = torch.zeros(m, k, dtype=torch.bfloat16, device="cuda")
+        x[:, -8:] = normal(g, m, 8)
+        ids = torch.full((m,), count - 1, device="cuda")
+        ids[1] = -1
+        want, bound = reference(x[:, -8:], w[:, -8:], last_a, last_b, torch.where(ids > 0, 0, -1))
+        got = arc.lora_linear(x, w, a, b, ids)
+        assert_within(got, want, bound, m)
+        assert (got[1] == 0).all()
+
+
+def test_two_streams_at_once(cuda_device):
+    calls = [_inputs(9, 264, 520, 16, 6, seed=1), _inputs(600, 264, 520, 16, 6, seed=2, runs=7), _inputs(40, 512, 1032, 72, 6)]
+
+    def call(v):
+        return arc.lora_linear(*v[:7], scales=v[7], activation="silu")
+
+    want = [call(v) for v in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for turn in range(10):
+        for j, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append(((turn + j) % 3, call(calls[(turn + j) % 3])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want[j]) for j, v in got) and arc.device_status(0) == 0
+
+
 def test_plain_call_strides_and_out(cuda_device):
     """No bias, residual or scales; operands and out inside wider buffers; the residual as out."""
     g = torch.Generator().manual_seed(2)

@@ -123,6 +123,65 @@ def test_unchosen_experts_are_not_read(cuda_device):
     assert_within(got[keep], want[keep], bound[keep], "beside a NaN token")
 
 
+def test_int4_nan_stays_in_its_token(cuda_device):
+    """Scales full of NaN of experts that nobody chooses are not read, and a token of infinities spoils its own row alone."""
+    for t in (7, 40):
+        x, w_in, w_out, ids, weights = _inputs(t, 2, 9, 256, 128, kind="int4", seed=t)
+        ids[ids == 4] = 5
+        want, bound = moe_reference(x, w_in, w_out, ids, weights, "silu")
+        w_in[1][4], w_out[1][4] = float("nan"), float("inf")
+        x[3] = float("inf")
+        got = arc.moe(x, w_in, w_out, ids, weights)
+        keep = [i for i in range(t) if i != 3]
+        assert not got[3].isfinite().any()
+        assert_within(got[keep], want[keep], bound[keep], t)
+
+
+@pytest.mark.parametrize("power", [-50, -20, 20, 50])
+def test_int4_large_and_small_activations(cuda_device, power):
+    """The kernel's scaled codes keep a sum's relative precision: without an activation or a gate y is linear in x. (What
+    the end of fp32's range takes, 2^-80 a product, is below the bound's 2^-23 of products of 2^-50.)"""
+    x, w_in, w_out, ids, weights = _inputs(9, 2, 6, 256, 128, kind="int4", gated=False, seed=3)
+    _check((x * 2.0 ** power, w_in, w_out, ids, weights), None, power)
+
+
+@pytest.mark.parametrize("t,top,e", [(1, 4096, 1024), (1, 33, 40), (2, 100, 8), (40, 102, 300)])
+def test_many_choices_of_a_token(cuda_device, t, top, e):
+    _check(_inputs(t, top, e, 72, 40, repeat=True, seed=top), "silu")
+
+
+def test_weights_beyond_32_bits_of_elements(cuda_device):
+    """The last of the experts, 2^33 and 2^32 elements into the weights."""
+    e, k, i = 17, 16384, 16384
+    w_in, w_out = (torch.empty(s, dtype=torch.bfloat16, device="cuda") for s in ((e, 2 * i, k), (e, k, i)))
+    small_in, small_out = normal(torch.Generator().manual_seed(1), 64, k, scale=k ** -0.5), normal(torch.Generator(), 2, k)
+    # h is nonzero in the last 32 gate and up rows alone, and in the last columns of w_out's rows.
+    w_in[-1].zero_(), w_out[-1].zero_()
+    w_in[-1, i - 32:i], w_in[-1, 2 * i - 32:] = small_in[:32], small_in[32:]
+    w_out[-1, :, i - 2:] = small_out.T
+    x = normal(torch.Generator().manual_seed(2), 2, k)
+    ids, weights = torch.tensor([[e - 1], [-1]], device="cuda"), torch.ones(2, 1, device="cuda")
+    got = arc.moe(x, w_in, w_out, ids, weights)
+    w = torch.cat((small_in[30:32], small_in[62:]))[None]
+    want, bound = moe_reference(x[:1], w, small_out.T.contiguous()[None], torch.zeros_like(ids[:1]), weights[:1], "silu")
+    assert_within(got[:1], want, bound, "the last expert")
+    assert (got[1] == 0).all()
+
+
+def test_two_streams_at_once(cuda_device):
+    calls = [_inputs(4, 2, 8, 512, 256, seed=1), _inputs(70, 4, 8, 512, 256, seed=2), _inputs(4, 2, 8, 512, 256, kind="int4")]
+    want = [arc.moe(*v) for v in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(3)]
+    got = []
+    for turn in range(10):
+        for j, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append(((turn + j) % 3, arc.moe(*calls[(turn + j) % 3])))
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want[j]) for j, v in got) and arc.device_status(0) == 0
+
+
 def test_strides_and_out(cuda_device):
     g = torch.Generator().manual_seed(3)
     x, w_in, w_out, ids, weights = _inputs(6, 2, 5, 72, 40, seed=1)

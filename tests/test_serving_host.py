@@ -34,6 +34,8 @@ def test_moe_checks(native_lib, p, monkeypatch):
     for name in ("t", "top", "e", "k", "i", "n"):
         assert call(**{name: 0}) == BAD, name
     assert call(t=257) == UNS and call(t=256, top=17) == UNS and call(e=1025, sti=1 << 30, sto=1 << 30) == UNS
+    for name in ("k", "i", "n"):
+        assert call(**{name: (1 << 20) + 128}) == UNS, name
     assert call(act=5) == BAD and call(act=-1) == BAD
     assert call(idb=2) == UNS and call(wtb=8) == UNS
     assert call(ldx=64) == BAD and call(ldi=64) == BAD and call(sti=128 * 128) == BAD and call(gated=0, sti=64 * 128) == BAD
