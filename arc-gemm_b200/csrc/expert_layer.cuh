@@ -154,7 +154,16 @@ __device__ __forceinline__ void tma_load_4d(const CUtensorMap* map, uint64_t* ba
       : "memory");
 }
 
-// The same with sums that start from zero.
+// The same with sums that start from others.
+__device__ __forceinline__ void mma_bf16_from(float (&d)[4], const float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2,
+                                              uint32_t a3, uint32_t b0, uint32_t b1) {
+  asm(
+      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
+      "{%10, %11, %12, %13};"
+      : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+      : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1), "f"(c[0]), "f"(c[1]), "f"(c[2]), "f"(c[3]));
+}
+// And from zero.
 __device__ __forceinline__ void mma_bf16_first(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                                uint32_t b0, uint32_t b1) {
   asm(
@@ -405,10 +414,10 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
 #pragma unroll
           for (uint32_t j = 0; j < J; ++j) {
             if (c == 0) {
-#pragma unroll
-              for (uint32_t i = 0; i < 4; ++i) part_sum[m2 + m][j][i] = x_sum[j][i];
+              mma_bf16_from(part_sum[m2 + m][j], x_sum[j], lo[0], hi[0], lo[1], hi[1], b[c][j][0], b[c][j][1]);
+            } else {
+              mma_bf16(part_sum[m2 + m][j], lo[0], hi[0], lo[1], hi[1], b[c][j][0], b[c][j][1]);
             }
-            mma_bf16(part_sum[m2 + m][j], lo[0], hi[0], lo[1], hi[1], b[c][j][0], b[c][j][1]);
             mma_bf16(part_sum[m2 + m][j], lo[2], hi[2], lo[3], hi[3], b[c][j][2], b[c][j][3]);
           }
         }
@@ -416,8 +425,8 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
     }
 #pragma unroll
     for (uint32_t m = 0; m < MR; ++m) {
-      const float s0 = __uint_as_float(__shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + g8) << 16);
-      const float s1 = __uint_as_float(__shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + 8u + g8) << 16);
+      const float s0 = __uint_as_float(__shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + g8));
+      const float s1 = __uint_as_float(__shfl_sync(0xffffffffu, sc[m / 2], (m & 1u) * 16u + 8u + g8));
 #pragma unroll
       for (uint32_t j = 0; j < J; ++j) {
 #pragma unroll
@@ -632,36 +641,50 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
     uint32_t item = item0, kb = kb_first + part;  // and where it lies
     bool ok = true;
 
-    // int4: the scales of a box, one a weight row, on their way a box ahead. Lane l has row l (and l + 32) of
-    // this warp's rows.
+    const auto locate = [&](uint32_t& of_item, uint32_t& of_kb) {
+      while (of_kb >= nkb) {
+        of_kb -= nkb;
+        of_item += item_step;
+      }
+    };
+    // int4: the scales of a box, one a weight row, on their way two boxes ahead. Lane l has row l (and l + 32) of
+    // this warp's rows (behind the last column: that one's again). Where an item's rows have theirs is computed once an item (for
+    // every box it took 25 us of 200). Scales have fewer than 2^32 elements: their codes are 64 times as many bytes.
     constexpr uint32_t kScaleRegs = MR / 2;
-    uint32_t scales[kScaleRegs];
-    const auto fetch_scales = [&]() {
-      if constexpr (INT4) {
-        const uint32_t pi = SECOND ? item : item / p.tiles;
-        const uint32_t f0 = (SECOND ? my_tile : item - pi * p.tiles) * tile_cols;
-        const uint32_t rows = p.gated ? 2u * p.cols : p.cols;
+    uint32_t scales[2][kScaleRegs], scale_at[kScaleRegs];
+    uint32_t scale_box = part, scale_item = item0, scale_kb = kb_first + part;
+    const auto locate_scales = [&]() {
+      const uint32_t pi = SECOND ? scale_item : scale_item / p.tiles;
+      const uint32_t f0 = (SECOND ? my_tile : scale_item - pi * p.tiles) * tile_cols;
+      const uint32_t rows0 = passes[pi].expert * (p.gated ? 2u * p.cols : p.cols);
 #pragma unroll
-        for (uint32_t i = 0; i < kScaleRegs; ++i) {
-          const uint32_t m = i * 2u + (lane >> 4);
-          const bool up = p.gated && m >= MR / 2;
-          const uint32_t f = f0 + ((up ? m - MR / 2 : m) * WR + wr) * 16u + (lane & 15u);
-          uint32_t bits = 0;
-          if (f < p.cols) bits = __ldg(p.sb + (size_t(passes[pi].expert) * rows + f + (up ? p.cols : 0u)) * p.groups + kb);
-          scales[i] = bits;
+      for (uint32_t i = 0; i < kScaleRegs; ++i) {
+        const uint32_t m = i * 2u + (lane >> 4);
+        const bool up = p.gated && m >= MR / 2;
+        const uint32_t f = min(f0 + ((up ? m - MR / 2 : m) * WR + wr) * 16u + (lane & 15u), p.cols - 1u);
+        scale_at[i] = (rows0 + f + (up ? p.cols : 0u)) * p.groups;
+      }
+    };
+    const auto fetch_scales = [&](uint32_t (&to)[kScaleRegs]) {
+      if constexpr (INT4) {
+        if (scale_box >= boxes) return;
+        if (scale_kb >= nkb) {
+          locate(scale_item, scale_kb);
+          locate_scales();
         }
+#pragma unroll
+        for (uint32_t i = 0; i < kScaleRegs; ++i) to[i] = __ldg(p.sb + (scale_at[i] + scale_kb));
+        scale_box += WK;
+        scale_kb += WK;
       }
     };
-    const auto locate = [&]() {
-      while (kb >= nkb) {
-        kb -= nkb;
-        item += item_step;
-      }
-    };
-    if (box < boxes) {
-      locate();
-      fetch_scales();
+    if (INT4 && box < boxes) {
+      locate(scale_item, scale_kb);
+      locate_scales();
     }
+    fetch_scales(scales[0]);
+    fetch_scales(scales[1]);
+    if (box < boxes) locate(item, kb);
 
     const uint32_t last = boxes == 0u ? 0u : kb_first + boxes;  // boxes from the first item's start to this block's last one
     for (uint32_t at = item0, before = 0; before < last; at += item_step, before += nkb) {
@@ -682,13 +705,14 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
         any = true;
         uint32_t sc[kScaleRegs];
 #pragma unroll
-        for (uint32_t i = 0; i < kScaleRegs; ++i) sc[i] = scales[i];
+        for (uint32_t i = 0; i < kScaleRegs; ++i) {
+          sc[i] = scales[0][i] << 16;  // bf16 as fp32
+          scales[0][i] = scales[1][i];
+        }
+        fetch_scales(scales[1]);
         box += WK;
         kb += WK;
-        if (box < boxes) {
-          locate();
-          fetch_scales();
-        }
+        if (box < boxes) locate(item, kb);
         if (ok) ok = __all_sync(0xffffffffu, mbar_wait(&full[stage], phase, abort, kStatusTimeoutMma));
         const uint32_t w_at = smem_u32(ring + stage * C::kStageBytes), x_at = w_at + C::kWBytes;
         if (ok) {
