@@ -11,8 +11,8 @@ namespace EX = arcb::experts;
 
 // The kernels by weights and columns of a pass. Tiles (blocks of 16 rows x row groups) as measured best, 4096 x 2048
 // experts, microseconds: bf16 16 tokens of 64 experts (8 columns) 2x2 334, 2x1 389, 4x2 366; 64 tokens (16 columns)
-// 2x4 both 495, 2x2 both 512; 128 tokens (32 columns) 2x4 and 2x2 659, 2x2 both 699; int4, with an earlier unpacking, 32
-// tokens (8 columns) 4x2 222, 2x2 272, 4x1 264; 64 tokens (16 columns) 2x4 and 2x2 338, 2x2 both 348.
+// 2x4 both 495, 2x2 both 512; 128 tokens (32 columns) 2x4 and 2x2 659, 2x2 both 699; int4, 32 tokens
+// (8 columns) 4x2 191, 4x2 and 2x2 194, 4x1 247; with an earlier unpacking 64 tokens (16 columns) 2x4 and 2x2 338, 2x2 both 348.
 using ExpertKernel = void (*)(EX::Params);
 struct ExpertVariant {
   ExpertKernel kernel;
@@ -105,7 +105,9 @@ bool expert_ring(const ExpertVariant& v, bool second, uint32_t columns, uint32_t
   ring->own_y = second && v.parts * v.rows * tokens * 4 <= 32 * 1024;
   const uint32_t rest =
       EX::layout_of(v.sum_bytes, v.parts, v.rows, columns, tokens, slots, experts, second, ring->own_y).total + 1024;
-  const uint32_t unit = v.parts < 4 ? 4 : v.parts;  // a whole number of parts and of batches
+  // A whole number of parts and of batches, so that a stage always has the same waiters: by its parity a wait tells a phase only from
+  // the one before, and whoever skipped a phase may take an older one for its own.
+  const uint32_t unit = v.parts < 4 ? 4 : v.parts;
   const auto stages = [&](uint32_t budget) {
     const uint32_t n = budget > rest ? (budget - rest) / v.stage_bytes : 0;
     return (n < EX::kMaxStages ? n : EX::kMaxStages) / unit * unit;

@@ -27,7 +27,8 @@
 //   its blocks' sums in rank order. The result does not depend on timing.
 //
 // Bound by HBM with bf16 weights (16 tokens, 64 experts of 4096 x 2048, 8 a token: 334 us for 339 at the measured copy
-// rate; one token 69 for 62), by the ALU pipe with int4 ones (32 tokens 201 us for 96: 34 instructions for 16 x 32 codes).
+// rate; one token 69 for 62). With int4 ones 32 tokens (60 passes over 48 experts) take 191 us for 96: the products alone
+// take 149, the loads alone 134, and two stages a warp do not hide all of either under the other.
 //
 // Sums are fp32. h is rounded to bf16, the tensor cores' operand type, and the weights of the choices multiply
 // fp32 sums. Codes of int4 weights enter as code + 8, exactly, and 8 times the group's sum of x, which the tensor cores give
@@ -382,8 +383,8 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
       b[2] = mul_bf16x2(__byte_perm(x[1], x[3], 0x5410), kScaleEven);
       b[3] = mul_bf16x2(__byte_perm(x[1], x[3], 0x7632), kScaleOdd);
     };
-    // Over the group: -8 x, which the sums of (code + 8) x start from (32 tokens 198 us; sums from zero and -8 x added
-    // to each 204).
+    // Over the group: -8 x, which the sums of (code + 8) x start from (32 tokens 200 us; sums from zero and 8 x
+    // taken off each 201).
     float part_sum[MR][J][4], x_sum[J][4];
     uint32_t b[4][J][4];
 #pragma unroll
@@ -649,7 +650,7 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
     };
     // int4: the scales of a box, one a weight row, on their way two boxes ahead. Lane l has row l (and l + 32) of
     // this warp's rows (behind the last column: that one's again). Where an item's rows have theirs is computed once an item (for
-    // every box it took 25 us of 200). Scales have fewer than 2^32 elements: their codes are 64 times as many bytes.
+    // every box 32 tokens took 201 us, so 191). Scales have fewer than 2^32 elements: their codes are 64 times as many bytes.
     constexpr uint32_t kScaleRegs = MR / 2;
     uint32_t scales[2][kScaleRegs], scale_at[kScaleRegs];
     uint32_t scale_box = part, scale_item = item0, scale_kb = kb_first + part;
