@@ -8,7 +8,8 @@ is reading the chosen experts' weights: nothing is sorted in memory, rows are ga
 an expert has many, and the second product's weights are on their way before the first has ended. Above 256 tokens the products are
 worth `grouped_matmul`'s tensor-core tiles; `moe` refuses them.
 
-Sums are fp32; h is rounded to bf16 as operand of the second product, the result is rounded once. It is the serving
+Sums are fp32; h is rounded to bf16 as operand of the second product, the result is rounded once. The same call gives the
+same bits; beside other tokens a token's sums may be added in another order, so its last bits may differ. It is the serving
 form: there is no gradient, and inputs that require one are refused (outside torch.no_grad()).
 """
 from __future__ import annotations

@@ -24,7 +24,10 @@
 //   pieces too coarse to share out.
 // * SECOND keeps a column tile's sums of all tokens in shared memory and adds the experts in their order:
 //   no atomics, no partial results in memory; where tiles are few a cluster shares the passes' boxes and adds
-//   its blocks' sums in rank order. The result does not depend on timing.
+//   its blocks' sums in rank order. The result does not depend on timing, but a token's last bits do on the other tokens: the
+//   boxes of all passes are shared evenly, so where its sums are cut is a matter of what the others chose. (Cuts that
+//   depend on the expert alone leave parts of a short contraction idle where the parts' sums meet: int4, 32 tokens, 198 us so
+//   and 255 with them.)
 //
 // Bound by HBM with bf16 weights (16 tokens, 64 experts of 4096 x 2048, 8 a token: 334 us for 339 at the measured copy
 // rate; one token 69 for 62). With int4 ones 32 tokens (60 passes over 48 experts) take 191 us for 96: the products alone

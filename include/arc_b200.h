@@ -400,7 +400,8 @@ int arc_group_rows(const void *ids, int id_bytes, int32_t *offsets, int32_t *row
  *   workspace     16-byte aligned, arc_moe_workspace_bytes, no initialisation needed
  * Requirements: T <= ARC_MOE_MAX_TOKENS, T * top <= ARC_MOE_MAX_CHOICES, E <= 1024; K, I and N <=
  * ARC_MOE_MAX_WIDTH; x and the weights 16-byte aligned, their leading dimensions and strides multiples of 8. out overlaps no operand. The result does not
- * depend on timing, nor a token's on the other tokens of a call of the same plan.
+ * depend on timing: the same call gives the same bits. A token's last bits depend on the other tokens' choices,
+ * since blocks and warps share the boxes of all that are chosen evenly, and so cut a token's sums in other places.
  */
 #define ARC_MOE_MAX_TOKENS 256
 #define ARC_MOE_MAX_CHOICES 4096

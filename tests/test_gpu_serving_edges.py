@@ -1,0 +1,62 @@
+"""arc.moe and arc.lora_linear on the B200: what their documentation promises beyond the values themselves."""
+from __future__ import annotations
+
+import pytest
+import torch
+
+import arc
+from linear_bounds import assert_within, normal
+from moe_reference import moe_reference
+
+pytestmark = pytest.mark.gpu
+
+
+def _cancelling_experts(g, kind, e, k, i, n):
+    """Experts whose rows of w_in come twice and whose columns of w_out come twice with opposite signs: every result is zero but for
+    the rounding of its sums, so that a sum's error is all that shows."""
+    half = i // 2
+    if kind == "bf16":
+        rows, cols = normal(g, e, 2, half, k, scale=k ** -0.5), normal(g, e, n, half, scale=i ** -0.5)
+        return torch.cat((rows, rows), 2).flatten(1, 2), torch.cat((cols, -cols), 2)
+    codes, signed = torch.randint(-8, 8, (e, 2, half, k), generator=g), torch.randint(-7, 8, (e, n, half), generator=g)
+    codes, signed = torch.cat((codes, codes), 2).flatten(1, 2), torch.cat((signed, -signed), 2)
+
+    def pack(c, scale):
+        c = (c & 15).to(torch.uint8)
+        return (c[..., 0::2] | c[..., 1::2] << 4).cuda(), torch.full((e, c.shape[1], c.shape[2] // 128), scale,
+                                                                    dtype=torch.bfloat16, device="cuda")
+
+    return pack(codes, 0.2 * k ** -0.5), pack(signed, 0.2 * i ** -0.5)
+
+
+# Contractions of 6 and 10 boxes, 7 and 5, 3 and 3: no multiple of the four parts that share them, nor of the blocks of a
+# cluster. 6 tokens are sorted by one warp, 40 by eight.
+@pytest.mark.parametrize("kind,k,i", [("bf16", 328, 584), ("int4", 896, 640), ("int4", 384, 384)])
+@pytest.mark.parametrize("t", [6, 40])
+@pytest.mark.parametrize("splits,ordered", [(None, None), (1, 0), (2, 1), (4, 0), (8, 1)])
+def test_a_token_beside_others(cuda_device, monkeypatch, kind, k, i, t, splits, ordered):
+    """One token's row, choices and weights beside different tokens and in different rows: the same bits for the same
+    batch, and within the error of its sums in every one, under each plan."""
+    g = torch.Generator().manual_seed(t + k)
+    e, top, n = 11, 3, 392
+    w_in, w_out = _cancelling_experts(g, kind, e, k, i, n)
+    x1, weights1, ids1 = normal(g, 1, k), torch.rand(1, top, generator=g).cuda(), torch.tensor([[7, 2, 10]], device="cuda")
+    want, bound = moe_reference(x1, w_in, w_out, ids1, weights1, "silu")
+    for columns in (8, 16) if splits else (0,):
+        if splits:
+            monkeypatch.setenv("ARC_EXPERT_PLAN", f"{columns}:{splits}:{ordered}")
+        for turn in range(6):
+            x, weights = normal(g, t, k), torch.rand(t, top, generator=g).cuda()
+            ids = torch.rand(t, e, generator=g).topk(top, dim=1).indices.cuda()
+            if turn == 1:
+                ids[:] = -1  # nobody else chooses
+            elif turn == 2:
+                ids[:] = ids1.flip(1)  # the same experts: several passes of each
+            elif turn == 3:
+                ids[:, 0] = 2  # a popular one in front of the other two
+            row = (0, 1, t - 1)[turn % 3]
+            x[row], weights[row], ids[row] = x1[0], weights1[0], ids1[0]
+            got = arc.moe(x, w_in, w_out, ids, weights)
+            assert torch.equal(arc.moe(x, w_in, w_out, ids, weights), got)
+            assert_within(got[row:row + 1], want, bound, (columns, turn))
+    assert arc.device_status(0) == 0
