@@ -442,7 +442,8 @@ __device__ __forceinline__ void multiply_box(float (&acc)[MR][N][4], uint32_t w_
   }
 }
 
-// The rows of x in the order of the sorted choices, for batches whose experts have many: xs [choices][ldxs].
+// The rows of x in the order of the sorted choices, for batches whose experts have many: xs [choices][ldxs]. (Plain loads:
+// the launch in front may write x while this one's blocks are there already, so it is not read-only to them.)
 template <uint32_t NT>
 __global__ void __launch_bounds__(kThreads) expert_rows_kernel(const __grid_constant__ Params p, uint16_t* xs, uint64_t ldxs,
                                                                const uint16_t* x, uint64_t ldx, uint32_t inner) {
@@ -460,9 +461,9 @@ __global__ void __launch_bounds__(kThreads) expert_rows_kernel(const __grid_cons
     const uint16_t* from = x + token_of(p, list[i]) * ldx;
     uint16_t* to = xs + i * ldxs;
     for (uint32_t v = threadIdx.x; v < inner / 8u; v += kThreads) {
-      reinterpret_cast<uint4*>(to)[v] = __ldg(reinterpret_cast<const uint4*>(from) + v);
+      reinterpret_cast<uint4*>(to)[v] = reinterpret_cast<const uint4*>(from)[v];
     }
-    for (uint32_t k = inner / 8u * 8u + threadIdx.x; k < inner; k += kThreads) to[k] = __ldg(from + k);
+    for (uint32_t k = inner / 8u * 8u + threadIdx.x; k < inner; k += kThreads) to[k] = from[k];
   }
 }
 
@@ -654,6 +655,7 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
     // int4: the scales of a box, one a weight row, on their way two boxes ahead. Lane l has row l (and l + 32) of
     // this warp's rows (behind the last column: that one's again). Where an item's rows have theirs is computed once an item (for
     // every box 32 tokens took 201 us, so 191). Scales have fewer than 2^32 elements: their codes are 64 times as many bytes.
+    // (Plain loads, as of x in expert_rows_kernel.)
     constexpr uint32_t kScaleRegs = MR / 2;
     uint32_t scales[2][kScaleRegs], scale_at[kScaleRegs];
     uint32_t scale_box = part, scale_item = item0, scale_kb = kb_first + part;
@@ -677,7 +679,7 @@ __global__ void __launch_bounds__(kThreads, 2) expert_layer_kernel(const __grid_
           locate_scales();
         }
 #pragma unroll
-        for (uint32_t i = 0; i < kScaleRegs; ++i) to[i] = __ldg(p.sb + (scale_at[i] + scale_kb));
+        for (uint32_t i = 0; i < kScaleRegs; ++i) to[i] = p.sb[scale_at[i] + scale_kb];
         scale_box += WK;
         scale_kb += WK;
       }

@@ -317,7 +317,7 @@ __device__ __forceinline__ void linear_stream(const P& p) {
     tc_fence_after_sync();
   }
   const bool mine = ok && f < p.cols;
-  const float bias = mine && p.epi.bias != nullptr ? bf16_bits_to_float(__ldg(p.epi.bias + f)) : 0.f;
+  const float bias = mine && p.epi.bias != nullptr ? bf16_bits_to_float(p.epi.bias[f]) : 0.f;
 
   if (p.splits == 1u) {
     if (ok) {

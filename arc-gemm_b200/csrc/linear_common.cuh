@@ -292,7 +292,7 @@ __device__ __forceinline__ void load_row32(const uint16_t* p, uint32_t (&v)[16],
   if (wide != 0u && cols >= 32u) {
 #pragma unroll
     for (uint32_t j = 0; j < 4; ++j) {
-      const uint4 x = __ldg(reinterpret_cast<const uint4*>(p + 8 * j));
+      const uint4 x = reinterpret_cast<const uint4*>(p)[j];
       v[4 * j] = x.x;
       v[4 * j + 1] = x.y;
       v[4 * j + 2] = x.z;
@@ -303,7 +303,7 @@ __device__ __forceinline__ void load_row32(const uint16_t* p, uint32_t (&v)[16],
     for (uint32_t j = 0; j < 16; ++j) v[j] = 0u;
 #pragma unroll
     for (uint32_t j = 0; j < 32; ++j) {
-      if (j < cols) v[j >> 1] |= static_cast<uint32_t>(__ldg(p + j)) << ((j & 1u) * 16u);
+      if (j < cols) v[j >> 1] |= static_cast<uint32_t>(p[j]) << ((j & 1u) * 16u);
     }
   }
 }

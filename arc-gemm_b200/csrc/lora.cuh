@@ -416,8 +416,9 @@ __global__ void __launch_bounds__(kDownThreads, 2) lora_down_kernel(const __grid
   float* sums = reinterpret_cast<float*>(ring);  // [kDownWarps][kDownRows][kDownCols]
   // What the cluster's blocks send this one, for the rows rank, rank + S, ...: [S][kDownRows / S][kDownCols].
   float* got = reinterpret_cast<float*>(ring + kDownWarps * kDownSlotBytes);
-  // A scale is on its way before it is needed.
-  const float scale = id != kNone && p.scales != nullptr ? __ldg(p.scales + id) : 1.f;
+  // A scale is on its way before it is needed. (A plain load: the launch in front may write the scales while this block is
+  // there already, so they are not read-only to it.)
+  const float scale = id != kNone && p.scales != nullptr ? p.scales[id] : 1.f;
 
   // The row tiles' lists are made by blocks that seldom have an adapter to work on.
   bool lists = p.lists != nullptr && warp == kDownWarps && rank == 0u && set + 1u == p.sets;

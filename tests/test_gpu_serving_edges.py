@@ -60,3 +60,74 @@ def test_a_token_beside_others(cuda_device, monkeypatch, kind, k, i, t, splits, 
             assert torch.equal(arc.moe(x, w_in, w_out, ids, weights), got)
             assert_within(got[row:row + 1], want, bound, (columns, turn))
     assert arc.device_status(0) == 0
+
+
+@pytest.mark.parametrize("t,kind,ordered", [(4, "bf16", 0), (4, "bf16", 1), (40, "bf16", 1), (4, "int4", 0), (40, "int4", 1)])
+def test_experts_read_what_was_written_just_before(cuda_device, monkeypatch, t, kind, ordered):
+    """Everything that a call reads is written by the launch in front of it, over other values that a call before has read: in a
+    graph, where nothing but the order of launches stands between them."""
+    monkeypatch.setenv("ARC_EXPERT_PLAN", f"8:2:{ordered}")
+    g = torch.Generator().manual_seed(t)
+
+    def values():
+        ids = torch.rand(t, 9, generator=g).topk(2, dim=1).indices.cuda()
+        w_in, w_out = _cancelling_experts(g, kind, 9, 512, 256, 264)
+        flat = [*w_in, *w_out] if kind == "int4" else [w_in, w_out]
+        return [normal(g, t, 512), ids, torch.rand(t, 2, generator=g).cuda(), *(v.clone() for v in flat)]
+
+    def call(x, ids, weights, *w):
+        w = (w[:2], w[2:]) if kind == "int4" else w
+        return arc.moe(x, *w, ids, weights)
+
+    sets = [values() for _ in range(4)]
+    want = [call(*v) for v in sets]
+    torch.cuda.synchronize()
+    for last in range(len(sets[0])):  # whose copy comes last, directly in front of the call
+        at = [v.clone() for v in sets[0]]
+        order = [i for i in range(len(at)) if i != last] + [last]
+        call(*at)
+        graph = torch.cuda.CUDAGraph()
+        got = []
+        with torch.cuda.graph(graph):
+            for v in sets * 3:
+                for i in order:
+                    at[i].copy_(v[i])
+                got.append(call(*at))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[j % 4]) for j, y in enumerate(got)), last
+    assert arc.device_status(0) == 0
+
+
+@pytest.mark.parametrize("m,plan", [(9, "16:2"), (150, "128:1"), (300, "pair:1"), (300, "pair:2")])
+def test_adapters_read_what_was_written_just_before(cuda_device, monkeypatch, m, plan):
+    monkeypatch.setenv("ARC_LINEAR_PLAN", plan)
+    g = torch.Generator().manual_seed(m)
+    n, k, r, count = 264, 520, 24, 5
+
+    def values():
+        return [normal(g, m, k), normal(g, n, k, scale=k ** -0.5), normal(g, count, r, k, scale=k ** -0.5),
+                normal(g, count, n, r, scale=r ** -0.5), torch.randint(-1, count, (m,), generator=g).cuda(), normal(g, n),
+                normal(g, m, n), torch.rand(count, generator=g).cuda()]
+
+    def call(x, w, a, b, ids, bias, residual, scales):
+        return arc.lora_linear(x, w, a, b, ids, bias, residual, scales=scales, activation="silu")
+
+    sets = [values() for _ in range(4)]
+    want = [call(*v) for v in sets]
+    torch.cuda.synchronize()
+    for last in range(len(sets[0])):
+        at = [v.clone() for v in sets[0]]
+        order = [i for i in range(len(at)) if i != last] + [last]
+        call(*at)
+        graph = torch.cuda.CUDAGraph()
+        got = []
+        with torch.cuda.graph(graph):
+            for v in sets * 3:
+                for i in order:
+                    at[i].copy_(v[i])
+                got.append(call(*at))
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(y, want[j % 4]) for j, y in enumerate(got)), last
+    assert arc.device_status(0) == 0
