@@ -28,7 +28,9 @@ def moe(x: torch.Tensor, w_in: torch.Tensor | TensorPair, w_out: torch.Tensor | 
     (h = act(x . w_in^T)); w_out [E, N, I] bf16. Or both int4, as pairs (packed uint8 [E, rows, K/2], scales
     bfloat16 [E, rows, K/128]) in the packing of `arc.a8w4_matmul` (not pre-packed), with K and I multiples
     of 128; the activations stay bf16, and those of 2^63 and more in magnitude (infinities among them) give
-    infinities or NaN in their token's result.
+    infinities or NaN in their token's result. Codes enter the fp32 sum of a group as code + 8, and 8 x is taken off: the
+    sum is rounded relative to 8 |x| beside |code x|, which shows where a large activation meets small codes. A product of a
+    code and an activation is held to 2^-80: below 2^-57 it loses bits. The same goes for h, the second product's operand.
     ids [T, top], int32 or int64, and weights [T, top], float32 or bfloat16: a router's choices. An id outside
     [0, E) chooses nobody; an expert chosen twice counts with the sum of its weights. T <= 256, T * top <= 4096,
     E <= 1024; K, I and N at most 2^20. activation: as for `arc.linear`. bf16 operands whose rows are not contiguous and

@@ -35,7 +35,8 @@
 //
 // Sums are fp32. h is rounded to bf16, the tensor cores' operand type, and the weights of the choices multiply
 // fp32 sums. Codes of int4 weights enter as code + 8, exactly, and 8 times the group's sum of x, which the tensor cores give
-// beside it, is taken off in fp32 before the scale is applied.
+// beside it, is taken off in fp32 before the scale is applied: the sum of a group is off by what 256 products of up to
+// (16 + code) |x| leave, more than |code x| would where a large x has small codes.
 #pragma once
 
 #include "linear_common.cuh"

@@ -394,7 +394,8 @@ int arc_group_rows(const void *ids, int id_bytes, int32_t *offsets, int32_t *row
  *   s_in, s_out   NULL: bf16 weights with leading dimensions ld_* and strides stride_* between experts
  *                 (elements). Else scales [E][rows][K/128] and [E][N][I/128], bf16: the weights are packed int4
  *                 as in arc_a8w4_gemm, contiguous (ld_* and stride_* are not used), K and I multiples of 128, and
- *                 |x| and |h| must be below 2^63 (a token beyond gets infinities or NaN)
+ *                 |x| and |h| must be below 2^63 (a token beyond gets infinities or NaN). A group's fp32 sum is
+ *                 of -8 x and (code + 8) x: off by at most 256 2^-23 of (16 + code) |x|, and by 2^-80 a product
  *   ids           [T][top] signed integers of id_bytes 4 or 8
  *   weights       [T][top] of weight_bytes 4 (fp32) or 2 (bf16)
  *   workspace     16-byte aligned, arc_moe_workspace_bytes, no initialisation needed

@@ -5,6 +5,7 @@ import pytest
 import torch
 
 import arc
+from int4_bounds import moe_int4_linear
 from linear_bounds import assert_within, normal
 from moe_reference import moe_reference
 
@@ -131,3 +132,40 @@ def test_adapters_read_what_was_written_just_before(cuda_device, monkeypatch, m,
         torch.cuda.synchronize()
         assert all(torch.equal(y, want[j % 4]) for j, y in enumerate(got)), last
     assert arc.device_status(0) == 0
+
+
+def _int4(g, e, n, k):
+    packed = torch.randint(0, 256, (e, n, k // 2), generator=g, dtype=torch.uint8).cuda()
+    return packed, ((0.5 + torch.rand(e, n, k // 128, generator=g)) * (0.2 * k ** -0.5)).to(torch.bfloat16).cuda()
+
+
+def _int4_layer(g, t, top=2, e=6, k=256, i=128):
+    x, w_in, w_out = normal(g, t, k), _int4(g, e, i, k), _int4(g, e, k, i)
+    ids = torch.rand(t, e, generator=g).topk(top, dim=1).indices.cuda()
+    return x, w_in, w_out, ids, torch.rand(t, top, generator=g).cuda()
+
+
+def _within_int4(args, what):
+    want, bound = moe_int4_linear(*args)
+    assert_within(arc.moe(*args, activation=None), want, bound, what)
+    assert arc.device_status(0) == 0
+
+
+@pytest.mark.parametrize("t", [3, 30])
+@pytest.mark.parametrize("power", [-90, -80, -70, -64, -60, -57, -30, 0, 40, 55])
+def test_int4_over_its_range(cuda_device, power, t):
+    """Activations down to where products of codes leave fp32's range: what is lost there is 2^-80 a product, no more."""
+    args = _int4_layer(torch.Generator().manual_seed(power + 200), t)
+    args[0].mul_(2.0 ** power)
+    _within_int4(args, power)
+
+
+@pytest.mark.parametrize("t", [3, 30])
+@pytest.mark.parametrize("power", [7, 14, 30, 60])
+def test_int4_outliers_on_zero_codes(cuda_device, power, t):
+    """A large activation whose codes are 0, and rows of zero codes: its 8 x cancels but for the rounding of the group's sum."""
+    x, w_in, w_out, ids, weights = _int4_layer(torch.Generator().manual_seed(power), t)
+    x[:, 5] = 1.4 * 2.0 ** power
+    w_in[0][:, :, 2] &= 0x0F  # code 5 of every row: the high nibble of byte 2
+    w_in[0][:, 7], w_out[0][:, 9] = 0, 0
+    _within_int4((x, w_in, w_out, ids, weights), power)
