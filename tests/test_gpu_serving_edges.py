@@ -5,9 +5,11 @@ import pytest
 import torch
 
 import arc
+from arc import _lib
 from int4_bounds import moe_int4_linear
 from linear_bounds import assert_within, normal
 from moe_reference import moe_reference
+from test_gpu_lora import reference as lora_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -169,3 +171,47 @@ def test_int4_outliers_on_zero_codes(cuda_device, power, t):
     w_in[0][:, :, 2] &= 0x0F  # code 5 of every row: the high nibble of byte 2
     w_in[0][:, 7], w_out[0][:, 9] = 0, 0
     _within_int4((x, w_in, w_out, ids, weights), power)
+
+
+def _adapter_layer(g, m, n, k, r, count, runs=0):
+    x, w = normal(g, m, k), normal(g, n, k, scale=k ** -0.5)
+    a, b = normal(g, count, r, k, scale=k ** -0.5), normal(g, count, n, r, scale=r ** -0.5)
+    if runs:
+        cuts = torch.randint(0, m + 1, (runs - 1,), generator=g).sort().values.tolist()
+        owner = torch.randint(-1, count, (runs,), generator=g)
+        ids = torch.repeat_interleave(owner, torch.tensor([q - p for p, q in zip([0] + cuts, cuts + [m])]))
+    else:
+        ids = torch.randint(-1, count, (m,), generator=g)
+    return x, w, a, b, ids.cuda(), normal(g, n), normal(g, m, n), (0.25 + torch.rand(count, generator=g)).cuda()
+
+
+def _within_adapters(args, act, what):
+    want, bound = lora_reference(*args, act)
+    got = arc.lora_linear(*args[:7], scales=args[7], activation=act)
+    assert_within(got, want, bound, what)
+    assert arc.device_status(0) == 0
+
+
+@pytest.mark.parametrize("plan", ["pair:1", "pair:2", "pair128:1", "pair128:2"])
+@pytest.mark.parametrize("r", [33, 64, 65, 100, 128, 136, 192, 200, 256])
+def test_ranks_of_several_blocks_by_pairs(cuda_device, monkeypatch, plan, r):
+    """The adapters' part of the contraction as one to four blocks of 64 for each adapter, the last one whole or not, in row tiles
+    of one adapter and of all five."""
+    monkeypatch.setenv("ARC_LINEAR_PLAN", plan)
+    g = torch.Generator().manual_seed(r)
+    _within_adapters(_adapter_layer(g, 300, 264, 200, r, 5), "silu", "mixed")
+    _within_adapters(_adapter_layer(g, 530, 520, 136, r, 5, runs=4), None, "prompts")
+
+
+@pytest.mark.parametrize("plan", ["pair:1", "pair128:1"])
+@pytest.mark.parametrize("r,count,runs", [(16, 12, 0), (72, 3, 0), (32, 9, 40), (256, 4, 9)])
+def test_pairs_that_walk_over_tiles(cuda_device, monkeypatch, plan, r, count, runs):
+    """Several tiles a pair, each with its own list of adapters."""
+    monkeypatch.setenv("ARC_LINEAR_PLAN", plan)
+    _within_adapters(_adapter_layer(torch.Generator().manual_seed(r), 2100, 5000, 72, r, count, runs), "gelu", plan)
+
+
+@pytest.mark.parametrize("m,n,k", [(2048, 2048, 256), (1500, 1500, 512)])
+def test_pairs_by_their_own_plan(cuda_device, m, n, k):
+    assert "pair" in arc.kernel_name(_lib.OP_LINEAR, m, n, k)
+    _within_adapters(_adapter_layer(torch.Generator().manual_seed(m), m, n, k, 128, 6, runs=7), "relu", (m, n, k))
