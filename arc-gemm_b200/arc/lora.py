@@ -5,7 +5,9 @@
 Two launches: u = scales[i] (x . a[i]^T) for every row, in bf16, then `arc.linear`'s product with u and b as the end
 of its contraction, so that bias, activation and residual stay in its epilogue. The shared product starts while u is
 computed. Rows of any order and any mix of adapters are right; rows of one request side by side are fastest, since a
-tile of rows pays for every adapter in it.
+tile of rows pays for every adapter in it. What the adapters add to `arc.linear`'s time is least for decode batches of mixed
+adapters and for long prompts. Some 64 to 256 rows that share one adapter pay the most (128 x 4096 x 4096, rank 64: 60 us,
+`arc.linear` 14), and hundreds of rows with an adapter each (512 x 4096 x 4096, rank 16, 64 adapters: 75, `arc.linear` 19).
 
 Sums are fp32, u is rounded to bf16 as operand, the result once. It is the serving form: there is no gradient, and
 inputs that require one are refused (outside torch.no_grad()).

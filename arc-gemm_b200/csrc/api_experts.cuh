@@ -11,8 +11,8 @@ namespace EX = arcb::experts;
 
 // The kernels by weights and columns of a pass. Tiles (blocks of 16 rows x row groups) as measured best, 4096 x 2048
 // experts, microseconds: bf16 16 tokens of 64 experts (8 columns) 2x2 334, 2x1 389, 4x2 366; 64 tokens (16 columns)
-// 2x4 both 495, 2x2 both 512; 128 tokens (32 columns) 2x4 and 2x2 659, 2x2 both 699; int4, 32 tokens
-// (8 columns) 4x2 191, 4x2 and 2x2 194, 4x1 247; with an earlier unpacking 64 tokens (16 columns) 2x4 and 2x2 338, 2x2 both 348.
+// 2x4 both 495, 2x2 both 512; 128 tokens (32 columns) 2x4 and 2x2 659, 2x2 both 699; int4, one token (8 columns)
+// 4x2 31, 2x2 41, 32 tokens 4x2 189, 2x2 248; 64 tokens (16 columns) 2x4 and 2x2 308, 2x2 both 321, 128 tokens 533 and 552.
 using ExpertKernel = void (*)(EX::Params);
 struct ExpertVariant {
   ExpertKernel kernel;
@@ -68,8 +68,10 @@ struct ExpertPlan {
 
 // An expert's choices fill a pass on average half: they are uneven, and a second pass reads the weights again, while
 // columns that stay empty cost shared memory. int4 weights stop at 16: the registers of 32 do not fit. Sorted rows
-// pay from 8 choices an expert (8 experts of 4096 x 7168, two a token, 32 tokens: 240 us with gathers, 224 sorted;
-// 64 experts of 4096 x 2048, 16 tokens of two choices an expert: 338 and 339).
+// pay from 8 choices an expert (8 experts of 4096 x 7168, two a token, 64 tokens: 333 us with gathers, 293 sorted; 32 tokens, 8 choices
+// an expert, 277 and 274, int4 153 and 138; 64 experts of 4096 x 2048, 16 tokens of two choices an expert: 338 and 337). A
+// layer of small experts loses the launch in front (32 experts of 2048 x 1024, 64 tokens: 101 and 104), and int4 would gain
+// earlier (32 tokens, four choices an expert: 189 and 182).
 //
 // ARC_EXPERT_PLAN="columns:S:sorted" (tests and tuning) forces them.
 int expert_plan(bool int4, uint32_t tokens, uint32_t slots, uint32_t experts, ExpertPlan* plan) {

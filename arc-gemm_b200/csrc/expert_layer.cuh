@@ -30,7 +30,7 @@
 //   and 255 with them.)
 //
 // Bound by HBM with bf16 weights (16 tokens, 64 experts of 4096 x 2048, 8 a token: 334 us for 339 at the measured copy
-// rate; one token 69 for 62). With int4 ones 32 tokens (60 passes over 48 experts) take 191 us for 96: the products alone
+// rate; one token 69 for 62). With int4 ones 32 tokens (60 passes over 48 experts) take 189 to 207 us for 96: the products alone
 // take 149, the loads alone 134, and two stages a warp do not hide all of either under the other.
 //
 // Sums are fp32. h is rounded to bf16, the tensor cores' operand type, and the weights of the choices multiply
