@@ -215,3 +215,43 @@ def test_pairs_that_walk_over_tiles(cuda_device, monkeypatch, plan, r, count, ru
 def test_pairs_by_their_own_plan(cuda_device, m, n, k):
     assert "pair" in arc.kernel_name(_lib.OP_LINEAR, m, n, k)
     _within_adapters(_adapter_layer(torch.Generator().manual_seed(m), m, n, k, 128, 6, runs=7), "relu", (m, n, k))
+
+
+@pytest.mark.parametrize("t,top,e,k,i,n", [(1, 1, 1, 1, 1, 1), (3, 2, 2, 1, 9, 2), (9, 1, 3, 65, 1, 7), (256, 1, 1, 8, 8, 1), (256, 16, 1024, 3, 2, 5)])
+@pytest.mark.parametrize("gated", [True, False])
+def test_smallest_experts(cuda_device, t, top, e, k, i, n, gated):
+    g = torch.Generator().manual_seed(t)
+    w_in, w_out = normal(g, e, 2 * i if gated else i, k), normal(g, e, n, i)
+    ids = torch.rand(t, e, generator=g).topk(top, dim=1).indices.cuda()
+    args = (normal(g, t, k), w_in, w_out, ids, torch.rand(t, top, generator=g).cuda())
+    want, bound = moe_reference(*args, "gelu")
+    assert_within(arc.moe(*args, activation="gelu"), want, bound, (t, k, i, n))
+    assert arc.device_status(0) == 0
+
+
+@pytest.mark.parametrize("m,n,k,r,count,runs", [(1, 1, 1, 1, 1, 0), (2, 3, 1, 1, 2, 0), (129, 1, 9, 2, 3, 2), (40000, 72, 64, 8, 1024, 0),
+                                               (40000, 520, 64, 24, 50, 300)])
+def test_smallest_and_longest_adapters(cuda_device, m, n, k, r, count, runs):
+    _within_adapters(_adapter_layer(torch.Generator().manual_seed(m), m, n, k, r, count, runs), "silu", (m, n, k, r))
+
+
+def test_serving_operators_beside_others_on_streams(cuda_device):
+    """Kernels with TMEM, clusters and early launches of several operators at once, each with the bits of its call alone."""
+    g = torch.Generator().manual_seed(3)
+    small, large = _adapter_layer(g, 40, 520, 512, 24, 6), _adapter_layer(g, 2048, 2048, 256, 72, 6, runs=7)
+    e_in, e_out = normal(g, 9, 512, 512, scale=512 ** -0.5), normal(g, 9, 512, 256, scale=256 ** -0.5)
+    x, ids, weights = normal(g, 40, 512), torch.rand(40, 9, generator=g).topk(3, dim=1).indices.cuda(), torch.rand(40, 3).cuda()
+    a, b = normal(g, 1024, 512), normal(g, 1024, 512)
+    calls = [lambda: arc.lora_linear(*small[:7], scales=small[7]), lambda: arc.lora_linear(*large[:7], scales=large[7]),
+             lambda: arc.moe(x, e_in, e_out, ids, weights), lambda: arc.matmul(a, b), lambda: arc.linear(a, b, activation="gelu")]
+    want = [f() for f in calls]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in calls]
+    got = []
+    for turn in range(20):
+        for j, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                i = (turn + j) % len(calls)
+                got.append((i, calls[i]()))
+    torch.cuda.synchronize()
+    assert all(torch.equal(v, want[i]) for i, v in got) and arc.device_status(0) == 0
